@@ -28,6 +28,8 @@ SCAN_KINDS = {"scanl": SKEL_SCANL, "scanl1": SKEL_SCANL1, "scanl'": SKEL_SCANLP,
 COMBINE_GENERIC, COMBINE_ADD, COMBINE_MIN, COMBINE_MAX, COMBINE_AND, COMBINE_OR, COMBINE_XOR = range(7)
 BOUNDARY = {"clamp": 0, "mirror": 1, "wrap": 2, "constant": 3}
 FLAG_FOLD_RIGHT, FLAG_FAST_MATH, FLAG_GUARDED, FLAG_TILED = 1, 2, 4, 8
+OP_PRODUCT, OP_ROUTE, OP_COMBINE, OP_MICRO = range(4)
+STRIDED_RANK = 4
 
 
 def FLAG_TILE_DIM(d):
@@ -77,6 +79,14 @@ class acc_skel_desc(C.Structure):
                 ("tap_offsets", C.POINTER(C.c_int32)), ("tap2_offsets", C.POINTER(C.c_int32))]
 
 
+class acc_op_desc(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32)]
+
+
+# the bytes of an acc_strided, by rank
+_STRIDED = [struct.Struct("@ii%dq%dx%dq%dxQ" % (r, 8 * (STRIDED_RANK - r), r, 8 * (STRIDED_RANK - r))).pack for r in range(STRIDED_RANK + 1)]
+
+
 class acc_device_props(C.Structure):
     _fields_ = [("name", C.c_char * 256), ("arch", C.c_char * 64), ("compute_units", C.c_int32),
                 ("wavefront_size", C.c_int32), ("max_threads_per_block", C.c_int32), ("clock_khz", C.c_int32),
@@ -115,7 +125,9 @@ acc_exec_stencil acc_exec_stencil2 acc_exec_stencil_iterate acc_guard_create acc
 acc_guard_latch acc_guard_read acc_stream_set_guard acc_trace_start acc_trace_stop acc_memtable_create acc_memtable_destroy
 acc_memtable_malloc acc_memtable_acquire acc_memtable_release acc_memtable_free acc_memtable_insert_unmanaged
 acc_memtable_reclaim acc_memtable_get_stats acc_skel_create_async acc_skel_wait acc_skel_poll acc_skel_prefetch acc_compile_threads acc_compile_drain
-acc_tuning_set acc_tuning_text acc_context_set_tuning""".split()
+acc_tuning_set acc_tuning_text acc_context_set_tuning acc_op_create acc_op_destroy acc_op_compile_only acc_exec_product_rows
+acc_exec_product_outer acc_exec_route acc_exec_route_gradient acc_exec_combine acc_exec_combine_gradient acc_exec_micro_quantise
+acc_exec_micro_values acc_exec_micro_rows""".split()
 
 
 def build(force=False):
@@ -196,6 +208,9 @@ def lib():
         L.acc_guard_latch.argtypes = [C.c_void_p, AP, C.c_void_p]
         L.acc_guard_read.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_int32), C.POINTER(C.c_int64)]
         L.acc_stream_set_guard.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
+        L.acc_op_create.argtypes = [C.c_void_p, C.POINTER(acc_op_desc), C.POINTER(C.c_void_p)]
+        L.acc_op_destroy.argtypes = [C.c_void_p]
+        L.acc_op_compile_only.argtypes = [C.c_char_p, C.POINTER(acc_op_desc), C.POINTER(C.c_int32), C.POINTER(C.c_size_t)]
         L.acc_trace_start.argtypes = [C.c_void_p]
         L.acc_trace_stop.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.POINTER(C.c_double)]
         L.acc_memtable_create.argtypes = [C.c_void_p, C.c_uint64, C.POINTER(C.c_void_p)]
@@ -629,7 +644,12 @@ class _Drivers(object):
               "acc_exec_foldseg_nd": (_P, _P, C.c_int32, _P, _P, _P, _P), "acc_exec_scan": (_P, _P, C.c_int64, _P, _P, _P),
               "acc_exec_scan_noalloc": (_P, _P, C.c_int64, _P, _P, _P), "acc_exec_permute": (_P, _P, C.c_int64, _P, _P, _P),
               "acc_exec_stencil": (_P, _P, _P, _P, _P), "acc_exec_stencil2": (_P, _P, _P, _P, _P, _P),
-              "acc_exec_stencil_iterate": (_P, _P, _P, _P, C.c_int32, _P, _P)}
+              "acc_exec_stencil_iterate": (_P, _P, _P, _P, C.c_int32, _P, _P),
+              "acc_exec_product_rows": (_P, _P, _P, _P, _P, C.c_int32, _P, _P), "acc_exec_product_outer": (_P, _P, _P, _P, _P, C.c_int32, _P, _P),
+              "acc_exec_route": (_P, _P, _P, _P, _P, _P, _P, _P), "acc_exec_route_gradient": (_P, _P, _P, _P, _P, _P, _P),
+              "acc_exec_combine": (_P, _P, _P, _P, _P, _P), "acc_exec_combine_gradient": (_P, _P, _P, _P, _P, _P, _P, _P),
+              "acc_exec_micro_quantise": (_P, _P, _P, _P, _P), "acc_exec_micro_values": (_P, _P, _P, _P, _P),
+              "acc_exec_micro_rows": (_P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P)}
 
     def __getattr__(self, name):               # (at its first call; an attribute of its own from then on)
         f = C.CFUNCTYPE(C.c_int, *self._TYPES[name])((name, lib()))
@@ -736,6 +756,154 @@ class Skeleton(object):
         if self.handle:
             lib().acc_skel_destroy(self.handle)
             self.handle = None
+
+
+# ---------------------------------------------------------------------------
+# operators on segments of rows (include/acc_hip.h, section D)
+
+class Strided(object):
+    """Device memory as an array with strides (in elements): a part of a larger array, or one with its dimensions
+    exchanged.  `owner` is whatever keeps the memory."""
+
+    def __init__(self, shape, strides, ptr, owner=None):
+        self.shape, self.strides, self.ptr, self.owner = tuple(shape), tuple(strides), ptr, owner
+
+    @classmethod
+    def of(cls, a):
+        """a DeviceArray as it lies"""
+        strides, step = [], 1
+        for n in reversed(a.shape):
+            strides.insert(0, step)
+            step *= n
+        return cls(a.shape, strides, a.ptr, a)
+
+    def swap(self):
+        """the last two dimensions exchanged"""
+        return Strided(self.shape[:-2] + (self.shape[-1], self.shape[-2]), self.strides[:-2] + (self.strides[-1], self.strides[-2]), self.ptr, self.owner)
+
+
+def _layout(a):
+    """the acc_strided of an array as bytes: a DeviceArray, a Strided, or any tensor that says where it lies (`data_ptr()`,
+    `shape`, `stride()`); None: no array"""
+    if a is None:
+        return None
+    where = getattr(a, "data_ptr", None)
+    if where is not None:
+        shape = a.shape
+        return _STRIDED[len(shape)](len(shape), 0, *shape, *a.stride(), where())
+    if not isinstance(a, Strided):
+        a = Strided.of(a)
+    return _STRIDED[len(a.shape)](len(a.shape), 0, *a.shape, *a.strides, a.ptr)
+
+
+def op_desc(kind, elt, choose=0, normalise=True):
+    d = acc_op_desc()
+    d.kind, d.elt_type, d.choose, d.normalise = kind, _b(elt), choose, int(normalise)
+    return d
+
+
+def op_compile_only(kind, elt, choose=0, normalise=True, target="gfx950"):
+    """(translation units, bytes of code) of everything that calls of an operator may need; needs no GPU"""
+    units, size = C.c_int32(), C.c_size_t()
+    check(lib().acc_op_compile_only(target.encode(), C.byref(op_desc(kind, elt, choose, normalise)), C.byref(units), C.byref(size)))
+    return units.value, size.value
+
+
+class _Operator(object):
+    """One acc_op.  Arrays are given as `_layout` takes them; results go to arrays that the caller has."""
+
+    def __init__(self, ctx, *args):
+        self.ctx = ctx
+        h = C.c_void_p()
+        check(lib().acc_op_create(ctx.handle, C.byref(op_desc(self.KIND, *args)), C.byref(h)))
+        self.handle = h
+
+    def destroy(self):
+        if self.handle:
+            lib().acc_op_destroy(self.handle)
+            self.handle = None
+
+
+class Product(_Operator):
+    """Products of segments of rows with a matrix each; `elt` is "float", "half" or "bfloat16"."""
+    KIND = OP_PRODUCT
+
+    def __init__(self, ctx, elt):
+        _Operator.__init__(self, ctx, elt)
+
+    def rows(self, x, w, offsets, out, index=None, per=0, stream=None):
+        """out[m, n] = sum_k x[r(m), k] w[e, n, k] for the rows m of expert e's segment"""
+        rc = _drivers.acc_exec_product_rows(self.handle, _layout(x), _layout(w), _layout(offsets), _layout(index), per, _layout(out), stream)
+        if rc:
+            check(rc)
+
+    def outer(self, a, b, offsets, out, index=None, per=0, stream=None):
+        """out[e, i, j] = sum over the rows m of e's segment of a[m, i] b[r(m), j]"""
+        rc = _drivers.acc_exec_product_outer(self.handle, _layout(a), _layout(b), _layout(offsets), _layout(index), per, _layout(out), stream)
+        if rc:
+            check(rc)
+
+
+class Router(_Operator):
+    """The `choose` best experts of every token, their weights, and the slots in the order of their experts."""
+    KIND = OP_ROUTE
+
+    def __init__(self, ctx, elt, choose, normalise=True):
+        _Operator.__init__(self, ctx, elt, choose, normalise)
+
+    def route(self, logits, experts, weights, offsets, order, place, stream=None):
+        rc = _drivers.acc_exec_route(self.handle, _layout(logits), _layout(experts), _layout(weights), _layout(offsets), _layout(order), _layout(place), stream)
+        if rc:
+            check(rc)
+
+    def gradient(self, logits, experts, weights, dweights, dlogits, stream=None):
+        rc = _drivers.acc_exec_route_gradient(self.handle, _layout(logits), _layout(experts), _layout(weights), _layout(dweights), _layout(dlogits), stream)
+        if rc:
+            check(rc)
+
+
+class Combiner(_Operator):
+    """The experts' rows of every token summed into one."""
+    KIND = OP_COMBINE
+
+    def __init__(self, ctx, elt):
+        _Operator.__init__(self, ctx, elt)
+
+    def combine(self, y, place, weights, out, stream=None):
+        """out[t] = sum_j weights[t, j] y[place[t, j]]; weights None: all 1"""
+        rc = _drivers.acc_exec_combine(self.handle, _layout(y), _layout(place), _layout(weights), _layout(out), stream)
+        if rc:
+            check(rc)
+
+    def gradient(self, dout, y, place, weights, dy, dweights, stream=None):
+        rc = _drivers.acc_exec_combine_gradient(self.handle, _layout(dout), _layout(y), _layout(place), _layout(weights), _layout(dy), _layout(dweights), stream)
+        if rc:
+            check(rc)
+
+
+class Microscale(_Operator):
+    """4-bit numbers, 32 under one scale: codes two a byte [rows, 16 ceil(k / 32)], scales [rows, ceil(k / 32)]."""
+    KIND = OP_MICRO
+
+    def __init__(self, ctx, elt):
+        _Operator.__init__(self, ctx, elt)
+
+    def quantise(self, x, codes, scales, stream=None):
+        rc = _drivers.acc_exec_micro_quantise(self.handle, _layout(x), _layout(codes), _layout(scales), stream)
+        if rc:
+            check(rc)
+
+    def values(self, codes, scales, out, stream=None):
+        rc = _drivers.acc_exec_micro_values(self.handle, _layout(codes), _layout(scales), _layout(out), stream)
+        if rc:
+            check(rc)
+
+    def rows(self, xcodes, xscales, wcodes, wscales, offsets, out, index=None, per=0, stream=None):
+        """out[m, n] = sum_k x[r(m), k] w[e, n, k], both in 4 bits"""
+        rc = _drivers.acc_exec_micro_rows(self.handle, _layout(xcodes), _layout(xscales), _layout(wcodes), _layout(wscales), _layout(offsets), _layout(index), per,
+                                          _layout(out), stream)
+        if rc:
+            check(rc)
 
 
 # ---------------------------------------------------------------------------

@@ -225,6 +225,9 @@ enum { HINT_WORDS = 1024 };
 // device-to-device copy of `bytes` bytes that does nothing when the guard word at `guard` is zero (guard.hip)
 int guarded_copy(uint64_t dst, uint64_t src, size_t bytes, uint64_t guard, hipStream_t stream);
 
+// a kernel of an operator (operators.cpp), traced and timed as the skeletons' are (execute.cpp)
+int launch_operator(acc_context ctx, const char *entry, hipFunction_t fn, unsigned grid, unsigned block, unsigned lds, hipStream_t stream, void **args);
+
 int scan_order_before(int device, hipStream_t stream);    // ACC_OK: the caller launches, then calls scan_order_after
 void scan_order_after(int device);
 void scan_order_forget(int device, hipStream_t stream);

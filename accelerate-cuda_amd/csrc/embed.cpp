@@ -31,6 +31,13 @@ ACC_EMBED(stencil, "device/skel_stencil.h")
 ACC_EMBED(stencil_nd, "device/skel_stencil_nd.h")
 ACC_EMBED(stencil_flat, "device/skel_stencil_flat.h")
 ACC_EMBED(stencil_pair, "device/skel_stencil_pair.h")
+ACC_EMBED(op_args, "operators/op_args.h")
+ACC_EMBED(op_common, "operators/op_common.h")
+ACC_EMBED(op_product, "operators/op_product.h")
+ACC_EMBED(op_route, "operators/op_route.h")
+ACC_EMBED(op_combine, "operators/op_combine.h")
+ACC_EMBED(op_micro, "operators/op_micro.h")
+ACC_EMBED(op_micro_product, "operators/op_micro_product.h")
 
 namespace acc {
 
@@ -51,6 +58,13 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"skel_stencil_nd.h", acc_embed_stencil_nd_begin, acc_embed_stencil_nd_end},
       {"skel_stencil_flat.h", acc_embed_stencil_flat_begin, acc_embed_stencil_flat_end},
       {"skel_stencil_pair.h", acc_embed_stencil_pair_begin, acc_embed_stencil_pair_end},
+      {"op_args.h", acc_embed_op_args_begin, acc_embed_op_args_end},
+      {"op_common.h", acc_embed_op_common_begin, acc_embed_op_common_end},
+      {"op_product.h", acc_embed_op_product_begin, acc_embed_op_product_end},
+      {"op_route.h", acc_embed_op_route_begin, acc_embed_op_route_end},
+      {"op_combine.h", acc_embed_op_combine_begin, acc_embed_op_combine_end},
+      {"op_micro.h", acc_embed_op_micro_begin, acc_embed_op_micro_end},
+      {"op_micro_product.h", acc_embed_op_micro_product_begin, acc_embed_op_micro_product_end},
   };
   return headers;
 }

@@ -259,6 +259,20 @@ int64_t resident(const acc_skel_s *s, int variant) { return (int64_t)s->ctx->pro
 
 }  // namespace
 
+namespace acc {
+
+int launch_operator(acc_context ctx, const char *entry, hipFunction_t fn, unsigned grid, unsigned block, unsigned lds, hipStream_t stream, void **args)
+{
+  const Running saved = t_run;
+  t_run.entry = entry;
+  t_run.dump_exec = ctx->dump_exec;
+  const hipError_t e = launch_kernel(fn, grid, 1, 1, block, 1, 1, lds, stream, args, nullptr);
+  t_run = saved;
+  return e == hipSuccess ? ACC_OK : fail_hip(e, entry);
+}
+
+}  // namespace acc
+
 extern "C" {
 
 int acc_trace_start(acc_context ctx)

@@ -1,0 +1,819 @@
+// Operators on segments of rows: the products, the router, the combination and the 4-bit numbers of a layer of experts
+// (operators/op_*.h), reached through acc_op_create and acc_exec_product_*, acc_exec_route*, acc_exec_combine*, acc_exec_micro_*.
+//
+// They are instances as the skeletons are: a few lines of definitions in front of an embedded header, compiled for the
+// device's ISA by hiprtc through the kernel cache.  An instance is made for a kind and an element type; its variants (tile
+// shapes, which way an operand lies, alignment) are compiled when a call first needs them.
+#include <algorithm>
+#include <cstring>
+#include <exception>
+#include <map>
+#include <new>
+
+#include "acc_internal.hpp"
+#include "operators/op_args.h"
+
+using acc::fail;
+
+// no exception leaves an entry point: what is thrown below them is a failure to allocate host memory
+#define ACC_OP_CATCH(who)                                                             \
+  catch (const std::bad_alloc &) { return fail(ACC_ERR_OOM, "%s: out of host memory", who); } \
+  catch (const std::exception &e) { return fail(ACC_ERR_INVALID, "%s: %s", who, e.what()); }
+
+namespace {
+
+struct OpVariant {
+  std::shared_ptr<acc::CompileJob> job;
+  hipModule_t module = nullptr;
+  hipFunction_t fn = nullptr, fn2 = nullptr, fn3 = nullptr;
+};
+
+// what an instance was asked for
+struct OpSpec {
+  int kind = 0;
+  int type = 0;                 // 0 float, 1 half, 2 bfloat16
+  int choose = 0;
+  bool normalise = true;
+};
+
+const char *const kKindName[] = {"product", "route", "combine", "micro"};
+int type_bytes(int type) { return type == 0 ? 4 : 2; }
+
+// ---- the variants of each kind ------------------------------------------------------
+
+// product: tile shapes, in waves of 64 lanes
+struct ProductTile { int bm, bn, wm, wn; };
+const ProductTile kProductTiles[] = {{16, 128, 1, 4}, {64, 128, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}};
+constexpr int kProductTileCount = 4;
+struct ProductVariant {
+  int tile = 0;
+  bool outer = false, b_fast = true, aligned = true;
+  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u); }
+};
+
+std::string product_source(const OpSpec &sp, const ProductVariant &v)
+{
+  const ProductTile &t = kProductTiles[v.tile];
+  char text[512];
+  std::snprintf(text, sizeof(text),
+                "#define OP_TYPE %d\n#define OP_BM %d\n#define OP_BN %d\n#define OP_WM %d\n#define OP_WN %d\n#define OP_OUTER %d\n"
+                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
+                sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0);
+  return text;
+}
+
+// route: how a token's logits are shared out
+struct RouteVariant {
+  int lanes = 1, per = 8, vec = 1, block = 256;
+  uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (uint32_t)vec << 16 | (uint32_t)block << 20; }
+};
+constexpr int kRouteThreads = 256, kRouteBlock = 256, kRouteMaxExperts = 2048;
+
+RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned)
+{
+  RouteVariant v;
+  const int epc = 16 / type_bytes(sp.type);
+  while (v.lanes < 64 && v.lanes * v.per < experts) v.lanes *= 2;
+  while (v.lanes * v.per < experts) v.per *= 2;
+  v.vec = aligned && experts % epc == 0 ? epc : 1;
+  v.block = kRouteBlock;
+  return v;
+}
+
+std::string route_source(const OpSpec &sp, const RouteVariant &v)
+{
+  char text[512];
+  std::snprintf(text, sizeof(text),
+                "#define OP_TYPE %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_BLOCK %d\n#define OP_THREADS %d\n"
+                "#include \"acc_hip_device.h\"\n#include \"op_route.h\"\n",
+                sp.type, v.lanes, v.per, v.vec, v.block, kRouteThreads);
+  return text;
+}
+
+constexpr int kCombineSlots = 4;
+std::string combine_source(const OpSpec &sp, bool aligned)
+{
+  char text[256];
+  std::snprintf(text, sizeof(text), "#define OP_TYPE %d\n#define OP_ALIGNED %d\n#define OP_SLOTS %d\n#include \"acc_hip_device.h\"\n#include \"op_combine.h\"\n",
+                sp.type, aligned ? 1 : 0, kCombineSlots);
+  return text;
+}
+
+std::string micro_source(const OpSpec &sp, bool aligned)
+{
+  char text[256];
+  std::snprintf(text, sizeof(text), "#define OP_TYPE %d\n#define OP_ALIGNED %d\n#include \"acc_hip_device.h\"\n#include \"op_micro.h\"\n", sp.type, aligned ? 1 : 0);
+  return text;
+}
+
+std::string micro_product_source(const OpSpec &sp)
+{
+  char text[256];
+  std::snprintf(text, sizeof(text), "#define OP_TYPE %d\n#include \"acc_hip_device.h\"\n#include \"op_micro_product.h\"\n", sp.type);
+  return text;
+}
+
+std::vector<std::string> op_options()
+{
+  // (sums of products may be contracted: nothing here has to round as a scalar expression of the array language does; packed
+  // Float32 arithmetic is off as for the skeletons)
+  return {"-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"};
+}
+
+// every translation unit an instance may need: the build check compiles them all
+std::vector<std::string> all_sources(const OpSpec &sp)
+{
+  std::vector<std::string> out;
+  if (sp.kind == ACC_OP_PRODUCT) {
+    for (int t = 0; t < kProductTileCount; ++t)
+      for (int form = 0; form < 6; ++form) {
+        ProductVariant v;
+        v.tile = t;
+        v.outer = form >= 4;
+        v.b_fast = !v.outer && (form & 1) == 0;
+        v.aligned = form >= 4 ? form == 4 : form < 2;
+        if (v.outer && t < 2) continue;
+        out.push_back(product_source(sp, v));
+      }
+  } else if (sp.kind == ACC_OP_ROUTE) {
+    for (int experts : {1, 8, 16, 32, 64, 128, 256, 512, 1024, 2048})
+      for (bool aligned : {true, false}) out.push_back(route_source(sp, route_variant(sp, experts, aligned)));
+  } else if (sp.kind == ACC_OP_COMBINE) {
+    for (bool aligned : {true, false}) out.push_back(combine_source(sp, aligned));
+  } else {
+    for (bool aligned : {true, false}) out.push_back(micro_source(sp, aligned));
+    out.push_back(micro_product_source(sp));
+  }
+  std::sort(out.begin(), out.end());
+  out.erase(std::unique(out.begin(), out.end()), out.end());
+  return out;
+}
+
+int make_spec(const acc_op_desc *d, OpSpec *sp)
+{
+  if (!d) return fail(ACC_ERR_INVALID, "acc_op_create: NULL description");
+  if (d->kind < 0 || d->kind >= ACC_OP_KIND_COUNT) return fail(ACC_ERR_INVALID, "acc_op_create: unknown kind %d", d->kind);
+  const std::string t = d->elt_type ? d->elt_type : "";
+  if (t == "float") sp->type = 0;
+  else if (t == "half") sp->type = 1;
+  else if (t == "bfloat16") sp->type = 2;
+  else return fail(ACC_ERR_INVALID, "acc_op_create: element type '%s' (float, half and bfloat16 are served)", t.c_str());
+  sp->kind = d->kind;
+  sp->choose = d->choose;
+  sp->normalise = d->normalise != 0;
+  if (d->kind == ACC_OP_ROUTE && (d->choose < 1 || d->choose > 64)) return fail(ACC_ERR_INVALID, "acc_op_create: a router chooses 1 to 64 experts, not %d", d->choose);
+  return ACC_OK;
+}
+
+// ---- arrays ---------------------------------------------------------------------------
+
+// the bytes that an array spans, and where they start
+struct Span { uint64_t from = 0, to = 0; };
+Span span_of(const acc_strided &a, int bytes)
+{
+  Span s;
+  uint64_t last = 0;
+  for (int d = 0; d < a.rank; ++d) {
+    if (a.shape[d] == 0) return s;
+    last += (uint64_t)(a.shape[d] - 1) * (uint64_t)a.stride[d];
+  }
+  s.from = a.ptr;
+  s.to = a.ptr + (last + 1) * (uint64_t)bytes;
+  return s;
+}
+
+bool is_empty(const acc_strided &a)
+{
+  for (int d = 0; d < a.rank; ++d)
+    if (a.shape[d] == 0) return true;
+  return false;
+}
+
+int check(const char *who, const char *what, const acc_strided *a, int rank)
+{
+  if (!a) return fail(ACC_ERR_INVALID, "%s: %s missing", who, what);
+  if (a->rank != rank) return fail(ACC_ERR_INVALID, "%s: %s has rank %d, expected %d", who, what, a->rank, rank);
+  for (int d = 0; d < rank; ++d) {
+    if (a->shape[d] < 0 || a->shape[d] > 0x7fffffff) return fail(ACC_ERR_INVALID, "%s: %s has an extent of %lld", who, what, (long long)a->shape[d]);
+    if (a->stride[d] < 0) return fail(ACC_ERR_INVALID, "%s: %s has a negative stride", who, what);
+  }
+  if (!a->ptr && !is_empty(*a)) return fail(ACC_ERR_INVALID, "%s: %s is NULL", who, what);
+  return ACC_OK;
+}
+
+// dimension d moves by one element (or does not move at all)
+bool unit(const acc_strided &a, int d) { return a.shape[d] <= 1 || a.stride[d] == 1; }
+
+int check_unit(const char *who, const char *what, const acc_strided *a, int rank)
+{
+  ACC_TRY(check(who, what, a, rank));
+  if (!unit(*a, rank - 1)) return fail(ACC_ERR_INVALID, "%s: the innermost dimension of %s is not contiguous", who, what);
+  return ACC_OK;
+}
+
+// rows of a result must not lie on one another
+int check_result(const char *who, const char *what, const acc_strided *a, int rank)
+{
+  ACC_TRY(check_unit(who, what, a, rank));
+  int64_t least = a->shape[rank - 1];
+  for (int d = rank - 2; d >= 0; --d) {
+    if (a->shape[d] > 1 && a->stride[d] < least) return fail(ACC_ERR_INVALID, "%s: rows of %s overlap", who, what);
+    least = std::max(least, a->stride[d] * std::max<int64_t>(1, a->shape[d]));
+  }
+  return ACC_OK;
+}
+
+int check_shape(const char *who, const char *what, const acc_strided &a, std::initializer_list<int64_t> shape)
+{
+  int d = 0;
+  for (int64_t s : shape) {
+    if (a.shape[d] != s) return fail(ACC_ERR_INVALID, "%s: dimension %d of %s is %lld, expected %lld", who, d, what, (long long)a.shape[d], (long long)s);
+    ++d;
+  }
+  return ACC_OK;
+}
+
+struct Named { const acc_strided *a; int bytes; const char *what; };
+int check_apart(const char *who, const Named &out, std::initializer_list<Named> others)
+{
+  const Span o = span_of(*out.a, out.bytes);
+  for (const Named &n : others) {
+    if (!n.a) continue;
+    const Span s = span_of(*n.a, n.bytes);
+    if (s.from < o.to && o.from < s.to) return fail(ACC_ERR_INVALID, "%s: %s shares memory with %s", who, out.what, n.what);
+  }
+  return ACC_OK;
+}
+
+// every row of an array starts on 16 bytes
+bool aligned_rows(const acc_strided &a, int bytes, int inner)
+{
+  if (a.ptr & 15u) return false;
+  for (int d = 0; d < a.rank; ++d)
+    if (d != inner && a.shape[d] > 1 && (a.stride[d] * bytes) % 16 != 0) return false;
+  return true;
+}
+
+template <typename T> T *device(const acc_strided *a) { return a ? reinterpret_cast<T *>(a->ptr) : nullptr; }
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// tiles of `height` rows that cover the segments, whatever their lengths: every segment with a row (and the rows before the
+// first and behind the last) may end amid a tile
+int64_t tiles_at_most(int64_t rows, int64_t experts, int64_t height)
+{
+  const int64_t parts = std::min(rows, experts + 2);
+  return (rows + parts * (height - 1)) / height;
+}
+
+}  // namespace
+
+struct acc_op_s {
+  acc_context ctx = nullptr;
+  OpSpec spec;
+  std::mutex mu;
+  std::map<uint32_t, OpVariant> variants;
+
+  // the kernels of a variant: compiled, loaded, `names` looked up (fn, fn2, fn3 in that order)
+  int variant(uint32_t key, const char *const *names, int n_names, std::string (*source)(const OpSpec &, uint32_t), const OpVariant **out);
+};
+
+namespace {
+
+std::string product_source_of(const OpSpec &sp, uint32_t key)
+{
+  ProductVariant v;
+  v.tile = (int)(key & 15u);
+  v.outer = key & 16u;
+  v.b_fast = key & 32u;
+  v.aligned = key & 64u;
+  return product_source(sp, v);
+}
+std::string route_source_of(const OpSpec &sp, uint32_t key)
+{
+  RouteVariant v;
+  v.lanes = (int)(key & 255u);
+  v.per = (int)(key >> 8 & 255u);
+  v.vec = (int)(key >> 16 & 15u);
+  v.block = (int)(key >> 20);
+  return route_source(sp, v);
+}
+std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_source(sp, key & 1u); }
+std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & 2u) ? micro_product_source(sp) : micro_source(sp, key & 1u); }
+
+const char *const kProductNames[] = {"product"};
+const char *const kRouteNames[] = {"route", "route_place", "route_gradient"};
+const char *const kCombineNames[] = {"combine", "combine_gradient"};
+const char *const kMicroNames[] = {"micro_quantise", "micro_values"};
+const char *const kMicroProductNames[] = {"micro_product"};
+
+// one call's stream and its guard (a loop enqueued ahead, see acc_guard_create)
+int begin(acc_op op, int kind, const char *who, acc_stream stream, const uint32_t **guard)
+{
+  if (!op) return fail(ACC_ERR_INVALID, "%s: NULL operator", who);
+  if (op->spec.kind != kind) return fail(ACC_ERR_INVALID, "%s: the operator is a '%s'", who, kKindName[op->spec.kind]);
+  *guard = reinterpret_cast<const uint32_t *>(op->ctx->guard_of(static_cast<hipStream_t>(stream)));
+  return op->ctx->make_current();
+}
+
+template <typename T>
+int launch(acc_op op, const char *entry, hipFunction_t fn, int64_t grid, int block, size_t lds, acc_stream stream, const T &args)
+{
+  if (grid < 1 || grid > 0x7fffffffLL) return fail(ACC_ERR_INVALID, "%s: grid of %lld workgroups", entry, (long long)grid);
+  T copy = args;
+  void *slots[] = {&copy};
+  return acc::launch_operator(op->ctx, entry, fn, static_cast<unsigned>(grid), static_cast<unsigned>(block), static_cast<unsigned>(lds),
+                              static_cast<hipStream_t>(stream), slots);
+}
+
+}  // namespace
+
+int acc_op_s::variant(uint32_t key, const char *const *names, int n_names, std::string (*source)(const OpSpec &, uint32_t), const OpVariant **out)
+{
+  std::lock_guard<std::mutex> lock(mu);
+  OpVariant &v = variants[key];              // (a map's elements stay where they are)
+  if (!v.fn) {
+    if (!v.job) {
+      auto job = std::make_shared<acc::CompileJob>();
+      job->target = ctx->arch;
+      job->source = source(spec, key);
+      job->options = op_options();
+      v.job = job;
+      job->run();
+    }
+    ACC_TRY(v.job->wait());
+    ACC_TRY(ctx->make_current());
+    hipModule_t module = nullptr;
+    ACC_HIP_TRY(hipModuleLoadData(&module, v.job->code));
+    hipFunction_t fn[3] = {nullptr, nullptr, nullptr};
+    for (int k = 0; k < n_names; ++k) {
+      const hipError_t e = hipModuleGetFunction(&fn[k], module, names[k]);
+      if (e != hipSuccess) {
+        (void)hipModuleUnload(module);
+        return acc::fail_hip(e, names[k]);
+      }
+    }
+    v.module = module;
+    v.fn2 = fn[1];
+    v.fn3 = fn[2];
+    v.fn = fn[0];
+  }
+  *out = &v;
+  return ACC_OK;
+}
+
+extern "C" {
+
+int acc_op_create(acc_context ctx, const acc_op_desc *desc, acc_op *out)
+try {
+  if (!ctx || !out) return fail(ACC_ERR_INVALID, "acc_op_create: NULL argument");
+  *out = nullptr;
+  OpSpec sp;
+  ACC_TRY(make_spec(desc, &sp));
+  acc_op_s *op = new acc_op_s();
+  op->ctx = ctx;
+  op->spec = sp;
+  *out = op;
+  return ACC_OK;
+} ACC_OP_CATCH("acc_op_create")
+
+int acc_op_destroy(acc_op op)
+try {
+  if (!op) return ACC_OK;
+  (void)op->ctx->make_current();
+  for (auto &kv : op->variants)
+    if (kv.second.module) (void)hipModuleUnload(kv.second.module);
+  delete op;
+  return ACC_OK;
+} ACC_OP_CATCH("acc_op_destroy")
+
+int acc_op_compile_only(const char *target, const acc_op_desc *desc, int32_t *units, size_t *code_size)
+try {
+  if (!target || !units || !code_size) return fail(ACC_ERR_INVALID, "acc_op_compile_only: NULL argument");
+  OpSpec sp;
+  ACC_TRY(make_spec(desc, &sp));
+  *units = 0;
+  *code_size = 0;
+  std::vector<std::shared_ptr<acc::CompileJob>> jobs;
+  for (const std::string &text : all_sources(sp)) {
+    auto job = std::make_shared<acc::CompileJob>();
+    job->target = target;
+    job->source = text;
+    job->options = op_options();
+    if (!acc::compile_submit(job)) job->run();
+    jobs.push_back(job);
+  }
+  int rc = ACC_OK;
+  for (auto &job : jobs) {
+    const int one = job->wait();
+    if (one != ACC_OK) rc = one;
+    *code_size += job->size;
+    ++*units;
+  }
+  return rc;
+} ACC_OP_CATCH("acc_op_compile_only")
+
+// ---- products -----------------------------------------------------------------------
+
+int acc_exec_product_rows(acc_op op, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
+                          const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_product_rows";
+  acc_product_args a = {};
+  ACC_TRY(begin(op, ACC_OP_PRODUCT, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "x", x, 2));
+  ACC_TRY(check(who, "w", w, 3));
+  ACC_TRY(check_unit(who, "offsets", offsets, 1));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  if (index) ACC_TRY(check_unit(who, "index", index, 1));
+  const int64_t experts = w->shape[0], n = w->shape[1], k = w->shape[2], rows = out->shape[0];
+  if (!unit(*w, 2) && !unit(*w, 1)) return fail(ACC_ERR_INVALID, "%s: neither the second nor the third dimension of w is contiguous", who);
+  if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
+  ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
+  ACC_TRY(check_shape(who, "the result", *out, {rows, n}));
+  if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
+  ACC_TRY(check_shape(who, "x", *x, {index ? x->shape[0] : rows, k}));
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "x"}, {w, bytes, "w"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
+  if (rows == 0 || n == 0) return ACC_OK;
+
+  ProductVariant v;
+  // (where both are contiguous -- one column, or a sum of one -- either way of reading will do)
+  v.b_fast = unit(*w, 2);
+  v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0);
+  const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
+  v.tile = mean <= 24 ? 0 : mean <= 96 ? 1 : mean < 512 || n < 256 ? 2 : 3;
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
+  const ProductTile &t = kProductTiles[v.tile];
+  a.a = device<const void>(x);
+  a.b = device<const void>(w);
+  a.out = device<void>(out);
+  a.offsets = device<const int32_t>(offsets);
+  a.index_a = device<const int32_t>(index);
+  a.a_stride = x->stride[0];
+  a.b_stride = w->stride[v.b_fast ? 1 : 2];
+  a.b_expert = w->stride[0];
+  a.out_stride = out->stride[0];
+  a.rows = rows;
+  a.a_rows = x->shape[0];
+  a.nj = (int32_t)n;
+  a.k = (int32_t)k;
+  a.experts = (int32_t)experts;
+  a.per = per;
+  a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
+  a.tiles_j = (int32_t)ceil_div(n, t.bn);
+  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_product_rows")
+
+int acc_exec_product_outer(acc_op op, const acc_strided *x, const acc_strided *y, const acc_strided *offsets, const acc_strided *index, int32_t per,
+                           const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_product_outer";
+  acc_product_args a = {};
+  ACC_TRY(begin(op, ACC_OP_PRODUCT, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "a", x, 2));
+  ACC_TRY(check_unit(who, "b", y, 2));
+  ACC_TRY(check_unit(who, "offsets", offsets, 1));
+  ACC_TRY(check(who, "the result", out, 3));
+  if (index) ACC_TRY(check_unit(who, "index", index, 1));
+  if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
+  const int64_t experts = out->shape[0], rows = x->shape[0];
+  ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
+  ACC_TRY(check_shape(who, "the result", *out, {experts, x->shape[1], y->shape[1]}));
+  if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
+  else ACC_TRY(check_shape(who, "b", *y, {rows, y->shape[1]}));
+  // the result's rows may run along either dimension: the other way round the operands change places
+  const bool turned = !unit(*out, 2);
+  acc_strided o = *out;
+  if (turned) {
+    std::swap(o.shape[1], o.shape[2]);
+    std::swap(o.stride[1], o.stride[2]);
+  }
+  ACC_TRY(check_result(who, "the result", &o, 3));
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "a"}, {y, bytes, "b"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
+  if (is_empty(o)) return ACC_OK;
+  const acc_strided *p = turned ? y : x, *q = turned ? x : y;
+
+  ProductVariant v;
+  v.outer = true;
+  v.b_fast = false;
+  v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1);
+  v.tile = o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2;
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
+  const ProductTile &t = kProductTiles[v.tile];
+  a.a = device<const void>(p);
+  a.b = device<const void>(q);
+  a.out = device<void>(out);
+  a.offsets = device<const int32_t>(offsets);
+  (turned ? a.index_a : a.index_b) = device<const int32_t>(index);
+  a.a_stride = p->stride[0];
+  a.b_stride = q->stride[0];
+  a.out_expert = o.stride[0];
+  a.out_stride = o.stride[1];
+  a.rows = rows;
+  a.a_rows = p->shape[0];
+  a.b_rows = q->shape[0];
+  a.ni = (int32_t)o.shape[1];
+  a.nj = (int32_t)o.shape[2];
+  a.experts = (int32_t)experts;
+  a.per = per;
+  a.tiles_i = (int32_t)ceil_div(o.shape[1], t.bm);
+  a.tiles_j = (int32_t)ceil_div(o.shape[2], t.bn);
+  return launch(op, who, var->fn, experts * a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_product_outer")
+
+// ---- router ---------------------------------------------------------------------------
+
+static size_t route_lds(int64_t experts) { return (size_t)(kRouteThreads / 64 + 2) * (size_t)experts * 4; }
+
+int acc_exec_route(acc_op op, const acc_strided *logits, const acc_strided *chosen, const acc_strided *weights, const acc_strided *offsets,
+                   const acc_strided *order, const acc_strided *place, acc_stream stream)
+try {
+  const char *who = "acc_exec_route";
+  acc_route_args a = {};
+  ACC_TRY(begin(op, ACC_OP_ROUTE, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "logits", logits, 2));
+  ACC_TRY(check_result(who, "experts", chosen, 2));
+  ACC_TRY(check_result(who, "weights", weights, 2));
+  ACC_TRY(check_result(who, "offsets", offsets, 1));
+  ACC_TRY(check_result(who, "order", order, 1));
+  ACC_TRY(check_result(who, "place", place, 2));
+  const int64_t tokens = logits->shape[0], experts = logits->shape[1], choose = op->spec.choose;
+  if (experts < choose || experts > kRouteMaxExperts)
+    return fail(ACC_ERR_INVALID, "%s: %lld experts (at least the %lld that are chosen, and at most %d)", who, (long long)experts, (long long)choose, kRouteMaxExperts);
+  ACC_TRY(check_shape(who, "experts", *chosen, {tokens, choose}));
+  ACC_TRY(check_shape(who, "weights", *weights, {tokens, choose}));
+  ACC_TRY(check_shape(who, "place", *place, {tokens, choose}));
+  ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
+  ACC_TRY(check_shape(who, "order", *order, {tokens * choose}));
+  for (const acc_strided *t : {chosen, weights, place})
+    if (tokens > 1 && t->stride[0] != choose) return fail(ACC_ERR_INVALID, "%s: experts, weights and place are dense arrays", who);
+  const int bytes = type_bytes(op->spec.type);
+  const Named all[] = {{chosen, 4, "experts"}, {weights, 4, "weights"}, {offsets, 4, "offsets"}, {order, 4, "order"}, {place, 4, "place"}};
+  for (int k = 0; k < 5; ++k) {
+    ACC_TRY(check_apart(who, all[k], {{logits, bytes, "logits"}}));
+    for (int m = 0; m < k; ++m) ACC_TRY(check_apart(who, all[k], {all[m]}));
+  }
+  const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1));
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kRouteNames, 3, route_source_of, &var));
+  a.logits = device<const void>(logits);
+  a.chosen = device<int32_t>(chosen);
+  a.weights = device<float>(weights);
+  a.offsets = device<int32_t>(offsets);
+  a.order = device<int32_t>(order);
+  a.place = device<int32_t>(place);
+  a.tokens = tokens;
+  a.logits_stride = logits->stride[0];
+  a.experts = (int32_t)experts;
+  a.choose = (int32_t)choose;
+  a.normalise = op->spec.normalise ? 1 : 0;
+  a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, v.block));
+  acc::ScratchRef scratch;
+  if (a.blocks > 1) {
+    ACC_TRY(op->ctx->scratch_acquire((size_t)a.blocks * (size_t)experts * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+    a.counts = static_cast<uint32_t *>(scratch.ptr);
+  }
+  int rc = launch(op, who, var->fn, a.blocks, kRouteThreads, route_lds(experts), stream, a);
+  if (rc == ACC_OK && a.blocks > 1) rc = launch(op, who, var->fn2, a.blocks, kRouteThreads, route_lds(experts), stream, a);
+  if (a.blocks > 1) op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));
+  return rc;
+} ACC_OP_CATCH("acc_exec_route")
+
+int acc_exec_route_gradient(acc_op op, const acc_strided *logits, const acc_strided *chosen, const acc_strided *weights, const acc_strided *dweights,
+                            const acc_strided *dlogits, acc_stream stream)
+try {
+  const char *who = "acc_exec_route_gradient";
+  acc_route_args a = {};
+  ACC_TRY(begin(op, ACC_OP_ROUTE, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "logits", logits, 2));
+  ACC_TRY(check_unit(who, "experts", chosen, 2));
+  ACC_TRY(check_unit(who, "weights", weights, 2));
+  ACC_TRY(check_unit(who, "dweights", dweights, 2));
+  ACC_TRY(check_result(who, "dlogits", dlogits, 2));
+  const int64_t tokens = logits->shape[0], experts = logits->shape[1], choose = op->spec.choose;
+  if (experts < choose || experts > kRouteMaxExperts)
+    return fail(ACC_ERR_INVALID, "%s: %lld experts (at least the %lld that are chosen, and at most %d)", who, (long long)experts, (long long)choose, kRouteMaxExperts);
+  ACC_TRY(check_shape(who, "experts", *chosen, {tokens, choose}));
+  ACC_TRY(check_shape(who, "weights", *weights, {tokens, choose}));
+  ACC_TRY(check_shape(who, "dweights", *dweights, {tokens, choose}));
+  ACC_TRY(check_shape(who, "dlogits", *dlogits, {tokens, experts}));
+  for (const acc_strided *t : {chosen, weights, dweights})
+    if (tokens > 1 && t->stride[0] != choose) return fail(ACC_ERR_INVALID, "%s: experts, weights and dweights are dense arrays", who);
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {dlogits, bytes, "dlogits"}, {{logits, bytes, "logits"}, {chosen, 4, "experts"}, {weights, 4, "weights"}, {dweights, 4, "dweights"}}));
+  if (tokens == 0) return ACC_OK;
+  const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1) && aligned_rows(*dlogits, bytes, 1));
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kRouteNames, 3, route_source_of, &var));
+  a.logits = device<const void>(logits);
+  a.chosen = device<int32_t>(chosen);
+  a.weights = device<float>(weights);
+  a.dweights = device<const float>(dweights);
+  a.dlogits = device<void>(dlogits);
+  a.tokens = tokens;
+  a.logits_stride = logits->stride[0];
+  a.dlogits_stride = dlogits->stride[0];
+  a.experts = (int32_t)experts;
+  a.choose = (int32_t)choose;
+  a.normalise = op->spec.normalise ? 1 : 0;
+  return launch(op, who, var->fn3, ceil_div(tokens, kRouteThreads / v.lanes), kRouteThreads, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_route_gradient")
+
+// ---- combination ----------------------------------------------------------------------
+
+static int check_slots(const char *who, const acc_strided *place, const acc_strided *weights, int64_t tokens)
+{
+  ACC_TRY(check_unit(who, "place", place, 2));
+  ACC_TRY(check_shape(who, "place", *place, {tokens, place->shape[1]}));
+  if (tokens > 1 && place->stride[0] != place->shape[1]) return fail(ACC_ERR_INVALID, "%s: place is a dense array", who);
+  if (!weights) return ACC_OK;
+  ACC_TRY(check_unit(who, "weights", weights, 2));
+  ACC_TRY(check_shape(who, "weights", *weights, {tokens, place->shape[1]}));
+  if (tokens > 1 && weights->stride[0] != weights->shape[1]) return fail(ACC_ERR_INVALID, "%s: weights is a dense array", who);
+  return ACC_OK;
+}
+
+int acc_exec_combine(acc_op op, const acc_strided *y, const acc_strided *place, const acc_strided *weights, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_combine";
+  acc_combine_args a = {};
+  ACC_TRY(begin(op, ACC_OP_COMBINE, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "y", y, 2));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  const int64_t tokens = out->shape[0], width = out->shape[1];
+  ACC_TRY(check_slots(who, place, weights, tokens));
+  ACC_TRY(check_shape(who, "y", *y, {y->shape[0], width}));
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{y, bytes, "y"}, {place, 4, "place"}, {weights, 4, "weights"}}));
+  if (is_empty(*out)) return ACC_OK;
+  const bool aligned = width % epc == 0 && aligned_rows(*y, bytes, 1) && aligned_rows(*out, bytes, 1);
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(aligned ? 1u : 0u, kCombineNames, 2, combine_source_of, &var));
+  a.y = device<const void>(y);
+  a.out = device<void>(out);
+  a.place = device<const int32_t>(place);
+  a.weights = device<const float>(weights);
+  a.tokens = tokens;
+  a.y_rows = y->shape[0];
+  a.y_stride = y->stride[0];
+  a.out_stride = out->stride[0];
+  a.choose = (int32_t)place->shape[1];
+  a.width = (int32_t)width;
+  return launch(op, who, var->fn, ceil_div(tokens * ceil_div(width, 8), 256), 256, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_combine")
+
+int acc_exec_combine_gradient(acc_op op, const acc_strided *dout, const acc_strided *y, const acc_strided *place, const acc_strided *weights,
+                              const acc_strided *dy, const acc_strided *dweights, acc_stream stream)
+try {
+  const char *who = "acc_exec_combine_gradient";
+  acc_combine_args a = {};
+  ACC_TRY(begin(op, ACC_OP_COMBINE, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "dout", dout, 2));
+  ACC_TRY(check_result(who, "dy", dy, 2));
+  const int64_t tokens = dout->shape[0], width = dout->shape[1];
+  ACC_TRY(check_slots(who, place, weights, tokens));
+  ACC_TRY(check_shape(who, "dy", *dy, {dy->shape[0], width}));
+  if ((dweights != nullptr) != (y != nullptr)) return fail(ACC_ERR_INVALID, "%s: y and dweights go together", who);
+  if (y) {
+    ACC_TRY(check_unit(who, "y", y, 2));
+    ACC_TRY(check_shape(who, "y", *y, {dy->shape[0], width}));
+    ACC_TRY(check_result(who, "dweights", dweights, 2));
+    ACC_TRY(check_shape(who, "dweights", *dweights, {tokens, place->shape[1]}));
+    if (tokens > 1 && dweights->stride[0] != dweights->shape[1]) return fail(ACC_ERR_INVALID, "%s: dweights is a dense array", who);
+  }
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  ACC_TRY(check_apart(who, {dy, bytes, "dy"}, {{dout, bytes, "dout"}, {y, bytes, "y"}, {place, 4, "place"}, {weights, 4, "weights"}, {dweights, 4, "dweights"}}));
+  if (dweights) ACC_TRY(check_apart(who, {dweights, 4, "dweights"}, {{dout, bytes, "dout"}, {y, bytes, "y"}, {place, 4, "place"}, {weights, 4, "weights"}}));
+  if (tokens == 0 || place->shape[1] == 0) return ACC_OK;
+  const bool aligned = width % epc == 0 && aligned_rows(*dout, bytes, 1) && aligned_rows(*dy, bytes, 1) && (!y || aligned_rows(*y, bytes, 1));
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(aligned ? 1u : 0u, kCombineNames, 2, combine_source_of, &var));
+  a.y = device<const void>(y);
+  a.dout = device<const void>(dout);
+  a.out = device<void>(dy);
+  a.place = device<const int32_t>(place);
+  a.weights = device<const float>(weights);
+  a.dweights = device<float>(dweights);
+  a.tokens = tokens;
+  a.y_rows = dy->shape[0];
+  a.y_stride = y ? y->stride[0] : 0;
+  a.out_stride = dy->stride[0];
+  a.dout_stride = dout->stride[0];
+  a.choose = (int32_t)place->shape[1];
+  a.width = (int32_t)width;
+  return launch(op, who, var->fn2, ceil_div(tokens, 4), 256, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_combine_gradient")
+
+// ---- 4-bit numbers --------------------------------------------------------------------
+
+// codes and scales of `rows` rows of `k` elements (in `batches` matrices where the arrays have rank 3)
+static int check_micro(const char *who, const char *what, const acc_strided *codes, const acc_strided *scales, int rank, bool result)
+{
+  ACC_TRY(result ? check_result(who, what, codes, rank) : check_unit(who, what, codes, rank));
+  ACC_TRY(result ? check_result(who, what, scales, rank) : check_unit(who, what, scales, rank));
+  for (int d = 0; d < rank - 1; ++d)
+    if (codes->shape[d] != scales->shape[d]) return fail(ACC_ERR_INVALID, "%s: %s: codes of %lld rows, scales of %lld", who, what, (long long)codes->shape[d], (long long)scales->shape[d]);
+  if (codes->shape[rank - 1] != 16 * scales->shape[rank - 1])
+    return fail(ACC_ERR_INVALID, "%s: %s: a row of %lld bytes of codes and %lld scales (16 bytes a scale)", who, what, (long long)codes->shape[rank - 1], (long long)scales->shape[rank - 1]);
+  if (!aligned_rows(*codes, 1, rank - 1)) return fail(ACC_ERR_INVALID, "%s: %s: rows of codes start on 16 bytes", who, what);
+  return ACC_OK;
+}
+
+static int micro_elements(acc_op op, const char *who, bool back, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, acc_stream stream, acc_micro_args a)
+{
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  const int64_t rows = x->shape[0], k = x->shape[1], blocks = ceil_div(k, 32);
+  ACC_TRY(check_shape(who, "codes", *codes, {rows, 16 * blocks}));
+  if (is_empty(*x)) return ACC_OK;
+  const bool aligned = k % epc == 0 && aligned_rows(*x, bytes, 1);
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(aligned ? 1u : 0u, kMicroNames, 2, micro_source_of, &var));
+  a.x = device<const void>(x);
+  a.out = device<void>(x);
+  a.codes = device<uint8_t>(codes);
+  a.scales = device<uint8_t>(scales);
+  a.rows = rows;
+  a.x_stride = x->stride[0];
+  a.codes_stride = codes->stride[0];
+  a.scales_stride = scales->stride[0];
+  a.k = (int32_t)k;
+  a.blocks = (int32_t)blocks;
+  return launch(op, who, back ? var->fn2 : var->fn, ceil_div(rows * blocks * 4, 256), 256, 0, stream, a);
+}
+
+int acc_exec_micro_quantise(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, acc_stream stream)
+try {
+  const char *who = "acc_exec_micro_quantise";
+  acc_micro_args a = {};
+  ACC_TRY(begin(op, ACC_OP_MICRO, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "x", x, 2));
+  ACC_TRY(check_micro(who, "the result", codes, scales, 2, true));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {codes, 1, "codes"}, {{x, bytes, "x"}, {scales, 1, "scales"}}));
+  ACC_TRY(check_apart(who, {scales, 1, "scales"}, {{x, bytes, "x"}}));
+  return micro_elements(op, who, false, x, codes, scales, stream, a);
+} ACC_OP_CATCH("acc_exec_micro_quantise")
+
+int acc_exec_micro_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_micro_values";
+  acc_micro_args a = {};
+  ACC_TRY(begin(op, ACC_OP_MICRO, who, stream, &a.guard));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  ACC_TRY(check_micro(who, "x", codes, scales, 2, false));
+  ACC_TRY(check_apart(who, {out, type_bytes(op->spec.type), "the result"}, {{codes, 1, "codes"}, {scales, 1, "scales"}}));
+  return micro_elements(op, who, true, out, codes, scales, stream, a);
+} ACC_OP_CATCH("acc_exec_micro_values")
+
+int acc_exec_micro_rows(acc_op op, const acc_strided *xcodes, const acc_strided *xscales, const acc_strided *wcodes, const acc_strided *wscales,
+                        const acc_strided *offsets, const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_micro_rows";
+  acc_micro_product_args a = {};
+  ACC_TRY(begin(op, ACC_OP_MICRO, who, stream, &a.guard));
+  ACC_TRY(check_micro(who, "x", xcodes, xscales, 2, false));
+  ACC_TRY(check_micro(who, "w", wcodes, wscales, 3, false));
+  ACC_TRY(check_unit(who, "offsets", offsets, 1));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  if (index) ACC_TRY(check_unit(who, "index", index, 1));
+  if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
+  const int64_t experts = wscales->shape[0], n = wscales->shape[1], blocks = wscales->shape[2], rows = out->shape[0];
+  ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
+  ACC_TRY(check_shape(who, "the result", *out, {rows, n}));
+  if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
+  ACC_TRY(check_shape(who, "x", *xscales, {index ? xscales->shape[0] : rows, blocks}));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{xcodes, 1, "x"}, {xscales, 1, "x's scales"}, {wcodes, 1, "w"}, {wscales, 1, "w's scales"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
+  if (is_empty(*out)) return ACC_OK;
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(2u, kMicroProductNames, 1, micro_source_of, &var));
+  a.a = device<const uint8_t>(xcodes);
+  a.sa = device<const uint8_t>(xscales);
+  a.b = device<const uint8_t>(wcodes);
+  a.sb = device<const uint8_t>(wscales);
+  a.out = device<void>(out);
+  a.offsets = device<const int32_t>(offsets);
+  a.index = device<const int32_t>(index);
+  a.a_stride = xcodes->stride[0];
+  a.sa_stride = xscales->stride[0];
+  a.b_stride = wcodes->stride[1];
+  a.sb_stride = wscales->stride[1];
+  a.b_expert = wcodes->stride[0];
+  a.sb_expert = wscales->stride[0];
+  a.out_stride = out->stride[0];
+  a.rows = rows;
+  a.a_rows = xscales->shape[0];
+  a.n = (int32_t)n;
+  a.blocks = (int32_t)blocks;
+  a.experts = (int32_t)experts;
+  a.per = per;
+  a.tiles_i = (int32_t)tiles_at_most(rows, experts, 16);
+  a.tiles_j = (int32_t)ceil_div(n, 256);
+  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 256, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_micro_rows")
+
+}  // extern "C"

@@ -1,0 +1,77 @@
+/*
+ * op_common.h -- what the operators' kernels share: element types and the segments of rows.
+ */
+#ifndef ACC_OP_COMMON_H
+#define ACC_OP_COMMON_H
+
+#include "op_args.h"
+
+typedef unsigned int acc_u4 __attribute__((ext_vector_type(4)));
+typedef unsigned int acc_u2 __attribute__((ext_vector_type(2)));
+typedef float acc_f4 __attribute__((ext_vector_type(4)));
+
+/* OP_TYPE: 0 float, 1 half, 2 bfloat16 */
+#if OP_TYPE == 0
+typedef float op_elt;
+#elif OP_TYPE == 1
+typedef _Float16 op_elt;
+#else
+typedef __bf16 op_elt;
+#endif
+#define OP_SIZE ((int)sizeof(op_elt))
+#define OP_EPC (16 / OP_SIZE)            /* elements of a chunk of 16 bytes */
+
+/* 16 bytes of memory that need not be aligned */
+struct __attribute__((packed, aligned(OP_SIZE))) op_loose { acc_u4 v; };
+
+/* `valid` elements from p on, zeros behind them; p may be anywhere if valid <= 0 */
+template <bool ALIGNED> ACC_DEV acc_u4 op_chunk(const op_elt *p, const int valid)
+{
+  if (ALIGNED) return valid > 0 ? *(const acc_u4 *)p : acc_u4{0, 0, 0, 0};
+  if (valid >= OP_EPC) return ((const op_loose *)p)->v;
+  op_elt e[OP_EPC];
+#pragma unroll
+  for (int k = 0; k < OP_EPC; ++k) e[k] = k < valid ? p[k] : (op_elt)0.0f;
+  acc_u4 v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
+}
+
+/* The segments of the rows 0 .. rows-1: number 0 is what lies before the first expert's rows, s the rows of expert s - 1,
+ * experts + 1 what lies behind the last one's.  Starts that are out of range or out of order are pulled into it, so that no
+ * row outside the array is ever named. */
+ACC_DEV void op_segment(const int *offsets, const int experts, const int rows, const int s, int *begin, int *end)
+{
+  const int b = s <= 0 ? 0 : offsets[s - 1], e = s > experts ? rows : offsets[s];
+  *begin = acc_min(acc_max(b, 0), rows);
+  *end = acc_max(*begin, acc_min(e, rows));
+}
+
+struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segment; begin >= end: no such tile */
+
+/* The `tile`-th run of up to `height` rows, counted segment after segment: a wave adds up the runs of 64 segments at a
+ * time.  Every wave of a workgroup works it out for itself, and the answer is the same in every lane. */
+ACC_DEV op_tile op_find_tile(const int *offsets, const int experts, const int rows, const int height, int tile)
+{
+  const int lane = acc_lane();
+  op_tile t = {-1, 0, 0};
+  for (int base = 0; base < experts + 2; base += 64) {
+    int b = 0, e = 0;
+    if (base + lane < experts + 2) op_segment(offsets, experts, rows, base + lane, &b, &e);
+    const int runs = (e - b + height - 1) / height;
+    const int upto = acc_wave_scan(runs, [](int x, int y) { return x + y; }, lane);
+    const unsigned long long beyond = __ballot(upto > tile);
+    if (beyond) {
+      const int at = __builtin_ctzll(beyond);
+      const int first = acc_readlane(b, at) + (tile - (acc_readlane(upto, at) - acc_readlane(runs, at))) * height;
+      t.begin = first;
+      t.end = acc_min(acc_readlane(e, at), first + height);
+      t.expert = base + at == experts + 1 ? -1 : base + at - 1;
+      return t;
+    }
+    tile -= acc_readlane(upto, 63);
+  }
+  return t;
+}
+
+#endif

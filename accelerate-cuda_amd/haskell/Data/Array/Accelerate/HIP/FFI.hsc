@@ -30,10 +30,12 @@ data CContext
 data CSkel
 data CMemTable
 data CGuard
+data COp
 type Context  = Ptr CContext
 type Skel     = Ptr CSkel
 type MemTable = Ptr CMemTable
 type Guard    = Ptr CGuard
+type Op       = Ptr COp
 type Stream   = Ptr ()               -- hipStream_t; nullPtr is the default stream
 type Event    = Ptr ()
 type Module   = Ptr ()
@@ -449,3 +451,67 @@ foreign import ccall safe   "acc_memtable_free"             c_memtableFree      
 foreign import ccall safe   "acc_memtable_insert_unmanaged" c_memtableInsertUnmanaged :: MemTable -> Word64 -> DevPtr -> Word64 -> IO Status
 foreign import ccall safe   "acc_memtable_reclaim"          c_memtableReclaim         :: MemTable -> IO Status
 foreign import ccall safe   "acc_memtable_get_stats"        c_memtableGetStats        :: MemTable -> Ptr MemTableStats -> IO Status
+
+-- Operators on segments of rows: products, routing, combination, 4-bit numbers.  An array of theirs has strides.
+accOpProduct, accOpRoute, accOpCombine, accOpMicro :: CInt
+accOpProduct = #{const ACC_OP_PRODUCT}
+accOpRoute   = #{const ACC_OP_ROUTE}
+accOpCombine = #{const ACC_OP_COMBINE}
+accOpMicro   = #{const ACC_OP_MICRO}
+
+data Strided = Strided
+  { stridedShape  :: [Int64]          -- outermost first
+  , stridedStride :: [Int64]          -- in elements
+  , stridedPtr    :: DevPtr
+  }
+
+instance Storable Strided where
+  sizeOf    _ = #{size acc_strided}
+  alignment _ = 8
+  peek p = do
+    r  <- fromIntegral `fmap` (#{peek acc_strided, rank} p :: IO Int32)
+    sh <- peekArray r (#{ptr acc_strided, shape} p)
+    st <- peekArray r (#{ptr acc_strided, stride} p)
+    d  <- #{peek acc_strided, ptr} p
+    return (Strided sh st d)
+  poke p (Strided sh st d) = do
+    fillBytes p 0 #{size acc_strided}
+    #{poke acc_strided, rank} p (fromIntegral (length sh) :: Int32)
+    pokeArray (#{ptr acc_strided, shape} p) sh
+    pokeArray (#{ptr acc_strided, stride} p) st
+    #{poke acc_strided, ptr} p d
+
+data OpDesc = OpDesc
+  { opKind      :: CInt
+  , opEltType   :: CString            -- "float", "half" or "bfloat16"
+  , opChoose    :: Int32
+  , opNormalise :: Bool
+  }
+
+instance Storable OpDesc where
+  sizeOf    _ = #{size acc_op_desc}
+  alignment _ = 8
+  peek p = do
+    k <- #{peek acc_op_desc, kind} p :: IO Int32
+    t <- #{peek acc_op_desc, elt_type} p
+    c <- #{peek acc_op_desc, choose} p
+    n <- #{peek acc_op_desc, normalise} p :: IO Int32
+    return (OpDesc (fromIntegral k) t c (n /= 0))
+  poke p (OpDesc k t c n) = do
+    #{poke acc_op_desc, kind} p (fromIntegral k :: Int32)
+    #{poke acc_op_desc, elt_type} p t
+    #{poke acc_op_desc, choose} p c
+    #{poke acc_op_desc, normalise} p (if n then 1 else 0 :: Int32)
+
+foreign import ccall safe   "acc_op_create"             c_opCreate            :: Context -> Ptr OpDesc -> Ptr Op -> IO Status
+foreign import ccall safe   "acc_op_destroy"            c_opDestroy           :: Op -> IO Status
+foreign import ccall safe   "acc_op_compile_only"       c_opCompileOnly       :: CString -> Ptr OpDesc -> Ptr Int32 -> Ptr CSize -> IO Status
+foreign import ccall safe   "acc_exec_product_rows"     c_execProductRows     :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_product_outer"    c_execProductOuter    :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_route"            c_execRoute           :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_route_gradient"   c_execRouteGradient   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_combine"          c_execCombine         :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_combine_gradient" c_execCombineGradient :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_micro_quantise"   c_execMicroQuantise   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_micro_values"     c_execMicroValues     :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_micro_rows"       c_execMicroRows       :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status

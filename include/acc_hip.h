@@ -5,7 +5,7 @@
  * through the `cuda` package (Foreign.CUDA.Driver / Foreign.CUDA.Analysis) and
  * the external `nvcc`.
  *
- * Two layers:
+ * Layers:
  *
  *   A. driver layer   -- devices, memory, transfers, streams, events, modules,
  *                        run-time compilation with a content-hashed code-object
@@ -16,7 +16,9 @@
  *                        temporaries, launch shapes and multi-kernel protocols
  *                        it needs (acc_exec_*).  These are the roles of
  *                        the CUDA/CodeGen modules (templates) and of the skeleton
- *                        drivers in CUDA/Execute.hs:264-450.
+ *                        drivers in CUDA/Execute.hs:264-450;
+ *   C. memory table   -- host arrays and their copies on the device;
+ *   D. operators      -- products of ragged segments, routing, 4-bit numbers.
  *
  * Conventions
  *   - plain C: pointers, sizes, fixed-width integers; no C++ or torch types;
@@ -635,6 +637,101 @@ typedef struct acc_memtable_stats {
   uint64_t evictions, writebacks, writeback_bytes;
 } acc_memtable_stats;
 int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
+
+/* =========================================================================
+ * D. operators on segments of rows
+ * ========================================================================= */
+
+/* What a layer of experts needs beside the skeletons: products of ragged segments of rows with a matrix each, on the
+ * matrix cores; the router that makes the segments; the weighted sum that brings the rows back; and the same products on
+ * 4-bit numbers.  Segments are offsets, as for acc_exec_foldseg.  The reference has no counterpart (its backend has no
+ * matrix instructions and no 16-bit types).
+ *
+ * All work is enqueued on `stream`; the calls return without waiting.  On a stream under a guard (acc_stream_set_guard)
+ * the kernels do nothing once the guard is down.  Sums, softmax statistics and weights are Float32 whatever the element
+ * type, and results are rounded once.  No result may share memory with another array of the call.
+ *
+ * Element types are "float", "half" and "bfloat16" (an acc_strided does not say which it holds; the operator does).
+ * Extents are below 2^31; strides are in elements, and addresses are computed in 64 bits.  Offsets, indices, places and
+ * orders are Int32 and are looked at on the device: values out of range name no row.                             */
+#define ACC_STRIDED_RANK 4
+typedef struct acc_strided {
+  int32_t    rank;
+  int32_t    reserved;
+  int64_t    shape[ACC_STRIDED_RANK];    /* outermost first                       */
+  int64_t    stride[ACC_STRIDED_RANK];   /* elements from one to the next, >= 0   */
+  acc_devptr ptr;
+} acc_strided;
+
+enum {
+  ACC_OP_PRODUCT = 0,
+  ACC_OP_ROUTE   = 1,
+  ACC_OP_COMBINE = 2,
+  ACC_OP_MICRO   = 3,
+  ACC_OP_KIND_COUNT = 4
+};
+
+typedef struct acc_op_desc {
+  int32_t     kind;          /* ACC_OP_*                                          */
+  const char *elt_type;      /* "float", "half" or "bfloat16"                     */
+  int32_t     choose;        /* ACC_OP_ROUTE: experts a token, 1 to 64            */
+  int32_t     normalise;     /* ACC_OP_ROUTE: softmax over the chosen (else over all experts) */
+} acc_op_desc;
+
+/* An instance; its kernels are compiled through the cache when a call first needs them (as the variants of a skeleton
+ * are).  It may be used from several threads.                                                                  */
+typedef struct acc_op_s *acc_op;
+int acc_op_create(acc_context ctx, const acc_op_desc *desc, acc_op *out);
+int acc_op_destroy(acc_op op);
+/* compile every translation unit that calls may need (no GPU needed): the build check */
+int acc_op_compile_only(const char *target, const acc_op_desc *desc, int32_t *units, size_t *code_size);
+
+/* out[m, n] = sum_k x[r(m), k] w[e, n, k] for every row m of expert e's segment, offsets[e] <= m < offsets[e+1].
+ *   x [rows, k], innermost dimension contiguous; w [experts, n, k], either of the last two dimensions contiguous (the
+ *   gradient with respect to x is the same call with w's last two dimensions exchanged); offsets [experts + 1];
+ *   out [rows, n].  index NULL: r(m) = m; else index [rows] and r(m) = index[m], divided by `per` if that is not 0 (the
+ *   token of slot index[m] where every token has `per` slots), and x has any number of rows.  A row of no segment, or
+ *   whose index names no row, is zeros.                                                                        */
+int acc_exec_product_rows(acc_op op, const acc_strided *x, const acc_strided *w, const acc_strided *offsets,
+                          const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream);
+
+/* out[e, i, j] = sum over the rows m of e's segment of a[m, i] b[r(m), j]: the gradient with respect to w.
+ *   a [rows, i], b [rows, j] (with index: any number of rows), out [experts, i, j], either of its last two dimensions
+ *   contiguous.  An empty segment gives zeros.                                                                 */
+int acc_exec_product_outer(acc_op op, const acc_strided *a, const acc_strided *b, const acc_strided *offsets,
+                           const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream);
+
+/* The `choose` largest of every row of logits [tokens, experts], largest first, of equal ones the lowest index first;
+ * minus infinity and what is not a number are never chosen, and a slot that has no choice left has expert -1, weight 0
+ * and place -1.  weights: softmax over the chosen, or over the row.  The slots t * choose + j are then sorted by
+ * expert, stably: offsets [experts + 1], order [tokens * choose] the slots by place (-1 behind the last one), place
+ * [tokens, choose] its inverse.  At most 2048 experts.  experts, order, place, offsets: Int32; weights: Float32; all dense.  */
+int acc_exec_route(acc_op op, const acc_strided *logits, const acc_strided *experts, const acc_strided *weights,
+                   const acc_strided *offsets, const acc_strided *order, const acc_strided *place, acc_stream stream);
+/* dlogits from the gradient of the weights, both as acc_exec_route made them */
+int acc_exec_route_gradient(acc_op op, const acc_strided *logits, const acc_strided *experts, const acc_strided *weights,
+                            const acc_strided *dweights, const acc_strided *dlogits, acc_stream stream);
+
+/* out[t] = sum_j weights[t, j] y[place[t, j]], slots in order; a place that names no row of y adds nothing.  weights
+ * NULL: all 1 (the gradient of rows that were taken by `index`).  place, weights [tokens, choose], dense.             */
+int acc_exec_combine(acc_op op, const acc_strided *y, const acc_strided *place, const acc_strided *weights,
+                     const acc_strided *out, acc_stream stream);
+/* dy[place[t, j]] = weights[t, j] dout[t] and dweights[t, j] = <dout[t], y[place[t, j]]> (0 where there is no row).  Rows
+ * of dy that no slot has are not written; two slots must not have the same row.  y and dweights may both be NULL.  */
+int acc_exec_combine_gradient(acc_op op, const acc_strided *dout, const acc_strided *y, const acc_strided *place,
+                              const acc_strided *weights, const acc_strided *dy, const acc_strided *dweights, acc_stream stream);
+
+/* 4-bit numbers (sign, 2 bits of exponent, 1 of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), every 32 neighbours of a row under
+ * one power of two, a byte of exponent (127 for 1; 255: the block is not a number).  codes [rows, 16 ceil(k / 32)] bytes,
+ * two elements a byte, the even place in the low half, rows on 16 bytes; scales [rows, ceil(k / 32)] bytes; what a row's
+ * last block has too many counts as zeros.  The scale is the largest magnitude's power of two less 2; elements are
+ * rounded to the nearest, ties to even, and to 6 beyond it.                                                     */
+int acc_exec_micro_quantise(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, acc_stream stream);
+int acc_exec_micro_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *out, acc_stream stream);
+/* acc_exec_product_rows with both operands in that form, w's codes [experts, n, ...]; out in the operator's type */
+int acc_exec_micro_rows(acc_op op, const acc_strided *xcodes, const acc_strided *xscales, const acc_strided *wcodes,
+                        const acc_strided *wscales, const acc_strided *offsets, const acc_strided *index, int32_t per,
+                        const acc_strided *out, acc_stream stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -1,0 +1,39 @@
+"""The operators' translation units compile for gfx950 without a GPU, and what cannot be served is refused there."""
+import os
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def A():
+    import acchip
+    return acchip
+
+
+@pytest.mark.parametrize("elt", ("float", "half", "bfloat16"))
+def test_every_unit_of_every_operator_compiles_for_gfx950(A, tmp_path, elt):
+    A.lib().acc_cache_set_dir(str(tmp_path).encode())
+    for kind, least in ((A.OP_PRODUCT, 16), (A.OP_ROUTE, 8), (A.OP_COMBINE, 2), (A.OP_MICRO, 3)):
+        units, size = A.op_compile_only(kind, elt, 2)
+        assert units >= least and size > 4000 * units
+
+
+def test_operators_that_there_are_not(A):
+    for kind, elt, choose in ((4, "float", 1), (-1, "float", 1), (A.OP_PRODUCT, "double", 1), (A.OP_PRODUCT, "", 1), (A.OP_PRODUCT, None, 1),
+                              (A.OP_ROUTE, "float", 0), (A.OP_ROUTE, "float", 65)):
+        with pytest.raises(A.AccError) as e:
+            A.op_compile_only(kind, elt, choose)
+        assert e.value.code == A.ERR_INVALID
+
+
+def test_layouts_of_arrays_as_the_library_reads_them(A):
+    """an acc_strided: rank, four extents, four strides, the address"""
+    import struct
+    text = A._layout(A.Strided((2, 3, 5), (99, 1, 7), 0x1234))
+    assert struct.unpack("@ii4q4qQ", text) == (3, 0, 2, 3, 5, 0, 99, 1, 7, 0, 0x1234)
+    assert struct.unpack("@ii4q4qQ", A._layout(A.Strided((2, 3, 5), (99, 1, 7), 16).swap()))[2:10] == (2, 5, 3, 0, 99, 7, 1, 0)
+    dense = A.DeviceArray.view(None, (4, 6), __import__("numpy").dtype("f4"), 24, 64)
+    assert struct.unpack("@ii4q4qQ", A._layout(dense)) == (2, 0, 4, 6, 0, 0, 6, 1, 0, 0, 64)
+    assert A._layout(None) is None
