@@ -37,7 +37,6 @@ ACC_EMBED(op_product, "operators/op_product.h")
 ACC_EMBED(op_route, "operators/op_route.h")
 ACC_EMBED(op_combine, "operators/op_combine.h")
 ACC_EMBED(op_micro, "operators/op_micro.h")
-ACC_EMBED(op_micro_product, "operators/op_micro_product.h")
 
 namespace acc {
 
@@ -64,7 +63,6 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"op_route.h", acc_embed_op_route_begin, acc_embed_op_route_end},
       {"op_combine.h", acc_embed_op_combine_begin, acc_embed_op_combine_end},
       {"op_micro.h", acc_embed_op_micro_begin, acc_embed_op_micro_end},
-      {"op_micro_product.h", acc_embed_op_micro_product_begin, acc_embed_op_micro_product_end},
   };
   return headers;
 }

@@ -48,7 +48,8 @@ constexpr int kProductTileCount = 4;
 struct ProductVariant {
   int tile = 0;
   bool outer = false, b_fast = true, aligned = true;
-  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u); }
+  int index = 0;                // outer: whose rows an index names: 1 b's, 2 a's
+  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u) | (uint32_t)index << 7; }
 };
 
 std::string product_source(const OpSpec &sp, const ProductVariant &v)
@@ -56,9 +57,9 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
   const ProductTile &t = kProductTiles[v.tile];
   char text[512];
   std::snprintf(text, sizeof(text),
-                "#define OP_TYPE %d\n#define OP_BM %d\n#define OP_BN %d\n#define OP_WM %d\n#define OP_WN %d\n#define OP_OUTER %d\n"
-                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
-                sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0);
+                "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_BN %d\n#define OP_WM %d\n#define OP_WN %d\n#define OP_OUTER %d\n"
+                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#define OP_INDEX %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
+                sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0, v.index);
   return text;
 }
 
@@ -84,7 +85,7 @@ std::string route_source(const OpSpec &sp, const RouteVariant &v)
 {
   char text[512];
   std::snprintf(text, sizeof(text),
-                "#define OP_TYPE %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_BLOCK %d\n#define OP_THREADS %d\n"
+                "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_BLOCK %d\n#define OP_THREADS %d\n"
                 "#include \"acc_hip_device.h\"\n#include \"op_route.h\"\n",
                 sp.type, v.lanes, v.per, v.vec, v.block, kRouteThreads);
   return text;
@@ -94,7 +95,7 @@ constexpr int kCombineSlots = 4;
 std::string combine_source(const OpSpec &sp, bool aligned)
 {
   char text[256];
-  std::snprintf(text, sizeof(text), "#define OP_TYPE %d\n#define OP_ALIGNED %d\n#define OP_SLOTS %d\n#include \"acc_hip_device.h\"\n#include \"op_combine.h\"\n",
+  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_ALIGNED %d\n#define OP_SLOTS %d\n#include \"acc_hip_device.h\"\n#include \"op_combine.h\"\n",
                 sp.type, aligned ? 1 : 0, kCombineSlots);
   return text;
 }
@@ -102,14 +103,7 @@ std::string combine_source(const OpSpec &sp, bool aligned)
 std::string micro_source(const OpSpec &sp, bool aligned)
 {
   char text[256];
-  std::snprintf(text, sizeof(text), "#define OP_TYPE %d\n#define OP_ALIGNED %d\n#include \"acc_hip_device.h\"\n#include \"op_micro.h\"\n", sp.type, aligned ? 1 : 0);
-  return text;
-}
-
-std::string micro_product_source(const OpSpec &sp)
-{
-  char text[256];
-  std::snprintf(text, sizeof(text), "#define OP_TYPE %d\n#include \"acc_hip_device.h\"\n#include \"op_micro_product.h\"\n", sp.type);
+  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_ALIGNED %d\n#include \"acc_hip_device.h\"\n#include \"op_micro.h\"\n", sp.type, aligned ? 1 : 0);
   return text;
 }
 
@@ -126,13 +120,14 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   std::vector<std::string> out;
   if (sp.kind == ACC_OP_PRODUCT) {
     for (int t = 0; t < kProductTileCount; ++t)
-      for (int form = 0; form < 6; ++form) {
+      for (int form = 0; form < 10; ++form) {
         ProductVariant v;
         v.tile = t;
         v.outer = form >= 4;
         v.b_fast = !v.outer && (form & 1) == 0;
-        v.aligned = form >= 4 ? form == 4 : form < 2;
-        if (v.outer && t < 2) continue;
+        v.aligned = v.outer ? (form & 1) == 0 : form < 2;
+        v.index = v.outer ? (form - 4) / 2 : 0;
+        if ((v.outer && t < 2) || (!v.aligned && t > 2)) continue;
         out.push_back(product_source(sp, v));
       }
   } else if (sp.kind == ACC_OP_ROUTE) {
@@ -142,7 +137,14 @@ std::vector<std::string> all_sources(const OpSpec &sp)
     for (bool aligned : {true, false}) out.push_back(combine_source(sp, aligned));
   } else {
     for (bool aligned : {true, false}) out.push_back(micro_source(sp, aligned));
-    out.push_back(micro_product_source(sp));
+    for (int t = 0; t < kProductTileCount; ++t)
+      for (bool aligned : {true, false}) {
+        ProductVariant v;
+        v.tile = t;
+        v.aligned = aligned;
+        if (!v.aligned && t > 2) continue;
+        out.push_back(product_source(sp, v));
+      }
   }
   std::sort(out.begin(), out.end());
   out.erase(std::unique(out.begin(), out.end()), out.end());
@@ -266,6 +268,43 @@ int64_t tiles_at_most(int64_t rows, int64_t experts, int64_t height)
   return (rows + parts * (height - 1)) / height;
 }
 
+// An index at is divided by `per` as (at * mul) >> (32 + shift), exact for 0 <= at < 2^31 (with l = ceil(log2 per), mul is
+// 2^(31 + l) / per rounded up: its excess times at stays below 2^(31 + l)).
+void set_divisor(int32_t per, acc_product_args *a)
+{
+  if (per < 2) return;
+  int l = 1;
+  while ((int64_t(1) << l) < per) ++l;
+  a->per_mul = static_cast<uint32_t>(((uint64_t(1) << (31 + l)) + (uint64_t)per - 1) / (uint64_t)per);
+  a->per_shift = static_cast<uint32_t>(l - 1);
+}
+
+// whether four neighbours of a result's rows, from every fourth on, can be written at once
+bool out_in_vectors(const acc_strided &o, int bytes)
+{
+  if (o.shape[o.rank - 1] % 4 != 0 || o.ptr % (uint64_t)(4 * bytes) != 0) return false;
+  for (int d = 0; d + 1 < o.rank; ++d)
+    if (o.shape[d] > 1 && o.stride[d] % 4 != 0) return false;
+  return true;
+}
+
+// Whether offsets of 32 bits (and buffers below 2 GB) do for an operand of the aligned form: rows of `row` bytes of which
+// `tile` (all `rows` of them, with an index) are reached from one base; rows must not overlap, as a buffer that ends with the
+// last row that counts would cut others short.
+constexpr int kTallest = 256;
+bool near_enough(const acc_strided &a, int rows_dim, int64_t row, int bytes, bool index)
+{
+  const int64_t stride = a.stride[rows_dim] * bytes, reached = index ? a.shape[rows_dim] : std::min<int64_t>(a.shape[rows_dim], kTallest);
+  return (a.shape[rows_dim] <= 1 || stride >= row) && stride <= 0x7fffffff && reached * stride + row < 0x7fff0000;
+}
+
+// the tile shape for products of `rows` rows of `experts` segments
+int rows_tile(int64_t rows, int64_t experts, int64_t n, bool aligned)
+{
+  const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
+  return mean <= 24 ? 0 : mean <= 96 ? 1 : !aligned || mean < 512 || n < 256 ? 2 : 3;
+}
+
 }  // namespace
 
 struct acc_op_s {
@@ -287,6 +326,7 @@ std::string product_source_of(const OpSpec &sp, uint32_t key)
   v.outer = key & 16u;
   v.b_fast = key & 32u;
   v.aligned = key & 64u;
+  v.index = (int)(key >> 7 & 3u);
   return product_source(sp, v);
 }
 std::string route_source_of(const OpSpec &sp, uint32_t key)
@@ -299,13 +339,13 @@ std::string route_source_of(const OpSpec &sp, uint32_t key)
   return route_source(sp, v);
 }
 std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_source(sp, key & 1u); }
-std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & 2u) ? micro_product_source(sp) : micro_source(sp, key & 1u); }
+constexpr uint32_t kMicroElements = 1024;            // (above the products' keys)
+std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & kMicroElements) ? micro_source(sp, key & 1u) : product_source_of(sp, key); }
 
 const char *const kProductNames[] = {"product"};
 const char *const kRouteNames[] = {"route", "route_place", "route_gradient"};
 const char *const kCombineNames[] = {"combine", "combine_gradient"};
 const char *const kMicroNames[] = {"micro_quantise", "micro_values"};
-const char *const kMicroProductNames[] = {"micro_product"};
 
 // one call's stream and its guard (a loop enqueued ahead, see acc_guard_create)
 int begin(acc_op op, int kind, const char *who, acc_stream stream, const uint32_t **guard)
@@ -440,9 +480,9 @@ try {
   ProductVariant v;
   // (where both are contiguous -- one column, or a sum of one -- either way of reading will do)
   v.b_fast = unit(*w, 2);
-  v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0);
-  const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
-  v.tile = mean <= 24 ? 0 : mean <= 96 ? 1 : mean < 512 || n < 256 ? 2 : 3;
+  v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
+              near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
+  v.tile = rows_tile(rows, experts, n, v.aligned);
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
@@ -456,11 +496,12 @@ try {
   a.b_expert = w->stride[0];
   a.out_stride = out->stride[0];
   a.rows = rows;
-  a.a_rows = x->shape[0];
+  a.a_rows = (int32_t)x->shape[0];
   a.nj = (int32_t)n;
   a.k = (int32_t)k;
   a.experts = (int32_t)experts;
-  a.per = per;
+  set_divisor(per, &a);
+  a.out_vectors = out_in_vectors(*out, bytes);
   a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
   a.tiles_j = (int32_t)ceil_div(n, t.bn);
   return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
@@ -499,8 +540,10 @@ try {
   ProductVariant v;
   v.outer = true;
   v.b_fast = false;
-  v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1);
-  v.tile = o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2;
+  v.index = !index ? 0 : turned ? 2 : 1;
+  v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1) &&
+              near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
+  v.tile = v.aligned && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2;
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
@@ -514,12 +557,13 @@ try {
   a.out_expert = o.stride[0];
   a.out_stride = o.stride[1];
   a.rows = rows;
-  a.a_rows = p->shape[0];
-  a.b_rows = q->shape[0];
+  a.a_rows = (int32_t)p->shape[0];
+  a.b_rows = (int32_t)q->shape[0];
   a.ni = (int32_t)o.shape[1];
   a.nj = (int32_t)o.shape[2];
   a.experts = (int32_t)experts;
-  a.per = per;
+  set_divisor(per, &a);
+  a.out_vectors = out_in_vectors(o, bytes);
   a.tiles_i = (int32_t)ceil_div(o.shape[1], t.bm);
   a.tiles_j = (int32_t)ceil_div(o.shape[2], t.bn);
   return launch(op, who, var->fn, experts * a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
@@ -731,7 +775,7 @@ static int micro_elements(acc_op op, const char *who, bool back, const acc_strid
   if (is_empty(*x)) return ACC_OK;
   const bool aligned = k % epc == 0 && aligned_rows(*x, bytes, 1);
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(aligned ? 1u : 0u, kMicroNames, 2, micro_source_of, &var));
+  ACC_TRY(op->variant(kMicroElements | (aligned ? 1u : 0u), kMicroNames, 2, micro_source_of, &var));
   a.x = device<const void>(x);
   a.out = device<void>(x);
   a.codes = device<uint8_t>(codes);
@@ -773,7 +817,7 @@ int acc_exec_micro_rows(acc_op op, const acc_strided *xcodes, const acc_strided 
                         const acc_strided *offsets, const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream)
 try {
   const char *who = "acc_exec_micro_rows";
-  acc_micro_product_args a = {};
+  acc_product_args a = {};
   ACC_TRY(begin(op, ACC_OP_MICRO, who, stream, &a.guard));
   ACC_TRY(check_micro(who, "x", xcodes, xscales, 2, false));
   ACC_TRY(check_micro(who, "w", wcodes, wscales, 3, false));
@@ -789,31 +833,42 @@ try {
   const int bytes = type_bytes(op->spec.type);
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{xcodes, 1, "x"}, {xscales, 1, "x's scales"}, {wcodes, 1, "w"}, {wscales, 1, "w's scales"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (is_empty(*out)) return ACC_OK;
+  ProductVariant v;
+  // (codes lie on 16 bytes; scales are taken four at a time where every row of them starts on 4 bytes and is whole fours)
+  v.aligned = blocks % 4 == 0 && near_enough(*xcodes, 0, 16 * blocks, 1, index != nullptr) && near_enough(*wcodes, 1, 16 * blocks, 1, false) &&
+              near_enough(*xscales, 0, blocks, 1, true) && near_enough(*wscales, 1, blocks, 1, true);
+  for (const acc_strided *t : {xscales, wscales}) {
+    v.aligned = v.aligned && t->ptr % 4 == 0;
+    for (int d = 0; d + 1 < t->rank; ++d) v.aligned = v.aligned && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
+  }
+  v.tile = rows_tile(rows, experts, n, v.aligned);
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(2u, kMicroProductNames, 1, micro_source_of, &var));
-  a.a = device<const uint8_t>(xcodes);
-  a.sa = device<const uint8_t>(xscales);
-  a.b = device<const uint8_t>(wcodes);
-  a.sb = device<const uint8_t>(wscales);
+  ACC_TRY(op->variant(v.key(), kProductNames, 1, micro_source_of, &var));
+  const ProductTile &t = kProductTiles[v.tile];
+  a.a = device<const void>(xcodes);
+  a.b = device<const void>(wcodes);
+  a.a_scales = device<const uint8_t>(xscales);
+  a.b_scales = device<const uint8_t>(wscales);
   a.out = device<void>(out);
   a.offsets = device<const int32_t>(offsets);
-  a.index = device<const int32_t>(index);
+  a.index_a = device<const int32_t>(index);
   a.a_stride = xcodes->stride[0];
-  a.sa_stride = xscales->stride[0];
+  a.a_scales_stride = xscales->stride[0];
   a.b_stride = wcodes->stride[1];
-  a.sb_stride = wscales->stride[1];
   a.b_expert = wcodes->stride[0];
-  a.sb_expert = wscales->stride[0];
+  a.b_scales_stride = wscales->stride[1];
+  a.b_scales_expert = wscales->stride[0];
   a.out_stride = out->stride[0];
   a.rows = rows;
-  a.a_rows = xscales->shape[0];
-  a.n = (int32_t)n;
-  a.blocks = (int32_t)blocks;
+  a.a_rows = (int32_t)xscales->shape[0];
+  a.nj = (int32_t)n;
+  a.k = (int32_t)(16 * blocks);
   a.experts = (int32_t)experts;
-  a.per = per;
-  a.tiles_i = (int32_t)tiles_at_most(rows, experts, 16);
-  a.tiles_j = (int32_t)ceil_div(n, 256);
-  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 256, 0, stream, a);
+  set_divisor(per, &a);
+  a.out_vectors = out_in_vectors(*out, bytes);
+  a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
+  a.tiles_j = (int32_t)ceil_div(n, t.bn);
+  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
 } ACC_OP_CATCH("acc_exec_micro_rows")
 
 }  // extern "C"

@@ -15,18 +15,21 @@ struct acc_product_args {
   const void *a, *b;            /* the operands */
   void *out;
   const int32_t *offsets;       /* experts + 1 segment starts */
-  const int32_t *index_a;       /* rows: which row of `a` (outer: and of `b`) each row of the segments is; 0: its own number */
+  const int32_t *index_a;       /* which row of `a` (outer: or of `b`) each row of the segments is; 0: its own number */
   const int32_t *index_b;
-  int64_t a_stride, b_stride;   /* from one row (of the array in memory) to the next */
+  const uint8_t *a_scales, *b_scales;   /* 4 bits: a byte for every 32 elements */
+  int64_t a_stride, b_stride;   /* from one row of the array in memory to the next (4 bits: in bytes, as every length along r) */
   int64_t b_expert;             /* rows: from one expert's matrix to the next */
+  int64_t a_scales_stride, b_scales_stride, b_scales_expert;
   int64_t out_stride, out_expert;
   int64_t rows;                 /* rows of the segments, all told */
-  int64_t a_rows, b_rows;       /* rows that an index may name */
+  int32_t a_rows, b_rows;       /* rows that an index may name */
   int32_t ni, nj;               /* the result's extents: rows: -, n; outer: i, j */
   int32_t k;                    /* rows: the summed dimension */
   int32_t experts;
-  int32_t per;                  /* an index is divided by this */
+  uint32_t per_mul, per_shift;  /* an index at is divided: (at * per_mul) >> (32 + per_shift); per_mul 0: it is not */
   int32_t tiles_i, tiles_j;     /* the grid's tiles */
+  int32_t out_vectors;          /* four neighbours of the result can be written at once */
   int32_t pad;
   const uint32_t *guard;
 };
@@ -65,18 +68,6 @@ struct acc_micro_args {
   uint8_t *codes, *scales;
   int64_t rows, x_stride, codes_stride, scales_stride;
   int32_t k, blocks;
-  const uint32_t *guard;
-};
-
-struct acc_micro_product_args {
-  const uint8_t *a, *sa, *b, *sb;   /* codes and scales of both operands */
-  void *out;
-  const int32_t *offsets, *index;
-  int64_t a_stride, sa_stride, b_stride, sb_stride, b_expert, sb_expert, out_stride;
-  int64_t rows, a_rows;
-  int32_t n, blocks;            /* columns of the result; blocks of 32 along the summed dimension */
-  int32_t experts, per;
-  int32_t tiles_i, tiles_j;
   const uint32_t *guard;
 };
 

@@ -12,32 +12,32 @@
 template <bool ALIGNED> ACC_DEV void op_load8(const op_elt *p, const int valid, float (&f)[8])
 {
 #pragma unroll
-  for (int h = 0; h < 8 / OP_EPC; ++h) {
-    const acc_u4 v = op_chunk<ALIGNED>(p + h * OP_EPC, valid - h * OP_EPC);
-    op_elt e[OP_EPC];
+  for (int h = 0; h < 8 / OP_VALUES; ++h) {
+    const acc_u4 v = op_chunk<ALIGNED>(p + h * OP_VALUES, valid - h * OP_VALUES);
+    op_elt e[OP_VALUES];
     __builtin_memcpy(e, &v, 16);
 #pragma unroll
-    for (int k = 0; k < OP_EPC; ++k) f[h * OP_EPC + k] = (float)e[k];
+    for (int k = 0; k < OP_VALUES; ++k) f[h * OP_VALUES + k] = (float)e[k];
   }
 }
 template <bool ALIGNED> ACC_DEV void op_store8(op_elt *p, const int valid, const float (&f)[8])
 {
 #pragma unroll
-  for (int h = 0; h < 8 / OP_EPC; ++h) {
-    op_elt e[OP_EPC];
+  for (int h = 0; h < 8 / OP_VALUES; ++h) {
+    op_elt e[OP_VALUES];
     acc_u4 v;
 #pragma unroll
-    for (int k = 0; k < OP_EPC; ++k) e[k] = (op_elt)f[h * OP_EPC + k];
+    for (int k = 0; k < OP_VALUES; ++k) e[k] = (op_elt)f[h * OP_VALUES + k];
     __builtin_memcpy(&v, e, 16);
-    const int left = valid - h * OP_EPC;
+    const int left = valid - h * OP_VALUES;
     if (ALIGNED) {
-      if (left > 0) *(acc_u4 *)(p + h * OP_EPC) = v;
-    } else if (left >= OP_EPC) {
-      ((op_loose *)(p + h * OP_EPC))->v = v;
+      if (left > 0) *(acc_u4 *)(p + h * OP_VALUES) = v;
+    } else if (left >= OP_VALUES) {
+      ((op_loose<op_elt> *)(p + h * OP_VALUES))->v = v;
     } else {
 #pragma unroll
-      for (int k = 0; k < OP_EPC; ++k)
-        if (k < left) p[h * OP_EPC + k] = e[k];
+      for (int k = 0; k < OP_VALUES; ++k)
+        if (k < left) p[h * OP_VALUES + k] = e[k];
     }
   }
 }

@@ -10,28 +10,27 @@ typedef unsigned int acc_u4 __attribute__((ext_vector_type(4)));
 typedef unsigned int acc_u2 __attribute__((ext_vector_type(2)));
 typedef float acc_f4 __attribute__((ext_vector_type(4)));
 
-/* OP_TYPE: 0 float, 1 half, 2 bfloat16 */
-#if OP_TYPE == 0
+/* OP_ELT: 0 float, 1 half, 2 bfloat16 */
+#if OP_ELT == 0
 typedef float op_elt;
-#elif OP_TYPE == 1
+#elif OP_ELT == 1
 typedef _Float16 op_elt;
 #else
 typedef __bf16 op_elt;
 #endif
-#define OP_SIZE ((int)sizeof(op_elt))
-#define OP_EPC (16 / OP_SIZE)            /* elements of a chunk of 16 bytes */
+#define OP_VALUES (16 / (int)sizeof(op_elt))       /* elements of a chunk of 16 bytes */
 
-/* 16 bytes of memory that need not be aligned */
-struct __attribute__((packed, aligned(OP_SIZE))) op_loose { acc_u4 v; };
+/* 16 bytes of memory that start wherever an element may */
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) op_loose { acc_u4 v; };
 
 /* `valid` elements from p on, zeros behind them; p may be anywhere if valid <= 0 */
 template <bool ALIGNED> ACC_DEV acc_u4 op_chunk(const op_elt *p, const int valid)
 {
   if (ALIGNED) return valid > 0 ? *(const acc_u4 *)p : acc_u4{0, 0, 0, 0};
-  if (valid >= OP_EPC) return ((const op_loose *)p)->v;
-  op_elt e[OP_EPC];
+  if (valid >= OP_VALUES) return ((const op_loose<op_elt> *)p)->v;
+  op_elt e[OP_VALUES];
 #pragma unroll
-  for (int k = 0; k < OP_EPC; ++k) e[k] = k < valid ? p[k] : (op_elt)0.0f;
+  for (int k = 0; k < OP_VALUES; ++k) e[k] = k < valid ? p[k] : (op_elt)0.0f;
   acc_u4 v;
   __builtin_memcpy(&v, e, 16);
   return v;
@@ -45,6 +44,26 @@ ACC_DEV void op_segment(const int *offsets, const int experts, const int rows, c
   const int b = s <= 0 ? 0 : offsets[s - 1], e = s > experts ? rows : offsets[s];
   *begin = acc_min(acc_max(b, 0), rows);
   *end = acc_max(*begin, acc_min(e, rows));
+}
+
+/* Workgroups go to the eight dies in turn: block b of n as a number such that every die has a run of neighbours. */
+ACC_DEV long long op_die_run(const long long b, const long long n)
+{
+  const long long q = n / ACC_XCDS, r = n % ACC_XCDS, die = b % ACC_XCDS;
+  return die * q + acc_min<long long>(die, r) + b / ACC_XCDS;
+}
+
+/* how many runs of up to `height` rows the segments have */
+ACC_DEV int op_count_tiles(const int *offsets, const int experts, const int rows, const int height)
+{
+  const int lane = acc_lane();
+  int all = 0;
+  for (int base = 0; base < experts + 2; base += 64) {
+    int b = 0, e = 0;
+    if (base + lane < experts + 2) op_segment(offsets, experts, rows, base + lane, &b, &e);
+    all += acc_wave_reduce((e - b + height - 1) / height, [](int x, int y) { return x + y; });
+  }
+  return all;
 }
 
 struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segment; begin >= end: no such tile */

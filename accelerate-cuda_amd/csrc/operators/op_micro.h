@@ -25,12 +25,12 @@ extern "C" __global__ void __launch_bounds__(256) micro_quantise(const acc_micro
   const bool here = row < p.rows;
   float f[8];
 #pragma unroll
-  for (int h = 0; h < 8 / OP_EPC; ++h) {
-    const acc_u4 v = op_chunk<OP_ALIGNED>((const op_elt *)p.x + row * p.x_stride + c + h * OP_EPC, here ? p.k - c - h * OP_EPC : 0);
-    op_elt e[OP_EPC];
+  for (int h = 0; h < 8 / OP_VALUES; ++h) {
+    const acc_u4 v = op_chunk<OP_ALIGNED>((const op_elt *)p.x + row * p.x_stride + c + h * OP_VALUES, here ? p.k - c - h * OP_VALUES : 0);
+    op_elt e[OP_VALUES];
     __builtin_memcpy(e, &v, 16);
 #pragma unroll
-    for (int k = 0; k < OP_EPC; ++k) f[h * OP_EPC + k] = (float)e[k];
+    for (int k = 0; k < OP_VALUES; ++k) f[h * OP_VALUES + k] = (float)e[k];
   }
   /* the largest magnitude by its bits: what is no number, or infinite, is larger than any other */
   unsigned int most = 0;
@@ -72,18 +72,18 @@ extern "C" __global__ void __launch_bounds__(256) micro_values(const acc_micro_a
     e[k] = (op_elt)v;
   }
 #pragma unroll
-  for (int h = 0; h < 8 / OP_EPC; ++h) {
-    const int left = p.k - c - h * OP_EPC;
+  for (int h = 0; h < 8 / OP_VALUES; ++h) {
+    const int left = p.k - c - h * OP_VALUES;
     acc_u4 v;
-    __builtin_memcpy(&v, e + h * OP_EPC, 16);
+    __builtin_memcpy(&v, e + h * OP_VALUES, 16);
     if (OP_ALIGNED) {
-      if (left > 0) *(acc_u4 *)(out + h * OP_EPC) = v;
-    } else if (left >= OP_EPC) {
-      ((op_loose *)(out + h * OP_EPC))->v = v;
+      if (left > 0) *(acc_u4 *)(out + h * OP_VALUES) = v;
+    } else if (left >= OP_VALUES) {
+      ((op_loose<op_elt> *)(out + h * OP_VALUES))->v = v;
     } else {
 #pragma unroll
-      for (int k = 0; k < OP_EPC; ++k)
-        if (k < left) out[h * OP_EPC + k] = e[h * OP_EPC + k];
+      for (int k = 0; k < OP_VALUES; ++k)
+        if (k < left) out[h * OP_VALUES + k] = e[h * OP_VALUES + k];
     }
   }
 }

@@ -5,12 +5,21 @@
  *   outer  out[e, i, j] = sum_{m in e} a[r(m), i] b[r(m), j]
  *
  * Both are C[i, j] = sum_r A(i, r) B(j, r) over tiles of OP_BM x OP_BN results; what differs is whether an operand's rows in
- * memory run along r (OP_A_FAST, OP_B_FAST) or across it.  A step of the sum covers 128 bytes along r of an operand
- * (64 elements of 16 bits, 32 of Float32).
+ * memory run along r (OP_A_FAST, OP_B_FAST) or across it.  A step of the sum covers 128 bytes of an operand along r, a cache
+ * line: 64 elements of 16 bits, 32 of Float32, 256 of 4 bits (OP_TYPE 3: both operands as op_micro.h makes them, each with
+ * its scales).  Two steps lie in LDS.  The matrix cores work on half a step, whose fragments are in registers, while the next
+ * half's are read; one barrier a step, in its middle, says that everybody's share of the next step has arrived and that
+ * nobody reads this one any more, so that the next but one may take its place.
  */
 #include "op_common.h"
 
-#define OP_BR (128 / OP_SIZE)                      /* the step of the sum, in elements */
+#if OP_TYPE == 3
+typedef unsigned char op_mem;
+#else
+typedef op_elt op_mem;
+#endif
+#define OP_EPC (16 / (int)sizeof(op_mem))          /* elements of a chunk of 16 bytes */
+#define OP_STEP (8 * OP_EPC)                       /* the step of the sum, in elements */
 #define OP_THREADS (64 * OP_WM * OP_WN)
 #define OP_FM (OP_BM / OP_WM / 16)                 /* fragments of 16 x 16 that a wave has of the result */
 #define OP_FN (OP_BN / OP_WN / 16)
@@ -26,115 +35,382 @@ ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, acc_f4 c)
 #elif OP_TYPE == 1
 typedef _Float16 op_frag __attribute__((ext_vector_type(8)));
 ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
-#else
+#elif OP_TYPE == 2
 typedef __bf16 op_frag __attribute__((ext_vector_type(8)));
 ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+#else
+typedef int op_i8 __attribute__((ext_vector_type(8)));
+struct op_frag { acc_u4 v; int scale; };           /* a block of 32 and its scale */
+ACC_DEV acc_f4 op_mfma(const op_frag &x, const op_frag &y, const acc_f4 c)
+{
+  const op_i8 a = {(int)x.v.x, (int)x.v.y, (int)x.v.z, (int)x.v.w, 0, 0, 0, 0}, b = {(int)y.v.x, (int)y.v.y, (int)y.v.z, (int)y.v.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, x.scale, 0, y.scale);
+}
 #endif
 
-/* One operand's tile of a step in LDS, in chunks of 16 bytes.
- *   rows along r: TILE rows of 8 chunks; row i's chunk c lies at c ^ (i & 7), so that the 16 rows of a fragment are read
- *   from all banks.
- *   rows across r: OP_BR rows of TILE elements.
+/* OP_INDEX, outer: 0: no index, 1: of b's rows, 2: of a's */
+#define OP_PLAIN 0
+#define OP_LISTED 1
+#define OP_GATED 2
+
+typedef __attribute__((address_space(3))) void *op_lds_ptr;
+#define OP_NOWHERE 0x80000000u                     /* an offset beyond the end of every buffer: reads as zeros */
+#define OP_FARTHEST 0x7fffffffll                   /* the longest buffer */
+
+/* v, `bytes` further down: what is shifted in is zeros */
+ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
+{
+  const unsigned long long lo = v.x | (unsigned long long)v.y << 32, hi = v.z | (unsigned long long)v.w << 32;
+  const int n = 8 * bytes;
+  unsigned long long a, b;
+  if (bytes >= 8) {
+    a = bytes >= 16 ? 0 : hi >> (n - 64);
+    b = 0;
+  } else {
+    a = bytes ? lo >> n | hi << (64 - n) : lo;
+    b = hi >> n;
+  }
+  return acc_u4{(unsigned int)a, (unsigned int)(a >> 32), (unsigned int)b, (unsigned int)(b >> 32)};
+}
+
+/* One operand's share of a step in LDS, in chunks of 16 bytes.
+ *   rows along r: TILE rows of 8 chunks; row i's chunk c lies at c ^ (i % 8): the eight lanes that are served together read
+ *     neighbouring rows' chunks from all banks.
+ *   rows across r: OP_STEP rows of TILE elements; a row's units of 16 elements lie at u ^ f(r), so that the rows that are
+ *     read together (four neighbours, for 16 bits, and those eight further on; every fourth, for Float32) lie in other banks.
  * A lane's fragment holds, for its i (lane % 16), the r of its quarter of the wave (lane / 16): 8 of 32 in a row for 16 bits,
- * 4 of 16 for Float32 -- any order of r will do that both operands keep. */
-template <bool FAST, int TILE> struct op_operand {
+ * 4 of 16 for Float32, a block of 32 for 4 bits.
+ *
+ * OP_ALIGNED: rows are whole chunks and start on one.  A lane's chunks go from memory straight to LDS, by way of a buffer
+ * that starts at the tile (or the step) and ends where the rows that count do: what lies beyond reads as zeros, and
+ * addresses are one offset of 32 bits a chunk (the driver sees to it that they suffice).
+ * Otherwise rows start anywhere; chunks go by way of registers, with addresses of 64 bits.  A chunk that would reach
+ * beyond its row's end is read that much earlier and shifted into place, so that no read leaves its row. */
+template <bool FAST, int TILE, int LIST> struct op_operand {
   static constexpr int CHUNKS = TILE * 8;                         /* of a step */
   static constexpr int MINE = (CHUNKS + OP_THREADS - 1) / OP_THREADS;
   static constexpr int PITCH = FAST ? 8 : TILE / OP_EPC;          /* chunks of a row */
+  static constexpr int UNITS = TILE / 16;                         /* across r: of a row */
+  static constexpr int SIZE = (int)sizeof(op_mem);
+  /* 4 bits: the rows' scales of a step, behind them: the first half's, four a row, then the second's (a wave brings 64
+   * rows', however few there are) */
+  static constexpr int SCALE_ROWS = TILE < 64 ? 64 : TILE;
+  static constexpr int SCALES = OP_TYPE == 3 ? 2 * SCALE_ROWS / 4 : 0;
+  static_assert(CHUNKS % 64 == 0 && (CHUNKS % OP_THREADS == 0 || OP_THREADS % CHUNKS == 0), "whole waves, the same number each");
 
-  const op_elt *base;
-  long long stride;
-  const int *index;              /* which row of memory row m of the segments is; 0: its own number */
-  const int *gate;               /* outer, the operand without an index: the other one's; a row that has no partner counts as none */
-  int per;
-  long long limit;               /* rows an index may name */
-  int lo, hi;                    /* the rows of memory that count: along r the i's, across it the r's */
-  int minor, extent;             /* across r: the tile's first element of a row, and the row's length; along r: -, the sum's length */
-  const op_elt *row[FAST ? MINE : 1];
+  const unsigned char *base;     /* along r: of the operand; across it: of the tile's first column */
+  long long stride;              /* of a row, in bytes */
+  const int *index;              /* which row of memory row m of the segments is; 0: its own number.  LIST: OP_PLAIN: there is none;
+                                  * OP_LISTED: along r perhaps one, across r one; OP_GATED: the other operand's (a row without
+                                  * a partner counts as none) */
+  unsigned int per_mul, per_shift;
+  int limit;                     /* rows an index may name */
+  int lo, hi;                    /* the rows that count: along r the i's, across it the r's */
+  int extent;                    /* elements of a row that count, from `base` on */
+  int rows[MINE];                /* across r, with an index: which rows of memory the next step's are that is to be asked for; -1: none */
+  int column;                    /* along r: the lane's chunks' first element (the same of all of them) */
+  /* whether a lane's chunks lie equally far apart in memory: the rows between them are as many, and swizzled alike (for
+   * Float32 across r they are not) */
+  static constexpr bool EVEN = FAST ? LIST == OP_PLAIN : OP_TYPE != 0;
+  static constexpr int APART = CHUNKS < OP_THREADS ? 0 : OP_THREADS / PITCH;
+#if OP_ALIGNED
+  unsigned int offset[EVEN ? 1 : MINE];   /* of the lane's chunks, in bytes: along r from the tile's first row, across it from the step's */
+  __amdgpu_buffer_rsrc_t buffer; /* along r */
+#else
+  long long offset[MINE];        /* along r: of the lane's rows from `base`; across r: of its chunks from their rows' beginning */
+#endif
+#if OP_TYPE == 3
+  const unsigned char *scales;
+  long long scales_stride;
+  long long scale_row;           /* where the scales of the lane's row lie; -1: no such row */
+  unsigned int scale_offset;
+  int blocks;
+#endif
 
-  ACC_DEV const op_elt *address(const int m) const
+  /* a lane's q-th chunk of a step: where there are fewer chunks than lanes, several waves bring the same ones */
+  ACC_DEV static int slot(const int tid, const int q) { return CHUNKS < OP_THREADS ? tid % CHUNKS : tid + q * OP_THREADS; }
+  ACC_DEV static int swizzle(const int r)
   {
-    if (m < lo || m >= hi) return (const op_elt *)0;
-    const int *named = index ? index : gate;
-    if (named) {
-      const int at = named[m], r = per > 1 ? at / per : at;
-      if (at < 0 || r >= limit) return (const op_elt *)0;
-      if (index) return base + (long long)r * stride;
-    }
-    return base + (long long)m * stride;
+    return (OP_TYPE == 0 ? r >> 2 & 3 : (r & 3) | (r >> 1 & 4)) & (UNITS - 1);
+  }
+  /* of a slot: its row, and its first element there */
+  ACC_DEV static int major(const int s) { return s / PITCH; }
+  ACC_DEV static int element(const int s)
+  {
+    const int i = s / PITCH, c = s % PITCH;
+    if (FAST) return (c ^ (i & 7)) * OP_EPC;
+    constexpr int U = 16 / OP_EPC;                                /* chunks of a unit: 2 of 16 bits, 4 of Float32 */
+    return ((c / U ^ swizzle(i)) * U + c % U) * OP_EPC;
   }
 
-  ACC_DEV void start(const int tid, const int first)              /* first: along r the tile's first i */
+  ACC_DEV int divided(const int at) const { return per_mul ? (int)(__umulhi((unsigned int)at, per_mul) >> per_shift) : at; }
+
+  /* which row of memory row m of the segments is, if the index says `at`; -1: none */
+  ACC_DEV int number(const int m, const int at) const
   {
+    const bool listed = FAST ? LIST == OP_LISTED && index != 0 : LIST != OP_PLAIN;
+    const int r = listed ? divided(at) : m;
+    const bool there = (m >= lo) & (m < hi) & (!listed | ((at >= 0) & (r < limit)));
+    return there ? LIST == OP_GATED ? m : r : -1;
+  }
+  /* what the index says of row m (of the nearest row that counts, if that one does not) */
+  ACC_DEV int ask(const int m) const { return (FAST ? LIST == OP_LISTED && index != 0 : LIST != OP_PLAIN) ? index[acc_max(lo, acc_min(m, hi - 1))] : 0; }
+
+  /* along r: where the lane's rows are, from row `first` on; across r: where its columns are, and what the index says of the
+   * first step's rows */
+  ACC_DEV void start(const int tid, const int first)
+  {
+    column = FAST ? element(slot(tid, 0)) : 0;
+#if OP_ALIGNED
     if (FAST) {
+      /* (rows behind the last that counts may be read if there are any: what comes of them is not written) */
+      const unsigned char *from = index ? base : base + first * stride;
+      const long long rows = index ? limit : hi - first;
+      buffer = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, (int)acc_min<long long>(OP_FARTHEST, rows > 0 ? (rows - 1) * stride + (long long)extent * SIZE : 0), 0x00020000);
+    }
+#endif
+#pragma unroll
+    for (int q = 0; q < MINE; ++q) {
+      const int s = slot(tid, q), m = first + major(s);
+      if (!FAST && LIST != OP_PLAIN) rows[q] = number(m, ask(m));
+#if OP_ALIGNED
+      if (EVEN && q > 0) continue;
+      if (FAST) {
+        /* (without an index, the rows that do not count lie behind the buffer's end) */
+        const int r = LIST == OP_PLAIN ? m : number(m, ask(m));
+        offset[q] = r < 0 ? OP_NOWHERE : (unsigned int)((LIST == OP_LISTED && index ? r : r - first) * (int)stride + element(s) * SIZE);
+      } else {
+        /* (columns beyond the result's: any will do) */
+        offset[q] = (unsigned int)(element(s) < extent ? element(s) : 0) * SIZE + (LIST == OP_LISTED ? 0 : (unsigned int)(major(s) * (int)stride));
+      }
+#else
+      /* (a row that does not count: the operand's first; what comes of it is not written) */
+      offset[q] = FAST ? acc_max(number(m, ask(m)), 0) * stride : element(s) * SIZE;
+#endif
+    }
+#if OP_TYPE == 3
+    const int m = acc_min(first + tid % TILE, hi - 1);
+    const int r = number(m, ask(m));
+    scale_row = r < 0 ? -1 : r * scales_stride;
+    scale_offset = r < 0 ? OP_NOWHERE : (unsigned int)scale_row;
+#endif
+  }
+
+#if OP_ALIGNED
+  /* ask for the lane's q-th chunk of the step at r, straight to LDS; `wave` is the same in all lanes, and known to be */
+  ACC_DEV void bring(acc_u4 *lds, const int tid, const int wave, const int q, const int r) const
+  {
+    const op_lds_ptr to = (op_lds_ptr)(lds + (CHUNKS < OP_THREADS ? wave * 64 % CHUNKS : wave * 64 + q * OP_THREADS));
+    const unsigned int at = offset[EVEN ? 0 : q];
+    const int further = EVEN ? q * APART * (int)stride : 0;       /* (the same in all lanes) */
+    if (FAST) {
+      const unsigned int from = r + column < extent ? at : OP_NOWHERE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to, 16, from, r * SIZE + further, 0, 0);
+    } else if (LIST == OP_LISTED) {
+      const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)OP_FARTHEST, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, to, 16, rows[q] < 0 ? OP_NOWHERE : (unsigned int)(rows[q] * (int)stride) + at, 0, 0, 0);
+    } else {
+      const __amdgpu_buffer_rsrc_t rest =
+          __builtin_amdgcn_make_buffer_rsrc((void *)(base + r * stride), 0, (int)acc_min<long long>(OP_FARTHEST, acc_max(0, hi - r) * stride), 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rest, to, 16, LIST == OP_GATED && rows[q] < 0 ? OP_NOWHERE : at, further, 0, 0);
+    }
+  }
+  /* what goes with a step beside its chunks: the scales, and what the index says of the next step's rows */
+  ACC_DEV void bring_rest(acc_u4 *lds, const int tid, const int wave, const int r)
+  {
+    if (!FAST && LIST != OP_PLAIN)
 #pragma unroll
       for (int q = 0; q < MINE; ++q) {
-        const int s = tid + q * OP_THREADS, i = s / 8;
-        row[q] = s < CHUNKS ? address(first + i) : (const op_elt *)0;
-        if (row[q]) row[q] += (((s % 8) ^ (i & 7))) * OP_EPC;
+        const int m = r + OP_STEP + major(slot(tid, q));
+        rows[q] = number(m, ask(m));
       }
-    }
-  }
-
-  ACC_DEV void load(acc_u4 (&v)[MINE], const int tid, const int r0) const
-  {
+#if OP_TYPE == 3
+    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void *)scales, 0, (int)OP_FARTHEST, 0x00020000);
 #pragma unroll
-    for (int q = 0; q < MINE; ++q) {
-      const int s = tid + q * OP_THREADS;
-      if (FAST) {
-        const int c = ((s % 8) ^ ((s / 8) & 7)) * OP_EPC;
-        v[q] = op_chunk<OP_ALIGNED>(row[q] + r0, row[q] ? extent - (r0 + c) : 0);
-      } else {
-        const op_elt *p = s < CHUNKS ? address(r0 + s / PITCH) : (const op_elt *)0;
-        const int c = minor + (s % PITCH) * OP_EPC;
-        v[q] = op_chunk<OP_ALIGNED>(p + c, p ? extent - c : 0);
+    for (int h = 0; h < 2; ++h) {
+      const int b = r / 16 + 4 * h;                               /* (blocks of a multiple of four: see the driver) */
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, (op_lds_ptr)((unsigned int *)(lds + CHUNKS) + h * SCALE_ROWS + wave * 64 % TILE), 4,
+                                               b < blocks ? scale_offset : OP_NOWHERE, b, 0, 0);
+    }
+#endif
+  }
+#else
+  /* the same by way of registers: `load` asks, whoever has asked puts what has come into LDS a step later.  `whole`: every
+   * chunk of the step lies within its row, and every row counts. */
+  ACC_DEV bool whole(const int r) const
+  {
+    return FAST ? r + OP_STEP <= extent : (r + OP_STEP <= hi) & (extent >= TILE) & (LIST == OP_PLAIN);
+  }
+  ACC_DEV void load(acc_u4 &v, const int tid, const int q, const int r, const bool whole) const
+  {
+    const int s = slot(tid, q);
+    if (whole) {
+      const unsigned char *p = FAST ? base + offset[q] + (long long)(r + column) * SIZE : base + (r + major(s)) * stride + offset[q];
+      v = ((const op_loose<op_mem> *)p)->v;
+      return;
+    }
+    /* elements of the row that are wanted first, and how many there are */
+    const int n = FAST ? 0 : LIST == OP_PLAIN ? number(r + major(s), 0) : rows[q], c = FAST ? r + column : element(s);
+    const unsigned char *row = FAST ? base + offset[q] : base + (long long)acc_max(n, 0) * stride;
+    if (extent < OP_EPC) {
+      op_mem e[OP_EPC];
+#pragma unroll
+      for (int k = 0; k < OP_EPC; ++k) e[k] = c + k < extent ? ((const op_mem *)row)[c + k] : (op_mem)0;
+      __builtin_memcpy(&v, e, 16);
+    } else {
+      const int at = acc_min(c, extent - OP_EPC);
+      v = op_shifted(((const op_loose<op_mem> *)(row + (long long)at * SIZE))->v, (c - at) * SIZE);
+    }
+    if (n < 0) v = acc_u4{0, 0, 0, 0};
+  }
+  ACC_DEV void load_rest(unsigned int (&w)[2], const int tid, const int r)
+  {
+    if (!FAST && LIST != OP_PLAIN)
+#pragma unroll
+      for (int q = 0; q < MINE; ++q) {
+        const int m = r + OP_STEP + major(slot(tid, q));
+        rows[q] = number(m, ask(m));
       }
-    }
-  }
-
-  ACC_DEV static void store(acc_u4 *lds, const acc_u4 (&v)[MINE], const int tid)
-  {
+#if OP_TYPE == 3
 #pragma unroll
-    for (int q = 0; q < MINE; ++q) {
-      const int s = tid + q * OP_THREADS;
-      if (CHUNKS % OP_THREADS == 0 || s < CHUNKS) lds[s] = v[q];
+    for (int h = 0; h < 2; ++h) {
+      const int b = r / 16 + 4 * h;
+      unsigned int four = 0;
+      if (scale_row >= 0)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) four |= (b + k < blocks ? (unsigned int)scales[scale_row + b + k] : 0u) << (8 * k);
+      w[h] = four;
     }
+#endif
   }
-
-  /* the fragment of rows i0 .. i0 + 15 and the step's half `h` */
-  ACC_DEV static op_frag fragment(const acc_u4 *lds, const int i0, const int h, const int lane)
+  ACC_DEV static void store_rest(acc_u4 *lds, const unsigned int (&w)[2], const int tid)
   {
-    const int i = i0 + (lane & 15), g = lane >> 4;
-    op_frag f;
+#if OP_TYPE == 3
+#pragma unroll
+    for (int h = 0; h < 2; ++h) ((unsigned int *)(lds + CHUNKS))[h * SCALE_ROWS + tid % TILE] = w[h];
+#endif
+  }
+#endif
+
+  /* Where a lane's part of the fragments of a wave lies whose first row is `first`, a multiple of 64 or all that the waves
+   * have: worked out once, so that a fragment is a constant further on (along r), or an exclusive or (across it). */
+  struct reader {
+    int at[2];                   /* along r: chunks, of either half; across r: elements */
+    int unit, flip;              /* across r: the wave's first unit, and what the lane's rows have theirs flipped by */
+    int scale;                   /* 4 bits: bytes, behind the chunks */
+  };
+  ACC_DEV static reader reads(const int first, const int lane)
+  {
+    const int l = lane & 15, g = lane >> 4;
+    reader w = {};
     if (FAST) {
-      const acc_u4 v = lds[i * 8 + ((h * 4 + g) ^ (i & 7))];
+      w.at[0] = (first + l) * 8 + (g ^ (l & 7));
+      w.at[1] = (first + l) * 8 + ((4 + g) ^ (l & 7));
+      w.scale = (first + l) * 4 + g;
+    } else {
+      const int r = OP_TYPE == 0 ? 4 * g : 8 * g + (l >> 2);
+      w.at[0] = r * TILE + (OP_TYPE == 0 ? l : (l & 3) * 4);
+      w.at[1] = w.at[0] + OP_STEP / 2 * TILE;
+      w.unit = first / 16;
+      w.flip = swizzle(r);
+    }
+    return w;
+  }
+  /* the n-th fragment of the step's half h */
+  ACC_DEV static op_frag fragment(const acc_u4 *lds, const reader &w, const int n, const int h)
+  {
+    op_frag f;
+#if OP_TYPE == 3
+    f.v = lds[w.at[h] + n * 128];
+    f.scale = ((const unsigned char *)(lds + CHUNKS))[w.scale + (h * SCALE_ROWS + n * 16) * 4];
+#else
+    if (FAST) {
+      const acc_u4 v = lds[w.at[h] + n * 128];
       __builtin_memcpy(&f, &v, 16);
     } else {
-      const op_elt *e = (const op_elt *)lds;
+      const int at = w.at[h] + (((w.unit + n) ^ w.flip) << 4);
+#if OP_TYPE == 0
+      const float *e = (const float *)lds + at;
 #pragma unroll
-      for (int t = 0; t < OP_EPC; ++t) f[t] = e[(h * (OP_BR / 2) + g * OP_EPC + t) * TILE + i];
+      for (int t = 0; t < 4; ++t) f[t] = e[t * TILE];
+#else
+      /* 4 x 16 elements at a time, turned on the way: lane l of a quarter names the four of row l / 4 from 4 (l % 4) on, and
+       * gets the four rows' l-th */
+      typedef short op_s4 __attribute__((ext_vector_type(4)));
+      const short *e = (const short *)lds + at;
+      const op_s4 one = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) op_s4 *)e);
+      const op_s4 two = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) op_s4 *)(e + 4 * TILE));
+      __builtin_memcpy(&f, &one, 8);
+      __builtin_memcpy((char *)&f + 8, &two, 8);
+#endif
     }
+#endif
     return f;
   }
 };
 
-typedef op_operand<OP_A_FAST, OP_BM> op_a;
-typedef op_operand<OP_B_FAST, OP_BN> op_b;
+typedef op_operand<OP_A_FAST, OP_BM, OP_A_FAST ? OP_LISTED : OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? OP_GATED : OP_LISTED> op_a;
+typedef op_operand<OP_B_FAST, OP_BN, OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? OP_LISTED : OP_GATED> op_b;
+
+/* a step of both operands */
+#define OP_STAGE (op_a::CHUNKS + op_a::SCALES + op_b::CHUNKS + op_b::SCALES)
+#define OP_B_AT (op_a::CHUNKS + op_a::SCALES)
+
+/* Half a step: the products of fa and fb; meanwhile half h of the step in `lds` is read into na and nb, a few fragments for
+ * every row of products, and `also(i)`, i from 0 to OP_FM - 1, goes on.  The order is kept as it stands here: left to itself
+ * the compiler puts all reads in front of all products.  b's fragment is the instruction's first operand: a lane then has
+ * four neighbouring j of one i.
+ * OP_ROLL: na is fa, a fragment of which is read anew as soon as its products are under way.  That is for the forms whose
+ * addresses and scales leave no registers for a second set. */
+#define OP_ROLL (OP_TYPE == 3 || OP_OUTER || (OP_TYPE == 0 && !OP_B_FAST))
+template <typename F>
+ACC_DEV void op_half(acc_f4 (&c)[OP_FM][OP_FN], op_frag (&fa)[OP_FM], op_frag (&fb)[OP_FN], op_frag (&na)[OP_FM], op_frag (&nb)[OP_FN],
+                     const acc_u4 *lds, op_a::reader wa, op_b::reader wb, const int h, F also)
+{
+  /* (not to be worked out for every fragment ahead of the loop: there are not the registers for that) */
+  if (!OP_A_FAST) asm volatile("" : "+v"(wa.flip));
+  if (!OP_B_FAST) asm volatile("" : "+v"(wb.flip));
+  constexpr int READS = OP_ROLL ? (OP_FN + OP_FM - 1) / OP_FM : (OP_FM + OP_FN + OP_FM - 1) / OP_FM;
+#pragma unroll
+  for (int i = 0; i < OP_FM; ++i) {
+#pragma unroll
+    for (int n = i * READS; n < (i + 1) * READS; ++n) {
+      if (n < OP_FN) nb[n] = op_b::fragment(lds + OP_B_AT, wb, n, h);
+      else if (!OP_ROLL && n < OP_FN + OP_FM) na[n - OP_FN] = op_a::fragment(lds, wa, n - OP_FN, h);
+    }
+    also(i);
+#pragma unroll
+    for (int j = 0; j < OP_FN; ++j) c[i][j] = op_mfma(fb[j], fa[i], c[i][j]);
+    if (OP_ROLL) fa[i] = op_a::fragment(lds, wa, i, h);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+/* everything that this wave has asked for has come (what it asked for LDS, too), then everybody's */
+ACC_DEV void op_meet(const bool loads)
+{
+  if (loads) __builtin_amdgcn_s_waitcnt(0 | 7 << 4);              /* vmcnt and lgkmcnt 0, in this target's encoding */
+  else __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 3 << 14);         /* lgkmcnt 0 */
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_product_args p)
 {
   if (p.guard && *p.guard == 0u) return;
-  __shared__ acc_u4 lds_a[2][op_a::CHUNKS], lds_b[2][op_b::CHUNKS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  /* (two variables, not one of two parts: loads to one are then known to leave the other alone) */
+  __shared__ acc_u4 lds0[OP_STAGE], lds1[OP_STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wi = (wave / OP_WN) * (OP_BM / OP_WM), wj = (wave % OP_WN) * (OP_BN / OP_WN);
 
-  /* the tile, and the sum's range */
+  /* the tile, and the sum's range; every die has a run of tiles of its own, neighbours of which share operands */
   int expert, i0, j0, iend, jend, r0, r1;
 #if OP_OUTER
   {
-    const long long b = blockIdx.x;
-    expert = (int)(b / ((long long)p.tiles_i * p.tiles_j));
-    const int t = (int)(b % ((long long)p.tiles_i * p.tiles_j));
+    const long long block = op_die_run(blockIdx.x, gridDim.x);
+    expert = (int)(block / ((long long)p.tiles_i * p.tiles_j));
+    const int t = (int)(block % ((long long)p.tiles_i * p.tiles_j));
     i0 = (t / p.tiles_j) * OP_BM;
     j0 = (t % p.tiles_j) * OP_BN;
     iend = p.ni;
@@ -143,9 +419,12 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
   }
 #else
   {
-    const int t = blockIdx.x / p.tiles_j;
-    j0 = (int)(blockIdx.x % p.tiles_j) * OP_BN;
-    const op_tile tile = op_find_tile(p.offsets, p.experts, (int)p.rows, OP_BM, t);
+    /* (the grid is for the worst lengths; the tiles that there are, are shared out evenly) */
+    const long long tiles = (long long)op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM) * p.tiles_j;
+    if (blockIdx.x >= tiles) return;
+    const long long block = op_die_run(blockIdx.x, tiles);
+    j0 = (int)(block % p.tiles_j) * OP_BN;
+    const op_tile tile = op_find_tile(p.offsets, p.experts, (int)p.rows, OP_BM, (int)(block / p.tiles_j));
     if (tile.begin >= tile.end) return;
     expert = tile.expert;
     i0 = tile.begin;
@@ -158,40 +437,53 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
 
   op_a a;
   op_b b;
-  a.base = (const op_elt *)p.a;
-  a.stride = p.a_stride;
+  a.base = (const unsigned char *)p.a;
+  b.base = (const unsigned char *)p.b;
+  a.stride = p.a_stride * op_a::SIZE;
+  b.stride = p.b_stride * op_b::SIZE;
   a.index = p.index_a;
   a.limit = p.a_rows;
-  a.gate = b.gate = (const int *)0;
-  a.per = b.per = p.per;
-  b.base = (const op_elt *)p.b;
-  b.stride = p.b_stride;
+  a.per_mul = b.per_mul = p.per_mul;
+  a.per_shift = b.per_shift = p.per_shift;
 #if OP_OUTER
   b.index = p.index_b;
   b.limit = p.b_rows;
-  if (!p.index_a && p.index_b) { a.gate = p.index_b; a.limit = p.b_rows; }
-  if (!p.index_b && p.index_a) { b.gate = p.index_a; b.limit = p.a_rows; }
+  if (OP_INDEX == 1) { a.index = p.index_b; a.limit = p.b_rows; }
+  if (OP_INDEX == 2) { b.index = p.index_a; b.limit = p.a_rows; }
   a.lo = b.lo = r0;
   a.hi = b.hi = r1;
-  a.minor = i0;
-  a.extent = p.ni;
-  b.minor = j0;
-  b.extent = p.nj;
+  a.base += (long long)i0 * op_a::SIZE;
+  b.base += (long long)j0 * op_b::SIZE;
+  a.extent = p.ni - i0;
+  b.extent = p.nj - j0;
+  a.start(tid, r0);
+  b.start(tid, r0);
 #else
-  b.base += (long long)acc_max(expert, 0) * p.b_expert;
+  b.base += acc_max(expert, 0) * p.b_expert * op_b::SIZE;
   b.index = (const int *)0;
   b.limit = 0;
   a.lo = i0;
   a.hi = iend;
-  a.minor = 0;
   a.extent = p.k;
   b.lo = 0;
-  b.hi = OP_B_FAST ? jend : p.k;
-  b.minor = j0;
-  b.extent = OP_B_FAST ? p.k : jend;
+  if (OP_B_FAST) {
+    b.hi = jend;
+    b.extent = p.k;
+  } else {
+    b.hi = p.k;
+    b.base += (long long)j0 * op_b::SIZE;
+    b.extent = jend - j0;
+  }
+#if OP_TYPE == 3
+  a.scales = p.a_scales;
+  a.scales_stride = p.a_scales_stride;
+  b.scales = p.b_scales + acc_max(expert, 0) * p.b_scales_expert;
+  b.scales_stride = p.b_scales_stride;
+  a.blocks = b.blocks = p.k / 16;
 #endif
   a.start(tid, i0);
-  b.start(tid, j0);
+  b.start(tid, OP_B_FAST ? j0 : 0);
+#endif
 
   acc_f4 c[OP_FM][OP_FN];
 #pragma unroll
@@ -199,37 +491,90 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
 #pragma unroll
     for (int j = 0; j < OP_FN; ++j) c[i][j] = acc_f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  acc_u4 va[op_a::MINE], vb[op_b::MINE];
   if (r0 < r1) {
-    a.load(va, tid, r0);
-    b.load(vb, tid, r0);
-  }
-  int buf = 0;
-  for (int r = r0; r < r1; r += OP_BR, buf ^= 1) {
-    /* two buffers, one barrier a step: whoever writes into a buffer has passed the barrier that every wave reached after
-     * it last read it */
-    op_a::store(lds_a[buf], va, tid);
-    op_b::store(lds_b[buf], vb, tid);
-    __syncthreads();
-    if (r + OP_BR < r1) {
-      a.load(va, tid, r + OP_BR);
-      b.load(vb, tid, r + OP_BR);
-    }
+    op_frag fa[OP_FM], fb[OP_FN], ga[OP_FM], gb[OP_FN];
+    const auto nothing = [](int) {};
+    const op_a::reader wa = op_a::reads(wi, lane);
+    const op_b::reader wb = op_b::reads(wj, lane);
+    const auto first = [&]() {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      op_frag fa[OP_FM], fb[OP_FN];
+      for (int j = 0; j < OP_FN; ++j) fb[j] = op_b::fragment(lds0 + OP_B_AT, wb, j, 0);
 #pragma unroll
-      for (int i = 0; i < OP_FM; ++i) fa[i] = op_a::fragment(lds_a[buf], wi + i * 16, h, lane);
+      for (int i = 0; i < OP_FM; ++i) fa[i] = op_a::fragment(lds0, wa, i, 0);
+    };
+    /* a lane's chunks of a step, shared out over the half's fragments */
+    constexpr int ALL = op_a::MINE + op_b::MINE, EACH = (ALL + OP_FM - 1) / OP_FM;
+#if OP_ALIGNED
+    const auto bring = [&](acc_u4 *lds, const int n, const int r) {
+      if (n < op_a::MINE) a.bring(lds, tid, wave, n, r);
+      else if (n < ALL) b.bring(lds + OP_B_AT, tid, wave, n - op_a::MINE, r);
+      if (n == ALL - 1) {
+        a.bring_rest(lds, tid, wave, r);
+        b.bring_rest(lds + OP_B_AT, tid, wave, r);
+      }
+    };
 #pragma unroll
-      for (int j = 0; j < OP_FN; ++j) fb[j] = op_b::fragment(lds_b[buf], wj + j * 16, h, lane);
+    for (int n = 0; n < ALL; ++n) bring(lds0, n, r0);
 #pragma unroll
-      for (int i = 0; i < OP_FM; ++i)
+    for (int n = 0; n < ALL; ++n) bring(lds1, n, r0 + OP_STEP);
+    op_meet(true);
+    first();
+    /* the step at r lies in `here`, the fragments of its first half in fa, fb */
+    const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
+      op_half(c, fa, fb, ga, gb, here, wa, wb, 1, nothing);
+      op_meet(true);
+      op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, there, wa, wb, 0, [&](const int i) {
 #pragma unroll
-        for (int j = 0; j < OP_FN; ++j) c[i][j] = op_mfma(fb[j], fa[i], c[i][j]);
-    }
+        for (int n = 0; n < EACH; ++n) bring(here, i * EACH + n, r + 2 * OP_STEP);
+      });
+    };
+#else
+    acc_u4 va[op_a::MINE], vb[op_b::MINE];
+    unsigned int sa[2], sb[2];
+#define OP_LOAD(r)                                                                          \
+    do {                                                                                    \
+      const bool whole = a.whole(r) & b.whole(r);                                           \
+      if (whole) {                                                                          \
+        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, true);  \
+        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, true);  \
+      } else {                                                                              \
+        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, false); \
+        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, false); \
+      }                                                                                     \
+      a.load_rest(sa, tid, r);                                                              \
+      b.load_rest(sb, tid, r);                                                              \
+    } while (0)
+#define OP_STORE(lds)                                                                       \
+    do {                                                                                    \
+      _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) lds[op_a::slot(tid, n)] = va[n];           \
+      _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) lds[OP_B_AT + op_b::slot(tid, n)] = vb[n]; \
+      op_a::store_rest(lds, sa, tid);                                                       \
+      op_b::store_rest(lds + OP_B_AT, sb, tid);                                             \
+    } while (0)
+    OP_LOAD(r0);
+    OP_STORE(lds0);
+    OP_LOAD(r0 + OP_STEP);
+    op_meet(false);
+    first();
+    const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
+      OP_STORE(there);
+      OP_LOAD(r + 2 * OP_STEP);
+      op_half(c, fa, fb, ga, gb, here, wa, wb, 1, nothing);
+      op_meet(false);
+      op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, there, wa, wb, 0, nothing);
+    };
+#endif
+    /* (an odd number of steps has one of zeros behind it: with a way out between the two, the sums would change registers) */
+    int r = r0;
+    do {
+      round(lds0, lds1, r);
+      round(lds1, lds0, r + OP_STEP);
+      r += 2 * OP_STEP;
+    } while (r < r1);
+    /* what is still on its way to LDS arrives before the workgroup gives it up */
+    __builtin_amdgcn_s_waitcnt(0 | 7 << 4);
   }
 
-  /* b's fragment is the instruction's first operand: a lane has four neighbouring j of one i */
 #pragma unroll
   for (int i = 0; i < OP_FM; ++i) {
     const int ri = i0 + wi + i * 16 + (lane & 15);
@@ -239,14 +584,22 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
 #if OP_OUTER
     out += (long long)expert * p.out_expert;
 #else
-    none = p.index_a && !a.address(ri);
+    none = p.index_a && a.number(ri, a.ask(ri)) < 0;
 #endif
 #pragma unroll
     for (int j = 0; j < OP_FN; ++j) {
       const int cj = j0 + wj + j * 16 + 4 * (lane >> 4);
+      typedef op_elt op_e4 __attribute__((ext_vector_type(4)));
+      op_e4 v;
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (cj + t < jend) out[cj + t] = (op_elt)(none ? 0.0f : c[i][j][t]);
+      for (int t = 0; t < 4; ++t) v[t] = (op_elt)(none ? 0.0f : c[i][j][t]);
+      if (p.out_vectors) {
+        if (cj < jend) *(op_e4 *)(out + cj) = v;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (cj + t < jend) out[cj + t] = v[t];
+      }
     }
   }
 }
