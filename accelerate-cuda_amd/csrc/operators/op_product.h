@@ -40,11 +40,16 @@ typedef __bf16 op_frag __attribute__((ext_vector_type(8)));
 ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
 #else
 typedef int op_i8 __attribute__((ext_vector_type(8)));
-struct op_frag { acc_u4 v; int scale; };           /* a block of 32 and its scale */
-ACC_DEV acc_f4 op_mfma(const op_frag &x, const op_frag &y, const acc_f4 c)
+typedef acc_u4 op_frag;                            /* a block of 32 */
+/* `sx` holds the scales of four fragments, x's the nx-th */
+ACC_DEV acc_f4 op_mfma_scaled(const op_frag &x, const op_frag &y, const acc_f4 c, const int sx, const int nx, const int sy, const int ny)
 {
-  const op_i8 a = {(int)x.v.x, (int)x.v.y, (int)x.v.z, (int)x.v.w, 0, 0, 0, 0}, b = {(int)y.v.x, (int)y.v.y, (int)y.v.z, (int)y.v.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, x.scale, 0, y.scale);
+  const op_i8 a = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}, b = {(int)y.x, (int)y.y, (int)y.z, (int)y.w, 0, 0, 0, 0};
+  /* (the byte to take is part of the instruction; which it is, is known once the loops are unrolled) */
+#define OP_CASE(i, j) case 4 * i + j: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, i, sx, j, sy);
+#define OP_CASES(i) OP_CASE(i, 0) OP_CASE(i, 1) OP_CASE(i, 2) OP_CASE(i, 3)
+  switch (4 * nx + ny) { OP_CASES(0) OP_CASES(1) OP_CASES(2) OP_CASES(3) }
+  return c;
 }
 #endif
 
@@ -86,16 +91,17 @@ ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
  * addresses are one offset of 32 bits a chunk (the driver sees to it that they suffice).
  * Otherwise rows start anywhere; chunks go by way of registers, with addresses of 64 bits.  A chunk that would reach
  * beyond its row's end is read that much earlier and shifted into place, so that no read leaves its row. */
-template <bool FAST, int TILE, int LIST> struct op_operand {
+template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
   static constexpr int CHUNKS = TILE * 8;                         /* of a step */
   static constexpr int MINE = (CHUNKS + OP_THREADS - 1) / OP_THREADS;
   static constexpr int PITCH = FAST ? 8 : TILE / OP_EPC;          /* chunks of a row */
   static constexpr int UNITS = TILE / 16;                         /* across r: of a row */
   static constexpr int SIZE = (int)sizeof(op_mem);
-  /* 4 bits: the rows' scales of a step, behind them: the first half's, four a row, then the second's (a wave brings 64
-   * rows', however few there are) */
-  static constexpr int SCALE_ROWS = TILE < 64 ? 64 : TILE;
-  static constexpr int SCALES = OP_TYPE == 3 ? 2 * SCALE_ROWS / 4 : 0;
+  /* 4 bits: the scales of a step's rows lie behind them, those of the first half, then of the second; in each, words that hold
+   * the same block of up to four rows 16 apart, as the fragments of a wave's up to 64 rows want them */
+  static constexpr int SHARE = TILE / WAVES < 64 ? TILE / WAVES : 64;
+  static constexpr int SCALE_WORDS = TILE / SHARE * 64;           /* of a half */
+  static constexpr int SCALES = OP_TYPE == 3 ? 2 * SCALE_WORDS / 4 : 0;
   static_assert(CHUNKS % 64 == 0 && (CHUNKS % OP_THREADS == 0 || OP_THREADS % CHUNKS == 0), "whole waves, the same number each");
 
   const unsigned char *base;     /* along r: of the operand; across it: of the tile's first column */
@@ -107,7 +113,10 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
   int limit;                     /* rows an index may name */
   int lo, hi;                    /* the rows that count: along r the i's, across it the r's */
   int extent;                    /* elements of a row that count, from `base` on */
-  int rows[MINE];                /* across r, with an index: which rows of memory the next step's are that is to be asked for; -1: none */
+  /* Across r, with an index: which rows of memory the next step's are that is to be asked for, -1: none.  The aligned form has
+   * them in scalar registers, for all rows that a wave has in a chunk. */
+  static constexpr int ROWS = OP_ALIGNED && !FAST ? (PITCH < 64 ? 64 / PITCH : 1) : 1;
+  int rows[MINE][ROWS];
   int column;                    /* along r: the lane's chunks' first element (the same of all of them) */
   /* whether a lane's chunks lie equally far apart in memory: the rows between them are as many, and swizzled alike (for
    * Float32 across r they are not) */
@@ -117,16 +126,9 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
   unsigned int offset[EVEN ? 1 : MINE];   /* of the lane's chunks, in bytes: along r from the tile's first row, across it from the step's */
   __amdgpu_buffer_rsrc_t buffer; /* along r */
 #else
-  long long offset[MINE];        /* along r: of the lane's rows from `base`; across r: of its chunks from their rows' beginning */
+  long long offset[!FAST && EVEN ? 1 : MINE];   /* of the lane's chunks, in bytes: along r from `base`, across it from the step's first row (with an index:
+                                  * from the row's beginning) */
 #endif
-#if OP_TYPE == 3
-  const unsigned char *scales;
-  long long scales_stride;
-  long long scale_row;           /* where the scales of the lane's row lie; -1: no such row */
-  unsigned int scale_offset;
-  int blocks;
-#endif
-
   /* a lane's q-th chunk of a step: where there are fewer chunks than lanes, several waves bring the same ones */
   ACC_DEV static int slot(const int tid, const int q) { return CHUNKS < OP_THREADS ? tid % CHUNKS : tid + q * OP_THREADS; }
   ACC_DEV static int swizzle(const int r)
@@ -153,6 +155,23 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
     const bool there = (m >= lo) & (m < hi) & (!listed | ((at >= 0) & (r < limit)));
     return there ? LIST == OP_GATED ? m : r : -1;
   }
+  /* across r: the rows of the step at r */
+  ACC_DEV void look(const int tid, const int wave, const int r)
+  {
+    if (FAST || LIST == OP_PLAIN) return;
+#pragma unroll
+    for (int q = 0; q < MINE; ++q)
+#pragma unroll
+      for (int n = 0; n < ROWS; ++n) {
+#if OP_ALIGNED
+        const int m = r + major(wave * 64 + q * OP_THREADS) + n;
+        const int at = ((__attribute__((address_space(4))) const int *)(unsigned long long)index)[acc_max(lo, acc_min(m, hi - 1))];
+#else
+        const int m = r + major(slot(tid, q)), at = ask(m);
+#endif
+        rows[q][n] = number(m, at);
+      }
+  }
   /* what the index says of row m (of the nearest row that counts, if that one does not) */
   ACC_DEV int ask(const int m) const { return (FAST ? LIST == OP_LISTED && index != 0 : LIST != OP_PLAIN) ? index[acc_max(lo, acc_min(m, hi - 1))] : 0; }
 
@@ -172,7 +191,6 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
 #pragma unroll
     for (int q = 0; q < MINE; ++q) {
       const int s = slot(tid, q), m = first + major(s);
-      if (!FAST && LIST != OP_PLAIN) rows[q] = number(m, ask(m));
 #if OP_ALIGNED
       if (EVEN && q > 0) continue;
       if (FAST) {
@@ -184,19 +202,25 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
         offset[q] = (unsigned int)(element(s) < extent ? element(s) : 0) * SIZE + (LIST == OP_LISTED ? 0 : (unsigned int)(major(s) * (int)stride));
       }
 #else
+      if (!FAST && EVEN && q > 0) continue;
       /* (a row that does not count: the operand's first; what comes of it is not written) */
-      offset[q] = FAST ? acc_max(number(m, ask(m)), 0) * stride : element(s) * SIZE;
+      offset[q] = FAST ? acc_max(number(m, ask(m)), 0) * stride + column * SIZE : element(s) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
 #endif
     }
-#if OP_TYPE == 3
-    const int m = acc_min(first + tid % TILE, hi - 1);
-    const int r = number(m, ask(m));
-    scale_row = r < 0 ? -1 : r * scales_stride;
-    scale_offset = r < 0 ? OP_NOWHERE : (unsigned int)scale_row;
-#endif
   }
 
 #if OP_ALIGNED
+  /* f of the lane's row among those of its wave's q-th chunks (f is worked out once for the wave) */
+  template <typename F> ACC_DEV unsigned int of_row(const int q, const int tid, F f) const
+  {
+    unsigned int v = f(rows[q][0]);
+#pragma unroll
+    for (int n = 1; n < ROWS; ++n) {
+      const unsigned int w = f(rows[q][n]);
+      v = (tid & 63) / PITCH == n ? w : v;
+    }
+    return v;
+  }
   /* ask for the lane's q-th chunk of the step at r, straight to LDS; `wave` is the same in all lanes, and known to be */
   ACC_DEV void bring(acc_u4 *lds, const int tid, const int wave, const int q, const int r) const
   {
@@ -208,50 +232,32 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to, 16, from, r * SIZE + further, 0, 0);
     } else if (LIST == OP_LISTED) {
       const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)OP_FARTHEST, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, to, 16, rows[q] < 0 ? OP_NOWHERE : (unsigned int)(rows[q] * (int)stride) + at, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, to, 16, of_row(q, tid, [&](const int n) { return n < 0 ? OP_NOWHERE : (unsigned int)(n * (int)stride); }) + at, 0, 0, 0);
     } else {
       const __amdgpu_buffer_rsrc_t rest =
           __builtin_amdgcn_make_buffer_rsrc((void *)(base + r * stride), 0, (int)acc_min<long long>(OP_FARTHEST, acc_max(0, hi - r) * stride), 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rest, to, 16, LIST == OP_GATED && rows[q] < 0 ? OP_NOWHERE : at, further, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rest, to, 16, LIST == OP_GATED ? of_row(q, tid, [](const int n) { return n < 0 ? OP_NOWHERE : 0u; }) | at : at, further, 0, 0);
     }
-  }
-  /* what goes with a step beside its chunks: the scales, and what the index says of the next step's rows */
-  ACC_DEV void bring_rest(acc_u4 *lds, const int tid, const int wave, const int r)
-  {
-    if (!FAST && LIST != OP_PLAIN)
-#pragma unroll
-      for (int q = 0; q < MINE; ++q) {
-        const int m = r + OP_STEP + major(slot(tid, q));
-        rows[q] = number(m, ask(m));
-      }
-#if OP_TYPE == 3
-    const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void *)scales, 0, (int)OP_FARTHEST, 0x00020000);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int b = r / 16 + 4 * h;                               /* (blocks of a multiple of four: see the driver) */
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, (op_lds_ptr)((unsigned int *)(lds + CHUNKS) + h * SCALE_ROWS + wave * 64 % TILE), 4,
-                                               b < blocks ? scale_offset : OP_NOWHERE, b, 0, 0);
-    }
-#endif
   }
 #else
   /* the same by way of registers: `load` asks, whoever has asked puts what has come into LDS a step later.  `whole`: every
-   * chunk of the step lies within its row, and every row counts. */
-  ACC_DEV bool whole(const int r) const
-  {
-    return FAST ? r + OP_STEP <= extent : (r + OP_STEP <= hi) & (extent >= TILE) & (LIST == OP_PLAIN);
-  }
+   * chunk of the step lies within its row (and across r, without an index, every row counts). */
+  ACC_DEV bool whole(const int r) const { return FAST ? r + OP_STEP <= extent : ((LIST != OP_PLAIN) | (r + OP_STEP <= hi)) & (extent >= TILE); }
   ACC_DEV void load(acc_u4 &v, const int tid, const int q, const int r, const bool whole) const
   {
     const int s = slot(tid, q);
     if (whole) {
-      const unsigned char *p = FAST ? base + offset[q] + (long long)(r + column) * SIZE : base + (r + major(s)) * stride + offset[q];
+      const unsigned char *p;
+      if (FAST) p = base + (long long)r * SIZE + offset[q];
+      else if (LIST == OP_PLAIN) p = base + (r + (EVEN ? q * APART : 0)) * stride + offset[EVEN ? 0 : q];
+      else p = base + acc_max(rows[q][0], 0) * stride + offset[EVEN ? 0 : q];
       v = ((const op_loose<op_mem> *)p)->v;
+      if (!FAST && LIST != OP_PLAIN && rows[q][0] < 0) v = acc_u4{0, 0, 0, 0};
       return;
     }
     /* elements of the row that are wanted first, and how many there are */
-    const int n = FAST ? 0 : LIST == OP_PLAIN ? number(r + major(s), 0) : rows[q], c = FAST ? r + column : element(s);
-    const unsigned char *row = FAST ? base + offset[q] : base + (long long)acc_max(n, 0) * stride;
+    const int n = FAST ? 0 : LIST == OP_PLAIN ? number(r + major(s), 0) : rows[q][0], c = FAST ? r + column : element(s);
+    const unsigned char *row = FAST ? base + offset[q] - column * SIZE : base + (long long)acc_max(n, 0) * stride;
     if (extent < OP_EPC) {
       op_mem e[OP_EPC];
 #pragma unroll
@@ -263,33 +269,6 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
     }
     if (n < 0) v = acc_u4{0, 0, 0, 0};
   }
-  ACC_DEV void load_rest(unsigned int (&w)[2], const int tid, const int r)
-  {
-    if (!FAST && LIST != OP_PLAIN)
-#pragma unroll
-      for (int q = 0; q < MINE; ++q) {
-        const int m = r + OP_STEP + major(slot(tid, q));
-        rows[q] = number(m, ask(m));
-      }
-#if OP_TYPE == 3
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int b = r / 16 + 4 * h;
-      unsigned int four = 0;
-      if (scale_row >= 0)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) four |= (b + k < blocks ? (unsigned int)scales[scale_row + b + k] : 0u) << (8 * k);
-      w[h] = four;
-    }
-#endif
-  }
-  ACC_DEV static void store_rest(acc_u4 *lds, const unsigned int (&w)[2], const int tid)
-  {
-#if OP_TYPE == 3
-#pragma unroll
-    for (int h = 0; h < 2; ++h) ((unsigned int *)(lds + CHUNKS))[h * SCALE_ROWS + tid % TILE] = w[h];
-#endif
-  }
 #endif
 
   /* Where a lane's part of the fragments of a wave lies whose first row is `first`, a multiple of 64 or all that the waves
@@ -297,7 +276,7 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
   struct reader {
     int at[2];                   /* along r: chunks, of either half; across r: elements */
     int unit, flip;              /* across r: the wave's first unit, and what the lane's rows have theirs flipped by */
-    int scale;                   /* 4 bits: bytes, behind the chunks */
+    int scale;                   /* 4 bits: words, behind the chunks */
   };
   ACC_DEV static reader reads(const int first, const int lane)
   {
@@ -306,7 +285,7 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
     if (FAST) {
       w.at[0] = (first + l) * 8 + (g ^ (l & 7));
       w.at[1] = (first + l) * 8 + ((4 + g) ^ (l & 7));
-      w.scale = (first + l) * 4 + g;
+      w.scale = first / SHARE * 64 + g * 16 + l;
     } else {
       const int r = OP_TYPE == 0 ? 4 * g : 8 * g + (l >> 2);
       w.at[0] = r * TILE + (OP_TYPE == 0 ? l : (l & 3) * 4);
@@ -320,10 +299,6 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
   ACC_DEV static op_frag fragment(const acc_u4 *lds, const reader &w, const int n, const int h)
   {
     op_frag f;
-#if OP_TYPE == 3
-    f.v = lds[w.at[h] + n * 128];
-    f.scale = ((const unsigned char *)(lds + CHUNKS))[w.scale + (h * SCALE_ROWS + n * 16) * 4];
-#else
     if (FAST) {
       const acc_u4 v = lds[w.at[h] + n * 128];
       __builtin_memcpy(&f, &v, 16);
@@ -344,13 +319,14 @@ template <bool FAST, int TILE, int LIST> struct op_operand {
       __builtin_memcpy((char *)&f + 8, &two, 8);
 #endif
     }
-#endif
     return f;
   }
+  /* 4 bits: the scales of fragments 4 n to 4 n + 3 */
+  ACC_DEV static int scale(const acc_u4 *lds, const reader &w, const int n, const int h) { return ((const int *)(lds + CHUNKS))[w.scale + h * SCALE_WORDS + n * 64]; }
 };
 
-typedef op_operand<OP_A_FAST, OP_BM, OP_A_FAST ? OP_LISTED : OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? OP_GATED : OP_LISTED> op_a;
-typedef op_operand<OP_B_FAST, OP_BN, OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? OP_LISTED : OP_GATED> op_b;
+typedef op_operand<OP_A_FAST, OP_BM, OP_WM, OP_A_FAST ? OP_LISTED : OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? OP_GATED : OP_LISTED> op_a;
+typedef op_operand<OP_B_FAST, OP_BN, OP_WN, OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? OP_LISTED : OP_GATED> op_b;
 
 /* a step of both operands */
 #define OP_STAGE (op_a::CHUNKS + op_a::SCALES + op_b::CHUNKS + op_b::SCALES)
@@ -362,9 +338,14 @@ typedef op_operand<OP_B_FAST, OP_BN, OP_INDEX == 0 ? OP_PLAIN : OP_INDEX == 1 ? 
  * four neighbouring j of one i.
  * OP_ROLL: na is fa, a fragment of which is read anew as soon as its products are under way.  That is for the forms whose
  * addresses and scales leave no registers for a second set. */
+#define OP_SM ((OP_FM + 3) / 4)
+#define OP_SN ((OP_FN + 3) / 4)
 #define OP_ROLL (OP_TYPE == 3 || OP_OUTER || (OP_TYPE == 0 && !OP_B_FAST))
 template <typename F>
 ACC_DEV void op_half(acc_f4 (&c)[OP_FM][OP_FN], op_frag (&fa)[OP_FM], op_frag (&fb)[OP_FN], op_frag (&na)[OP_FM], op_frag (&nb)[OP_FN],
+#if OP_TYPE == 3
+                     const int (&sa)[OP_SM], const int (&sb)[OP_SN], int (&nsa)[OP_SM], int (&nsb)[OP_SN],
+#endif
                      const acc_u4 *lds, op_a::reader wa, op_b::reader wb, const int h, F also)
 {
   /* (not to be worked out for every fragment ahead of the loop: there are not the registers for that) */
@@ -375,12 +356,20 @@ ACC_DEV void op_half(acc_f4 (&c)[OP_FM][OP_FN], op_frag (&fa)[OP_FM], op_frag (&
   for (int i = 0; i < OP_FM; ++i) {
 #pragma unroll
     for (int n = i * READS; n < (i + 1) * READS; ++n) {
+#if OP_TYPE == 3
+      if (n % 4 == 0 && n < OP_FN) nsb[n / 4] = op_b::scale(lds + OP_B_AT, wb, n / 4, h);
+#endif
       if (n < OP_FN) nb[n] = op_b::fragment(lds + OP_B_AT, wb, n, h);
       else if (!OP_ROLL && n < OP_FN + OP_FM) na[n - OP_FN] = op_a::fragment(lds, wa, n - OP_FN, h);
     }
     also(i);
 #pragma unroll
+#if OP_TYPE == 3
+    for (int j = 0; j < OP_FN; ++j) c[i][j] = op_mfma_scaled(fb[j], fa[i], c[i][j], sb[j / 4], j % 4, sa[i / 4], i % 4);
+    if (i % 4 == 0) nsa[i / 4] = op_a::scale(lds, wa, i / 4, h);
+#else
     for (int j = 0; j < OP_FN; ++j) c[i][j] = op_mfma(fb[j], fa[i], c[i][j]);
+#endif
     if (OP_ROLL) fa[i] = op_a::fragment(lds, wa, i, h);
     __builtin_amdgcn_sched_barrier(0);
   }
@@ -396,7 +385,8 @@ ACC_DEV void op_meet(const bool loads)
   asm volatile("" ::: "memory");
 }
 
-extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_product_args p)
+/* (at least two waves a SIMD: more than 256 registers would leave a compute unit to a workgroup of four waves) */
+extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_waves_per_eu(2))) product(const acc_product_args p)
 {
   if (p.guard && *p.guard == 0u) return;
   /* (two variables, not one of two parts: loads to one are then known to leave the other alone) */
@@ -474,13 +464,6 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
     b.base += (long long)j0 * op_b::SIZE;
     b.extent = jend - j0;
   }
-#if OP_TYPE == 3
-  a.scales = p.a_scales;
-  a.scales_stride = p.a_scales_stride;
-  b.scales = p.b_scales + acc_max(expert, 0) * p.b_scales_expert;
-  b.scales_stride = p.b_scales_stride;
-  a.blocks = b.blocks = p.k / 16;
-#endif
   a.start(tid, i0);
   b.start(tid, OP_B_FAST ? j0 : 0);
 #endif
@@ -494,6 +477,53 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
   if (r0 < r1) {
     op_frag fa[OP_FM], fb[OP_FN], ga[OP_FM], gb[OP_FN];
     const auto nothing = [](int) {};
+#if OP_TYPE == 3
+    /* The scales go by way of registers, a lane a row of either operand: asked for two steps ahead of their use, put into LDS
+     * one step ahead. */
+    int fsa[OP_SM], fsb[OP_SN], gsa[OP_SM], gsb[OP_SN];
+    static_assert(OP_BM + OP_BN <= OP_THREADS, "a lane a row");
+    const int at = tid % (OP_BM + OP_BN), blocks = p.k / 16;
+    const bool of_a = at < OP_BM;
+    const int si = of_a ? at : at - OP_BM, share = of_a ? op_a::SHARE : op_b::SHARE;
+    const int scale_row = of_a ? a.number(i0 + si, a.ask(i0 + si)) : b.number(j0 + si, 0);
+    /* (a row that there is not reads the matrix's first scales: what comes of it is not written) */
+    const unsigned char *scales = of_a && scale_row >= 0 ? p.a_scales + scale_row * p.a_scales_stride
+                                                         : p.b_scales + expert * p.b_scales_expert + acc_max(scale_row, 0) * p.b_scales_stride;
+    const int scale_byte = (of_a ? op_a::CHUNKS * 16 : (OP_B_AT + op_b::CHUNKS) * 16) + (si / share * 64 + si % 16) * 4 + si % share / 16;
+    const int scale_half = (of_a ? op_a::SCALE_WORDS : op_b::SCALE_WORDS) * 4;
+    unsigned int scale[2];
+    const auto ask_scales = [&](const int r) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = r / 16 + 4 * h;
+#if OP_ALIGNED
+        /* (blocks are whole fours; behind the last one a scale of zeros, as the codes there) */
+        const unsigned int four = *(const unsigned int *)(scales + acc_min(k, blocks - 4));
+        scale[h] = k < blocks ? four : 0u;
+#else
+        scale[h] = 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const unsigned int one = scales[acc_min(k + n, blocks - 1)];
+          scale[h] |= (k + n < blocks ? one : 0u) << (8 * n);
+        }
+#endif
+      }
+    };
+    const auto put_scales = [&](acc_u4 *lds) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) ((unsigned char *)lds)[scale_byte + h * scale_half + n * 64] = (unsigned char)(scale[h] >> (8 * n));
+    };
+#define OP_SCALES_F fsa, fsb, gsa, gsb,
+#define OP_SCALES_G gsa, gsb, fsa, fsb,
+#else
+#define OP_SCALES_F
+#define OP_SCALES_G
+    const auto ask_scales = [](int) {};
+    const auto put_scales = [](acc_u4 *) {};
+#endif
     const op_a::reader wa = op_a::reads(wi, lane);
     const op_b::reader wb = op_b::reads(wj, lane);
     const auto first = [&]() {
@@ -501,6 +531,12 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
       for (int j = 0; j < OP_FN; ++j) fb[j] = op_b::fragment(lds0 + OP_B_AT, wb, j, 0);
 #pragma unroll
       for (int i = 0; i < OP_FM; ++i) fa[i] = op_a::fragment(lds0, wa, i, 0);
+#if OP_TYPE == 3
+#pragma unroll
+      for (int j = 0; j < OP_SN; ++j) fsb[j] = op_b::scale(lds0 + OP_B_AT, wb, j, 0);
+#pragma unroll
+      for (int i = 0; i < OP_SM; ++i) fsa[i] = op_a::scale(lds0, wa, i, 0);
+#endif
     };
     /* a lane's chunks of a step, shared out over the half's fragments */
     constexpr int ALL = op_a::MINE + op_b::MINE, EACH = (ALL + OP_FM - 1) / OP_FM;
@@ -509,48 +545,57 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
       if (n < op_a::MINE) a.bring(lds, tid, wave, n, r);
       else if (n < ALL) b.bring(lds + OP_B_AT, tid, wave, n - op_a::MINE, r);
       if (n == ALL - 1) {
-        a.bring_rest(lds, tid, wave, r);
-        b.bring_rest(lds + OP_B_AT, tid, wave, r);
+        a.look(tid, wave, r + OP_STEP);
+        b.look(tid, wave, r + OP_STEP);
       }
     };
+    a.look(tid, wave, r0);
+    b.look(tid, wave, r0);
+    ask_scales(r0);
 #pragma unroll
     for (int n = 0; n < ALL; ++n) bring(lds0, n, r0);
+    put_scales(lds0);
+    ask_scales(r0 + OP_STEP);
 #pragma unroll
     for (int n = 0; n < ALL; ++n) bring(lds1, n, r0 + OP_STEP);
+    put_scales(lds1);
+    ask_scales(r0 + 2 * OP_STEP);
     op_meet(true);
     first();
     /* the step at r lies in `here`, the fragments of its first half in fa, fb */
     const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
-      op_half(c, fa, fb, ga, gb, here, wa, wb, 1, nothing);
+      op_half(c, fa, fb, ga, gb, OP_SCALES_F here, wa, wb, 1, nothing);
       op_meet(true);
-      op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, there, wa, wb, 0, [&](const int i) {
+      put_scales(here);
+      ask_scales(r + 3 * OP_STEP);
+      op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, OP_SCALES_G there, wa, wb, 0, [&](const int i) {
 #pragma unroll
         for (int n = 0; n < EACH; ++n) bring(here, i * EACH + n, r + 2 * OP_STEP);
       });
     };
 #else
     acc_u4 va[op_a::MINE], vb[op_b::MINE];
-    unsigned int sa[2], sb[2];
 #define OP_LOAD(r)                                                                          \
     do {                                                                                    \
-      const bool whole = a.whole(r) & b.whole(r);                                           \
-      if (whole) {                                                                          \
+      if (a.whole(r) & b.whole(r)) {                                                        \
         _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, true);  \
         _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, true);  \
       } else {                                                                              \
         _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, false); \
         _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, false); \
       }                                                                                     \
-      a.load_rest(sa, tid, r);                                                              \
-      b.load_rest(sb, tid, r);                                                              \
+      a.look(tid, wave, (r) + OP_STEP);                                                     \
+      b.look(tid, wave, (r) + OP_STEP);                                                     \
+      ask_scales(r);                                                                        \
     } while (0)
 #define OP_STORE(lds)                                                                       \
     do {                                                                                    \
       _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) lds[op_a::slot(tid, n)] = va[n];           \
       _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) lds[OP_B_AT + op_b::slot(tid, n)] = vb[n]; \
-      op_a::store_rest(lds, sa, tid);                                                       \
-      op_b::store_rest(lds + OP_B_AT, sb, tid);                                             \
+      put_scales(lds);                                                                      \
     } while (0)
+    a.look(tid, wave, r0);
+    b.look(tid, wave, r0);
     OP_LOAD(r0);
     OP_STORE(lds0);
     OP_LOAD(r0 + OP_STEP);
@@ -559,9 +604,9 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) product(const acc_produ
     const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
       OP_STORE(there);
       OP_LOAD(r + 2 * OP_STEP);
-      op_half(c, fa, fb, ga, gb, here, wa, wb, 1, nothing);
+      op_half(c, fa, fb, ga, gb, OP_SCALES_F here, wa, wb, 1, nothing);
       op_meet(false);
-      op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, there, wa, wb, 0, nothing);
+      op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, OP_SCALES_G there, wa, wb, 0, nothing);
     };
 #endif
     /* (an odd number of steps has one of zeros behind it: with a way out between the two, the sums would change registers) */
