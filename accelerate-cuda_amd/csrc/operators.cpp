@@ -34,6 +34,7 @@ struct OpSpec {
   int type = 0;                 // 0 float, 1 half, 2 bfloat16
   int choose = 0;
   bool normalise = true;
+  int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
 const char *const kKindName[] = {"product", "route", "combine", "micro"};
@@ -298,6 +299,13 @@ bool near_enough(const acc_strided &a, int rows_dim, int64_t row, int bytes, boo
   return (a.shape[rows_dim] <= 1 || stride >= row) && stride <= 0x7fffffff && reached * stride + row < 0x7fff0000;
 }
 
+// the knob's tile, where the form has it
+int tile_of(const OpSpec &sp, const ProductVariant &v, int tile)
+{
+  const bool there = sp.tile >= (v.outer ? 2 : 0) && sp.tile < kProductTileCount && (v.aligned || sp.tile < 3);
+  return there ? sp.tile : tile;
+}
+
 // the tile shape for products of `rows` rows of `experts` segments
 int rows_tile(int64_t rows, int64_t experts, int64_t n, bool aligned)
 {
@@ -342,7 +350,7 @@ std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_s
 constexpr uint32_t kMicroElements = 1024;            // (above the products' keys)
 std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & kMicroElements) ? micro_source(sp, key & 1u) : product_source_of(sp, key); }
 
-const char *const kProductNames[] = {"product"};
+const char *const kProductNames[] = {"product", "product_places"};
 const char *const kRouteNames[] = {"route", "route_place", "route_gradient"};
 const char *const kCombineNames[] = {"combine", "combine_gradient"};
 const char *const kMicroNames[] = {"micro_quantise", "micro_values"};
@@ -413,6 +421,7 @@ try {
   acc_op_s *op = new acc_op_s();
   op->ctx = ctx;
   op->spec = sp;
+  op->spec.tile = ctx->tuning_now()->get("product.tile", -1);
   *out = op;
   return ACC_OK;
 } ACC_OP_CATCH("acc_op_create")
@@ -482,7 +491,7 @@ try {
   v.b_fast = unit(*w, 2);
   v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
               near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
-  v.tile = rows_tile(rows, experts, n, v.aligned);
+  v.tile = tile_of(op->spec, v, rows_tile(rows, experts, n, v.aligned));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
@@ -543,9 +552,11 @@ try {
   v.index = !index ? 0 : turned ? 2 : 1;
   v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1) &&
               near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
-  v.tile = v.aligned && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2;
+  v.tile = tile_of(op->spec, v, v.aligned && rows < (1 << 28) && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2);
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
+  // (a tile of 256 x 256 has the rows that an index names looked up by a kernel in front: see OP_PLACES)
+  const bool places = v.index != 0 && v.aligned && kProductTiles[v.tile].bm == 256 && rows > 0;
+  ACC_TRY(op->variant(v.key(), kProductNames, v.index != 0 && v.aligned && kProductTiles[v.tile].bm == 256 ? 2 : 1, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
   a.a = device<const void>(p);
   a.b = device<const void>(q);
@@ -566,7 +577,16 @@ try {
   a.out_vectors = out_in_vectors(o, bytes);
   a.tiles_i = (int32_t)ceil_div(o.shape[1], t.bm);
   a.tiles_j = (int32_t)ceil_div(o.shape[2], t.bn);
-  return launch(op, who, var->fn, experts * a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+  acc::ScratchRef scratch;
+  int rc = ACC_OK;
+  if (places) {
+    ACC_TRY(op->ctx->scratch_acquire((size_t)rows * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+    a.places = static_cast<uint32_t *>(scratch.ptr);
+    rc = launch(op, who, var->fn2, ceil_div(rows, 256), 256, 0, stream, a);
+  }
+  if (rc == ACC_OK) rc = launch(op, who, var->fn, experts * a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+  if (places) op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));
+  return rc;
 } ACC_OP_CATCH("acc_exec_product_outer")
 
 // ---- router ---------------------------------------------------------------------------
@@ -841,7 +861,7 @@ try {
     v.aligned = v.aligned && t->ptr % 4 == 0;
     for (int d = 0; d + 1 < t->rank; ++d) v.aligned = v.aligned && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
   }
-  v.tile = rows_tile(rows, experts, n, v.aligned);
+  v.tile = tile_of(op->spec, v, rows_tile(rows, experts, n, v.aligned));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, micro_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];

@@ -66,6 +66,23 @@ ACC_DEV int op_count_tiles(const int *offsets, const int experts, const int rows
   return all;
 }
 
+/* The expert with the n-th longest segment, of up to 64 experts (of more: number n): what takes longest is begun first, and
+ * the workgroups that are left at the end have little to do. */
+ACC_DEV int op_nth_longest(const int *offsets, const int experts, const int rows, const int n)
+{
+  if (experts > 64) return n;
+  const int lane = acc_lane();
+  int b = 0, e = -1;
+  if (lane < experts) op_segment(offsets, experts, rows, lane + 1, &b, &e);
+  const int length = e - b;
+  int longer = 0;
+  for (int k = 0; k < experts; ++k) {
+    const int other = acc_readlane(length, k);
+    longer += (other > length) | ((other == length) & (k < lane));
+  }
+  return __builtin_ctzll(__ballot((longer == n) & (lane < experts)) | 1ull << 63);
+}
+
 struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segment; begin >= end: no such tile */
 
 /* The `tile`-th run of up to `height` rows, counted segment after segment: a wave adds up the runs of 64 segments at a

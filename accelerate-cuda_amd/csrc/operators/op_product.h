@@ -78,6 +78,20 @@ ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
   return acc_u4{(unsigned int)a, (unsigned int)(a >> 32), (unsigned int)b, (unsigned int)(b >> 32)};
 }
 
+/* which row an index of rows lo .. hi - 1 names for row m, divided as the arguments say; -1: none */
+ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi, const int limit, const unsigned int per_mul, const unsigned int per_shift)
+{
+  const int at = index[(unsigned int)acc_max(lo, acc_min(m, hi - 1))];
+  /* (by nothing: per_mul is 0) */
+  const int r = (int)(__umulhi((unsigned int)at, per_mul) >> per_shift) + (at & (per_mul ? 0 : -1));
+  return (m >= lo) & (m < hi) & ((unsigned int)at < 0x80000000u) & (r < limit) ? r : -1;
+}
+
+/* Where row r of an operand lies, in bytes, as a load takes it whose buffer ends before 2 GB: the top bit set, and none (r < 0)
+ * is 0 -- as a load of such a number beyond the end of a buffer of them is.  With that bit turned, it is an offset, and none
+ * is beyond the end of every buffer. */
+ACC_DEV unsigned int op_place_of(const int r, const int stride) { return r < 0 ? 0u : (unsigned int)(r * stride) | OP_NOWHERE; }
+
 /* One operand's share of a step in LDS, in chunks of 16 bytes.
  *   rows along r: TILE rows of 8 chunks; row i's chunk c lies at c ^ (i % 8): the eight lanes that are served together read
  *     neighbouring rows' chunks from all banks.
@@ -113,10 +127,6 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
   int limit;                     /* rows an index may name */
   int lo, hi;                    /* the rows that count: along r the i's, across it the r's */
   int extent;                    /* elements of a row that count, from `base` on */
-  /* Across r, with an index: which rows of memory the next step's are that is to be asked for, -1: none.  The aligned form has
-   * them in scalar registers, for all rows that a wave has in a chunk. */
-  static constexpr int ROWS = OP_ALIGNED && !FAST ? (PITCH < 64 ? 64 / PITCH : 1) : 1;
-  int rows[MINE][ROWS];
   int column;                    /* along r: the lane's chunks' first element (the same of all of them) */
   /* whether a lane's chunks lie equally far apart in memory: the rows between them are as many, and swizzled alike (for
    * Float32 across r they are not) */
@@ -145,38 +155,14 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
     return ((c / U ^ swizzle(i)) * U + c % U) * OP_EPC;
   }
 
-  ACC_DEV int divided(const int at) const { return per_mul ? (int)(__umulhi((unsigned int)at, per_mul) >> per_shift) : at; }
-
-  /* which row of memory row m of the segments is, if the index says `at`; -1: none */
-  ACC_DEV int number(const int m, const int at) const
+  /* which row of memory row m is, along r; -1: none */
+  ACC_DEV int number(const int m) const
   {
-    const bool listed = FAST ? LIST == OP_LISTED && index != 0 : LIST != OP_PLAIN;
-    const int r = listed ? divided(at) : m;
-    const bool there = (m >= lo) & (m < hi) & (!listed | ((at >= 0) & (r < limit)));
-    return there ? LIST == OP_GATED ? m : r : -1;
+    if (LIST == OP_PLAIN || !index) return m < hi ? m : -1;
+    return op_listed(index, m, lo, hi, limit, per_mul, per_shift);
   }
-  /* across r: the rows of the step at r */
-  ACC_DEV void look(const int tid, const int wave, const int r)
-  {
-    if (FAST || LIST == OP_PLAIN) return;
-#pragma unroll
-    for (int q = 0; q < MINE; ++q)
-#pragma unroll
-      for (int n = 0; n < ROWS; ++n) {
-#if OP_ALIGNED
-        const int m = r + major(wave * 64 + q * OP_THREADS) + n;
-        const int at = ((__attribute__((address_space(4))) const int *)(unsigned long long)index)[acc_max(lo, acc_min(m, hi - 1))];
-#else
-        const int m = r + major(slot(tid, q)), at = ask(m);
-#endif
-        rows[q][n] = number(m, at);
-      }
-  }
-  /* what the index says of row m (of the nearest row that counts, if that one does not) */
-  ACC_DEV int ask(const int m) const { return (FAST ? LIST == OP_LISTED && index != 0 : LIST != OP_PLAIN) ? index[acc_max(lo, acc_min(m, hi - 1))] : 0; }
 
-  /* along r: where the lane's rows are, from row `first` on; across r: where its columns are, and what the index says of the
-   * first step's rows */
+  /* along r: where the lane's rows are, from row `first` on; across r: where its columns are */
   ACC_DEV void start(const int tid, const int first)
   {
     column = FAST ? element(slot(tid, 0)) : 0;
@@ -195,7 +181,7 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
       if (EVEN && q > 0) continue;
       if (FAST) {
         /* (without an index, the rows that do not count lie behind the buffer's end) */
-        const int r = LIST == OP_PLAIN ? m : number(m, ask(m));
+        const int r = LIST == OP_PLAIN ? m : number(m);
         offset[q] = r < 0 ? OP_NOWHERE : (unsigned int)((LIST == OP_LISTED && index ? r : r - first) * (int)stride + element(s) * SIZE);
       } else {
         /* (columns beyond the result's: any will do) */
@@ -204,25 +190,15 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
 #else
       if (!FAST && EVEN && q > 0) continue;
       /* (a row that does not count: the operand's first; what comes of it is not written) */
-      offset[q] = FAST ? acc_max(number(m, ask(m)), 0) * stride + column * SIZE : element(s) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
+      offset[q] = FAST ? acc_max(number(m), 0) * stride + column * SIZE : element(s) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
 #endif
     }
   }
 
 #if OP_ALIGNED
-  /* f of the lane's row among those of its wave's q-th chunks (f is worked out once for the wave) */
-  template <typename F> ACC_DEV unsigned int of_row(const int q, const int tid, F f) const
-  {
-    unsigned int v = f(rows[q][0]);
-#pragma unroll
-    for (int n = 1; n < ROWS; ++n) {
-      const unsigned int w = f(rows[q][n]);
-      v = (tid & 63) / PITCH == n ? w : v;
-    }
-    return v;
-  }
-  /* ask for the lane's q-th chunk of the step at r, straight to LDS; `wave` is the same in all lanes, and known to be */
-  ACC_DEV void bring(acc_u4 *lds, const int tid, const int wave, const int q, const int r) const
+  /* ask for the lane's q-th chunk of the step at r, straight to LDS; `wave` is the same in all lanes, and known to be.
+   * `named`, across r with an index: where the chunk's row lies (see op_place_of) */
+  ACC_DEV void bring(acc_u4 *lds, const int wave, const int q, const int r, const int named) const
   {
     const op_lds_ptr to = (op_lds_ptr)(lds + (CHUNKS < OP_THREADS ? wave * 64 % CHUNKS : wave * 64 + q * OP_THREADS));
     const unsigned int at = offset[EVEN ? 0 : q];
@@ -232,31 +208,31 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, to, 16, from, r * SIZE + further, 0, 0);
     } else if (LIST == OP_LISTED) {
       const __amdgpu_buffer_rsrc_t all = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)OP_FARTHEST, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, to, 16, of_row(q, tid, [&](const int n) { return n < 0 ? OP_NOWHERE : (unsigned int)(n * (int)stride); }) + at, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(all, to, 16, ((unsigned int)named ^ OP_NOWHERE) + at, 0, 0, 0);
     } else {
       const __amdgpu_buffer_rsrc_t rest =
           __builtin_amdgcn_make_buffer_rsrc((void *)(base + r * stride), 0, (int)acc_min<long long>(OP_FARTHEST, acc_max(0, hi - r) * stride), 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rest, to, 16, LIST == OP_GATED ? of_row(q, tid, [](const int n) { return n < 0 ? OP_NOWHERE : 0u; }) | at : at, further, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rest, to, 16, LIST == OP_GATED ? (((unsigned int)named ^ OP_NOWHERE) & OP_NOWHERE) | at : at, further, 0, 0);
     }
   }
 #else
   /* the same by way of registers: `load` asks, whoever has asked puts what has come into LDS a step later.  `whole`: every
    * chunk of the step lies within its row (and across r, without an index, every row counts). */
   ACC_DEV bool whole(const int r) const { return FAST ? r + OP_STEP <= extent : ((LIST != OP_PLAIN) | (r + OP_STEP <= hi)) & (extent >= TILE); }
-  ACC_DEV void load(acc_u4 &v, const int tid, const int q, const int r, const bool whole) const
+  ACC_DEV void load(acc_u4 &v, const int tid, const int q, const int r, const int named, const bool whole) const
   {
     const int s = slot(tid, q);
     if (whole) {
       const unsigned char *p;
       if (FAST) p = base + (long long)r * SIZE + offset[q];
       else if (LIST == OP_PLAIN) p = base + (r + (EVEN ? q * APART : 0)) * stride + offset[EVEN ? 0 : q];
-      else p = base + acc_max(rows[q][0], 0) * stride + offset[EVEN ? 0 : q];
+      else p = base + acc_max(LIST == OP_GATED ? r + major(s) : named, 0) * stride + offset[EVEN ? 0 : q];
       v = ((const op_loose<op_mem> *)p)->v;
-      if (!FAST && LIST != OP_PLAIN && rows[q][0] < 0) v = acc_u4{0, 0, 0, 0};
+      if (!FAST && LIST != OP_PLAIN && named < 0) v = acc_u4{0, 0, 0, 0};
       return;
     }
     /* elements of the row that are wanted first, and how many there are */
-    const int n = FAST ? 0 : LIST == OP_PLAIN ? number(r + major(s), 0) : rows[q][0], c = FAST ? r + column : element(s);
+    const int m = r + major(s), n = FAST ? 0 : LIST == OP_PLAIN ? (m < hi ? m : -1) : LIST == OP_GATED && named >= 0 ? m : named, c = FAST ? r + column : element(s);
     const unsigned char *row = FAST ? base + offset[q] - column * SIZE : base + (long long)acc_max(n, 0) * stride;
     if (extent < OP_EPC) {
       op_mem e[OP_EPC];
@@ -385,6 +361,18 @@ ACC_DEV void op_meet(const bool loads)
   asm volatile("" ::: "memory");
 }
 
+#define OP_PLACES (OP_INDEX != 0 && OP_ALIGNED && OP_BM == 256)
+#if OP_PLACES
+extern "C" __global__ void __launch_bounds__(256) product_places(const acc_product_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  const int m = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (m >= p.rows) return;
+  const int r = op_listed(OP_INDEX == 1 ? p.index_b : p.index_a, m, 0, (int)p.rows, OP_INDEX == 1 ? p.b_rows : p.a_rows, p.per_mul, p.per_shift);
+  p.places[m] = op_place_of(r, (int)(OP_INDEX == 1 ? p.b_stride : p.a_stride) * (int)sizeof(op_mem));
+}
+#endif
+
 /* (at least two waves a SIMD: more than 256 registers would leave a compute unit to a workgroup of four waves) */
 extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_waves_per_eu(2))) product(const acc_product_args p)
 {
@@ -398,9 +386,10 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
   int expert, i0, j0, iend, jend, r0, r1;
 #if OP_OUTER
   {
-    const long long block = op_die_run(blockIdx.x, gridDim.x);
-    expert = (int)(block / ((long long)p.tiles_i * p.tiles_j));
-    const int t = (int)(block % ((long long)p.tiles_i * p.tiles_j));
+    /* (segments are of any length: the longest first, each on all dies) */
+    const int tiles = p.tiles_i * p.tiles_j;
+    expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, (int)(blockIdx.x / tiles));
+    const int t = (int)op_die_run(blockIdx.x % tiles, tiles);
     i0 = (t / p.tiles_j) * OP_BM;
     j0 = (t % p.tiles_j) * OP_BN;
     iend = p.ni;
@@ -436,10 +425,8 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
   a.per_mul = b.per_mul = p.per_mul;
   a.per_shift = b.per_shift = p.per_shift;
 #if OP_OUTER
-  b.index = p.index_b;
-  b.limit = p.b_rows;
-  if (OP_INDEX == 1) { a.index = p.index_b; a.limit = p.b_rows; }
-  if (OP_INDEX == 2) { b.index = p.index_a; b.limit = p.a_rows; }
+  b.index = (const int *)0;
+  b.limit = 0;
   a.lo = b.lo = r0;
   a.hi = b.hi = r1;
   a.base += (long long)i0 * op_a::SIZE;
@@ -477,6 +464,32 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
   if (r0 < r1) {
     op_frag fa[OP_FM], fb[OP_FN], ga[OP_FM], gb[OP_FN];
     const auto nothing = [](int) {};
+    /* outer, with an index: which rows of memory the rows of the lane's chunks are, of the step that is to be asked for next
+     * -- in the aligned form, where they lie.  (The tile is square: the same rows for both operands.)  With OP_PLACES another
+     * kernel has worked that out: the tile of 256 x 256 leaves no registers for it, and its spilled registers' loads would
+     * wait for the chunks' (8192^3: 825 TFLOP/s). */
+    int named[op_a::MINE > op_b::MINE ? op_a::MINE : op_b::MINE] = {};
+#if OP_PLACES
+    const __amdgpu_buffer_rsrc_t places = __builtin_amdgcn_make_buffer_rsrc((void *)p.places, 0, r1 * 4, 0x00020000);
+    const int mine_at = op_a::major(op_a::slot(tid, 0)) * 4;
+#endif
+    const auto look_at = [&](const int q, const int r) {
+#if OP_PLACES
+      if (q < op_a::MINE) named[q] = (int)__builtin_amdgcn_raw_buffer_load_b32(places, mine_at, (r + q * op_a::APART) * 4, 0);
+#elif OP_INDEX != 0
+      static_assert(OP_BM == OP_BN, "a row for both");
+      if (q < op_a::MINE) {
+        named[q] = op_listed(OP_INDEX == 1 ? p.index_b : p.index_a, r + op_a::major(op_a::slot(tid, q)), r0, r1, OP_INDEX == 1 ? p.b_rows : p.a_rows, p.per_mul, p.per_shift);
+#if OP_ALIGNED
+        named[q] = (int)op_place_of(named[q], (int)(OP_INDEX == 1 ? b.stride : a.stride));
+#endif
+      }
+#endif
+    };
+    const auto look = [&](const int r) {
+#pragma unroll
+      for (int q = 0; q < op_a::MINE; ++q) look_at(q, r);
+    };
 #if OP_TYPE == 3
     /* The scales go by way of registers, a lane a row of either operand: asked for two steps ahead of their use, put into LDS
      * one step ahead. */
@@ -485,7 +498,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     const int at = tid % (OP_BM + OP_BN), blocks = p.k / 16;
     const bool of_a = at < OP_BM;
     const int si = of_a ? at : at - OP_BM, share = of_a ? op_a::SHARE : op_b::SHARE;
-    const int scale_row = of_a ? a.number(i0 + si, a.ask(i0 + si)) : b.number(j0 + si, 0);
+    const int scale_row = of_a ? a.number(i0 + si) : b.number(j0 + si);
     /* (a row that there is not reads the matrix's first scales: what comes of it is not written) */
     const unsigned char *scales = of_a && scale_row >= 0 ? p.a_scales + scale_row * p.a_scales_stride
                                                          : p.b_scales + expert * p.b_scales_expert + acc_max(scale_row, 0) * p.b_scales_stride;
@@ -542,20 +555,16 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     constexpr int ALL = op_a::MINE + op_b::MINE, EACH = (ALL + OP_FM - 1) / OP_FM;
 #if OP_ALIGNED
     const auto bring = [&](acc_u4 *lds, const int n, const int r) {
-      if (n < op_a::MINE) a.bring(lds, tid, wave, n, r);
-      else if (n < ALL) b.bring(lds + OP_B_AT, tid, wave, n - op_a::MINE, r);
-      if (n == ALL - 1) {
-        a.look(tid, wave, r + OP_STEP);
-        b.look(tid, wave, r + OP_STEP);
-      }
+      if (n < op_a::MINE) a.bring(lds, wave, n, r, named[n]);
+      else if (n < ALL) b.bring(lds + OP_B_AT, wave, n - op_a::MINE, r, named[n - op_a::MINE]);
     };
-    a.look(tid, wave, r0);
-    b.look(tid, wave, r0);
+    look(r0);
     ask_scales(r0);
 #pragma unroll
     for (int n = 0; n < ALL; ++n) bring(lds0, n, r0);
     put_scales(lds0);
     ask_scales(r0 + OP_STEP);
+    look(r0 + OP_STEP);
 #pragma unroll
     for (int n = 0; n < ALL; ++n) bring(lds1, n, r0 + OP_STEP);
     put_scales(lds1);
@@ -564,7 +573,9 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     first();
     /* the step at r lies in `here`, the fragments of its first half in fa, fb */
     const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
-      op_half(c, fa, fb, ga, gb, OP_SCALES_F here, wa, wb, 1, nothing);
+      op_half(c, fa, fb, ga, gb, OP_SCALES_F here, wa, wb, 1, [&](const int i) {
+        look_at(i, r + 2 * OP_STEP);
+      });
       op_meet(true);
       put_scales(here);
       ask_scales(r + 3 * OP_STEP);
@@ -578,14 +589,13 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #define OP_LOAD(r)                                                                          \
     do {                                                                                    \
       if (a.whole(r) & b.whole(r)) {                                                        \
-        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, true);  \
-        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, true);  \
+        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, named[n], true);  \
+        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, named[n], true);  \
       } else {                                                                              \
-        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, false); \
-        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, false); \
+        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, named[n], false); \
+        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, named[n], false); \
       }                                                                                     \
-      a.look(tid, wave, (r) + OP_STEP);                                                     \
-      b.look(tid, wave, (r) + OP_STEP);                                                     \
+      look((r) + OP_STEP);                                                                  \
       ask_scales(r);                                                                        \
     } while (0)
 #define OP_STORE(lds)                                                                       \
@@ -594,8 +604,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
       _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) lds[OP_B_AT + op_b::slot(tid, n)] = vb[n]; \
       put_scales(lds);                                                                      \
     } while (0)
-    a.look(tid, wave, r0);
-    b.look(tid, wave, r0);
+    look(r0);
     OP_LOAD(r0);
     OP_STORE(lds0);
     OP_LOAD(r0 + OP_STEP);
@@ -629,7 +638,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #if OP_OUTER
     out += (long long)expert * p.out_expert;
 #else
-    none = p.index_a && a.number(ri, a.ask(ri)) < 0;
+    none = p.index_a && a.number(ri) < 0;
 #endif
 #pragma unroll
     for (int j = 0; j < OP_FN; ++j) {
