@@ -37,6 +37,8 @@ struct OpSpec {
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 const char *const kKindName[] = {"product", "route", "combine", "micro"};
 int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
@@ -66,19 +68,23 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
 
 // route: how a token's logits are shared out
 struct RouteVariant {
-  int lanes = 1, per = 8, vec = 1, block = 256;
-  uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (uint32_t)vec << 16 | (uint32_t)block << 20; }
+  int lanes = 1, per = 8, vec = 1, sels = 1;
+  bool tall = false;            // a lane a token
+  uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (uint32_t)vec << 16 | (uint32_t)sels << 24 | (tall ? 1u << 31 : 0u); }
 };
-constexpr int kRouteThreads = 256, kRouteBlock = 256, kRouteMaxExperts = 2048;
+constexpr int kRouteThreads = 1024, kRouteTallThreads = 256, kRouteMaxExperts = 2048;
 
-RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned)
+constexpr int64_t kRouteTallFrom = 16384;
+// The form with a lane a token is for tokens that fill the SIMDs with waves of 64, and up to eight choices.
+RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned, int64_t tokens)
 {
   RouteVariant v;
+  v.tall = tokens >= kRouteTallFrom && sp.choose <= 8;
   const int epc = 16 / type_bytes(sp.type);
   while (v.lanes < 64 && v.lanes * v.per < experts) v.lanes *= 2;
   while (v.lanes * v.per < experts) v.per *= 2;
   v.vec = aligned && experts % epc == 0 ? epc : 1;
-  v.block = kRouteBlock;
+  v.sels = (sp.choose + v.lanes - 1) / v.lanes;
   return v;
 }
 
@@ -86,11 +92,15 @@ std::string route_source(const OpSpec &sp, const RouteVariant &v)
 {
   char text[512];
   std::snprintf(text, sizeof(text),
-                "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_BLOCK %d\n#define OP_THREADS %d\n"
+                "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_SELS %d\n#define OP_THREADS %d\n#define OP_TALL %d\n#define OP_CHOOSE %d\n"
                 "#include \"acc_hip_device.h\"\n#include \"op_route.h\"\n",
-                sp.type, v.lanes, v.per, v.vec, v.block, kRouteThreads);
+                sp.type, v.lanes, v.per, v.vec, v.sels, kRouteThreads, v.tall ? 1 : 0, sp.choose);
   return text;
 }
+
+// Tokens of a workgroup: at most 256 workgroups, each of which adds up the counts of all; up to 256 tokens go to one, which
+// places its slots itself (a launch less).
+int route_block(int64_t tokens) { return (int)(tokens <= 256 ? 256 : std::max<int64_t>(64, ceil_div(tokens, 256))); }
 
 constexpr int kCombineSlots = 4;
 std::string combine_source(const OpSpec &sp, bool aligned)
@@ -132,8 +142,9 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         out.push_back(product_source(sp, v));
       }
   } else if (sp.kind == ACC_OP_ROUTE) {
-    for (int experts : {1, 8, 16, 32, 64, 128, 256, 512, 1024, 2048})
-      for (bool aligned : {true, false}) out.push_back(route_source(sp, route_variant(sp, experts, aligned)));
+    for (int experts : {1, 8, 16, 32, 64, 128, 256, 512, 1024, 2048}) if (experts >= sp.choose)
+      for (bool aligned : {true, false})
+        for (int64_t tokens : {int64_t(1), kRouteTallFrom}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (bool aligned : {true, false}) out.push_back(combine_source(sp, aligned));
   } else {
@@ -259,8 +270,6 @@ bool aligned_rows(const acc_strided &a, int bytes, int inner)
 
 template <typename T> T *device(const acc_strided *a) { return a ? reinterpret_cast<T *>(a->ptr) : nullptr; }
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // tiles of `height` rows that cover the segments, whatever their lengths: every segment with a row (and the rows before the
 // first and behind the last) may end amid a tile
 int64_t tiles_at_most(int64_t rows, int64_t experts, int64_t height)
@@ -342,8 +351,9 @@ std::string route_source_of(const OpSpec &sp, uint32_t key)
   RouteVariant v;
   v.lanes = (int)(key & 255u);
   v.per = (int)(key >> 8 & 255u);
-  v.vec = (int)(key >> 16 & 15u);
-  v.block = (int)(key >> 20);
+  v.vec = (int)(key >> 16 & 255u);
+  v.sels = (int)(key >> 24 & 127u);
+  v.tall = key >> 31;
   return route_source(sp, v);
 }
 std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_source(sp, key & 1u); }
@@ -621,7 +631,7 @@ try {
     ACC_TRY(check_apart(who, all[k], {{logits, bytes, "logits"}}));
     for (int m = 0; m < k; ++m) ACC_TRY(check_apart(who, all[k], {all[m]}));
   }
-  const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1));
+  const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1), tokens);
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kRouteNames, 3, route_source_of, &var));
   a.logits = device<const void>(logits);
@@ -635,13 +645,15 @@ try {
   a.experts = (int32_t)experts;
   a.choose = (int32_t)choose;
   a.normalise = op->spec.normalise ? 1 : 0;
-  a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, v.block));
+  a.block = route_block(tokens);
+  a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, a.block));
   acc::ScratchRef scratch;
   if (a.blocks > 1) {
     ACC_TRY(op->ctx->scratch_acquire((size_t)a.blocks * (size_t)experts * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
     a.counts = static_cast<uint32_t *>(scratch.ptr);
   }
-  int rc = launch(op, who, var->fn, a.blocks, kRouteThreads, route_lds(experts), stream, a);
+  int rc = v.tall ? launch(op, who, var->fn, a.blocks, kRouteTallThreads, (size_t)experts * 4, stream, a)
+                  : launch(op, who, var->fn, a.blocks, kRouteThreads, route_lds(experts), stream, a);
   if (rc == ACC_OK && a.blocks > 1) rc = launch(op, who, var->fn2, a.blocks, kRouteThreads, route_lds(experts), stream, a);
   if (a.blocks > 1) op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));
   return rc;
@@ -670,7 +682,7 @@ try {
   const int bytes = type_bytes(op->spec.type);
   ACC_TRY(check_apart(who, {dlogits, bytes, "dlogits"}, {{logits, bytes, "logits"}, {chosen, 4, "experts"}, {weights, 4, "weights"}, {dweights, 4, "dweights"}}));
   if (tokens == 0) return ACC_OK;
-  const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1) && aligned_rows(*dlogits, bytes, 1));
+  const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1) && aligned_rows(*dlogits, bytes, 1), 0);
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kRouteNames, 3, route_source_of, &var));
   a.logits = device<const void>(logits);

@@ -47,6 +47,7 @@ struct acc_route_args {
   int64_t tokens, logits_stride, dlogits_stride;
   int32_t experts, choose;
   int32_t normalise, blocks;
+  int32_t block, pad;           /* tokens of a workgroup */
   const uint32_t *guard;
 };
 

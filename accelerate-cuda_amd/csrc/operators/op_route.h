@@ -2,8 +2,11 @@
  * op_route.h -- the router of a layer of experts: the largest logits of every token, their weights, and the tokens' slots
  * sorted by expert, stably: a row-wise selection, a histogram, a scan and a permutation in one or two launches.
  *
- * A token has OP_LANES neighbouring lanes with OP_PER neighbouring logits each.  The lanes agree on the largest value left; of
- * equal ones the lowest lane has the lowest index.
+ * A token has OP_LANES neighbouring lanes with OP_PER logits each.  A logit is a key: its bits, made to compare as whole
+ * numbers do, above the index turned round, so that of equal ones the lowest index is the largest -- 32 bits for logits of
+ * 16, 64 for Float32; 0 is no logit.  A lane sorts its keys once; then the token's lanes agree on the largest of their first
+ * ones, `choose` times, and whoever had it moves up.  (65536 tokens of 128 bfloat16 logits, eight chosen: about 150 vector
+ * instructions for four tokens, 4 us of a bound of 5 by memory.)
  */
 #include "op_common.h"
 
@@ -11,57 +14,139 @@
 #define OP_WAVES (OP_THREADS / 64)
 #define OP_NONE (-__builtin_inff())
 
-/* the largest of a token's lanes, in all of them */
-ACC_DEV float op_group_max(float v)
-{
-#pragma unroll
-  for (int d = 1; d < OP_LANES; d *= 2) v = __builtin_fmaxf(v, __shfl_xor(v, d));
-  return v;
-}
-ACC_DEV float op_group_sum(float v)
-{
-#pragma unroll
-  for (int d = 1; d < OP_LANES; d *= 2) v += __shfl_xor(v, d);
-  return v;
-}
+#if OP_ELT == 0
+typedef unsigned long long op_key;
+typedef unsigned int op_bits_t;
+#define OP_SHIFT 32
+#else
+typedef unsigned int op_key;
+typedef unsigned short op_bits_t;
+#define OP_SHIFT 16
+#endif
+#define OP_SIGN ((op_bits_t)1 << (OP_SHIFT - 1))
 
-/* a lane's logits: what is not a number counts as minus infinity, as what lies behind the row's end does */
-ACC_DEV void op_logits(const acc_route_args &p, const long long t, const int sub, float (&v)[OP_PER])
+/* minus infinity and what is not a number: 0; minus zero counts as zero */
+ACC_DEV op_key op_key_of(const op_elt x, const int index)
 {
-  const op_elt *x = (const op_elt *)p.logits + t * p.logits_stride;
+  const float f = (float)x;
+  op_bits_t b;
+  __builtin_memcpy(&b, &x, sizeof(b));
+  b = f == 0.0f ? (op_bits_t)0 : b;
+  b = b & OP_SIGN ? (op_bits_t)~b : (op_bits_t)(b | OP_SIGN);
+  return f > OP_NONE ? (op_key)b << OP_SHIFT | (op_key)(0xffffu - (unsigned int)index) : (op_key)0;
+}
+ACC_DEV float op_value_of(const op_key k)
+{
+  op_bits_t b = (op_bits_t)(k >> OP_SHIFT);
+  b = b & OP_SIGN ? (op_bits_t)(b ^ OP_SIGN) : (op_bits_t)~b;
+  op_elt x;
+  __builtin_memcpy(&x, &b, sizeof(x));
+  return k ? (float)x : OP_NONE;
+}
+ACC_DEV int op_index_of(const op_key k) { return k ? (int)(0xffffu - ((unsigned int)k & 0xffffu)) : -1; }
+
+/* f over a token's lanes, in all of them (f in any order): within 16 lanes by neighbours, pairs, mirrored halves; beyond by
+ * exchanges of rows */
+template <typename T, typename F> ACC_DEV T op_group(T v, F f)
+{
+  if (OP_LANES > 1) v = f(v, acc_dpp<0xB1, 0xf>(v, v));
+  if (OP_LANES > 2) v = f(v, acc_dpp<0x4E, 0xf>(v, v));
+  if (OP_LANES > 4) v = f(v, acc_dpp<0x141, 0xf>(v, v));
+  if (OP_LANES > 8) v = f(v, acc_dpp<0x140, 0xf>(v, v));
+  if (OP_LANES > 16) {
+    unsigned int w[sizeof(T) / 4], a[sizeof(T) / 4], b[sizeof(T) / 4];
+    T x, y;
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(T) / 4); ++k) {
+      const auto r = __builtin_amdgcn_permlane16_swap(w[k], w[k], false, false);
+      a[k] = r[0];
+      b[k] = r[1];
+    }
+    __builtin_memcpy(&x, a, sizeof(T));
+    __builtin_memcpy(&y, b, sizeof(T));
+    v = f(x, y);
+  }
+  if (OP_LANES > 32) {
+    unsigned int w[sizeof(T) / 4], a[sizeof(T) / 4], b[sizeof(T) / 4];
+    T x, y;
+    __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(T) / 4); ++k) {
+      const auto r = __builtin_amdgcn_permlane32_swap(w[k], w[k], false, false);
+      a[k] = r[0];
+      b[k] = r[1];
+    }
+    __builtin_memcpy(&x, a, sizeof(T));
+    __builtin_memcpy(&y, b, sizeof(T));
+    v = f(x, y);
+  }
+  return v;
+}
+ACC_DEV float op_group_max(const float v) { return op_group(v, [](float x, float y) { return __builtin_fmaxf(x, y); }); }
+ACC_DEV float op_group_sum(const float v) { return op_group(v, [](float x, float y) { return x + y; }); }
+
+/* a lane's logits as they lie in memory; beyond the row's end (or for no token) minus infinity */
+ACC_DEV void op_logits(const acc_route_args &p, const long long t, const bool here, const int sub, op_elt (&v)[OP_PER])
+{
+  const op_elt *x = (const op_elt *)p.logits + (here ? t : 0) * p.logits_stride;
 #pragma unroll
   for (int c = 0; c < OP_PER; c += OP_VEC) {
     const int e = sub * OP_PER + c;
-    op_elt w[OP_VEC];
+    const bool some = here && e < p.experts;
     if (OP_VEC > 1) {
       /* (rows of a multiple of OP_VEC elements, aligned to as many) */
       typedef op_elt vec __attribute__((ext_vector_type(OP_VEC)));
-      if (t < p.tokens && e < p.experts) {
-        const vec u = *(const vec *)(x + e);
-        __builtin_memcpy(w, &u, sizeof(w));
-      }
-    } else if (t < p.tokens && e < p.experts) {
-      w[0] = x[e];
-    }
+      vec u;
 #pragma unroll
-    for (int k = 0; k < OP_VEC; ++k) {
-      const float f = t < p.tokens && e + k < p.experts ? (float)w[k] : OP_NONE;
-      v[c + k] = f > OP_NONE ? f : OP_NONE;
+      for (int k = 0; k < OP_VEC; ++k) u[k] = (op_elt)OP_NONE;
+      if (some) u = *(const vec *)(x + e);
+#pragma unroll
+      for (int k = 0; k < OP_VEC; ++k) v[c + k] = u[k];
+    } else {
+      v[c] = some ? x[e] : (op_elt)OP_NONE;
     }
   }
 }
 
-/* exp(x - most), where an infinite `most` leaves the values that reach it */
-ACC_DEV float op_power(const float x, const float most) { return x == OP_NONE ? 0.0f : x == most ? 1.0f : __expf(x - most); }
-
-/* place of every slot of a workgroup's tokens: `start[w * experts + e]` is the place of the first slot that wave w has of
- * expert e; a wave takes its slots 64 at a time, in order.  Lanes of the same expert find one another bit by bit. */
-ACC_DEV void op_place(const acc_route_args &p, const long long first, const long long last, int *start, const int bits, const int wave, const int lane)
+/* exp(x - most) for an x up to `most`, by the power of two; an infinite `most` leaves the values that reach it.  (Without a
+ * branch; where `most` is minus infinity there is nothing to choose, and no use for what comes of it.) */
+ACC_DEV float op_power(const float x, const float most)
 {
-  const long long slots = last - first, share = (slots + OP_WAVES * 64 - 1) / (OP_WAVES * 64) * 64;
-  for (long long s = first + wave * share; s < acc_min(last, first + (wave + 1) * share); s += 64) {
+  const float d = x == most ? 0.0f : x - most;
+  return __builtin_amdgcn_exp2f(d * 1.44269504f);
+}
+
+/* largest first: bitonic over a power of two of keys, every comparison known */
+ACC_DEV void op_sort(op_key (&k)[OP_PER])
+{
+#pragma unroll
+  for (int size = 2; size <= OP_PER; size *= 2)
+#pragma unroll
+    for (int step = size / 2; step > 0; step /= 2)
+#pragma unroll
+      for (int i = 0; i < OP_PER; ++i) {
+        const int j = i ^ step;
+        if (j > i) {
+          const op_key x = k[i], y = k[j];
+          const bool down = (i & size) == 0;
+          const op_key most = x > y ? x : y, least = x > y ? y : x;
+          k[i] = down ? most : least;
+          k[j] = down ? least : most;
+        }
+      }
+}
+
+/* the slots first .. last - 1 of a workgroup that wave w takes: whole tokens, in order */
+ACC_DEV long long op_share(const acc_route_args &p) { return (long long)((p.block + OP_WAVES * OP_TOKENS - 1) / (OP_WAVES * OP_TOKENS)) * OP_TOKENS; }
+
+/* Place of every slot from first on, below last, of one wave: `start[e]` is the place of its first slot of expert e.  64 at a
+ * time, in order; lanes of the same expert find one another bit by bit. */
+ACC_DEV void op_place(const acc_route_args &p, const long long first, const long long last, int *start, const int bits, const int lane)
+{
+  for (long long s = first; s < last; s += 64) {
     const long long mine = s + lane;
-    const int e = mine < acc_min(last, first + (wave + 1) * share) ? p.chosen[mine] : -1;
+    const int e = mine < last ? p.chosen[mine] : -1;
     unsigned long long same = __ballot(e >= 0);
     for (int b = 0; b < bits; ++b) {
       const unsigned long long has = __ballot((e >> b) & 1);
@@ -69,30 +154,17 @@ ACC_DEV void op_place(const acc_route_args &p, const long long first, const long
     }
     if (e >= 0) {
       const int before = __popcll(same & ((1ull << lane) - 1));
-      const int at = start[wave * p.experts + e] + before;
-      if (before == 0) start[wave * p.experts + e] = at + __popcll(same);
+      const int at = start[e] + before;
+      if (before == 0) start[e] = at + __popcll(same);
       p.order[at] = (int)mine;
       p.place[mine] = at;
-    } else if (mine < last && mine < first + (wave + 1) * share) {
+    } else if (mine < last) {
       p.place[mine] = -1;
     }
   }
 }
 
-/* how many slots each wave has of each expert, of the workgroup's slots first .. last-1 */
-ACC_DEV void op_count(const acc_route_args &p, const long long first, const long long last, int *counts, const int tid)
-{
-  for (int i = tid; i < OP_WAVES * p.experts; i += OP_THREADS) counts[i] = 0;
-  __syncthreads();
-  const long long slots = last - first, share = (slots + OP_WAVES * 64 - 1) / (OP_WAVES * 64) * 64;
-  for (long long s = first + tid; s < last; s += OP_THREADS) {
-    const int e = p.chosen[s];
-    if (e >= 0) atomicAdd(&counts[(int)((s - first) / share) * p.experts + e], 1);
-  }
-  __syncthreads();
-}
-
-ACC_DEV int op_bits(const int experts) { return experts > 1 ? 32 - __builtin_clz(experts - 1) : 0; }
+ACC_DEV int op_index_bits(const int experts) { return experts > 1 ? 32 - __builtin_clz(experts - 1) : 0; }
 
 /* counts[w][e] -> the place of wave w's first slot of expert e, where the workgroup's first one is at base[e] */
 ACC_DEV void op_starts(const acc_route_args &p, int *counts, const int *base, const int tid)
@@ -108,7 +180,7 @@ ACC_DEV void op_starts(const acc_route_args &p, int *counts, const int *base, co
   __syncthreads();
 }
 
-/* base[e] += the sum of total[0 .. e-1], by the first wave; the offsets go out if asked for; returns nothing but the sum of all */
+/* base[e] += the sum of total[0 .. e-1], by the first wave; *all is the sum of all; the offsets go out if asked for */
 ACC_DEV void op_bases(const acc_route_args &p, int *base, const int *total, const bool write, const int tid, int *all)
 {
   if (tid < 64) {
@@ -130,71 +202,181 @@ ACC_DEV void op_bases(const acc_route_args &p, int *base, const int *total, cons
   __syncthreads();
 }
 
-/* workgroup b has the tokens b * OP_BLOCK .. ; with one workgroup the slots are placed at once, otherwise the counts go out */
+#if OP_TALL
+/* The selection for many tokens: a lane has a token and OP_CHOOSE keys in order, and puts every logit of its row where it
+ * belongs among them: the new j-th key is the middle one of the j-th, the one in front of it and the logit's, an
+ * instruction for keys of 32 bits.  That is 15 instructions a logit for 64 tokens at once -- a third of what the lanes of a
+ * token need to agree on as many -- but a wave's time is the same for one token as for 64: it takes over where the tokens
+ * fill the SIMDs.  Rows come by way of LDS, 128 bytes of 64 rows at a time, so that lines are read whole; a row's share lies
+ * 144 bytes from the next one's, which spreads the lanes' reads over the banks. */
+#define OP_COLUMNS (128 / (int)sizeof(op_elt))
+#define OP_APART 144
+typedef op_elt op_vec __attribute__((ext_vector_type(OP_VALUES)));
+
+ACC_DEV op_key op_middle(const op_key a, const op_key b, const op_key c)
+{
+  /* (spelt in full, as the compiler knows the instruction) */
+  const op_key low = a < b ? a : b, high = a < b ? b : a, most = high < c ? high : c;
+  return low > most ? low : most;
+}
+
+extern "C" __global__ void __launch_bounds__(256) route(const acc_route_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  extern __shared__ int shared[];
+  __shared__ __align__(16) unsigned char tiles[4][64 * OP_APART];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const long long first = (long long)blockIdx.x * p.block, last = acc_min<long long>(p.tokens, first + p.block);
+  unsigned char *tile = tiles[wave];
+  for (int e = tid; e < p.experts; e += 256) shared[e] = 0;
+  __syncthreads();
+  for (long long at = first + wave * 64; at < last; at += 256) {
+    const int rows = (int)acc_min<long long>(64, last - at);
+    const op_elt *x = (const op_elt *)p.logits + at * p.logits_stride;
+    op_key k[OP_CHOOSE];
+    float total = 0.0f, most = OP_NONE;
+#pragma unroll
+    for (int j = 0; j < OP_CHOOSE; ++j) k[j] = 0;
+    op_vec next[8];
+    const auto ask = [&](const int c0) {           /* (rows that there are not: the last one; columns: minus infinity) */
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = acc_min(i * 8 + lane / 8, rows - 1), c = c0 + lane % 8 * OP_VALUES;
+#pragma unroll
+        for (int n = 0; n < OP_VALUES; ++n) next[i][n] = (op_elt)OP_NONE;
+        if (c < p.experts) next[i] = *(const op_vec *)(x + r * p.logits_stride + c);
+      }
+    };
+    if (OP_VEC > 1) ask(0);
+    for (int c0 = 0; c0 < p.experts; c0 += OP_COLUMNS) {
+      if (OP_VEC > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *(op_vec *)(tile + (i * 8 + lane / 8) * OP_APART + lane % 8 * 16) = next[i];
+        if (c0 + OP_COLUMNS < p.experts) ask(c0 + OP_COLUMNS);
+      } else {
+        const int c = c0 + lane % OP_COLUMNS;
+#pragma unroll 8
+        for (int r = lane / OP_COLUMNS; r < 64; r += 64 / OP_COLUMNS)
+          ((op_elt *)(tile + r * OP_APART))[lane % OP_COLUMNS] = c < p.experts ? x[acc_min(r, rows - 1) * p.logits_stride + c] : (op_elt)OP_NONE;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      for (int i = 0; i < 8; ++i) {
+        const op_vec v = *(const op_vec *)(tile + lane * OP_APART + i * 16);
+#pragma unroll
+        for (int n = 0; n < OP_VALUES; ++n) {
+          const op_key y = op_key_of(v[n], c0 + i * OP_VALUES + n);
+#pragma unroll
+          for (int j = OP_CHOOSE - 1; j > 0; --j) k[j] = op_middle(k[j - 1], k[j], y);
+          k[0] = k[0] > y ? k[0] : y;
+        }
+      }
+      if (!p.normalise) {
+        const float now = op_value_of(k[0]);
+        total *= op_power(most, now);
+        most = now;
+        for (int i = 0; i < 8; ++i) {
+          const op_vec v = *(const op_vec *)(tile + lane * OP_APART + i * 16);
+#pragma unroll
+          for (int n = 0; n < OP_VALUES; ++n) {
+            const float f = (float)v[n];
+            total += op_power(f > OP_NONE ? f : OP_NONE, most);
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (lane >= rows) continue;
+    most = op_value_of(k[0]);
+    float power[OP_CHOOSE];
+#pragma unroll
+    for (int j = 0; j < OP_CHOOSE; ++j) {
+      power[j] = op_power(op_value_of(k[j]), most);
+      if (p.normalise) total += power[j];
+    }
+#pragma unroll
+    for (int j = 0; j < OP_CHOOSE; ++j) {
+      const int e = op_index_of(k[j]);
+      p.chosen[(at + lane) * OP_CHOOSE + j] = e;
+      p.weights[(at + lane) * OP_CHOOSE + j] = e < 0 ? 0.0f : power[j] / total;
+      if (e >= 0) atomicAdd(&shared[e], 1);
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < p.experts; e += 256) p.counts[(long long)blockIdx.x * p.experts + e] = shared[e];
+}
+#else
+/* workgroup b has the tokens b * block .. ; with one workgroup the slots are placed at once, otherwise the counts go out */
 extern "C" __global__ void __launch_bounds__(OP_THREADS) route(const acc_route_args p)
 {
   if (p.guard && *p.guard == 0u) return;
   extern __shared__ int shared[];                  /* OP_WAVES * experts counts, experts bases, experts totals */
   __shared__ int all;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int sub = lane % OP_LANES;
-  const long long first = (long long)blockIdx.x * OP_BLOCK, last = acc_min<long long>(p.tokens, first + OP_BLOCK);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = lane % OP_LANES;
+  const long long first = (long long)blockIdx.x * p.block, last = acc_min<long long>(p.tokens, first + p.block), share = op_share(p);
+  const long long mine = first + wave * share, end = acc_min(last, mine + share);
+  int *counts = shared, *base = shared + OP_WAVES * p.experts, *sums = base + p.experts;
+  for (int i = tid; i < OP_WAVES * p.experts; i += OP_THREADS) counts[i] = 0;
+  __syncthreads();
 
-  for (long long base = first + wave * OP_TOKENS; base < last; base += OP_WAVES * OP_TOKENS) {
-    const long long t = base + lane / OP_LANES;
-    float v[OP_PER];
-    op_logits(p, t, sub, v);
+  op_elt next[OP_PER];
+  op_logits(p, mine + lane / OP_LANES, mine + lane / OP_LANES < end, sub, next);
+  for (long long at = mine; at < end; at += OP_TOKENS) {
+    const long long t = at + lane / OP_LANES;
+    const bool here = t < end;
+    op_elt x[OP_PER];
+    op_key k[OP_PER];
+#pragma unroll
+    for (int i = 0; i < OP_PER; ++i) x[i] = next[i];
+    op_logits(p, t + OP_TOKENS, t + OP_TOKENS < end, sub, next);     /* (on its way while these are sorted) */
+#pragma unroll
+    for (int i = 0; i < OP_PER; ++i) k[i] = op_key_of(x[i], sub * OP_PER + i);
+    op_sort(k);
+    /* the j-th choice stays with lane j of the token, OP_SELS of them a lane */
+    op_key chosen[OP_SELS];
     float total = 0.0f, most = OP_NONE;
-    if (!p.normalise) {
-      float m = OP_NONE;
 #pragma unroll
-      for (int k = 0; k < OP_PER; ++k) m = __builtin_fmaxf(m, v[k]);
-      most = op_group_max(m);
+    for (int s = 0; s < OP_SELS; ++s) {
+      chosen[s] = 0;
+      const int n = acc_min(OP_LANES, p.choose - s * OP_LANES);
+      for (int j = 0; j < n; ++j) {
+        const op_key best = op_group(k[0], [](op_key a, op_key b) { return a > b ? a : b; });
+        const bool owner = k[0] == best;           /* (no two keys are the same, but for 0) */
+        chosen[s] = sub == j ? best : chosen[s];
 #pragma unroll
-      for (int k = 0; k < OP_PER; ++k) total += op_power(v[k], most);
-      total = op_group_sum(total);
+        for (int i = 0; i + 1 < OP_PER; ++i) k[i] = owner ? k[i + 1] : k[i];
+        k[OP_PER - 1] = owner ? (op_key)0 : k[OP_PER - 1];
+      }
+      if (s == 0) most = op_value_of(op_group(chosen[0], [](op_key a, op_key b) { return a > b ? a : b; }));
     }
-    for (int j = 0; j < p.choose; ++j) {
-      float m = OP_NONE;
+    float power[OP_SELS];
 #pragma unroll
-      for (int k = 0; k < OP_PER; ++k) m = __builtin_fmaxf(m, v[k]);
-      const float best = op_group_max(m);
-      if (j == 0) most = best;
-      /* the lowest lane of the token that has it, and there the lowest index */
-      unsigned long long have = __ballot(m == best && best > OP_NONE);
-      if (OP_LANES < 64) have &= ((1ull << OP_LANES) - 1) << (lane / OP_LANES * OP_LANES);
-      const bool owner = have != 0 && __builtin_ctzll(have) == lane;
-      int at = -1;
-      bool taken = !owner;
+    for (int s = 0; s < OP_SELS; ++s) {
+      power[s] = op_power(op_value_of(chosen[s]), most);
+      if (p.normalise) total += power[s];
+    }
+    if (!p.normalise)
 #pragma unroll
-      for (int k = 0; k < OP_PER; ++k) {
-        const bool it = !taken && v[k] == best;
-        if (it) {
-          at = sub * OP_PER + k;
-          v[k] = OP_NONE;
-          taken = true;
-        }
+      for (int i = 0; i < OP_PER; ++i) {
+        const float f = (float)x[i];
+        total += op_power(f > OP_NONE ? f : OP_NONE, most);
       }
-      const float power = op_power(best, most);
-      if (p.normalise) total += power;
-      if (t < last && (owner || (have == 0 && sub == 0))) {
-        p.chosen[t * p.choose + j] = at;
-        p.weights[t * p.choose + j] = power;
+    total = op_group_sum(total);
+#pragma unroll
+    for (int s = 0; s < OP_SELS; ++s) {
+      const int j = s * OP_LANES + sub;
+      if (here && j < p.choose) {
+        const int e = op_index_of(chosen[s]);
+        p.chosen[t * p.choose + j] = e;
+        p.weights[t * p.choose + j] = e < 0 ? 0.0f : power[s] / total;
+        if (e >= 0) atomicAdd(&counts[wave * p.experts + e], 1);
       }
     }
-    /* the powers become weights: the lanes that wrote them have made them visible to their wave */
-    __threadfence_block();
-    if (t < last)
-      for (int j = sub; j < p.choose; j += OP_LANES) {
-        const float w = p.weights[t * p.choose + j];
-        p.weights[t * p.choose + j] = w > 0.0f ? w / total : 0.0f;
-      }
   }
   __threadfence_block();
   __syncthreads();
 
-  int *counts = shared, *base = shared + OP_WAVES * p.experts, *sums = base + p.experts;
-  op_count(p, first * p.choose, last * p.choose, counts, tid);
   for (int e = tid; e < p.experts; e += OP_THREADS) {
     int n = 0;
     for (int w = 0; w < OP_WAVES; ++w) n += counts[w * p.experts + e];
@@ -206,37 +388,51 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route(const acc_route_a
   __syncthreads();
   op_bases(p, base, sums, true, tid, &all);
   op_starts(p, counts, base, tid);
-  op_place(p, 0, p.tokens * p.choose, counts, op_bits(p.experts), wave, lane);
+  op_place(p, mine * p.choose, end * p.choose, counts + wave * p.experts, op_index_bits(p.experts), lane);
   for (long long s = all + tid; s < p.tokens * p.choose; s += OP_THREADS) p.order[s] = -1;
 }
 
-/* behind it, where there are several workgroups: everybody adds up the counts, those before it and all */
+#endif
+
+/* behind it, where there are several workgroups (256 at most): everybody adds up the counts, those before it and all */
 extern "C" __global__ void __launch_bounds__(OP_THREADS) route_place(const acc_route_args p)
 {
   if (p.guard && *p.guard == 0u) return;
   extern __shared__ int shared[];
   __shared__ int all;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long long first = (long long)blockIdx.x * OP_BLOCK, last = acc_min<long long>(p.tokens, first + OP_BLOCK);
+  const long long first = (long long)blockIdx.x * p.block, last = acc_min<long long>(p.tokens, first + p.block), share = op_share(p);
+  const long long mine = (first + wave * share) * p.choose, end = acc_min(last, first + (wave + 1) * share) * p.choose;
   int *counts = shared, *base = shared + OP_WAVES * p.experts, *sums = base + p.experts;
-  for (int e = tid; e < p.experts; e += OP_THREADS) {
+  for (int i = tid; i < (OP_WAVES + 2) * p.experts; i += OP_THREADS) counts[i] = 0;
+  __syncthreads();
+  /* the wave's own slots, once more */
+  for (long long s = mine + lane; s < end; s += 64) {
+    const int e = p.chosen[s];
+    if (e >= 0) atomicAdd(&counts[wave * p.experts + e], 1);
+  }
+  /* wave w adds up every OP_WAVES-th workgroup's counts, eight at a time on their way */
+  for (int e = lane; e < p.experts; e += 64) {
     int before = 0, total = 0;
-    for (int b = 0; b < p.blocks; ++b) {
-      const int n = (int)p.counts[(long long)b * p.experts + e];
-      total += n;
-      before += b < (int)blockIdx.x ? n : 0;
+    for (int b = wave; b < p.blocks; b += 8 * OP_WAVES) {
+      int n[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) n[k] = b + k * OP_WAVES < p.blocks ? (int)p.counts[(long long)(b + k * OP_WAVES) * p.experts + e] : 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        total += n[k];
+        before += b + k * OP_WAVES < (int)blockIdx.x ? n[k] : 0;
+      }
     }
-    base[e] = before;
-    sums[e] = total;
+    atomicAdd(&base[e], before);
+    atomicAdd(&sums[e], total);
   }
   __syncthreads();
   op_bases(p, base, sums, blockIdx.x == 0, tid, &all);
-  op_count(p, first * p.choose, last * p.choose, counts, tid);
   op_starts(p, counts, base, tid);
-  op_place(p, first * p.choose, last * p.choose, counts, op_bits(p.experts), wave, lane);
+  op_place(p, mine, end, counts + wave * p.experts, op_index_bits(p.experts), lane);
   /* what lies behind the last expert's slots, each workgroup its part */
-  const long long slots = p.tokens * p.choose, mine = first * p.choose, end = last * p.choose;
-  for (long long s = acc_max<long long>(all, mine) + tid; s < acc_min(end, slots); s += OP_THREADS) p.order[s] = -1;
+  for (long long s = acc_max<long long>(all, first * p.choose) + tid; s < last * p.choose; s += OP_THREADS) p.order[s] = -1;
 }
 
 /* d logit_i = w_i (dw_i - sum_j w_j dw_j) of the chosen ones; where the weights are not normalised over them, of all:
@@ -249,10 +445,15 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route_gradient(const ac
   const bool here = t < p.tokens;
   float v[OP_PER], d[OP_PER], inner = 0.0f;
   if (!p.normalise) {
-    op_logits(p, t, sub, v);
+    op_elt x[OP_PER];
+    op_logits(p, t, here, sub, x);
     float m = OP_NONE, total = 0.0f;
 #pragma unroll
-    for (int k = 0; k < OP_PER; ++k) m = __builtin_fmaxf(m, v[k]);
+    for (int k = 0; k < OP_PER; ++k) {
+      const float f = (float)x[k];
+      v[k] = f > OP_NONE ? f : OP_NONE;
+      m = __builtin_fmaxf(m, v[k]);
+    }
     m = op_group_max(m);
 #pragma unroll
     for (int k = 0; k < OP_PER; ++k) total += v[k] = op_power(v[k], m);
@@ -279,16 +480,14 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route_gradient(const ac
   for (int c = 0; c < OP_PER; c += OP_VEC) {
     const int e = sub * OP_PER + c;
     if (e >= p.experts) break;
-    typedef op_elt vec __attribute__((ext_vector_type(OP_VEC)));
-    op_elt w[OP_VEC];
-#pragma unroll
-    for (int k = 0; k < OP_VEC; ++k) w[k] = (op_elt)d[c + k];
     if (OP_VEC > 1) {
+      typedef op_elt vec __attribute__((ext_vector_type(OP_VEC)));
       vec u;
-      __builtin_memcpy(&u, w, sizeof(w));
+#pragma unroll
+      for (int k = 0; k < OP_VEC; ++k) u[k] = (op_elt)d[c + k];
       *(vec *)(out + e) = u;
     } else {
-      out[e] = w[0];
+      out[e] = (op_elt)d[c];
     }
   }
 }
