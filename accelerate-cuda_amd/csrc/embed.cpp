@@ -33,7 +33,9 @@ ACC_EMBED(stencil_flat, "device/skel_stencil_flat.h")
 ACC_EMBED(stencil_pair, "device/skel_stencil_pair.h")
 ACC_EMBED(op_args, "operators/op_args.h")
 ACC_EMBED(op_common, "operators/op_common.h")
+ACC_EMBED(op_matrix, "operators/op_matrix.h")
 ACC_EMBED(op_product, "operators/op_product.h")
+ACC_EMBED(op_skinny, "operators/op_skinny.h")
 ACC_EMBED(op_route, "operators/op_route.h")
 ACC_EMBED(op_combine, "operators/op_combine.h")
 ACC_EMBED(op_micro, "operators/op_micro.h")
@@ -59,6 +61,8 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"skel_stencil_pair.h", acc_embed_stencil_pair_begin, acc_embed_stencil_pair_end},
       {"op_args.h", acc_embed_op_args_begin, acc_embed_op_args_end},
       {"op_common.h", acc_embed_op_common_begin, acc_embed_op_common_end},
+      {"op_matrix.h", acc_embed_op_matrix_begin, acc_embed_op_matrix_end},
+      {"op_skinny.h", acc_embed_op_skinny_begin, acc_embed_op_skinny_end},
       {"op_product.h", acc_embed_op_product_begin, acc_embed_op_product_end},
       {"op_route.h", acc_embed_op_route_begin, acc_embed_op_route_end},
       {"op_combine.h", acc_embed_op_combine_begin, acc_embed_op_combine_end},

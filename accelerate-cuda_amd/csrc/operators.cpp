@@ -34,6 +34,7 @@ struct OpSpec {
   int type = 0;                 // 0 float, 1 half, 2 bfloat16
   int choose = 0;
   bool normalise = true;
+  int ahead = 4, once = 0;      // knobs product.ahead and product.once of the form for a few rows
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
@@ -46,8 +47,8 @@ int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 // product: tile shapes, in waves of 64 lanes
 struct ProductTile { int bm, bn, wm, wn; };
-const ProductTile kProductTiles[] = {{16, 128, 1, 4}, {64, 128, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}};
-constexpr int kProductTileCount = 4;
+const ProductTile kProductTiles[] = {{32, 64, 2, 2}, {64, 128, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}, {16, 32, 1, 4}, {16, 64, 1, 4}};
+constexpr int kProductTileCount = 6, kLow = 0, kSkinny = 4;      // the last two: op_skinny.h
 struct ProductVariant {
   int tile = 0;
   bool outer = false, b_fast = true, aligned = true;
@@ -59,6 +60,14 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
 {
   const ProductTile &t = kProductTiles[v.tile];
   char text[512];
+  if (v.tile >= kSkinny) {
+    // (the matrices' loads are marked as read once where they are: nontemporal.  Steps ahead: as many as 128 registers hold)
+    std::snprintf(text, sizeof(text),
+                  "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_AHEAD %d\n#define OP_ONCE %d\n"
+                  "#include \"acc_hip_device.h\"\n#include \"op_skinny.h\"\n",
+                  sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn / 16, sp.ahead, sp.once);
+    return text;
+  }
   std::snprintf(text, sizeof(text),
                 "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_BN %d\n#define OP_WM %d\n#define OP_WN %d\n#define OP_OUTER %d\n"
                 "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#define OP_INDEX %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
@@ -138,7 +147,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         v.b_fast = !v.outer && (form & 1) == 0;
         v.aligned = v.outer ? (form & 1) == 0 : form < 2;
         v.index = v.outer ? (form - 4) / 2 : 0;
-        if ((v.outer && t < 2) || (!v.aligned && t > 2)) continue;
+        if ((v.outer && (t < 2 || t >= kSkinny)) || (!v.aligned && t > 2) || (t >= kSkinny && !v.b_fast)) continue;
         out.push_back(product_source(sp, v));
       }
   } else if (sp.kind == ACC_OP_ROUTE) {
@@ -311,15 +320,24 @@ bool near_enough(const acc_strided &a, int rows_dim, int64_t row, int bytes, boo
 // the knob's tile, where the form has it
 int tile_of(const OpSpec &sp, const ProductVariant &v, int tile)
 {
-  const bool there = sp.tile >= (v.outer ? 2 : 0) && sp.tile < kProductTileCount && (v.aligned || sp.tile < 3);
+  const bool there = sp.tile >= (v.outer ? 2 : 0) && sp.tile < (v.outer || !v.b_fast ? kSkinny : kProductTileCount) && (v.aligned || sp.tile < 3);
   return there ? sp.tile : tile;
 }
 
 // the tile shape for products of `rows` rows of `experts` segments
-int rows_tile(int64_t rows, int64_t experts, int64_t n, bool aligned)
+int rows_tile(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, bool aligned, bool b_fast)
 {
   const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
-  return mean <= 24 ? 0 : mean <= 96 ? 1 : !aligned || mean < 512 || n < 256 ? 2 : 3;
+  const bool wide = sp.kind == ACC_OP_MICRO, word = !wide && sp.type == 0;
+  // matrices that a few workgroups would read alone, and those for a few rows of 16 bits each: see op_skinny.h
+  if (aligned && b_fast && mean <= 12) {
+    const bool few = std::min(rows, experts) * ceil_div(n, 64) < 192;
+    if (few) return kSkinny;
+    if (!wide && !word) return kSkinny + 1;
+  }
+  if (mean <= 24) return kLow;
+  if (mean <= 96 || word) return 1;
+  return !aligned || mean < 512 || n < 256 ? 2 : 3;
 }
 
 }  // namespace
@@ -431,6 +449,8 @@ try {
   acc_op_s *op = new acc_op_s();
   op->ctx = ctx;
   op->spec = sp;
+  op->spec.ahead = ctx->tuning_now()->get("product.ahead", sp.ahead);
+  op->spec.once = ctx->tuning_now()->get("product.once", sp.once);
   op->spec.tile = ctx->tuning_now()->get("product.tile", -1);
   *out = op;
   return ACC_OK;
@@ -501,7 +521,7 @@ try {
   v.b_fast = unit(*w, 2);
   v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
               near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
-  v.tile = tile_of(op->spec, v, rows_tile(rows, experts, n, v.aligned));
+  v.tile = tile_of(op->spec, v, rows_tile(op->spec, rows, experts, n, v.aligned, v.b_fast));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
@@ -562,7 +582,7 @@ try {
   v.index = !index ? 0 : turned ? 2 : 1;
   v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1) &&
               near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
-  v.tile = tile_of(op->spec, v, v.aligned && rows < (1 << 28) && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2);
+  v.tile = tile_of(op->spec, v, v.aligned && op->spec.type != 0 && rows < (1 << 28) && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2);
   const OpVariant *var = nullptr;
   // (a tile of 256 x 256 has the rows that an index names looked up by a kernel in front: see OP_PLACES)
   const bool places = v.index != 0 && v.aligned && kProductTiles[v.tile].bm == 256 && rows > 0;
@@ -873,7 +893,7 @@ try {
     v.aligned = v.aligned && t->ptr % 4 == 0;
     for (int d = 0; d + 1 < t->rank; ++d) v.aligned = v.aligned && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
   }
-  v.tile = tile_of(op->spec, v, rows_tile(rows, experts, n, v.aligned));
+  v.tile = tile_of(op->spec, v, rows_tile(op->spec, rows, experts, n, v.aligned, v.b_fast));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, micro_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];

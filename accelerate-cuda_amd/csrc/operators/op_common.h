@@ -53,17 +53,26 @@ ACC_DEV long long op_die_run(const long long b, const long long n)
   return die * q + acc_min<long long>(die, r) + b / ACC_XCDS;
 }
 
-/* how many runs of up to `height` rows the segments have */
-ACC_DEV int op_count_tiles(const int *offsets, const int experts, const int rows, const int height)
+/* Tile x of ti x tj as (i, j), x counting down `height` rows of tiles, then on to the next column: the tiles that a die works
+ * on at a time are about as many rows as columns, and few of either's operands are wanted. */
+ACC_DEV void op_grouped(const int x, const int ti, const int tj, const int height, int *i, int *j)
+{
+  const int group = x / (height * tj), first = group * height, here = acc_min(height, ti - first), y = x - first * tj;
+  *i = first + y % here;
+  *j = y / here;
+}
+
+/* Whole tiles of `height` rows that the segments have, and segments that end amid another one. */
+ACC_DEV void op_count_tiles(const int *offsets, const int experts, const int rows, const int height, int *whole, int *parts)
 {
   const int lane = acc_lane();
-  int all = 0;
+  *whole = *parts = 0;
   for (int base = 0; base < experts + 2; base += 64) {
     int b = 0, e = 0;
     if (base + lane < experts + 2) op_segment(offsets, experts, rows, base + lane, &b, &e);
-    all += acc_wave_reduce((e - b + height - 1) / height, [](int x, int y) { return x + y; });
+    *whole += acc_wave_reduce((e - b) / height, [](int x, int y) { return x + y; });
+    *parts += __popcll(__ballot((e - b) % height > 0));
   }
-  return all;
 }
 
 /* The expert with the n-th longest segment, of up to 64 experts (of more: number n): what takes longest is begun first, and
@@ -85,16 +94,23 @@ ACC_DEV int op_nth_longest(const int *offsets, const int experts, const int rows
 
 struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segment; begin >= end: no such tile */
 
-/* The `tile`-th run of up to `height` rows, counted segment after segment: a wave adds up the runs of 64 segments at a
- * time.  Every wave of a workgroup works it out for itself, and the answer is the same in every lane. */
-ACC_DEV op_tile op_find_tile(const int *offsets, const int experts, const int rows, const int height, int tile)
+/* How segments are cut into runs of `height` rows: all runs, the last of a segment shorter; its whole runs only; or what is
+ * left behind those. */
+#define OP_ALL 0
+#define OP_WHOLE 1
+#define OP_REST 2
+
+/* The `tile`-th such run, counted segment after segment: a wave adds up the runs of 64 segments at a time.  Every wave of a
+ * workgroup works it out for itself, and the answer is the same in every lane. */
+template <int KIND> ACC_DEV op_tile op_find_tile(const int *offsets, const int experts, const int rows, const int height, int tile)
 {
   const int lane = acc_lane();
   op_tile t = {-1, 0, 0};
   for (int base = 0; base < experts + 2; base += 64) {
     int b = 0, e = 0;
     if (base + lane < experts + 2) op_segment(offsets, experts, rows, base + lane, &b, &e);
-    const int runs = (e - b + height - 1) / height;
+    if (KIND == OP_REST) b = e - (e - b) % height;
+    const int runs = KIND == OP_WHOLE ? (e - b) / height : (e - b + height - 1) / height;
     const int upto = acc_wave_scan(runs, [](int x, int y) { return x + y; }, lane);
     const unsigned long long beyond = __ballot(upto > tile);
     if (beyond) {

@@ -1,0 +1,75 @@
+/*
+ * op_matrix.h -- what the products' kernels share: elements in memory, fragments, the matrix instructions.
+ */
+#ifndef ACC_OP_MATRIX_H
+#define ACC_OP_MATRIX_H
+
+#include "op_common.h"
+
+#if OP_TYPE == 3
+typedef unsigned char op_mem;
+#else
+typedef op_elt op_mem;
+#endif
+#define OP_EPC (16 / (int)sizeof(op_mem))          /* elements of a chunk of 16 bytes */
+#define OP_STEP (8 * OP_EPC)                       /* the step of the sum, in elements */
+
+#if OP_TYPE == 0
+typedef acc_f4 op_frag;                            /* four values of r for one i */
+ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, acc_f4 c)
+{
+#pragma unroll
+  for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t], y[t], c, 0, 0, 0);
+  return c;
+}
+#elif OP_TYPE == 1
+typedef _Float16 op_frag __attribute__((ext_vector_type(8)));
+ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
+#elif OP_TYPE == 2
+typedef __bf16 op_frag __attribute__((ext_vector_type(8)));
+ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
+#else
+typedef int op_i8 __attribute__((ext_vector_type(8)));
+typedef acc_u4 op_frag;                            /* a block of 32 */
+/* `sx` holds the scales of four fragments, x's the nx-th */
+ACC_DEV acc_f4 op_mfma_scaled(const op_frag &x, const op_frag &y, const acc_f4 c, const int sx, const int nx, const int sy, const int ny)
+{
+  const op_i8 a = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}, b = {(int)y.x, (int)y.y, (int)y.z, (int)y.w, 0, 0, 0, 0};
+  /* (the byte to take is part of the instruction; which it is, is known once the loops are unrolled) */
+#define OP_CASE(i, j) case 4 * i + j: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, i, sx, j, sy);
+#define OP_CASES(i) OP_CASE(i, 0) OP_CASE(i, 1) OP_CASE(i, 2) OP_CASE(i, 3)
+  switch (4 * nx + ny) { OP_CASES(0) OP_CASES(1) OP_CASES(2) OP_CASES(3) }
+  return c;
+}
+#endif
+
+#define OP_NOWHERE 0x80000000u                     /* an offset beyond the end of every buffer: reads as zeros */
+#define OP_FARTHEST 0x7fffffffll                   /* the longest buffer */
+
+/* which row an index of rows lo .. hi - 1 names for row m, divided as the arguments say; -1: none */
+ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi, const int limit, const unsigned int per_mul, const unsigned int per_shift)
+{
+  const int at = index[(unsigned int)acc_max(lo, acc_min(m, hi - 1))];
+  /* (by nothing: per_mul is 0) */
+  const int r = (int)(__umulhi((unsigned int)at, per_mul) >> per_shift) + (at & (per_mul ? 0 : -1));
+  return (m >= lo) & (m < hi) & ((unsigned int)at < 0x80000000u) & (r < limit) ? r : -1;
+}
+
+/* four neighbours of a row of the result, from column j on; `none`: of no row, whatever the sums say (a matrix may hold
+ * infinities: no row times that is zeros all the same) */
+ACC_DEV void op_write4(op_elt *out, const int j, const int end, const acc_f4 c, const bool none, const bool vectors)
+{
+  typedef op_elt op_e4 __attribute__((ext_vector_type(4)));
+  op_e4 v;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) v[t] = (op_elt)(none ? 0.0f : c[t]);
+  if (vectors) {
+    if (j < end) *(op_e4 *)(out + j) = v;
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (j + t < end) out[j + t] = v[t];
+  }
+}
+
+#endif

@@ -11,47 +11,12 @@
  * half's are read; one barrier a step, in its middle, says that everybody's share of the next step has arrived and that
  * nobody reads this one any more, so that the next but one may take its place.
  */
-#include "op_common.h"
+#include "op_matrix.h"
 
-#if OP_TYPE == 3
-typedef unsigned char op_mem;
-#else
-typedef op_elt op_mem;
-#endif
-#define OP_EPC (16 / (int)sizeof(op_mem))          /* elements of a chunk of 16 bytes */
-#define OP_STEP (8 * OP_EPC)                       /* the step of the sum, in elements */
 #define OP_THREADS (64 * OP_WM * OP_WN)
+#define OP_GROUP (OP_BM >= 256 ? 4 : OP_BM >= 128 ? 8 : 16)   /* rows of tiles that are gone through together */
 #define OP_FM (OP_BM / OP_WM / 16)                 /* fragments of 16 x 16 that a wave has of the result */
 #define OP_FN (OP_BN / OP_WN / 16)
-
-#if OP_TYPE == 0
-typedef acc_f4 op_frag;                            /* four values of r for one i */
-ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, acc_f4 c)
-{
-#pragma unroll
-  for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t], y[t], c, 0, 0, 0);
-  return c;
-}
-#elif OP_TYPE == 1
-typedef _Float16 op_frag __attribute__((ext_vector_type(8)));
-ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); }
-#elif OP_TYPE == 2
-typedef __bf16 op_frag __attribute__((ext_vector_type(8)));
-ACC_DEV acc_f4 op_mfma(const op_frag x, const op_frag y, const acc_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0); }
-#else
-typedef int op_i8 __attribute__((ext_vector_type(8)));
-typedef acc_u4 op_frag;                            /* a block of 32 */
-/* `sx` holds the scales of four fragments, x's the nx-th */
-ACC_DEV acc_f4 op_mfma_scaled(const op_frag &x, const op_frag &y, const acc_f4 c, const int sx, const int nx, const int sy, const int ny)
-{
-  const op_i8 a = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, 0, 0, 0, 0}, b = {(int)y.x, (int)y.y, (int)y.z, (int)y.w, 0, 0, 0, 0};
-  /* (the byte to take is part of the instruction; which it is, is known once the loops are unrolled) */
-#define OP_CASE(i, j) case 4 * i + j: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, i, sx, j, sy);
-#define OP_CASES(i) OP_CASE(i, 0) OP_CASE(i, 1) OP_CASE(i, 2) OP_CASE(i, 3)
-  switch (4 * nx + ny) { OP_CASES(0) OP_CASES(1) OP_CASES(2) OP_CASES(3) }
-  return c;
-}
-#endif
 
 /* OP_INDEX, outer: 0: no index, 1: of b's rows, 2: of a's */
 #define OP_PLAIN 0
@@ -59,8 +24,6 @@ ACC_DEV acc_f4 op_mfma_scaled(const op_frag &x, const op_frag &y, const acc_f4 c
 #define OP_GATED 2
 
 typedef __attribute__((address_space(3))) void *op_lds_ptr;
-#define OP_NOWHERE 0x80000000u                     /* an offset beyond the end of every buffer: reads as zeros */
-#define OP_FARTHEST 0x7fffffffll                   /* the longest buffer */
 
 /* v, `bytes` further down: what is shifted in is zeros */
 ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
@@ -76,15 +39,6 @@ ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
     b = hi >> n;
   }
   return acc_u4{(unsigned int)a, (unsigned int)(a >> 32), (unsigned int)b, (unsigned int)(b >> 32)};
-}
-
-/* which row an index of rows lo .. hi - 1 names for row m, divided as the arguments say; -1: none */
-ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi, const int limit, const unsigned int per_mul, const unsigned int per_shift)
-{
-  const int at = index[(unsigned int)acc_max(lo, acc_min(m, hi - 1))];
-  /* (by nothing: per_mul is 0) */
-  const int r = (int)(__umulhi((unsigned int)at, per_mul) >> per_shift) + (at & (per_mul ? 0 : -1));
-  return (m >= lo) & (m < hi) & ((unsigned int)at < 0x80000000u) & (r < limit) ? r : -1;
 }
 
 /* Where row r of an operand lies, in bytes, as a load takes it whose buffer ends before 2 GB: the top bit set, and none (r < 0)
@@ -389,21 +343,31 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     /* (segments are of any length: the longest first, each on all dies) */
     const int tiles = p.tiles_i * p.tiles_j;
     expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, (int)(blockIdx.x / tiles));
-    const int t = (int)op_die_run(blockIdx.x % tiles, tiles);
-    i0 = (t / p.tiles_j) * OP_BM;
-    j0 = (t % p.tiles_j) * OP_BN;
+    int i, j;
+    op_grouped((int)op_die_run(blockIdx.x % tiles, tiles), p.tiles_i, p.tiles_j, OP_GROUP, &i, &j);
+    i0 = i * OP_BM;
+    j0 = j * OP_BN;
     iend = p.ni;
     jend = p.nj;
     op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
   }
 #else
   {
-    /* (the grid is for the worst lengths; the tiles that there are, are shared out evenly) */
-    const long long tiles = (long long)op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM) * p.tiles_j;
-    if (blockIdx.x >= tiles) return;
-    const long long block = op_die_run(blockIdx.x, tiles);
-    j0 = (int)(block % p.tiles_j) * OP_BN;
-    const op_tile tile = op_find_tile(p.offsets, p.experts, (int)p.rows, OP_BM, (int)(block / p.tiles_j));
+    /* Whole tiles first, then those that end a segment, which take less long.  (The grid is for the worst lengths; the tiles
+     * that there are, are shared out evenly.) */
+    int whole, rest, i, j;
+    op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM, &whole, &rest);
+    const long long first = (long long)whole * p.tiles_j, all = first + (long long)rest * p.tiles_j;
+    if (blockIdx.x >= all) return;
+    op_tile tile;
+    if (blockIdx.x < first) {
+      op_grouped((int)op_die_run(blockIdx.x, first), whole, p.tiles_j, OP_GROUP, &i, &j);
+      tile = op_find_tile<OP_WHOLE>(p.offsets, p.experts, (int)p.rows, OP_BM, i);
+    } else {
+      op_grouped((int)op_die_run(blockIdx.x - first, all - first), rest, p.tiles_j, OP_GROUP, &i, &j);
+      tile = op_find_tile<OP_REST>(p.offsets, p.experts, (int)p.rows, OP_BM, i);
+    }
+    j0 = j * OP_BN;
     if (tile.begin >= tile.end) return;
     expert = tile.expert;
     i0 = tile.begin;
@@ -620,6 +584,25 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #endif
     /* (an odd number of steps has one of zeros behind it: with a way out between the two, the sums would change registers) */
     int r = r0;
+#if OP_ALIGNED
+    if (i0 + wi >= iend) {
+      /* a wave whose rows lie behind the segment's end only brings its share */
+      const auto idle = [&](acc_u4 *here, const int r) {
+#pragma unroll
+        for (int q = 0; q < op_a::MINE; ++q) look_at(q, r + 2 * OP_STEP);
+        op_meet(true);
+        put_scales(here);
+        ask_scales(r + 3 * OP_STEP);
+#pragma unroll
+        for (int n = 0; n < ALL; ++n) bring(here, n, r + 2 * OP_STEP);
+      };
+      do {
+        idle(lds0, r);
+        idle(lds1, r + OP_STEP);
+        r += 2 * OP_STEP;
+      } while (r < r1);
+    } else
+#endif
     do {
       round(lds0, lds1, r);
       round(lds1, lds0, r + OP_STEP);
@@ -634,26 +617,13 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     const int ri = i0 + wi + i * 16 + (lane & 15);
     if (ri >= iend) continue;
     op_elt *out = (op_elt *)p.out + (long long)ri * p.out_stride;
-    bool none = false;           /* (a matrix may hold infinities: no row times that is zeros all the same) */
+    bool none = false;
 #if OP_OUTER
     out += (long long)expert * p.out_expert;
 #else
     none = p.index_a && a.number(ri) < 0;
 #endif
 #pragma unroll
-    for (int j = 0; j < OP_FN; ++j) {
-      const int cj = j0 + wj + j * 16 + 4 * (lane >> 4);
-      typedef op_elt op_e4 __attribute__((ext_vector_type(4)));
-      op_e4 v;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) v[t] = (op_elt)(none ? 0.0f : c[i][j][t]);
-      if (p.out_vectors) {
-        if (cj < jend) *(op_e4 *)(out + cj) = v;
-      } else {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (cj + t < jend) out[cj + t] = v[t];
-      }
-    }
+    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none, p.out_vectors);
   }
 }
