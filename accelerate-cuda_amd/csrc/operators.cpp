@@ -52,8 +52,9 @@ constexpr int kProductTileCount = 6, kLow = 0, kSkinny = 4;      // the last two
 struct ProductVariant {
   int tile = 0;
   bool outer = false, b_fast = true, aligned = true;
+  bool tiny = false;            // not aligned: a row is shorter than 16 bytes
   int index = 0;                // outer: whose rows an index names: 1 b's, 2 a's
-  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u) | (uint32_t)index << 7; }
+  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u) | (uint32_t)index << 7 | (tiny ? 512u : 0u); }
 };
 
 std::string product_source(const OpSpec &sp, const ProductVariant &v)
@@ -70,8 +71,8 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
   }
   std::snprintf(text, sizeof(text),
                 "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_BN %d\n#define OP_WM %d\n#define OP_WN %d\n#define OP_OUTER %d\n"
-                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#define OP_INDEX %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
-                sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0, v.index);
+                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#define OP_INDEX %d\n#define OP_TINY %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
+                sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0, v.index, v.tiny ? 1 : 0);
   return text;
 }
 
@@ -140,13 +141,14 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   std::vector<std::string> out;
   if (sp.kind == ACC_OP_PRODUCT) {
     for (int t = 0; t < kProductTileCount; ++t)
-      for (int form = 0; form < 10; ++form) {
+      for (int form = 0; form < 15; ++form) {
         ProductVariant v;
         v.tile = t;
-        v.outer = form >= 4;
+        v.outer = form >= 6;
         v.b_fast = !v.outer && (form & 1) == 0;
-        v.aligned = v.outer ? (form & 1) == 0 : form < 2;
-        v.index = v.outer ? (form - 4) / 2 : 0;
+        v.aligned = v.outer ? form % 3 == 0 : form < 2;
+        v.tiny = v.outer ? form % 3 == 2 : form >= 4;
+        v.index = v.outer ? (form - 6) / 3 : 0;
         if ((v.outer && (t < 2 || t >= kSkinny)) || (!v.aligned && t > 2) || (t >= kSkinny && !v.b_fast)) continue;
         out.push_back(product_source(sp, v));
       }
@@ -298,15 +300,6 @@ void set_divisor(int32_t per, acc_product_args *a)
   a->per_shift = static_cast<uint32_t>(l - 1);
 }
 
-// whether four neighbours of a result's rows, from every fourth on, can be written at once
-bool out_in_vectors(const acc_strided &o, int bytes)
-{
-  if (o.shape[o.rank - 1] % 4 != 0 || o.ptr % (uint64_t)(4 * bytes) != 0) return false;
-  for (int d = 0; d + 1 < o.rank; ++d)
-    if (o.shape[d] > 1 && o.stride[d] % 4 != 0) return false;
-  return true;
-}
-
 // Whether offsets of 32 bits (and buffers below 2 GB) do for an operand of the aligned form: rows of `row` bytes of which
 // `tile` (all `rows` of them, with an index) are reached from one base; rows must not overlap, as a buffer that ends with the
 // last row that counts would cut others short.
@@ -362,6 +355,7 @@ std::string product_source_of(const OpSpec &sp, uint32_t key)
   v.b_fast = key & 32u;
   v.aligned = key & 64u;
   v.index = (int)(key >> 7 & 3u);
+  v.tiny = key & 512u;
   return product_source(sp, v);
 }
 std::string route_source_of(const OpSpec &sp, uint32_t key)
@@ -521,6 +515,7 @@ try {
   v.b_fast = unit(*w, 2);
   v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
               near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
+  v.tiny = !v.aligned && (k < epc || (!v.b_fast && n < epc));
   v.tile = tile_of(op->spec, v, rows_tile(op->spec, rows, experts, n, v.aligned, v.b_fast));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
@@ -540,7 +535,6 @@ try {
   a.k = (int32_t)k;
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
-  a.out_vectors = out_in_vectors(*out, bytes);
   a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
   a.tiles_j = (int32_t)ceil_div(n, t.bn);
   return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
@@ -582,6 +576,7 @@ try {
   v.index = !index ? 0 : turned ? 2 : 1;
   v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1) &&
               near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
+  v.tiny = !v.aligned && (o.shape[1] < epc || o.shape[2] < epc);
   v.tile = tile_of(op->spec, v, v.aligned && op->spec.type != 0 && rows < (1 << 28) && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2);
   const OpVariant *var = nullptr;
   // (a tile of 256 x 256 has the rows that an index names looked up by a kernel in front: see OP_PLACES)
@@ -604,7 +599,6 @@ try {
   a.nj = (int32_t)o.shape[2];
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
-  a.out_vectors = out_in_vectors(o, bytes);
   a.tiles_i = (int32_t)ceil_div(o.shape[1], t.bm);
   a.tiles_j = (int32_t)ceil_div(o.shape[2], t.bn);
   acc::ScratchRef scratch;
@@ -917,7 +911,6 @@ try {
   a.k = (int32_t)(16 * blocks);
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
-  a.out_vectors = out_in_vectors(*out, bytes);
   a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
   a.tiles_j = (int32_t)ceil_div(n, t.bn);
   return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);

@@ -30,8 +30,6 @@ struct acc_product_args {
   uint32_t per_mul, per_shift;  /* an index at is divided: (at * per_mul) >> (32 + per_shift); per_mul 0: it is not */
   int32_t tiles_i, tiles_j;     /* the grid's tiles */
   uint32_t *places;             /* outer, with an index, in large tiles: where the rows lie that it names, a number a row */
-  int32_t out_vectors;          /* four neighbours of the result can be written at once */
-  int32_t pad;
   const uint32_t *guard;
 };
 

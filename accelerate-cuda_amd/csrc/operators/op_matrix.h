@@ -55,20 +55,20 @@ ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi,
   return (m >= lo) & (m < hi) & ((unsigned int)at < 0x80000000u) & (r < limit) ? r : -1;
 }
 
-/* four neighbours of a row of the result, from column j on; `none`: of no row, whatever the sums say (a matrix may hold
- * infinities: no row times that is zeros all the same) */
-ACC_DEV void op_write4(op_elt *out, const int j, const int end, const acc_f4 c, const bool none, const bool vectors)
+/* four neighbours of a row of the result, from column j on, wherever it starts; `none`: of no row, whatever the sums say (a
+ * matrix may hold infinities: no row times that is zeros all the same) */
+ACC_DEV void op_write4(op_elt *out, const int j, const int end, const acc_f4 c, const bool none)
 {
-  typedef op_elt op_e4 __attribute__((ext_vector_type(4)));
-  op_e4 v;
+  struct __attribute__((packed, aligned(sizeof(op_elt)))) op_e4 { op_elt v[4]; };
+  op_e4 e;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) v[t] = (op_elt)(none ? 0.0f : c[t]);
-  if (vectors) {
-    if (j < end) *(op_e4 *)(out + j) = v;
+  for (int t = 0; t < 4; ++t) e.v[t] = (op_elt)(none ? 0.0f : c[t]);
+  if (j + 4 <= end) {
+    *(op_e4 *)(out + j) = e;
   } else {
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      if (j + t < end) out[j + t] = v[t];
+      if (j + t < end) out[j + t] = e.v[t];
   }
 }
 

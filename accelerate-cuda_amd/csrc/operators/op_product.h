@@ -171,8 +171,9 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
   }
 #else
   /* the same by way of registers: `load` asks, whoever has asked puts what has come into LDS a step later.  `whole`: every
-   * chunk of the step lies within its row (and across r, without an index, every row counts). */
-  ACC_DEV bool whole(const int r) const { return FAST ? r + OP_STEP <= extent : ((LIST != OP_PLAIN) | (r + OP_STEP <= hi)) & (extent >= TILE); }
+   * chunk of the step lies within its row (and across r, without an index, every row counts).  OP_TINY: a row is shorter than a
+   * chunk. */
+  ACC_DEV bool whole(const int r) const { return OP_TINY ? false : FAST ? r + OP_STEP <= extent : ((LIST != OP_PLAIN) | (r + OP_STEP <= hi)) & (extent >= TILE); }
   ACC_DEV void load(acc_u4 &v, const int tid, const int q, const int r, const int named, const bool whole) const
   {
     const int s = slot(tid, q);
@@ -188,15 +189,15 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
     /* elements of the row that are wanted first, and how many there are */
     const int m = r + major(s), n = FAST ? 0 : LIST == OP_PLAIN ? (m < hi ? m : -1) : LIST == OP_GATED && named >= 0 ? m : named, c = FAST ? r + column : element(s);
     const unsigned char *row = FAST ? base + offset[q] - column * SIZE : base + (long long)acc_max(n, 0) * stride;
-    if (extent < OP_EPC) {
-      op_mem e[OP_EPC];
+#if OP_TINY
+    op_mem e[OP_EPC];
 #pragma unroll
-      for (int k = 0; k < OP_EPC; ++k) e[k] = c + k < extent ? ((const op_mem *)row)[c + k] : (op_mem)0;
-      __builtin_memcpy(&v, e, 16);
-    } else {
-      const int at = acc_min(c, extent - OP_EPC);
-      v = op_shifted(((const op_loose<op_mem> *)(row + (long long)at * SIZE))->v, (c - at) * SIZE);
-    }
+    for (int k = 0; k < OP_EPC; ++k) e[k] = c + k < extent ? ((const op_mem *)row)[c + k] : (op_mem)0;
+    __builtin_memcpy(&v, e, 16);
+#else
+    const int at = acc_min(c, extent - OP_EPC);
+    v = op_shifted(((const op_loose<op_mem> *)(row + (long long)at * SIZE))->v, (c - at) * SIZE);
+#endif
     if (n < 0) v = acc_u4{0, 0, 0, 0};
   }
 #endif
@@ -378,6 +379,12 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
   }
 #endif
 
+#if !OP_ALIGNED
+  /* (a last column of tiles that would reach beyond the result's edge across r starts earlier: some results are worked out
+   * twice, to the same value, and no chunk reaches beyond its row) */
+  if (OP_OUTER) i0 = acc_max(0, acc_min(i0, p.ni - OP_BM));
+  if (!OP_B_FAST) j0 = acc_max(0, acc_min(j0, p.nj - OP_BN));
+#endif
   op_a a;
   op_b b;
   a.base = (const unsigned char *)p.a;
@@ -624,6 +631,6 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     none = p.index_a && a.number(ri) < 0;
 #endif
 #pragma unroll
-    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none, p.out_vectors);
+    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none);
   }
 }

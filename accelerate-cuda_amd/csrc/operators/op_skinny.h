@@ -120,6 +120,6 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) product(const acc_pr
     if (m >= tile.end) continue;
     op_elt *out = (op_elt *)p.out + (long long)m * p.out_stride;
 #pragma unroll
-    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + j * 16 + 4 * g, p.nj, c[i][j], arow[i] < 0, p.out_vectors);
+    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + j * 16 + 4 * g, p.nj, c[i][j], arow[i] < 0);
   }
 }
