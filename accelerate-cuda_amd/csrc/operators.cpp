@@ -34,7 +34,7 @@ struct OpSpec {
   int type = 0;                 // 0 float, 1 half, 2 bfloat16
   int choose = 0;
   bool normalise = true;
-  int ahead = 4, once = 0;      // knobs product.ahead and product.once of the form for a few rows
+  int ahead = 3, once = 0;      // knobs product.ahead and product.once of the form for a few rows
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
@@ -113,11 +113,12 @@ std::string route_source(const OpSpec &sp, const RouteVariant &v)
 int route_block(int64_t tokens) { return (int)(tokens <= 256 ? 256 : std::max<int64_t>(64, ceil_div(tokens, 256))); }
 
 constexpr int kCombineSlots = 4;
-std::string combine_source(const OpSpec &sp, bool aligned)
+// rows 0 anywhere, 1 aligned, 2 of fewer than eight elements
+std::string combine_source(const OpSpec &sp, int rows)
 {
   char text[256];
-  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_ALIGNED %d\n#define OP_SLOTS %d\n#include \"acc_hip_device.h\"\n#include \"op_combine.h\"\n",
-                sp.type, aligned ? 1 : 0, kCombineSlots);
+  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_ALIGNED %d\n#define OP_TINY %d\n#define OP_SLOTS %d\n#include \"acc_hip_device.h\"\n#include \"op_combine.h\"\n",
+                sp.type, rows == 1 ? 1 : 0, rows == 2 ? 1 : 0, kCombineSlots);
   return text;
 }
 
@@ -157,7 +158,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
       for (bool aligned : {true, false})
         for (int64_t tokens : {int64_t(1), kRouteTallFrom}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
-    for (bool aligned : {true, false}) out.push_back(combine_source(sp, aligned));
+    for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
   } else {
     for (bool aligned : {true, false}) out.push_back(micro_source(sp, aligned));
     for (int t = 0; t < kProductTileCount; ++t)
@@ -291,7 +292,7 @@ int64_t tiles_at_most(int64_t rows, int64_t experts, int64_t height)
 
 // An index at is divided by `per` as (at * mul) >> (32 + shift), exact for 0 <= at < 2^31 (with l = ceil(log2 per), mul is
 // 2^(31 + l) / per rounded up: its excess times at stays below 2^(31 + l)).
-void set_divisor(int32_t per, acc_product_args *a)
+template <typename T> void set_divisor(int32_t per, T *a)
 {
   if (per < 2) return;
   int l = 1;
@@ -368,7 +369,7 @@ std::string route_source_of(const OpSpec &sp, uint32_t key)
   v.tall = key >> 31;
   return route_source(sp, v);
 }
-std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_source(sp, key & 1u); }
+std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_source(sp, (int)(key & 3u)); }
 constexpr uint32_t kMicroElements = 1024;            // (above the products' keys)
 std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & kMicroElements) ? micro_source(sp, key & 1u) : product_source_of(sp, key); }
 
@@ -737,12 +738,12 @@ try {
   const int64_t tokens = out->shape[0], width = out->shape[1];
   ACC_TRY(check_slots(who, place, weights, tokens));
   ACC_TRY(check_shape(who, "y", *y, {y->shape[0], width}));
-  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  const int bytes = type_bytes(op->spec.type);
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{y, bytes, "y"}, {place, 4, "place"}, {weights, 4, "weights"}}));
   if (is_empty(*out)) return ACC_OK;
-  const bool aligned = width % epc == 0 && aligned_rows(*y, bytes, 1) && aligned_rows(*out, bytes, 1);
+  const bool aligned = width % 8 == 0 && aligned_rows(*y, bytes, 1) && aligned_rows(*out, bytes, 1);
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(aligned ? 1u : 0u, kCombineNames, 2, combine_source_of, &var));
+  ACC_TRY(op->variant(aligned ? 1u : width < 8 ? 2u : 0u, kCombineNames, 2, combine_source_of, &var));
   a.y = device<const void>(y);
   a.out = device<void>(out);
   a.place = device<const int32_t>(place);
@@ -753,7 +754,17 @@ try {
   a.out_stride = out->stride[0];
   a.choose = (int32_t)place->shape[1];
   a.width = (int32_t)width;
-  return launch(op, who, var->fn, ceil_div(tokens * ceil_div(width, 8), 256), 256, 0, stream, a);
+  const int64_t pieces = ceil_div(width, 8), most = std::max<int64_t>(1, 0x7fffff00 / pieces);
+  set_divisor((int32_t)pieces, &a);
+  for (int64_t first = 0; first < tokens; first += most) {           // (a lane's number has 31 bits)
+    acc_combine_args part = a;
+    part.tokens = std::min(most, tokens - first);
+    part.out = static_cast<char *>(a.out) + first * a.out_stride * bytes;
+    part.place = a.place + first * a.choose;
+    part.weights = a.weights ? a.weights + first * a.choose : nullptr;
+    ACC_TRY(launch(op, who, var->fn, ceil_div(part.tokens * pieces, 256), 256, 0, stream, part));
+  }
+  return ACC_OK;
 } ACC_OP_CATCH("acc_exec_combine")
 
 int acc_exec_combine_gradient(acc_op op, const acc_strided *dout, const acc_strided *y, const acc_strided *place, const acc_strided *weights,
@@ -775,13 +786,13 @@ try {
     ACC_TRY(check_shape(who, "dweights", *dweights, {tokens, place->shape[1]}));
     if (tokens > 1 && dweights->stride[0] != dweights->shape[1]) return fail(ACC_ERR_INVALID, "%s: dweights is a dense array", who);
   }
-  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  const int bytes = type_bytes(op->spec.type);
   ACC_TRY(check_apart(who, {dy, bytes, "dy"}, {{dout, bytes, "dout"}, {y, bytes, "y"}, {place, 4, "place"}, {weights, 4, "weights"}, {dweights, 4, "dweights"}}));
   if (dweights) ACC_TRY(check_apart(who, {dweights, 4, "dweights"}, {{dout, bytes, "dout"}, {y, bytes, "y"}, {place, 4, "place"}, {weights, 4, "weights"}}));
   if (tokens == 0 || place->shape[1] == 0) return ACC_OK;
-  const bool aligned = width % epc == 0 && aligned_rows(*dout, bytes, 1) && aligned_rows(*dy, bytes, 1) && (!y || aligned_rows(*y, bytes, 1));
+  const bool aligned = width % 8 == 0 && aligned_rows(*dout, bytes, 1) && aligned_rows(*dy, bytes, 1) && (!y || aligned_rows(*y, bytes, 1));
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(aligned ? 1u : 0u, kCombineNames, 2, combine_source_of, &var));
+  ACC_TRY(op->variant(aligned ? 1u : width < 8 ? 2u : 0u, kCombineNames, 2, combine_source_of, &var));
   a.y = device<const void>(y);
   a.dout = device<const void>(dout);
   a.out = device<void>(dy);
@@ -795,7 +806,7 @@ try {
   a.dout_stride = dout->stride[0];
   a.choose = (int32_t)place->shape[1];
   a.width = (int32_t)width;
-  return launch(op, who, var->fn2, ceil_div(tokens, 4), 256, 0, stream, a);
+  return launch(op, who, var->fn2, tokens, 64 * (int)std::max<int64_t>(1, std::min<int64_t>(4, ceil_div(width, 512))), 0, stream, a);
 } ACC_OP_CATCH("acc_exec_combine_gradient")
 
 // ---- 4-bit numbers --------------------------------------------------------------------
@@ -832,7 +843,19 @@ static int micro_elements(acc_op op, const char *who, bool back, const acc_strid
   a.scales_stride = scales->stride[0];
   a.k = (int32_t)k;
   a.blocks = (int32_t)blocks;
-  return launch(op, who, back ? var->fn2 : var->fn, ceil_div(rows * blocks * 4, 256), 256, 0, stream, a);
+  set_divisor((int32_t)blocks, &a);
+  // (rows by the bound of a lane's block number, see op_mine)
+  const int64_t most = std::max<int64_t>(1, 0x7fffff00 / blocks);
+  for (int64_t first = 0; first < rows; first += most) {
+    acc_micro_args part = a;
+    part.rows = std::min(most, rows - first);
+    part.x = static_cast<const char *>(a.x) + first * a.x_stride * bytes;
+    part.out = static_cast<char *>(a.out) + first * a.x_stride * bytes;
+    part.codes = a.codes + first * a.codes_stride;
+    part.scales = a.scales + first * a.scales_stride;
+    ACC_TRY(launch(op, who, back ? var->fn2 : var->fn, ceil_div(part.rows * blocks * 4, 256), 256, 0, stream, part));
+  }
+  return ACC_OK;
 }
 
 int acc_exec_micro_quantise(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, acc_stream stream)

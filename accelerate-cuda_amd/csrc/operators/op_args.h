@@ -58,6 +58,7 @@ struct acc_combine_args {
   float *dweights;
   int64_t tokens, y_rows, y_stride, out_stride, dout_stride;
   int32_t choose, width;
+  uint32_t per_mul, per_shift;  /* combine: division by a row's pieces of eight */
   const uint32_t *guard;
 };
 
@@ -68,6 +69,7 @@ struct acc_micro_args {
   uint8_t *codes, *scales;
   int64_t rows, x_stride, codes_stride, scales_stride;
   int32_t k, blocks;
+  uint32_t per_mul, per_shift;  /* division by `blocks`, as for the products' indices */
   const uint32_t *guard;
 };
 

@@ -8,25 +8,45 @@
  */
 #include "op_common.h"
 
-/* the code of x * scale */
-ACC_DEV unsigned int op_code(const float x, const float scale)
+/* two elements' codes in byte `n` of `to`: the target's own conversion rounds as said above, and takes the scale as the
+ * exponent of a Float32 */
+template <int N> ACC_DEV unsigned int op_codes(const unsigned int to, const float x, const float y, const float scale)
 {
-  const float v = x * scale, a = __builtin_fabsf(v);
-  const unsigned int m = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.0f);
-  return m | (__float_as_uint(x) >> 31 << 3);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(to, x, y, scale, N);
+}
+template <int N> ACC_DEV void op_values(const unsigned int codes, const float scale, float *to)
+{
+  const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, N);
+  to[0] = v[0];
+  to[1] = v[1];
+}
+
+/* A lane's place: eight elements of a block, four lanes a block, blocks row after row.  (Rows by multiplication, the driver's
+ * divisor; a call has fewer than 2^31 blocks.) */
+struct op_eight { long long row; int block, first; bool here; };
+ACC_DEV op_eight op_mine(const acc_micro_args &p)
+{
+  const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
+  const unsigned int block = (unsigned int)(n >> 2);
+  const unsigned int row = p.per_mul ? __umulhi(block, p.per_mul) >> p.per_shift : block;
+  op_eight e;
+  e.row = row;
+  e.block = (int)(block - row * (unsigned int)p.blocks);
+  e.first = e.block * 32 + (int)(n & 3) * 8;
+  e.here = row < p.rows;
+  return e;
 }
 
 /* four lanes have a block of 32, 8 elements each; a lane's elements are 4 bytes of codes */
 extern "C" __global__ void __launch_bounds__(256) micro_quantise(const acc_micro_args p)
 {
   if (p.guard && *p.guard == 0u) return;
-  const long long n = (long long)blockIdx.x * 256 + threadIdx.x, block = n >> 2, row = block / p.blocks;
-  const int b = (int)(block % p.blocks), c = b * 32 + (int)(n & 3) * 8;
-  const bool here = row < p.rows;
+  const op_eight at = op_mine(p);
+  const int quarter = (int)threadIdx.x & 3;
   float f[8];
 #pragma unroll
   for (int h = 0; h < 8 / OP_VALUES; ++h) {
-    const acc_u4 v = op_chunk<OP_ALIGNED>((const op_elt *)p.x + row * p.x_stride + c + h * OP_VALUES, here ? p.k - c - h * OP_VALUES : 0);
+    const acc_u4 v = op_chunk<OP_ALIGNED>((const op_elt *)p.x + at.row * p.x_stride + at.first + h * OP_VALUES, at.here ? p.k - at.first - h * OP_VALUES : 0);
     op_elt e[OP_VALUES];
     __builtin_memcpy(e, &v, 16);
 #pragma unroll
@@ -36,44 +56,44 @@ extern "C" __global__ void __launch_bounds__(256) micro_quantise(const acc_micro
   unsigned int most = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) most = acc_max(most, __float_as_uint(f[k]) & 0x7fffffffu);
-  most = acc_max(most, (unsigned int)__shfl_xor((int)most, 1));
-  most = acc_max(most, (unsigned int)__shfl_xor((int)most, 2));
+  most = acc_max(most, acc_dpp<0xB1, 0xf>(most, most));          /* the neighbour's, then the other pair's */
+  most = acc_max(most, acc_dpp<0x4E, 0xf>(most, most));
   /* a subnormal Float32 is below 2^-126: its scale is the smallest one anyway */
   const int exponent = (int)(most >> 23);
   const int byte = exponent == 255 ? 255 : acc_max(exponent - 2, 0);
-  const float scale = __builtin_ldexpf(1.0f, 127 - acc_min(byte, 254));
+  const float scale = __uint_as_float((unsigned int)byte << 23);
   unsigned int codes = 0;
-  if (byte < 255)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) codes |= op_code(f[k], scale) << (4 * k);
-  if (!here) return;
-  *(unsigned int *)(p.codes + row * p.codes_stride + b * 16 + (n & 3) * 4) = codes;
-  if ((n & 3) == 0) p.scales[row * p.scales_stride + b] = (unsigned char)byte;
+  codes = op_codes<0>(codes, f[0], f[1], scale);
+  codes = op_codes<1>(codes, f[2], f[3], scale);
+  codes = op_codes<2>(codes, f[4], f[5], scale);
+  codes = op_codes<3>(codes, f[6], f[7], scale);
+  if (byte == 255) codes = 0;
+  if (!at.here) return;
+  *(unsigned int *)(p.codes + at.row * p.codes_stride + at.block * 16 + quarter * 4) = codes;
+  if (quarter == 0) p.scales[at.row * p.scales_stride + at.block] = (unsigned char)byte;
 }
 
 /* a lane has 8 elements */
 extern "C" __global__ void __launch_bounds__(256) micro_values(const acc_micro_args p)
 {
   if (p.guard && *p.guard == 0u) return;
-  const long long n = (long long)blockIdx.x * 256 + threadIdx.x, block = n >> 2, row = block / p.blocks;
-  if (row >= p.rows) return;
-  const int b = (int)(block % p.blocks), c = b * 32 + (int)(n & 3) * 8;
-  const unsigned int codes = *(const unsigned int *)(p.codes + row * p.codes_stride + b * 16 + (n & 3) * 4);
-  const int byte = p.scales[row * p.scales_stride + b];
-  op_elt *out = (op_elt *)p.out + row * p.x_stride + c;
+  const op_eight at = op_mine(p);
+  if (!at.here) return;
+  const unsigned int codes = *(const unsigned int *)(p.codes + at.row * p.codes_stride + at.block * 16 + ((int)threadIdx.x & 3) * 4);
+  const int byte = p.scales[at.row * p.scales_stride + at.block];
+  const float scale = __uint_as_float((unsigned int)byte << 23);
+  op_elt *out = (op_elt *)p.out + at.row * p.x_stride + at.first;
+  float f[8];
+  op_values<0>(codes, scale, f);
+  op_values<1>(codes, scale, f + 2);
+  op_values<2>(codes, scale, f + 4);
+  op_values<3>(codes, scale, f + 6);
   op_elt e[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const unsigned int code = codes >> (4 * k);
-    /* 0, 1/2, then 2^(e - 1) (1 + m / 2) */
-    const unsigned int m = code & 7u;
-    const float a = m < 2 ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-    const float v = byte == 255 ? __builtin_nanf("") : __builtin_ldexpf(code & 8u ? -a : a, byte - 127);
-    e[k] = (op_elt)v;
-  }
+  for (int k = 0; k < 8; ++k) e[k] = (op_elt)(byte == 255 ? __builtin_nanf("") : f[k]);
 #pragma unroll
   for (int h = 0; h < 8 / OP_VALUES; ++h) {
-    const int left = p.k - c - h * OP_VALUES;
+    const int left = p.k - at.first - h * OP_VALUES;
     acc_u4 v;
     __builtin_memcpy(&v, e + h * OP_VALUES, 16);
     if (OP_ALIGNED) {

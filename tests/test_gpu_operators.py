@@ -473,7 +473,8 @@ def test_gradient_of_the_router(A, ctx, ops, elt, tokens, experts, choose):
 # ------------------------------------------------------------------------------ the combination
 
 @pytest.mark.parametrize("elt", TYPES)
-@pytest.mark.parametrize("tokens,choose,width,lead,extra", [(1, 1, 1, 0, 0), (3, 2, 8, 0, 0), (50, 4, 264, 0, 8), (33, 6, 131, 1, 2), (130, 9, 72, 0, 0), (7, 3, 2048, 8, 0), (5, 2, 1501, 0, 0)])
+@pytest.mark.parametrize("tokens,choose,width,lead,extra", [(1, 1, 1, 0, 0), (3, 2, 8, 0, 0), (50, 4, 264, 0, 8), (33, 6, 131, 1, 2), (130, 9, 72, 0, 0), (7, 3, 2048, 8, 0), (5, 2, 1501, 0, 0),
+                                                               (6, 67, 40, 0, 0), (5, 130, 19, 1, 1), (4, 3, 5003, 0, 3), (9, 5, 7, 0, 0), (3, 64, 12, 0, 4)])
 def test_combination_and_its_gradient(A, ctx, ops, elt, tokens, choose, width, lead, extra):
     say("combine", elt, tokens, choose, width, lead, extra)
     rng = np.random.default_rng(tokens + width)
@@ -745,3 +746,14 @@ def test_nothing_to_do_is_no_error(A, ctx, ops):
     ops("Combiner", "float").combine(f(0, 8), ctx.array(np.zeros((3, 2), np.int32)), None, out)
     assert np.array_equal(out.get(), np.zeros((3, 8)))
     ops("Microscale", "float").quantise(f(0, 40), ctx.empty((0, 32), np.uint8), ctx.empty((0, 2), np.uint8))
+
+
+def test_weights_of_rows_without_columns_have_a_gradient_of_zero(A, ctx, ops):
+    say("combine", "no columns")
+    op = ops("Combiner", "float")
+    place, weights = ctx.array(np.arange(6, dtype=np.int32).reshape(3, 2)), ctx.array(np.ones((3, 2), np.float32))
+    dw = ctx.array(np.full((3, 2), np.nan, np.float32))
+    empty = lambda rows: ctx.empty((rows, 0), np.float32)
+    op.gradient(empty(3), empty(6), place, weights, empty(6), dw)
+    assert np.array_equal(dw.get(), np.zeros((3, 2), np.float32))
+    op.combine(empty(6), place, weights, empty(3))
