@@ -143,7 +143,7 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
       }
 #else
       if (!FAST && EVEN && q > 0) continue;
-      /* (a row that does not count: the operand's first; what comes of it is not written) */
+      /* (a row that does not count: the operand's first, which there is where there are steps at all; what comes of it is not written) */
       offset[q] = FAST ? acc_max(number(m), 0) * stride + column * SIZE : element(s) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
 #endif
     }
@@ -181,7 +181,7 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
       const unsigned char *p;
       if (FAST) p = base + (long long)r * SIZE + offset[q];
       else if (LIST == OP_PLAIN) p = base + (r + (EVEN ? q * APART : 0)) * stride + offset[EVEN ? 0 : q];
-      else p = base + acc_max(LIST == OP_GATED ? r + major(s) : named, 0) * stride + offset[EVEN ? 0 : q];
+      else p = base + (named < 0 ? 0 : LIST == OP_GATED ? r + major(s) : named) * stride + offset[EVEN ? 0 : q];
       v = ((const op_loose<op_mem> *)p)->v;
       if (!FAST && LIST != OP_PLAIN && named < 0) v = acc_u4{0, 0, 0, 0};
       return;
@@ -384,6 +384,8 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
    * twice, to the same value, and no chunk reaches beyond its row) */
   if (OP_OUTER) i0 = acc_max(0, acc_min(i0, p.ni - OP_BM));
   if (!OP_B_FAST) j0 = acc_max(0, acc_min(j0, p.nj - OP_BN));
+  /* (rows of an operand that has none: there is nothing to add up, and no first row to read in their place) */
+  if ((OP_INDEX == 1 ? p.b_rows : p.a_rows) < 1) r1 = r0;
 #endif
   op_a a;
   op_b b;
@@ -562,9 +564,12 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
       if (a.whole(r) & b.whole(r)) {                                                        \
         _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, named[n], true);  \
         _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, named[n], true);  \
-      } else {                                                                              \
+      } else if ((r) < r1) {                                                                \
         _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, named[n], false); \
         _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, named[n], false); \
+      } else {                                                                              \
+        _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) va[n] = acc_u4{0, 0, 0, 0};  \
+        _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) vb[n] = acc_u4{0, 0, 0, 0};  \
       }                                                                                     \
       look((r) + OP_STEP);                                                                  \
       ask_scales(r);                                                                        \

@@ -342,6 +342,40 @@ def test_a_sum_of_no_products_is_zero(A, ctx, ops):
     assert np.array_equal(out.get(), np.zeros((6, 5)))
 
 
+@pytest.mark.parametrize("order", ["ij", "ji"])
+@pytest.mark.parametrize("elt,rows,ni,nj", [("float", 1049, 999, 131), ("bfloat16", 2086, 1005, 260)])
+def test_no_row_behind_the_last_one_is_read(A, ctx, ops, elt, rows, ni, nj, order):
+    """both operands end where an allocation of 2 MB pages does, but for less than a row; the last segment ends amid a step, and an
+    index names the other operand's rows"""
+    say("outer, at the end", elt, rows, ni, nj, order)
+    rng = np.random.default_rng(rows)
+    a = store(rng.integers(-4, 5, (rows, ni)).astype(float), elt)
+    assert 0 <= -a.nbytes % (2 << 20) < a.nbytes // rows
+    b = store(rng.integers(-4, 5, (rows // 2, nj)).astype(float), elt)
+    offsets, index = np.array([0, 31, 900, rows], np.int32), rng.integers(0, rows, rows).astype(np.int32)
+    out = Boxed(A, ctx, np.zeros((3, ni, nj), STORED[elt]), elt, 0, 0, 7.0, swap=order == "ji")
+    ops("Product", elt).outer(ctx.array(a), ctx.array(b), ctx.array(offsets), out.array, index=ctx.array(index), per=2)
+    want, _ = plain_outer(values(a, elt), values(b, elt), offsets, 3, index, 2)
+    assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
+
+
+@pytest.mark.parametrize("elt", TYPES)
+@pytest.mark.parametrize("n,k", [(40, 64), (37, 33), (300, 130), (3, 2)])
+def test_an_index_of_an_operand_without_rows_names_none(A, ctx, ops, elt, n, k):
+    say("no rows", elt, n, k)
+    rows, offsets, index = 70, ctx.array(np.array([0, 30, 70], np.int32)), ctx.array(np.arange(70, dtype=np.int32))
+    none = A.Strided((0, k), (k, 1), 0)
+    out = Boxed(A, ctx, np.ones((rows, n), STORED[elt]), elt, 0, 0, 7.0)
+    for order in ("nk", "kn"):
+        w = Boxed(A, ctx, store(np.full((2, n, k), np.inf), elt), elt, swap=order == "kn")
+        ops("Product", elt).rows(none, w.array, offsets, out.array, index=index)
+        assert np.array_equal(values(out.get(), elt), np.zeros((rows, n)))
+    for order in ("ij", "ji"):
+        dw = Boxed(A, ctx, np.ones((2, n, k), STORED[elt]), elt, 0, 0, 7.0, swap=order == "ji")
+        ops("Product", elt).outer(ctx.array(store(np.full((rows, n), np.inf), elt)), none, offsets, dw.array, index=index)
+        assert np.array_equal(values(dw.get(), elt), np.zeros((2, n, k)))
+
+
 # ------------------------------------------------------------------------------ the router
 
 def plain_route(logits, choose, normalise):
