@@ -35,6 +35,7 @@ struct OpSpec {
   int choose = 0;
   bool normalise = true;
   int ahead = 3, once = 0;      // knobs product.ahead and product.once of the form for a few rows
+  int split_below = 192, split_groups = 512, split_steps = 8;
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
@@ -47,8 +48,8 @@ int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 // product: tile shapes, in waves of 64 lanes
 struct ProductTile { int bm, bn, wm, wn; };
-const ProductTile kProductTiles[] = {{32, 64, 2, 2}, {64, 128, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}, {16, 32, 1, 4}, {16, 64, 1, 4}};
-constexpr int kProductTileCount = 6, kLow = 0, kSkinny = 4;      // the last two: op_skinny.h
+const ProductTile kProductTiles[] = {{32, 64, 2, 2}, {64, 64, 2, 2}, {64, 128, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}, {16, 32, 1, 4}, {16, 64, 1, 4}};
+constexpr int kProductTileCount = 7, kLow = 0, kSquare = 1, kWide = 2, kMiddle = 3, kLarge = 4, kSkinny = 5;      // the last two: op_skinny.h
 struct ProductVariant {
   int tile = 0;
   bool outer = false, b_fast = true, aligned = true;
@@ -137,6 +138,17 @@ std::vector<std::string> op_options()
 }
 
 // every translation unit an instance may need: the build check compiles them all
+// whether products of this form come in that tile
+bool has_tile(const OpSpec &sp, const ProductVariant &v, int t)
+{
+  const bool wide = sp.kind == ACC_OP_MICRO, word = !wide && sp.type == 0;
+  if (t >= kSkinny) return !v.outer && v.aligned && v.b_fast && (t == kSkinny || (!wide && !word));
+  if (t == kLarge) return v.aligned && !word;
+  if (t == kMiddle) return v.outer || !word;
+  if (t == kWide) return !v.outer && !word;
+  return t == kSquare ? v.outer || word : !v.outer;
+}
+
 std::vector<std::string> all_sources(const OpSpec &sp)
 {
   std::vector<std::string> out;
@@ -150,7 +162,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         v.aligned = v.outer ? form % 3 == 0 : form < 2;
         v.tiny = v.outer ? form % 3 == 2 : form >= 4;
         v.index = v.outer ? (form - 6) / 3 : 0;
-        if ((v.outer && (t < 2 || t >= kSkinny)) || (!v.aligned && t > 2) || (t >= kSkinny && !v.b_fast)) continue;
+        if (!has_tile(sp, v, t)) continue;
         out.push_back(product_source(sp, v));
       }
   } else if (sp.kind == ACC_OP_ROUTE) {
@@ -166,7 +178,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         ProductVariant v;
         v.tile = t;
         v.aligned = aligned;
-        if (!v.aligned && t > 2) continue;
+        if (!has_tile(sp, v, t)) continue;
         out.push_back(product_source(sp, v));
       }
   }
@@ -314,24 +326,56 @@ bool near_enough(const acc_strided &a, int rows_dim, int64_t row, int bytes, boo
 // the knob's tile, where the form has it
 int tile_of(const OpSpec &sp, const ProductVariant &v, int tile)
 {
-  const bool there = sp.tile >= (v.outer ? 2 : 0) && sp.tile < (v.outer || !v.b_fast ? kSkinny : kProductTileCount) && (v.aligned || sp.tile < 3);
-  return there ? sp.tile : tile;
+  return sp.tile >= 0 && sp.tile < kProductTileCount && has_tile(sp, v, sp.tile) ? sp.tile : tile;
 }
 
 // the tile shape for products of `rows` rows of `experts` segments
-int rows_tile(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, bool aligned, bool b_fast)
+int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t n)
 {
   const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
   const bool wide = sp.kind == ACC_OP_MICRO, word = !wide && sp.type == 0;
+  const auto groups = [&](int t) {
+    return std::max(ceil_div(rows, kProductTiles[t].bm), std::min(rows, experts)) * ceil_div(n, kProductTiles[t].bn);
+  };
   // matrices that a few workgroups would read alone, and those for a few rows of 16 bits each: see op_skinny.h
-  if (aligned && b_fast && mean <= 12) {
-    const bool few = std::min(rows, experts) * ceil_div(n, 64) < 192;
-    if (few) return kSkinny;
+  if (v.aligned && v.b_fast && mean <= 12) {
+    if (std::min(rows, experts) * ceil_div(n, 64) < 192) return kSkinny;
     if (!wide && !word) return kSkinny + 1;
   }
-  if (mean <= 24) return kLow;
-  if (mean <= 96 || word) return 1;
-  return !aligned || mean < 512 || n < 256 ? 2 : 3;
+  if (word) return groups(kSquare) >= 1024 ? kSquare : kLow;
+  if (v.aligned && n >= 256 && groups(kLarge) >= 128 && mean > (wide ? 48 : 128)) return kLarge;
+  if (groups(kMiddle) >= 256 && mean > 64) return kMiddle;
+  if (groups(kWide) >= 256 && mean > (wide ? 12 : 32)) return kWide;
+  return kLow;
+}
+
+// A sum of `length` elements (steps of `step`) over `groups` workgroups' tiles, cut into pieces that fill the target: elements
+// of a piece, or 0 where one does.
+int32_t rows_piece(const OpSpec &sp, const ProductVariant &v, int64_t groups, int64_t length, int64_t step)
+{
+  if (v.tile >= kSkinny || groups >= sp.split_below) return 0;
+  const int64_t steps = ceil_div(length, step), least = sp.split_steps;
+  const int64_t each = std::max(least, ceil_div(steps * groups, sp.split_groups));
+  return each * 2 > steps ? 0 : (int32_t)(each * step);
+}
+
+// outer: the tile shape, and the rows of a piece (0: segments are not cut).  A tile is worth its size where there are
+// enough of them, cut as short as pays, to fill the target.
+int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t ni, int64_t nj)
+{
+  const auto groups = [&](int t, int64_t steps) {
+    const int64_t tiles = ceil_div(ni, kProductTiles[t].bm) * ceil_div(nj, kProductTiles[t].bn), least = steps * 128 / type_bytes(sp.type);
+    return tiles * std::max(experts, rows / least);
+  };
+  if (has_tile(sp, v, kLarge) && rows < (1 << 28) && ni >= 256 && nj >= 256 && groups(kLarge, 16) >= 128) return kLarge;
+  return groups(kMiddle, 8) >= (sp.type == 0 ? 1024 : 256) ? kMiddle : kSquare;
+}
+int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t tiles)
+{
+  const int64_t target = v.tile == kLarge ? 256 : v.tile == kMiddle ? 512 : 1024, step = 128 / type_bytes(sp.type);
+  if (experts * tiles >= target) return 0;
+  const int64_t least = (v.tile == kLarge ? 16 : 8) * step, piece = ceil_div(std::max(least, ceil_div(rows * tiles, target - experts * tiles)), step) * step;
+  return experts * piece >= 2 * rows ? 0 : (int32_t)piece;
 }
 
 }  // namespace
@@ -373,7 +417,7 @@ std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_s
 constexpr uint32_t kMicroElements = 1024;            // (above the products' keys)
 std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & kMicroElements) ? micro_source(sp, key & 1u) : product_source_of(sp, key); }
 
-const char *const kProductNames[] = {"product", "product_places"};
+const char *const kProductNames[] = {"product", "product_join", "product_places"};
 const char *const kRouteNames[] = {"route", "route_place", "route_gradient"};
 const char *const kCombineNames[] = {"combine", "combine_gradient"};
 const char *const kMicroNames[] = {"micro_quantise", "micro_values"};
@@ -447,6 +491,9 @@ try {
   op->spec.ahead = ctx->tuning_now()->get("product.ahead", sp.ahead);
   op->spec.once = ctx->tuning_now()->get("product.once", sp.once);
   op->spec.tile = ctx->tuning_now()->get("product.tile", -1);
+  op->spec.split_below = ctx->tuning_now()->get("product.split_below", sp.split_below);
+  op->spec.split_groups = ctx->tuning_now()->get("product.split_groups", sp.split_groups);
+  op->spec.split_steps = ctx->tuning_now()->get("product.split_steps", sp.split_steps);
   *out = op;
   return ACC_OK;
 } ACC_OP_CATCH("acc_op_create")
@@ -489,6 +536,26 @@ try {
 
 // ---- products -----------------------------------------------------------------------
 
+// the tiles of all rows, and their sums in pieces where they are too few
+static int launch_rows(acc_op op, const char *who, const ProductVariant &v, const OpVariant *var, acc_product_args &a, acc_stream stream)
+{
+  const ProductTile &t = kProductTiles[v.tile];
+  const int64_t step = 128 / (op->spec.kind == ACC_OP_MICRO ? 1 : type_bytes(op->spec.type));
+  a.tiles_i = (int32_t)tiles_at_most(a.rows, a.experts, t.bm);
+  a.tiles_j = (int32_t)ceil_div(a.nj, t.bn);
+  const int64_t groups = std::max(ceil_div(a.rows, t.bm), std::min<int64_t>(a.rows, a.experts)) * a.tiles_j, grid = (int64_t)a.tiles_i * a.tiles_j;
+  a.piece = rows_piece(op->spec, v, groups, a.k, step);
+  a.pieces = a.piece ? (int32_t)ceil_div(a.k, a.piece) : 1;
+  if (!a.piece) return launch(op, who, var->fn, grid, 64 * t.wm * t.wn, 0, stream, a);
+  acc::ScratchRef scratch;
+  ACC_TRY(op->ctx->scratch_acquire((size_t)a.pieces * a.rows * a.nj * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+  a.parts = static_cast<float *>(scratch.ptr);
+  int rc = launch(op, who, var->fn, grid * a.pieces, 64 * t.wm * t.wn, 0, stream, a);
+  if (rc == ACC_OK) rc = launch(op, who, var->fn2, ceil_div(a.rows * ceil_div(a.nj, 4), 256), 256, 0, stream, a);
+  op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));
+  return rc;
+}
+
 int acc_exec_product_rows(acc_op op, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
                           const acc_strided *out, acc_stream stream)
 try {
@@ -517,10 +584,9 @@ try {
   v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
               near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
   v.tiny = !v.aligned && (k < epc || (!v.b_fast && n < epc));
-  v.tile = tile_of(op->spec, v, rows_tile(op->spec, rows, experts, n, v.aligned, v.b_fast));
+  v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n));
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(v.key(), kProductNames, 1, product_source_of, &var));
-  const ProductTile &t = kProductTiles[v.tile];
+  ACC_TRY(op->variant(v.key(), kProductNames, v.tile >= kSkinny ? 1 : 2, product_source_of, &var));
   a.a = device<const void>(x);
   a.b = device<const void>(w);
   a.out = device<void>(out);
@@ -536,9 +602,7 @@ try {
   a.k = (int32_t)k;
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
-  a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
-  a.tiles_j = (int32_t)ceil_div(n, t.bn);
-  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+  return launch_rows(op, who, v, var, a, stream);
 } ACC_OP_CATCH("acc_exec_product_rows")
 
 int acc_exec_product_outer(acc_op op, const acc_strided *x, const acc_strided *y, const acc_strided *offsets, const acc_strided *index, int32_t per,
@@ -578,11 +642,11 @@ try {
   v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1) &&
               near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
   v.tiny = !v.aligned && (o.shape[1] < epc || o.shape[2] < epc);
-  v.tile = tile_of(op->spec, v, v.aligned && op->spec.type != 0 && rows < (1 << 28) && o.shape[1] >= 256 && o.shape[2] >= 256 && experts * ceil_div(o.shape[1], 256) * ceil_div(o.shape[2], 256) >= 128 ? 3 : 2);
+  v.tile = tile_of(op->spec, v, outer_tile(op->spec, v, rows, experts, o.shape[1], o.shape[2]));
   const OpVariant *var = nullptr;
   // (a tile of 256 x 256 has the rows that an index names looked up by a kernel in front: see OP_PLACES)
-  const bool places = v.index != 0 && v.aligned && kProductTiles[v.tile].bm == 256 && rows > 0;
-  ACC_TRY(op->variant(v.key(), kProductNames, v.index != 0 && v.aligned && kProductTiles[v.tile].bm == 256 ? 2 : 1, product_source_of, &var));
+  const bool looked_up = v.index != 0 && v.tile == kLarge, places = looked_up && rows > 0;
+  ACC_TRY(op->variant(v.key(), kProductNames, looked_up ? 3 : 2, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
   a.a = device<const void>(p);
   a.b = device<const void>(q);
@@ -602,15 +666,20 @@ try {
   set_divisor(per, &a);
   a.tiles_i = (int32_t)ceil_div(o.shape[1], t.bm);
   a.tiles_j = (int32_t)ceil_div(o.shape[2], t.bn);
+  a.piece = outer_piece(op->spec, v, rows, experts, (int64_t)a.tiles_i * a.tiles_j);
+  const int64_t runs = a.piece ? tiles_at_most(rows, experts, a.piece) : experts;
+  const size_t front = places ? ((size_t)rows * 4 + 255) / 256 * 256 : 0, bytes_of_parts = a.piece ? (size_t)runs * a.ni * a.nj * 4 : 0;
   acc::ScratchRef scratch;
   int rc = ACC_OK;
-  if (places) {
-    ACC_TRY(op->ctx->scratch_acquire((size_t)rows * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+  if (front + bytes_of_parts) {
+    ACC_TRY(op->ctx->scratch_acquire(front + bytes_of_parts, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
     a.places = static_cast<uint32_t *>(scratch.ptr);
-    rc = launch(op, who, var->fn2, ceil_div(rows, 256), 256, 0, stream, a);
+    a.parts = reinterpret_cast<float *>(static_cast<char *>(scratch.ptr) + front);
   }
-  if (rc == ACC_OK) rc = launch(op, who, var->fn, experts * a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
-  if (places) op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));
+  if (places) rc = launch(op, who, var->fn3, ceil_div(rows, 256), 256, 0, stream, a);
+  if (rc == ACC_OK) rc = launch(op, who, var->fn, runs * a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+  if (rc == ACC_OK && a.piece) rc = launch(op, who, var->fn2, experts * ceil_div((int64_t)a.ni * ceil_div(a.nj, 4), 256), 256, 0, stream, a);
+  if (front + bytes_of_parts) op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));
   return rc;
 } ACC_OP_CATCH("acc_exec_product_outer")
 
@@ -910,10 +979,9 @@ try {
     v.aligned = v.aligned && t->ptr % 4 == 0;
     for (int d = 0; d + 1 < t->rank; ++d) v.aligned = v.aligned && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
   }
-  v.tile = tile_of(op->spec, v, rows_tile(op->spec, rows, experts, n, v.aligned, v.b_fast));
+  v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n));
   const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(v.key(), kProductNames, 1, micro_source_of, &var));
-  const ProductTile &t = kProductTiles[v.tile];
+  ACC_TRY(op->variant(v.key(), kProductNames, v.tile >= kSkinny ? 1 : 2, micro_source_of, &var));
   a.a = device<const void>(xcodes);
   a.b = device<const void>(wcodes);
   a.a_scales = device<const uint8_t>(xscales);
@@ -934,9 +1002,7 @@ try {
   a.k = (int32_t)(16 * blocks);
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
-  a.tiles_i = (int32_t)tiles_at_most(rows, experts, t.bm);
-  a.tiles_j = (int32_t)ceil_div(n, t.bn);
-  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * t.wm * t.wn, 0, stream, a);
+  return launch_rows(op, who, v, var, a, stream);
 } ACC_OP_CATCH("acc_exec_micro_rows")
 
 }  // extern "C"

@@ -29,6 +29,8 @@ struct acc_product_args {
   int32_t experts;
   uint32_t per_mul, per_shift;  /* an index at is divided: (at * per_mul) >> (32 + per_shift); per_mul 0: it is not */
   int32_t tiles_i, tiles_j;     /* the grid's tiles */
+  int32_t piece, pieces;        /* a sum in pieces (0: in one): outer: of up to `piece` rows; rows: `pieces` of `piece` elements of k */
+  float *parts;                 /* their results */
   uint32_t *places;             /* outer, with an index, in large tiles: where the rows lie that it names, a number a row */
   const uint32_t *guard;
 };

@@ -57,12 +57,12 @@ ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi,
 
 /* four neighbours of a row of the result, from column j on, wherever it starts; `none`: of no row, whatever the sums say (a
  * matrix may hold infinities: no row times that is zeros all the same) */
-ACC_DEV void op_write4(op_elt *out, const int j, const int end, const acc_f4 c, const bool none)
+template <typename T> ACC_DEV void op_write4(T *out, const int j, const int end, const acc_f4 c, const bool none)
 {
-  struct __attribute__((packed, aligned(sizeof(op_elt)))) op_e4 { op_elt v[4]; };
+  struct __attribute__((packed, aligned(sizeof(T)))) op_e4 { T v[4]; };
   op_e4 e;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) e.v[t] = (op_elt)(none ? 0.0f : c[t]);
+  for (int t = 0; t < 4; ++t) e.v[t] = (T)(none ? 0.0f : c[t]);
   if (j + 4 <= end) {
     *(op_e4 *)(out + j) = e;
   } else {

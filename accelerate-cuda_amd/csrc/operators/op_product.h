@@ -78,7 +78,7 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
                                   * OP_LISTED: along r perhaps one, across r one; OP_GATED: the other operand's (a row without
                                   * a partner counts as none) */
   unsigned int per_mul, per_shift;
-  int limit;                     /* rows an index may name */
+  int limit;                     /* rows of the operand that an index may name; across r: rows that there are */
   int lo, hi;                    /* the rows that count: along r the i's, across it the r's */
   int extent;                    /* elements of a row that count, from `base` on */
   int column;                    /* along r: the lane's chunks' first element (the same of all of them) */
@@ -144,7 +144,7 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
 #else
       if (!FAST && EVEN && q > 0) continue;
       /* (a row that does not count: the operand's first, which there is where there are steps at all; what comes of it is not written) */
-      offset[q] = FAST ? acc_max(number(m), 0) * stride + column * SIZE : element(s) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
+      offset[q] = FAST ? acc_max(number(m), 0) * stride + column * SIZE : (element(s) < extent ? element(s) : 0) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
 #endif
     }
   }
@@ -171,9 +171,26 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
   }
 #else
   /* the same by way of registers: `load` asks, whoever has asked puts what has come into LDS a step later.  `whole`: every
-   * chunk of the step lies within its row (and across r, without an index, every row counts).  OP_TINY: a row is shorter than a
-   * chunk. */
-  ACC_DEV bool whole(const int r) const { return OP_TINY ? false : FAST ? r + OP_STEP <= extent : ((LIST != OP_PLAIN) | (r + OP_STEP <= hi)) & (extent >= TILE); }
+   * chunk of the step is read where it lies.  Along r, all of them end within their rows.  Across r, without an index every row
+   * counts; and a chunk that reaches beyond its row's end ends within the next one (what it holds of that makes results that
+   * are not written), so that none of the step's rows may be the operand's last.  OP_TINY: a row is shorter than a chunk. */
+  template <int N> ACC_DEV bool whole(const int r, const int (&named)[N]) const
+  {
+    if (OP_TINY) return false;
+    if (FAST) return r + OP_STEP <= extent;
+    bool inside = extent >= TILE;
+    if (!inside && stride >= 16) {
+      if (LIST == OP_LISTED) {
+        bool last = limit < 2;
+#pragma unroll
+        for (int q = 0; q < MINE; ++q) last |= named[q] == limit - 1;
+        inside = __ballot(last) == 0;
+      } else {
+        inside = r + OP_STEP < limit;
+      }
+    }
+    return inside & ((LIST != OP_PLAIN) | (r + OP_STEP <= hi));
+  }
   ACC_DEV void load(acc_u4 &v, const int tid, const int q, const int r, const int named, const bool whole) const
   {
     const int s = slot(tid, q);
@@ -339,18 +356,29 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 
   /* the tile, and the sum's range; every die has a run of tiles of its own, neighbours of which share operands */
   int expert, i0, j0, iend, jend, r0, r1;
+  float *part = (float *)0;     /* where a piece of a sum goes */
 #if OP_OUTER
   {
     /* (segments are of any length: the longest first, each on all dies) */
-    const int tiles = p.tiles_i * p.tiles_j;
-    expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, (int)(blockIdx.x / tiles));
+    const int tiles = p.tiles_i * p.tiles_j, n = (int)(blockIdx.x / tiles);
     int i, j;
+    if (p.piece == 0) {
+      expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, n);
+      op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
+    } else {
+      const op_tile run = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, p.piece, n);
+      if (run.expert < 0) return;
+      expert = run.expert;
+      op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
+      if (r1 - r0 > p.piece) part = p.parts + (long long)n * p.ni * p.nj;
+      r0 = run.begin;
+      r1 = run.end;
+    }
     op_grouped((int)op_die_run(blockIdx.x % tiles, tiles), p.tiles_i, p.tiles_j, OP_GROUP, &i, &j);
     i0 = i * OP_BM;
     j0 = j * OP_BN;
     iend = p.ni;
     jend = p.nj;
-    op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
   }
 #else
   {
@@ -358,14 +386,15 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
      * that there are, are shared out evenly.) */
     int whole, rest, i, j;
     op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM, &whole, &rest);
+    const unsigned int grid = (unsigned int)(p.tiles_i * p.tiles_j), n = p.piece ? blockIdx.x / grid : 0u, at = blockIdx.x - n * grid;
     const long long first = (long long)whole * p.tiles_j, all = first + (long long)rest * p.tiles_j;
-    if (blockIdx.x >= all) return;
+    if (at >= all) return;
     op_tile tile;
-    if (blockIdx.x < first) {
-      op_grouped((int)op_die_run(blockIdx.x, first), whole, p.tiles_j, OP_GROUP, &i, &j);
+    if (at < first) {
+      op_grouped((int)op_die_run(at, first), whole, p.tiles_j, OP_GROUP, &i, &j);
       tile = op_find_tile<OP_WHOLE>(p.offsets, p.experts, (int)p.rows, OP_BM, i);
     } else {
-      op_grouped((int)op_die_run(blockIdx.x - first, all - first), rest, p.tiles_j, OP_GROUP, &i, &j);
+      op_grouped((int)op_die_run(at - first, all - first), rest, p.tiles_j, OP_GROUP, &i, &j);
       tile = op_find_tile<OP_REST>(p.offsets, p.experts, (int)p.rows, OP_BM, i);
     }
     j0 = j * OP_BN;
@@ -376,6 +405,11 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     jend = p.nj;
     r0 = 0;
     r1 = expert < 0 ? 0 : p.k;
+    if (p.piece) {
+      part = p.parts + n * p.rows * p.nj;
+      r0 = acc_min(r1, (int)n * p.piece);
+      r1 = acc_min(r1, r0 + p.piece);
+    }
   }
 #endif
 
@@ -399,7 +433,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
   a.per_shift = b.per_shift = p.per_shift;
 #if OP_OUTER
   b.index = (const int *)0;
-  b.limit = 0;
+  b.limit = p.b_rows;
   a.lo = b.lo = r0;
   a.hi = b.hi = r1;
   a.base += (long long)i0 * op_a::SIZE;
@@ -411,7 +445,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #else
   b.base += acc_max(expert, 0) * p.b_expert * op_b::SIZE;
   b.index = (const int *)0;
-  b.limit = 0;
+  b.limit = p.k;
   a.lo = i0;
   a.hi = iend;
   a.extent = p.k;
@@ -561,7 +595,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     acc_u4 va[op_a::MINE], vb[op_b::MINE];
 #define OP_LOAD(r)                                                                          \
     do {                                                                                    \
-      if (a.whole(r) & b.whole(r)) {                                                        \
+      if (a.whole(r, named) & b.whole(r, named)) {                                                        \
         _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) a.load(va[n], tid, n, r, named[n], true);  \
         _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) b.load(vb[n], tid, n, r, named[n], true);  \
       } else if ((r) < r1) {                                                                \
@@ -635,7 +669,64 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #else
     none = p.index_a && a.number(ri) < 0;
 #endif
+    if (part) {
 #pragma unroll
-    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none);
+      for (int j = 0; j < OP_FN; ++j) op_write4(part + (long long)ri * p.nj, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none);
+    } else {
+#pragma unroll
+      for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none);
+    }
   }
+}
+
+/* The pieces of a sum added up, in order; a lane has four neighbours of a row.  Outer: of the experts with more pieces than one, and
+ * zeros for those without rows. */
+extern "C" __global__ void __launch_bounds__(256) product_join(const acc_product_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  const int quads = (p.nj + 3) / 4;
+  op_elt *out = (op_elt *)p.out;
+  const float *from = p.parts;
+#if OP_OUTER
+  const int blocks = (int)(((long long)p.ni * quads + 255) / 256), expert = (int)(blockIdx.x / blocks), rows = p.ni;
+  const long long u = (long long)(blockIdx.x % blocks) * 256 + threadIdx.x, apart = (long long)p.ni * p.nj;
+  int begin, end, first = 0;
+  op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &begin, &end);
+  const int pieces = (end - begin + p.piece - 1) / p.piece;
+  if (pieces == 1) return;
+  for (int base = 0; base <= expert; base += 64) {
+    int b = 0, e = 0;
+    if (base + acc_lane() <= expert) op_segment(p.offsets, p.experts, (int)p.rows, base + acc_lane(), &b, &e);
+    first += acc_wave_reduce((e - b + p.piece - 1) / p.piece, [](int x, int y) { return x + y; });
+  }
+  from += first * apart;
+  out += (long long)expert * p.out_expert;
+#else
+  const long long u = (long long)blockIdx.x * 256 + threadIdx.x, apart = p.rows * p.nj, rows = p.rows;
+  const int pieces = p.pieces;
+#endif
+  const long long i = u / quads;
+  const int j = (int)(u - i * quads) * 4, left = acc_min(4, p.nj - j);
+  if (i >= rows) return;
+  from += i * p.nj + j;
+  acc_f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int n = 0; n < pieces; n += 4) {
+    struct __attribute__((packed, aligned(4))) op_f4 { float v[4]; } v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float *q = from + acc_min(n + k, pieces - 1) * apart;
+      if (left == 4) {
+        v[k] = *(const op_f4 *)q;
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[k].v[t] = t < left ? q[t] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < pieces)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) sum[t] += v[k].v[t];
+  }
+  op_write4(out + i * p.out_stride, j, p.nj, sum, false);
 }

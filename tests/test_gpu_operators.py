@@ -156,6 +156,11 @@ ROWS = [
     (2100, 2, 512, 200, "even", "nk", 0, 0, 0),
     (2100, 2, 300, 77, "gaps", "kn", 2, 5, 2),
     (3000, 1, 513, 130, "even", "nk", 2, 0, 8),
+    # few rows and columns, long sums: in pieces
+    (33, 3, 100, 2104, "even", "nk", 0, 0, 0),
+    (70, 2, 33, 2101, "gaps", "kn", 2, 0, 1),
+    (300, 1, 64, 1600, "even", "kn", 0, 0, 0),
+    (19, 5, 7, 4099, "skewed", "nk", 0, 1, 0),
 ]
 
 
@@ -195,6 +200,12 @@ OUTER = [
     (1000, 5, 256, 128, "skewed", "ij", 0, 0, 0),
     (260, 130, 264, 256, "even", "ij", 0, 0, 0),
     (400, 131, 257, 259, "skewed", "ji", 1, 3, 0),
+    # few results and long segments: sums in pieces
+    (5000, 2, 70, 90, "even", "ij", 0, 0, 0),
+    (3001, 3, 130, 264, "skewed", "ji", 2, 0, 0),
+    (2777, 70, 33, 5, "skewed", "ij", 1, 1, 2),
+    (4100, 1, 264, 256, "gaps", "ij", 2, 0, 0),
+    (9000, 4, 256, 512, "gaps", "ji", 0, 0, 0),
 ]
 
 
@@ -343,7 +354,7 @@ def test_a_sum_of_no_products_is_zero(A, ctx, ops):
 
 
 @pytest.mark.parametrize("order", ["ij", "ji"])
-@pytest.mark.parametrize("elt,rows,ni,nj", [("float", 1049, 999, 131), ("bfloat16", 2086, 1005, 260)])
+@pytest.mark.parametrize("elt,rows,ni,nj", [("float", 1049, 999, 131), ("bfloat16", 2086, 1005, 260), ("half", 17476, 60, 131)])
 def test_no_row_behind_the_last_one_is_read(A, ctx, ops, elt, rows, ni, nj, order):
     """both operands end where an allocation of 2 MB pages does, but for less than a row; the last segment ends amid a step, and an
     index names the other operand's rows"""
@@ -632,7 +643,7 @@ def test_four_bit_numbers(A, ctx, ops, elt, rows, k, lead, extra):
 
 
 @pytest.mark.parametrize("elt", TYPES)
-@pytest.mark.parametrize("rows,experts,n,k,kind,per", [(1, 1, 1, 1, "even", 0), (5, 3, 40, 70, "even", 2), (33, 8, 256, 128, "skewed", 0), (90, 2, 129, 544, "gaps", 3),
+@pytest.mark.parametrize("rows,experts,n,k,kind,per", [(60, 3, 130, 4000, "gaps", 0), (100, 2, 64, 4096, "even", 2), (1, 1, 1, 1, "even", 0), (5, 3, 40, 70, "even", 2), (33, 8, 256, 128, "skewed", 0), (90, 2, 129, 544, "gaps", 3),
                                                        (300, 4, 300, 1000, "skewed", 0), (1100, 2, 520, 256, "even", 2), (600, 1, 256, 1040, "gaps", 0)])
 def test_products_of_four_bit_numbers(A, ctx, ops, elt, rows, experts, n, k, kind, per):
     say("micro rows", elt, rows, experts, n, k, kind, per)
