@@ -330,7 +330,7 @@ int tile_of(const OpSpec &sp, const ProductVariant &v, int tile)
 }
 
 // the tile shape for products of `rows` rows of `experts` segments
-int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t n)
+int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t n, int64_t steps)
 {
   const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
   const bool wide = sp.kind == ACC_OP_MICRO, word = !wide && sp.type == 0;
@@ -343,7 +343,7 @@ int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t e
     if (!wide && !word) return kSkinny + 1;
   }
   if (word) return groups(kSquare) >= 1024 ? kSquare : kLow;
-  if (v.aligned && n >= 256 && groups(kLarge) >= 128 && mean > (wide ? 48 : 128)) return kLarge;
+  if (v.aligned && n >= 256 && steps >= 8 && groups(kLarge) >= 192 && mean > (wide ? 48 : 128)) return kLarge;
   if (groups(kMiddle) >= 256 && mean > 64) return kMiddle;
   if (groups(kWide) >= 256 && mean > (wide ? 12 : 32)) return kWide;
   return kLow;
@@ -584,7 +584,7 @@ try {
   v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
               near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
   v.tiny = !v.aligned && (k < epc || (!v.b_fast && n < epc));
-  v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n));
+  v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n, ceil_div(k * bytes, 128)));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, v.tile >= kSkinny ? 1 : 2, product_source_of, &var));
   a.a = device<const void>(x);
@@ -979,7 +979,7 @@ try {
     v.aligned = v.aligned && t->ptr % 4 == 0;
     for (int d = 0; d + 1 < t->rank; ++d) v.aligned = v.aligned && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
   }
-  v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n));
+  v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n, ceil_div(blocks, 8)));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, v.tile >= kSkinny ? 1 : 2, micro_source_of, &var));
   a.a = device<const void>(xcodes);

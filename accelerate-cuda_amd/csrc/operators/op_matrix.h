@@ -72,4 +72,37 @@ template <typename T> ACC_DEV void op_write4(T *out, const int j, const int end,
   }
 }
 
+/* Two neighbouring fragments of the result, columns j .. j + 31, of which a lane has four of either (g: its quarter of the wave).  Of
+ * 16 bits, quarters exchange halves first, so that a lane has eight neighbours, and four lanes half a cache line: with 8 bytes a
+ * lane, 230 MB of gradients took 97 us. */
+ACC_DEV void op_write_pair(op_elt *out, const int j, const int end, const int g, const acc_f4 c, const acc_f4 d, const bool none)
+{
+#if OP_ELT == 0
+  op_write4(out, j + 4 * g, end, c, none);
+  op_write4(out, j + 16 + 4 * g, end, d, none);
+#else
+  op_elt x[4], y[4];
+  unsigned int u[2], v[2];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    x[t] = (op_elt)(none ? 0.0f : c[t]);
+    y[t] = (op_elt)(none ? 0.0f : d[t]);
+  }
+  __builtin_memcpy(u, x, 8);
+  __builtin_memcpy(v, y, 8);
+  const auto lo = __builtin_amdgcn_permlane16_swap(u[0], v[0], false, false), hi = __builtin_amdgcn_permlane16_swap(u[1], v[1], false, false);
+  const acc_u4 all = {lo[0], hi[0], lo[1], hi[1]};
+  const int at = j + (g & 1) * 16 + (g >> 1) * 8;
+  if (at + 8 <= end) {
+    ((op_loose<op_elt> *)(out + at))->v = all;
+  } else {
+    op_elt e[8];
+    __builtin_memcpy(e, &all, 16);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (at + t < end) out[at + t] = e[t];
+  }
+#endif
+}
+
 #endif

@@ -674,7 +674,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
       for (int j = 0; j < OP_FN; ++j) op_write4(part + (long long)ri * p.nj, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none);
     } else {
 #pragma unroll
-      for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + wj + j * 16 + 4 * (lane >> 4), jend, c[i][j], none);
+      for (int j = 0; j < OP_FN; j += 2) op_write_pair(out, j0 + wj + j * 16, jend, lane >> 4, c[i][j], c[i][j + 1], none);
     }
   }
 }

@@ -120,6 +120,6 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) product(const acc_pr
     if (m >= tile.end) continue;
     op_elt *out = (op_elt *)p.out + (long long)m * p.out_stride;
 #pragma unroll
-    for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + j * 16 + 4 * g, p.nj, c[i][j], arow[i] < 0);
+    for (int j = 0; j < OP_FN; j += 2) op_write_pair(out, j0 + j * 16, p.nj, g, c[i][j], c[i][j + 1], arow[i] < 0);
   }
 }
