@@ -41,9 +41,22 @@ template <bool ALIGNED> ACC_DEV acc_u4 op_chunk(const op_elt *p, const int valid
  * row outside the array is ever named. */
 ACC_DEV void op_segment(const int *offsets, const int experts, const int rows, const int s, int *begin, int *end)
 {
-  const int b = s <= 0 ? 0 : offsets[s - 1], e = s > experts ? rows : offsets[s];
+  /* (both are read whether they count or not: two loads at once, and no branch) */
+  const int before = offsets[acc_max(s - 1, 0)], at = offsets[acc_min(s, experts)];
+  const int b = s <= 0 ? 0 : before, e = s > experts ? rows : at;
   *begin = acc_min(acc_max(b, 0), rows);
   *end = acc_max(*begin, acc_min(e, rows));
+}
+
+/* the lane's of 64 segments from number `base` on; behind the last one none */
+struct op_lot { int begin, end; };
+ACC_DEV op_lot op_segments(const int *offsets, const int experts, const int rows, const int base)
+{
+  const int s = base + acc_lane();
+  op_lot l;
+  op_segment(offsets, experts, rows, acc_min(s, experts + 1), &l.begin, &l.end);
+  if (s > experts + 1) l.end = l.begin;
+  return l;
 }
 
 /* Workgroups go to the eight dies in turn: block b of n as a number such that every die has a run of neighbours. */
@@ -62,34 +75,38 @@ ACC_DEV void op_grouped(const int x, const int ti, const int tj, const int heigh
   *j = y / here;
 }
 
-/* Whole tiles of `height` rows that the segments have, and segments that end amid another one. */
-ACC_DEV void op_count_tiles(const int *offsets, const int experts, const int rows, const int height, int *whole, int *parts)
+/* Whole tiles of `height` rows that the segments have, and segments that end amid another one.  `lot`: the first 64 segments. */
+ACC_DEV void op_count_tiles(const int *offsets, const int experts, const int rows, const int height, op_lot lot, int *whole, int *parts)
 {
-  const int lane = acc_lane();
   *whole = *parts = 0;
-  for (int base = 0; base < experts + 2; base += 64) {
-    int b = 0, e = 0;
-    if (base + lane < experts + 2) op_segment(offsets, experts, rows, base + lane, &b, &e);
-    *whole += acc_wave_reduce((e - b) / height, [](int x, int y) { return x + y; });
-    *parts += __popcll(__ballot((e - b) % height > 0));
+  for (int base = 0;;) {
+    *whole += acc_wave_reduce((lot.end - lot.begin) / height, [](int x, int y) { return x + y; });
+    *parts += __popcll(__ballot((lot.end - lot.begin) % height > 0));
+    base += 64;
+    if (base >= experts + 2) return;
+    lot = op_segments(offsets, experts, rows, base);
   }
 }
 
-/* The expert with the n-th longest segment, of up to 64 experts (of more: number n): what takes longest is begun first, and
- * the workgroups that are left at the end have little to do. */
-ACC_DEV int op_nth_longest(const int *offsets, const int experts, const int rows, const int n)
+/* The expert with the n-th longest segment, of up to 62 experts (of more: number n), and that: what takes longest is begun
+ * first, and the workgroups that are left at the end have little to do. */
+ACC_DEV int op_nth_longest(const int *offsets, const int experts, const int rows, const int n, int *begin, int *end)
 {
-  if (experts > 64) return n;
-  const int lane = acc_lane();
-  int b = 0, e = -1;
-  if (lane < experts) op_segment(offsets, experts, rows, lane + 1, &b, &e);
-  const int length = e - b;
-  int longer = 0;
-  for (int k = 0; k < experts; ++k) {
-    const int other = acc_readlane(length, k);
-    longer += (other > length) | ((other == length) & (k < lane));
+  if (experts > 62) {
+    op_segment(offsets, experts, rows, n + 1, begin, end);
+    return n;
   }
-  return __builtin_ctzll(__ballot((longer == n) & (lane < experts)) | 1ull << 63);
+  const op_lot lot = op_segments(offsets, experts, rows, 0);
+  const int s = acc_lane();
+  /* (no two of these are the same; a length beyond 2^26 counts as that) */
+  const unsigned int mine = s >= 1 && s <= experts ? (unsigned int)(acc_min(lot.end - lot.begin, (1 << 26) - 2) + 1) << 6 | (63 - s) : 0;
+  int longer = 0;
+#pragma unroll 4
+  for (int k = 1; k <= experts; ++k) longer += (unsigned int)acc_readlane((int)mine, k) > mine;
+  const int at = __builtin_ctzll(__ballot((longer == n) & (mine > 0)) | 1ull << 63);
+  *begin = acc_readlane(lot.begin, at);
+  *end = acc_readlane(lot.end, at);
+  return at - 1;
 }
 
 struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segment; begin >= end: no such tile */
@@ -101,14 +118,14 @@ struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segmen
 #define OP_REST 2
 
 /* The `tile`-th such run, counted segment after segment: a wave adds up the runs of 64 segments at a time.  Every wave of a
- * workgroup works it out for itself, and the answer is the same in every lane. */
-template <int KIND> ACC_DEV op_tile op_find_tile(const int *offsets, const int experts, const int rows, const int height, int tile)
+ * workgroup works it out for itself, and the answer is the same in every lane.  `lot`: the first 64 segments. */
+template <int KIND> ACC_DEV op_tile op_find_tile(const int *offsets, const int experts, const int rows, const int height, op_lot lot, int tile)
 {
   const int lane = acc_lane();
   op_tile t = {-1, 0, 0};
-  for (int base = 0; base < experts + 2; base += 64) {
-    int b = 0, e = 0;
-    if (base + lane < experts + 2) op_segment(offsets, experts, rows, base + lane, &b, &e);
+  for (int base = 0;;) {
+    int b = lot.begin;
+    const int e = lot.end;
     if (KIND == OP_REST) b = e - (e - b) % height;
     const int runs = KIND == OP_WHOLE ? (e - b) / height : (e - b + height - 1) / height;
     const int upto = acc_wave_scan(runs, [](int x, int y) { return x + y; }, lane);
@@ -122,8 +139,10 @@ template <int KIND> ACC_DEV op_tile op_find_tile(const int *offsets, const int e
       return t;
     }
     tile -= acc_readlane(upto, 63);
+    base += 64;
+    if (base >= experts + 2) return t;
+    lot = op_segments(offsets, experts, rows, base);
   }
-  return t;
 }
 
 #endif

@@ -46,13 +46,18 @@ ACC_DEV acc_f4 op_mfma_scaled(const op_frag &x, const op_frag &y, const acc_f4 c
 #define OP_NOWHERE 0x80000000u                     /* an offset beyond the end of every buffer: reads as zeros */
 #define OP_FARTHEST 0x7fffffffll                   /* the longest buffer */
 
-/* which row an index of rows lo .. hi - 1 names for row m, divided as the arguments say; -1: none */
-ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi, const int limit, const unsigned int per_mul, const unsigned int per_shift)
+/* what an index of rows lo .. hi - 1 says of row m (of one beside them: something), and which row that is, divided as the arguments
+ * say; -1: none */
+ACC_DEV int op_entry(const int *index, const int m, const int lo, const int hi) { return index[(unsigned int)acc_max(lo, acc_min(m, hi - 1))]; }
+ACC_DEV int op_named(const int at, const int m, const int lo, const int hi, const int limit, const unsigned int per_mul, const unsigned int per_shift)
 {
-  const int at = index[(unsigned int)acc_max(lo, acc_min(m, hi - 1))];
   /* (by nothing: per_mul is 0) */
   const int r = (int)(__umulhi((unsigned int)at, per_mul) >> per_shift) + (at & (per_mul ? 0 : -1));
   return (m >= lo) & (m < hi) & ((unsigned int)at < 0x80000000u) & (r < limit) ? r : -1;
+}
+ACC_DEV int op_listed(const int *index, const int m, const int lo, const int hi, const int limit, const unsigned int per_mul, const unsigned int per_shift)
+{
+  return op_named(op_entry(index, m, lo, hi), m, lo, hi, limit, per_mul, per_shift);
 }
 
 /* four neighbours of a row of the result, from column j on, wherever it starts; `none`: of no row, whatever the sums say (a

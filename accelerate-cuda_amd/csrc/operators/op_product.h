@@ -128,14 +128,27 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
       buffer = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, (int)acc_min<long long>(OP_FARTHEST, rows > 0 ? (rows - 1) * stride + (long long)extent * SIZE : 0), 0x00020000);
     }
 #endif
+    /* (an index is read of all rows at once: one after the other, four times its latency stood in front of a tile) */
+    int rows_of[MINE];
+    if (FAST && LIST != OP_PLAIN) {
+      if (index) {
+#pragma unroll
+        for (int q = 0; q < MINE; ++q) rows_of[q] = op_entry(index, first + major(slot(tid, q)), lo, hi);
+#pragma unroll
+        for (int q = 0; q < MINE; ++q) rows_of[q] = op_named(rows_of[q], first + major(slot(tid, q)), lo, hi, limit, per_mul, per_shift);
+      } else {
+#pragma unroll
+        for (int q = 0; q < MINE; ++q) rows_of[q] = first + major(slot(tid, q)) < hi ? first + major(slot(tid, q)) : -1;
+      }
+    }
 #pragma unroll
     for (int q = 0; q < MINE; ++q) {
-      const int s = slot(tid, q), m = first + major(s);
+      const int s = slot(tid, q), m = first + major(s), number = FAST && LIST != OP_PLAIN ? rows_of[q] : m < hi ? m : -1;
 #if OP_ALIGNED
       if (EVEN && q > 0) continue;
       if (FAST) {
         /* (without an index, the rows that do not count lie behind the buffer's end) */
-        const int r = LIST == OP_PLAIN ? m : number(m);
+        const int r = LIST == OP_PLAIN ? m : number;
         offset[q] = r < 0 ? OP_NOWHERE : (unsigned int)((LIST == OP_LISTED && index ? r : r - first) * (int)stride + element(s) * SIZE);
       } else {
         /* (columns beyond the result's: any will do) */
@@ -144,7 +157,7 @@ template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
 #else
       if (!FAST && EVEN && q > 0) continue;
       /* (a row that does not count: the operand's first, which there is where there are steps at all; what comes of it is not written) */
-      offset[q] = FAST ? acc_max(number(m), 0) * stride + column * SIZE : (element(s) < extent ? element(s) : 0) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
+      offset[q] = FAST ? acc_max(number, 0) * stride + column * SIZE : (element(s) < extent ? element(s) : 0) * SIZE + (LIST == OP_PLAIN ? major(s) * stride : 0);
 #endif
     }
   }
@@ -363,10 +376,9 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     const int tiles = p.tiles_i * p.tiles_j, n = (int)(blockIdx.x / tiles);
     int i, j;
     if (p.piece == 0) {
-      expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, n);
-      op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
+      expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, n, &r0, &r1);
     } else {
-      const op_tile run = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, p.piece, n);
+      const op_tile run = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, p.piece, op_segments(p.offsets, p.experts, (int)p.rows, 0), n);
       if (run.expert < 0) return;
       expert = run.expert;
       op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
@@ -385,17 +397,18 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     /* Whole tiles first, then those that end a segment, which take less long.  (The grid is for the worst lengths; the tiles
      * that there are, are shared out evenly.) */
     int whole, rest, i, j;
-    op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM, &whole, &rest);
+    const op_lot lot = op_segments(p.offsets, p.experts, (int)p.rows, 0);
+    op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM, lot, &whole, &rest);
     const unsigned int grid = (unsigned int)(p.tiles_i * p.tiles_j), n = p.piece ? blockIdx.x / grid : 0u, at = blockIdx.x - n * grid;
     const long long first = (long long)whole * p.tiles_j, all = first + (long long)rest * p.tiles_j;
     if (at >= all) return;
     op_tile tile;
     if (at < first) {
       op_grouped((int)op_die_run(at, first), whole, p.tiles_j, OP_GROUP, &i, &j);
-      tile = op_find_tile<OP_WHOLE>(p.offsets, p.experts, (int)p.rows, OP_BM, i);
+      tile = op_find_tile<OP_WHOLE>(p.offsets, p.experts, (int)p.rows, OP_BM, lot, i);
     } else {
       op_grouped((int)op_die_run(at - first, all - first), rest, p.tiles_j, OP_GROUP, &i, &j);
-      tile = op_find_tile<OP_REST>(p.offsets, p.experts, (int)p.rows, OP_BM, i);
+      tile = op_find_tile<OP_REST>(p.offsets, p.experts, (int)p.rows, OP_BM, lot, i);
     }
     j0 = j * OP_BN;
     if (tile.begin >= tile.end) return;
@@ -572,11 +585,15 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     put_scales(lds0);
     ask_scales(r0 + OP_STEP);
     look(r0 + OP_STEP);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int n = 0; n < ALL; ++n) bring(lds1, n, r0 + OP_STEP);
+    __builtin_amdgcn_sched_barrier(0);
+    /* the first step has come when no more than the second one's loads, which were asked for behind it, are under way */
+    __builtin_amdgcn_s_waitcnt((ALL & 15) | 7 << 4 | (ALL >> 4) << 14);
+    op_meet(false);
     put_scales(lds1);
     ask_scales(r0 + 2 * OP_STEP);
-    op_meet(true);
     first();
     /* the step at r lies in `here`, the fragments of its first half in fa, fb */
     const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
