@@ -55,7 +55,8 @@ struct ProductVariant {
   bool outer = false, b_fast = true, aligned = true;
   bool tiny = false;            // not aligned: a row is shorter than 16 bytes
   int index = 0;                // outer: whose rows an index names: 1 b's, 2 a's
-  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u) | (uint32_t)index << 7 | (tiny ? 512u : 0u); }
+  bool places = false;          // ... which a kernel in front has looked up
+  uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u) | (uint32_t)index << 7 | (tiny ? 512u : 0u) | (places ? 2048u : 0u); }
 };
 
 std::string product_source(const OpSpec &sp, const ProductVariant &v)
@@ -72,8 +73,9 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
   }
   std::snprintf(text, sizeof(text),
                 "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_BN %d\n#define OP_WM %d\n#define OP_WN %d\n#define OP_OUTER %d\n"
-                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#define OP_INDEX %d\n#define OP_TINY %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
-                sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0, v.index, v.tiny ? 1 : 0);
+                "#define OP_A_FAST %d\n#define OP_B_FAST %d\n#define OP_ALIGNED %d\n#define OP_INDEX %d\n#define OP_PLACES %d\n#define OP_TINY %d\n#include \"acc_hip_device.h\"\n#include \"op_product.h\"\n",
+                sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn, t.wm, t.wn, v.outer ? 1 : 0, v.outer ? 0 : 1, v.outer ? 0 : v.b_fast ? 1 : 0, v.aligned ? 1 : 0, v.index, v.places ? 1 : 0,
+                v.tiny ? 1 : 0);
   return text;
 }
 
@@ -163,6 +165,10 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         v.tiny = v.outer ? form % 3 == 2 : form >= 4;
         v.index = v.outer ? (form - 6) / 3 : 0;
         if (!has_tile(sp, v, t)) continue;
+        v.places = v.index != 0 && !v.tiny;
+        out.push_back(product_source(sp, v));
+        if (!v.places || t == kLarge) continue;
+        v.places = false;
         out.push_back(product_source(sp, v));
       }
   } else if (sp.kind == ACC_OP_ROUTE) {
@@ -367,7 +373,7 @@ int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t 
     const int64_t tiles = ceil_div(ni, kProductTiles[t].bm) * ceil_div(nj, kProductTiles[t].bn), least = steps * 128 / type_bytes(sp.type);
     return tiles * std::max(experts, rows / least);
   };
-  if (has_tile(sp, v, kLarge) && rows < (1 << 28) && ni >= 256 && nj >= 256 && groups(kLarge, 16) >= 128) return kLarge;
+  if (has_tile(sp, v, kLarge) && rows < (1 << 28) && ni >= 256 && nj >= 256 && groups(kLarge, 16) >= 256) return kLarge;
   return groups(kMiddle, 8) >= (sp.type == 0 ? 1024 : 256) ? kMiddle : kSquare;
 }
 int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t tiles)
@@ -401,6 +407,7 @@ std::string product_source_of(const OpSpec &sp, uint32_t key)
   v.aligned = key & 64u;
   v.index = (int)(key >> 7 & 3u);
   v.tiny = key & 512u;
+  v.places = key & 2048u;
   return product_source(sp, v);
 }
 std::string route_source_of(const OpSpec &sp, uint32_t key)
@@ -644,9 +651,12 @@ try {
   v.tiny = !v.aligned && (o.shape[1] < epc || o.shape[2] < epc);
   v.tile = tile_of(op->spec, v, outer_tile(op->spec, v, rows, experts, o.shape[1], o.shape[2]));
   const OpVariant *var = nullptr;
-  // (a tile of 256 x 256 has the rows that an index names looked up by a kernel in front: see OP_PLACES)
-  const bool looked_up = v.index != 0 && v.tile == kLarge, places = looked_up && rows > 0;
-  ACC_TRY(op->variant(v.key(), kProductNames, looked_up ? 3 : 2, product_source_of, &var));
+  // (Where an index names rows, a kernel in front looks them up once for all tiles: a launch, 3 us, for 8192 rows of 8 segments
+  // and 1024 x 1024 results 4 us less of 44, for 32768 and 4096 x 2048 in tiles of 128 x 128 328 of 976.  Tiles of 256 x 256 have no
+  // registers for anything else.)
+  v.places = v.index != 0 && !v.tiny && (v.tile == kLarge || rows >= 4096);
+  const bool places = v.places && rows > 0;
+  ACC_TRY(op->variant(v.key(), kProductNames, v.places ? 3 : 2, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];
   a.a = device<const void>(p);
   a.b = device<const void>(q);

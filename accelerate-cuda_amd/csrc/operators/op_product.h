@@ -346,7 +346,8 @@ ACC_DEV void op_meet(const bool loads)
   asm volatile("" ::: "memory");
 }
 
-#define OP_PLACES (OP_INDEX != 0 && OP_ALIGNED && OP_BM == 256)
+/* outer, OP_PLACES: where the rows lie that an index names, worked out once for all tiles (not OP_ALIGNED: their numbers, and one
+ * more; 0, as beyond the end, is none) */
 #if OP_PLACES
 extern "C" __global__ void __launch_bounds__(256) product_places(const acc_product_args p)
 {
@@ -354,7 +355,7 @@ extern "C" __global__ void __launch_bounds__(256) product_places(const acc_produ
   const int m = (int)(blockIdx.x * 256 + threadIdx.x);
   if (m >= p.rows) return;
   const int r = op_listed(OP_INDEX == 1 ? p.index_b : p.index_a, m, 0, (int)p.rows, OP_INDEX == 1 ? p.b_rows : p.a_rows, p.per_mul, p.per_shift);
-  p.places[m] = op_place_of(r, (int)(OP_INDEX == 1 ? p.b_stride : p.a_stride) * (int)sizeof(op_mem));
+  p.places[m] = OP_ALIGNED ? op_place_of(r, (int)(OP_INDEX == 1 ? p.b_stride : p.a_stride) * (int)sizeof(op_mem)) : (unsigned int)(r + 1);
 }
 #endif
 
@@ -495,7 +496,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #endif
     const auto look_at = [&](const int q, const int r) {
 #if OP_PLACES
-      if (q < op_a::MINE) named[q] = (int)__builtin_amdgcn_raw_buffer_load_b32(places, mine_at, (r + q * op_a::APART) * 4, 0);
+      if (q < op_a::MINE) named[q] = (int)__builtin_amdgcn_raw_buffer_load_b32(places, mine_at, (r + q * op_a::APART) * 4, 0) - (OP_ALIGNED ? 0 : 1);
 #elif OP_INDEX != 0
       static_assert(OP_BM == OP_BN, "a row for both");
       if (q < op_a::MINE) {
