@@ -53,7 +53,8 @@ constexpr int kProductTileCount = 7, kLow = 0, kSquare = 1, kWide = 2, kMiddle =
 struct ProductVariant {
   int tile = 0;
   bool outer = false, b_fast = true, aligned = true;
-  bool tiny = false;            // not aligned: a row is shorter than 16 bytes
+  bool fours = true;            // 4 bits, in the form for a few rows: scales are whole words of four
+  bool tiny = false;            // not aligned: a row is shorter than 16 bytes; 4 bits: it has fewer than four scales
   int index = 0;                // outer: whose rows an index names: 1 b's, 2 a's
   bool places = false;          // ... which a kernel in front has looked up
   uint32_t key() const { return (uint32_t)tile | (outer ? 16u : 0u) | (b_fast ? 32u : 0u) | (aligned ? 64u : 0u) | (uint32_t)index << 7 | (tiny ? 512u : 0u) | (places ? 2048u : 0u); }
@@ -144,7 +145,7 @@ std::vector<std::string> op_options()
 bool has_tile(const OpSpec &sp, const ProductVariant &v, int t)
 {
   const bool wide = sp.kind == ACC_OP_MICRO, word = !wide && sp.type == 0;
-  if (t >= kSkinny) return !v.outer && v.aligned && v.b_fast && (t == kSkinny || (!wide && !word));
+  if (t >= kSkinny) return !v.outer && v.aligned && v.fours && v.b_fast && (t == kSkinny || (!wide && !word));
   if (t == kLarge) return v.aligned && !word;
   if (t == kMiddle) return v.outer || !word;
   if (t == kWide) return !v.outer && !word;
@@ -180,10 +181,12 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   } else {
     for (bool aligned : {true, false}) out.push_back(micro_source(sp, aligned));
     for (int t = 0; t < kProductTileCount; ++t)
-      for (bool aligned : {true, false}) {
+      for (int form = 0; form < 4; ++form) {
         ProductVariant v;
         v.tile = t;
-        v.aligned = aligned;
+        v.aligned = form < 2;
+        v.tiny = form % 2 == 1;
+        if (v.tiny && t == kLarge) continue;
         if (!has_tile(sp, v, t)) continue;
         out.push_back(product_source(sp, v));
       }
@@ -344,14 +347,14 @@ int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t e
     return std::max(ceil_div(rows, kProductTiles[t].bm), std::min(rows, experts)) * ceil_div(n, kProductTiles[t].bn);
   };
   // matrices that a few workgroups would read alone, and those for a few rows of 16 bits each: see op_skinny.h
-  if (v.aligned && v.b_fast && mean <= 12) {
+  if (v.aligned && v.fours && v.b_fast && mean <= 12) {
     if (std::min(rows, experts) * ceil_div(n, 64) < 192) return kSkinny;
     if (!wide && !word) return kSkinny + 1;
   }
   if (word) return groups(kSquare) >= 1024 ? kSquare : kLow;
-  if (v.aligned && n >= 256 && steps >= 8 && groups(kLarge) >= 192 && mean > (wide ? 48 : 128)) return kLarge;
+  if (v.aligned && n >= 256 && (wide || steps > 8) && groups(kLarge) >= 192 && mean > (wide ? 48 : 128)) return kLarge;
   if (groups(kMiddle) >= 256 && mean > 64) return kMiddle;
-  if (groups(kWide) >= 256 && mean > (wide ? 12 : 32)) return kWide;
+  if (groups(kWide) >= 256 && (wide || mean > 32)) return kWide;
   return kLow;
 }
 
@@ -983,11 +986,13 @@ try {
   if (is_empty(*out)) return ACC_OK;
   ProductVariant v;
   // (codes lie on 16 bytes; scales are taken four at a time where every row of them starts on 4 bytes and is whole fours)
-  v.aligned = blocks % 4 == 0 && near_enough(*xcodes, 0, 16 * blocks, 1, index != nullptr) && near_enough(*wcodes, 1, 16 * blocks, 1, false) &&
+  v.fours = blocks % 4 == 0;
+  v.tiny = blocks < 4;
+  v.aligned = near_enough(*xcodes, 0, 16 * blocks, 1, index != nullptr) && near_enough(*wcodes, 1, 16 * blocks, 1, false) &&
               near_enough(*xscales, 0, blocks, 1, true) && near_enough(*wscales, 1, blocks, 1, true);
   for (const acc_strided *t : {xscales, wscales}) {
-    v.aligned = v.aligned && t->ptr % 4 == 0;
-    for (int d = 0; d + 1 < t->rank; ++d) v.aligned = v.aligned && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
+    v.fours = v.fours && t->ptr % 4 == 0;
+    for (int d = 0; d + 1 < t->rank; ++d) v.fours = v.fours && (t->shape[d] <= 1 || t->stride[d] % 4 == 0);
   }
   v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n, ceil_div(blocks, 8)));
   const OpVariant *var = nullptr;

@@ -525,30 +525,34 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
                                                          : p.b_scales + expert * p.b_scales_expert + acc_max(scale_row, 0) * p.b_scales_stride;
     const int scale_byte = (of_a ? op_a::CHUNKS * 16 : (OP_B_AT + op_b::CHUNKS) * 16) + (si / share * 64 + si % 16) * 4 + si % share / 16;
     const int scale_half = (of_a ? op_a::SCALE_WORDS : op_b::SCALE_WORDS) * 4;
+    struct __attribute__((packed)) op_word { unsigned int v; };
     unsigned int scale[2];
     const auto ask_scales = [&](const int r) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = r / 16 + 4 * h;
-#if OP_ALIGNED
-        /* (blocks are whole fours; behind the last one a scale of zeros, as the codes there) */
-        const unsigned int four = *(const unsigned int *)(scales + acc_min(k, blocks - 4));
-        scale[h] = k < blocks ? four : 0u;
-#else
+#if OP_TINY
+        /* (a row has fewer than four) */
         scale[h] = 0;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           const unsigned int one = scales[acc_min(k + n, blocks - 1)];
           scale[h] |= (k + n < blocks ? one : 0u) << (8 * n);
         }
+#else
+        /* four, wherever they start; beyond the row's end its last four, which are shifted into place when they have come */
+        scale[h] = ((const op_word *)(scales + acc_min(k, blocks - 4)))->v;
 #endif
       }
     };
-    const auto put_scales = [&](acc_u4 *lds) {
+    const auto put_scales = [&](acc_u4 *lds, const int r) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const int beyond = OP_TINY ? 0 : acc_max(0, r / 16 + 4 * h - (blocks - 4));
+        const unsigned int four = beyond < 4 ? scale[h] >> (8 * beyond) : 0u;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) ((unsigned char *)lds)[scale_byte + h * scale_half + n * 64] = (unsigned char)(scale[h] >> (8 * n));
+        for (int n = 0; n < 4; ++n) ((unsigned char *)lds)[scale_byte + h * scale_half + n * 64] = (unsigned char)(four >> (8 * n));
+      }
     };
 #define OP_SCALES_F fsa, fsb, gsa, gsb,
 #define OP_SCALES_G gsa, gsb, fsa, fsb,
@@ -556,7 +560,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #define OP_SCALES_F
 #define OP_SCALES_G
     const auto ask_scales = [](int) {};
-    const auto put_scales = [](acc_u4 *) {};
+    const auto put_scales = [](acc_u4 *, int) {};
 #endif
     const op_a::reader wa = op_a::reads(wi, lane);
     const op_b::reader wb = op_b::reads(wj, lane);
@@ -583,7 +587,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     ask_scales(r0);
 #pragma unroll
     for (int n = 0; n < ALL; ++n) bring(lds0, n, r0);
-    put_scales(lds0);
+    put_scales(lds0, r0);
     ask_scales(r0 + OP_STEP);
     look(r0 + OP_STEP);
     __builtin_amdgcn_sched_barrier(0);
@@ -593,7 +597,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     /* the first step has come when no more than the second one's loads, which were asked for behind it, are under way */
     __builtin_amdgcn_s_waitcnt((ALL & 15) | 7 << 4 | (ALL >> 4) << 14);
     op_meet(false);
-    put_scales(lds1);
+    put_scales(lds1, r0 + OP_STEP);
     ask_scales(r0 + 2 * OP_STEP);
     first();
     /* the step at r lies in `here`, the fragments of its first half in fa, fb */
@@ -602,7 +606,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
         look_at(i, r + 2 * OP_STEP);
       });
       op_meet(true);
-      put_scales(here);
+      put_scales(here, r + 2 * OP_STEP);
       ask_scales(r + 3 * OP_STEP);
       op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, OP_SCALES_G there, wa, wb, 0, [&](const int i) {
 #pragma unroll
@@ -626,20 +630,20 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
       look((r) + OP_STEP);                                                                  \
       ask_scales(r);                                                                        \
     } while (0)
-#define OP_STORE(lds)                                                                       \
+#define OP_STORE(lds, r)                                                                     \
     do {                                                                                    \
       _Pragma("unroll") for (int n = 0; n < op_a::MINE; ++n) lds[op_a::slot(tid, n)] = va[n];           \
       _Pragma("unroll") for (int n = 0; n < op_b::MINE; ++n) lds[OP_B_AT + op_b::slot(tid, n)] = vb[n]; \
-      put_scales(lds);                                                                      \
+      put_scales(lds, r);                                                                   \
     } while (0)
     look(r0);
     OP_LOAD(r0);
-    OP_STORE(lds0);
+    OP_STORE(lds0, r0);
     OP_LOAD(r0 + OP_STEP);
     op_meet(false);
     first();
     const auto round = [&](acc_u4 *here, acc_u4 *there, const int r) {
-      OP_STORE(there);
+      OP_STORE(there, r + OP_STEP);
       OP_LOAD(r + 2 * OP_STEP);
       op_half(c, fa, fb, ga, gb, OP_SCALES_F here, wa, wb, 1, nothing);
       op_meet(false);
@@ -655,7 +659,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
 #pragma unroll
         for (int q = 0; q < op_a::MINE; ++q) look_at(q, r + 2 * OP_STEP);
         op_meet(true);
-        put_scales(here);
+        put_scales(here, r + 2 * OP_STEP);
         ask_scales(r + 3 * OP_STEP);
 #pragma unroll
         for (int n = 0; n < ALL; ++n) bring(here, n, r + 2 * OP_STEP);
