@@ -88,17 +88,20 @@ struct RouteVariant {
 };
 constexpr int kRouteThreads = 1024, kRouteTallThreads = 256, kRouteMaxExperts = 2048;
 
-constexpr int64_t kRouteTallFrom = 16384;
-// The form with a lane a token is for tokens that fill the SIMDs with waves of 64, and up to eight choices.
+// The form with a lane a token is for tokens that fill the SIMDs with waves of 64, up to eight choices, and rows that are read
+// 16 bytes at a time: bfloat16, 8 of 128, 32768 tokens take 21 us with it and 25 without, 65536 24 and 40, but 16384 19 and 17.
+// (Float32, 4 of 64: 65536 tokens 23 and 24, 32768 21 and 15: its keys are twice as long.)
+constexpr int64_t kRouteTallFrom = 32768;
 RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned, int64_t tokens)
 {
   RouteVariant v;
-  v.tall = tokens >= kRouteTallFrom && sp.choose <= 8;
+
   const int epc = 16 / type_bytes(sp.type);
   while (v.lanes < 64 && v.lanes * v.per < experts) v.lanes *= 2;
   while (v.lanes * v.per < experts) v.per *= 2;
   v.vec = aligned && experts % epc == 0 ? epc : 1;
   v.sels = (sp.choose + v.lanes - 1) / v.lanes;
+  v.tall = v.vec > 1 && sp.choose <= 8 && tokens >= (sp.type == 0 ? 2 : 1) * kRouteTallFrom;
   return v;
 }
 
@@ -112,9 +115,14 @@ std::string route_source(const OpSpec &sp, const RouteVariant &v)
   return text;
 }
 
-// Tokens of a workgroup: at most 256 workgroups, each of which adds up the counts of all; up to 256 tokens go to one, which
-// places its slots itself (a launch less).
-int route_block(int64_t tokens) { return (int)(tokens <= 256 ? 256 : std::max<int64_t>(64, ceil_div(tokens, 256))); }
+// Tokens of a workgroup: what its waves take at once or up to 64, and more where that were more than 256 workgroups, each of
+// which reads the counts of all.  A single one places its slots itself, a launch less: 128 tokens of 16 experts take 6 us, in two
+// 9; 256 of 64 16 and 9.
+int route_block(const RouteVariant &v, int64_t tokens, int64_t experts)
+{
+  if (tokens * experts <= 8192) return (int)std::max<int64_t>(1, tokens);
+  return (int)std::max<int64_t>(std::min(64, kRouteThreads / v.lanes), ceil_div(tokens, 256));
+}
 
 constexpr int kCombineSlots = 4;
 // rows 0 anywhere, 1 aligned, 2 of fewer than eight elements
@@ -175,7 +183,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   } else if (sp.kind == ACC_OP_ROUTE) {
     for (int experts : {1, 8, 16, 32, 64, 128, 256, 512, 1024, 2048}) if (experts >= sp.choose)
       for (bool aligned : {true, false})
-        for (int64_t tokens : {int64_t(1), kRouteTallFrom}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
+        for (int64_t tokens : {int64_t(1), 2 * kRouteTallFrom}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
   } else {
@@ -742,7 +750,7 @@ try {
   a.experts = (int32_t)experts;
   a.choose = (int32_t)choose;
   a.normalise = op->spec.normalise ? 1 : 0;
-  a.block = route_block(tokens);
+  a.block = route_block(v, tokens, experts);
   a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, a.block));
   acc::ScratchRef scratch;
   if (a.blocks > 1) {

@@ -170,11 +170,13 @@ ACC_DEV int op_index_bits(const int experts) { return experts > 1 ? 32 - __built
 ACC_DEV void op_starts(const acc_route_args &p, int *counts, const int *base, const int tid)
 {
   for (int e = tid; e < p.experts; e += OP_THREADS) {
-    int at = base[e];
+    int at = base[e], n[OP_WAVES];
+#pragma unroll
+    for (int w = 0; w < OP_WAVES; ++w) n[w] = counts[w * p.experts + e];
+#pragma unroll
     for (int w = 0; w < OP_WAVES; ++w) {
-      const int n = counts[w * p.experts + e];
       counts[w * p.experts + e] = at;
-      at += n;
+      at += n[w];
     }
   }
   __syncthreads();
@@ -247,18 +249,11 @@ extern "C" __global__ void __launch_bounds__(256) route(const acc_route_args p)
         if (c < p.experts) next[i] = *(const op_vec *)(x + r * p.logits_stride + c);
       }
     };
-    if (OP_VEC > 1) ask(0);
+    ask(0);
     for (int c0 = 0; c0 < p.experts; c0 += OP_COLUMNS) {
-      if (OP_VEC > 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *(op_vec *)(tile + (i * 8 + lane / 8) * OP_APART + lane % 8 * 16) = next[i];
-        if (c0 + OP_COLUMNS < p.experts) ask(c0 + OP_COLUMNS);
-      } else {
-        const int c = c0 + lane % OP_COLUMNS;
-#pragma unroll 8
-        for (int r = lane / OP_COLUMNS; r < 64; r += 64 / OP_COLUMNS)
-          ((op_elt *)(tile + r * OP_APART))[lane % OP_COLUMNS] = c < p.experts ? x[acc_min(r, rows - 1) * p.logits_stride + c] : (op_elt)OP_NONE;
-      }
+      for (int i = 0; i < 8; ++i) *(op_vec *)(tile + (i * 8 + lane / 8) * OP_APART + lane % 8 * 16) = next[i];
+      if (c0 + OP_COLUMNS < p.experts) ask(c0 + OP_COLUMNS);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       for (int i = 0; i < 8; ++i) {
@@ -379,6 +374,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route(const acc_route_a
 
   for (int e = tid; e < p.experts; e += OP_THREADS) {
     int n = 0;
+#pragma unroll
     for (int w = 0; w < OP_WAVES; ++w) n += counts[w * p.experts + e];
     if (p.blocks > 1) p.counts[(long long)blockIdx.x * p.experts + e] = n;
     base[e] = 0;
@@ -411,21 +407,36 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route_place(const acc_r
     const int e = p.chosen[s];
     if (e >= 0) atomicAdd(&counts[wave * p.experts + e], 1);
   }
-  /* wave w adds up every OP_WAVES-th workgroup's counts, eight at a time on their way */
-  for (int e = lane; e < p.experts; e += 64) {
+  /* a wave adds up the counts of 64 experts, of every workgroup or of every few, 16 of them on their way at once */
+  const int lots = (p.experts + 63) / 64, shares = lots < OP_WAVES ? OP_WAVES / lots : 1;
+  for (int lot = wave % acc_min(lots, OP_WAVES); lot < lots; lot += OP_WAVES) {
+    const int e = lot * 64 + lane, mine_from = lots < OP_WAVES ? wave / lots : 0;
+    if (mine_from >= shares) break;
     int before = 0, total = 0;
-    for (int b = wave; b < p.blocks; b += 8 * OP_WAVES) {
-      int n[8];
+    /* (256 workgroups' counts of 2048 experts: offsets of 32 bits do) */
+    unsigned int at = (unsigned int)(mine_from * p.experts + acc_min(e, p.experts - 1));
+    const unsigned int apart = (unsigned int)(shares * p.experts);
+    int b = mine_from;
+    for (; b + 15 * shares < p.blocks; b += 16 * shares) {
+      int n[16];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) n[k] = b + k * OP_WAVES < p.blocks ? (int)p.counts[(long long)(b + k * OP_WAVES) * p.experts + e] : 0;
+      for (int k = 0; k < 16; ++k, at += apart) n[k] = (int)p.counts[at];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 16; ++k) {
         total += n[k];
-        before += b + k * OP_WAVES < (int)blockIdx.x ? n[k] : 0;
+        before += b + k * shares < (int)blockIdx.x ? n[k] : 0;
       }
     }
-    atomicAdd(&base[e], before);
-    atomicAdd(&sums[e], total);
+#pragma unroll 4
+    for (; b < p.blocks; b += shares, at += apart) {
+      const int n = (int)p.counts[at];
+      total += n;
+      before += b < (int)blockIdx.x ? n : 0;
+    }
+    if (e < p.experts) {
+      atomicAdd(&base[e], before);
+      atomicAdd(&sums[e], total);
+    }
   }
   __syncthreads();
   op_bases(p, base, sums, blockIdx.x == 0, tid, &all);
