@@ -34,8 +34,6 @@ struct OpSpec {
   int type = 0;                 // 0 float, 1 half, 2 bfloat16
   int choose = 0;
   bool normalise = true;
-  int ahead = 3, once = 0;      // knobs product.ahead and product.once of the form for a few rows
-  int split_below = 192, split_groups = 512, split_steps = 8;
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
@@ -46,7 +44,7 @@ int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 // ---- the variants of each kind ------------------------------------------------------
 
-// product: tile shapes, in waves of 64 lanes
+// product: tile shapes, in waves of 64 lanes.  Which a call takes is said at rows_tile and outer_tile.
 struct ProductTile { int bm, bn, wm, wn; };
 const ProductTile kProductTiles[] = {{32, 64, 2, 2}, {64, 64, 2, 2}, {64, 128, 2, 2}, {128, 128, 2, 2}, {256, 256, 2, 4}, {16, 32, 1, 4}, {16, 64, 1, 4}};
 constexpr int kProductTileCount = 7, kLow = 0, kSquare = 1, kWide = 2, kMiddle = 3, kLarge = 4, kSkinny = 5;      // the last two: op_skinny.h
@@ -65,11 +63,9 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
   const ProductTile &t = kProductTiles[v.tile];
   char text[512];
   if (v.tile >= kSkinny) {
-    // (the matrices' loads are marked as read once where they are: nontemporal.  Steps ahead: as many as 128 registers hold)
     std::snprintf(text, sizeof(text),
-                  "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_AHEAD %d\n#define OP_ONCE %d\n"
-                  "#include \"acc_hip_device.h\"\n#include \"op_skinny.h\"\n",
-                  sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn / 16, sp.ahead, sp.once);
+                  "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#include \"acc_hip_device.h\"\n#include \"op_skinny.h\"\n",
+                  sp.type, sp.kind == ACC_OP_MICRO ? 3 : sp.type, t.bm, t.bn / 16);
     return text;
   }
   std::snprintf(text, sizeof(text),
@@ -346,7 +342,21 @@ int tile_of(const OpSpec &sp, const ProductVariant &v, int tile)
   return sp.tile >= 0 && sp.tile < kProductTileCount && has_tile(sp, v, sp.tile) ? sp.tile : tile;
 }
 
-// the tile shape for products of `rows` rows of `experts` segments
+// The tile shape for products of `rows` rows of `experts` segments, of sums of `steps` cache lines.  A larger tile reads less
+// (an operand goes by once for every tile of the other's) and has more products for a load, a smaller one fills more compute
+// units; what a segment leaves over is a tile of its own.  Measured in us, 16 segments unless said:
+//   few rows (op_skinny.h): 16 rows, 8 of 1024 x 1024: 6.4 in columns of 32, 10 in tiles of 32 x 64; 64 rows, 32 of 4096 x 2048: 85 in
+//     columns of 32, 94 in those of 64, 121 in tiles; 128 rows of 4096 x 4096: 122, 107 and 128; Float32, 16 rows of 2048 x 2048: 45,
+//     52 in tiles.  4 bits only where the matrices are few: 32 rows of 4096 x 4096: 41 and 33 in tiles of 64 x 128
+//   Float32, bound by the matrix cores, wants them full to the end: 8192 rows, 8 of 1024 x 1536: 207 in 32 x 64 or 64 x 64, 225 in
+//     64 x 128, 270 in 128 x 128; 1024, 4 of 512 x 2048: 38, 37, 66, 124; 20000, 8 of 768 x 1024: 247, 233, 244, 244
+//   256 x 256 from 128 rows a segment on: 2048 rows of 4096 x 4096: 137 in 128 x 128, 141 in 256 x 256; 3072: 259 and 144; 4096: 227
+//     and 147.  Not for few tiles (8192 rows, 8 of 1024 x 1024, 128 tiles: 37 and 60) or short sums (16384, 8 of 2048 x 256: 36 and 41).
+//     4 bits already from 48 rows on, and for any sum: 1024 rows of 4096 x 4096: 42 and 39; 22272, 4 of 1976 x 44: 48 and 44
+//   128 x 128 from 64 rows on, 64 x 128 from 32, where there are 256 tiles: 1536 rows of 4096 x 2048: 104 in 64 x 128, 74 in
+//     128 x 128; 768: 97 in 32 x 64, 70 in 64 x 128; 512: 67 and 70; but 1024 of 1000 x 1000, with 128 tiles of 64 x 128: 13 and 16
+//   64 x 128 for long sums that 32 x 64 would not cut: 256 rows, 1 of 4096 x 4096: 28 in 32 x 64, 22 in pieces of 64 x 128
+constexpr int64_t kCutBelow = 192;                   // workgroups, see rows_piece
 int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t n, int64_t steps)
 {
   const int64_t mean = ceil_div(rows, std::max<int64_t>(1, experts));
@@ -354,30 +364,33 @@ int rows_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t e
   const auto groups = [&](int t) {
     return std::max(ceil_div(rows, kProductTiles[t].bm), std::min(rows, experts)) * ceil_div(n, kProductTiles[t].bn);
   };
-  // matrices that a few workgroups would read alone, and those for a few rows of 16 bits each: see op_skinny.h
   if (v.aligned && v.fours && v.b_fast && mean <= 12) {
-    if (std::min(rows, experts) * ceil_div(n, 64) < 192) return kSkinny;
-    if (!wide && !word) return kSkinny + 1;
+    if (word || std::min(rows, experts) * ceil_div(n, 64) < 192 || (!wide && steps <= 32)) return kSkinny;
+    if (!wide) return kSkinny + 1;
   }
   if (word) return groups(kSquare) >= 1024 ? kSquare : kLow;
   if (v.aligned && n >= 256 && (wide || steps > 8) && groups(kLarge) >= 192 && mean > (wide ? 48 : 128)) return kLarge;
   if (groups(kMiddle) >= 256 && mean > 64) return kMiddle;
   if (groups(kWide) >= 256 && (wide || mean > 32)) return kWide;
+  if (steps >= 48 && mean > 32 && groups(kLow) >= kCutBelow) return kWide;
   return kLow;
 }
 
-// A sum of `length` elements (steps of `step`) over `groups` workgroups' tiles, cut into pieces that fill the target: elements
-// of a piece, or 0 where one does.
-int32_t rows_piece(const OpSpec &sp, const ProductVariant &v, int64_t groups, int64_t length, int64_t step)
+// Sums of `length` elements, in steps of `step`, in fewer workgroups than kCutBelow are cut into pieces of eight steps or more
+// that make 512 of them, two a compute unit: elements of a piece, or 0 for one.  Another kernel adds the pieces up, 3 us.
+// 64 rows, 4 matrices of 1024 x 4096 bfloat16: 13 us and 28 uncut; 8 Float32 rows of 611 x 3059: 20 and 48; 1094 half rows, 2 of
+// 320 x 1005: 13 and 12.  (256 workgroups: 14, 22, 12; pieces of four steps: 13, 20, 13.)
+int32_t rows_piece(const ProductVariant &v, int64_t groups, int64_t length, int64_t step)
 {
-  if (v.tile >= kSkinny || groups >= sp.split_below) return 0;
-  const int64_t steps = ceil_div(length, step), least = sp.split_steps;
-  const int64_t each = std::max(least, ceil_div(steps * groups, sp.split_groups));
+  if (v.tile >= kSkinny || groups >= kCutBelow) return 0;
+  const int64_t steps = ceil_div(length, step), each = std::max<int64_t>(8, ceil_div(steps * groups, 512));
   return each * 2 > steps ? 0 : (int32_t)(each * step);
 }
 
-// outer: the tile shape, and the rows of a piece (0: segments are not cut).  A tile is worth its size where there are
-// enough of them, cut as short as pays, to fill the target.
+// Outer: the tile shape.  A tile is worth its size where there are enough of them, cut as short as pays, to fill the
+// compute units.  In us: 32000 rows, 16 bfloat16 results of 2048 x 2048: 246 in 256 x 256, 321 in 128 x 128; 8192, 8 of 1024 x 1024: 52
+// and 42, and 40 in 64 x 64; 1664, 13 of 800 x 2160: 38 in 64 x 64 and 33 in 128 x 128; 12416, 6 of 41 x 448: 25 and 41.  Float32:
+// 2240 rows, 15 of 3014 x 192: 48 in 64 x 64 and 83 in 128 x 128; 8192, 8 of 1024 x 1536: 209 and 203.
 int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t ni, int64_t nj)
 {
   const auto groups = [&](int t, int64_t steps) {
@@ -387,6 +400,8 @@ int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t 
   if (has_tile(sp, v, kLarge) && rows < (1 << 28) && ni >= 256 && nj >= 256 && groups(kLarge, 16) >= 256) return kLarge;
   return groups(kMiddle, 8) >= (sp.type == 0 ? 1024 : 256) ? kMiddle : kSquare;
 }
+// ... and the rows of a piece (0: segments are not cut), where whole segments make too few tiles to fill the compute units:
+// 17110 Float32 rows, 13 results of 64 x 64: 18 us and 369 uncut; 11200 bfloat16 rows, one of 3072 x 59: 22 and 590.
 int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t tiles)
 {
   const int64_t target = v.tile == kLarge ? 256 : v.tile == kMiddle ? 512 : 1024, step = 128 / type_bytes(sp.type);
@@ -506,12 +521,7 @@ try {
   acc_op_s *op = new acc_op_s();
   op->ctx = ctx;
   op->spec = sp;
-  op->spec.ahead = ctx->tuning_now()->get("product.ahead", sp.ahead);
-  op->spec.once = ctx->tuning_now()->get("product.once", sp.once);
   op->spec.tile = ctx->tuning_now()->get("product.tile", -1);
-  op->spec.split_below = ctx->tuning_now()->get("product.split_below", sp.split_below);
-  op->spec.split_groups = ctx->tuning_now()->get("product.split_groups", sp.split_groups);
-  op->spec.split_steps = ctx->tuning_now()->get("product.split_steps", sp.split_steps);
   *out = op;
   return ACC_OK;
 } ACC_OP_CATCH("acc_op_create")
@@ -562,7 +572,7 @@ static int launch_rows(acc_op op, const char *who, const ProductVariant &v, cons
   a.tiles_i = (int32_t)tiles_at_most(a.rows, a.experts, t.bm);
   a.tiles_j = (int32_t)ceil_div(a.nj, t.bn);
   const int64_t groups = std::max(ceil_div(a.rows, t.bm), std::min<int64_t>(a.rows, a.experts)) * a.tiles_j, grid = (int64_t)a.tiles_i * a.tiles_j;
-  a.piece = rows_piece(op->spec, v, groups, a.k, step);
+  a.piece = rows_piece(v, groups, a.k, step);
   a.pieces = a.piece ? (int32_t)ceil_div(a.k, a.piece) : 1;
   if (!a.piece) return launch(op, who, var->fn, grid, 64 * t.wm * t.wn, 0, stream, a);
   acc::ScratchRef scratch;
@@ -665,7 +675,7 @@ try {
   // (Where an index names rows, a kernel in front looks them up once for all tiles: a launch, 3 us, for 8192 rows of 8 segments
   // and 1024 x 1024 results 4 us less of 44, for 32768 and 4096 x 2048 in tiles of 128 x 128 328 of 976.  Tiles of 256 x 256 have no
   // registers for anything else.)
-  v.places = v.index != 0 && !v.tiny && (v.tile == kLarge || rows >= 4096);
+  v.places = v.index != 0 && !v.tiny && rows < (1 << 28) && (v.tile == kLarge || rows >= 4096);
   const bool places = v.places && rows > 0;
   ACC_TRY(op->variant(v.key(), kProductNames, v.places ? 3 : 2, product_source_of, &var));
   const ProductTile &t = kProductTiles[v.tile];

@@ -443,7 +443,8 @@ def router_logits(rng, tokens, experts, elt):
 
 
 ROUTE = [(1, 1, 1), (1, 4, 4), (8, 64, 4), (9, 7, 3), (12, 2, 1), (64, 8, 2), (255, 16, 2), (256, 60, 4), (257, 128, 8), (700, 33, 5), (1000, 256, 8), (300, 513, 6),
-         (40, 2048, 16), (530, 100, 64), (16400, 72, 8), (16384, 37, 3), (20011, 8, 1)]
+         (40, 2048, 16), (530, 100, 64), (16400, 72, 8), (16384, 37, 3), (20011, 8, 1),
+         (32768, 72, 8), (32801, 128, 7), (65537, 40, 4), (65600, 8, 1), (100, 512, 8), (515, 300, 3)]
 
 
 @pytest.mark.parametrize("elt", TYPES)
