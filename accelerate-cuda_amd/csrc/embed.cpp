@@ -38,6 +38,7 @@ ACC_EMBED(op_product, "operators/op_product.h")
 ACC_EMBED(op_skinny, "operators/op_skinny.h")
 ACC_EMBED(op_route, "operators/op_route.h")
 ACC_EMBED(op_combine, "operators/op_combine.h")
+ACC_EMBED(op_pack, "operators/op_pack.h")
 ACC_EMBED(op_micro, "operators/op_micro.h")
 
 namespace acc {
@@ -66,6 +67,7 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"op_product.h", acc_embed_op_product_begin, acc_embed_op_product_end},
       {"op_route.h", acc_embed_op_route_begin, acc_embed_op_route_end},
       {"op_combine.h", acc_embed_op_combine_begin, acc_embed_op_combine_end},
+      {"op_pack.h", acc_embed_op_pack_begin, acc_embed_op_pack_end},
       {"op_micro.h", acc_embed_op_micro_begin, acc_embed_op_micro_end},
   };
   return headers;

@@ -130,6 +130,13 @@ std::string combine_source(const OpSpec &sp, int rows)
   return text;
 }
 
+std::string pack_source(const OpSpec &sp)
+{
+  char text[128];
+  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#include \"acc_hip_device.h\"\n#include \"op_pack.h\"\n", sp.type);
+  return text;
+}
+
 std::string micro_source(const OpSpec &sp, bool aligned)
 {
   char text[256];
@@ -160,6 +167,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
 {
   std::vector<std::string> out;
   if (sp.kind == ACC_OP_PRODUCT) {
+    if (sp.type != 0) out.push_back(pack_source(sp));
     for (int t = 0; t < kProductTileCount; ++t)
       for (int form = 0; form < 15; ++form) {
         ProductVariant v;
@@ -424,8 +432,10 @@ struct acc_op_s {
 
 namespace {
 
+constexpr uint32_t kPack = 1u << 20;                 // (beside the products' keys)
 std::string product_source_of(const OpSpec &sp, uint32_t key)
 {
+  if (key == kPack) return pack_source(sp);
   ProductVariant v;
   v.tile = (int)(key & 15u);
   v.outer = key & 16u;
@@ -451,6 +461,7 @@ constexpr uint32_t kMicroElements = 1024;            // (above the products' key
 std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & kMicroElements) ? micro_source(sp, key & 1u) : product_source_of(sp, key); }
 
 const char *const kProductNames[] = {"product", "product_join", "product_places"};
+const char *const kPackNames[] = {"pack"};
 const char *const kRouteNames[] = {"route", "route_place", "route_gradient"};
 const char *const kCombineNames[] = {"combine", "combine_gradient"};
 const char *const kMicroNames[] = {"micro_quantise", "micro_values"};
@@ -564,6 +575,60 @@ try {
 
 // ---- products -----------------------------------------------------------------------
 
+// scratch memory until the call's kernels are enqueued
+struct ScratchHold {
+  acc_context ctx = nullptr;
+  hipStream_t stream = nullptr;
+  acc::ScratchRef ref;
+  int acquire(acc_op op, acc_stream s, size_t bytes)
+  {
+    ACC_TRY(op->ctx->scratch_acquire(bytes, static_cast<hipStream_t>(s), acc::SCRATCH_FOLD, &ref));
+    ctx = op->ctx;
+    stream = static_cast<hipStream_t>(s);
+    return ACC_OK;
+  }
+  ~ScratchHold() { if (ctx) ctx->scratch_release(ref, stream); }
+};
+
+// Whether operands of 16 bits that the aligned form cannot take are worth a copy that it can (op_pack.h): `count` copies move
+// `bytes` twice, at 4.8 TB/s and a launch each; what they save is, for every factor pair, 2.4 10^-15 s in gradients, 2.2 in
+// products of two such operands, 0.4 of one.  In us, as they lie and with the copies: 5000 half rows, 1 of 5001 x 5001: 475 and
+// 295; 4690 bfloat16 rows, 5 of 2021 x 3367: 184 and 157; 5760, 1 of 3557 x 1344, whose rows alone start anywhere: 88 and 92;
+// gradients: 8487 rows, 44 of 960 x 2722: 221 and 166.
+static bool worth_packing(const OpSpec &sp, const ProductVariant &v, double pairs, double bytes, int count)
+{
+  const double each = v.outer ? 2.4e-15 : count == 2 ? 2.2e-15 : 0.4e-15;
+  return sp.type != 0 && !v.tiny && count > 0 && bytes < 2e9 && pairs * each > 1.25 * (2 * bytes / 4.8e12 + 6e-6 * count);
+}
+
+// `from` ([batches,] rows, cols; `cols` contiguous) as rows of `cols_out` elements, rows_out of them a batch, at `to`
+static int pack(acc_op op, const char *who, const acc_strided &from, int cols_dim, int64_t rows_out, int64_t cols_out, uint64_t to, const uint32_t *guard, acc_stream stream, acc_strided *out)
+{
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(kPack, kPackNames, 1, product_source_of, &var));
+  const int rank = from.rank, rows_dim = cols_dim == rank - 1 ? rank - 2 : rank - 1;
+  acc_pack_args a = {};
+  a.in = device<const void>(&from);
+  a.out = reinterpret_cast<void *>(to);
+  a.batches = rank == 3 ? (uint32_t)from.shape[0] : 1u;
+  a.batch_stride = rank == 3 ? from.stride[0] : 0;
+  a.row_stride = from.stride[rows_dim];
+  a.rows = (uint32_t)from.shape[rows_dim];
+  a.rows_out = (uint32_t)rows_out;
+  a.cols = (int32_t)from.shape[cols_dim];
+  a.chunks = (uint32_t)(cols_out * type_bytes(op->spec.type) / 16);
+  set_divisor((int32_t)a.chunks, &a);
+  a.guard = guard;
+  *out = from;
+  out->ptr = to;
+  out->shape[rows_dim] = rows_out;
+  out->shape[cols_dim] = cols_out;
+  out->stride[cols_dim] = 1;
+  out->stride[rows_dim] = cols_out;
+  if (rank == 3) out->stride[0] = rows_out * cols_out;
+  return launch(op, who, var->fn, ceil_div((int64_t)a.batches * rows_out * a.chunks, 256), 256, 0, stream, a);
+}
+
 // the tiles of all rows, and their sums in pieces where they are too few
 static int launch_rows(acc_op op, const char *who, const ProductVariant &v, const OpVariant *var, acc_product_args &a, acc_stream stream)
 {
@@ -595,7 +660,8 @@ try {
   ACC_TRY(check_unit(who, "offsets", offsets, 1));
   ACC_TRY(check_result(who, "the result", out, 2));
   if (index) ACC_TRY(check_unit(who, "index", index, 1));
-  const int64_t experts = w->shape[0], n = w->shape[1], k = w->shape[2], rows = out->shape[0];
+  const int64_t experts = w->shape[0], n = w->shape[1], rows = out->shape[0];
+  int64_t k = w->shape[2];
   if (!unit(*w, 2) && !unit(*w, 1)) return fail(ACC_ERR_INVALID, "%s: neither the second nor the third dimension of w is contiguous", who);
   if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
   ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
@@ -609,9 +675,32 @@ try {
   ProductVariant v;
   // (where both are contiguous -- one column, or a sum of one -- either way of reading will do)
   v.b_fast = unit(*w, 2);
-  v.aligned = k % epc == 0 && aligned_rows(*x, bytes, 1) && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
-              near_enough(*x, 0, k * bytes, bytes, index != nullptr) && near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
+  const bool x_good = k % epc == 0 && aligned_rows(*x, bytes, 1) && near_enough(*x, 0, k * bytes, bytes, index != nullptr);
+  const bool w_good = k % epc == 0 && aligned_rows(*w, bytes, v.b_fast ? 2 : 1) && (v.b_fast || n % epc == 0) &&
+                      near_enough(*w, v.b_fast ? 1 : 2, (v.b_fast ? k : n) * bytes, bytes, false);
+  v.aligned = x_good && w_good;
   v.tiny = !v.aligned && (k < epc || (!v.b_fast && n < epc));
+  ScratchHold packed;
+  acc_strided xp, wp;
+  if (!v.aligned) {
+    // (all rows of x are copied: an index may name any)
+    const int64_t kp = ceil_div(k, epc) * epc, np = ceil_div(n, epc) * epc;
+    const int64_t xb = x_good ? 0 : x->shape[0] * kp * bytes, wb = w_good ? 0 : experts * (v.b_fast ? n : np) * kp * bytes, front = (xb + 255) / 256 * 256;
+    if (worth_packing(op->spec, v, (double)rows * (double)n * (double)k, (double)xb + (double)wb, (xb > 0) + (wb > 0))) {
+      ACC_TRY(packed.acquire(op, stream, (size_t)(front + wb)));
+      const uint64_t at = reinterpret_cast<uint64_t>(packed.ref.ptr);
+      if (xb) {
+        ACC_TRY(pack(op, who, *x, 1, x->shape[0], kp, at, a.guard, stream, &xp));
+        x = &xp;
+      }
+      if (wb) {
+        ACC_TRY(v.b_fast ? pack(op, who, *w, 2, n, kp, at + front, a.guard, stream, &wp) : pack(op, who, *w, 1, kp, np, at + front, a.guard, stream, &wp));
+        w = &wp;
+      }
+      k = kp;
+      v.aligned = true;
+    }
+  }
   v.tile = tile_of(op->spec, v, rows_tile(op->spec, v, rows, experts, n, ceil_div(k * bytes, 128)));
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kProductNames, v.tile >= kSkinny ? 1 : 2, product_source_of, &var));
@@ -667,9 +756,29 @@ try {
   v.outer = true;
   v.b_fast = false;
   v.index = !index ? 0 : turned ? 2 : 1;
-  v.aligned = p->shape[1] % epc == 0 && q->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && aligned_rows(*q, bytes, 1) &&
-              near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
+  const bool p_good = p->shape[1] % epc == 0 && aligned_rows(*p, bytes, 1) && near_enough(*p, 0, p->shape[1] * bytes, bytes, turned && index);
+  const bool q_good = q->shape[1] % epc == 0 && aligned_rows(*q, bytes, 1) && near_enough(*q, 0, q->shape[1] * bytes, bytes, !turned && index);
+  v.aligned = p_good && q_good;
   v.tiny = !v.aligned && (o.shape[1] < epc || o.shape[2] < epc);
+  ScratchHold packed;
+  acc_strided pp, qp;
+  if (!v.aligned) {
+    const int64_t ip = ceil_div(o.shape[1], epc) * epc, jp = ceil_div(o.shape[2], epc) * epc;
+    const int64_t pb = p_good ? 0 : p->shape[0] * ip * bytes, qb = q_good ? 0 : q->shape[0] * jp * bytes, front = (pb + 255) / 256 * 256;
+    if (worth_packing(op->spec, v, (double)rows * (double)ip * (double)jp, (double)pb + (double)qb, (pb > 0) + (qb > 0))) {
+      ACC_TRY(packed.acquire(op, stream, (size_t)(front + qb)));
+      const uint64_t at = reinterpret_cast<uint64_t>(packed.ref.ptr);
+      if (pb) {
+        ACC_TRY(pack(op, who, *p, 1, p->shape[0], ip, at, a.guard, stream, &pp));
+        p = &pp;
+      }
+      if (qb) {
+        ACC_TRY(pack(op, who, *q, 1, q->shape[0], jp, at + front, a.guard, stream, &qp));
+        q = &qp;
+      }
+      v.aligned = true;
+    }
+  }
   v.tile = tile_of(op->spec, v, outer_tile(op->spec, v, rows, experts, o.shape[1], o.shape[2]));
   const OpVariant *var = nullptr;
   // (Where an index names rows, a kernel in front looks them up once for all tiles: a launch, 3 us, for 8192 rows of 8 segments

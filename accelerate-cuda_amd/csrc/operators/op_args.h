@@ -35,6 +35,17 @@ struct acc_product_args {
   const uint32_t *guard;
 };
 
+/* an operand copied into rows of whole chunks: see op_pack.h */
+struct acc_pack_args {
+  const void *in;
+  void *out;                    /* batches x rows_out rows of `chunks` chunks */
+  int64_t batch_stride, row_stride;
+  uint32_t batches, rows, rows_out, chunks;
+  int32_t cols, pad;
+  uint32_t per_mul, per_shift;  /* a division by `chunks` */
+  const uint32_t *guard;
+};
+
 /* the router: see op_route.h */
 struct acc_route_args {
   const void *logits;

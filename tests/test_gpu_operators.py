@@ -353,6 +353,33 @@ def test_a_sum_of_no_products_is_zero(A, ctx, ops):
     assert np.array_equal(out.get(), np.zeros((6, 5)))
 
 
+@pytest.mark.parametrize("elt,order,lead,extra", [("half", "nk", 0, 0), ("half", "kn", 1, 2), ("bfloat16", "nk", 3, 8), ("bfloat16", "kn", 0, 0)])
+def test_large_products_of_rows_that_start_anywhere(A, ctx, ops, elt, order, lead, extra):
+    """operands that are copied into whole chunks first; whole numbers, whose sums are exact"""
+    rows, n, k = 2100, 1501, 1605
+    say("packed", elt, order, lead, extra)
+    rng = np.random.default_rng(k + lead)
+    offsets, index = np.array([3, 1000, 1400, 2098], np.int32), rng.integers(-2, 2 * rows, rows).astype(np.int32)
+    x, w = rng.integers(-3, 4, (rows, k)).astype(float), rng.integers(-3, 4, (3, n, k)).astype(float)
+    dx, dw = Boxed(A, ctx, store(x, elt), elt, lead, extra, np.nan), Boxed(A, ctx, store(w, elt), elt, lead, extra, np.nan, swap=order == "kn")
+    doff, dindex = ctx.array(offsets), ctx.array(index)
+    named = np.where(index < 0, -1, index // 2)
+    for use in (False, True):
+        taken = np.where(named[:, None] >= 0, x[named], 0.0) if use else x
+        want = np.zeros((rows, n))
+        for e in range(3):
+            want[offsets[e]:offsets[e + 1]] = taken[offsets[e]:offsets[e + 1]] @ w[e].T
+        out = Boxed(A, ctx, np.ones((rows, n), STORED[elt]), elt, lead, extra, 7.0)
+        ops("Product", elt).rows(dx.array, dw.array, doff, out.array, index=dindex if use else None, per=2 if use else 0)
+        assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
+        g = rng.integers(-3, 4, (rows, n)).astype(float)
+        dg = Boxed(A, ctx, store(g, elt), elt, lead, extra, np.nan)
+        grad = Boxed(A, ctx, np.ones((3, n, k), STORED[elt]), elt, lead, extra, 7.0, swap=order == "kn")
+        ops("Product", elt).outer(dg.array, dx.array, doff, grad.array, index=dindex if use else None, per=2 if use else 0)
+        want = np.stack([g[offsets[e]:offsets[e + 1]].T @ taken[offsets[e]:offsets[e + 1]] for e in range(3)])
+        assert np.array_equal(values(grad.get(), elt), values(store(want, elt), elt))
+
+
 @pytest.mark.parametrize("order", ["ij", "ji"])
 @pytest.mark.parametrize("elt,rows,ni,nj", [("float", 1049, 999, 131), ("bfloat16", 2086, 1005, 260), ("half", 17476, 60, 131)])
 def test_no_row_behind_the_last_one_is_read(A, ctx, ops, elt, rows, ni, nj, order):
