@@ -79,25 +79,30 @@ std::string product_source(const OpSpec &sp, const ProductVariant &v)
 // route: how a token's logits are shared out
 struct RouteVariant {
   int lanes = 1, per = 8, vec = 1, sels = 1;
-  bool tall = false;            // a lane a token
-  uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (uint32_t)vec << 16 | (uint32_t)sels << 24 | (tall ? 1u << 31 : 0u); }
+  bool tall = false;            // a lane a token, or `halves` of them
+  int halves = 1;
+  uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (uint32_t)vec << 16 | (uint32_t)sels << 24 | (tall ? (halves == 1 ? 1u : halves == 2 ? 2u : 3u) << 30 : 0u); }
 };
 constexpr int kRouteThreads = 1024, kRouteTallThreads = 256, kRouteMaxExperts = 2048;
+constexpr int64_t kRouteAlone = 8192;                // up to as many logits go to one workgroup, see route_block
 
-// The form with a lane a token is for tokens that fill the SIMDs with waves of 64, up to eight choices, and rows that are read
-// 16 bytes at a time: bfloat16, 8 of 128, 32768 tokens take 21 us with it and 25 without, 65536 24 and 40, but 16384 19 and 17.
-// (Float32, 4 of 64: 65536 tokens 23 and 24, 32768 21 and 15: its keys are twice as long.)
-constexpr int64_t kRouteTallFrom = 32768;
+// The form with a lane a token, or two or four that share its logits, is for up to eight choices and rows that are read 16 bytes
+// at a time.  Of 16 bits it takes over beyond 64 experts, with two lanes for up to 128 and four for more, and for fewer experts
+// where there are tokens enough for a wave of 64 a SIMD.  In us, eight chosen of bfloat16, the other form's time last: 4096 tokens of
+// 128: 17 with one lane, 14 with two, 14 with four, 15; 16384 of 512: 51, 35, 28, 47; 65536 of 128: 24, 23, 30, 41; of 64: 17, 20, 27,
+// 25; 16384 of 64: 13 and 12.  Float32 has keys twice as long: 65536 of 128: 57, 48, 53, 56; 16384 of 128: 49, 36, 27, 20, of 512: 173,
+// 114, 63, 65.
 RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned, int64_t tokens)
 {
   RouteVariant v;
-
   const int epc = 16 / type_bytes(sp.type);
   while (v.lanes < 64 && v.lanes * v.per < experts) v.lanes *= 2;
   while (v.lanes * v.per < experts) v.per *= 2;
   v.vec = aligned && experts % epc == 0 ? epc : 1;
   v.sels = (sp.choose + v.lanes - 1) / v.lanes;
-  v.tall = v.vec > 1 && sp.choose <= 8 && tokens >= (sp.type == 0 ? 2 : 1) * kRouteTallFrom;
+  const int64_t from = sp.type == 0 ? (experts >= 256 ? 16384 : 65536) : experts > 64 ? 65 : 32768;      // (65: more than one workgroup)
+  v.tall = v.vec > 1 && sp.choose <= 8 && tokens >= from && tokens * experts > kRouteAlone;
+  if (v.tall) v.halves = experts <= (sp.type == 0 ? 32 : 64) ? 1 : experts <= 128 ? 2 : 4;
   return v;
 }
 
@@ -105,9 +110,9 @@ std::string route_source(const OpSpec &sp, const RouteVariant &v)
 {
   char text[512];
   std::snprintf(text, sizeof(text),
-                "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_SELS %d\n#define OP_THREADS %d\n#define OP_TALL %d\n#define OP_CHOOSE %d\n"
+                "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_VEC %d\n#define OP_SELS %d\n#define OP_THREADS %d\n#define OP_TALL %d\n#define OP_HALVES %d\n#define OP_CHOOSE %d\n"
                 "#include \"acc_hip_device.h\"\n#include \"op_route.h\"\n",
-                sp.type, v.lanes, v.per, v.vec, v.sels, kRouteThreads, v.tall ? 1 : 0, sp.choose);
+                sp.type, v.lanes, v.per, v.vec, v.sels, kRouteThreads, v.tall ? 1 : 0, v.halves, sp.choose);
   return text;
 }
 
@@ -116,7 +121,7 @@ std::string route_source(const OpSpec &sp, const RouteVariant &v)
 // 9; 256 of 64 16 and 9.
 int route_block(const RouteVariant &v, int64_t tokens, int64_t experts)
 {
-  if (tokens * experts <= 8192) return (int)std::max<int64_t>(1, tokens);
+  if (tokens * experts <= kRouteAlone) return (int)std::max<int64_t>(1, tokens);
   return (int)std::max<int64_t>(std::min(64, kRouteThreads / v.lanes), ceil_div(tokens, 256));
 }
 
@@ -187,7 +192,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   } else if (sp.kind == ACC_OP_ROUTE) {
     for (int experts : {1, 8, 16, 32, 64, 128, 256, 512, 1024, 2048}) if (experts >= sp.choose)
       for (bool aligned : {true, false})
-        for (int64_t tokens : {int64_t(1), 2 * kRouteTallFrom}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
+        for (int64_t tokens : {int64_t(1), int64_t(1) << 20}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
   } else {
@@ -452,8 +457,9 @@ std::string route_source_of(const OpSpec &sp, uint32_t key)
   v.lanes = (int)(key & 255u);
   v.per = (int)(key >> 8 & 255u);
   v.vec = (int)(key >> 16 & 255u);
-  v.sels = (int)(key >> 24 & 127u);
-  v.tall = key >> 31;
+  v.sels = (int)(key >> 24 & 63u);
+  v.tall = key >> 30;
+  v.halves = key >> 30 == 3u ? 4 : key >> 30 == 2u ? 2 : 1;
   return route_source(sp, v);
 }
 std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_source(sp, (int)(key & 3u)); }
@@ -876,7 +882,7 @@ try {
     ACC_TRY(op->ctx->scratch_acquire((size_t)a.blocks * (size_t)experts * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
     a.counts = static_cast<uint32_t *>(scratch.ptr);
   }
-  int rc = v.tall ? launch(op, who, var->fn, a.blocks, kRouteTallThreads, (size_t)experts * 4, stream, a)
+  int rc = v.tall ? launch(op, who, var->fn, a.blocks, kRouteTallThreads * v.halves, (size_t)experts * 4, stream, a)
                   : launch(op, who, var->fn, a.blocks, kRouteThreads, route_lds(experts), stream, a);
   if (rc == ACC_OK && a.blocks > 1) rc = launch(op, who, var->fn2, a.blocks, kRouteThreads, route_lds(experts), stream, a);
   if (a.blocks > 1) op->ctx->scratch_release(scratch, static_cast<hipStream_t>(stream));

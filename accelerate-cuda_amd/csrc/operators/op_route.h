@@ -5,8 +5,8 @@
  * A token has OP_LANES neighbouring lanes with OP_PER logits each.  A logit is a key: its bits, made to compare as whole
  * numbers do, above the index turned round, so that of equal ones the lowest index is the largest -- 32 bits for logits of
  * 16, 64 for Float32; 0 is no logit.  A lane sorts its keys once; then the token's lanes agree on the largest of their first
- * ones, `choose` times, and whoever had it moves up.  (65536 tokens of 128 bfloat16 logits, eight chosen: about 150 vector
- * instructions for four tokens, 4 us of a bound of 5 by memory.)
+ * ones, `choose` times, and whoever had it moves up.  Bound by that agreement: 16384 tokens of 64 Float32 logits, four chosen, take
+ * 12 us in all where memory is 1.
  */
 #include "op_common.h"
 
@@ -205,14 +205,17 @@ ACC_DEV void op_bases(const acc_route_args &p, int *base, const int *total, cons
 }
 
 #if OP_TALL
-/* The selection for many tokens: a lane has a token and OP_CHOOSE keys in order, and puts every logit of its row where it
- * belongs among them: the new j-th key is the middle one of the j-th, the one in front of it and the logit's, an
- * instruction for keys of 32 bits.  That is 15 instructions a logit for 64 tokens at once -- a third of what the lanes of a
- * token need to agree on as many -- but a wave's time is the same for one token as for 64: it takes over where the tokens
- * fill the SIMDs.  Rows come by way of LDS, 128 bytes of 64 rows at a time, so that lines are read whole; a row's share lies
- * 144 bytes from the next one's, which spreads the lanes' reads over the banks. */
+/* The selection for many tokens or experts: a lane has a token (OP_HALVES lanes, which share its logits) and OP_CHOOSE keys in
+ * order, and puts every logit where it belongs among them: the new j-th key is the middle one of the j-th, the one in front of
+ * it and the logit's, an instruction for keys of 32 bits.  That is 15 instructions a logit for 64 lanes at once, a third of what
+ * the lanes of a token need to agree on as many.  Rows come by way of LDS, 128 bytes of them a lane at a time, so that lines are
+ * read whole; a row's share lies 16 bytes further than as many lines, which spreads the lanes' reads over the banks.  65536 tokens
+ * of 128 bfloat16 logits, eight chosen, with a lane a token: 15.7 us of a bound of 4 by memory (17 MB read, 4 written) and of about
+ * 5 by instructions; a SIMD has one wave then, whose waits nothing covers. */
 #define OP_COLUMNS (128 / (int)sizeof(op_elt))
-#define OP_APART 144
+#define OP_TALL_TOKENS (64 / OP_HALVES)            /* of a wave; a token has OP_HALVES lanes, as many apart */
+#define OP_TALL_THREADS (256 * OP_HALVES)
+#define OP_APART (128 * OP_HALVES + 16)
 typedef op_elt op_vec __attribute__((ext_vector_type(OP_VALUES)));
 
 ACC_DEV op_key op_middle(const op_key a, const op_key b, const op_key c)
@@ -222,18 +225,40 @@ ACC_DEV op_key op_middle(const op_key a, const op_key b, const op_key c)
   return low > most ? low : most;
 }
 
-extern "C" __global__ void __launch_bounds__(256) route(const acc_route_args p)
+/* what the first and the second of two lanes hold that are 16 or 32 apart, in both */
+template <typename T> ACC_DEV void op_both(const T v, const int apart, T *first, T *second)
+{
+  unsigned int w[sizeof(T) / 4], a[sizeof(T) / 4], b[sizeof(T) / 4];
+  __builtin_memcpy(w, &v, sizeof(T));
+#pragma unroll
+  for (int k = 0; k < (int)(sizeof(T) / 4); ++k) {
+    const auto r = apart == 16 ? __builtin_amdgcn_permlane16_swap(w[k], w[k], false, false) : __builtin_amdgcn_permlane32_swap(w[k], w[k], false, false);
+    a[k] = r[0];
+    b[k] = r[1];
+  }
+  __builtin_memcpy(first, a, sizeof(T));
+  __builtin_memcpy(second, b, sizeof(T));
+}
+
+ACC_DEV void op_insert(op_key (&k)[OP_CHOOSE], const op_key y)
+{
+#pragma unroll
+  for (int j = OP_CHOOSE - 1; j > 0; --j) k[j] = op_middle(k[j - 1], k[j], y);
+  k[0] = k[0] > y ? k[0] : y;
+}
+
+extern "C" __global__ void __launch_bounds__(OP_TALL_THREADS) route(const acc_route_args p)
 {
   if (p.guard && *p.guard == 0u) return;
   extern __shared__ int shared[];
-  __shared__ __align__(16) unsigned char tiles[4][64 * OP_APART];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) unsigned char tiles[OP_TALL_THREADS / 64][OP_TALL_TOKENS * OP_APART];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, token = lane % OP_TALL_TOKENS, share = lane / OP_TALL_TOKENS;
   const long long first = (long long)blockIdx.x * p.block, last = acc_min<long long>(p.tokens, first + p.block);
   unsigned char *tile = tiles[wave];
-  for (int e = tid; e < p.experts; e += 256) shared[e] = 0;
+  for (int e = tid; e < p.experts; e += OP_TALL_THREADS) shared[e] = 0;
   __syncthreads();
-  for (long long at = first + wave * 64; at < last; at += 256) {
-    const int rows = (int)acc_min<long long>(64, last - at);
+  for (long long at = first + wave * OP_TALL_TOKENS; at < last; at += 256) {
+    const int rows = (int)acc_min<long long>(OP_TALL_TOKENS, last - at);
     const op_elt *x = (const op_elt *)p.logits + at * p.logits_stride;
     op_key k[OP_CHOOSE];
     float total = 0.0f, most = OP_NONE;
@@ -243,35 +268,31 @@ extern "C" __global__ void __launch_bounds__(256) route(const acc_route_args p)
     const auto ask = [&](const int c0) {           /* (rows that there are not: the last one; columns: minus infinity) */
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int r = acc_min(i * 8 + lane / 8, rows - 1), c = c0 + lane % 8 * OP_VALUES;
+        const int n8 = i * 64 + lane, r = acc_min(n8 / (8 * OP_HALVES), rows - 1), c = c0 + n8 % (8 * OP_HALVES) * OP_VALUES;
 #pragma unroll
         for (int n = 0; n < OP_VALUES; ++n) next[i][n] = (op_elt)OP_NONE;
         if (c < p.experts) next[i] = *(const op_vec *)(x + r * p.logits_stride + c);
       }
     };
     ask(0);
-    for (int c0 = 0; c0 < p.experts; c0 += OP_COLUMNS) {
+    for (int c0 = 0; c0 < p.experts; c0 += OP_HALVES * OP_COLUMNS) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *(op_vec *)(tile + (i * 8 + lane / 8) * OP_APART + lane % 8 * 16) = next[i];
-      if (c0 + OP_COLUMNS < p.experts) ask(c0 + OP_COLUMNS);
+      for (int i = 0; i < 8; ++i) *(op_vec *)(tile + (i * 64 + lane) / (8 * OP_HALVES) * OP_APART + lane % (8 * OP_HALVES) * 16) = next[i];
+      if (c0 + OP_HALVES * OP_COLUMNS < p.experts) ask(c0 + OP_HALVES * OP_COLUMNS);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
+      const unsigned char *mine = tile + token * OP_APART + share * 128;
       for (int i = 0; i < 8; ++i) {
-        const op_vec v = *(const op_vec *)(tile + lane * OP_APART + i * 16);
+        const op_vec v = *(const op_vec *)(mine + i * 16);
 #pragma unroll
-        for (int n = 0; n < OP_VALUES; ++n) {
-          const op_key y = op_key_of(v[n], c0 + i * OP_VALUES + n);
-#pragma unroll
-          for (int j = OP_CHOOSE - 1; j > 0; --j) k[j] = op_middle(k[j - 1], k[j], y);
-          k[0] = k[0] > y ? k[0] : y;
-        }
+        for (int n = 0; n < OP_VALUES; ++n) op_insert(k, op_key_of(v[n], c0 + share * OP_COLUMNS + i * OP_VALUES + n));
       }
       if (!p.normalise) {
         const float now = op_value_of(k[0]);
         total *= op_power(most, now);
         most = now;
         for (int i = 0; i < 8; ++i) {
-          const op_vec v = *(const op_vec *)(tile + lane * OP_APART + i * 16);
+          const op_vec v = *(const op_vec *)(mine + i * 16);
 #pragma unroll
           for (int n = 0; n < OP_VALUES; ++n) {
             const float f = (float)v[n];
@@ -282,9 +303,29 @@ extern "C" __global__ void __launch_bounds__(256) route(const acc_route_args p)
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
-    if (lane >= rows) continue;
+    /* a token's lanes put together what they have */
+#pragma unroll
+    for (int apart = OP_TALL_TOKENS; apart < 64; apart *= 2) {
+      op_key other[OP_CHOOSE];
+      float here, there, here_most, there_most;
+      op_both(total, apart, &here, &there);
+#pragma unroll
+      for (int j = 0; j < OP_CHOOSE; ++j) {
+        op_key one;
+        op_both(k[j], apart, &one, &other[j]);
+        k[j] = one;
+      }
+      here_most = op_value_of(k[0]);
+      there_most = op_value_of(other[0]);
+#pragma unroll
+      for (int j = 0; j < OP_CHOOSE; ++j) op_insert(k, other[j]);
+      most = op_value_of(k[0]);
+      total = here * op_power(here_most, most) + there * op_power(there_most, most);
+    }
+    if (token >= rows) continue;
     most = op_value_of(k[0]);
     float power[OP_CHOOSE];
+    int expert[OP_CHOOSE];
 #pragma unroll
     for (int j = 0; j < OP_CHOOSE; ++j) {
       power[j] = op_power(op_value_of(k[j]), most);
@@ -292,14 +333,19 @@ extern "C" __global__ void __launch_bounds__(256) route(const acc_route_args p)
     }
 #pragma unroll
     for (int j = 0; j < OP_CHOOSE; ++j) {
-      const int e = op_index_of(k[j]);
-      p.chosen[(at + lane) * OP_CHOOSE + j] = e;
-      p.weights[(at + lane) * OP_CHOOSE + j] = e < 0 ? 0.0f : power[j] / total;
-      if (e >= 0) atomicAdd(&shared[e], 1);
+      expert[j] = op_index_of(k[j]);
+      power[j] = expert[j] < 0 ? 0.0f : power[j] / total;
     }
+    if (share == 0) {
+      __builtin_memcpy(p.chosen + (at + token) * OP_CHOOSE, expert, sizeof expert);
+#pragma unroll
+      for (int j = 0; j < OP_CHOOSE; ++j)
+        if (expert[j] >= 0) atomicAdd(&shared[expert[j]], 1);
+    }
+    if (share == OP_HALVES - 1) __builtin_memcpy(p.weights + (at + token) * OP_CHOOSE, power, sizeof power);
   }
   __syncthreads();
-  for (int e = tid; e < p.experts; e += 256) p.counts[(long long)blockIdx.x * p.experts + e] = shared[e];
+  for (int e = tid; e < p.experts; e += OP_TALL_THREADS) p.counts[(long long)blockIdx.x * p.experts + e] = shared[e];
 }
 #else
 /* workgroup b has the tokens b * block .. ; with one workgroup the slots are placed at once, otherwise the counts go out */
