@@ -363,8 +363,8 @@ int tile_of(const OpSpec &sp, const ProductVariant &v, int tile)
 //     52 in tiles.  4 bits only where the matrices are few: 32 rows of 4096 x 4096: 41 and 33 in tiles of 64 x 128
 //   Float32, bound by the matrix cores, wants them full to the end: 8192 rows, 8 of 1024 x 1536: 207 in 32 x 64 or 64 x 64, 225 in
 //     64 x 128, 270 in 128 x 128; 1024, 4 of 512 x 2048: 38, 37, 66, 124; 20000, 8 of 768 x 1024: 247, 233, 244, 244
-//   256 x 256 from 128 rows a segment on: 2048 rows of 4096 x 4096: 137 in 128 x 128, 141 in 256 x 256; 3072: 259 and 144; 4096: 227
-//     and 147.  Not for few tiles (8192 rows, 8 of 1024 x 1024, 128 tiles: 37 and 60) or short sums (16384, 8 of 2048 x 256: 36 and 41).
+//   256 x 256 from 128 rows a segment on: 2048 rows of 4096 x 4096: 137 in 128 x 128, 141 in 256 x 256; 4096: 227 and 147; 5120: 350
+//     and 276.  Not for few tiles (8192 rows, 8 of 1024 x 1024, 128 tiles: 37 and 60) or short sums (16384, 8 of 2048 x 256: 36 and 41).
 //     4 bits already from 48 rows on, and for any sum: 1024 rows of 4096 x 4096: 42 and 39; 22272, 4 of 1976 x 44: 48 and 44
 //   128 x 128 from 64 rows on, 64 x 128 from 32, where there are 256 tiles: 1536 rows of 4096 x 2048: 104 in 64 x 128, 74 in
 //     128 x 128; 768: 97 in 32 x 64, 70 in 64 x 128; 512: 67 and 70; but 1024 of 1000 x 1000, with 128 tiles of 64 x 128: 13 and 16
@@ -401,9 +401,9 @@ int32_t rows_piece(const ProductVariant &v, int64_t groups, int64_t length, int6
 }
 
 // Outer: the tile shape.  A tile is worth its size where there are enough of them, cut as short as pays, to fill the
-// compute units.  In us: 32000 rows, 16 bfloat16 results of 2048 x 2048: 246 in 256 x 256, 321 in 128 x 128; 8192, 8 of 1024 x 1024: 52
-// and 42, and 40 in 64 x 64; 1664, 13 of 800 x 2160: 38 in 64 x 64 and 33 in 128 x 128; 12416, 6 of 41 x 448: 25 and 41.  Float32:
-// 2240 rows, 15 of 3014 x 192: 48 in 64 x 64 and 83 in 128 x 128; 8192, 8 of 1024 x 1536: 209 and 203.
+// compute units.  In us: 32000 rows, 16 bfloat16 results of 2048 x 2048: 249 in 256 x 256, 309 in 128 x 128, 465 in 64 x 64; 8192, 8 of
+// 1024 x 1024: 52, 42 and 40; 1664, 13 of 800 x 2160: 29 in 128 x 128 and 36 in 64 x 64; 12416, 6 of 41 x 448: 23 and 20.  Float32: 2240
+// rows, 15 of 3014 x 192: 85 and 48; 8192, 8 of 1024 x 1536: 203 and 209.
 int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t ni, int64_t nj)
 {
   const auto groups = [&](int t, int64_t steps) {
@@ -414,7 +414,7 @@ int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t 
   return groups(kMiddle, 8) >= (sp.type == 0 ? 1024 : 256) ? kMiddle : kSquare;
 }
 // ... and the rows of a piece (0: segments are not cut), where whole segments make too few tiles to fill the compute units:
-// 17110 Float32 rows, 13 results of 64 x 64: 18 us and 369 uncut; 11200 bfloat16 rows, one of 3072 x 59: 22 and 590.
+// 17110 Float32 rows, 13 results of 64 x 64: 17 us and 369 uncut; 30043, 3 of 64 x 768: 45 and 799.
 int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t tiles)
 {
   const int64_t target = v.tile == kLarge ? 256 : v.tile == kMiddle ? 512 : 1024, step = 128 / type_bytes(sp.type);

@@ -10,11 +10,17 @@
  * its scales).  Two steps lie in LDS.  The matrix cores work on half a step, whose fragments are in registers, while the next
  * half's are read; one barrier a step, in its middle, says that everybody's share of the next step has arrived and that
  * nobody reads this one any more, so that the next but one may take its place.
+ *
+ * A wave of the largest tile has 128 x 64 results in 128 registers, and reads 12 fragments of LDS for 32 products of a half step;
+ * what bounds it is that LDS and the matrix cores together leave no time over, then, where sums are short, the 10 us a tile has
+ * in front of its first product and behind its last.  Measured: bfloat16 8192^3 along the sum 768 us, 1431 TFLOP/s; the matrix
+ * turned 782, both turned (outer) 819, with an index 868; 4 bits 295, 3730; Float32 4096^3 962, 143.  A sum may be in pieces (few
+ * tiles, long sums): each is a workgroup's, goes out in Float32, and product_join adds them up in order.
  */
 #include "op_matrix.h"
 
 #define OP_THREADS (64 * OP_WM * OP_WN)
-#define OP_GROUP (OP_BM >= 256 ? 4 : OP_BM >= 128 ? 8 : 16)   /* rows of tiles that are gone through together */
+#define OP_GROUP (OP_BM >= 256 ? 4 : OP_BM >= 128 ? 8 : 16)   /* rows of tiles that are gone through together: 8192^3 takes a tenth less than column by column */
 #define OP_FM (OP_BM / OP_WM / 16)                 /* fragments of 16 x 16 that a wave has of the result */
 #define OP_FN (OP_BN / OP_WN / 16)
 
