@@ -298,13 +298,24 @@ int check_shape(const char *who, const char *what, const acc_strided &a, std::in
 }
 
 struct Named { const acc_strided *a; int bytes; const char *what; };
+// whether two arrays of rows are different columns of one: rows as far apart, whose stretches lie beside each other
+bool beside(const Named &a, const Named &b)
+{
+  if (a.a->rank != 2 || b.a->rank != 2 || !unit(*a.a, 1) || !unit(*b.a, 1)) return false;
+  const int64_t pitch = a.a->stride[0] * a.bytes, a_row = a.a->shape[1] * a.bytes, b_row = b.a->shape[1] * b.bytes;
+  if (pitch <= 0 || pitch != b.a->stride[0] * b.bytes) return false;
+  // (how far a's stretch begins behind b's, of whichever rows)
+  const uint64_t p = (uint64_t)pitch;
+  const int64_t at = (int64_t)(a.a->ptr >= b.a->ptr ? (a.a->ptr - b.a->ptr) % p : (p - (b.a->ptr - a.a->ptr) % p) % p);
+  return at >= b_row && at + a_row <= pitch;
+}
 int check_apart(const char *who, const Named &out, std::initializer_list<Named> others)
 {
   const Span o = span_of(*out.a, out.bytes);
   for (const Named &n : others) {
     if (!n.a) continue;
     const Span s = span_of(*n.a, n.bytes);
-    if (s.from < o.to && o.from < s.to) return fail(ACC_ERR_INVALID, "%s: %s shares memory with %s", who, out.what, n.what);
+    if (s.from < o.to && o.from < s.to && !beside(out, n)) return fail(ACC_ERR_INVALID, "%s: %s shares memory with %s", who, out.what, n.what);
   }
   return ACC_OK;
 }

@@ -650,7 +650,8 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * All work is enqueued on `stream`; the calls return without waiting.  On a stream under a guard (acc_stream_set_guard)
  * the kernels do nothing once the guard is down.  Sums, softmax statistics and weights are Float32 whatever the element
  * type, and results are rounded once; they are taken in an order that shapes and segments alone decide, so that a call
- * gives the same bits every time.  No result may share memory with another array of the call.  Scratch memory -- pieces of
+ * gives the same bits every time.  No result may share memory with another array of the call (other columns of the same
+ * rows are apart).  Scratch memory -- pieces of
  * long sums, 16-bit operands whose rows start anywhere copied to where they do not (2 GB at most), a router's counts --
  * comes from the context's pool, in stream order.
  *

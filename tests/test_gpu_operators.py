@@ -830,3 +830,128 @@ def test_weights_of_rows_without_columns_have_a_gradient_of_zero(A, ctx, ops):
     op.gradient(empty(3), empty(6), place, weights, empty(6), dw)
     assert np.array_equal(dw.get(), np.zeros((3, 2), np.float32))
     op.combine(empty(6), place, weights, empty(3))
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_columns_of_one_array_are_operand_and_result(A, ctx, ops, first):
+    """the result beside the operand in the same rows, on either side; a column in common is refused"""
+    rng = np.random.default_rng(2)
+    rows, n, k, pitch = 60, 24, 40, 70
+    x, w = rng.integers(-3, 4, (rows, k)).astype(np.float32), rng.integers(-3, 4, (2, n, k)).astype(np.float32)
+    host = np.full((rows, pitch), 9, np.float32)
+    x_at, out_at = (0, 41) if first else (29, 5)
+    host[:, x_at:x_at + k] = x
+    both, offsets = ctx.array(host), np.array([0, 25, 60], np.int32)
+    part = lambda at, width: A.Strided((rows, width), (pitch, 1), both.ptr + 4 * at, both)
+    ops("Product", "float").rows(part(x_at, k), ctx.array(w), ctx.array(offsets), part(out_at, n))
+    got = both.get()
+    assert np.array_equal(got[:, out_at:out_at + n], np.concatenate([x[:25] @ w[0].T, x[25:] @ w[1].T]))
+    got[:, out_at:out_at + n] = 9
+    assert np.array_equal(got, host)
+    for at in (x_at + k - 1, x_at - n + 1):
+        if 0 <= at <= pitch - n:
+            with pytest.raises(A.AccError):
+                ops("Product", "float").rows(part(x_at, k), ctx.array(w), ctx.array(offsets), part(at, n))
+
+
+# ------------------------------------------------------------------------------ far apart
+
+class Far(object):
+    """rows (or matrices) `apart` bytes from one another in one large allocation"""
+
+    def __init__(self, A, ctx, whole, host, apart, at=0):
+        self.A, self.ctx, self.host, self.apart, self.base = A, ctx, host, apart, whole.ptr + at
+        assert at + (host.shape[0] - 1) * apart + host[0].nbytes <= whole.nbytes and apart % host.itemsize == 0
+        inner, step = [], 1
+        for n in reversed(host.shape[1:]):
+            inner.insert(0, step)
+            step *= n
+        self.array = A.Strided(host.shape, [apart // host.itemsize] + inner, self.base, whole)
+        self.set(host)
+
+    def part(self, i):
+        one = self.host[i]
+        return self.A.DeviceArray.view(self.ctx, one.shape, one.dtype, one.size, self.base + i * self.apart)
+
+    def set(self, host):
+        for i in range(host.shape[0]):
+            self.part(i).set(host[i])
+
+    def get(self):
+        return np.stack([self.part(i).get() for i in range(self.host.shape[0])])
+
+
+@pytest.mark.parametrize("apart", [(700 << 20) + 64, (700 << 20) + 66, (280 << 20) + 16])
+def test_arrays_beyond_two_and_four_gigabytes(A, ctx, ops, apart):
+    """seven rows, 280 or 700 MB apart: 1.7 GB, where offsets of 32 bits still do, and 4.2; every operand in turn"""
+    say("far", apart)
+    rng = np.random.default_rng(apart)
+    wholes = [ctx.empty((5 << 30,), np.uint8) for _ in range(3)]           # (a result interleaved with an operand is refused)
+    rows, n, k = 7, 40, 64
+    far = lambda v, at, which=0: Far(A, ctx, wholes[which], v, apart, at)
+    small = lambda *s: rng.integers(-3, 4, s).astype(np.float16)
+    offsets, index = np.array([0, 3, 7], np.int32), np.array([6, 0, 5, -1, 4, 6, 1], np.int32)
+    doff, dindex = ctx.array(offsets), ctx.array(index)
+    x, w, g = small(rows, k), small(2, n, k), small(rows, n)
+    named = np.where((index >= 0)[:, None], x[index].astype(float), 0.0)
+    product, zeros = ops("Product", "half"), np.zeros
+    # the rows that are multiplied, the result's rows; by an index, too
+    for use in (False, True):
+        fx, fo = far(x, 0), far(zeros((rows, n), np.float16), 1 << 20, 1)
+        product.rows(fx.array, ctx.array(w), doff, fo.array, index=dindex if use else None)
+        taken = named if use else x.astype(float)
+        want = np.concatenate([taken[:3] @ w[0].T.astype(float), taken[3:] @ w[1].T.astype(float)])
+        assert np.array_equal(fo.get().astype(float), want)
+        fg, dw = far(g, 2 << 20), ctx.empty((2, n, k), np.float16)
+        product.outer(fg.array, fx.array, doff, dw, index=dindex if use else None)
+        want = np.stack([g[:3].T.astype(float) @ taken[:3], g[3:].T.astype(float) @ taken[3:]])
+        assert np.array_equal(dw.get().astype(float), want)
+    # the matrices, as operand and as result
+    many = small(rows, n, k)
+    fw, each, out = far(many, 0), ctx.array(np.arange(rows + 1, dtype=np.int32)), ctx.empty((rows, n), np.float16)
+    product.rows(ctx.array(x), fw.array, each, out)
+    assert np.array_equal(out.get().astype(float), np.einsum("enk,ek->en", many.astype(float), x.astype(float)))
+    fd = far(zeros((rows, n, k), np.float16), 1 << 20, 1)
+    product.outer(ctx.array(g), ctx.array(x), each, fd.array)
+    assert np.array_equal(fd.get().astype(float), g[:, :, None].astype(float) * x[:, None, :])
+    # combination
+    place = np.array([[6, 0], [5, 4], [1, -1]], np.int32)
+    y, dout = small(rows, k), small(3, k)
+    fy, fs, fdo = far(y, 0), far(zeros((3, k), np.float16), 1 << 20, 1), far(dout, 2 << 20)
+    comb = ops("Combiner", "half")
+    comb.combine(fy.array, ctx.array(place), None, fs.array)
+    there = place >= 0
+    assert np.array_equal(fs.get().astype(float), (y[place].astype(float) * there[:, :, None]).sum(1))
+    fdy, dweights = far(zeros((rows, k), np.float16), 3 << 20, 1), ctx.empty((3, 2), np.float32)
+    comb.gradient(fdo.array, fy.array, ctx.array(place), None, fdy.array, dweights)
+    want = zeros((rows, k))
+    for t in range(3):
+        for j in range(2):
+            if place[t, j] >= 0:
+                want[place[t, j]] = dout[t]
+    assert np.array_equal(fdy.get().astype(float), want)
+    assert np.array_equal(dweights.get(), (dout[:, None, :].astype(float) * y[place]).sum(2) * there)
+    # the router
+    logits = rng.permutation(rows * 24).reshape(rows, 24).astype(np.float16)
+    fl = far(logits, 0)
+    ints = [ctx.empty(s, np.int32) for s in ((rows, 2), (25,), (rows * 2,), (rows, 2))]
+    weights = ctx.empty((rows, 2), np.float32)
+    ops("Router", "half", 2, True).route(fl.array, ints[0], weights, ints[1], ints[2], ints[3])
+    assert np.array_equal(ints[0].get(), np.argsort(-logits.astype(float), 1)[:, :2])
+    # 4 bits
+    micro = ops("Microscale", "half")
+    v = rng.choice([-6, -4, -3, -2, -1.5, -1, -0.5, 0, 0.5, 1, 1.5, 2, 3, 4, 6], (rows, k)).astype(np.float16)
+    v[:, ::32] = 6                                          # (scales of one, so that codes are the values)
+    if apart % 16:
+        return                                              # (rows of codes start on 16 bytes)
+    fv, fc, fe = far(v, 0), far(zeros((rows, 32), np.uint8), 1 << 20, 1), far(zeros((rows, 2), np.uint8), 2 << 20, 2)
+    micro.quantise(fv.array, fc.array, fe.array)
+    fb = far(zeros((rows, k), np.float16), 3 << 20, 0)
+    micro.values(fc.array, fe.array, fb.array)
+    assert np.array_equal(fb.get(), v)
+    fo = far(zeros((rows, rows), np.float16), 4 << 20, 0)
+    wc, ws = fc.array, fe.array
+    turned = lambda a, m: A.Strided((1, rows, m), (0,) + tuple(a.strides), a.ptr, a.owner)
+    micro.rows(fc.array, fe.array, turned(wc, 32), turned(ws, 2), ctx.array(np.array([0, rows], np.int32)), fo.array)
+    want = v.astype(float) @ v.T.astype(float)
+    assert np.array_equal(fo.get(), want.astype(np.float16))
