@@ -651,9 +651,10 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * the kernels do nothing once the guard is down.  Sums, softmax statistics and weights are Float32 whatever the element
  * type, and results are rounded once; they are taken in an order that shapes and segments alone decide, so that a call
  * gives the same bits every time.  No result may share memory with another array of the call (other columns of the same
- * rows are apart).  Scratch memory -- pieces of
- * long sums, 16-bit operands whose rows start anywhere copied to where they do not (2 GB at most), a router's counts --
- * comes from the context's pool, in stream order.
+ * rows are apart).  Scratch memory -- pieces of long sums, 16-bit operands whose rows start anywhere copied to where they
+ * do not (2 GB at most), a router's counts -- comes from the context's pool, in stream order.  Calls may be recorded into a
+ * graph once the same ones have run on that stream (their kernels are loaded then, and the pool has what they need); the
+ * graph keeps that scratch memory, so it is replayed on the stream it was recorded on.
  *
  * Element types are "float", "half" and "bfloat16" (an acc_strided does not say which it holds; the operator does).
  * Extents are below 2^31; strides are in elements, and addresses are computed in 64 bits.  Offsets, indices, places and

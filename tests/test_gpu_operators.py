@@ -854,6 +854,64 @@ def test_columns_of_one_array_are_operand_and_result(A, ctx, ops, first):
                 ops("Product", "float").rows(part(x_at, k), ctx.array(w), ctx.array(offsets), part(at, n))
 
 
+def test_a_layer_recorded_into_a_graph_and_replayed_on_changing_inputs(A, ops):
+    """router, products with pieces and copies, combination and gradient in one graph; eager calls of the same between the replays"""
+    import ctypes as C
+    hip = C.CDLL("libamdhip64.so")
+    hip.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+    hip.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+    hip.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    hip.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+    hip.hipGraphExecDestroy.argtypes = hip.hipGraphDestroy.argtypes = [C.c_void_p]
+    ctx = A.Context(0)
+    stream, rng = ctx.stream(), np.random.default_rng(8)
+    tokens, experts, choose, width, hidden = 1200, 96, 2, 515, 2051
+    slots = tokens * choose
+    x, logits = ctx.empty((tokens, width), np.float16), ctx.empty((tokens, experts), np.float16)
+    w = ctx.array(rng.integers(-2, 3, (experts, hidden, width)).astype(np.float16))
+    router, product, comb = A.Router(ctx, "half", choose, True), A.Product(ctx, "half"), A.Combiner(ctx, "half")
+
+    def arrays():
+        return dict(chosen=ctx.empty((tokens, choose), np.int32), weights=ctx.empty((tokens, choose), np.float32), offsets=ctx.empty((experts + 1,), np.int32),
+                    order=ctx.empty((slots,), np.int32), place=ctx.empty((tokens, choose), np.int32), h=ctx.empty((slots, hidden), np.float16),
+                    out=ctx.empty((tokens, hidden), np.float16), few=ctx.empty((2, 40, 24), np.float16))
+
+    def call(r):
+        router.route(logits, r["chosen"], r["weights"], r["offsets"], r["order"], r["place"], stream=stream)
+        product.rows(x, w, r["offsets"], r["h"], index=r["order"], per=choose, stream=stream)
+        comb.combine(r["h"], r["place"], r["weights"], r["out"], stream=stream)
+        column = lambda n: A.Strided((tokens, n), (width, 1), x.ptr, x)
+        product.outer(column(40), column(24), halves, r["few"], stream=stream)
+    halves = ctx.array(np.array([0, 600, tokens], np.int32))
+    recorded, eager = arrays(), arrays()
+    fill = lambda: (x.set(rng.integers(-2, 3, (tokens, width)).astype(np.float16)), logits.set(rng.standard_normal((tokens, experts)).astype(np.float16)))
+    fill()
+    call(eager)
+    ctx.sync()
+    graph, graph_exec = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0
+    try:
+        call(recorded)
+    finally:
+        rc = hip.hipStreamEndCapture(stream, C.byref(graph))
+    assert rc == 0 and graph.value and hip.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+    for replay in range(4):
+        say("replay", replay)
+        fill()
+        assert hip.hipGraphLaunch(graph_exec, stream) == 0
+        ctx.sync()
+        call(eager)
+        ctx.sync()
+        for name in recorded:
+            if name != "h":
+                assert np.array_equal(recorded[name].get(), eager[name].get()), (replay, name)
+    hip.hipGraphExecDestroy(graph_exec)
+    hip.hipGraphDestroy(graph)
+    for op in (router, product, comb):
+        op.destroy()
+    ctx.close()
+
+
 # ------------------------------------------------------------------------------ far apart
 
 class Far(object):
