@@ -86,8 +86,7 @@ struct RouteVariant {
 constexpr int kRouteThreads = 1024, kRouteTallThreads = 256, kRouteMaxExperts = 2048;
 constexpr int64_t kRouteAlone = 8192;                // up to as many logits go to one workgroup, see route_block
 
-// The form with a lane a token, or two or four that share its logits, is for up to eight choices and rows that are read 16 bytes
-// at a time.  Of 16 bits it takes over beyond 64 experts, with two lanes for up to 128 and four for more, and for fewer experts
+// The form with a lane a token, or two or four that share its logits, is for up to eight choices and rows of 16 bytes or more.  Of 16 bits it takes over beyond 64 experts, with two lanes for up to 128 and four for more, and for fewer experts
 // where there are tokens enough for a wave of 64 a SIMD.  In us, eight chosen of bfloat16, the other form's time last: 4096 tokens of
 // 128: 17 with one lane, 14 with two, 14 with four, 15; 16384 of 512: 51, 35, 28, 47; 65536 of 128: 24, 23, 30, 41; of 64: 17, 20, 27,
 // 25; 16384 of 64: 13 and 12.  Float32 has keys twice as long: 65536 of 128: 57, 48, 53, 56; 16384 of 128: 49, 36, 27, 20, of 512: 173,
@@ -101,7 +100,7 @@ RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned, int64_t 
   v.vec = aligned && experts % epc == 0 ? epc : 1;
   v.sels = (sp.choose + v.lanes - 1) / v.lanes;
   const int64_t from = sp.type == 0 ? (experts >= 256 ? 16384 : 65536) : experts > 64 ? 65 : 32768;      // (65: more than one workgroup)
-  v.tall = v.vec > 1 && sp.choose <= 8 && tokens >= from && tokens * experts > kRouteAlone;
+  v.tall = experts >= epc && sp.choose <= 8 && tokens >= from && tokens * experts > kRouteAlone;
   if (v.tall) v.halves = experts <= (sp.type == 0 ? 32 : 64) ? 1 : experts <= 128 ? 2 : 4;
   return v;
 }

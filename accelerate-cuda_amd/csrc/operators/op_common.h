@@ -36,6 +36,22 @@ template <bool ALIGNED> ACC_DEV acc_u4 op_chunk(const op_elt *p, const int valid
   return v;
 }
 
+/* v, `bytes` further down: what is shifted in is zeros */
+ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
+{
+  const unsigned long long lo = v.x | (unsigned long long)v.y << 32, hi = v.z | (unsigned long long)v.w << 32;
+  const int n = 8 * bytes;
+  unsigned long long a, b;
+  if (bytes >= 8) {
+    a = bytes >= 16 ? 0 : hi >> (n - 64);
+    b = 0;
+  } else {
+    a = bytes ? lo >> n | hi << (64 - n) : lo;
+    b = hi >> n;
+  }
+  return acc_u4{(unsigned int)a, (unsigned int)(a >> 32), (unsigned int)b, (unsigned int)(b >> 32)};
+}
+
 /* The segments of the rows 0 .. rows-1: number 0 is what lies before the first expert's rows, s the rows of expert s - 1,
  * experts + 1 what lies behind the last one's.  Starts that are out of range or out of order are pulled into it, so that no
  * row outside the array is ever named. */

@@ -31,22 +31,6 @@
 
 typedef __attribute__((address_space(3))) void *op_lds_ptr;
 
-/* v, `bytes` further down: what is shifted in is zeros */
-ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
-{
-  const unsigned long long lo = v.x | (unsigned long long)v.y << 32, hi = v.z | (unsigned long long)v.w << 32;
-  const int n = 8 * bytes;
-  unsigned long long a, b;
-  if (bytes >= 8) {
-    a = bytes >= 16 ? 0 : hi >> (n - 64);
-    b = 0;
-  } else {
-    a = bytes ? lo >> n | hi << (64 - n) : lo;
-    b = hi >> n;
-  }
-  return acc_u4{(unsigned int)a, (unsigned int)(a >> 32), (unsigned int)b, (unsigned int)(b >> 32)};
-}
-
 /* Where row r of an operand lies, in bytes, as a load takes it whose buffer ends before 2 GB: the top bit set, and none (r < 0)
  * is 0 -- as a load of such a number beyond the end of a buffer of them is.  With that bit turned, it is an offset, and none
  * is beyond the end of every buffer. */

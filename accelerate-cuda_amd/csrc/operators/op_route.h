@@ -240,6 +240,9 @@ template <typename T> ACC_DEV void op_both(const T v, const int apart, T *first,
   __builtin_memcpy(second, b, sizeof(T));
 }
 
+/* what a shifted chunk has behind the row's end is no logit (whole chunks have none there) */
+ACC_DEV op_elt op_there(const acc_route_args &p, const op_elt v, const int index) { return OP_VEC > 1 || index < p.experts ? v : (op_elt)OP_NONE; }
+
 ACC_DEV void op_insert(op_key (&k)[OP_CHOOSE], const op_key y)
 {
 #pragma unroll
@@ -271,7 +274,18 @@ extern "C" __global__ void __launch_bounds__(OP_TALL_THREADS) route(const acc_ro
         const int n8 = i * 64 + lane, r = acc_min(n8 / (8 * OP_HALVES), rows - 1), c = c0 + n8 % (8 * OP_HALVES) * OP_VALUES;
 #pragma unroll
         for (int n = 0; n < OP_VALUES; ++n) next[i][n] = (op_elt)OP_NONE;
-        if (c < p.experts) next[i] = *(const op_vec *)(x + r * p.logits_stride + c);
+        if (c < p.experts) {
+          const op_elt *row = x + r * p.logits_stride;
+          if (OP_VEC > 1) {
+            next[i] = *(const op_vec *)(row + c);
+          } else {
+            /* (rows start anywhere; what would reach beyond the row's end is read earlier and shifted into place) */
+            const int from = acc_min(c, p.experts - OP_VALUES);
+            acc_u4 u = ((const op_loose<op_elt> *)(row + from))->v;
+            if (from < c) u = op_shifted(u, (c - from) * (int)sizeof(op_elt));
+            __builtin_memcpy(&next[i], &u, 16);
+          }
+        }
       }
     };
     ask(0);
@@ -285,7 +299,7 @@ extern "C" __global__ void __launch_bounds__(OP_TALL_THREADS) route(const acc_ro
       for (int i = 0; i < 8; ++i) {
         const op_vec v = *(const op_vec *)(mine + i * 16);
 #pragma unroll
-        for (int n = 0; n < OP_VALUES; ++n) op_insert(k, op_key_of(v[n], c0 + share * OP_COLUMNS + i * OP_VALUES + n));
+        for (int n = 0; n < OP_VALUES; ++n) op_insert(k, op_key_of(op_there(p, v[n], c0 + share * OP_COLUMNS + i * OP_VALUES + n), c0 + share * OP_COLUMNS + i * OP_VALUES + n));
       }
       if (!p.normalise) {
         const float now = op_value_of(k[0]);
@@ -295,7 +309,7 @@ extern "C" __global__ void __launch_bounds__(OP_TALL_THREADS) route(const acc_ro
           const op_vec v = *(const op_vec *)(mine + i * 16);
 #pragma unroll
           for (int n = 0; n < OP_VALUES; ++n) {
-            const float f = (float)v[n];
+            const float f = (float)op_there(p, v[n], c0 + share * OP_COLUMNS + i * OP_VALUES + n);
             total += op_power(f > OP_NONE ? f : OP_NONE, most);
           }
         }
