@@ -412,8 +412,9 @@ int32_t rows_piece(const ProductVariant &v, int64_t groups, int64_t length, int6
 
 // Outer: the tile shape.  A tile is worth its size where there are enough of them, cut as short as pays, to fill the
 // compute units.  In us: 32000 rows, 16 bfloat16 results of 2048 x 2048: 249 in 256 x 256, 309 in 128 x 128, 465 in 64 x 64; 8192, 8 of
-// 1024 x 1024: 52, 42 and 40; 1664, 13 of 800 x 2160: 29 in 128 x 128 and 36 in 64 x 64; 12416, 6 of 41 x 448: 23 and 20.  Float32: 2240
-// rows, 15 of 3014 x 192: 85 and 48; 8192, 8 of 1024 x 1536: 203 and 209.
+// 1024 x 1024: 52, 42 and 40; 1664, 13 of 800 x 2160: 29 in 128 x 128 and 36 in 64 x 64; 17385, 2 of 64 x 988: 29 and 25; 30000, 4 of
+// 64 x 2048: 38 and 45.  Float32: 2240 rows, 15 of 3014 x 192: 85 and 48; 8192, 8 of 1024 x 1024, skewed: 235 and 147, of 1024 x 1536:
+// 203 and 209.
 int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t experts, int64_t ni, int64_t nj)
 {
   const auto groups = [&](int t, int64_t steps) {
@@ -421,7 +422,7 @@ int outer_tile(const OpSpec &sp, const ProductVariant &v, int64_t rows, int64_t 
     return tiles * std::max(experts, rows / least);
   };
   if (has_tile(sp, v, kLarge) && rows < (1 << 28) && ni >= 256 && nj >= 256 && groups(kLarge, 16) >= 256) return kLarge;
-  return groups(kMiddle, 8) >= (sp.type == 0 ? 1024 : 256) ? kMiddle : kSquare;
+  return groups(kMiddle, 8) >= (sp.type == 0 ? 3000 : 512) ? kMiddle : kSquare;
 }
 // ... and the rows of a piece (0: segments are not cut), where whole segments make too few tiles to fill the compute units:
 // 17110 Float32 rows, 13 results of 64 x 64: 17 us and 369 uncut; 30043, 3 of 64 x 768: 45 and 799.
