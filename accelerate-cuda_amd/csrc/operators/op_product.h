@@ -48,7 +48,9 @@ ACC_DEV unsigned int op_place_of(const int r, const int stride) { return r < 0 ?
  * that starts at the tile (or the step) and ends where the rows that count do: what lies beyond reads as zeros, and
  * addresses are one offset of 32 bits a chunk (the driver sees to it that they suffice).
  * Otherwise rows start anywhere; chunks go by way of registers, with addresses of 64 bits.  A chunk that would reach
- * beyond its row's end is read that much earlier and shifted into place, so that no read leaves its row. */
+ * beyond its row's end is read that much earlier and shifted into place, or, across r, where it ends within the next row
+ * and that is there, read as it lies (see `whole`): no read leaves the operand.  128 x 128 tiles, half, 5003 rows of 24 segments
+ * by 1333 x 1001: 46 us, 41 in the aligned form by 1336 x 1000; 5000 x 5001 x 5001: 475, so that large ones are copied first. */
 template <bool FAST, int TILE, int WAVES, int LIST> struct op_operand {
   static constexpr int CHUNKS = TILE * 8;                         /* of a step */
   static constexpr int MINE = (CHUNKS + OP_THREADS - 1) / OP_THREADS;

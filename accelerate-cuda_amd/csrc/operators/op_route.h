@@ -142,11 +142,11 @@ ACC_DEV long long op_share(const acc_route_args &p) { return (long long)((p.bloc
 
 /* Place of every slot from first on, below last, of one wave: `start[e]` is the place of its first slot of expert e.  64 at a
  * time, in order; lanes of the same expert find one another bit by bit. */
-ACC_DEV void op_place(const acc_route_args &p, const long long first, const long long last, int *start, const int bits, const int lane)
+ACC_DEV void op_place(const acc_route_args &p, const int *chosen, const long long first, const long long last, int *start, const int bits, const int lane)
 {
   for (long long s = first; s < last; s += 64) {
     const long long mine = s + lane;
-    const int e = mine < last ? p.chosen[mine] : -1;
+    const int e = mine < last ? chosen[mine] : -1;
     unsigned long long same = __ballot(e >= 0);
     for (int b = 0; b < bits; ++b) {
       const unsigned long long has = __ballot((e >> b) & 1);
@@ -366,12 +366,12 @@ extern "C" __global__ void __launch_bounds__(OP_TALL_THREADS) route(const acc_ro
 extern "C" __global__ void __launch_bounds__(OP_THREADS) route(const acc_route_args p)
 {
   if (p.guard && *p.guard == 0u) return;
-  extern __shared__ int shared[];                  /* OP_WAVES * experts counts, experts bases, experts totals */
+  extern __shared__ int shared[];                  /* OP_WAVES * experts counts, experts bases, experts totals, a single workgroup's slots */
   __shared__ int all;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sub = lane % OP_LANES;
   const long long first = (long long)blockIdx.x * p.block, last = acc_min<long long>(p.tokens, first + p.block), share = op_share(p);
   const long long mine = first + wave * share, end = acc_min(last, mine + share);
-  int *counts = shared, *base = shared + OP_WAVES * p.experts, *sums = base + p.experts;
+  int *counts = shared, *base = shared + OP_WAVES * p.experts, *sums = base + p.experts, *slots = sums + p.experts;
   for (int i = tid; i < OP_WAVES * p.experts; i += OP_THREADS) counts[i] = 0;
   __syncthreads();
 
@@ -424,6 +424,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route(const acc_route_a
       if (here && j < p.choose) {
         const int e = op_index_of(chosen[s]);
         p.chosen[t * p.choose + j] = e;
+        if (p.blocks == 1) slots[t * p.choose + j] = e;
         p.weights[t * p.choose + j] = e < 0 ? 0.0f : power[s] / total;
         if (e >= 0) atomicAdd(&counts[wave * p.experts + e], 1);
       }
@@ -444,7 +445,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route(const acc_route_a
   __syncthreads();
   op_bases(p, base, sums, true, tid, &all);
   op_starts(p, counts, base, tid);
-  op_place(p, mine * p.choose, end * p.choose, counts + wave * p.experts, op_index_bits(p.experts), lane);
+  op_place(p, slots, mine * p.choose, end * p.choose, counts + wave * p.experts, op_index_bits(p.experts), lane);
   for (long long s = all + tid; s < p.tokens * p.choose; s += OP_THREADS) p.order[s] = -1;
 }
 
@@ -501,7 +502,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route_place(const acc_r
   __syncthreads();
   op_bases(p, base, sums, blockIdx.x == 0, tid, &all);
   op_starts(p, counts, base, tid);
-  op_place(p, mine, end, counts + wave * p.experts, op_index_bits(p.experts), lane);
+  op_place(p, p.chosen, mine, end, counts + wave * p.experts, op_index_bits(p.experts), lane);
   /* what lies behind the last expert's slots, each workgroup its part */
   for (long long s = acc_max<long long>(all, first * p.choose) + tid; s < last * p.choose; s += OP_THREADS) p.order[s] = -1;
 }
