@@ -435,7 +435,9 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
 {
   const int64_t target = v.tile == kLarge ? 256 : v.tile == kMiddle ? 512 : 1024, step = 128 / type_bytes(sp.type);
   if (experts * tiles >= target) return 0;
-  const int64_t least = (v.tile == kLarge ? 16 : 8) * step, piece = ceil_div(std::max(least, ceil_div(rows * tiles, target - experts * tiles)), step) * step;
+  const int64_t least = (v.tile == kLarge ? 16 : 8) * step, most = std::max(least, ceil_div(rows * tiles, target - experts * tiles));
+  // (segments of about the mean length in equal pieces, with a tenth to spare: 23602 rows, 11 of 431 x 576: 55 us, 65 otherwise)
+  const int64_t mean = ceil_div(rows, experts), each = ceil_div(mean, ceil_div(mean, most)), piece = ceil_div(std::max(least, std::min(most, each + each / 10)), step) * step;
   return experts * piece >= 2 * rows ? 0 : (int32_t)piece;
 }
 
