@@ -437,7 +437,7 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
   if (experts * tiles >= target) return 0;
   const int64_t least = (v.tile == kLarge ? 16 : 8) * step, most = std::max(least, ceil_div(rows * tiles, target - experts * tiles));
   // (segments of about the mean length in equal pieces, with a tenth to spare: 23602 rows, 11 of 431 x 576: 55 us, 65 otherwise)
-  const int64_t mean = ceil_div(rows, experts), each = ceil_div(mean, ceil_div(mean, most)), piece = ceil_div(std::max(least, std::min(most, each + each / 10)), step) * step;
+  const int64_t mean = std::max<int64_t>(1, ceil_div(rows, experts)), each = ceil_div(mean, ceil_div(mean, most)), piece = ceil_div(std::max(least, std::min(most, each + each / 10)), step) * step;
   return experts * piece >= 2 * rows ? 0 : (int32_t)piece;
 }
 
