@@ -452,15 +452,16 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
   b.base += acc_max(expert, 0) * p.b_expert * op_b::SIZE;
   b.index = (const int *)0;
   b.limit = p.k;
+  /* (both end where the sum does, which in pieces is not where the rows do: the step behind it has to be zeros, see the loop) */
   a.lo = i0;
   a.hi = iend;
-  a.extent = p.k;
+  a.extent = r1;
   b.lo = 0;
   if (OP_B_FAST) {
     b.hi = jend;
-    b.extent = p.k;
+    b.extent = r1;
   } else {
-    b.hi = p.k;
+    b.hi = r1;
     b.base += (long long)j0 * op_b::SIZE;
     b.extent = jend - j0;
   }
@@ -508,7 +509,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
      * one step ahead. */
     int fsa[OP_SM], fsb[OP_SN], gsa[OP_SM], gsb[OP_SN];
     static_assert(OP_BM + OP_BN <= OP_THREADS, "a lane a row");
-    const int at = tid % (OP_BM + OP_BN), blocks = p.k / 16;
+    const int at = tid % (OP_BM + OP_BN), blocks = r1 / 16;
     const bool of_a = at < OP_BM;
     const int si = of_a ? at : at - OP_BM, share = of_a ? op_a::SHARE : op_b::SHARE;
     const int scale_row = of_a ? a.number(i0 + si) : b.number(j0 + si);
@@ -642,7 +643,8 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
       op_half(c, OP_ROLL ? fa : ga, gb, fa, fb, OP_SCALES_G there, wa, wb, 0, nothing);
     };
 #endif
-    /* (an odd number of steps has one of zeros behind it: with a way out between the two, the sums would change registers) */
+    /* (An odd number of steps has one of zeros behind it: with a way out between the two, the sums would change registers.  What
+     * makes it zeros is that operands end at r1 -- extent along r, hi across it -- and not where their rows do.) */
     int r = r0;
 #if OP_ALIGNED
     if (i0 + wi >= iend) {

@@ -1013,3 +1013,57 @@ def test_arrays_beyond_two_and_four_gigabytes(A, ctx, ops, apart):
     micro.rows(fc.array, fe.array, turned(wc, 32), turned(ws, 2), ctx.array(np.array([0, rows], np.int32)), fo.array)
     want = v.astype(float) @ v.T.astype(float)
     assert np.array_equal(fo.get(), want.astype(np.float16))
+
+
+# ------------------------------------------------------------------------------ sums in pieces of an odd number of steps
+
+# A tile of 32 x 64 or 64 x 128, few enough that sums are cut; a step of a sum is 128 bytes, and pieces of nine steps or more are
+# wanted of which there are an odd number: steps * tiles / 512, rounded up.  rows, experts, n, k, segments, w's order, index
+PIECES = {
+    "half": [(128, 1, 1152, 4096, "even", "nk", 0), (128, 1, 1152, 4096, "even", "kn", 2), (256, 1, 2304, 4096, "gaps", "nk", 0), (127, 2, 1086, 4090, "skewed", "kn", 0),
+             (12, 3, 1472, 4096, "even", "kn", 0)],
+    "bfloat16": [(128, 1, 1152, 4096, "gaps", "nk", 2), (128, 1, 1152, 4096, "even", "kn", 0), (125, 1, 1151, 4093, "even", "nk", 0)],
+    "float": [(150, 1, 960, 4096, "even", "nk", 0), (150, 1, 960, 4096, "gaps", "kn", 3), (12, 7, 1472, 1024, "even", "kn", 0), (149, 1, 959, 4095, "even", "nk", 2)],
+}
+
+
+@pytest.mark.parametrize("lead,extra", [(0, 0), (8, 8), (1, 3)])
+@pytest.mark.parametrize("elt,case", [(elt, case) for elt in TYPES for case in PIECES[elt]])
+def test_every_step_of_a_sum_in_pieces_counts_once(A, ctx, ops, elt, case, lead, extra):
+    """whole numbers, whose sums are exact; a step counted twice, or not at all, is another sum"""
+    rows, experts, n, k, kind, order, per = case
+    say("pieces", elt, case, lead, extra)
+    rng = np.random.default_rng(rows + n + k)
+    offsets = segments(rng, rows, experts, kind)
+    tokens = rows if not per else rows // per + 1
+    index = rng.integers(0, tokens * per, rows).astype(np.int32) if per else None
+    if per:
+        index[[0, rows - 1]] = (-1, tokens * per)
+    x, w = rng.integers(-1, 2, (tokens, k)).astype(float), rng.integers(-1, 2, (experts, n, k)).astype(float)
+    named = np.arange(rows) if not per else np.where(index < 0, tokens, index // per)
+    taken = np.concatenate([x, np.zeros((1, k))])[np.minimum(named, tokens)]
+    want = np.zeros((rows, n))
+    for e in range(experts):
+        want[offsets[e]:offsets[e + 1]] = taken[offsets[e]:offsets[e + 1]] @ w[e].T
+    dx, dw = Boxed(A, ctx, store(x, elt), elt, lead, extra, np.nan), Boxed(A, ctx, store(w, elt), elt, lead, extra, np.nan, swap=order == "kn")
+    out = Boxed(A, ctx, np.ones((rows, n), STORED[elt]), elt, lead, extra, 7.0)
+    ops("Product", elt).rows(dx.array, dw.array, ctx.array(offsets), out.array, index=None if index is None else ctx.array(index), per=per)
+    assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
+
+
+@pytest.mark.parametrize("elt,rows,n,k", [("half", 128, 1280, 13824), ("bfloat16", 128, 1280, 13824), ("float", 127, 1277, 13800), ("half", 128, 1280, 13696)])
+def test_every_step_of_a_sum_of_four_bit_numbers_in_pieces_counts_once(A, ctx, ops, elt, rows, n, k):
+    say("micro pieces", elt, rows, n, k)
+    rng = np.random.default_rng(k)
+    # ones, halves and their negatives under scales of one: quarters, whose sums are exact
+    grid = np.array([0.0, 0.5, 1.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, -0.5, -1.0])
+    blocks = (k + 31) // 32
+    cx, cw = rng.choice([0, 1, 2, 9, 10], (rows, blocks * 32)), rng.choice([0, 1, 2, 9, 10], (n, blocks * 32))
+    ones = lambda m: ctx.array(np.full((m, blocks), 127, np.uint8))
+    sw = ones(n)
+    out = Boxed(A, ctx, np.ones((rows, n), STORED[elt]), elt, 8, 8, 7.0)
+    dw = ctx.array(packed(cw))
+    ops("Microscale", elt).rows(ctx.array(packed(cx)), ones(rows), A.Strided((1, n, 16 * blocks), (n * 16 * blocks, 16 * blocks, 1), dw.ptr, dw),
+                                A.Strided((1, n, blocks), (n * blocks, blocks, 1), sw.ptr, sw), ctx.array(np.array([0, rows], np.int32)), out.array)
+    want = grid[cx] @ grid[cw].T
+    assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
