@@ -53,27 +53,37 @@ ACC_DEV acc_u4 op_shifted(const acc_u4 v, const int bytes)
 }
 
 /* The segments of the rows 0 .. rows-1: number 0 is what lies before the first expert's rows, s the rows of expert s - 1,
- * experts + 1 what lies behind the last one's.  Starts that are out of range or out of order are pulled into it, so that no
- * row outside the array is ever named. */
-ACC_DEV void op_segment(const int *offsets, const int experts, const int rows, const int s, int *begin, int *end)
+ * experts + 1 what lies behind the last one's.  A start that is out of range counts as the nearest row, one that goes back as the
+ * largest before it: whatever the starts say, a row is in one segment, so that no row outside the array is ever named, and all
+ * segments together have no more tiles than the driver has allowed for. */
+ACC_DEV int op_start(const int *offsets, const int experts, const int rows, const int s)
 {
-  /* (both are read whether they count or not: two loads at once, and no branch) */
-  const int before = offsets[acc_max(s - 1, 0)], at = offsets[acc_min(s, experts)];
-  const int b = s <= 0 ? 0 : before, e = s > experts ? rows : at;
-  *begin = acc_min(acc_max(b, 0), rows);
-  *end = acc_max(*begin, acc_min(e, rows));
+  /* (read whether it counts or not: no branch) */
+  const int at = offsets[acc_min(s, experts)];
+  return s > experts ? rows : acc_min(acc_max(at, 0), rows);
 }
 
-/* the lane's of 64 segments from number `base` on; behind the last one none */
+/* the lane's of 64 segments from number `base` on, of which the first begins at row `from` (0, or the end of the 64 before
+ * them); behind the last one none */
 struct op_lot { int begin, end; };
-ACC_DEV op_lot op_segments(const int *offsets, const int experts, const int rows, const int base)
+ACC_DEV op_lot op_segments(const int *offsets, const int experts, const int rows, const int base, const int from)
 {
-  const int s = base + acc_lane();
+  const int lane = acc_lane();
+  const int upto = acc_wave_scan(op_start(offsets, experts, rows, base + lane), [](int x, int y) { return acc_max(x, y); }, lane);
   op_lot l;
-  op_segment(offsets, experts, rows, acc_min(s, experts + 1), &l.begin, &l.end);
-  if (s > experts + 1) l.end = l.begin;
+  l.end = acc_max(from, upto);
+  l.begin = acc_wave_shift_up1(l.end);
+  if (lane == 0) l.begin = from;
   return l;
 }
+/* the next 64, from number `base` on */
+ACC_DEV op_lot op_segments_behind(const int *offsets, const int experts, const int rows, const int base, const op_lot lot)
+{
+  return op_segments(offsets, experts, rows, base, acc_readlane(lot.end, 63));
+}
+
+/* runs of `height` rows that `n` rows make, the last of them shorter (n + height may pass 2^31) */
+ACC_DEV int op_runs(const int n, const int height) { return (int)(((unsigned int)n + (unsigned int)height - 1u) / (unsigned int)height); }
 
 /* Workgroups go to the eight dies in turn: block b of n as a number such that every die has a run of neighbours. */
 ACC_DEV long long op_die_run(const long long b, const long long n)
@@ -100,7 +110,7 @@ ACC_DEV void op_count_tiles(const int *offsets, const int experts, const int row
     *parts += __popcll(__ballot((lot.end - lot.begin) % height > 0));
     base += 64;
     if (base >= experts + 2) return;
-    lot = op_segments(offsets, experts, rows, base);
+    lot = op_segments_behind(offsets, experts, rows, base, lot);
   }
 }
 
@@ -109,10 +119,13 @@ ACC_DEV void op_count_tiles(const int *offsets, const int experts, const int row
 ACC_DEV int op_nth_longest(const int *offsets, const int experts, const int rows, const int n, int *begin, int *end)
 {
   if (experts > 62) {
-    op_segment(offsets, experts, rows, n + 1, begin, end);
+    int from = 0;                                  /* the largest start up to the segment's own */
+    for (int s = acc_lane(); s <= n; s += 64) from = acc_max(from, op_start(offsets, experts, rows, s));
+    *begin = acc_wave_reduce(from, [](int x, int y) { return acc_max(x, y); });
+    *end = acc_max(*begin, op_start(offsets, experts, rows, n + 1));
     return n;
   }
-  const op_lot lot = op_segments(offsets, experts, rows, 0);
+  const op_lot lot = op_segments(offsets, experts, rows, 0, 0);
   const int s = acc_lane();
   /* (no two of these are the same; a length beyond 2^26 counts as that) */
   const unsigned int mine = s >= 1 && s <= experts ? (unsigned int)(acc_min(lot.end - lot.begin, (1 << 26) - 2) + 1) << 6 | (63 - s) : 0;
@@ -125,7 +138,8 @@ ACC_DEV int op_nth_longest(const int *offsets, const int experts, const int rows
   return at - 1;
 }
 
-struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segment; begin >= end: no such tile */
+/* expert -1: rows of no segment; begin >= end: no such tile; `all`: rows of its segment */
+struct op_tile { int expert, begin, end, all; };
 
 /* How segments are cut into runs of `height` rows: all runs, the last of a segment shorter; its whole runs only; or what is
  * left behind those. */
@@ -138,26 +152,45 @@ struct op_tile { int expert, begin, end; };      /* expert -1: rows of no segmen
 template <int KIND> ACC_DEV op_tile op_find_tile(const int *offsets, const int experts, const int rows, const int height, op_lot lot, int tile)
 {
   const int lane = acc_lane();
-  op_tile t = {-1, 0, 0};
+  op_tile t = {-1, 0, 0, 0};
   for (int base = 0;;) {
     int b = lot.begin;
     const int e = lot.end;
     if (KIND == OP_REST) b = e - (e - b) % height;
-    const int runs = KIND == OP_WHOLE ? (e - b) / height : (e - b + height - 1) / height;
+    const int runs = KIND == OP_WHOLE ? (e - b) / height : op_runs(e - b, height);
     const int upto = acc_wave_scan(runs, [](int x, int y) { return x + y; }, lane);
     const unsigned long long beyond = __ballot(upto > tile);
     if (beyond) {
       const int at = __builtin_ctzll(beyond);
       const int first = acc_readlane(b, at) + (tile - (acc_readlane(upto, at) - acc_readlane(runs, at))) * height;
       t.begin = first;
-      t.end = acc_min(acc_readlane(e, at), first + height);
+      t.end = first + acc_min(acc_readlane(e, at) - first, height);
+      t.all = acc_readlane(e, at) - acc_readlane(lot.begin, at);
       t.expert = base + at == experts + 1 ? -1 : base + at - 1;
       return t;
     }
     tile -= acc_readlane(upto, 63);
     base += 64;
     if (base >= experts + 2) return t;
-    lot = op_segments(offsets, experts, rows, base);
+    lot = op_segments_behind(offsets, experts, rows, base, lot);
+  }
+}
+
+/* Of the runs of `height` rows, counted segment after segment: the first of segment number s, and how many that has. */
+ACC_DEV int op_first_run(const int *offsets, const int experts, const int rows, const int height, const int s, int *runs)
+{
+  const int lane = acc_lane();
+  int first = 0;
+  op_lot lot = op_segments(offsets, experts, rows, 0, 0);
+  for (int base = 0;;) {
+    const int mine = op_runs(lot.end - lot.begin, height);
+    first += acc_wave_reduce(base + lane < s ? mine : 0, [](int x, int y) { return x + y; });
+    if (s - base < 64) {
+      *runs = acc_readlane(mine, s - base);
+      return first;
+    }
+    base += 64;
+    lot = op_segments_behind(offsets, experts, rows, base, lot);
   }
 }
 

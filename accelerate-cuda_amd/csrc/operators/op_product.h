@@ -371,11 +371,10 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     if (p.piece == 0) {
       expert = op_nth_longest(p.offsets, p.experts, (int)p.rows, n, &r0, &r1);
     } else {
-      const op_tile run = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, p.piece, op_segments(p.offsets, p.experts, (int)p.rows, 0), n);
+      const op_tile run = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, p.piece, op_segments(p.offsets, p.experts, (int)p.rows, 0, 0), n);
       if (run.expert < 0) return;
       expert = run.expert;
-      op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &r0, &r1);
-      if (r1 - r0 > p.piece) part = p.parts + (long long)n * p.ni * p.nj;
+      if (run.all > p.piece) part = p.parts + (long long)n * p.ni * p.nj;
       r0 = run.begin;
       r1 = run.end;
     }
@@ -390,7 +389,7 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) __attribute__((amdgpu_w
     /* Whole tiles first, then those that end a segment, which take less long.  (The grid is for the worst lengths; the tiles
      * that there are, are shared out evenly.) */
     int whole, rest, i, j;
-    const op_lot lot = op_segments(p.offsets, p.experts, (int)p.rows, 0);
+    const op_lot lot = op_segments(p.offsets, p.experts, (int)p.rows, 0, 0);
     op_count_tiles(p.offsets, p.experts, (int)p.rows, OP_BM, lot, &whole, &rest);
     const unsigned int grid = (unsigned int)(p.tiles_i * p.tiles_j), n = p.piece ? blockIdx.x / grid : 0u, at = blockIdx.x - n * grid;
     const long long first = (long long)whole * p.tiles_j, all = first + (long long)rest * p.tiles_j;
@@ -706,15 +705,9 @@ extern "C" __global__ void __launch_bounds__(256) product_join(const acc_product
 #if OP_OUTER
   const int blocks = (int)(((long long)p.ni * quads + 255) / 256), expert = (int)(blockIdx.x / blocks), rows = p.ni;
   const long long u = (long long)(blockIdx.x % blocks) * 256 + threadIdx.x, apart = (long long)p.ni * p.nj;
-  int begin, end, first = 0;
-  op_segment(p.offsets, p.experts, (int)p.rows, expert + 1, &begin, &end);
-  const int pieces = (end - begin + p.piece - 1) / p.piece;
+  int pieces;
+  const int first = op_first_run(p.offsets, p.experts, (int)p.rows, p.piece, expert + 1, &pieces);
   if (pieces == 1) return;
-  for (int base = 0; base <= expert; base += 64) {
-    int b = 0, e = 0;
-    if (base + acc_lane() <= expert) op_segment(p.offsets, p.experts, (int)p.rows, base + acc_lane(), &b, &e);
-    first += acc_wave_reduce((e - b + p.piece - 1) / p.piece, [](int x, int y) { return x + y; });
-  }
   from += first * apart;
   out += (long long)expert * p.out_expert;
 #else

@@ -20,7 +20,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) product(const acc_pr
   if (p.guard && *p.guard == 0u) return;
   __shared__ acc_f4 parts[OP_WAVES - 1][OP_FM * OP_FN][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
-  const op_tile tile = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, OP_BM, op_segments(p.offsets, p.experts, (int)p.rows, 0), (int)(blockIdx.x / p.tiles_j));
+  const op_tile tile = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, OP_BM, op_segments(p.offsets, p.experts, (int)p.rows, 0, 0), (int)(blockIdx.x / p.tiles_j));
   if (tile.begin >= tile.end) return;
   const int j0 = (int)(blockIdx.x % p.tiles_j) * 16 * OP_FN;
 

@@ -1067,3 +1067,30 @@ def test_every_step_of_a_sum_of_four_bit_numbers_in_pieces_counts_once(A, ctx, o
                                 A.Strided((1, n, blocks), (n * blocks, blocks, 1), sw.ptr, sw), ctx.array(np.array([0, rows], np.int32)), out.array)
     want = grid[cx] @ grid[cw].T
     assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
+
+
+# ------------------------------------------------------------------------------ starts in any order
+
+@pytest.mark.parametrize("elt", TYPES)
+@pytest.mark.parametrize("rows,experts,ni,nj", [(5000, 2, 70, 90), (5000, 9, 70, 90), (3001, 70, 33, 40), (6000, 8, 264, 256), (400, 131, 60, 72), (64, 6, 24, 40)])
+def test_starts_that_go_back_count_as_the_largest_before_them(A, ctx, ops, elt, rows, experts, ni, nj):
+    """whole sums and sums in pieces: a row is in one segment, whatever the starts say, and nothing beside the results changes"""
+    say("starts", elt, rows, experts, ni, nj)
+    rng = np.random.default_rng(rows + experts)
+    a, b, w = rng.integers(-1, 2, (rows, ni)).astype(float), rng.integers(-1, 2, (rows, nj)).astype(float), rng.integers(-1, 2, (experts, nj, ni)).astype(float)
+    da, db, dw = (Boxed(A, ctx, store(v, elt), elt, 8, 8, np.nan) for v in (a, b, w))
+    for offsets in (np.resize([0, rows], experts + 1), np.resize([rows // 2, rows, 0], experts + 1), np.sort(rng.integers(0, rows + 1, experts + 1))[::-1],
+                    rng.integers(-rows, 2 * rows, experts + 1)):
+        offsets = offsets.astype(np.int32)
+        upto = np.maximum.accumulate(np.clip(offsets, 0, rows))
+        do = ctx.array(offsets)
+        out = Boxed(A, ctx, np.ones((experts, ni, nj), STORED[elt]), elt, 8, 8, 7.0)
+        ops("Product", elt).outer(da.array, db.array, do, out.array)
+        want, _ = plain_outer(a, b, upto, experts)
+        assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
+        out = Boxed(A, ctx, np.ones((rows, nj), STORED[elt]), elt, 8, 8, 7.0)
+        ops("Product", elt).rows(da.array, dw.array, do, out.array)
+        want = np.zeros((rows, nj))
+        for e in range(experts):
+            want[upto[e]:upto[e + 1]] = a[upto[e]:upto[e + 1]] @ w[e].T
+        assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
