@@ -818,8 +818,9 @@ try {
   a.out = device<void>(out);
   a.offsets = device<const int32_t>(offsets);
   (turned ? a.index_a : a.index_b) = device<const int32_t>(index);
-  a.a_stride = p->stride[0];
-  a.b_stride = q->stride[0];
+  // (the kernel takes a stride as the length of a row that it may read; that of a single row says nothing)
+  a.a_stride = p->shape[0] > 1 ? p->stride[0] : p->shape[1];
+  a.b_stride = q->shape[0] > 1 ? q->stride[0] : q->shape[1];
   a.out_expert = o.stride[0];
   a.out_stride = o.stride[1];
   a.rows = rows;

@@ -1094,3 +1094,25 @@ def test_starts_that_go_back_count_as_the_largest_before_them(A, ctx, ops, elt, 
         for e in range(experts):
             want[upto[e]:upto[e + 1]] = a[upto[e]:upto[e + 1]] @ w[e].T
         assert np.array_equal(values(out.get(), elt), values(store(want, elt), elt))
+
+
+# ------------------------------------------------------------------------------ strides of a dimension of one
+
+@pytest.mark.parametrize("elt", TYPES)
+@pytest.mark.parametrize("stride", [0, 1, 8, 40, 1 << 40])
+@pytest.mark.parametrize("ni,nj", [(64, 128), (40, 24), (33, 65), (256, 512)])
+def test_a_single_row_is_read_whole_whatever_its_stride(A, ctx, ops, elt, stride, ni, nj):
+    """the stride of a dimension of one element says nothing: a turned column has one of 1, a broadcast one of 0"""
+    rng = np.random.default_rng(ni + nj)
+    a, b, w = (rng.integers(-3, 4, s).astype(float) for s in ((1, ni), (1, nj), (1, nj, ni)))
+    da, db, dw = (ctx.array(store(v, elt)) for v in (a, b, w))
+    row = lambda d, n: A.Strided((1, n), (stride, 1), d.ptr, d)
+    offsets, index = ctx.array(np.array([0, 1], np.int32)), ctx.array(np.array([0], np.int32))
+    for use in (None, index):
+        for order in ("ij", "ji"):
+            out = Boxed(A, ctx, np.ones((1, ni, nj), STORED[elt]), elt, 8, 8, 7.0, swap=order == "ji")
+            ops("Product", elt).outer(row(da, ni), row(db, nj), offsets, out.array, index=use)
+            assert np.array_equal(values(out.get(), elt), a[:, :, None] * b[:, None, :])
+        out = Boxed(A, ctx, np.ones((1, nj), STORED[elt]), elt, 8, 8, 7.0)
+        ops("Product", elt).rows(row(da, ni), A.Strided((1, nj, ni), (stride, ni, 1), dw.ptr, dw), offsets, out.array, index=use)
+        assert np.array_equal(values(out.get(), elt), values(store(a @ w[0].T, elt), elt))
