@@ -500,10 +500,13 @@ int begin(acc_op op, int kind, const char *who, acc_stream stream, const uint32_
   return op->ctx->make_current();
 }
 
+// threads of a launch: their number has 32 bits, and HIP starts those of a larger one that are left over 2^32 without a word
+constexpr int64_t kThreads = 0xffffffffll;
+
 template <typename T>
 int launch(acc_op op, const char *entry, hipFunction_t fn, int64_t grid, int block, size_t lds, acc_stream stream, const T &args)
 {
-  if (grid < 1 || grid > 0x7fffffffLL) return fail(ACC_ERR_INVALID, "%s: grid of %lld workgroups", entry, (long long)grid);
+  if (grid < 1 || grid > kThreads / block) return fail(ACC_ERR_INVALID, "%s: grid of %lld workgroups of %d", entry, (long long)grid, block);
   T copy = args;
   void *slots[] = {&copy};
   return acc::launch_operator(op->ctx, entry, fn, static_cast<unsigned>(grid), static_cast<unsigned>(block), static_cast<unsigned>(lds),
@@ -946,7 +949,18 @@ try {
   a.experts = (int32_t)experts;
   a.choose = (int32_t)choose;
   a.normalise = op->spec.normalise ? 1 : 0;
-  return launch(op, who, var->fn3, ceil_div(tokens, kRouteThreads / v.lanes), kRouteThreads, 0, stream, a);
+  const int64_t each = kRouteThreads / v.lanes, most = kThreads / kRouteThreads * each;
+  for (int64_t first = 0; first < tokens; first += most) {
+    acc_route_args part = a;
+    part.tokens = std::min(most, tokens - first);
+    part.logits = static_cast<const char *>(a.logits) + first * a.logits_stride * bytes;
+    part.dlogits = static_cast<char *>(a.dlogits) + first * a.dlogits_stride * bytes;
+    part.chosen = a.chosen + first * choose;
+    part.weights = a.weights + first * choose;
+    part.dweights = a.dweights + first * choose;
+    ACC_TRY(launch(op, who, var->fn3, ceil_div(part.tokens, each), kRouteThreads, 0, stream, part));
+  }
+  return ACC_OK;
 } ACC_OP_CATCH("acc_exec_route_gradient")
 
 // ---- combination ----------------------------------------------------------------------
@@ -1041,7 +1055,18 @@ try {
   a.dout_stride = dout->stride[0];
   a.choose = (int32_t)place->shape[1];
   a.width = (int32_t)width;
-  return launch(op, who, var->fn2, tokens, 64 * (int)std::max<int64_t>(1, std::min<int64_t>(4, ceil_div(width, 512))), 0, stream, a);
+  const int block = 64 * (int)std::max<int64_t>(1, std::min<int64_t>(4, ceil_div(width, 512)));
+  const int64_t most = kThreads / block;
+  for (int64_t first = 0; first < tokens; first += most) {
+    acc_combine_args part = a;
+    part.tokens = std::min(most, tokens - first);
+    part.dout = static_cast<const char *>(a.dout) + first * a.dout_stride * bytes;
+    part.place = a.place + first * a.choose;
+    part.weights = a.weights ? a.weights + first * a.choose : nullptr;
+    part.dweights = a.dweights ? a.dweights + first * a.choose : nullptr;
+    ACC_TRY(launch(op, who, var->fn2, part.tokens, block, 0, stream, part));
+  }
+  return ACC_OK;
 } ACC_OP_CATCH("acc_exec_combine_gradient")
 
 // ---- 4-bit numbers --------------------------------------------------------------------
@@ -1079,8 +1104,8 @@ static int micro_elements(acc_op op, const char *who, bool back, const acc_strid
   a.k = (int32_t)k;
   a.blocks = (int32_t)blocks;
   set_divisor((int32_t)blocks, &a);
-  // (rows by the bound of a lane's block number, see op_mine)
-  const int64_t most = std::max<int64_t>(1, 0x7fffff00 / blocks);
+  // (four threads a block)
+  const int64_t most = std::max<int64_t>(1, (kThreads - 255) / 4 / blocks);
   for (int64_t first = 0; first < rows; first += most) {
     acc_micro_args part = a;
     part.rows = std::min(most, rows - first);

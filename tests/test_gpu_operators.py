@@ -1116,3 +1116,59 @@ def test_a_single_row_is_read_whole_whatever_its_stride(A, ctx, ops, elt, stride
         out = Boxed(A, ctx, np.ones((1, nj), STORED[elt]), elt, 8, 8, 7.0)
         ops("Product", elt).rows(row(da, ni), A.Strided((1, nj, ni), (stride, ni, 1), dw.ptr, dw), offsets, out.array, index=use)
         assert np.array_equal(values(out.get(), elt), values(store(a @ w[0].T, elt), elt))
+
+
+# ------------------------------------------------------------------------------ calls of more than 2^32 threads
+
+def peek(A, ctx, array, first, count):
+    """`count` rows of a dense array from row `first` on"""
+    n = array.shape[-1]
+    return A.DeviceArray.view(ctx, (count, n), array.dtype, count * n, array.ptr + first * n * array.dtype.itemsize).get()
+
+
+def test_gradient_of_a_combination_of_more_tokens_than_a_launch_has(A, ctx, ops):
+    """a workgroup of 64 threads a token, 2^26 tokens and five"""
+    say("combine_gradient, many tokens")
+    tokens = (1 << 26) + 5
+    place = np.full((tokens, 1), -1, np.int32)
+    named = np.array([0, 7, (1 << 26) - 1, 1 << 26, tokens - 1])
+    place[named, 0] = [3, 0, 4, 1, 2]
+    rng = np.random.default_rng(1)
+    y, dout = rng.integers(-3, 4, (5, 8)).astype(np.float16), rng.integers(-3, 4, (1, 8)).astype(np.float16)
+    one, dy, dweights = ctx.array(dout), ctx.array(np.full((5, 8), 9, np.float16)), ctx.array(np.full((tokens, 1), np.nan, np.float32))
+    ops("Combiner", "half").gradient(A.Strided((tokens, 8), (0, 1), one.ptr, one), ctx.array(y), ctx.array(place), None, dy, dweights)
+    assert np.array_equal(dy.get(), np.repeat(dout, 5, 0))
+    want = np.zeros((tokens, 1), np.float32)
+    want[named, 0] = (y[place[named, 0]].astype(float) * dout).sum(1)
+    assert np.array_equal(dweights.get(), want)
+
+
+def test_more_numbers_in_four_bits_than_a_launch_has_threads(A, ctx, ops):
+    """four threads a block of 32, 2^30 blocks and some: every row the same one"""
+    say("quantise, many blocks")
+    rows, k = (1 << 26) + 3, 512
+    v = np.resize([6, -4, 3, -2, 1.5, -1, 0.5, 0], (1, k)).astype(np.float16)
+    x, codes, scales = ctx.array(v), ctx.empty((rows, k // 2), np.uint8), ctx.empty((rows, k // 32), np.uint8)
+    ops("Microscale", "half").quantise(A.Strided((rows, k), (0, 1), x.ptr, x), codes, scales)
+    want, one, _ = plain_quantise(v.astype(float))
+    for first in (0, (1 << 25) - 2, (1 << 26) - 2, rows - 4):
+        assert np.array_equal(peek(A, ctx, codes, first, 4), np.repeat(packed(want), 4, 0))
+        assert np.array_equal(peek(A, ctx, scales, first, 4), np.repeat(one, 4, 0))
+
+
+def test_gradient_of_more_logits_than_a_launch_has_threads(A, ctx, ops):
+    """64 lanes a token of 257 experts, 2^26 tokens and three, every one with the same logits"""
+    say("route_gradient, many tokens")
+    tokens, experts = (1 << 26) + 3, 257
+    logits = ctx.array(np.zeros((1, experts), np.float16))
+    chosen, weights, dweights = (ctx.empty((tokens, 1), t) for t in (np.int32, np.float32, np.float32))
+    e = (np.arange(tokens) % experts).astype(np.int32)
+    chosen.set(e[:, None])
+    weights.set(np.full((tokens, 1), 1 / 257, np.float32))
+    dweights.set(np.full((tokens, 1), 257.0, np.float32))
+    out = ctx.empty((tokens, experts), np.float16)
+    ops("Router", "half", 1, False).gradient(A.Strided((tokens, experts), (0, 1), logits.ptr, logits), chosen, weights, dweights, out)
+    for first in (0, (1 << 26) - 2, tokens - 4):
+        want = np.full((4, experts), -1 / 257)                # p ([chosen] dw - w dw), of equal p
+        want[np.arange(4), e[first:first + 4]] = 256 / 257
+        assert (np.abs(peek(A, ctx, out, first, 4).astype(float) - want) <= 2.0 ** -10 * np.abs(want)).all()
