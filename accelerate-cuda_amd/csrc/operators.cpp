@@ -301,6 +301,16 @@ int check_shape(const char *who, const char *what, const acc_strided &a, std::in
   return ACC_OK;
 }
 
+// The products' kernels count rows, columns and elements of a sum in 32 bits, and a tile, or the step of a sum asked for ahead, reaches
+// up to 1024 of them beyond the last.
+constexpr int64_t kLongest = 0x7fffffff - 4095;
+int check_extents(const char *who, std::initializer_list<int64_t> extents)
+{
+  for (int64_t n : extents)
+    if (n > kLongest) return fail(ACC_ERR_INVALID, "%s: an extent of %lld (at most %lld)", who, (long long)n, (long long)kLongest);
+  return ACC_OK;
+}
+
 struct Named { const acc_strided *a; int bytes; const char *what; };
 // whether two arrays of rows are different columns of one: rows as far apart, whose stretches lie beside each other
 bool beside(const Named &a, const Named &b)
@@ -696,6 +706,7 @@ try {
   ACC_TRY(check_shape(who, "the result", *out, {rows, n}));
   if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
   ACC_TRY(check_shape(who, "x", *x, {index ? x->shape[0] : rows, k}));
+  ACC_TRY(check_extents(who, {experts, n, k, rows, x->shape[0]}));
   const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "x"}, {w, bytes, "w"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (rows == 0 || n == 0) return ACC_OK;
@@ -775,6 +786,7 @@ try {
     std::swap(o.stride[1], o.stride[2]);
   }
   ACC_TRY(check_result(who, "the result", &o, 3));
+  ACC_TRY(check_extents(who, {experts, out->shape[1], out->shape[2], rows, y->shape[0]}));
   const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "a"}, {y, bytes, "b"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (is_empty(o)) return ACC_OK;
@@ -1159,6 +1171,7 @@ try {
   ACC_TRY(check_shape(who, "the result", *out, {rows, n}));
   if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
   ACC_TRY(check_shape(who, "x", *xscales, {index ? xscales->shape[0] : rows, blocks}));
+  ACC_TRY(check_extents(who, {experts, n, wcodes->shape[2], rows, xcodes->shape[0]}));
   const int bytes = type_bytes(op->spec.type);
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{xcodes, 1, "x"}, {xscales, 1, "x's scales"}, {wcodes, 1, "w"}, {wscales, 1, "w's scales"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (is_empty(*out)) return ACC_OK;

@@ -657,9 +657,9 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * graph keeps that scratch memory, so it is replayed on the stream it was recorded on.
  *
  * Element types are "float", "half" and "bfloat16" (an acc_strided does not say which it holds; the operator does).
- * Extents are below 2^31; strides are in elements, and addresses are computed in 64 bits.  Offsets, indices, places and
- * orders are Int32 and are looked at on the device: values out of range name no row.  An offset counts as the nearest
- * row there is, and one that goes back as the largest before it.                                                */
+ * Extents are below 2^31, those of a product at most 2^31 - 4096; strides are in elements, and addresses are computed in
+ * 64 bits.  Offsets, indices, places and orders are Int32 and are looked at on the device: values out of range name no
+ * row.  An offset counts as the nearest row there is, and one that goes back as the largest before it.           */
 #define ACC_STRIDED_RANK 4
 typedef struct acc_strided {
   int32_t    rank;

@@ -1172,3 +1172,22 @@ def test_gradient_of_more_logits_than_a_launch_has_threads(A, ctx, ops):
         want = np.full((4, experts), -1 / 257)                # p ([chosen] dw - w dw), of equal p
         want[np.arange(4), e[first:first + 4]] = 256 / 257
         assert (np.abs(peek(A, ctx, out, first, 4).astype(float) - want) <= 2.0 ** -10 * np.abs(want)).all()
+
+
+def test_products_of_extents_that_numbers_of_32_bits_would_pass_are_refused(A, ctx, ops):
+    """row 2^31 - 1 and a tile's height are beyond 2^31; arrays of one row over and over, so that nothing large is needed to say it"""
+    p, m = ops("Product", "half"), ops("Microscale", "half")
+    room = ctx.empty((1 << 16,), np.uint8)
+    S = lambda shape, strides: A.Strided(shape, strides, room.ptr, room)
+    offsets = ctx.array(np.array([0, 0], np.int32))
+    for n in (2 ** 31 - 4095, 2 ** 31 - 1):
+        for call in (lambda: p.rows(S((n, 8), (0, 1)), S((1, 8, 8), (64, 8, 1)), offsets, A.Strided((n, 8), (8, 1), 1 << 46)),
+                     lambda: p.rows(S((8, 8), (8, 1)), S((1, n, 8), (0, 0, 1)), offsets, A.Strided((8, n), (n, 1), 1 << 46)),
+                     lambda: p.rows(S((0, n), (0, 1)), S((1, 8, n), (0, 0, 1)), offsets, A.Strided((0, 8), (8, 1), 1 << 46)),
+                     lambda: p.rows(S((n, 8), (0, 1)), S((1, 8, 8), (64, 8, 1)), offsets, A.Strided((8, 8), (8, 1), 1 << 46), index=S((8,), (1,))),
+                     lambda: p.outer(S((n, 8), (0, 1)), S((n, 8), (0, 1)), offsets, A.Strided((1, 8, 8), (64, 8, 1), 1 << 46)),
+                     lambda: p.outer(S((0, n), (0, 1)), S((0, 8), (0, 1)), offsets, A.Strided((1, n, 8), (8 * n, 8, 1), 1 << 46)),
+                     lambda: m.rows(S((n, 16), (0, 1)), S((n, 1), (0, 1)), S((1, 8, 16), (0, 16, 1)), S((1, 8, 1), (0, 1, 1)), offsets, A.Strided((n, 8), (8, 1), 1 << 46))):
+            with pytest.raises(A.AccError) as e:
+                call()
+            assert e.value.code == A.ERR_INVALID and "extent" in e.value.message
