@@ -199,6 +199,7 @@ struct ScratchBlock {
   hipEvent_t done = nullptr;
   bool busy = false;
   bool recorded = false;   // `done` was recorded at the last release
+  bool kept = false;       // calls recorded into a graph on `stream` have it: lent to such calls only, not freed, until the stream goes
   bool dirty = false;      // SCRATCH_LOCKS / SCRATCH_CARRY: a launch may have left it non-zero: cleared again before it is lent
   uint32_t epoch = 0;
 };
@@ -287,11 +288,14 @@ struct acc_context_s {
   int make_current() const;
   // zero-initialised when first allocated; contents persist between uses and
   // follow the block's protocol
-  int scratch_acquire(size_t bytes, hipStream_t stream, int protocol, acc::ScratchRef *out);
+  // `recorded` (SCRATCH_FOLD only): the call goes into a graph, which will use the block whenever it is replayed
+  int scratch_acquire(size_t bytes, hipStream_t stream, int protocol, acc::ScratchRef *out, bool recorded = false);
   void scratch_release(const acc::ScratchRef &ref, hipStream_t stream);
   // a borrower could not leave a SCRATCH_LOCKS / SCRATCH_CARRY block as it found it: cleared before it is lent again
   void scratch_mark_dirty(const acc::ScratchRef &ref);
-  // free every block that is not lent and whose last use has completed; returns the bytes given back
+  // a stream is about to go, and with it the graphs that were recorded on it: their blocks are anybody's again
+  void scratch_forget(hipStream_t stream);
+  // free every block that is neither lent nor a graph's and whose last use has completed; returns the bytes given back
   size_t scratch_trim();
   size_t scratch_bytes();
   // ACC_ERR_STUCK (once) if a kernel has reported a wait that ran out since the last call

@@ -613,6 +613,14 @@ try {
 
 // ---- products -----------------------------------------------------------------------
 
+// scratch memory; a graph's own where the call is being recorded into one
+static int scratch_of(acc_op op, acc_stream stream, size_t bytes, acc::ScratchRef *out)
+{
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) != hipSuccess) (void)hipGetLastError();
+  return op->ctx->scratch_acquire(bytes, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, out, capture != hipStreamCaptureStatusNone);
+}
+
 // scratch memory until the call's kernels are enqueued
 struct ScratchHold {
   acc_context ctx = nullptr;
@@ -620,7 +628,7 @@ struct ScratchHold {
   acc::ScratchRef ref;
   int acquire(acc_op op, acc_stream s, size_t bytes)
   {
-    ACC_TRY(op->ctx->scratch_acquire(bytes, static_cast<hipStream_t>(s), acc::SCRATCH_FOLD, &ref));
+    ACC_TRY(scratch_of(op, s, bytes, &ref));
     ctx = op->ctx;
     stream = static_cast<hipStream_t>(s);
     return ACC_OK;
@@ -679,7 +687,7 @@ static int launch_rows(acc_op op, const char *who, const ProductVariant &v, cons
   a.pieces = a.piece ? (int32_t)ceil_div(a.k, a.piece) : 1;
   if (!a.piece) return launch(op, who, var->fn, grid, 64 * t.wm * t.wn, 0, stream, a);
   acc::ScratchRef scratch;
-  ACC_TRY(op->ctx->scratch_acquire((size_t)a.pieces * a.rows * a.nj * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+  ACC_TRY(scratch_of(op, stream, (size_t)a.pieces * a.rows * a.nj * 4, &scratch));
   a.parts = static_cast<float *>(scratch.ptr);
   int rc = launch(op, who, var->fn, grid * a.pieces, 64 * t.wm * t.wn, 0, stream, a);
   if (rc == ACC_OK) rc = launch(op, who, var->fn2, ceil_div(a.rows * ceil_div(a.nj, 4), 256), 256, 0, stream, a);
@@ -853,7 +861,7 @@ try {
   acc::ScratchRef scratch;
   int rc = ACC_OK;
   if (front + bytes_of_parts) {
-    ACC_TRY(op->ctx->scratch_acquire(front + bytes_of_parts, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+    ACC_TRY(scratch_of(op, stream, front + bytes_of_parts, &scratch));
     a.places = static_cast<uint32_t *>(scratch.ptr);
     a.parts = reinterpret_cast<float *>(static_cast<char *>(scratch.ptr) + front);
   }
@@ -914,7 +922,7 @@ try {
   a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, a.block));
   acc::ScratchRef scratch;
   if (a.blocks > 1) {
-    ACC_TRY(op->ctx->scratch_acquire((size_t)a.blocks * (size_t)experts * 4, static_cast<hipStream_t>(stream), acc::SCRATCH_FOLD, &scratch));
+    ACC_TRY(scratch_of(op, stream, (size_t)a.blocks * (size_t)experts * 4, &scratch));
     a.counts = static_cast<uint32_t *>(scratch.ptr);
   }
   int rc = v.tall ? launch(op, who, var->fn, a.blocks, kRouteTallThreads * v.halves, (size_t)experts * 4, stream, a)

@@ -110,7 +110,7 @@ int acc_context_s::make_current() const
   return ACC_OK;
 }
 
-int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protocol, acc::ScratchRef *out)
+int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protocol, acc::ScratchRef *out, bool recorded)
 {
   std::lock_guard<std::mutex> lock(mu);
   if (!scratch_any_stream) {
@@ -126,6 +126,7 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
   for (size_t i = 0; i < scratch.size(); ++i) {
     acc::ScratchBlock &b = scratch[i];
     if (b.busy || b.bytes < bytes || b.protocol != protocol) continue;
+    if (b.kept && !(recorded && b.stream == stream)) continue;       // (a stream's graphs are replayed one behind the other)
     bool reusable = (b.stream == stream) || !b.recorded;
     if (!reusable) reusable = (hipEventQuery(b.done) == hipSuccess);
     if (reusable && (pick < 0 || b.bytes < scratch[pick].bytes)) pick = static_cast<int>(i);
@@ -144,7 +145,8 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
       if (e != hipSuccess) { (void)hipFree(b.ptr); return acc::fail_hip(e, "hipEventCreateWithFlags"); }
     }
     b.protocol = protocol;
-    b.dirty = true;         // cleared below, on the stream that first uses it (not meant to be captured into a graph)
+    // cleared below, on the stream that first uses it; not in a graph, whose blocks' contents do not matter
+    b.dirty = !recorded;
     if (pick >= 0) {
       scratch[pick] = b;
     } else {
@@ -163,6 +165,7 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
   }
   if (protocol == acc::SCRATCH_SCAN || protocol == acc::SCRATCH_FLAGS) ++b.epoch;
   b.busy = true;
+  b.kept = b.kept || recorded;
   b.stream = stream;
   out->index = pick;
   out->ptr = b.ptr;
@@ -177,7 +180,7 @@ void acc_context_s::scratch_release(const acc::ScratchRef &ref, hipStream_t stre
   std::lock_guard<std::mutex> lock(mu);
   acc::ScratchBlock &b = scratch[ref.index];
   b.recorded = false;
-  if (scratch_multi_stream) b.recorded = (hipEventRecord(b.done, stream) == hipSuccess);
+  if (scratch_multi_stream && !b.kept) b.recorded = (hipEventRecord(b.done, stream) == hipSuccess);
   b.stream = stream;
   b.busy = false;
 }
@@ -187,6 +190,17 @@ void acc_context_s::scratch_mark_dirty(const acc::ScratchRef &ref)
   if (ref.index < 0) return;
   std::lock_guard<std::mutex> lock(mu);
   scratch[ref.index].dirty = true;
+}
+
+void acc_context_s::scratch_forget(hipStream_t stream)
+{
+  std::lock_guard<std::mutex> lock(mu);
+  for (acc::ScratchBlock &b : scratch) {
+    if (!b.kept || b.stream != stream) continue;
+    b.kept = false;
+    b.recorded = (hipEventRecord(b.done, stream) == hipSuccess);      // behind whatever of a replay is still under way
+    if (!b.recorded) { (void)hipGetLastError(); (void)hipStreamSynchronize(stream); }
+  }
 }
 
 size_t acc_context_s::scratch_bytes()
@@ -204,7 +218,7 @@ size_t acc_context_s::scratch_trim()
   std::lock_guard<std::mutex> lock(mu);
   size_t freed = 0;
   for (acc::ScratchBlock &b : scratch) {
-    if (b.busy || !b.ptr) continue;
+    if (b.busy || b.kept || !b.ptr) continue;
     if (hipFree(b.ptr) != hipSuccess) { (void)hipGetLastError(); continue; }      // hipFree waits for the device itself
     freed += b.bytes;
     b.ptr = nullptr;
@@ -612,6 +626,7 @@ int acc_stream_destroy(acc_context ctx, acc_stream s)
   if (!ctx) return fail(ACC_ERR_INVALID, "acc_stream_destroy: NULL context");
   ACC_TRY(ctx->make_current());
   acc::scan_order_forget(ctx->device, static_cast<hipStream_t>(s));
+  ctx->scratch_forget(static_cast<hipStream_t>(s));
   {
     // a guard set on the stream goes with it: a later stream commonly gets the same handle value
     std::lock_guard<std::mutex> lock(ctx->mu);

@@ -110,8 +110,8 @@ int acc_context_sync(acc_context ctx);                 /* CUDA.sync */
 
 /* Scratch memory the skeleton drivers keep per context (fold partials, scan descriptors, permute tables and locks,
  * Execute.hs:304-315,402-405 allocate theirs per use) is reused between calls and grows to the largest request.
- * acc_context_trim frees every block that is not in use (it waits for the device first) and reports the bytes
- * given back; acc_context_scratch_bytes says how much is held.  acc_memtable_malloc trims by itself before it
+ * acc_context_trim frees every block that is not in use (it waits for the device first; what a graph's calls were lent
+ * is, see section D) and reports the bytes given back; acc_context_scratch_bytes says how much is held.  acc_memtable_malloc trims by itself before it
  * gives up. */
 int acc_context_trim(acc_context ctx, size_t *freed_bytes);
 int acc_context_scratch_bytes(acc_context ctx, size_t *bytes);
@@ -653,8 +653,10 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * gives the same bits every time.  No result may share memory with another array of the call (other columns of the same
  * rows are apart).  Scratch memory -- pieces of long sums, 16-bit operands whose rows start anywhere copied to where they
  * do not (2 GB at most), a router's counts -- comes from the context's pool, in stream order.  Calls may be recorded into a
- * graph once the same ones have run on that stream (their kernels are loaded then, and the pool has what they need); the
- * graph keeps that scratch memory, so it is replayed on the stream it was recorded on.
+ * graph once the same ones have run on that stream (their kernels are loaded then, and the pool has what they need).  What
+ * scratch memory they take is from then on lent to calls recorded on that stream alone, whose graphs must therefore not run
+ * side by side: replay them on the stream they were recorded on.  It is the pool's again when acc_stream_destroy is called
+ * for the stream, and goes with the context; no graph may be replayed after that.
  *
  * Element types are "float", "half" and "bfloat16" (an acc_strided does not say which it holds; the operator does).
  * Extents are below 2^31, those of a product at most 2^31 - 4096; strides are in elements, and addresses are computed in

@@ -1191,3 +1191,84 @@ def test_products_of_extents_that_numbers_of_32_bits_would_pass_are_refused(A, c
             with pytest.raises(A.AccError) as e:
                 call()
             assert e.value.code == A.ERR_INVALID and "extent" in e.value.message
+
+
+def test_a_graph_keeps_its_scratch_memory_beside_other_streams_and_behind_a_trim(A):
+    """replays of one stream and eager calls of two others at the same time, scratch memory given back in between"""
+    import ctypes as C
+    hip = C.CDLL("libamdhip64.so")
+    hip.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+    hip.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+    hip.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    hip.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+    hip.hipGraphExecDestroy.argtypes = hip.hipGraphDestroy.argtypes = [C.c_void_p]
+    ctx = A.Context(0)
+    rng = np.random.default_rng(11)
+    tokens, experts, choose, width, hidden, rows = 3000, 40, 2, 1500, 96, 40
+    router, product = A.Router(ctx, "float", choose, True), A.Product(ctx, "float")
+
+    class Run(object):
+        """inputs of its own, what they give, and a stream"""
+        def __init__(self):
+            self.stream = ctx.stream()
+            f = lambda *s: rng.integers(-2, 3, s).astype(np.float32)
+            self.x, self.w, self.logits = f(rows, width), f(1, hidden, width), rng.standard_normal((tokens, experts)).astype(np.float32)
+            self.dx, self.dw, self.dl, self.a = ctx.array(self.x), ctx.array(self.w), ctx.array(self.logits), f(tokens, 24)
+            self.da, self.all, self.few = ctx.array(self.a), ctx.array(np.array([0, rows], np.int32)), ctx.array(np.array([0, tokens // 2, tokens], np.int32))
+            whole = lambda *s: ctx.empty(s, np.int32)
+            self.out = dict(chosen=whole(tokens, choose), offsets=whole(experts + 1), order=whole(tokens * choose), place=whole(tokens, choose),
+                            weights=ctx.empty((tokens, choose), np.float32), long=ctx.empty((rows, hidden), np.float32), outer=ctx.empty((2, 24, 24), np.float32))
+            r = plain_route(self.logits.astype(float), choose, True)
+            self.want = dict(chosen=r[0], offsets=r[2], order=r[3], place=r[4], long=self.x @ self.w[0].T,
+                             outer=np.stack([h.T @ h for h in (self.a[:tokens // 2], self.a[tokens // 2:])]))
+
+        def call(self):
+            o = self.out
+            router.route(self.dl, o["chosen"], o["weights"], o["offsets"], o["order"], o["place"], stream=self.stream)
+            product.rows(self.dx, self.dw, self.all, o["long"], stream=self.stream)
+            product.outer(self.da, self.da, self.few, o["outer"], stream=self.stream)
+
+        def right(self):
+            for name, v in self.want.items():
+                assert np.array_equal(self.out[name].get(), v), name
+
+        def clear(self):
+            for v in self.out.values():
+                v.set(np.full(v.shape, 77, v.dtype))
+    one, others = Run(), [Run(), Run()]
+    for r in [one] + others:
+        r.call()
+    ctx.sync()
+    graph, graph_exec = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(one.stream, 2) == 0
+    try:
+        one.call()
+    finally:
+        rc = hip.hipStreamEndCapture(one.stream, C.byref(graph))
+    assert rc == 0 and graph.value and hip.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+    freed, held = C.c_size_t(), C.c_size_t()
+    for replay in range(4):
+        say("replay", replay)
+        for r in [one] + others:
+            r.clear()
+        ctx.sync()
+        A.check(A.lib().acc_context_trim(ctx.handle, C.byref(freed)))
+        A.check(A.lib().acc_context_scratch_bytes(ctx.handle, C.byref(held)))
+        assert held.value > 0                     # (before anything is replayed: the graph's blocks are there)
+        for _ in range(5):
+            assert hip.hipGraphLaunch(graph_exec, one.stream) == 0
+            for r in others:
+                r.call()
+        ctx.sync()
+        for r in [one] + others:
+            r.right()
+    hip.hipGraphExecDestroy(graph_exec)
+    hip.hipGraphDestroy(graph)
+    for r in [one] + others:
+        A.check(A.lib().acc_stream_destroy(ctx.handle, r.stream))
+    A.check(A.lib().acc_context_trim(ctx.handle, C.byref(freed)))
+    A.check(A.lib().acc_context_scratch_bytes(ctx.handle, C.byref(held)))
+    assert held.value == 0
+    for op in (router, product):
+        op.destroy()
+    ctx.close()

@@ -37,3 +37,13 @@ def test_layouts_of_arrays_as_the_library_reads_them(A):
     dense = A.DeviceArray.view(None, (4, 6), __import__("numpy").dtype("f4"), 24, 64)
     assert struct.unpack("@ii4q4qQ", A._layout(dense)) == (2, 0, 4, 6, 0, 0, 6, 1, 0, 0, 64)
     assert A._layout(None) is None
+
+
+def test_scratch_memory_of_recorded_calls_stays_with_the_graph(tmp_path):
+    """on a stand-in for the HIP runtime: what a call recorded into a graph was lent goes to nobody else while the stream lives"""
+    import subprocess
+    here = os.path.join(os.path.dirname(os.path.abspath(__file__)), "operators_host")
+    build = subprocess.run(["make", "-j4", "-C", here, "OUT=%s" % tmp_path, "%s/driver" % tmp_path], capture_output=True, text=True)
+    assert build.returncode == 0, build.stdout[-3000:] + build.stderr[-3000:]
+    run = subprocess.run([str(tmp_path / "driver")], capture_output=True, text=True, env=dict(os.environ, ACC_HIP_CACHE_DIR=str(tmp_path)), timeout=300)
+    assert run.returncode == 0 and "wrong 0" in run.stdout, run.stdout + run.stderr
