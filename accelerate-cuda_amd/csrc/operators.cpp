@@ -160,7 +160,6 @@ std::vector<std::string> op_options()
   return {"-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"};
 }
 
-// every translation unit an instance may need: the build check compiles them all
 // whether products of this form come in that tile
 bool has_tile(const OpSpec &sp, const ProductVariant &v, int t)
 {
@@ -172,6 +171,7 @@ bool has_tile(const OpSpec &sp, const ProductVariant &v, int t)
   return t == kSquare ? v.outer || word : !v.outer;
 }
 
+// every translation unit an instance may need: the build check compiles them all
 std::vector<std::string> all_sources(const OpSpec &sp)
 {
   std::vector<std::string> out;
@@ -207,7 +207,6 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         v.tile = t;
         v.aligned = form < 2;
         v.tiny = form % 2 == 1;
-        if (v.tiny && t == kLarge) continue;
         if (!has_tile(sp, v, t)) continue;
         out.push_back(product_source(sp, v));
       }

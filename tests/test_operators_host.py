@@ -47,3 +47,18 @@ def test_scratch_memory_of_recorded_calls_stays_with_the_graph(tmp_path):
     assert build.returncode == 0, build.stdout[-3000:] + build.stderr[-3000:]
     run = subprocess.run([str(tmp_path / "driver")], capture_output=True, text=True, env=dict(os.environ, ACC_HIP_CACHE_DIR=str(tmp_path)), timeout=300)
     assert run.returncode == 0 and "wrong 0" in run.stdout, run.stdout + run.stderr
+
+
+def test_calls_of_every_size_find_their_units_compiled_and_their_pieces_covered(A, tmp_path):
+    """12 operators, 4000 calls each on the stand-in: what op_compile_only has compiled is all they need, and sums that are cut are
+    cut into pieces that cover them once"""
+    import subprocess
+    here = os.path.join(os.path.dirname(os.path.abspath(__file__)), "operators_host")
+    build = subprocess.run(["make", "-j4", "-C", here, "OUT=%s" % tmp_path, "%s/walk" % tmp_path], capture_output=True, text=True)
+    assert build.returncode == 0, build.stdout[-3000:] + build.stderr[-3000:]
+    A.lib()
+    os.symlink(os.path.join(os.path.dirname(os.path.abspath(A.LIB_PATH)), "acc_compile_worker"), tmp_path / "acc_compile_worker")
+    (tmp_path / "cache").mkdir()
+    run = subprocess.run([str(tmp_path / "walk"), str(tmp_path / "cache")], capture_output=True, text=True, timeout=900)
+    assert run.returncode == 0 and "wrong 0" in run.stdout, run.stdout[-3000:] + run.stderr[-3000:]
+    assert all(int(line.split()[-4]) > 500 for line in run.stdout.splitlines() if line.startswith("bfloat16"))
