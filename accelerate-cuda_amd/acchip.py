@@ -354,6 +354,7 @@ def cache_stats():
 
 class DeviceArray(object):
     """A device-resident array: owner of one acc_malloc'd buffer."""
+    data_ptr = None                                # (what tells a tensor from it, see _layout)
 
     def __init__(self, ctx, shape, dtype, ptr=None, owner=True):
         self.ctx, self.shape, self.dtype = ctx, tuple(int(s) for s in shape), np.dtype(dtype)
@@ -764,6 +765,7 @@ class Skeleton(object):
 class Strided(object):
     """Device memory as an array with strides (in elements): a part of a larger array, or one with its dimensions
     exchanged.  `owner` is whatever keeps the memory."""
+    data_ptr = None
 
     def __init__(self, shape, strides, ptr, owner=None):
         self.shape, self.strides, self.ptr, self.owner = tuple(shape), tuple(strides), ptr, owner
@@ -782,16 +784,26 @@ class Strided(object):
         return Strided(self.shape[:-2] + (self.shape[-1], self.shape[-2]), self.strides[:-2] + (self.strides[-1], self.strides[-2]), self.ptr, self.owner)
 
 
-def _layout(a):
+def _layout(a, size=None):
     """the acc_strided of an array as bytes: a DeviceArray, a Strided, or any tensor that says where it lies (`data_ptr()`,
-    `shape`, `stride()`); None: no array"""
+    `shape`, `stride()`); None: no array.  `size`: the bytes of an element that the operator takes there (an acc_strided does not
+    say; a Strided is taken at its word)"""
     if a is None:
         return None
-    where = getattr(a, "data_ptr", None)
+    where = a.data_ptr
     if where is not None:
-        shape = a.shape
-        return _STRIDED[len(shape)](len(shape), 0, *shape, *a.stride(), where())
+        try:
+            fits = size is None or a.itemsize == size and a.is_cuda
+        except AttributeError:                     # (a tensor that does not say is taken at its word, too)
+            fits = True
+        if not fits:
+            raise AccError(ERR_INVALID, "elements of %d bytes on the device are wanted, not %s on %s" % (size, a.dtype, a.device))
+        stride = a.stride()
+        rank = len(stride)
+        return _STRIDED[rank](rank, 0, *a.shape, *stride, where())
     if not isinstance(a, Strided):
+        if size is not None and a.dtype.itemsize != size:
+            raise AccError(ERR_INVALID, "elements of %d bytes are wanted, not %s" % (size, a.dtype))
         a = Strided.of(a)
     return _STRIDED[len(a.shape)](len(a.shape), 0, *a.shape, *a.strides, a.ptr)
 
@@ -813,7 +825,7 @@ class _Operator(object):
     """One acc_op.  Arrays are given as `_layout` takes them; results go to arrays that the caller has."""
 
     def __init__(self, ctx, *args):
-        self.ctx = ctx
+        self.ctx, self.size = ctx, 4 if args[0] == "float" else 2
         h = C.c_void_p()
         check(lib().acc_op_create(ctx.handle, C.byref(op_desc(self.KIND, *args)), C.byref(h)))
         self.handle = h
@@ -833,13 +845,13 @@ class Product(_Operator):
 
     def rows(self, x, w, offsets, out, index=None, per=0, stream=None):
         """out[m, n] = sum_k x[r(m), k] w[e, n, k] for the rows m of expert e's segment"""
-        rc = _drivers.acc_exec_product_rows(self.handle, _layout(x), _layout(w), _layout(offsets), _layout(index), per, _layout(out), stream)
+        rc = _drivers.acc_exec_product_rows(self.handle, _layout(x, self.size), _layout(w, self.size), _layout(offsets, 4), _layout(index, 4), per, _layout(out, self.size), stream)
         if rc:
             check(rc)
 
     def outer(self, a, b, offsets, out, index=None, per=0, stream=None):
         """out[e, i, j] = sum over the rows m of e's segment of a[m, i] b[r(m), j]"""
-        rc = _drivers.acc_exec_product_outer(self.handle, _layout(a), _layout(b), _layout(offsets), _layout(index), per, _layout(out), stream)
+        rc = _drivers.acc_exec_product_outer(self.handle, _layout(a, self.size), _layout(b, self.size), _layout(offsets, 4), _layout(index, 4), per, _layout(out, self.size), stream)
         if rc:
             check(rc)
 
@@ -852,12 +864,12 @@ class Router(_Operator):
         _Operator.__init__(self, ctx, elt, choose, normalise)
 
     def route(self, logits, experts, weights, offsets, order, place, stream=None):
-        rc = _drivers.acc_exec_route(self.handle, _layout(logits), _layout(experts), _layout(weights), _layout(offsets), _layout(order), _layout(place), stream)
+        rc = _drivers.acc_exec_route(self.handle, _layout(logits, self.size), _layout(experts, 4), _layout(weights, 4), _layout(offsets, 4), _layout(order, 4), _layout(place, 4), stream)
         if rc:
             check(rc)
 
     def gradient(self, logits, experts, weights, dweights, dlogits, stream=None):
-        rc = _drivers.acc_exec_route_gradient(self.handle, _layout(logits), _layout(experts), _layout(weights), _layout(dweights), _layout(dlogits), stream)
+        rc = _drivers.acc_exec_route_gradient(self.handle, _layout(logits, self.size), _layout(experts, 4), _layout(weights, 4), _layout(dweights, 4), _layout(dlogits, self.size), stream)
         if rc:
             check(rc)
 
@@ -871,12 +883,12 @@ class Combiner(_Operator):
 
     def combine(self, y, place, weights, out, stream=None):
         """out[t] = sum_j weights[t, j] y[place[t, j]]; weights None: all 1"""
-        rc = _drivers.acc_exec_combine(self.handle, _layout(y), _layout(place), _layout(weights), _layout(out), stream)
+        rc = _drivers.acc_exec_combine(self.handle, _layout(y, self.size), _layout(place, 4), _layout(weights, 4), _layout(out, self.size), stream)
         if rc:
             check(rc)
 
     def gradient(self, dout, y, place, weights, dy, dweights, stream=None):
-        rc = _drivers.acc_exec_combine_gradient(self.handle, _layout(dout), _layout(y), _layout(place), _layout(weights), _layout(dy), _layout(dweights), stream)
+        rc = _drivers.acc_exec_combine_gradient(self.handle, _layout(dout, self.size), _layout(y, self.size), _layout(place, 4), _layout(weights, 4), _layout(dy, self.size), _layout(dweights, 4), stream)
         if rc:
             check(rc)
 
@@ -889,19 +901,19 @@ class Microscale(_Operator):
         _Operator.__init__(self, ctx, elt)
 
     def quantise(self, x, codes, scales, stream=None):
-        rc = _drivers.acc_exec_micro_quantise(self.handle, _layout(x), _layout(codes), _layout(scales), stream)
+        rc = _drivers.acc_exec_micro_quantise(self.handle, _layout(x, self.size), _layout(codes, 1), _layout(scales, 1), stream)
         if rc:
             check(rc)
 
     def values(self, codes, scales, out, stream=None):
-        rc = _drivers.acc_exec_micro_values(self.handle, _layout(codes), _layout(scales), _layout(out), stream)
+        rc = _drivers.acc_exec_micro_values(self.handle, _layout(codes, 1), _layout(scales, 1), _layout(out, self.size), stream)
         if rc:
             check(rc)
 
     def rows(self, xcodes, xscales, wcodes, wscales, offsets, out, index=None, per=0, stream=None):
         """out[m, n] = sum_k x[r(m), k] w[e, n, k], both in 4 bits"""
-        rc = _drivers.acc_exec_micro_rows(self.handle, _layout(xcodes), _layout(xscales), _layout(wcodes), _layout(wscales), _layout(offsets), _layout(index), per,
-                                          _layout(out), stream)
+        rc = _drivers.acc_exec_micro_rows(self.handle, _layout(xcodes, 1), _layout(xscales, 1), _layout(wcodes, 1), _layout(wscales, 1), _layout(offsets, 4), _layout(index, 4), per,
+                                          _layout(out, self.size), stream)
         if rc:
             check(rc)
 

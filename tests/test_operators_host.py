@@ -62,3 +62,45 @@ def test_calls_of_every_size_find_their_units_compiled_and_their_pieces_covered(
     run = subprocess.run([str(tmp_path / "walk"), str(tmp_path / "cache")], capture_output=True, text=True, timeout=900)
     assert run.returncode == 0 and "wrong 0" in run.stdout, run.stdout[-3000:] + run.stderr[-3000:]
     assert all(int(line.split()[-4]) > 500 for line in run.stdout.splitlines() if line.startswith("bfloat16"))
+
+
+def test_tensors_that_an_operator_cannot_read_are_refused(A):
+    """on the host, or of elements of another size: the kernels would read what is not there"""
+    import numpy as np
+    import torch
+    for t, size in ((torch.zeros(3, 4), 4), (torch.zeros(3, dtype=torch.int64), 4)):
+        with pytest.raises(A.AccError) as e:
+            A._layout(t, size)
+        assert e.value.code == A.ERR_INVALID
+
+    class There(object):                       # a tensor on the device, as far as a layout asks
+        is_cuda, device, shape = True, "cuda:0", (3, 4)
+
+        def __init__(self, itemsize):
+            self.itemsize, self.dtype = itemsize, "of %d bytes" % itemsize
+
+        def data_ptr(self):
+            return 4096
+
+        def stride(self):
+            return (4, 1)
+    assert A._layout(There(2), 2) == A._layout(A.Strided((3, 4), (4, 1), 4096))
+    for itemsize, size in ((4, 2), (2, 4), (8, 4), (4, 1)):
+        with pytest.raises(A.AccError):
+            A._layout(There(itemsize), size)
+        with pytest.raises(A.AccError):
+            A._layout(A.DeviceArray.view(None, (4, 6), np.dtype("f%d" % itemsize), 24, 64), size)
+    # every argument of every call asks
+    class Op(object):
+        def __init__(self, cls, size):
+            self.cls, self.size, self.handle = cls, size, None
+    wrong = There(16)
+    for cls, call, n in ((A.Product, "rows", 4), (A.Product, "outer", 4), (A.Router, "route", 6), (A.Router, "gradient", 5), (A.Combiner, "combine", 4),
+                         (A.Combiner, "gradient", 6), (A.Microscale, "quantise", 3), (A.Microscale, "values", 3), (A.Microscale, "rows", 6)):
+        for k in range(n):
+            with pytest.raises(A.AccError) as e:
+                getattr(cls, call)(Op(cls, 2), *[wrong if k == m else None for m in range(n)])
+            assert "16 bytes" in str(e.value)
+    for cls in (A.Product, A.Microscale):
+        with pytest.raises(A.AccError):
+            cls.rows(Op(cls, 2), *[None] * (4 if cls is A.Product else 6), index=wrong)
