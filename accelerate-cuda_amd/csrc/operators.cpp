@@ -89,11 +89,21 @@ struct RouteVariant {
 
 constexpr int64_t kRouteAlone = 8192;                // up to as many logits go to one workgroup, see route_block
 
-// The form with a lane a token, or two or four that share its logits, is for up to eight choices and rows of 16 bytes or more.  Of 16 bits it takes over beyond 64 experts, with two lanes for up to 128 and four for more, and for fewer experts
-// where there are tokens enough for a wave of 64 a SIMD.  In us, eight chosen of bfloat16, the other form's time last: 4096 tokens of
-// 128: 17 with one lane, 14 with two, 14 with four, 15; 16384 of 512: 51, 35, 28, 47; 65536 of 128: 24, 23, 30, 41; of 64: 17, 20, 27,
-// 25; 16384 of 64: 13 and 12.  Float32 has keys twice as long: 65536 of 128: 57, 48, 53, 56; 16384 of 128: 49, 36, 27, 20, of 512: 173,
-// 114, 63, 65.
+// The form with a lane a token, or two or four that share its logits, is for up to eight choices and rows of 16 bytes or more.  us,
+// bfloat16, eight chosen unless said.
+// How many lanes: one for up to 64 experts, two for up to 128, four for more: with one, two, four, 65536 tokens of 64: 17, 20, 27; 4096
+// of 128: 17, 14, 14; 16384 of 512: 51, 35, 28; Float32, whose keys are twice as long, up to 32: 65536 of 128: 57, 48, 53.
+// From how many tokens on, the other form's time last:
+//   up to 64 experts enough for a wave of 64 a SIMD: 65536 of 64: 17 and 25; 16384: 13 and 12
+//   up to 256 from the second workgroup on: 65 tokens of 128: 10.3 and 13.0, of 256: 11.9 and 14.4; 4096 of 128: 12.0 and 14.8; two
+//     chosen of 65 to 128: 9.8 to 10.7 and 9.9 to 11.1
+//   up to 512, which the other form has eight a lane of: 65: 15.7 and 15.9, four chosen 14.3 and 13.4, one 13.5 and 11.5, one of 501
+//     15.2 and 12.2; 4096, four chosen: 21.5 and 20.7; 6000: 22.0 and 23.4
+//   up to 1024, sixteen a lane: 65 of 576: 19.0 and 35.8, one chosen 15.8 and 15.5; of 1024: 23.7 and 37.9, 19.8 and 17.7
+//   beyond, in rows of whole chunks: 65 of 2048: 39.8 and 28.3; 4096: 67.9 and 58.5; 6000: 67.8 and 65.3, four chosen 63.3 and 61.0; 8192:
+//     67.3 and 70.0; of 1104: 65: 27.3 and 23.6, 6000: 44.4 and 49.1; in other rows 65 of 2047: 44.8 and 40.9, one chosen 38.0 and 39.3;
+//     of 1500, four: 32.1 and 33.6
+//   Float32: 65536 of 128: 48 and 56; 16384 of 128: 27 and 20, of 512: 63 and 65
 RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned, int64_t tokens)
 {
   RouteVariant v;
@@ -104,7 +114,8 @@ RouteVariant route_variant(const OpSpec &sp, int experts, bool aligned, int64_t 
   v.sels = (sp.choose + v.lanes - 1) / v.lanes;
   // (8 tokens of 64: 5.1 us on the device, 5.6 with sixteen waves and the choices read back from memory)
   v.few = tokens > 0 && tokens * v.lanes <= kRouteFewThreads && tokens * experts <= kRouteAlone;
-  const int64_t from = sp.type == 0 ? (experts >= 256 ? 16384 : 65536) : experts > 64 ? 65 : 32768;      // (65: more than one workgroup)
+  const bool early = (experts > 64 && experts <= 256) || (experts > 512 && (experts <= 1024 || v.vec == 1));
+  const int64_t from = sp.type == 0 ? (experts >= 256 ? 16384 : 65536) : early ? 65 : experts > 256 ? 5000 : 32768;      // (65: more than one workgroup)
   v.tall = experts >= epc && sp.choose <= 8 && tokens >= from && tokens * experts > kRouteAlone;
   if (v.tall) v.halves = experts <= (sp.type == 0 ? 32 : 64) ? 1 : experts <= 128 ? 2 : 4;
   return v;

@@ -1272,3 +1272,9 @@ def test_a_graph_keeps_its_scratch_memory_beside_other_streams_and_behind_a_trim
     for op in (router, product):
         op.destroy()
     ctx.close()
+
+
+@pytest.mark.parametrize("elt", TYPES)
+@pytest.mark.parametrize("tokens,experts,choose", [(5003, 300, 3), (5120, 512, 8), (5000, 512, 1), (70, 512, 8), (4999, 384, 4), (100, 1024, 4), (90, 769, 2), (66, 2048, 5), (5100, 2048, 5), (80, 1501, 7)])
+def test_routes_on_both_sides_of_where_its_forms_change(A, ctx, ops, elt, tokens, experts, choose):
+    test_routes(A, ctx, ops, elt, tokens, experts, choose)
