@@ -7,7 +7,7 @@
  * rounded to the nearest, of two as near to the one with the even code, and to 6 above it.
  *
  * Bound by memory: 16384 x 4096 bfloat16 numbers, 134 MB read and 36 written, take 32 us to quantise, 5.3 TB/s (55 with comparisons in
- * place of the target's conversions, and a division by the blocks of a row).
+ * place of the target's conversions, and a division by the blocks of a row), and 35 us to make again, 4.9 TB/s; Float32 52 and 75.
  */
 #include "op_common.h"
 
@@ -25,7 +25,7 @@ template <int N> ACC_DEV void op_values(const unsigned int codes, const float sc
 }
 
 /* A lane's place: eight elements of a block, four lanes a block, blocks row after row.  (Rows by multiplication, the driver's
- * divisor; a call has fewer than 2^31 blocks.) */
+ * divisor; a launch has fewer than 2^30 blocks.) */
 struct op_eight { long long row; int block, first; bool here; };
 ACC_DEV op_eight op_mine(const acc_micro_args &p)
 {

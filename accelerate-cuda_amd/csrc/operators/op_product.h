@@ -11,9 +11,11 @@
  * half's are read; one barrier a step, in its middle, says that everybody's share of the next step has arrived and that
  * nobody reads this one any more, so that the next but one may take its place.
  *
- * A wave of the largest tile has 128 x 64 results in 128 registers, and reads 12 fragments of LDS for 32 products of a half step;
- * what bounds it is that LDS and the matrix cores together leave no time over, then, where sums are short, the 10 us a tile has
- * in front of its first product and behind its last.  Measured: bfloat16 8192^3 along the sum 768 us, 1431 TFLOP/s; the matrix
+ * A wave of the largest tile has 128 x 64 results in 128 registers, and reads 12 fragments of LDS for 32 products of a half step.
+ * Of the cycles in which a compute unit has work, the matrix cores are busy in 78 % (8192^3 bfloat16; outer 72, 4 bits 45) and LDS
+ * in 29 (27, 22), without a bank conflict; what is left are waits for one another at the barrier, two waves a SIMD covering them
+ * only in part, then, where sums are short, the 10 us a tile has in front of its first product and behind its last (32768 rows, 16
+ * of 4096 x 2048: 60 %).  Measured: bfloat16 8192^3 along the sum 768 us, 1431 TFLOP/s; the matrix
  * turned 782, both turned (outer) 819, with an index 868; 4 bits 295, 3730; Float32 4096^3 962, 143.  A sum may be in pieces (few
  * tiles, long sums): each is a workgroup's, goes out in Float32, and product_join adds them up in order.
  */

@@ -508,7 +508,9 @@ extern "C" __global__ void __launch_bounds__(OP_THREADS) route_place(const acc_r
 }
 
 /* d logit_i = w_i (dw_i - sum_j w_j dw_j) of the chosen ones; where the weights are not normalised over them, of all:
- * p_i ([i chosen] dw_i - sum) */
+ * p_i ([i chosen] dw_i - sum).  Bound by waiting: a choice is read, then its weights, and those once more for the lane that has it.
+ * 65536 tokens of 128 bfloat16 logits, eight chosen: 13.8 us normalised (a floor of 4.8 by memory), 19.5 not (8.3); Float32 16.5
+ * (8.3) and 22.7 (15.3); 8 tokens of 64 a launch. */
 extern "C" __global__ void __launch_bounds__(OP_THREADS) route_gradient(const acc_route_args p)
 {
   if (p.guard && *p.guard == 0u) return;
