@@ -29,6 +29,8 @@ COMBINE_GENERIC, COMBINE_ADD, COMBINE_MIN, COMBINE_MAX, COMBINE_AND, COMBINE_OR,
 BOUNDARY = {"clamp": 0, "mirror": 1, "wrap": 2, "constant": 3}
 FLAG_FOLD_RIGHT, FLAG_FAST_MATH, FLAG_GUARDED, FLAG_TILED = 1, 2, 4, 8
 OP_PRODUCT, OP_ROUTE, OP_COMBINE, OP_MICRO = range(4)
+OP_RECUR = 5
+GATES = {"given": 0, "sigmoid": 1}
 STRIDED_RANK = 4
 
 
@@ -80,7 +82,7 @@ class acc_skel_desc(C.Structure):
 
 
 class acc_op_desc(C.Structure):
-    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32)]
+    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32), ("gate", C.c_int32)]
 
 
 # the bytes of an acc_strided, by rank
@@ -127,7 +129,7 @@ acc_memtable_malloc acc_memtable_acquire acc_memtable_release acc_memtable_free 
 acc_memtable_reclaim acc_memtable_get_stats acc_skel_create_async acc_skel_wait acc_skel_poll acc_skel_prefetch acc_compile_threads acc_compile_drain
 acc_tuning_set acc_tuning_text acc_context_set_tuning acc_op_create acc_op_destroy acc_op_compile_only acc_exec_product_rows
 acc_exec_product_outer acc_exec_route acc_exec_route_gradient acc_exec_combine acc_exec_combine_gradient acc_exec_micro_quantise
-acc_exec_micro_values acc_exec_micro_rows""".split()
+acc_exec_micro_values acc_exec_micro_rows acc_exec_recur acc_exec_recur_gradient acc_exec_recur_step""".split()
 
 
 def build(force=False):
@@ -650,7 +652,8 @@ class _Drivers(object):
               "acc_exec_route": (_P, _P, _P, _P, _P, _P, _P, _P), "acc_exec_route_gradient": (_P, _P, _P, _P, _P, _P, _P),
               "acc_exec_combine": (_P, _P, _P, _P, _P, _P), "acc_exec_combine_gradient": (_P, _P, _P, _P, _P, _P, _P, _P),
               "acc_exec_micro_quantise": (_P, _P, _P, _P, _P), "acc_exec_micro_values": (_P, _P, _P, _P, _P),
-              "acc_exec_micro_rows": (_P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P)}
+              "acc_exec_micro_rows": (_P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P),
+              "acc_exec_recur": (_P,) * 9, "acc_exec_recur_gradient": (_P,) * 12, "acc_exec_recur_step": (_P,) * 8}
 
     def __getattr__(self, name):               # (at its first call; an attribute of its own from then on)
         f = C.CFUNCTYPE(C.c_int, *self._TYPES[name])((name, lib()))
@@ -808,26 +811,28 @@ def _layout(a, size=None):
     return _STRIDED[len(a.shape)](len(a.shape), 0, *a.shape, *a.strides, a.ptr)
 
 
-def op_desc(kind, elt, choose=0, normalise=True):
+def op_desc(kind, elt, choose=0, normalise=True, gate="given"):
+    if gate not in GATES:
+        raise AccError(ERR_INVALID, "gates are %s, not %r" % (" or ".join(sorted(GATES)), gate))
     d = acc_op_desc()
-    d.kind, d.elt_type, d.choose, d.normalise = kind, _b(elt), choose, int(normalise)
+    d.kind, d.elt_type, d.choose, d.normalise, d.gate = kind, _b(elt), choose, int(normalise), GATES[gate]
     return d
 
 
-def op_compile_only(kind, elt, choose=0, normalise=True, target="gfx950"):
+def op_compile_only(kind, elt, choose=0, normalise=True, target="gfx950", **more):
     """(translation units, bytes of code) of everything that calls of an operator may need; needs no GPU"""
     units, size = C.c_int32(), C.c_size_t()
-    check(lib().acc_op_compile_only(target.encode(), C.byref(op_desc(kind, elt, choose, normalise)), C.byref(units), C.byref(size)))
+    check(lib().acc_op_compile_only(target.encode(), C.byref(op_desc(kind, elt, choose, normalise, **more)), C.byref(units), C.byref(size)))
     return units.value, size.value
 
 
 class _Operator(object):
     """One acc_op.  Arrays are given as `_layout` takes them; results go to arrays that the caller has."""
 
-    def __init__(self, ctx, *args):
+    def __init__(self, ctx, *args, **more):
         self.ctx, self.size = ctx, 4 if args[0] == "float" else 2
         h = C.c_void_p()
-        check(lib().acc_op_create(ctx.handle, C.byref(op_desc(self.KIND, *args)), C.byref(h)))
+        check(lib().acc_op_create(ctx.handle, C.byref(op_desc(self.KIND, *args, **more)), C.byref(h)))
         self.handle = h
 
     def destroy(self):
@@ -914,6 +919,35 @@ class Microscale(_Operator):
         """out[m, n] = sum_k x[r(m), k] w[e, n, k], both in 4 bits"""
         rc = _drivers.acc_exec_micro_rows(self.handle, _layout(xcodes, 1), _layout(xscales, 1), _layout(wcodes, 1), _layout(wscales, 1), _layout(offsets, 4), _layout(index, 4), per,
                                           _layout(out, self.size), stream)
+        if rc:
+            check(rc)
+
+
+class Recurrence(_Operator):
+    """A gated linear recurrence along the rows of ragged sequences, h[t] = a[t] h[t-1] + b[t] channel by channel.  `gate`: "given", gates
+    are a and values b; "sigmoid", a = 1 / (1 + exp(-gates)) and b = (1 - a) values.  States are Float32."""
+    KIND = OP_RECUR
+
+    def __init__(self, ctx, elt, gate="sigmoid"):
+        _Operator.__init__(self, ctx, elt, gate=gate)
+
+    def scan(self, gates, values, offsets, out, state=None, last=None, index=None, stream=None):
+        """out = h; sequences begin with their row of `state` (None: zeros) and leave what they end with in `last`"""
+        rc = _drivers.acc_exec_recur(self.handle, _layout(gates, self.size), _layout(values, self.size), _layout(offsets, 4), _layout(index, 4), _layout(state, 4), _layout(last, 4),
+                                     _layout(out, self.size), stream)
+        if rc:
+            check(rc)
+
+    def gradient(self, gates, values, offsets, h, dout, dgates, dvalues, state=None, dlast=None, dstate=None, stream=None):
+        """the gradients of gates, values and the states, from those of h and of the states behind the last rows"""
+        rc = _drivers.acc_exec_recur_gradient(self.handle, _layout(gates, self.size), _layout(values, self.size), _layout(offsets, 4), _layout(h, self.size), _layout(dout, self.size),
+                                              _layout(state, 4), _layout(dlast, 4), _layout(dgates, self.size), _layout(dvalues, self.size), _layout(dstate, 4), stream)
+        if rc:
+            check(rc)
+
+    def step(self, gates, values, state, last, out, index=None, stream=None):
+        """one row of many sequences: out[m] = last[index[m]] = a[m] state[index[m]] + b[m]"""
+        rc = _drivers.acc_exec_recur_step(self.handle, _layout(gates, self.size), _layout(values, self.size), _layout(index, 4), _layout(state, 4), _layout(last, 4), _layout(out, self.size), stream)
         if rc:
             check(rc)
 

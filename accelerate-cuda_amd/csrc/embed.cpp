@@ -40,6 +40,7 @@ ACC_EMBED(op_route, "operators/op_route.h")
 ACC_EMBED(op_combine, "operators/op_combine.h")
 ACC_EMBED(op_pack, "operators/op_pack.h")
 ACC_EMBED(op_micro, "operators/op_micro.h")
+ACC_EMBED(op_recur, "operators/op_recur.h")
 
 namespace acc {
 
@@ -69,6 +70,7 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"op_combine.h", acc_embed_op_combine_begin, acc_embed_op_combine_end},
       {"op_pack.h", acc_embed_op_pack_begin, acc_embed_op_pack_end},
       {"op_micro.h", acc_embed_op_micro_begin, acc_embed_op_micro_end},
+      {"op_recur.h", acc_embed_op_recur_begin, acc_embed_op_recur_end},
   };
   return headers;
 }

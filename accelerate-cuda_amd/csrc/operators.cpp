@@ -34,12 +34,13 @@ struct OpSpec {
   int type = 0;                 // 0 float, 1 half, 2 bfloat16
   int choose = 0;
   bool normalise = true;
+  int gate = 0;
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-const char *const kKindName[] = {"product", "route", "combine", "micro"};
+const char *const kKindName[] = {"product", "route", "combine", "micro", "", "recur"};
 int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 // ---- the variants of each kind ------------------------------------------------------
@@ -164,6 +165,22 @@ std::string micro_source(const OpSpec &sp, bool aligned)
   return text;
 }
 
+// recur: a workgroup's tile is eight waves' rows of 64 words of channels.  Rows of a wave, which are held in registers: the
+// gradient has twice as many arrays
+struct RecurVariant {
+  bool back = false, step = false;
+  int rows() const { return back ? 16 : 32; }
+  uint32_t key() const { return (back ? 1u : 0u) | (step ? 2u : 0u); }
+};
+constexpr int kRecurWaves = 8;
+std::string recur_source(const OpSpec &sp, const RecurVariant &v)
+{
+  char text[256];
+  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_GATE %d\n#define OP_BACK %d\n#define OP_STEP %d\n#define OP_R %d\n#include \"acc_hip_device.h\"\n#include \"op_recur.h\"\n",
+                sp.type, sp.gate, v.back ? 1 : 0, v.step ? 1 : 0, v.rows());
+  return text;
+}
+
 std::vector<std::string> op_options()
 {
   // (sums of products may be contracted: nothing here has to round as a scalar expression of the array language does; packed
@@ -210,6 +227,13 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         for (int64_t tokens : {int64_t(0), int64_t(1), int64_t(1) << 20}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
+  } else if (sp.kind == ACC_OP_RECUR) {
+    for (int form = 0; form < 3; ++form) {
+      RecurVariant v;
+      v.back = form == 1;
+      v.step = form == 2;
+      out.push_back(recur_source(sp, v));
+    }
   } else {
     for (bool aligned : {true, false}) out.push_back(micro_source(sp, aligned));
     for (int t = 0; t < kProductTileCount; ++t)
@@ -230,7 +254,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
 int make_spec(const acc_op_desc *d, OpSpec *sp)
 {
   if (!d) return fail(ACC_ERR_INVALID, "acc_op_create: NULL description");
-  if (d->kind < 0 || d->kind >= ACC_OP_KIND_COUNT) return fail(ACC_ERR_INVALID, "acc_op_create: unknown kind %d", d->kind);
+  if (d->kind < 0 || d->kind >= ACC_OP_KIND_COUNT || !*kKindName[d->kind]) return fail(ACC_ERR_INVALID, "acc_op_create: unknown kind %d", d->kind);
   const std::string t = d->elt_type ? d->elt_type : "";
   if (t == "float") sp->type = 0;
   else if (t == "half") sp->type = 1;
@@ -239,6 +263,10 @@ int make_spec(const acc_op_desc *d, OpSpec *sp)
   sp->kind = d->kind;
   sp->choose = d->choose;
   sp->normalise = d->normalise != 0;
+  if (d->kind == ACC_OP_RECUR) {
+    if (d->gate != ACC_GATE_GIVEN && d->gate != ACC_GATE_SIGMOID) return fail(ACC_ERR_INVALID, "acc_op_create: unknown gate %d", d->gate);
+    sp->gate = d->gate;
+  }
   if (d->kind == ACC_OP_ROUTE && (d->choose < 1 || d->choose > 64)) return fail(ACC_ERR_INVALID, "acc_op_create: a router chooses 1 to 64 experts, not %d", d->choose);
   return ACC_OK;
 }
@@ -505,6 +533,16 @@ std::string combine_source_of(const OpSpec &sp, uint32_t key) { return combine_s
 constexpr uint32_t kMicroElements = 1024;            // (above the products' keys)
 std::string micro_source_of(const OpSpec &sp, uint32_t key) { return (key & kMicroElements) ? micro_source(sp, key & 1u) : product_source_of(sp, key); }
 
+std::string recur_source_of(const OpSpec &sp, uint32_t key)
+{
+  RecurVariant v;
+  v.back = key & 1u;
+  v.step = key & 2u;
+  return recur_source(sp, v);
+}
+
+const char *const kRecurNames[] = {"recur", "recur_clear"};
+const char *const kRecurStepNames[] = {"recur_step"};
 const char *const kProductNames[] = {"product", "product_join", "product_places"};
 const char *const kPackNames[] = {"pack"};
 const char *const kRouteNames[] = {"route", "route_place", "route_gradient"};
@@ -1228,5 +1266,221 @@ try {
   set_divisor(per, &a);
   return launch_rows(op, who, v, var, a, stream);
 } ACC_OP_CATCH("acc_exec_micro_rows")
+
+// ---- recurrence -------------------------------------------------------------------------
+
+// states: a Float32 array of `width` columns, or none
+static int check_states(const char *who, const char *what, const acc_strided *a, int64_t width, bool result)
+{
+  if (!a) return ACC_OK;
+  ACC_TRY(result ? check_result(who, what, a, 2) : check_unit(who, what, a, 2));
+  return check_shape(who, what, *a, {a->shape[0], width});
+}
+
+static bool same_array(const acc_strided &a, const acc_strided &b)
+{
+  return a.ptr == b.ptr && a.shape[0] == b.shape[0] && (a.shape[0] <= 1 || a.stride[0] == b.stride[0]);
+}
+
+// where sequences begin and end: states that are replaced in place are the same array
+static int check_replaced(const char *who, const acc_strided *state, const acc_strided *last)
+{
+  if (!state || !last) return ACC_OK;
+  if (state->shape[0] != last->shape[0]) return fail(ACC_ERR_INVALID, "%s: %lld states to begin with, %lld to end with", who, (long long)state->shape[0], (long long)last->shape[0]);
+  return same_array(*state, *last) ? ACC_OK : check_apart(who, {last, 4, "last"}, {{state, 4, "state"}});
+}
+
+// the tiles of all rows, forward or back: a.gates ... are there, the rest is filled in
+static int launch_recur(acc_op op, const char *who, const RecurVariant &v, acc_recur_args &a, acc_stream stream)
+{
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t channels = 64 * (4 / type_bytes(op->spec.type)), tiles = std::max<int64_t>(1, ceil_div(a.rows, (int64_t)kRecurWaves * v.rows())), strips = ceil_div(a.width, channels);
+  if (tiles * strips > kThreads / (64 * kRecurWaves)) return fail(ACC_ERR_INVALID, "%s: %lld rows of %d channels are too many", who, (long long)a.rows, a.width);
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kRecurNames, 2, recur_source_of, &var));
+  a.tiles = (int32_t)tiles;
+  a.strips = (int32_t)strips;
+  a.status = reinterpret_cast<uint32_t *>(op->ctx->status_dev);
+  const int64_t words = tiles * strips * 3 * channels;
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &capture) != hipSuccess) (void)hipGetLastError();
+  const bool recorded = capture != hipStreamCaptureStatusNone;
+  // Workgroups that wait for others are the device's alone, as with the scans; what runs beside a graph nobody knows, so there tiles
+  // are drawn in the order in which workgroups start.
+  const bool ordered = tiles > 1 && !recorded;
+  if (ordered) ACC_TRY(acc::scan_order_before(op->ctx->device, st));
+  acc::ScratchRef scratch;
+  int rc = op->ctx->scratch_acquire(256 + (size_t)words * 8, st, acc::SCRATCH_FLAGS, &scratch, recorded);
+  if (rc == ACC_OK) {
+    a.words = reinterpret_cast<uint64_t *>(static_cast<char *>(scratch.ptr) + 256);
+    a.tag = scratch.epoch;
+    if (recorded) {
+      a.ticket = static_cast<uint32_t *>(scratch.ptr);
+      rc = launch(op, who, var->fn2, ceil_div(words, 256), 256, 0, stream, a);
+    }
+    if (rc == ACC_OK) rc = launch(op, who, var->fn, tiles * strips, 64 * kRecurWaves, 0, stream, a);
+    op->ctx->scratch_release(scratch, st);
+  }
+  if (ordered) acc::scan_order_after(op->ctx->device);
+  return rc;
+}
+
+int acc_exec_recur(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *offsets, const acc_strided *index,
+                   const acc_strided *state, const acc_strided *last, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_recur";
+  acc_recur_args a = {};
+  ACC_TRY(begin(op, ACC_OP_RECUR, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "gates", gates, 2));
+  ACC_TRY(check_unit(who, "values", values, 2));
+  ACC_TRY(check_unit(who, "offsets", offsets, 1));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  if (index) ACC_TRY(check_unit(who, "index", index, 1));
+  const int64_t rows = out->shape[0], width = out->shape[1], sequences = offsets->shape[0] - 1;
+  if (sequences < 0) return fail(ACC_ERR_INVALID, "%s: offsets are one more than sequences", who);
+  ACC_TRY(check_shape(who, "gates", *gates, {rows, width}));
+  ACC_TRY(check_shape(who, "values", *values, {rows, width}));
+  if (index) ACC_TRY(check_shape(who, "index", *index, {sequences}));
+  ACC_TRY(check_states(who, "state", state, width, false));
+  ACC_TRY(check_states(who, "last", last, width, true));
+  ACC_TRY(check_extents(who, {rows, width, sequences}));
+  ACC_TRY(check_replaced(who, state, last));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{gates, bytes, "gates"}, {values, bytes, "values"}, {offsets, 4, "offsets"}, {index, 4, "index"}, {state, 4, "state"}, {last, 4, "last"}}));
+  if (last) ACC_TRY(check_apart(who, {last, 4, "last"}, {{gates, bytes, "gates"}, {values, bytes, "values"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
+  if (width == 0 || sequences == 0 || (rows == 0 && !last)) return ACC_OK;
+  a.gates = device<const void>(gates);
+  a.values = device<const void>(values);
+  a.out = device<void>(out);
+  a.offsets = device<const int32_t>(offsets);
+  a.index = device<const int32_t>(index);
+  a.enter = device<const float>(state);
+  a.leave = device<float>(last);
+  a.gates_stride = gates->stride[0];
+  a.values_stride = values->stride[0];
+  a.out_stride = out->stride[0];
+  a.enter_stride = state ? state->stride[0] : 0;
+  a.leave_stride = last ? last->stride[0] : 0;
+  a.rows = rows;
+  a.width = (int32_t)width;
+  a.sequences = (int32_t)sequences;
+  a.states = (int32_t)(state ? state->shape[0] : last ? last->shape[0] : 0);
+  return launch_recur(op, who, RecurVariant(), a, stream);
+} ACC_OP_CATCH("acc_exec_recur")
+
+int acc_exec_recur_gradient(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *offsets, const acc_strided *h,
+                            const acc_strided *dout, const acc_strided *state, const acc_strided *dlast, const acc_strided *dgates,
+                            const acc_strided *dvalues, const acc_strided *dstate, acc_stream stream)
+try {
+  const char *who = "acc_exec_recur_gradient";
+  acc_recur_args a = {};
+  ACC_TRY(begin(op, ACC_OP_RECUR, who, stream, &a.guard));
+  if (op->spec.gate == ACC_GATE_GIVEN) values = nullptr;
+  ACC_TRY(check_unit(who, "gates", gates, 2));
+  if (op->spec.gate != ACC_GATE_GIVEN) ACC_TRY(check_unit(who, "values", values, 2));
+  ACC_TRY(check_unit(who, "offsets", offsets, 1));
+  ACC_TRY(check_unit(who, "h", h, 2));
+  ACC_TRY(check_unit(who, "dout", dout, 2));
+  ACC_TRY(check_result(who, "dgates", dgates, 2));
+  ACC_TRY(check_result(who, "dvalues", dvalues, 2));
+  const int64_t rows = dout->shape[0], width = dout->shape[1], sequences = offsets->shape[0] - 1;
+  if (sequences < 0) return fail(ACC_ERR_INVALID, "%s: offsets are one more than sequences", who);
+  const Named arrays[] = {{gates, 0, "gates"}, {values, 0, "values"}, {h, 0, "h"}, {dgates, 0, "dgates"}, {dvalues, 0, "dvalues"}};
+  for (const Named &n : arrays)
+    if (n.a) ACC_TRY(check_shape(who, n.what, *n.a, {rows, width}));
+  const Named states[] = {{state, 0, "state"}, {dlast, 0, "dlast"}, {dstate, 1, "dstate"}};
+  for (const Named &n : states)
+    if (n.a) {
+      ACC_TRY(check_states(who, n.what, n.a, width, n.bytes == 1));
+      ACC_TRY(check_shape(who, n.what, *n.a, {sequences, width}));
+    }
+  ACC_TRY(check_extents(who, {rows, width, sequences}));
+  if (dlast && dstate && !same_array(*dlast, *dstate)) ACC_TRY(check_apart(who, {dstate, 4, "dstate"}, {{dlast, 4, "dlast"}}));
+  const int bytes = type_bytes(op->spec.type);
+  const Named results[] = {{dgates, bytes, "dgates"}, {dvalues, bytes, "dvalues"}, {dstate, 4, "dstate"}};
+  for (int k = 0; k < 3; ++k) {
+    if (!results[k].a) continue;
+    ACC_TRY(check_apart(who, results[k], {{gates, bytes, "gates"}, {values, bytes, "values"}, {offsets, 4, "offsets"}, {h, bytes, "h"}, {dout, bytes, "dout"}, {state, 4, "state"}}));
+    if (k < 2) ACC_TRY(check_apart(who, results[k], {{dlast, 4, "dlast"}}));
+    for (int m = 0; m < k; ++m) ACC_TRY(check_apart(who, results[k], {results[m]}));
+  }
+  if (width == 0 || sequences == 0 || (rows == 0 && !dstate)) return ACC_OK;
+  a.gates = device<const void>(gates);
+  a.values = device<const void>(values);
+  a.h = device<const void>(h);
+  a.dout = device<const void>(dout);
+  a.dgates = device<void>(dgates);
+  a.dvalues = device<void>(dvalues);
+  a.offsets = device<const int32_t>(offsets);
+  a.enter = device<const float>(dlast);
+  a.leave = device<float>(dstate);
+  a.state = device<const float>(state);
+  a.gates_stride = gates->stride[0];
+  a.values_stride = values ? values->stride[0] : 0;
+  a.h_stride = h->stride[0];
+  a.dout_stride = dout->stride[0];
+  a.dgates_stride = dgates->stride[0];
+  a.dvalues_stride = dvalues->stride[0];
+  a.enter_stride = dlast ? dlast->stride[0] : 0;
+  a.leave_stride = dstate ? dstate->stride[0] : 0;
+  a.state_stride = state ? state->stride[0] : 0;
+  a.rows = rows;
+  a.width = (int32_t)width;
+  a.sequences = a.states = (int32_t)sequences;
+  RecurVariant v;
+  v.back = true;
+  return launch_recur(op, who, v, a, stream);
+} ACC_OP_CATCH("acc_exec_recur_gradient")
+
+int acc_exec_recur_step(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *index, const acc_strided *state,
+                        const acc_strided *last, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_recur_step";
+  acc_recur_args a = {};
+  ACC_TRY(begin(op, ACC_OP_RECUR, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "gates", gates, 2));
+  ACC_TRY(check_unit(who, "values", values, 2));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  if (index) ACC_TRY(check_unit(who, "index", index, 1));
+  const int64_t rows = out->shape[0], width = out->shape[1];
+  ACC_TRY(check_shape(who, "gates", *gates, {rows, width}));
+  ACC_TRY(check_shape(who, "values", *values, {rows, width}));
+  if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
+  if (!state || !last) return fail(ACC_ERR_INVALID, "%s: %s missing", who, state ? "last" : "state");
+  ACC_TRY(check_states(who, "state", state, width, false));
+  ACC_TRY(check_states(who, "last", last, width, true));
+  ACC_TRY(check_extents(who, {rows, width}));
+  ACC_TRY(check_replaced(who, state, last));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{gates, bytes, "gates"}, {values, bytes, "values"}, {index, 4, "index"}, {state, 4, "state"}, {last, 4, "last"}}));
+  ACC_TRY(check_apart(who, {last, 4, "last"}, {{gates, bytes, "gates"}, {values, bytes, "values"}, {index, 4, "index"}}));
+  if (is_empty(*out)) return ACC_OK;
+  RecurVariant v;
+  v.step = true;
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kRecurStepNames, 1, recur_source_of, &var));
+  a.gates_stride = gates->stride[0];
+  a.values_stride = values->stride[0];
+  a.out_stride = out->stride[0];
+  a.enter_stride = state->stride[0];
+  a.leave_stride = last->stride[0];
+  a.width = (int32_t)width;
+  a.strips = (int32_t)ceil_div(width, 256 * (4 / bytes));
+  const int64_t most = kThreads / 256 / a.strips;
+  for (int64_t first = 0; first < rows; first += most) {
+    // (without index the states' rows go along)
+    const int64_t at = index ? 0 : first;
+    a.gates = device<const char>(gates) + first * gates->stride[0] * bytes;
+    a.values = device<const char>(values) + first * values->stride[0] * bytes;
+    a.out = device<char>(out) + first * out->stride[0] * bytes;
+    a.index = index ? device<const int32_t>(index) + first : nullptr;
+    a.enter = device<const float>(state) + at * state->stride[0];
+    a.leave = device<float>(last) + at * last->stride[0];
+    a.states = (int32_t)std::max<int64_t>(0, state->shape[0] - at);
+    a.rows = std::min(most, rows - first);
+    ACC_TRY(launch(op, who, var->fn, a.rows * a.strips, 256, 0, stream, a));
+  }
+  return ACC_OK;
+} ACC_OP_CATCH("acc_exec_recur_step")
 
 }  // extern "C"

@@ -86,4 +86,25 @@ struct acc_micro_args {
   const uint32_t *guard;
 };
 
+/* the recurrence: see op_recur.h */
+struct acc_recur_args {
+  const void *gates, *values;
+  const void *h, *dout;         /* gradient only: what the recurrence gave, and the gradient of that */
+  void *out;
+  void *dgates, *dvalues;
+  const int32_t *offsets, *index;
+  const float *enter;           /* the states that sequences begin with; gradient: the gradient of those they end with; 0: zeros */
+  float *leave;                 /* ... and where those go that they end with; 0: nowhere */
+  const float *state;           /* gradient: the states that they began with */
+  uint64_t *words;              /* scratch: what tiles leave for those behind them */
+  uint32_t *ticket, *status;    /* ticket 0: workgroups are tiles by their number */
+  int64_t gates_stride, values_stride, h_stride, dout_stride, out_stride, dgates_stride, dvalues_stride;
+  int64_t enter_stride, leave_stride, state_stride;
+  int64_t rows;
+  int32_t width, sequences, states;
+  int32_t tiles, strips;
+  uint32_t tag;
+  const uint32_t *guard;
+};
+
 #endif

@@ -1,0 +1,424 @@
+/*
+ * op_recur.h -- a gated linear recurrence along the rows of ragged sequences, its gradient, and one step of it.
+ *
+ *   h[t] = a[t] h[t-1] + b[t]       per channel; a = gates, b = values (OP_GATE 0), or a = s(gates), b = (1 - a) values with
+ *                                   s(z) = 1 / (1 + e^-z) (OP_GATE 1)
+ *   u[t] = a[t] (dh[t] + u[t+1])    the gradient that goes on to the row before; g = dh[t] + u[t+1] is that of h[t], then
+ *                                   da = g h[t-1], db = g, and for OP_GATE 1  dz = g (h[t-1] - x) a (1 - a), dx = g (1 - a)
+ *
+ * Both are scans of the maps h -> A h + B, the second from the last row to the first (OP_BACK; rows are counted from the end
+ * then).  A row that begins a sequence takes nothing of the row before: it replaces, it does not multiply, so that no infinity
+ * and nothing that is not a number passes from one sequence to the next.
+ *
+ * Bound by memory: every array passes by once.  A workgroup has a tile of 64 OP_V channels and 8 OP_R rows, a wave OP_R of those, all
+ * of them in registers; it goes over them twice, first for the tile's map, and once what comes in from the rows before is known for
+ * the results.  That it finds in what the tiles before have left: their maps (A, B), or the state behind them (H), as 64-bit words
+ * of a Float32 and the launch's tag, which need no fence.  A tile in which a sequence begins leaves a state at once.  Every tile
+ * leaves its map without having waited, so waits end as long as the tiles before are on the device: workgroups start in the order of
+ * their numbers, or (in a graph, beside which anything may run) draw them from a counter.
+ */
+#include "op_common.h"
+
+#define OP_V (4 / (int)sizeof(op_elt))             /* channels of a lane: a word of a row */
+#define OP_WAVES 8
+#define OP_NEAR 32                                 /* tiles in front that are looked at, at once */
+
+/* 32 bits of memory that start wherever an element may */
+typedef unsigned int __attribute__((aligned(sizeof(op_elt)))) op_word;
+
+struct op_pair { float v[OP_V]; };
+ACC_DEV op_pair op_floats(const unsigned int w)
+{
+  op_elt e[OP_V];
+  __builtin_memcpy(e, &w, 4);
+  op_pair f;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) f.v[k] = (float)e[k];
+  return f;
+}
+
+/* a lane's word of a row, which is the same for all lanes, from element `at` on; `valid` of its channels there are (1 to OP_V) */
+ACC_DEV unsigned int op_read(const op_elt *row, const unsigned int at, const int valid)
+{
+  const op_elt *const p = (const op_elt *)((const char *)row + at * (unsigned int)sizeof(op_elt));
+  if (valid == OP_V) return __builtin_nontemporal_load((const op_word *)p);
+  unsigned short h = 0;
+  __builtin_memcpy(&h, p, sizeof(h));
+  return h;
+}
+ACC_DEV void op_write(op_elt *row, const unsigned int at, const int valid, const op_pair &f)
+{
+  op_elt *const p = (op_elt *)((char *)row + at * (unsigned int)sizeof(op_elt));
+  op_elt e[OP_V];
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) e[k] = (op_elt)f.v[k];
+  if (valid == OP_V) {
+    unsigned int w;
+    __builtin_memcpy(&w, e, 4);
+    __builtin_nontemporal_store(w, (op_word *)p);
+  } else if (valid == 1) {
+    *p = e[0];
+  }
+}
+
+/* what a gate keeps and what it takes in, for a gate of OP_GATE 1: 1 / (1 + e) and e / (1 + e) with e = e^-z, of which neither
+ * loses its digits; an exponent beyond 2^126 stays there (the first is below 2^-125 then, and the second 1) */
+struct op_gate { float keep, take; };
+ACC_DEV op_gate op_gate_of(const float z)
+{
+  op_gate g;
+#if OP_GATE
+  const float y = z * -1.44269504f;
+  float t = sizeof(op_elt) == 4 ? __builtin_fmaf(z, -1.44269504f, -y) + z * -1.92596303e-8f : 0.0f;
+  t = __builtin_fabsf(y) <= 126.0f ? t : 0.0f;     /* (what the product's rounding has lost; Float32 alone can show it) */
+  const float most = y > 126.0f ? 126.0f : y;
+  const float e = __builtin_amdgcn_exp2f(most) * (1.0f + t * 0.693147181f);
+  g.keep = sizeof(op_elt) == 4 ? 1.0f / (1.0f + e) : __builtin_amdgcn_rcpf(1.0f + e);
+  g.take = e * g.keep;
+#else
+  g.keep = z;
+  g.take = 1.0f;
+#endif
+  return g;
+}
+
+/* how many of the n offsets, which ascend, are at most `row`; they count as the nearest row there is */
+ACC_DEV int op_upto(const int *offsets, const int n, const int rows, const int row)
+{
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if (acc_min(acc_max(offsets[mid], 0), rows) <= row) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+/* a row of the states, or -1 */
+ACC_DEV long long op_slot(const acc_recur_args &p, const int sequence)
+{
+  const int at = p.index ? p.index[sequence] : sequence;
+  return at >= 0 && at < p.states ? at : -1;
+}
+ACC_DEV op_pair op_state(const float *states, const long long stride, const long long at, const int channel, const int valid)
+{
+  op_pair f;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) f.v[k] = states && at >= 0 && k < valid ? states[at * stride + channel + k] : 0.0f;
+  return f;
+}
+ACC_DEV void op_keep(float *states, const long long stride, const long long at, const int channel, const int valid, const op_pair &f)
+{
+  if (!states || at < 0) return;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k)
+    if (k < valid) states[at * stride + channel + k] = f.v[k];
+}
+
+ACC_DEV void op_put(unsigned long long *d, const unsigned int tag, const op_pair &f)
+{
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) __hip_atomic_store(d + k, (unsigned long long)tag << 32 | __float_as_uint(f.v[k]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+/* whether all of the lane's words carry the tag */
+ACC_DEV bool op_get(const unsigned long long *d, const unsigned int tag, op_pair *f)
+{
+  bool all = true;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) {
+    const unsigned long long w = __hip_atomic_load(d + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    all = all && (unsigned int)(w >> 32) == tag;
+    f->v[k] = __uint_as_float((unsigned int)w);
+  }
+  return all;
+}
+
+#if OP_STEP
+/* one row a sequence: a lane has a word of a row */
+extern "C" __global__ void __launch_bounds__(256) recur_step(const acc_recur_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  const int channel = ((int)blockIdx.x % p.strips * 256 + (int)threadIdx.x) * OP_V, valid = acc_min(p.width - channel, OP_V);
+  const long long row = blockIdx.x / p.strips;
+  if (valid <= 0) return;
+  /* (asked for before it is known whether the row counts) */
+  const op_pair z = op_floats(op_read((const op_elt *)p.gates + row * p.gates_stride, channel, valid));
+  const op_pair x = op_floats(op_read((const op_elt *)p.values + row * p.values_stride, channel, valid));
+  const long long at = op_slot(p, (int)row);
+  if (at < 0) return;
+  op_pair h = op_state(p.enter, p.enter_stride, at, channel, valid);
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) {
+    const op_gate g = op_gate_of(z.v[k]);
+    h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
+  }
+  op_keep(p.leave, p.leave_stride, at, channel, valid, h);
+  op_write((op_elt *)p.out + row * p.out_stride, channel, valid, h);
+}
+#else
+
+struct op_map { op_pair a, b; };
+
+/* the words of a tile's strip: A, B, H */
+ACC_DEV unsigned long long *op_words(const acc_recur_args &p, const long long tile, const int strip, const int plane, const int lane)
+{
+  return (unsigned long long *)p.words + (((tile * p.strips + strip) * 3 + plane) * 64 + lane) * OP_V;
+}
+
+/* sequences without a row leave what they enter with: every tile looks at a share of the sequences */
+ACC_DEV void op_empty_sequences(const acc_recur_args &p, const int rows, const int share, const int lane, const int channel, const int valid)
+{
+  if (!p.leave) return;
+  for (int base = share * 64; base < p.sequences; base += p.tiles * OP_WAVES * 64) {
+    const int s = base + lane, n = acc_min(s, p.sequences - 1);
+    const int begin = acc_min(acc_max(p.offsets[n], 0), rows), end = acc_min(acc_max(p.offsets[n + 1], 0), rows);
+    unsigned long long none = __ballot(s < p.sequences && end <= begin);
+    while (none) {
+      const int j = __builtin_ctzll(none);
+      none &= none - 1;
+      const long long at = op_slot(p, base + j);
+      op_keep(p.leave, p.leave_stride, at, channel, valid, op_state(p.enter, p.enter_stride, at, channel, valid));
+    }
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recur_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  __shared__ op_map maps[OP_NEAR][64];             /* of the waves' rows; then of the tiles before */
+  __shared__ int ends[OP_NEAR];                    /* whether a wave's map forgets what comes in (1), from its first row on (2); then what is there */
+  __shared__ unsigned int drawn;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), rows = (int)p.rows;
+  unsigned int number = blockIdx.x;
+  if (p.ticket) {
+    if (tid == 0) {
+      drawn = atomicAdd(p.ticket, 1u);
+      if (drawn + 1 == gridDim.x) *p.ticket = 0u;  /* (the last there is: the next launch begins with 0) */
+    }
+    __syncthreads();
+    number = __builtin_amdgcn_readfirstlane(drawn);
+  }
+  const int tile = (int)(number / (unsigned int)p.strips), strip = (int)(number % (unsigned int)p.strips);
+  const int channel = (strip * 64 + lane) * OP_V, valid = acc_max(acc_min(p.width - channel, OP_V), 0);
+  if (rows == 0) {
+    op_empty_sequences(p, rows, tile * OP_WAVES + wave, lane, channel, valid);
+    return;
+  }
+
+  /* The wave's rows, in the order of the recurrence: physical row first + r, or (back) first + OP_R - 1 - r.  Rows that there are
+   * not are read as the nearest one, lanes without a channel as the first. */
+  const long long from = ((long long)tile * OP_WAVES + wave) * OP_R, first = OP_BACK ? rows - from - OP_R : from;
+  const int at = valid > 0 ? channel : 0, some = valid > 0 ? valid : acc_min(p.width, OP_V);
+  const bool whole = __ballot(some != OP_V) == 0;
+  const auto row_of = [&](const int r) { return acc_max<long long>(acc_min<long long>(first + (OP_BACK ? OP_R - 1 - r : r), rows - 1), 0); };
+  const auto read_rows = [&](const void *base, const long long stride, const int back, unsigned int (&to)[OP_R]) {
+    if (whole && first >= back && first + OP_R <= rows) {
+      const op_elt *x = (const op_elt *)base + (first + (OP_BACK ? OP_R - 1 : 0) - back) * stride;
+#pragma unroll
+      for (int r = 0; r < OP_R; ++r, x += OP_BACK ? -stride : stride) to[r] = op_read(x, at, OP_V);
+    } else {
+#pragma unroll
+      for (int r = 0; r < OP_R; ++r) to[r] = op_read((const op_elt *)base + acc_max<long long>(row_of(r) - back, 0) * stride, at, some);
+    }
+  };
+  unsigned int zw[OP_R], xw[OP_R];
+  read_rows(p.gates, p.gates_stride, 0, zw);
+  read_rows(OP_BACK ? p.dout : p.values, OP_BACK ? p.dout_stride : p.values_stride, 0, xw);
+
+  /* sequences: lane j counts those that begin up to row first - 1 + j */
+  const long long row = first - 1 + lane;
+  const int upto = op_upto(p.offsets, p.sequences + 1, rows, (int)acc_max<long long>(row, -1)), before = acc_wave_shift_up1(upto);
+  const bool inside = row >= 0 && row < rows && upto >= 1 && upto <= p.sequences, change = lane > 0 && upto > before;
+  const unsigned long long mask = (1ull << OP_R) - 1;
+  const unsigned long long within = __ballot(inside) >> 1 & mask, begins = __ballot(change && inside) >> 1 & mask, stops = __ballot(change) >> 2 & within;
+  const auto turned = [](const unsigned long long m) { return OP_BACK ? __brevll(m) >> (64 - OP_R) : m; };
+  const unsigned long long here = turned(within), resets = turned(OP_BACK ? stops : begins), leaves = turned(OP_BACK ? begins : stops);
+  const auto sequence_of = [&](const int r) { return acc_readlane(upto, (OP_BACK ? OP_R - 1 - r : r) + 1) - 1; };
+  const auto entering = [&](const int r) { return op_state(p.enter, p.enter_stride, op_slot(p, sequence_of(r)), channel, valid); };
+
+  /* The wave's map: from the last row on that begins a sequence.  What enters there is kept: where states are replaced in place, it
+   * may be gone by the time of the second pass.  (Sequences that begin before end in these rows, too.) */
+  const int latest = resets ? 63 - __builtin_clzll(resets) : -1;
+  op_map own;
+  op_pair entered;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) {
+    own.a.v[k] = 1.0f;
+    entered.v[k] = 0.0f;
+  }
+  if (latest >= 0) entered = entering(latest);
+  own.b = entered;
+  const unsigned long long live = latest >= 0 ? here >> latest << latest : here;
+#pragma unroll
+  for (int r = 0; r < OP_R; ++r) {
+    if (!(live >> r & 1)) continue;
+    const op_pair z = op_floats(zw[r]), x = op_floats(xw[r]);
+#pragma unroll
+    for (int k = 0; k < OP_V; ++k) {
+      const op_gate g = op_gate_of(z.v[k]);
+      own.a.v[k] *= g.keep;
+      own.b.v[k] = OP_BACK ? g.keep * (x.v[k] + own.b.v[k]) : __builtin_fmaf(g.keep, own.b.v[k], g.take * x.v[k]);
+    }
+  }
+  /* (the words as they are stay, not what has been made of them: that takes twice the registers) */
+#pragma unroll
+  for (int r = 0; r < OP_R; ++r) {
+    acc_pin(zw[r]);
+    acc_pin(xw[r]);
+  }
+#if OP_BACK
+  /* (on their way while the tiles before are looked at) */
+  unsigned int hw[OP_R], vw[OP_R];
+  read_rows(p.h, p.h_stride, 1, hw);
+  if (OP_GATE) read_rows(p.values, p.values_stride, 0, vw);
+#endif
+  maps[wave][lane] = own;
+  if (lane == 0) ends[wave] = resets & 1 ? 2 : resets ? 1 : 0;
+  __syncthreads();
+
+  /* the waves' maps put together: up to this wave's, and of all */
+  op_map mine, all;
+  bool mine_ends = false, all_ends = false;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) {
+    all.a.v[k] = 1.0f;
+    all.b.v[k] = 0.0f;
+  }
+  mine = all;
+  const bool fresh = __builtin_amdgcn_readfirstlane(ends[0]) == 2;
+#pragma unroll
+  for (int w = 0; w < OP_WAVES; ++w) {
+    if (w == wave) {
+      mine = all;
+      mine_ends = all_ends;
+    }
+    const op_map m = maps[w][lane];
+    const bool e = __builtin_amdgcn_readfirstlane(ends[w]) != 0;
+#pragma unroll
+    for (int k = 0; k < OP_V; ++k) {
+      all.b.v[k] = e ? m.b.v[k] : __builtin_fmaf(m.a.v[k], all.b.v[k], m.b.v[k]);
+      all.a.v[k] *= m.a.v[k];
+    }
+    all_ends = all_ends || e;
+  }
+  const bool known = all_ends || tile == 0;
+  __syncthreads();                                 /* (everybody has read them) */
+  if (wave == 0) {
+    if (known) {
+      op_put(op_words(p, tile, strip, 2, lane), p.tag, all.b);
+    } else {
+      op_put(op_words(p, tile, strip, 0, lane), p.tag, all.a);
+      op_put(op_words(p, tile, strip, 1, lane), p.tag, all.b);
+    }
+  }
+
+  /* What comes in.  Of the tiles in front the nearest OP_NEAR are looked at, a wave takes every eighth, until the nearest state among
+   * them is followed by maps alone; those are applied to it one after the other.  (So a state is the same whoever has put it
+   * together, to the last bit.) */
+  op_pair in;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) in.v[k] = 0.0f;
+  if (tile > 0 && !fresh) {
+    int got[OP_NEAR / OP_WAVES];                   /* 0 nothing, 1 a map, 2 a state */
+#pragma unroll
+    for (int q = 0; q < OP_NEAR / OP_WAVES; ++q) got[q] = 0;
+    int nearest = OP_NEAR;
+    for (int polls = 0;;) {
+#pragma unroll
+      for (int q = 0; q < OP_NEAR / OP_WAVES; ++q) {
+        const int n = q * OP_WAVES + wave, t = tile - 1 - n;
+        if (t < 0 || got[q] == 2) continue;
+        op_map m;
+        if (__ballot(!op_get(op_words(p, t, strip, 2, lane), p.tag, &m.b)) == 0) {
+          got[q] = 2;
+          maps[n][lane].b = m.b;
+        } else if (got[q] == 0) {
+          const bool a = op_get(op_words(p, t, strip, 0, lane), p.tag, &m.a), b = op_get(op_words(p, t, strip, 1, lane), p.tag, &m.b);
+          if (__ballot(!a || !b) == 0) {
+            got[q] = 1;
+            maps[n][lane] = m;
+          }
+        }
+        if (lane == 0) ends[n] = got[q];
+      }
+      __syncthreads();
+      const int seen = lane < OP_NEAR && lane < tile ? ends[lane] : 0;
+      const unsigned long long states = __ballot(seen == 2), nothing = __ballot(seen == 0);
+      __syncthreads();
+      nearest = __builtin_ctzll(states | 1ull << 63);
+      if (nearest < __builtin_ctzll(nothing)) break;           /* (lane 63 has seen nothing) */
+      if (++polls >= ACC_SPIN_LIMIT) {
+        if (tid == 0) acc_report(p.status, ACC_STATUS_SCAN_LOOKBACK);
+        nearest = 0;
+        break;
+      }
+    }
+    in = maps[nearest][lane].b;
+    for (int n = nearest - 1; n >= 0; --n) {
+      const op_map m = maps[n][lane];
+#pragma unroll
+      for (int k = 0; k < OP_V; ++k) in.v[k] = __builtin_fmaf(m.a.v[k], in.v[k], m.b.v[k]);
+    }
+    if (wave == 0 && !known) {
+      op_pair h;
+#pragma unroll
+      for (int k = 0; k < OP_V; ++k) h.v[k] = __builtin_fmaf(all.a.v[k], in.v[k], all.b.v[k]);
+      op_put(op_words(p, tile, strip, 2, lane), p.tag, h);
+    }
+  }
+
+  /* the results */
+  op_pair h;
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) h.v[k] = mine_ends ? mine.b.v[k] : __builtin_fmaf(mine.a.v[k], in.v[k], mine.b.v[k]);
+#pragma unroll
+  for (int r = 0; r < OP_R; ++r) {
+    if (!(here >> r & 1)) continue;
+    if (resets >> r & 1) {
+      h = entered;
+      if (r != latest) h = entering(r);
+    }
+    const long long to = first + (OP_BACK ? OP_R - 1 - r : r);
+    const op_pair z = op_floats(zw[r]), x = op_floats(xw[r]);
+#if OP_BACK
+    op_pair b = op_floats(hw[r]), dz, dx;
+    if (leaves >> r & 1) b = op_state(p.state, p.state_stride, op_slot(p, sequence_of(r)), channel, valid);
+#if OP_GATE
+    const op_pair v = op_floats(vw[r]);
+#endif
+#pragma unroll
+    for (int k = 0; k < OP_V; ++k) {
+      const op_gate g = op_gate_of(z.v[k]);
+      const float d = x.v[k] + h.v[k];
+      h.v[k] = g.keep * d;
+#if OP_GATE
+      dx.v[k] = g.take * d;
+      dz.v[k] = (b.v[k] - v.v[k]) * (g.keep * dx.v[k]);
+#else
+      dx.v[k] = d;
+      dz.v[k] = b.v[k] * d;
+#endif
+    }
+    op_write((op_elt *)p.dgates + to * p.dgates_stride, channel, valid, dz);
+    op_write((op_elt *)p.dvalues + to * p.dvalues_stride, channel, valid, dx);
+#else
+#pragma unroll
+    for (int k = 0; k < OP_V; ++k) {
+      const op_gate g = op_gate_of(z.v[k]);
+      h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
+    }
+    op_write((op_elt *)p.out + to * p.out_stride, channel, valid, h);
+#endif
+    if (leaves >> r & 1) op_keep(p.leave, p.leave_stride, op_slot(p, sequence_of(r)), channel, valid, h);
+  }
+  op_empty_sequences(p, rows, tile * OP_WAVES + wave, lane, channel, valid);
+}
+
+/* in a graph: no tile has left anything yet.  (The launches of a graph carry one tag.) */
+extern "C" __global__ void __launch_bounds__(256) recur_clear(const acc_recur_args p)
+{
+  const long long words = (long long)p.tiles * p.strips * 3 * 64 * OP_V, i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i < words) p.words[i] = 0;
+  if (i == 0) *p.ticket = 0u;
+}
+#endif

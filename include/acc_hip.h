@@ -676,7 +676,14 @@ enum {
   ACC_OP_ROUTE   = 1,
   ACC_OP_COMBINE = 2,
   ACC_OP_MICRO   = 3,
-  ACC_OP_KIND_COUNT = 4
+  ACC_OP_RECUR   = 5,        /* (4 is no kind)                                    */
+  ACC_OP_KIND_COUNT = 6
+};
+
+/* what a recurrence's gates are */
+enum {
+  ACC_GATE_GIVEN   = 0,      /* h[t] = gates h[t-1] + values                      */
+  ACC_GATE_SIGMOID = 1       /* h[t] = a h[t-1] + (1 - a) values, a = 1 / (1 + e^-gates) */
 };
 
 typedef struct acc_op_desc {
@@ -684,6 +691,7 @@ typedef struct acc_op_desc {
   const char *elt_type;      /* "float", "half" or "bfloat16"                     */
   int32_t     choose;        /* ACC_OP_ROUTE: experts a token, 1 to 64            */
   int32_t     normalise;     /* ACC_OP_ROUTE: softmax over the chosen (else over all experts) */
+  int32_t     gate;          /* ACC_OP_RECUR: ACC_GATE_*                          */
 } acc_op_desc;
 
 /* An instance; its kernels are compiled through the cache when a call first needs them (as the variants of a skeleton
@@ -740,6 +748,29 @@ int acc_exec_micro_values(acc_op op, const acc_strided *codes, const acc_strided
 int acc_exec_micro_rows(acc_op op, const acc_strided *xcodes, const acc_strided *xscales, const acc_strided *wcodes,
                         const acc_strided *wscales, const acc_strided *offsets, const acc_strided *index, int32_t per,
                         const acc_strided *out, acc_stream stream);
+
+/* A gated linear recurrence along the rows of every sequence, channel by channel: h[t] = a[t] h[t-1] + b[t] (ACC_GATE_*), the
+ * state Float32 throughout.  gates, values, out [rows, width], innermost dimension contiguous; the rows of sequence s are
+ * offsets[s] <= t < offsets[s+1], offsets [sequences + 1] ascending (with others some rows are in no sequence or states are left
+ * by the wrong one; no other memory is touched).  Rows of no sequence are left as they were.  state, last [states, width] Float32
+ * or NULL: what sequences begin with (NULL: zeros) and where the states behind their last rows go; both may be the same array.
+ * Sequence s has row index[s] of them, or row s without index; one that the states do not have begins with zeros and is not
+ * kept.  A sequence without rows leaves the state that it begins with.  No two sequences may leave the same row.
+ * (For long sequences tiles of rows wait for what earlier ones leave, as those of acc_exec_scan do: ACC_ERR_STUCK.) */
+int acc_exec_recur(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *offsets, const acc_strided *index,
+                   const acc_strided *state, const acc_strided *last, const acc_strided *out, acc_stream stream);
+/* Its gradient.  h: the result as acc_exec_recur gave it; dout its gradient; state what the sequences began with, row s for
+ * sequence s (not replaced since; NULL: zeros); dlast [sequences, width] the gradient of the states behind the last rows (NULL:
+ * zeros).  dgates, dvalues [rows, width] (rows of no sequence are left as they were), dstate [sequences, width] Float32 or NULL.
+ * ACC_GATE_GIVEN does not look at values, which may be NULL.                                                  */
+int acc_exec_recur_gradient(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *offsets, const acc_strided *h,
+                            const acc_strided *dout, const acc_strided *state, const acc_strided *dlast, const acc_strided *dgates,
+                            const acc_strided *dvalues, const acc_strided *dstate, acc_stream stream);
+/* One row of many sequences, as a decoding step has them: out[m] = last[i] = a[m] state[i] + b[m], i = index[m], or m without
+ * index.  A row whose index names no state is left out: nothing is written.  state and last may be the same array; no two rows
+ * may name the same state.                                                                                    */
+int acc_exec_recur_step(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *index, const acc_strided *state,
+                        const acc_strided *last, const acc_strided *out, acc_stream stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
