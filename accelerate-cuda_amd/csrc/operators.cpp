@@ -169,15 +169,37 @@ std::string micro_source(const OpSpec &sp, bool aligned)
 // gradient has twice as many arrays
 struct RecurVariant {
   bool back = false, step = false;
-  int rows() const { return back ? 16 : 32; }
-  uint32_t key() const { return (back ? 1u : 0u) | (step ? 2u : 0u); }
+  bool thin = false;            // rows of up to 64 channels of 16 bits: one a lane (and a row of one has no word of two)
+  int rows = 32;                // of a wave: 8, 16 or (forward) 32
+  int channels(int type) const { return thin ? 64 : 64 * (4 / type_bytes(type)); }
+  uint32_t key() const { return (back ? 1u : 0u) | (step ? 2u : 0u) | (thin ? 4u : 0u) | (uint32_t)rows << 4; }
 };
 constexpr int kRecurWaves = 8;
+
+// Rows of a wave.  512 tiles are on the device at once, two a compute unit; a tile takes about as long as its rows and sixteen more
+// (what it waits for), eight where it has a compute unit for itself, and a state takes a fifth of a row to go on to the next tile of a
+// long sequence.  us, with 8, 16 and 32 rows a wave: forward, bfloat16, 32768 x 2048: 156, 103, 89; 4096 x 2048: 25, 18, 19; 2048 x 2048:
+// 15, 12, 17; 512 x 1024: 8, 10, 14; half, one sequence, 65536 x 64: 56, 33, 25; 16384 x 128: 23, 17, 18; Float32 9001 x 1001: 38, 36, 39; gradient,
+// bfloat16, 32768 x 2048: 205, 170; 1024 x 1024: 12, 14.
+int recur_rows(bool back, int64_t rows, int64_t strips)
+{
+  int best = 0;
+  int64_t least = 0;
+  for (int r : {32, 16, 8}) {
+    if (back && r == 32) continue;
+    const int64_t tiles = ceil_div(rows, (int64_t)kRecurWaves * r), groups = tiles * strips, cost = 5 * (groups <= 256 ? r + 8 : ceil_div(groups, 512) * (r + 16)) + tiles;
+    if (best == 0 || cost < least) {
+      best = r;
+      least = cost;
+    }
+  }
+  return best;
+}
 std::string recur_source(const OpSpec &sp, const RecurVariant &v)
 {
   char text[256];
-  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_GATE %d\n#define OP_BACK %d\n#define OP_STEP %d\n#define OP_R %d\n#include \"acc_hip_device.h\"\n#include \"op_recur.h\"\n",
-                sp.type, sp.gate, v.back ? 1 : 0, v.step ? 1 : 0, v.rows());
+  std::snprintf(text, sizeof(text), "#define OP_ELT %d\n#define OP_GATE %d\n#define OP_BACK %d\n#define OP_STEP %d\n#define OP_THIN %d\n#define OP_R %d\n#include \"acc_hip_device.h\"\n#include \"op_recur.h\"\n",
+                sp.type, sp.gate, v.back ? 1 : 0, v.step ? 1 : 0, v.thin ? 1 : 0, v.rows);
   return text;
 }
 
@@ -228,12 +250,15 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
   } else if (sp.kind == ACC_OP_RECUR) {
-    for (int form = 0; form < 3; ++form) {
-      RecurVariant v;
-      v.back = form == 1;
-      v.step = form == 2;
-      out.push_back(recur_source(sp, v));
-    }
+    for (int form = 0; form < 6; ++form)
+      for (int rows : {8, 16, 32}) {
+        RecurVariant v;
+        v.step = form >= 4;
+        v.thin = form & 1;
+        v.back = form & 2 && !v.step;
+        if (!v.step) v.rows = rows;
+        if (!(v.thin && sp.type == 0) && !(v.back && rows == 32)) out.push_back(recur_source(sp, v));
+      }
   } else {
     for (bool aligned : {true, false}) out.push_back(micro_source(sp, aligned));
     for (int t = 0; t < kProductTileCount; ++t)
@@ -538,6 +563,8 @@ std::string recur_source_of(const OpSpec &sp, uint32_t key)
   RecurVariant v;
   v.back = key & 1u;
   v.step = key & 2u;
+  v.thin = key & 4u;
+  v.rows = (int)(key >> 4);
   return recur_source(sp, v);
 }
 
@@ -1291,10 +1318,15 @@ static int check_replaced(const char *who, const acc_strided *state, const acc_s
 }
 
 // the tiles of all rows, forward or back: a.gates ... are there, the rest is filled in
-static int launch_recur(acc_op op, const char *who, const RecurVariant &v, acc_recur_args &a, acc_stream stream)
+static int launch_recur(acc_op op, const char *who, bool back, acc_recur_args &a, acc_stream stream)
 {
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t channels = 64 * (4 / type_bytes(op->spec.type)), tiles = std::max<int64_t>(1, ceil_div(a.rows, (int64_t)kRecurWaves * v.rows())), strips = ceil_div(a.width, channels);
+  RecurVariant v;
+  v.back = back;
+  v.thin = op->spec.type != 0 && a.width <= 64;
+  const int64_t channels = v.channels(op->spec.type);
+  v.rows = recur_rows(back, a.rows, ceil_div(a.width, channels));
+  const int64_t tiles = std::max<int64_t>(1, ceil_div(a.rows, (int64_t)kRecurWaves * v.rows)), strips = ceil_div(a.width, channels);
   if (tiles * strips > kThreads / (64 * kRecurWaves)) return fail(ACC_ERR_INVALID, "%s: %lld rows of %d channels are too many", who, (long long)a.rows, a.width);
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kRecurNames, 2, recur_source_of, &var));
@@ -1365,7 +1397,7 @@ try {
   a.width = (int32_t)width;
   a.sequences = (int32_t)sequences;
   a.states = (int32_t)(state ? state->shape[0] : last ? last->shape[0] : 0);
-  return launch_recur(op, who, RecurVariant(), a, stream);
+  return launch_recur(op, who, false, a, stream);
 } ACC_OP_CATCH("acc_exec_recur")
 
 int acc_exec_recur_gradient(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *offsets, const acc_strided *h,
@@ -1427,9 +1459,7 @@ try {
   a.rows = rows;
   a.width = (int32_t)width;
   a.sequences = a.states = (int32_t)sequences;
-  RecurVariant v;
-  v.back = true;
-  return launch_recur(op, who, v, a, stream);
+  return launch_recur(op, who, true, a, stream);
 } ACC_OP_CATCH("acc_exec_recur_gradient")
 
 int acc_exec_recur_step(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *index, const acc_strided *state,
@@ -1457,6 +1487,7 @@ try {
   if (is_empty(*out)) return ACC_OK;
   RecurVariant v;
   v.step = true;
+  v.thin = op->spec.type != 0 && width == 1;
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kRecurStepNames, 1, recur_source_of, &var));
   a.gates_stride = gates->stride[0];
@@ -1465,7 +1496,7 @@ try {
   a.enter_stride = state->stride[0];
   a.leave_stride = last->stride[0];
   a.width = (int32_t)width;
-  a.strips = (int32_t)ceil_div(width, 256 * (4 / bytes));
+  a.strips = (int32_t)ceil_div(width, 4 * v.channels(op->spec.type));
   const int64_t most = kThreads / 256 / a.strips;
   for (int64_t first = 0; first < rows; first += most) {
     // (without index the states' rows go along)

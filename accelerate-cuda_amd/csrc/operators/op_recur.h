@@ -19,46 +19,57 @@
  */
 #include "op_common.h"
 
-#define OP_V (4 / (int)sizeof(op_elt))             /* channels of a lane: a word of a row */
+/* OP_V: channels of a lane, a word of a row; OP_THIN: one of 16 bits, for rows of up to 64 */
+#if OP_THIN
+#define OP_V 1
+#else
+#define OP_V (4 / (int)sizeof(op_elt))
+#endif
 #define OP_WAVES 8
 #define OP_NEAR 32                                 /* tiles in front that are looked at, at once */
 
-/* 32 bits of memory that start wherever an element may */
+/* a word of memory, which starts wherever an element may */
+#if OP_THIN
+typedef unsigned short op_word;
+#else
 typedef unsigned int __attribute__((aligned(sizeof(op_elt)))) op_word;
+#endif
 
 struct op_pair { float v[OP_V]; };
 ACC_DEV op_pair op_floats(const unsigned int w)
 {
   op_elt e[OP_V];
-  __builtin_memcpy(e, &w, 4);
+  __builtin_memcpy(e, &w, sizeof(e));
   op_pair f;
 #pragma unroll
   for (int k = 0; k < OP_V; ++k) f.v[k] = (float)e[k];
   return f;
 }
 
-/* a lane's word of a row, which is the same for all lanes, from element `at` on; `valid` of its channels there are (1 to OP_V) */
-ACC_DEV unsigned int op_read(const op_elt *row, const unsigned int at, const int valid)
+/* the same, made where it is wanted: what has been made of all rows' words, kept from one pass to the next, takes twice their registers */
+ACC_DEV op_pair op_again(unsigned int w)
 {
-  const op_elt *const p = (const op_elt *)((const char *)row + at * (unsigned int)sizeof(op_elt));
-  if (valid == OP_V) return __builtin_nontemporal_load((const op_word *)p);
-  unsigned short h = 0;
-  __builtin_memcpy(&h, p, sizeof(h));
-  return h;
+  acc_pin(w);
+  return op_floats(w);
 }
-ACC_DEV void op_write(op_elt *row, const unsigned int at, const int valid, const op_pair &f)
+
+/* A lane's word of a row (the same for all lanes) from element `at` on.  Where a row ends amid a lane's word, the lane reads one
+ * element earlier and shifts (`down` bits): no read goes past the row. */
+ACC_DEV unsigned int op_read(const op_elt *row, const unsigned int at)
+{
+  return __builtin_nontemporal_load((const op_word *)((const char *)row + at * (unsigned int)sizeof(op_elt)));
+}
+/* `valid` of a lane's channels there are (0 to OP_V); `whole`: in all lanes OP_V */
+ACC_DEV void op_write(op_elt *row, const unsigned int at, const bool whole, const int valid, const op_pair &f)
 {
   op_elt *const p = (op_elt *)((char *)row + at * (unsigned int)sizeof(op_elt));
   op_elt e[OP_V];
 #pragma unroll
   for (int k = 0; k < OP_V; ++k) e[k] = (op_elt)f.v[k];
-  if (valid == OP_V) {
-    unsigned int w;
-    __builtin_memcpy(&w, e, 4);
-    __builtin_nontemporal_store(w, (op_word *)p);
-  } else if (valid == 1) {
-    *p = e[0];
-  }
+  unsigned int w = 0;
+  __builtin_memcpy(&w, e, sizeof(e));
+  if (whole || valid == OP_V) __builtin_nontemporal_store((op_word)w, (op_word *)p);
+  else if (valid == 1) *p = e[0];
 }
 
 /* what a gate keeps and what it takes in, for a gate of OP_GATE 1: 1 / (1 + e) and e / (1 + e) with e = e^-z, of which neither
@@ -82,13 +93,31 @@ ACC_DEV op_gate op_gate_of(const float z)
   return g;
 }
 
-/* how many of the n offsets, which ascend, are at most `row`; they count as the nearest row there is */
-ACC_DEV int op_upto(const int *offsets, const int n, const int rows, const int row)
+/* How many of the n offsets, which ascend, are at most a lane's `row`; they count as the nearest row there is.  Lanes' rows ascend
+ * by one.  The wave looks at 64 offsets at a time until 64 are left that the first lane's row lies among, and the lanes search
+ * those; where the last lane's lies behind them, offsets lie close, and every lane searches memory. */
+ACC_DEV int op_upto(const int *offsets, const int n, const int rows, const int row, const int lane)
 {
-  int lo = 0, hi = n;
+  const auto value = [&](const int i) { return i < n ? acc_min(acc_max(offsets[i], 0), rows) : 0x7fffffff; };
+  const int least = acc_readlane(row, 0), most = acc_readlane(row, 63);
+  int lo = 0, hi = n;                              /* the count of the first lane's row lies in between */
+  while (hi - lo > 63) {
+    const int step = (hi - lo) / 64;               /* (one at least) */
+    const int c = __popcll(__ballot(value(lo + lane * step) <= least));
+    if (c < 64) hi = acc_min(hi, lo + c * step);
+    lo += acc_max(c - 1, 0) * step;
+  }
+  const int mine = value(lo + lane);
+  int found = 0;
+  if (acc_readlane(mine, 63) > most) {
+#pragma unroll
+    for (int step = 32; step > 0; step /= 2) found += __builtin_amdgcn_ds_bpermute((found + step - 1) * 4, mine) <= row ? step : 0;
+    return lo + found;
+  }
+  hi = n;
   while (lo < hi) {
     const int mid = lo + (hi - lo) / 2;
-    if (acc_min(acc_max(offsets[mid], 0), rows) <= row) lo = mid + 1;
+    if (value(mid) <= row) lo = mid + 1;
     else hi = mid;
   }
   return lo;
@@ -142,18 +171,19 @@ extern "C" __global__ void __launch_bounds__(256) recur_step(const acc_recur_arg
   const long long row = blockIdx.x / p.strips;
   if (valid <= 0) return;
   /* (asked for before it is known whether the row counts) */
-  const op_pair z = op_floats(op_read((const op_elt *)p.gates + row * p.gates_stride, channel, valid));
-  const op_pair x = op_floats(op_read((const op_elt *)p.values + row * p.values_stride, channel, valid));
-  const long long at = op_slot(p, (int)row);
-  if (at < 0) return;
-  op_pair h = op_state(p.enter, p.enter_stride, at, channel, valid);
+  const int at = acc_min(channel, p.width - OP_V), down = (channel - at) * 8 * (int)sizeof(op_elt);
+  const op_pair z = op_floats(op_read((const op_elt *)p.gates + row * p.gates_stride, at) >> down);
+  const op_pair x = op_floats(op_read((const op_elt *)p.values + row * p.values_stride, at) >> down);
+  const long long slot = op_slot(p, (int)row);
+  if (slot < 0) return;
+  op_pair h = op_state(p.enter, p.enter_stride, slot, channel, valid);
 #pragma unroll
   for (int k = 0; k < OP_V; ++k) {
     const op_gate g = op_gate_of(z.v[k]);
     h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
   }
-  op_keep(p.leave, p.leave_stride, at, channel, valid, h);
-  op_write((op_elt *)p.out + row * p.out_stride, channel, valid, h);
+  op_keep(p.leave, p.leave_stride, slot, channel, valid, h);
+  op_write((op_elt *)p.out + row * p.out_stride, channel, false, valid, h);
 }
 #else
 
@@ -182,7 +212,7 @@ ACC_DEV void op_empty_sequences(const acc_recur_args &p, const int rows, const i
   }
 }
 
-extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recur_args p)
+extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgpu_waves_per_eu(4))) recur(const acc_recur_args p)
 {
   if (p.guard && *p.guard == 0u) return;
   __shared__ op_map maps[OP_NEAR][64];             /* of the waves' rows; then of the tiles before */
@@ -206,28 +236,33 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recu
   }
 
   /* The wave's rows, in the order of the recurrence: physical row first + r, or (back) first + OP_R - 1 - r.  Rows that there are
-   * not are read as the nearest one, lanes without a channel as the first. */
+   * not are read as the nearest one, lanes without a channel as the last word of the row. */
   const long long from = ((long long)tile * OP_WAVES + wave) * OP_R, first = OP_BACK ? rows - from - OP_R : from;
-  const int at = valid > 0 ? channel : 0, some = valid > 0 ? valid : acc_min(p.width, OP_V);
-  const bool whole = __ballot(some != OP_V) == 0;
-  const auto row_of = [&](const int r) { return acc_max<long long>(acc_min<long long>(first + (OP_BACK ? OP_R - 1 - r : r), rows - 1), 0); };
+  const int at = acc_min(channel, p.width - OP_V), down = valid > 0 ? (channel - at) * 8 * (int)sizeof(op_elt) : 0;
+  const bool whole = __ballot(valid != OP_V) == 0;
   const auto read_rows = [&](const void *base, const long long stride, const int back, unsigned int (&to)[OP_R]) {
-    if (whole && first >= back && first + OP_R <= rows) {
+    if (first >= back && first + OP_R <= rows) {
       const op_elt *x = (const op_elt *)base + (first + (OP_BACK ? OP_R - 1 : 0) - back) * stride;
 #pragma unroll
-      for (int r = 0; r < OP_R; ++r, x += OP_BACK ? -stride : stride) to[r] = op_read(x, at, OP_V);
+      for (int r = 0; r < OP_R; ++r, x += OP_BACK ? -stride : stride) to[r] = op_read(x, at);
     } else {
 #pragma unroll
-      for (int r = 0; r < OP_R; ++r) to[r] = op_read((const op_elt *)base + acc_max<long long>(row_of(r) - back, 0) * stride, at, some);
+      for (int r = 0; r < OP_R; ++r)
+        to[r] = op_read((const op_elt *)base + acc_max<long long>(acc_min<long long>(first + (OP_BACK ? OP_R - 1 - r : r), rows - 1) - back, 0) * stride, at);
     }
+  };
+  const auto shift_rows = [&](unsigned int (&w)[OP_R]) {
+    if (!whole)
+#pragma unroll
+      for (int r = 0; r < OP_R; ++r) w[r] >>= down;
   };
   unsigned int zw[OP_R], xw[OP_R];
   read_rows(p.gates, p.gates_stride, 0, zw);
   read_rows(OP_BACK ? p.dout : p.values, OP_BACK ? p.dout_stride : p.values_stride, 0, xw);
 
-  /* sequences: lane j counts those that begin up to row first - 1 + j */
-  const long long row = first - 1 + lane;
-  const int upto = op_upto(p.offsets, p.sequences + 1, rows, (int)acc_max<long long>(row, -1)), before = acc_wave_shift_up1(upto);
+  /* sequences: lane j counts those that begin up to row first - 1 + j (as 32 bits: rows end well below 2^31) */
+  const int row = (int)(first - 1) + lane;
+  const int upto = op_upto(p.offsets, p.sequences + 1, rows, row, lane), before = acc_wave_shift_up1(upto);
   const bool inside = row >= 0 && row < rows && upto >= 1 && upto <= p.sequences, change = lane > 0 && upto > before;
   const unsigned long long mask = (1ull << OP_R) - 1;
   const unsigned long long within = __ballot(inside) >> 1 & mask, begins = __ballot(change && inside) >> 1 & mask, stops = __ballot(change) >> 2 & within;
@@ -249,6 +284,8 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recu
   if (latest >= 0) entered = entering(latest);
   own.b = entered;
   const unsigned long long live = latest >= 0 ? here >> latest << latest : here;
+  shift_rows(zw);
+  shift_rows(xw);
 #pragma unroll
   for (int r = 0; r < OP_R; ++r) {
     if (!(live >> r & 1)) continue;
@@ -259,12 +296,6 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recu
       own.a.v[k] *= g.keep;
       own.b.v[k] = OP_BACK ? g.keep * (x.v[k] + own.b.v[k]) : __builtin_fmaf(g.keep, own.b.v[k], g.take * x.v[k]);
     }
-  }
-  /* (the words as they are stay, not what has been made of them: that takes twice the registers) */
-#pragma unroll
-  for (int r = 0; r < OP_R; ++r) {
-    acc_pin(zw[r]);
-    acc_pin(xw[r]);
   }
 #if OP_BACK
   /* (on their way while the tiles before are looked at) */
@@ -327,7 +358,11 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recu
 #pragma unroll
       for (int q = 0; q < OP_NEAR / OP_WAVES; ++q) {
         const int n = q * OP_WAVES + wave, t = tile - 1 - n;
-        if (t < 0 || got[q] == 2) continue;
+        if (t < 0 || (q > 0 && polls == 0)) {      /* (the nearest eight will often do) */
+          if (lane == 0) ends[n] = 0;
+          continue;
+        }
+        if (got[q] == 2) continue;
         op_map m;
         if (__ballot(!op_get(op_words(p, t, strip, 2, lane), p.tag, &m.b)) == 0) {
           got[q] = 2;
@@ -354,10 +389,14 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recu
       }
     }
     in = maps[nearest][lane].b;
-    for (int n = nearest - 1; n >= 0; --n) {
-      const op_map m = maps[n][lane];
+    for (; nearest > 0; nearest -= 8) {            /* (eight at a time, those that there are not change nothing) */
+      op_map m[8];
 #pragma unroll
-      for (int k = 0; k < OP_V; ++k) in.v[k] = __builtin_fmaf(m.a.v[k], in.v[k], m.b.v[k]);
+      for (int n = 0; n < 8; ++n) m[n] = maps[acc_max(nearest - 1 - n, 0)][lane];
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int k = 0; k < OP_V; ++k) in.v[k] = n < nearest ? __builtin_fmaf(m[n].a.v[k], in.v[k], m[n].b.v[k]) : in.v[k];
     }
     if (wave == 0 && !known) {
       op_pair h;
@@ -367,49 +406,75 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) recur(const acc_recu
     }
   }
 
-  /* the results */
+  /* the results, sequence after sequence: what comes in, or what one that begins here enters with */
   op_pair h;
 #pragma unroll
   for (int k = 0; k < OP_V; ++k) h.v[k] = mine_ends ? mine.b.v[k] : __builtin_fmaf(mine.a.v[k], in.v[k], mine.b.v[k]);
-#pragma unroll
-  for (int r = 0; r < OP_R; ++r) {
-    if (!(here >> r & 1)) continue;
-    if (resets >> r & 1) {
-      h = entered;
-      if (r != latest) h = entering(r);
-    }
-    const long long to = first + (OP_BACK ? OP_R - 1 - r : r);
-    const op_pair z = op_floats(zw[r]), x = op_floats(xw[r]);
 #if OP_BACK
-    op_pair b = op_floats(hw[r]), dz, dx;
-    if (leaves >> r & 1) b = op_state(p.state, p.state_stride, op_slot(p, sequence_of(r)), channel, valid);
-#if OP_GATE
-    const op_pair v = op_floats(vw[r]);
+  shift_rows(hw);
+  if (OP_GATE) shift_rows(vw);
+#endif
+  for (int begin = 0; begin < OP_R;) {
+    const unsigned long long more = resets & ~0ull << begin << 1;
+    const int next = more ? __builtin_ctzll(more) : OP_R;
+    const unsigned long long run = here & ~0ull << begin & ((1ull << next) - 1);
+    if (resets >> begin & 1) {
+      h = entered;
+      if (begin != latest) h = entering(begin);
+    }
+    const int final = run & leaves ? __builtin_ctzll(run & leaves) : -1;
+    const long long slot = final >= 0 ? op_slot(p, sequence_of(final)) : -1;
+#if OP_BACK
+    const op_pair started = op_state(p.state, p.state_stride, slot, channel, valid);
+    op_elt *dgates = (op_elt *)p.dgates + (first + OP_R - 1) * p.dgates_stride, *dvalues = (op_elt *)p.dvalues + (first + OP_R - 1) * p.dvalues_stride;
+    asm volatile("" : "+s"(dgates), "+s"(dvalues));      /* (or the rows' addresses are kept in registers from sequence to sequence) */
+#else
+    op_elt *out = (op_elt *)p.out + first * p.out_stride;
+    asm volatile("" : "+s"(out));                        /* (or the rows' addresses are kept in registers from sequence to sequence) */
 #endif
 #pragma unroll
-    for (int k = 0; k < OP_V; ++k) {
-      const op_gate g = op_gate_of(z.v[k]);
-      const float d = x.v[k] + h.v[k];
-      h.v[k] = g.keep * d;
+    for (int r = 0; r < OP_R; ++r) {
+      if (run >> r & 1) {
+        const op_pair z = op_again(zw[r]), x = op_again(xw[r]);
+#if OP_BACK
+        op_pair b = op_again(hw[r]), dz, dx;
+        if (r == final) b = started;
 #if OP_GATE
-      dx.v[k] = g.take * d;
-      dz.v[k] = (b.v[k] - v.v[k]) * (g.keep * dx.v[k]);
-#else
-      dx.v[k] = d;
-      dz.v[k] = b.v[k] * d;
+        const op_pair v = op_again(vw[r]);
 #endif
-    }
-    op_write((op_elt *)p.dgates + to * p.dgates_stride, channel, valid, dz);
-    op_write((op_elt *)p.dvalues + to * p.dvalues_stride, channel, valid, dx);
+#pragma unroll
+        for (int k = 0; k < OP_V; ++k) {
+          const op_gate g = op_gate_of(z.v[k]);
+          const float d = x.v[k] + h.v[k];
+          h.v[k] = g.keep * d;
+#if OP_GATE
+          dx.v[k] = g.take * d;
+          dz.v[k] = (b.v[k] - v.v[k]) * (g.keep * dx.v[k]);
+#else
+          dx.v[k] = d;
+          dz.v[k] = b.v[k] * d;
+#endif
+        }
+        op_write(dgates, channel, whole, valid, dz);
+        op_write(dvalues, channel, whole, valid, dx);
 #else
 #pragma unroll
-    for (int k = 0; k < OP_V; ++k) {
-      const op_gate g = op_gate_of(z.v[k]);
-      h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
-    }
-    op_write((op_elt *)p.out + to * p.out_stride, channel, valid, h);
+        for (int k = 0; k < OP_V; ++k) {
+          const op_gate g = op_gate_of(z.v[k]);
+          h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
+        }
+        op_write(out, channel, whole, valid, h);
 #endif
-    if (leaves >> r & 1) op_keep(p.leave, p.leave_stride, op_slot(p, sequence_of(r)), channel, valid, h);
+      }
+#if OP_BACK
+      dgates -= p.dgates_stride;
+      dvalues -= p.dvalues_stride;
+#else
+      out += p.out_stride;
+#endif
+    }
+    if (final >= 0) op_keep(p.leave, p.leave_stride, slot, channel, valid, h);
+    begin = next;
   }
   op_empty_sequences(p, rows, tile * OP_WAVES + wave, lane, channel, valid);
 }
