@@ -29,7 +29,7 @@ COMBINE_GENERIC, COMBINE_ADD, COMBINE_MIN, COMBINE_MAX, COMBINE_AND, COMBINE_OR,
 BOUNDARY = {"clamp": 0, "mirror": 1, "wrap": 2, "constant": 3}
 FLAG_FOLD_RIGHT, FLAG_FAST_MATH, FLAG_GUARDED, FLAG_TILED = 1, 2, 4, 8
 OP_PRODUCT, OP_ROUTE, OP_COMBINE, OP_MICRO = range(4)
-OP_RECUR = 5
+OP_RECUR, OP_GROUPED = 5, 6
 GATES = {"given": 0, "sigmoid": 1}
 STRIDED_RANK = 4
 
@@ -82,7 +82,7 @@ class acc_skel_desc(C.Structure):
 
 
 class acc_op_desc(C.Structure):
-    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32), ("gate", C.c_int32)]
+    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32), ("gate", C.c_int32), ("group", C.c_int32)]
 
 
 # the bytes of an acc_strided, by rank
@@ -129,7 +129,8 @@ acc_memtable_malloc acc_memtable_acquire acc_memtable_release acc_memtable_free 
 acc_memtable_reclaim acc_memtable_get_stats acc_skel_create_async acc_skel_wait acc_skel_poll acc_skel_prefetch acc_compile_threads acc_compile_drain
 acc_tuning_set acc_tuning_text acc_context_set_tuning acc_op_create acc_op_destroy acc_op_compile_only acc_exec_product_rows
 acc_exec_product_outer acc_exec_route acc_exec_route_gradient acc_exec_combine acc_exec_combine_gradient acc_exec_micro_quantise
-acc_exec_micro_values acc_exec_micro_rows acc_exec_recur acc_exec_recur_gradient acc_exec_recur_step""".split()
+acc_exec_micro_values acc_exec_micro_rows acc_exec_recur acc_exec_recur_gradient acc_exec_recur_step
+acc_exec_grouped_quantise acc_exec_grouped_values acc_exec_grouped_rows""".split()
 
 
 def build(force=False):
@@ -653,7 +654,8 @@ class _Drivers(object):
               "acc_exec_combine": (_P, _P, _P, _P, _P, _P), "acc_exec_combine_gradient": (_P, _P, _P, _P, _P, _P, _P, _P),
               "acc_exec_micro_quantise": (_P, _P, _P, _P, _P), "acc_exec_micro_values": (_P, _P, _P, _P, _P),
               "acc_exec_micro_rows": (_P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P),
-              "acc_exec_recur": (_P,) * 9, "acc_exec_recur_gradient": (_P,) * 12, "acc_exec_recur_step": (_P,) * 8}
+              "acc_exec_recur": (_P,) * 9, "acc_exec_recur_gradient": (_P,) * 12, "acc_exec_recur_step": (_P,) * 8,
+              "acc_exec_grouped_quantise": (_P,) * 6, "acc_exec_grouped_values": (_P,) * 6, "acc_exec_grouped_rows": (_P,) * 7 + (C.c_int32, _P, _P)}
 
     def __getattr__(self, name):               # (at its first call; an attribute of its own from then on)
         f = C.CFUNCTYPE(C.c_int, *self._TYPES[name])((name, lib()))
@@ -811,11 +813,11 @@ def _layout(a, size=None):
     return _STRIDED[len(a.shape)](len(a.shape), 0, *a.shape, *a.strides, a.ptr)
 
 
-def op_desc(kind, elt, choose=0, normalise=True, gate="given"):
+def op_desc(kind, elt, choose=0, normalise=True, gate="given", group=0):
     if gate not in GATES:
         raise AccError(ERR_INVALID, "gates are %s, not %r" % (" or ".join(sorted(GATES)), gate))
     d = acc_op_desc()
-    d.kind, d.elt_type, d.choose, d.normalise, d.gate = kind, _b(elt), choose, int(normalise), GATES[gate]
+    d.kind, d.elt_type, d.choose, d.normalise, d.gate, d.group = kind, _b(elt), choose, int(normalise), GATES[gate], group
     return d
 
 
@@ -919,6 +921,32 @@ class Microscale(_Operator):
         """out[m, n] = sum_k x[r(m), k] w[e, n, k], both in 4 bits"""
         rc = _drivers.acc_exec_micro_rows(self.handle, _layout(xcodes, 1), _layout(xscales, 1), _layout(wcodes, 1), _layout(wscales, 1), _layout(offsets, 4), _layout(index, 4), per,
                                           _layout(out, self.size), stream)
+        if rc:
+            check(rc)
+
+
+class Grouped(_Operator):
+    """Matrices of 4-bit whole numbers, (q - z) s with a scale and a zero for every `group` neighbours of a row: codes two a byte
+    [experts, n, 16 ceil(k / 32)], scales [experts, ceil(k / group), n], zeros the same in bytes, or None: all 8."""
+    KIND = OP_GROUPED
+
+    def __init__(self, ctx, elt, group=128):
+        _Operator.__init__(self, ctx, elt, group=group)
+
+    def quantise(self, w, codes, scales, zeros=None, stream=None):
+        rc = _drivers.acc_exec_grouped_quantise(self.handle, _layout(w, self.size), _layout(codes, 1), _layout(scales, self.size), _layout(zeros, 1), stream)
+        if rc:
+            check(rc)
+
+    def values(self, codes, scales, out, zeros=None, stream=None):
+        rc = _drivers.acc_exec_grouped_values(self.handle, _layout(codes, 1), _layout(scales, self.size), _layout(zeros, 1), _layout(out, self.size), stream)
+        if rc:
+            check(rc)
+
+    def rows(self, x, codes, scales, offsets, out, zeros=None, index=None, per=0, stream=None):
+        """out[m, n] = sum_k x[r(m), k] w[e, n, k] for the rows m of expert e's segment"""
+        rc = _drivers.acc_exec_grouped_rows(self.handle, _layout(x, self.size), _layout(codes, 1), _layout(scales, self.size), _layout(zeros, 1), _layout(offsets, 4), _layout(index, 4), per,
+                                            _layout(out, self.size), stream)
         if rc:
             check(rc)
 

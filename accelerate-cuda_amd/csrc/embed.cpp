@@ -41,6 +41,7 @@ ACC_EMBED(op_combine, "operators/op_combine.h")
 ACC_EMBED(op_pack, "operators/op_pack.h")
 ACC_EMBED(op_micro, "operators/op_micro.h")
 ACC_EMBED(op_recur, "operators/op_recur.h")
+ACC_EMBED(op_grouped, "operators/op_grouped.h")
 
 namespace acc {
 
@@ -71,6 +72,7 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"op_pack.h", acc_embed_op_pack_begin, acc_embed_op_pack_end},
       {"op_micro.h", acc_embed_op_micro_begin, acc_embed_op_micro_end},
       {"op_recur.h", acc_embed_op_recur_begin, acc_embed_op_recur_end},
+      {"op_grouped.h", acc_embed_op_grouped_begin, acc_embed_op_grouped_end},
   };
   return headers;
 }

@@ -35,12 +35,13 @@ struct OpSpec {
   int choose = 0;
   bool normalise = true;
   int gate = 0;
+  int group = 0;
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-const char *const kKindName[] = {"product", "route", "combine", "micro", "", "recur"};
+const char *const kKindName[] = {"product", "route", "combine", "micro", "", "recur", "grouped"};
 int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 // ---- the variants of each kind ------------------------------------------------------
@@ -203,6 +204,24 @@ std::string recur_source(const OpSpec &sp, const RecurVariant &v)
   return text;
 }
 
+// grouped: rows and columns of a tile, in sixteens; what a lane asks for at once is less where a tile has many rows
+struct GroupedVariant {
+  int bm = 16, fn = 1;
+  bool elements = false;
+  int ahead(int type) const { return elements || bm > 32 || (bm > 16 && type == 0) ? 1 : bm > 16 || fn > 1 || type == 0 ? 2 : 4; }
+  uint32_t key() const { return kGroupedKeys | (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u); }
+  static constexpr uint32_t kGroupedKeys = 1u << 21;               // (beside the products' keys)
+};
+constexpr int kGroupedWaves = 8;
+std::string grouped_source(const OpSpec &sp, const GroupedVariant &v)
+{
+  char text[512];
+  std::snprintf(text, sizeof(text),
+                "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_GROUP %d\n#define OP_AHEAD %d\n#define OP_ELEMENTS %d\n#include \"acc_hip_device.h\"\n#include \"op_grouped.h\"\n",
+                sp.type, sp.type == 1 ? 1 : 2, v.bm, v.fn, v.elements ? 4 : std::min(4, sp.group / 32), v.ahead(sp.type), v.elements ? 1 : 0);
+  return text;
+}
+
 std::vector<std::string> op_options()
 {
   // (sums of products may be contracted: nothing here has to round as a scalar expression of the array language does; packed
@@ -249,6 +268,27 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         for (int64_t tokens : {int64_t(0), int64_t(1), int64_t(1) << 20}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
+  } else if (sp.kind == ACC_OP_GROUPED) {
+    for (int bm : {16, 32, 64})
+      for (int fn : {1, 2}) {
+        GroupedVariant v;
+        v.bm = bm;
+        v.fn = fn;
+        out.push_back(grouped_source(sp, v));
+      }
+    GroupedVariant v;
+    v.elements = true;
+    out.push_back(grouped_source(sp, v));
+    // (and the products of matrices that have been made again)
+    if (sp.type != 0) out.push_back(pack_source(sp));
+    for (int t = 0; t < kSkinny; ++t)
+      for (int form = 0; form < 3; ++form) {
+        ProductVariant p;
+        p.tile = t;
+        p.aligned = form == 0;
+        p.tiny = form == 2;
+        if (has_tile(sp, p, t)) out.push_back(product_source(sp, p));
+      }
   } else if (sp.kind == ACC_OP_RECUR) {
     for (int form = 0; form < 6; ++form)
       for (int rows : {8, 16, 32}) {
@@ -288,6 +328,10 @@ int make_spec(const acc_op_desc *d, OpSpec *sp)
   sp->kind = d->kind;
   sp->choose = d->choose;
   sp->normalise = d->normalise != 0;
+  if (d->kind == ACC_OP_GROUPED) {
+    if (d->group < 32 || (d->group & (d->group - 1)) != 0) return fail(ACC_ERR_INVALID, "acc_op_create: a group of %d neighbours (a power of two, 32 or more)", d->group);
+    sp->group = d->group;
+  }
   if (d->kind == ACC_OP_RECUR) {
     if (d->gate != ACC_GATE_GIVEN && d->gate != ACC_GATE_SIGMOID) return fail(ACC_ERR_INVALID, "acc_op_create: unknown gate %d", d->gate);
     sp->gate = d->gate;
@@ -514,6 +558,16 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
   return experts * piece >= 2 * rows ? 0 : (int32_t)piece;
 }
 
+// grouped: the tile for `mean` rows a segment, and from how many on the matrices are made again for tiles that use them often
+constexpr int64_t kGroupedMost = 96;
+GroupedVariant grouped_variant(int64_t rows, int64_t experts, int64_t n, int64_t mean)
+{
+  GroupedVariant v;
+  v.bm = mean > 32 ? 64 : mean > 16 ? 32 : 16;
+  v.fn = std::min(rows, experts) * ceil_div(n, 32) >= 512 ? 2 : 1;
+  return v;
+}
+
 }  // namespace
 
 struct acc_op_s {
@@ -568,6 +622,18 @@ std::string recur_source_of(const OpSpec &sp, uint32_t key)
   return recur_source(sp, v);
 }
 
+std::string grouped_source_of(const OpSpec &sp, uint32_t key)
+{
+  if (!(key & GroupedVariant::kGroupedKeys)) return product_source_of(sp, key);
+  GroupedVariant v;
+  v.bm = (int)(key & 15u) * 16;
+  v.fn = (int)(key >> 4 & 15u);
+  v.elements = key & 256u;
+  return grouped_source(sp, v);
+}
+
+const char *const kGroupedNames[] = {"grouped"};
+const char *const kGroupedElementNames[] = {"grouped_quantise", "grouped_values"};
 const char *const kRecurNames[] = {"recur", "recur_clear"};
 const char *const kRecurStepNames[] = {"recur_step"};
 const char *const kProductNames[] = {"product", "product_join", "product_places"};
@@ -770,6 +836,9 @@ static int launch_rows(acc_op op, const char *who, const ProductVariant &v, cons
   return rc;
 }
 
+static int product_of_rows(acc_op op, const char *who, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
+                           const acc_strided *out, acc_product_args a, acc_stream stream);
+
 int acc_exec_product_rows(acc_op op, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
                           const acc_strided *out, acc_stream stream)
 try {
@@ -782,7 +851,7 @@ try {
   ACC_TRY(check_result(who, "the result", out, 2));
   if (index) ACC_TRY(check_unit(who, "index", index, 1));
   const int64_t experts = w->shape[0], n = w->shape[1], rows = out->shape[0];
-  int64_t k = w->shape[2];
+  const int64_t k = w->shape[2];
   if (!unit(*w, 2) && !unit(*w, 1)) return fail(ACC_ERR_INVALID, "%s: neither the second nor the third dimension of w is contiguous", who);
   if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
   ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
@@ -790,10 +859,19 @@ try {
   if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
   ACC_TRY(check_shape(who, "x", *x, {index ? x->shape[0] : rows, k}));
   ACC_TRY(check_extents(who, {experts, n, k, rows, x->shape[0]}));
-  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
+  const int bytes = type_bytes(op->spec.type);
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "x"}, {w, bytes, "w"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (rows == 0 || n == 0) return ACC_OK;
+  return product_of_rows(op, who, x, w, offsets, index, per, out, a, stream);
+} ACC_OP_CATCH("acc_exec_product_rows")
 
+// ... the same behind the checks, for a result that has elements
+static int product_of_rows(acc_op op, const char *who, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
+                           const acc_strided *out, acc_product_args a, acc_stream stream)
+{
+  const int64_t experts = w->shape[0], n = w->shape[1], rows = out->shape[0];
+  int64_t k = w->shape[2];
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
   ProductVariant v;
   // (where both are contiguous -- one column, or a sum of one -- either way of reading will do)
   v.b_fast = unit(*w, 2);
@@ -842,7 +920,7 @@ try {
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
   return launch_rows(op, who, v, var, a, stream);
-} ACC_OP_CATCH("acc_exec_product_rows")
+}
 
 int acc_exec_product_outer(acc_op op, const acc_strided *x, const acc_strided *y, const acc_strided *offsets, const acc_strided *index, int32_t per,
                            const acc_strided *out, acc_stream stream)
@@ -1293,6 +1371,144 @@ try {
   set_divisor(per, &a);
   return launch_rows(op, who, v, var, a, stream);
 } ACC_OP_CATCH("acc_exec_micro_rows")
+
+// ---- 4-bit whole numbers in groups --------------------------------------------------------
+
+// codes [experts, n, 16 blocks], scales and zeros [experts, groups, n] of matrices of k columns (k 0: as many as the codes have)
+static int check_grouped(acc_op op, const char *who, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, int64_t k, bool result, acc_grouped_args *a)
+{
+  ACC_TRY(result ? check_result(who, "codes", codes, 3) : check_unit(who, "codes", codes, 3));
+  ACC_TRY(result ? check_result(who, "scales", scales, 3) : check_unit(who, "scales", scales, 3));
+  if (zeros) ACC_TRY(result ? check_result(who, "zeros", zeros, 3) : check_unit(who, "zeros", zeros, 3));
+  const int64_t experts = codes->shape[0], n = codes->shape[1], blocks = ceil_div(k, 32), groups = ceil_div(k, op->spec.group);
+  ACC_TRY(check_shape(who, "codes", *codes, {experts, n, 16 * blocks}));
+  ACC_TRY(check_shape(who, "scales", *scales, {experts, groups, n}));
+  if (zeros) ACC_TRY(check_shape(who, "zeros", *zeros, {experts, groups, n}));
+  if (!aligned_rows(*codes, 1, 2)) return fail(ACC_ERR_INVALID, "%s: rows of codes start on 16 bytes", who);
+  ACC_TRY(check_extents(who, {experts, n, k}));
+  a->codes = device<void>(codes);
+  a->scales = device<void>(scales);
+  a->zeros = device<void>(zeros);
+  a->codes_expert = codes->stride[0];
+  a->codes_stride = codes->stride[1];
+  a->scales_expert = scales->stride[0];
+  a->scales_stride = scales->stride[1];
+  a->zeros_expert = zeros ? zeros->stride[0] : 0;
+  a->zeros_stride = zeros ? zeros->stride[1] : 0;
+  a->experts = (int32_t)experts;
+  a->nj = (int32_t)n;
+  a->k = (int32_t)k;
+  a->blocks = (int32_t)blocks;
+  a->group = (int32_t)std::min<int64_t>(op->spec.group, int64_t(1) << 30);
+  a->groups = (int32_t)groups;
+  for (a->group_shift = 5; (1 << a->group_shift) < a->group; ++a->group_shift) {}
+  return ACC_OK;
+}
+
+static int launch_elements(acc_op op, const char *who, bool back, int64_t threads, const acc_grouped_args &a, acc_stream stream)
+{
+  GroupedVariant v;
+  v.elements = true;
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kGroupedElementNames, 2, grouped_source_of, &var));
+  return launch(op, who, back ? var->fn2 : var->fn, ceil_div(threads, 256), 256, 0, stream, a);
+}
+
+int acc_exec_grouped_quantise(acc_op op, const acc_strided *w, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, acc_stream stream)
+try {
+  const char *who = "acc_exec_grouped_quantise";
+  acc_grouped_args a = {};
+  ACC_TRY(begin(op, ACC_OP_GROUPED, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "w", w, 3));
+  ACC_TRY(check_grouped(op, who, codes, scales, zeros, w->shape[2], true, &a));
+  ACC_TRY(check_shape(who, "w", *w, {codes->shape[0], codes->shape[1], w->shape[2]}));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {codes, 1, "codes"}, {{w, bytes, "w"}, {scales, bytes, "scales"}, {zeros, 1, "zeros"}}));
+  ACC_TRY(check_apart(who, {scales, bytes, "scales"}, {{w, bytes, "w"}, {zeros, 1, "zeros"}}));
+  if (zeros) ACC_TRY(check_apart(who, {zeros, 1, "zeros"}, {{w, bytes, "w"}}));
+  if (is_empty(*w)) return ACC_OK;
+  a.w = device<const void>(w);
+  a.w_expert = w->stride[0];
+  a.w_stride = w->stride[1];
+  return launch_elements(op, who, false, (int64_t)a.experts * a.nj * a.groups * std::min(64, a.group / 8), a, stream);
+} ACC_OP_CATCH("acc_exec_grouped_quantise")
+
+int acc_exec_grouped_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_grouped_values";
+  acc_grouped_args a = {};
+  ACC_TRY(begin(op, ACC_OP_GROUPED, who, stream, &a.guard));
+  ACC_TRY(check_result(who, "the result", out, 3));
+  ACC_TRY(check_grouped(op, who, codes, scales, zeros, out->shape[2], false, &a));
+  ACC_TRY(check_shape(who, "the result", *out, {codes->shape[0], codes->shape[1], out->shape[2]}));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{codes, 1, "codes"}, {scales, bytes, "scales"}, {zeros, 1, "zeros"}}));
+  if (is_empty(*out)) return ACC_OK;
+  a.out = device<void>(out);
+  a.out_expert = out->stride[0];
+  a.out_stride = out->stride[1];
+  return launch_elements(op, who, true, (int64_t)a.experts * a.nj * a.blocks * 4, a, stream);
+} ACC_OP_CATCH("acc_exec_grouped_values")
+
+int acc_exec_grouped_rows(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros,
+                          const acc_strided *offsets, const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream)
+try {
+  const char *who = "acc_exec_grouped_rows";
+  acc_grouped_args a = {};
+  ACC_TRY(begin(op, ACC_OP_GROUPED, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "x", x, 2));
+  ACC_TRY(check_grouped(op, who, codes, scales, zeros, x->shape[1], false, &a));
+  ACC_TRY(check_unit(who, "offsets", offsets, 1));
+  ACC_TRY(check_result(who, "the result", out, 2));
+  if (index) ACC_TRY(check_unit(who, "index", index, 1));
+  if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
+  const int64_t experts = a.experts, n = a.nj, rows = out->shape[0], k = a.k;
+  ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
+  ACC_TRY(check_shape(who, "the result", *out, {rows, n}));
+  if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
+  ACC_TRY(check_shape(who, "x", *x, {index ? x->shape[0] : rows, k}));
+  ACC_TRY(check_extents(who, {rows, x->shape[0]}));
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "x"}, {codes, 1, "codes"}, {scales, bytes, "scales"}, {zeros, 1, "zeros"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
+  if (is_empty(*out)) return ACC_OK;
+  const int64_t mean = ceil_div(rows, std::max<int64_t>(1, std::min(rows, experts)));
+  if (mean > kGroupedMost && k > 0 && x->shape[0] > 0) {
+    ScratchHold made;
+    ACC_TRY(made.acquire(op, stream, (size_t)(experts * n * ceil_div(k, 8) * 8 * bytes)));
+    acc_strided w = {};
+    w.rank = 3;
+    w.shape[0] = experts;
+    w.shape[1] = n;
+    w.shape[2] = k;
+    w.stride[2] = 1;
+    w.stride[1] = ceil_div(k, 8) * 8;
+    w.stride[0] = n * w.stride[1];
+    w.ptr = reinterpret_cast<uint64_t>(made.ref.ptr);
+    acc_grouped_args b = a;
+    b.out = made.ref.ptr;
+    b.out_expert = w.stride[0];
+    b.out_stride = w.stride[1];
+    ACC_TRY(launch_elements(op, who, true, experts * n * a.blocks * 4, b, stream));
+    acc_product_args product = {};
+    product.guard = a.guard;
+    return product_of_rows(op, who, x, &w, offsets, index, per, out, product, stream);
+  }
+  const GroupedVariant v = grouped_variant(rows, experts, n, mean);
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kGroupedNames, 1, grouped_source_of, &var));
+  a.x = device<const void>(x);
+  a.out = device<void>(out);
+  a.offsets = device<const int32_t>(offsets);
+  a.index = device<const int32_t>(index);
+  a.x_stride = x->stride[0];
+  a.out_stride = out->stride[0];
+  a.rows = rows;
+  a.x_rows = (int32_t)x->shape[0];
+  set_divisor(per, &a);
+  a.tiles_i = (int32_t)tiles_at_most(rows, experts, v.bm);
+  a.tiles_j = (int32_t)ceil_div(n, 16 * v.fn);
+  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * kGroupedWaves, 0, stream, a);
+} ACC_OP_CATCH("acc_exec_grouped_rows")
 
 // ---- recurrence -------------------------------------------------------------------------
 

@@ -86,6 +86,22 @@ struct acc_micro_args {
   const uint32_t *guard;
 };
 
+/* matrices of 4-bit whole numbers in groups: see op_grouped.h */
+struct acc_grouped_args {
+  const void *x, *w;            /* rows: the rows; quantise: the matrices */
+  void *out;                    /* rows, values */
+  void *codes, *scales, *zeros; /* zeros 0: all 8 */
+  const int32_t *offsets, *index;
+  int64_t x_stride, w_stride, w_expert, out_stride, out_expert;
+  int64_t codes_stride, codes_expert, scales_stride, scales_expert, zeros_stride, zeros_expert;   /* scales, zeros: from one group to the next */
+  int64_t rows;
+  int32_t x_rows, experts, nj, k;
+  int32_t blocks, group, groups, group_shift;
+  int32_t tiles_i, tiles_j;
+  uint32_t per_mul, per_shift;
+  const uint32_t *guard;
+};
+
 /* the recurrence: see op_recur.h */
 struct acc_recur_args {
   const void *gates, *values;

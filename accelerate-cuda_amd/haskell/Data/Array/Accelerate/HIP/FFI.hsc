@@ -453,12 +453,13 @@ foreign import ccall safe   "acc_memtable_reclaim"          c_memtableReclaim   
 foreign import ccall safe   "acc_memtable_get_stats"        c_memtableGetStats        :: MemTable -> Ptr MemTableStats -> IO Status
 
 -- Operators on segments of rows: products, routing, combination, 4-bit numbers.  An array of theirs has strides.
-accOpProduct, accOpRoute, accOpCombine, accOpMicro, accOpRecur :: CInt
+accOpProduct, accOpRoute, accOpCombine, accOpMicro, accOpRecur, accOpGrouped :: CInt
 accOpProduct = #{const ACC_OP_PRODUCT}
 accOpRoute   = #{const ACC_OP_ROUTE}
 accOpCombine = #{const ACC_OP_COMBINE}
 accOpMicro   = #{const ACC_OP_MICRO}
 accOpRecur   = #{const ACC_OP_RECUR}
+accOpGrouped = #{const ACC_OP_GROUPED}
 
 accGateGiven, accGateSigmoid :: Int32
 accGateGiven   = #{const ACC_GATE_GIVEN}
@@ -492,6 +493,7 @@ data OpDesc = OpDesc
   , opChoose    :: Int32
   , opNormalise :: Bool
   , opGate      :: Int32              -- a recurrence's: accGate*
+  , opGroup     :: Int32              -- of grouped 4-bit numbers: neighbours under a scale
   }
 
 instance Storable OpDesc where
@@ -503,14 +505,16 @@ instance Storable OpDesc where
     c <- #{peek acc_op_desc, choose} p
     n <- #{peek acc_op_desc, normalise} p :: IO Int32
     g <- #{peek acc_op_desc, gate} p
-    return (OpDesc (fromIntegral k) t c (n /= 0) g)
-  poke p (OpDesc k t c n g) = do
+    w <- #{peek acc_op_desc, group} p
+    return (OpDesc (fromIntegral k) t c (n /= 0) g w)
+  poke p (OpDesc k t c n g w) = do
     fillBytes p 0 #{size acc_op_desc}
     #{poke acc_op_desc, kind} p (fromIntegral k :: Int32)
     #{poke acc_op_desc, elt_type} p t
     #{poke acc_op_desc, choose} p c
     #{poke acc_op_desc, normalise} p (if n then 1 else 0 :: Int32)
     #{poke acc_op_desc, gate} p g
+    #{poke acc_op_desc, group} p w
 
 foreign import ccall safe   "acc_op_create"             c_opCreate            :: Context -> Ptr OpDesc -> Ptr Op -> IO Status
 foreign import ccall safe   "acc_op_destroy"            c_opDestroy           :: Op -> IO Status
@@ -524,6 +528,9 @@ foreign import ccall safe   "acc_exec_combine_gradient" c_execCombineGradient ::
 foreign import ccall safe   "acc_exec_micro_quantise"   c_execMicroQuantise   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_micro_values"     c_execMicroValues     :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_micro_rows"       c_execMicroRows       :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_grouped_quantise" c_execGroupedQuantise :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_grouped_values"   c_execGroupedValues   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_grouped_rows"     c_execGroupedRows     :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_recur"            c_execRecur           :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_recur_gradient"   c_execRecurGradient   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_recur_step"       c_execRecurStep       :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status

@@ -677,7 +677,8 @@ enum {
   ACC_OP_COMBINE = 2,
   ACC_OP_MICRO   = 3,
   ACC_OP_RECUR   = 5,        /* (4 is no kind)                                    */
-  ACC_OP_KIND_COUNT = 6
+  ACC_OP_GROUPED = 6,
+  ACC_OP_KIND_COUNT = 7
 };
 
 /* what a recurrence's gates are */
@@ -692,6 +693,7 @@ typedef struct acc_op_desc {
   int32_t     choose;        /* ACC_OP_ROUTE: experts a token, 1 to 64            */
   int32_t     normalise;     /* ACC_OP_ROUTE: softmax over the chosen (else over all experts) */
   int32_t     gate;          /* ACC_OP_RECUR: ACC_GATE_*                          */
+  int32_t     group;         /* ACC_OP_GROUPED: neighbours under a scale, a power of two of 32 or more */
 } acc_op_desc;
 
 /* An instance; its kernels are compiled through the cache when a call first needs them (as the variants of a skeleton
@@ -748,6 +750,22 @@ int acc_exec_micro_values(acc_op op, const acc_strided *codes, const acc_strided
 int acc_exec_micro_rows(acc_op op, const acc_strided *xcodes, const acc_strided *xscales, const acc_strided *wcodes,
                         const acc_strided *wscales, const acc_strided *offsets, const acc_strided *index, int32_t per,
                         const acc_strided *out, acc_stream stream);
+
+/* Matrices of 4-bit whole numbers: w[e, n, k] = (q - z) s, the codes q from 0 to 15, a scale s and a zero z for every `group`
+ * neighbours of a row.  codes [experts, n, 16 ceil(k / 32)] bytes as for acc_exec_micro_quantise (two numbers a byte, the even place
+ * in the low half, rows on 16 bytes); scales [experts, ceil(k / group), n] in the operator's type, zeros the same in bytes, both with
+ * n contiguous; zeros NULL: all 8.  quantise, of w [experts, n, k]: with zeros s = (high - low) / 15 of a group's range, which has 0 in
+ * it, z = -low / s, without s = the largest magnitude / 7; s is rounded to the type, then the numbers, ties to even.  A group with an
+ * infinity or what is not a number has a scale that is not a number.                                          */
+int acc_exec_grouped_quantise(acc_op op, const acc_strided *w, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros,
+                              acc_stream stream);
+int acc_exec_grouped_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, const acc_strided *out,
+                            acc_stream stream);
+/* acc_exec_product_rows with such matrices and rows x [.., k] of the operator's type.  (For a few rows of each matrix the numbers
+ * are multiplied as they are; for many the matrices are first made again in the operator's type, in scratch memory.)  A row
+ * with an infinity in it gives what is not a number. */
+int acc_exec_grouped_rows(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros,
+                          const acc_strided *offsets, const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream);
 
 /* A gated linear recurrence along the rows of every sequence, channel by channel: h[t] = a[t] h[t-1] + b[t] (ACC_GATE_*), the
  * state Float32 throughout.  gates, values, out [rows, width], innermost dimension contiguous; the rows of sequence s are
