@@ -204,21 +204,31 @@ std::string recur_source(const OpSpec &sp, const RecurVariant &v)
   return text;
 }
 
-// grouped: rows and columns of a tile, in sixteens; what a lane asks for at once is less where a tile has many rows
+// grouped: rows and columns of a tile, in sixteens, and the steps that are asked for ahead
 struct GroupedVariant {
   int bm = 16, fn = 1;
+  bool zeros = false;
+  int wide = 16;                // ... waves of that form
+  bool few = false;             // ... and each has a few steps
+  bool sixteen = false;         // tiles of sixteen rows, whose places are known when the kernel is compiled
+  bool stream = false;          // rows in LDS, waves that go over columns (else they read rows and codes for every tile)
   bool elements = false;
-  int ahead(int type) const { return elements || bm > 32 || (bm > 16 && type == 0) ? 1 : bm > 16 || fn > 1 || type == 0 ? 2 : 4; }
-  uint32_t key() const { return kGroupedKeys | (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u); }
+  int waves() const { return stream || fn == 1 ? wide : 4; }
+  int ahead(const OpSpec &sp) const
+  {
+    // (their scales and zeros are a load of 64 lanes)
+    if (stream) return few || sp.group == 32 || (sp.group == 64 && sp.type == 0) ? 2 : 4;
+    return elements || bm > 32 || (bm > 16 && sp.type == 0) ? 1 : bm > 16 || fn > 1 || sp.type == 0 ? 2 : 4;
+  }
+  uint32_t key() const { return kGroupedKeys | (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u) | (stream ? 512u : 0u) | (zeros ? 1024u : 0u) | (wide == 8 ? 2048u : 0u) | (sixteen ? 4096u : 0u) | (few ? 8192u : 0u); }
   static constexpr uint32_t kGroupedKeys = 1u << 21;               // (beside the products' keys)
 };
-constexpr int kGroupedWaves = 8;
 std::string grouped_source(const OpSpec &sp, const GroupedVariant &v)
 {
   char text[512];
   std::snprintf(text, sizeof(text),
-                "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_GROUP %d\n#define OP_AHEAD %d\n#define OP_ELEMENTS %d\n#include \"acc_hip_device.h\"\n#include \"op_grouped.h\"\n",
-                sp.type, sp.type == 1 ? 1 : 2, v.bm, v.fn, v.elements ? 4 : std::min(4, sp.group / 32), v.ahead(sp.type), v.elements ? 1 : 0);
+                "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_GROUP %d\n#define OP_AHEAD %d\n#define OP_STREAM %d\n#define OP_WAVES %d\n#define OP_ZEROS %d\n#define OP_HEIGHT %d\n#define OP_ELEMENTS %d\n#include \"acc_hip_device.h\"\n#include \"op_grouped.h\"\n",
+                sp.type, sp.type == 1 ? 1 : 2, v.bm, v.fn, v.elements ? 4 : std::min(4, sp.group / 32), v.ahead(sp), v.stream ? 1 : 0, v.waves(), v.zeros ? 1 : 0, v.sixteen ? 16 : 0, v.elements ? 1 : 0);
   return text;
 }
 
@@ -270,11 +280,19 @@ std::vector<std::string> all_sources(const OpSpec &sp)
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
   } else if (sp.kind == ACC_OP_GROUPED) {
     for (int bm : {16, 32, 64})
-      for (int fn : {1, 2}) {
+      for (int form = 0; form < 12; ++form) {
         GroupedVariant v;
         v.bm = bm;
-        v.fn = fn;
-        out.push_back(grouped_source(sp, v));
+        v.zeros = form & 1;
+        v.stream = form >= 4;
+        if (!v.stream) v.fn = 1 + form / 2;
+        if (!v.stream && bm > 32 && v.fn == 1) continue;
+        v.wide = form & 2 || !v.stream ? 8 : 16;
+        v.sixteen = form >= 8;
+        for (bool few : {false, true}) {
+          v.few = few;
+          if (!(few && !v.stream) && !(v.stream && bm > 32) && !(v.sixteen && bm > 16)) out.push_back(grouped_source(sp, v));
+        }
       }
     GroupedVariant v;
     v.elements = true;
@@ -558,13 +576,45 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
   return experts * piece >= 2 * rows ? 0 : (int32_t)piece;
 }
 
-// grouped: the tile for `mean` rows a segment, and from how many on the matrices are made again for tiles that use them often
-constexpr int64_t kGroupedMost = 96;
-GroupedVariant grouped_variant(int64_t rows, int64_t experts, int64_t n, int64_t mean)
+// grouped: from how many rows a segment on the matrices are made again for tiles that use them often.  us, as they are and made again:
+// 160 rows, 2 of 4096 x 4096: 41 and 53; 512, 8: 83 and 162; 2048, 8: some 330 and 229
+constexpr int64_t kGroupedMost = 128;
+// ... LDS of the form with rows in it: `height` of them, their sums by groups, and the waves' results where they share columns
+int64_t grouped_lds(const OpSpec &sp, int64_t height, int64_t steps, int64_t waves)
+{
+  const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
+  return steps * height * (256 * (sp.type == 0 ? 3 : 1) + chunks * (sp.type == 1 ? 8 : 4)) + waves * ceil_div(height, 16) * 1024;
+}
+constexpr int64_t kGroupedLds = 160 << 10;
+// ... and the tiles of 16 columns from which on rows in LDS are worth what it takes to put them there.  us, with and without, tiles: 1 row,
+// 4096 x 4096, 256: 8.2 and 7.2; 16 rows: 14 and 11; 2 rows of 4096 x 11008, 256: 16 and 15; of 11008 x 4096, 688: 13 and 18; 1 row, 8192 x 8192,
+// 512: 16 and 23; 64 rows, 16 half of 4096 x 2048, 4096: 23 and 34; 16, 8 of 4096 x 4096 in groups of 32: 29 and 44; Float32, 64, 16 of
+// 1024 x 2048, 1024: 14 and 12
+constexpr int64_t kGroupedStream = 384;
+// the tile for `mean` rows a segment; *height: its rows.  (Where LDS holds fewer rows than a segment has, their codes are read again:
+// 64 rows, 2 of 4096 x 4096: 18 us in tiles of 16, 26 without LDS.)
+GroupedVariant grouped_variant(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean, int64_t *height)
 {
   GroupedVariant v;
+  const int64_t steps = ceil_div(k, 128);
   v.bm = mean > 32 ? 64 : mean > 16 ? 32 : 16;
-  v.fn = std::min(rows, experts) * ceil_div(n, 32) >= 512 ? 2 : 1;
+  *height = v.bm;
+  if (v.bm < 64 && n >= 16 && pitch < (1 << 27) && steps > 0) {
+    int64_t h = v.bm;
+    while (h > 1 && grouped_lds(sp, h, steps, 16) > kGroupedLds) h /= 2;
+    const int64_t tiles = std::max(ceil_div(rows, h), std::min(rows, experts)) * ceil_div(n, 16);
+    if (grouped_lds(sp, h, steps, 16) <= kGroupedLds && h * 4 >= mean && tiles >= kGroupedStream) {
+      v.stream = true;
+      v.bm = h > 16 ? 32 : 16;
+      v.sixteen = h == 16;
+      // (two workgroups a compute unit where there is room: one begins while the other is at its columns)
+      v.wide = grouped_lds(sp, h, steps, 16) <= kGroupedLds / 2 ? 8 : 16;
+      *height = h;
+      return v;
+    }
+  }
+  v.wide = 8;
+  v.fn = v.bm > 32 || std::min(rows, experts) * ceil_div(n, 32) >= 512 ? 2 : 1;
   return v;
 }
 
@@ -629,6 +679,11 @@ std::string grouped_source_of(const OpSpec &sp, uint32_t key)
   v.bm = (int)(key & 15u) * 16;
   v.fn = (int)(key >> 4 & 15u);
   v.elements = key & 256u;
+  v.stream = key & 512u;
+  v.zeros = key & 1024u;
+  v.wide = key & 2048u ? 8 : 16;
+  v.sixteen = key & 4096u;
+  v.few = key & 8192u;
   return grouped_source(sp, v);
 }
 
@@ -1493,9 +1548,9 @@ try {
     product.guard = a.guard;
     return product_of_rows(op, who, x, &w, offsets, index, per, out, product, stream);
   }
-  const GroupedVariant v = grouped_variant(rows, experts, n, mean);
-  const OpVariant *var = nullptr;
-  ACC_TRY(op->variant(v.key(), kGroupedNames, 1, grouped_source_of, &var));
+  int64_t height = 0;
+  GroupedVariant v = grouped_variant(op->spec, rows, experts, n, k, codes->stride[1], mean, &height);
+  v.zeros = zeros != nullptr;
   a.x = device<const void>(x);
   a.out = device<void>(out);
   a.offsets = device<const int32_t>(offsets);
@@ -1505,9 +1560,23 @@ try {
   a.rows = rows;
   a.x_rows = (int32_t)x->shape[0];
   set_divisor(per, &a);
-  a.tiles_i = (int32_t)tiles_at_most(rows, experts, v.bm);
-  a.tiles_j = (int32_t)ceil_div(n, 16 * v.fn);
-  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * kGroupedWaves, 0, stream, a);
+  a.tiles_i = (int32_t)tiles_at_most(rows, experts, height);
+  a.height = (int32_t)height;
+  a.run = v.fn;
+  size_t lds = 0;
+  if (v.stream) {
+    // a workgroup a compute unit; where it has fewer tiles of columns than waves, those share them
+    const int64_t all = std::max(ceil_div(rows, height), std::min(rows, experts)) * ceil_div(n, 16);
+    a.run = (int32_t)std::max<int64_t>(1, std::min(ceil_div(n, 16), ceil_div(all, v.wide == 8 ? 512 : 256)));
+    a.split = 1;
+    while (a.split < v.waves() && a.split * a.run < v.waves() && a.split < ceil_div(k, 128)) a.split *= 2;
+    lds = (size_t)grouped_lds(op->spec, height, ceil_div(k, 128), v.waves());
+    v.few = ceil_div(ceil_div(k, 128), a.split) <= 2;
+  }
+  a.tiles_j = (int32_t)ceil_div(n, 16 * a.run);
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kGroupedNames, 1, grouped_source_of, &var));
+  return launch(op, who, var->fn, (int64_t)a.tiles_i * a.tiles_j, 64 * v.waves(), lds, stream, a);
 } ACC_OP_CATCH("acc_exec_grouped_rows")
 
 // ---- recurrence -------------------------------------------------------------------------

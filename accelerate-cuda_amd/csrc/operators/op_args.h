@@ -97,6 +97,9 @@ struct acc_grouped_args {
   int64_t rows;
   int32_t x_rows, experts, nj, k;
   int32_t blocks, group, groups, group_shift;
+  int32_t run;                  /* tiles of 16 columns of a workgroup */
+  int32_t height, split;        /* rows of a tile; waves that share a tile's k */
+  int32_t pad;
   int32_t tiles_i, tiles_j;
   uint32_t per_mul, per_shift;
   const uint32_t *guard;

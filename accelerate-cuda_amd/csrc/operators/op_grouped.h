@@ -4,43 +4,50 @@
  *   w[e, n, k] = (q[e, n, k] - z[e, g, n]) s[e, g, n],   g = k / group;   z = 8 where there are no zeros
  *   out[m, n]  = sum_k x[r(m), k] w[e(m), n, k]          for a few rows of each matrix
  *
- * The products are taken of the numbers as they are: a code's four bits are the mantissa's first, of 16 + q (exact in both 16-bit
- * types), the matrix cores add up x (16 + q) and x alone over what a group has of a step, and then
+ * The products are taken of the numbers as they are: a code's four bits become the mantissa of d + q, exact in either 16-bit type,
+ * with a d that its place in the word decides (half: 1024, 64; bfloat16: 128; for Float32 rows 16); the matrix cores add up x (d + q)
+ * over what a group has of a step, beginning with -(z sum x + sum d x), and that times s is added up in Float32: no weight is ever
+ * rounded.  What is taken off again costs some of the 24 bits of a sum: of half ones eight of those beyond a 4-bit number's own, in
+ * bfloat16 five, Float32 two.  Float32 rows are cut into three bfloat16 each, which hold all 24 bits.  (An infinity in a row makes the
+ * row's results NaN.)
  *
- *   sum += s (sum x (16 + q)) - s (16 + z) (sum x)
- *
- * in Float32: no weight is ever rounded.  What is taken off again is 16 to 31 times a row's sum at most, of whose 24 bits it costs
- * two or three beside the 4-bit numbers' own.  Float32 rows are cut into three bfloat16 each, which hold all 24 bits.  (An infinity
- * in a row makes the row's results NaN.)
- *
- * What counts is that the matrices pass by once.  A lane loads 16 bytes of codes, 32 numbers of a row, straight into registers,
- * OP_AHEAD steps of 128 numbers of k at a time; four lanes then exchange words so that a fragment is 32 neighbours of one
- * group.  The eight waves of a workgroup take every eighth step of the same 16 OP_FN columns and add up what they have by way of
- * LDS, in order.
+ * What counts is that the matrices pass by once, and that their codes are nearly all that is read.  A lane loads 16 bytes of them, 32
+ * numbers of a row.  Where a matrix has many columns for a compute unit, the rows lie in LDS and waves go over the columns (OP_STREAM);
+ * where it has few, what counts is how soon all of it is on its way, and the waves of a workgroup take every so many steps of the same
+ * 16 OP_FN columns and add up what they have by way of LDS, in order.  64 half rows, 16 matrices of 4096 x 2048 in groups of 64 with
+ * zeros: 23 us, of which the codes' loads alone take 13 (5.8 TB/s), what is in front of them 8 with the launch; bfloat16 in groups of 128,
+ * 16 rows, 8 of 4096 x 4096: 19 us; 1 row, 1 of 4096 x 4096: 7.2.
  */
 #include "op_matrix.h"
 
 #define OP_FM (OP_BM / 16)
-#define OP_WAVES 8
 
-#if OP_TYPE == 1
-#define OP_SIXTEEN 0x4C004C00u
-#define OP_FOUR_BITS 0x03C003C0u
+/* 8 codes as d + q: of neighbours 0 4, 1 5, 2 6, 3 7; and the d alone */
+#if OP_ELT == 1
 #define OP_ONES 0x3C003C00u
-#define OP_UP 6                                    /* where a number of the low bits goes */
-#else
-#define OP_SIXTEEN 0x41804180u
-#define OP_FOUR_BITS 0x00780078u
-#define OP_ONES 0x3F803F80u
-#define OP_UP 3
-#endif
-
-/* 8 codes as 16 + q: of neighbours 0 4, 1 5, 2 6, 3 7 */
-ACC_DEV acc_u4 op_sixteens(const unsigned int w)
+ACC_DEV acc_u4 op_numbers(const unsigned int w)
 {
-  const auto at = [](const unsigned int v) { return (v & OP_FOUR_BITS) | OP_SIXTEEN; };
-  return acc_u4{at(w << OP_UP), at(OP_UP >= 4 ? w << (OP_UP - 4) : w >> (4 - OP_UP)), at(w >> (8 - OP_UP)), at(w >> (12 - OP_UP))};
+  const unsigned int v = w >> 8;
+  return acc_u4{(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x54005400u, (v & 0x000F000Fu) | 0x64006400u, (v & 0x00F000F0u) | 0x54005400u};
 }
+ACC_DEV acc_u4 op_offsets() { return acc_u4{0x64006400u, 0x54005400u, 0x64006400u, 0x54005400u}; }
+#elif OP_ELT == 2
+#define OP_ONES 0x3F803F80u
+ACC_DEV acc_u4 op_numbers(const unsigned int w)
+{
+  const auto at = [](const unsigned int v) { return (v & 0x000F000Fu) | 0x43004300u; };
+  return acc_u4{at(w), at(w >> 4), at(w >> 8), at(w >> 12)};
+}
+ACC_DEV acc_u4 op_offsets() { return acc_u4{0x43004300u, 0x43004300u, 0x43004300u, 0x43004300u}; }
+#else
+#define OP_ONES 0x3F803F80u
+ACC_DEV acc_u4 op_numbers(const unsigned int w)
+{
+  const auto at = [](const unsigned int v) { return (v & 0x00780078u) | 0x41804180u; };
+  return acc_u4{at(w << 3), at(w >> 1), at(w >> 5), at(w >> 9)};
+}
+ACC_DEV acc_u4 op_offsets() { return acc_u4{0x41804180u, 0x41804180u, 0x41804180u, 0x41804180u}; }
+#endif
 
 /* a row's 8 neighbours in that order, in OP_PARTS parts that add up to them */
 #if OP_ELT == 0
@@ -84,19 +91,24 @@ ACC_DEV op_eight op_row8(const op_elt *p, const int valid)
   return x;
 }
 
-/* four lanes' words w[f] of numbers 32 g + 8 f on: w[b] becomes those of 32 b + 8 g on */
+/* Four lanes have words w[f] of numbers 32 g + 8 f on.  Where a step has one group that is as good an order as any; where it has
+ * several, w[b] becomes those of 32 b + 8 g on.  OP_FIRST: the first number of a lane's b-th word. */
+#define OP_CHUNKS (OP_GROUP >= 4 ? 1 : 4 / OP_GROUP)        /* groups of a step (OP_GROUP: blocks of 32 of a group, 4: or more) */
+#define OP_BLOCKS (4 / OP_CHUNKS)                  /* words of a group in a step */
+#define OP_FIRST(b, g) (OP_CHUNKS > 1 ? 32 * (b) + 8 * (g) : 32 * (g) + 8 * (b))
 ACC_DEV void op_turn(acc_u4 &w)
 {
+  if (OP_CHUNKS == 1) return;
   const auto a = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false), b = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
   const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
   w = acc_u4{c[0], c[1], d[0], d[1]};
 }
 
-/* four neighbours of a row of scales (or zeros), of which the last ones may not be there */
+/* four neighbours of a row of scales (or zeros); `whole`: they are all there, in every lane */
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) op_e4 { T v[4]; };
-template <typename T> ACC_DEV op_e4<T> op_four(const T *p, const int at, const int end)
+template <typename T> ACC_DEV op_e4<T> op_four(const T *p, const bool whole, const int at, const int end)
 {
-  if (at + 4 <= end) return *(const op_e4<T> *)(p + at);
+  if (whole) return *(const op_e4<T> *)(p + at);
   op_e4<T> e;
 #pragma unroll
   for (int t = 0; t < 4; ++t) e.v[t] = p[acc_min(at + t, end - 1)];
@@ -180,7 +192,201 @@ extern "C" __global__ void __launch_bounds__(256) grouped_values(const acc_group
 }
 #else
 
-#define OP_CHUNKS (OP_GROUP >= 4 ? 1 : 4 / OP_GROUP)        /* groups of a step (OP_GROUP: blocks of 32 of a group, 4: or more) */
+/* what products of a group begin with, -(z sum x + sum d x), in column r */
+ACC_DEV float op_begin(const float sum, const float offset, const float zero) { return __builtin_fmaf(-zero, sum, -offset); }
+
+#if OP_STREAM
+/* The form whose rows lie in LDS, cut and in the order of fragments, with their sums by groups: p.height rows of a tile (a power of
+ * two up to 16, or 16 OP_FM).  A wave goes over columns, 16 at a time, or over a part of k of the same columns as its neighbours where
+ * there are few (p.split of them, whose sums then meet in LDS).  It takes OP_AHEAD steps at a time while the codes of the next ones
+ * are on their way; their scales and zeros, of 16 columns, are a load of 16 bytes in as many lanes as it takes, and go round by way of
+ * LDS (asked for by every lane that wants them they cost more of the cache's time than the codes).  No load is behind a branch, so that
+ * what is on its way can be counted: steps and columns that there are not are read as the last ones. */
+#define OP_NOTED (OP_AHEAD * OP_CHUNKS)            /* groups of so many steps */
+#define OP_SIZE ((int)sizeof(op_elt))              /* lanes of a group's 16 scales; one has its zeros */
+
+extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_grouped_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  extern __shared__ acc_u4 shared[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
+  const op_tile tile = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, p.height, op_segments(p.offsets, p.experts, (int)p.rows, 0, 0), (int)(blockIdx.x / p.tiles_j));
+  if (tile.begin >= tile.end) return;
+  const int steps = (p.blocks + 3) / 4, rows = tile.end - tile.begin, tiles = (p.nj + 15) / 16, height = OP_HEIGHT ? OP_HEIGHT : p.height;
+  const int j0 = (int)(blockIdx.x % p.tiles_j) * p.run, here = acc_min(p.run, tiles - j0);       /* tiles of columns */
+  const bool sums = tile.expert >= 0 && p.x_rows > 0 && steps > 0;
+  acc_u4 *const notes = shared;                    /* [waves][OP_FM][64]: a wave's scales and zeros; its sums, where they meet */
+  acc_u4 *const x = notes + OP_WAVES * OP_FM * 64; /* [steps][4][parts][4][height] */
+  float *const sum = (float *)(x + steps * 16 * OP_PARTS * height);       /* [steps][chunks][height], and of half the offsets' */
+  float *const offset = OP_ELT == 1 ? sum + steps * OP_CHUNKS * height : sum;
+  const auto row_of = [&](const int i) { return p.index ? op_listed(p.index, tile.begin + i, tile.begin, tile.end, p.x_rows, p.per_mul, p.per_shift) : tile.begin + i; };
+  const auto write = [&](const int jt, const acc_f4 (&c)[OP_FM]) {
+#pragma unroll
+    for (int i = 0; i < OP_FM; ++i) {
+      const int m = i * 16 + l;
+      if (m < rows) op_write4((op_elt *)p.out + (long long)(tile.begin + m) * p.out_stride, jt * 16 + 4 * g, p.nj, c[i], !sums || row_of(m) < 0);
+    }
+  };
+  if (!sums) {
+    const acc_f4 none[OP_FM] = {};
+    for (int t = wave; t < here; t += OP_WAVES) write(j0 + t, none);
+    return;
+  }
+
+  const unsigned char *const codes = (const unsigned char *)p.codes + tile.expert * p.codes_expert, *const zeros = (const unsigned char *)p.zeros + tile.expert * p.zeros_expert;
+  const op_elt *const scales = (const op_elt *)p.scales + tile.expert * p.scales_expert;
+  const int split = p.split, each = (steps + split - 1) / split, n0 = wave % split * each, n1 = acc_min(steps, n0 + each), stride = OP_WAVES / split;
+  const int mine = wave / split, turns = (here + stride - 1) / stride, own = n1 > n0 && mine < here ? (here - mine + stride - 1) / stride : 0;
+  const int last_tile = p.nj % 16 ? tiles - 1 : -1, last_step = p.blocks % 4 ? steps - 1 : -1;      /* that are not whole */
+  const unsigned int pitch = (unsigned int)p.codes_stride, row = l * pitch + g * 16, last_row = acc_min(l, p.nj - 1 - last_tile * 16) * pitch + g * 16;
+  const unsigned int early = (unsigned int)acc_max(0, g - (p.blocks - 1 - last_step * 4)) * 16;
+  /* codes of columns jt, step n: an address that is the same in all lanes, and 32 bits of the lane's */
+  const auto load = [&](const int jt, const int n, acc_u4 &w) {
+    const unsigned int at = (jt != last_tile ? row : last_row) - (n != last_step ? 0u : early);
+    w = __builtin_nontemporal_load((const acc_u4 *)(codes + ((long long)jt * 16 * p.codes_stride + n * 64) + at));
+  };
+  /* the lane's part of the scales and zeros of 16 columns from step n on (of the last columns: the last 16 there are) */
+  const bool scale_lane = lane < OP_NOTED * OP_SIZE;
+  const int noted = scale_lane ? lane / OP_SIZE : acc_min(lane - OP_NOTED * OP_SIZE, OP_NOTED - 1);
+  const char *const note_base = scale_lane || !OP_ZEROS ? (const char *)scales + lane % OP_SIZE * 16 : (const char *)zeros;
+  const long long note_stride = scale_lane || !OP_ZEROS ? p.scales_stride * OP_SIZE : p.zeros_stride;
+  const auto load_note = [&](const int jt, const int n, acc_u4 &note) {
+    const int column = jt != last_tile ? jt * 16 : p.nj - 16, group = acc_min(((n * 128) >> p.group_shift) + noted, p.groups - 1);
+    note = ((const op_loose<unsigned char> *)(note_base + (group * note_stride + column * (scale_lane || !OP_ZEROS ? OP_SIZE : 1))))->v;
+  };
+  acc_f4 c[OP_FM];
+  const char *const my_notes = (const char *)(notes + wave * OP_FM * 64);
+  /* step n's products, the first of its groups being the at-th that is noted; `down`: the columns' places among the noted 16 */
+  const auto add = [&](const int n, const int at, const int down, acc_u4 w) {
+    op_turn(w);
+#pragma unroll
+    for (int q = 0; q < OP_CHUNKS; ++q) {
+      const int noted_at = at + q;
+      op_e4<op_elt> s;
+      op_e4<unsigned char> z;
+      if (down == 0) {
+        __builtin_memcpy(&s, __builtin_assume_aligned(my_notes + (noted_at * 16 + g * 4) * OP_SIZE, 4 * OP_SIZE), sizeof(s));
+        if (OP_ZEROS) __builtin_memcpy(&z, __builtin_assume_aligned(my_notes + OP_NOTED * OP_SIZE * 16 + noted_at * 16 + g * 4, 4), sizeof(z));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int k = acc_min(g * 4 + r + down, 15);
+          s.v[r] = *(const op_elt *)(my_notes + (noted_at * 16 + k) * OP_SIZE);
+          if (OP_ZEROS) z.v[r] = *(const unsigned char *)(my_notes + OP_NOTED * OP_SIZE * 16 + noted_at * 16 + k);
+        }
+      }
+      acc_f4 t[OP_FM];
+#pragma unroll
+      for (int i = 0; i < OP_FM; ++i) {
+        const int place = (n * OP_CHUNKS + q) * height + ((i * 16 + l) & (height - 1));
+        const float f = sum[place], d = OP_ELT == 1 ? offset[place] : (OP_ELT == 2 ? 128.0f : 16.0f) * f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, d, OP_ZEROS ? (float)z.v[r] : 8.0f);
+      }
+#pragma unroll
+      for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
+        const op_frag v = op_as_frag(op_numbers(w[b]));
+#pragma unroll
+        for (int i = 0; i < OP_FM; ++i)
+#pragma unroll
+          for (int part = OP_PARTS - 1; part >= 0; --part) t[i] = op_mfma(v, op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]), t[i]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < OP_FM; ++i) c[i][r] = __builtin_fmaf((float)s.v[r], t[i][r], c[i][r]);
+    }
+  };
+  const auto clear = [&]() {
+#pragma unroll
+    for (int i = 0; i < OP_FM; ++i) c[i] = acc_f4{0.0f, 0.0f, 0.0f, 0.0f};
+  };
+  const int lots = n1 > n0 ? (n1 - n0 + OP_AHEAD - 1) / OP_AHEAD : 0, all = own * lots;
+  acc_u4 ring[OP_AHEAD], note;
+  if (all > 0) {
+    load_note(j0 + mine, n0, note);
+#pragma unroll
+    for (int u = 0; u < OP_AHEAD; ++u) load(j0 + mine, acc_min(n0 + u, n1 - 1), ring[u]);
+  }
+
+  /* the rows: a lane has eight neighbours of one; rows that there are not stay as LDS is, and nobody's */
+  for (int at = tid; at < steps * 16 * rows; at += 64 * OP_WAVES) {
+    const int i = at / (steps * 16), k = (at - i * steps * 16) * 8, n = k / 128, kk = k % 128, r = row_of(i);
+    const int b = OP_CHUNKS > 1 ? kk / 32 : kk / 8 % 4, quarter = OP_CHUNKS > 1 ? kk / 8 % 4 : kk / 32;
+    acc_u4 v[OP_PARTS];
+    op_parts(op_row8((const op_elt *)p.x + (long long)acc_max(r, 0) * p.x_stride + k, p.k - k), v);
+#pragma unroll
+    for (int part = 0; part < OP_PARTS; ++part) x[(((n * 4 + b) * OP_PARTS + part) * 4 + quarter) * height + i] = v[part];
+  }
+  __syncthreads();
+  for (int n = wave; n < steps; n += OP_WAVES)
+#pragma unroll
+    for (int q = 0; q < OP_CHUNKS; ++q)
+#pragma unroll
+      for (int i = 0; i < OP_FM; ++i) {
+        acc_f4 t = {0.0f, 0.0f, 0.0f, 0.0f}, d = t;
+#pragma unroll
+        for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b)
+#pragma unroll
+          for (int part = OP_PARTS - 1; part >= 0; --part) {
+            const op_frag y = op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]);
+            t = op_mfma(op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), y, t);
+            if (OP_ELT == 1) d = op_mfma(op_as_frag(op_offsets()), y, d);
+          }
+        const int at = (n * OP_CHUNKS + q) * height + i * 16 + l;
+        if (g == 0 && i * 16 + l < height) {
+          sum[at] = t[0];
+          if (OP_ELT == 1) offset[at] = d[0];
+        }
+      }
+  __syncthreads();
+
+  int jt = j0 + mine, n = n0;
+  clear();
+  for (int at = 0; at < all; ++at) {
+    notes[wave * OP_FM * 64 + lane] = note;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const bool end = n + OP_AHEAD >= n1, more = at + 1 < all;
+    const int next_jt = end & more ? jt + stride : jt, next_n = !more ? n : end ? n0 : n + OP_AHEAD;
+    load_note(next_jt, next_n, note);
+    const int down = jt == last_tile ? 16 - p.nj % 16 : 0, group = (n * 128) >> p.group_shift;
+#pragma unroll
+    for (int u = 0; u < OP_AHEAD; u += 2) {        /* (two at a time: a line of memory has two steps of a row) */
+      if (n + u < n1) add(n + u, OP_CHUNKS > 1 ? u * OP_CHUNKS : (((n + u) * 128) >> p.group_shift) - group, down, ring[u]);
+      __builtin_amdgcn_sched_barrier(0);           /* (a step's rows out of LDS when it is their turn: registers) */
+      if (n + u + 1 < n1) add(n + u + 1, OP_CHUNKS > 1 ? (u + 1) * OP_CHUNKS : (((n + u + 1) * 128) >> p.group_shift) - group, down, ring[u + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      load(next_jt, acc_min(next_n + u, n1 - 1), ring[u]);
+      load(next_jt, acc_min(next_n + u + 1, n1 - 1), ring[u + 1]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (end) {
+      /* (waves of the same columns meet twice for each of their tiles) */
+      if (split > 1) {
+#pragma unroll
+        for (int i = 0; i < OP_FM; ++i) ((acc_f4 *)notes)[(wave * OP_FM + i) * 64 + lane] = c[i];
+        __syncthreads();
+        if (wave % split == 0)
+#pragma unroll
+          for (int i = 0; i < OP_FM; ++i)
+            for (int w = 1; w * each < steps; ++w) c[i] += ((const acc_f4 *)notes)[((wave + w) * OP_FM + i) * 64 + lane];
+        __syncthreads();
+      }
+      if (wave % split == 0) write(jt, c);
+      clear();
+    }
+    jt = next_jt;
+    n = next_n;
+  }
+  if (split > 1)
+    for (int t = own; t < turns; ++t) {
+      __syncthreads();
+      __syncthreads();
+    }
+}
+#else
 struct op_step {
   acc_u4 w[OP_FN];
   op_eight x[OP_FM][4];
@@ -218,7 +424,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
 #pragma unroll
     for (int i = 0; i < OP_FM; ++i) x[i] = (const op_elt *)p.x + (long long)acc_max(arow[i], 0) * p.x_stride;
     const int steps = (p.blocks + 3) / 4;
-    const auto load = [&](const int n, op_step &s) {
+    const auto load_as = [&](const bool whole, const int n, op_step &s) {
       const int k = n * 128;
 #pragma unroll
       for (int j = 0; j < OP_FN; ++j) s.w[j] = __builtin_nontemporal_load((const acc_u4 *)(w[j] + acc_min(n * 4 + g, p.blocks - 1) * 16));
@@ -227,41 +433,38 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
         const int at = acc_min((k + q * (128 / OP_CHUNKS)) >> p.group_shift, p.groups - 1);
 #pragma unroll
         for (int j = 0; j < OP_FN; ++j) {
-          s.s[q][j] = op_four(scales + at * p.scales_stride, j0 + j * 16 + g * 4, p.nj);
-          if (p.zeros) s.z[q][j] = op_four(zeros + at * p.zeros_stride, j0 + j * 16 + g * 4, p.nj);
+          s.s[q][j] = op_four(scales + at * p.scales_stride, whole, j0 + j * 16 + g * 4, p.nj);
+          if (OP_ZEROS) s.z[q][j] = op_four(zeros + at * p.zeros_stride, whole, j0 + j * 16 + g * 4, p.nj);
         }
       }
-      if (k + 128 <= p.k) {
 #pragma unroll
-        for (int i = 0; i < OP_FM; ++i)
+      for (int i = 0; i < OP_FM; ++i)
 #pragma unroll
-          for (int b = 0; b < 4; ++b) s.x[i][b] = op_row8(x[i] + k + b * 32 + g * 8, 8);
-      } else {
-#pragma unroll
-        for (int i = 0; i < OP_FM; ++i)
-#pragma unroll
-          for (int b = 0; b < 4; ++b) s.x[i][b] = op_row8(x[i] + k + b * 32 + g * 8, p.k - k - b * 32 - g * 8);
-      }
+        for (int b = 0; b < 4; ++b) s.x[i][b] = op_row8(x[i] + k + OP_FIRST(b, g), whole ? 8 : p.k - k - OP_FIRST(b, g));
+    };
+    const auto load = [&](const int n, op_step &s) {
+      if (n * 128 + 128 <= p.k && j0 + 16 * OP_FN <= p.nj) load_as(true, n, s);
+      else load_as(false, n, s);
     };
     const auto add = [&](op_step &s) {
       const acc_f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-      const op_frag ones = op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES});
+      const op_frag ones = op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), offsets = op_as_frag(op_offsets());
 #pragma unroll
       for (int j = 0; j < OP_FN; ++j) op_turn(s.w[j]);
 #pragma unroll
       for (int q = 0; q < OP_CHUNKS; ++q) {
-        acc_f4 t[OP_FM][OP_FN], sum[OP_FM];
+        acc_f4 t[OP_FM][OP_FN], sum[OP_FM], offset[OP_FM];
 #pragma unroll
         for (int i = 0; i < OP_FM; ++i) {
-          sum[i] = none;
+          sum[i] = offset[i] = none;
 #pragma unroll
           for (int j = 0; j < OP_FN; ++j) t[i][j] = none;
         }
 #pragma unroll
-        for (int b = q * 4 / OP_CHUNKS; b < (q + 1) * 4 / OP_CHUNKS; ++b) {
+        for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
           op_frag v[OP_FN];
 #pragma unroll
-          for (int j = 0; j < OP_FN; ++j) v[j] = op_as_frag(op_sixteens(s.w[j][b]));
+          for (int j = 0; j < OP_FN; ++j) v[j] = op_as_frag(op_numbers(s.w[j][b]));
 #pragma unroll
           for (int i = 0; i < OP_FM; ++i) {
             acc_u4 part[OP_PARTS];
@@ -270,6 +473,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
             for (int n = OP_PARTS - 1; n >= 0; --n) {
               const op_frag y = op_as_frag(part[n]);
               sum[i] = op_mfma(ones, y, sum[i]);
+              if (OP_ELT == 1) offset[i] = op_mfma(offsets, y, offset[i]);
 #pragma unroll
               for (int j = 0; j < OP_FN; ++j) t[i][j] = op_mfma(v[j], y, t[i][j]);
             }
@@ -279,21 +483,22 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
         for (int j = 0; j < OP_FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float scale = (float)s.s[q][j].v[r], off = scale * (16.0f + (p.zeros ? (float)s.z[q][j].v[r] : 8.0f));
+            const float scale = (float)s.s[q][j].v[r], zero = OP_ZEROS ? (float)s.z[q][j].v[r] : 8.0f;
 #pragma unroll
-            for (int i = 0; i < OP_FM; ++i) c[i][j][r] += __builtin_fmaf(scale, t[i][j][r], -off * sum[i][r]);
+            for (int i = 0; i < OP_FM; ++i)
+              c[i][j][r] = __builtin_fmaf(scale, t[i][j][r] + op_begin(sum[i][r], OP_ELT == 1 ? offset[i][r] : (OP_ELT == 2 ? 128.0f : 16.0f) * sum[i][r], zero), c[i][j][r]);
           }
       }
     };
-    for (int n = wave; n < steps; n += OP_WAVES * OP_AHEAD) {
+    for (int n = wave * OP_AHEAD; n < steps; n += OP_WAVES * OP_AHEAD) {
       op_step s[OP_AHEAD];
 #pragma unroll
       for (int u = 0; u < OP_AHEAD; ++u)
-        if (n + u * OP_WAVES < steps) load(n + u * OP_WAVES, s[u]);
+        if (n + u < steps) load(n + u, s[u]);
       __builtin_amdgcn_sched_barrier(0);           /* (all loads first) */
 #pragma unroll
       for (int u = 0; u < OP_AHEAD; ++u)
-        if (n + u * OP_WAVES < steps) add(s[u]);
+        if (n + u < steps) add(s[u]);
     }
   }
 
@@ -317,4 +522,5 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
     for (int j = 0; j < OP_FN; ++j) op_write4(out, j0 + j * 16 + 4 * g, p.nj, c[i][j], arow[i] < 0 || tile.expert < 0);
   }
 }
+#endif
 #endif
