@@ -29,7 +29,7 @@ COMBINE_GENERIC, COMBINE_ADD, COMBINE_MIN, COMBINE_MAX, COMBINE_AND, COMBINE_OR,
 BOUNDARY = {"clamp": 0, "mirror": 1, "wrap": 2, "constant": 3}
 FLAG_FOLD_RIGHT, FLAG_FAST_MATH, FLAG_GUARDED, FLAG_TILED = 1, 2, 4, 8
 OP_PRODUCT, OP_ROUTE, OP_COMBINE, OP_MICRO = range(4)
-OP_RECUR, OP_GROUPED = 5, 6
+OP_RECUR, OP_GROUPED, OP_SCORE = 5, 6, 7
 GATES = {"given": 0, "sigmoid": 1}
 STRIDED_RANK = 4
 
@@ -82,7 +82,8 @@ class acc_skel_desc(C.Structure):
 
 
 class acc_op_desc(C.Structure):
-    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32), ("gate", C.c_int32), ("group", C.c_int32)]
+    _fields_ = [("kind", C.c_int32), ("elt_type", C.c_char_p), ("choose", C.c_int32), ("normalise", C.c_int32), ("gate", C.c_int32), ("groups", C.c_int32), ("keep", C.c_int32),
+                ("scale", C.c_float), ("group", C.c_int32)]
 
 
 # the bytes of an acc_strided, by rank
@@ -130,7 +131,7 @@ acc_memtable_reclaim acc_memtable_get_stats acc_skel_create_async acc_skel_wait 
 acc_tuning_set acc_tuning_text acc_context_set_tuning acc_op_create acc_op_destroy acc_op_compile_only acc_exec_product_rows
 acc_exec_product_outer acc_exec_route acc_exec_route_gradient acc_exec_combine acc_exec_combine_gradient acc_exec_micro_quantise
 acc_exec_micro_values acc_exec_micro_rows acc_exec_recur acc_exec_recur_gradient acc_exec_recur_step
-acc_exec_grouped_quantise acc_exec_grouped_values acc_exec_grouped_rows""".split()
+acc_exec_grouped_quantise acc_exec_grouped_values acc_exec_grouped_rows acc_exec_score acc_exec_score_gradient""".split()
 
 
 def build(force=False):
@@ -655,7 +656,8 @@ class _Drivers(object):
               "acc_exec_micro_quantise": (_P, _P, _P, _P, _P), "acc_exec_micro_values": (_P, _P, _P, _P, _P),
               "acc_exec_micro_rows": (_P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P),
               "acc_exec_recur": (_P,) * 9, "acc_exec_recur_gradient": (_P,) * 12, "acc_exec_recur_step": (_P,) * 8,
-              "acc_exec_grouped_quantise": (_P,) * 6, "acc_exec_grouped_values": (_P,) * 6, "acc_exec_grouped_rows": (_P,) * 7 + (C.c_int32, _P, _P)}
+              "acc_exec_grouped_quantise": (_P,) * 6, "acc_exec_grouped_values": (_P,) * 6, "acc_exec_grouped_rows": (_P,) * 7 + (C.c_int32, _P, _P),
+              "acc_exec_score": (_P,) * 9, "acc_exec_score_gradient": (_P,) * 6}
 
     def __getattr__(self, name):               # (at its first call; an attribute of its own from then on)
         f = C.CFUNCTYPE(C.c_int, *self._TYPES[name])((name, lib()))
@@ -813,11 +815,12 @@ def _layout(a, size=None):
     return _STRIDED[len(a.shape)](len(a.shape), 0, *a.shape, *a.strides, a.ptr)
 
 
-def op_desc(kind, elt, choose=0, normalise=True, gate="given", group=0):
+def op_desc(kind, elt, choose=0, normalise=True, gate="given", group=0, groups=1, keep=1, scale=1.0):
     if gate not in GATES:
         raise AccError(ERR_INVALID, "gates are %s, not %r" % (" or ".join(sorted(GATES)), gate))
     d = acc_op_desc()
     d.kind, d.elt_type, d.choose, d.normalise, d.gate, d.group = kind, _b(elt), choose, int(normalise), GATES[gate], group
+    d.groups, d.keep, d.scale = groups, keep, scale
     return d
 
 
@@ -877,6 +880,26 @@ class Router(_Operator):
 
     def gradient(self, logits, experts, weights, dweights, dlogits, stream=None):
         rc = _drivers.acc_exec_route_gradient(self.handle, _layout(logits, self.size), _layout(experts, 4), _layout(weights, 4), _layout(dweights, 4), _layout(dlogits, self.size), stream)
+        if rc:
+            check(rc)
+
+
+class ScoreRouter(_Operator):
+    """A Router that scores experts by themselves, 1 / (1 + exp(-logit)), and chooses by score + bias the `choose` best of the `keep` best of
+    `groups` groups of experts; the weights are `scale` times the scores, or their shares of the chosen ones' sum."""
+    KIND = OP_SCORE
+
+    def __init__(self, ctx, elt, choose, groups=1, keep=1, normalise=True, scale=1.0):
+        _Operator.__init__(self, ctx, elt, choose, normalise, groups=groups, keep=keep, scale=scale)
+
+    def route(self, logits, experts, weights, offsets, order, place, bias=None, stream=None):
+        rc = _drivers.acc_exec_score(self.handle, _layout(logits, self.size), _layout(bias, 4), _layout(experts, 4), _layout(weights, 4), _layout(offsets, 4), _layout(order, 4), _layout(place, 4),
+                                     stream)
+        if rc:
+            check(rc)
+
+    def gradient(self, logits, experts, dweights, dlogits, stream=None):
+        rc = _drivers.acc_exec_score_gradient(self.handle, _layout(logits, self.size), _layout(experts, 4), _layout(dweights, 4), _layout(dlogits, self.size), stream)
         if rc:
             check(rc)
 

@@ -36,7 +36,9 @@ ACC_EMBED(op_common, "operators/op_common.h")
 ACC_EMBED(op_matrix, "operators/op_matrix.h")
 ACC_EMBED(op_product, "operators/op_product.h")
 ACC_EMBED(op_skinny, "operators/op_skinny.h")
+ACC_EMBED(op_place, "operators/op_place.h")
 ACC_EMBED(op_route, "operators/op_route.h")
+ACC_EMBED(op_score, "operators/op_score.h")
 ACC_EMBED(op_combine, "operators/op_combine.h")
 ACC_EMBED(op_pack, "operators/op_pack.h")
 ACC_EMBED(op_micro, "operators/op_micro.h")
@@ -67,7 +69,9 @@ const std::vector<EmbeddedHeader> &embedded_headers()
       {"op_matrix.h", acc_embed_op_matrix_begin, acc_embed_op_matrix_end},
       {"op_skinny.h", acc_embed_op_skinny_begin, acc_embed_op_skinny_end},
       {"op_product.h", acc_embed_op_product_begin, acc_embed_op_product_end},
+      {"op_place.h", acc_embed_op_place_begin, acc_embed_op_place_end},
       {"op_route.h", acc_embed_op_route_begin, acc_embed_op_route_end},
+      {"op_score.h", acc_embed_op_score_begin, acc_embed_op_score_end},
       {"op_combine.h", acc_embed_op_combine_begin, acc_embed_op_combine_end},
       {"op_pack.h", acc_embed_op_pack_begin, acc_embed_op_pack_end},
       {"op_micro.h", acc_embed_op_micro_begin, acc_embed_op_micro_end},

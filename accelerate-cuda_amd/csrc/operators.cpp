@@ -36,12 +36,14 @@ struct OpSpec {
   bool normalise = true;
   int gate = 0;
   int group = 0;
+  int groups = 1, keep = 1;
+  float scale = 1.0f;
   int tile = -1;                // knob product.tile: the products' tile shape, for measurement
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-const char *const kKindName[] = {"product", "route", "combine", "micro", "", "recur", "grouped"};
+const char *const kKindName[] = {"product", "route", "combine", "micro", "", "recur", "grouped", "score"};
 int type_bytes(int type) { return type == 0 ? 4 : 2; }
 
 // ---- the variants of each kind ------------------------------------------------------
@@ -166,6 +168,42 @@ std::string micro_source(const OpSpec &sp, bool aligned)
   return text;
 }
 
+// score: how a token's logits are shared out
+struct ScoreVariant {
+  int lanes = 4, per = 64;
+  bool few = false;             // one workgroup, which places the slots, too
+  int threads() const { return few ? kRouteFewThreads : kRouteThreads; }
+  uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (few ? 1u << 16 : 0u); }
+};
+constexpr int kScoreThreads = 256;
+// logits of a lane: whole groups, or a part of one
+int64_t score_slice(const OpSpec &sp, int64_t experts, int lanes)
+{
+  const int64_t size = experts / sp.groups;
+  return sp.groups >= lanes ? sp.groups / lanes * size : ceil_div(size, lanes / sp.groups);
+}
+std::string score_source(const OpSpec &sp, const ScoreVariant &v)
+{
+  int row = 8;
+  while (row < sp.choose) row *= 2;
+  char text[512];
+  std::snprintf(text, sizeof(text),
+                "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_CHOOSE %d\n#define OP_ROW %d\n#define OP_FEW %d\n#define OP_THREADS %d\n"
+                "#include \"acc_hip_device.h\"\n#include \"op_score.h\"\n",
+                sp.type, v.lanes, v.per, sp.choose, std::max(row, 32), v.few ? 1 : 0, v.threads());
+  return text;
+}
+ScoreVariant score_variant(const OpSpec &sp, int64_t experts, int64_t tokens)
+{
+  ScoreVariant v;
+  v.few = tokens * experts <= kRouteAlone;
+  // (four lanes a token where that makes two waves a SIMD and a lane has 64 logits at most)
+  while (v.lanes < 64 && (score_slice(sp, experts, v.lanes) > 64 || (tokens * v.lanes < 64 * 2048 && score_slice(sp, experts, v.lanes) > 8))) v.lanes *= 4;
+  v.per = 8;
+  while (v.per < score_slice(sp, experts, v.lanes)) v.per *= 2;
+  return v;
+}
+
 // recur: a workgroup's tile is eight waves' rows of 64 words of channels.  Rows of a wave, which are held in registers: the
 // gradient has twice as many arrays
 struct RecurVariant {
@@ -278,6 +316,16 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         for (int64_t tokens : {int64_t(0), int64_t(1), int64_t(1) << 20}) out.push_back(route_source(sp, route_variant(sp, experts, aligned, tokens)));
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
+  } else if (sp.kind == ACC_OP_SCORE) {
+    for (int lanes : {4, 16, 64})
+      for (int per : {8, 16, 32, 64})
+        for (bool few : {true, false}) {
+          ScoreVariant v;
+          v.lanes = lanes;
+          v.per = per;
+          v.few = few;
+          if (per <= 32 || lanes < 64) out.push_back(score_source(sp, v));
+        }
   } else if (sp.kind == ACC_OP_GROUPED) {
     for (int bm : {16, 32, 64})
       for (int form = 0; form < 12; ++form) {
@@ -346,6 +394,15 @@ int make_spec(const acc_op_desc *d, OpSpec *sp)
   sp->kind = d->kind;
   sp->choose = d->choose;
   sp->normalise = d->normalise != 0;
+  if (d->kind == ACC_OP_SCORE) {
+    if (d->choose < 1 || d->choose > 32) return fail(ACC_ERR_INVALID, "acc_op_create: a router by scores chooses 1 to 32 experts, not %d", d->choose);
+    if (d->groups < 1 || d->groups > 64 || (d->groups & (d->groups - 1)) != 0) return fail(ACC_ERR_INVALID, "acc_op_create: %d groups (a power of two up to 64)", d->groups);
+    if (d->keep < 1 || d->keep > d->groups) return fail(ACC_ERR_INVALID, "acc_op_create: %d of %d groups are kept", d->keep, d->groups);
+    if (!(d->scale - d->scale == 0.0f)) return fail(ACC_ERR_INVALID, "acc_op_create: a scale that is not finite");
+    sp->groups = d->groups;
+    sp->keep = d->keep;
+    sp->scale = d->scale;
+  }
   if (d->kind == ACC_OP_GROUPED) {
     if (d->group < 32 || (d->group & (d->group - 1)) != 0) return fail(ACC_ERR_INVALID, "acc_op_create: a group of %d neighbours (a power of two, 32 or more)", d->group);
     sp->group = d->group;
@@ -687,6 +744,16 @@ std::string grouped_source_of(const OpSpec &sp, uint32_t key)
   return grouped_source(sp, v);
 }
 
+std::string score_source_of(const OpSpec &sp, uint32_t key)
+{
+  ScoreVariant v;
+  v.lanes = (int)(key & 127u);
+  v.per = (int)(key >> 8 & 127u);
+  v.few = key >> 16 & 1u;
+  return score_source(sp, v);
+}
+
+const char *const kScoreNames[] = {"score", "route_place", "score_gradient"};
 const char *const kGroupedNames[] = {"grouped"};
 const char *const kGroupedElementNames[] = {"grouped_quantise", "grouped_values"};
 const char *const kRecurNames[] = {"recur", "recur_clear"};
@@ -1084,12 +1151,10 @@ try {
 
 static size_t route_lds(const RouteVariant &v, int64_t experts, int64_t slots) { return ((size_t)(v.threads() / 64 + 2) * (size_t)experts + (size_t)slots) * 4; }
 
-int acc_exec_route(acc_op op, const acc_strided *logits, const acc_strided *chosen, const acc_strided *weights, const acc_strided *offsets,
-                   const acc_strided *order, const acc_strided *place, acc_stream stream)
-try {
-  const char *who = "acc_exec_route";
-  acc_route_args a = {};
-  ACC_TRY(begin(op, ACC_OP_ROUTE, who, stream, &a.guard));
+// what a router is given, and where its results go
+static int check_routing(acc_op op, const char *who, const acc_strided *logits, const acc_strided *chosen, const acc_strided *weights, const acc_strided *offsets,
+                         const acc_strided *order, const acc_strided *place)
+{
   ACC_TRY(check_unit(who, "logits", logits, 2));
   ACC_TRY(check_result(who, "experts", chosen, 2));
   ACC_TRY(check_result(who, "weights", weights, 2));
@@ -1112,6 +1177,18 @@ try {
     ACC_TRY(check_apart(who, all[k], {{logits, bytes, "logits"}}));
     for (int m = 0; m < k; ++m) ACC_TRY(check_apart(who, all[k], {all[m]}));
   }
+  return ACC_OK;
+}
+
+int acc_exec_route(acc_op op, const acc_strided *logits, const acc_strided *chosen, const acc_strided *weights, const acc_strided *offsets,
+                   const acc_strided *order, const acc_strided *place, acc_stream stream)
+try {
+  const char *who = "acc_exec_route";
+  acc_route_args a = {};
+  ACC_TRY(begin(op, ACC_OP_ROUTE, who, stream, &a.guard));
+  ACC_TRY(check_routing(op, who, logits, chosen, weights, offsets, order, place));
+  const int64_t tokens = logits->shape[0], experts = logits->shape[1], choose = op->spec.choose;
+  const int bytes = type_bytes(op->spec.type);
   const RouteVariant v = route_variant(op->spec, (int)experts, aligned_rows(*logits, bytes, 1), tokens);
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kRouteNames, 3, route_source_of, &var));
@@ -1190,6 +1267,109 @@ try {
   }
   return ACC_OK;
 } ACC_OP_CATCH("acc_exec_route_gradient")
+
+// ---- router by scores -------------------------------------------------------------------
+
+static int check_score_experts(acc_op op, const char *who, int64_t experts)
+{
+  const OpSpec &sp = op->spec;
+  if (experts > kRouteMaxExperts || experts % sp.groups != 0 || experts / sp.groups * sp.keep < sp.choose)
+    return fail(ACC_ERR_INVALID, "%s: %lld experts (a multiple of %d, at most %d; %d are chosen of those of %d groups)", who, (long long)experts, sp.groups, kRouteMaxExperts, sp.choose, sp.keep);
+  return ACC_OK;
+}
+
+int acc_exec_score(acc_op op, const acc_strided *logits, const acc_strided *bias, const acc_strided *chosen, const acc_strided *weights,
+                   const acc_strided *offsets, const acc_strided *order, const acc_strided *place, acc_stream stream)
+try {
+  const char *who = "acc_exec_score";
+  acc_route_args a = {};
+  ACC_TRY(begin(op, ACC_OP_SCORE, who, stream, &a.guard));
+  ACC_TRY(check_routing(op, who, logits, chosen, weights, offsets, order, place));
+  const int64_t tokens = logits->shape[0], experts = logits->shape[1], choose = op->spec.choose;
+  ACC_TRY(check_score_experts(op, who, experts));
+  if (bias) {
+    ACC_TRY(check_unit(who, "bias", bias, 1));
+    ACC_TRY(check_shape(who, "bias", *bias, {experts}));
+    for (const Named &n : {Named{chosen, 4, "experts"}, Named{weights, 4, "weights"}, Named{offsets, 4, "offsets"}, Named{order, 4, "order"}, Named{place, 4, "place"}})
+      ACC_TRY(check_apart(who, n, {{bias, 4, "bias"}}));
+  }
+  const ScoreVariant v = score_variant(op->spec, experts, tokens);
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kScoreNames, 3, score_source_of, &var));
+  a.logits = device<const void>(logits);
+  a.bias = device<const float>(bias);
+  a.chosen = device<int32_t>(chosen);
+  a.weights = device<float>(weights);
+  a.offsets = device<int32_t>(offsets);
+  a.order = device<int32_t>(order);
+  a.place = device<int32_t>(place);
+  a.tokens = tokens;
+  a.logits_stride = logits->stride[0];
+  a.experts = (int32_t)experts;
+  a.choose = (int32_t)choose;
+  a.normalise = op->spec.normalise ? 1 : 0;
+  a.groups = op->spec.groups;
+  a.keep = op->spec.keep;
+  a.scale = op->spec.scale;
+  // (as the other router's: a single workgroup, or up to 256 of which each reads the counts of all)
+  const int64_t at_once = kScoreThreads / v.lanes;
+  a.block = v.few ? (int)std::max<int64_t>(1, tokens) : (int)std::max<int64_t>(at_once, ceil_div(ceil_div(tokens, 256), at_once) * at_once);
+  a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, a.block));
+  const size_t groups = (size_t)at_once * (size_t)op->spec.groups * 4;
+  if (v.few) return launch(op, who, var->fn, 1, kScoreThreads, (size_t)(6 * experts + tokens * choose) * 4 + groups, stream, a);
+  ScratchHold counts;
+  ACC_TRY(counts.acquire(op, stream, (size_t)a.blocks * (size_t)experts * 4));
+  a.counts = static_cast<uint32_t *>(counts.ref.ptr);
+  ACC_TRY(launch(op, who, var->fn, a.blocks, kScoreThreads, (size_t)experts * 4 + groups, stream, a));
+  return launch(op, who, var->fn2, a.blocks, kRouteThreads, ((size_t)(kRouteThreads / 64 + 2) * (size_t)experts) * 4, stream, a);
+} ACC_OP_CATCH("acc_exec_score")
+
+int acc_exec_score_gradient(acc_op op, const acc_strided *logits, const acc_strided *chosen, const acc_strided *dweights, const acc_strided *dlogits, acc_stream stream)
+try {
+  const char *who = "acc_exec_score_gradient";
+  acc_route_args a = {};
+  ACC_TRY(begin(op, ACC_OP_SCORE, who, stream, &a.guard));
+  ACC_TRY(check_unit(who, "logits", logits, 2));
+  ACC_TRY(check_unit(who, "experts", chosen, 2));
+  ACC_TRY(check_unit(who, "dweights", dweights, 2));
+  ACC_TRY(check_result(who, "dlogits", dlogits, 2));
+  const int64_t tokens = logits->shape[0], experts = logits->shape[1], choose = op->spec.choose;
+  ACC_TRY(check_score_experts(op, who, experts));
+  ACC_TRY(check_shape(who, "experts", *chosen, {tokens, choose}));
+  ACC_TRY(check_shape(who, "dweights", *dweights, {tokens, choose}));
+  ACC_TRY(check_shape(who, "dlogits", *dlogits, {tokens, experts}));
+  for (const acc_strided *t : {chosen, dweights})
+    if (tokens > 1 && t->stride[0] != choose) return fail(ACC_ERR_INVALID, "%s: experts and dweights are dense arrays", who);
+  const int bytes = type_bytes(op->spec.type);
+  ACC_TRY(check_apart(who, {dlogits, bytes, "dlogits"}, {{logits, bytes, "logits"}, {chosen, 4, "experts"}, {dweights, 4, "dweights"}}));
+  if (tokens == 0) return ACC_OK;
+  ScoreVariant v;                                  // (any: the gradient is the same in all)
+  v.lanes = 4;
+  v.per = 8;
+  const OpVariant *var = nullptr;
+  ACC_TRY(op->variant(v.key(), kScoreNames, 3, score_source_of, &var));
+  a.logits = device<const void>(logits);
+  a.chosen = device<int32_t>(chosen);
+  a.dweights = device<const float>(dweights);
+  a.dlogits = device<void>(dlogits);
+  a.logits_stride = logits->stride[0];
+  a.dlogits_stride = dlogits->stride[0];
+  a.experts = (int32_t)experts;
+  a.choose = (int32_t)choose;
+  a.normalise = op->spec.normalise ? 1 : 0;
+  a.scale = op->spec.scale;
+  const int64_t each = 256 / 32, most = kThreads / 256 * each;      // (tokens of a workgroup: 32 lanes each)
+  for (int64_t first = 0; first < tokens; first += most) {
+    acc_route_args part = a;
+    part.tokens = std::min(most, tokens - first);
+    part.logits = static_cast<const char *>(a.logits) + first * a.logits_stride * bytes;
+    part.dlogits = static_cast<char *>(a.dlogits) + first * a.dlogits_stride * bytes;
+    part.chosen = a.chosen + first * choose;
+    part.dweights = a.dweights + first * choose;
+    ACC_TRY(launch(op, who, var->fn3, ceil_div(part.tokens, each), 256, 0, stream, part));
+  }
+  return ACC_OK;
+} ACC_OP_CATCH("acc_exec_score_gradient")
 
 // ---- combination ----------------------------------------------------------------------
 

@@ -60,6 +60,9 @@ struct acc_route_args {
   int32_t normalise, blocks;
   int32_t block, pad;           /* tokens of a workgroup */
   const uint32_t *guard;
+  const float *bias;            /* op_score.h: beside the scores, for the choice alone; 0: none */
+  int32_t groups, keep;
+  float scale;
 };
 
 /* the combination: see op_combine.h */

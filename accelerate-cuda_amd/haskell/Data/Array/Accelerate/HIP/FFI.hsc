@@ -453,13 +453,14 @@ foreign import ccall safe   "acc_memtable_reclaim"          c_memtableReclaim   
 foreign import ccall safe   "acc_memtable_get_stats"        c_memtableGetStats        :: MemTable -> Ptr MemTableStats -> IO Status
 
 -- Operators on segments of rows: products, routing, combination, 4-bit numbers.  An array of theirs has strides.
-accOpProduct, accOpRoute, accOpCombine, accOpMicro, accOpRecur, accOpGrouped :: CInt
+accOpProduct, accOpRoute, accOpCombine, accOpMicro, accOpRecur, accOpGrouped, accOpScore :: CInt
 accOpProduct = #{const ACC_OP_PRODUCT}
 accOpRoute   = #{const ACC_OP_ROUTE}
 accOpCombine = #{const ACC_OP_COMBINE}
 accOpMicro   = #{const ACC_OP_MICRO}
 accOpRecur   = #{const ACC_OP_RECUR}
 accOpGrouped = #{const ACC_OP_GROUPED}
+accOpScore   = #{const ACC_OP_SCORE}
 
 accGateGiven, accGateSigmoid :: Int32
 accGateGiven   = #{const ACC_GATE_GIVEN}
@@ -493,6 +494,9 @@ data OpDesc = OpDesc
   , opChoose    :: Int32
   , opNormalise :: Bool
   , opGate      :: Int32              -- a recurrence's: accGate*
+  , opGroups    :: Int32              -- of a router by scores: groups of experts, those that are kept, and of the weights
+  , opKeep      :: Int32
+  , opScale     :: CFloat
   , opGroup     :: Int32              -- of grouped 4-bit numbers: neighbours under a scale
   }
 
@@ -506,14 +510,20 @@ instance Storable OpDesc where
     n <- #{peek acc_op_desc, normalise} p :: IO Int32
     g <- #{peek acc_op_desc, gate} p
     w <- #{peek acc_op_desc, group} p
-    return (OpDesc (fromIntegral k) t c (n /= 0) g w)
-  poke p (OpDesc k t c n g w) = do
+    gs <- #{peek acc_op_desc, groups} p
+    ks <- #{peek acc_op_desc, keep} p
+    sc <- #{peek acc_op_desc, scale} p
+    return (OpDesc (fromIntegral k) t c (n /= 0) g gs ks sc w)
+  poke p (OpDesc k t c n g gs ks sc w) = do
     fillBytes p 0 #{size acc_op_desc}
     #{poke acc_op_desc, kind} p (fromIntegral k :: Int32)
     #{poke acc_op_desc, elt_type} p t
     #{poke acc_op_desc, choose} p c
     #{poke acc_op_desc, normalise} p (if n then 1 else 0 :: Int32)
     #{poke acc_op_desc, gate} p g
+    #{poke acc_op_desc, groups} p gs
+    #{poke acc_op_desc, keep} p ks
+    #{poke acc_op_desc, scale} p sc
     #{poke acc_op_desc, group} p w
 
 foreign import ccall safe   "acc_op_create"             c_opCreate            :: Context -> Ptr OpDesc -> Ptr Op -> IO Status
@@ -528,6 +538,8 @@ foreign import ccall safe   "acc_exec_combine_gradient" c_execCombineGradient ::
 foreign import ccall safe   "acc_exec_micro_quantise"   c_execMicroQuantise   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_micro_values"     c_execMicroValues     :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_micro_rows"       c_execMicroRows       :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_score"            c_execScore           :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
+foreign import ccall safe   "acc_exec_score_gradient"   c_execScoreGradient   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_grouped_quantise" c_execGroupedQuantise :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_grouped_values"   c_execGroupedValues   :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Stream -> IO Status
 foreign import ccall safe   "acc_exec_grouped_rows"     c_execGroupedRows     :: Op -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Ptr Strided -> Int32 -> Ptr Strided -> Stream -> IO Status

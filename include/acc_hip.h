@@ -678,7 +678,8 @@ enum {
   ACC_OP_MICRO   = 3,
   ACC_OP_RECUR   = 5,        /* (4 is no kind)                                    */
   ACC_OP_GROUPED = 6,
-  ACC_OP_KIND_COUNT = 7
+  ACC_OP_SCORE   = 7,
+  ACC_OP_KIND_COUNT = 8
 };
 
 /* what a recurrence's gates are */
@@ -690,9 +691,11 @@ enum {
 typedef struct acc_op_desc {
   int32_t     kind;          /* ACC_OP_*                                          */
   const char *elt_type;      /* "float", "half" or "bfloat16"                     */
-  int32_t     choose;        /* ACC_OP_ROUTE: experts a token, 1 to 64            */
-  int32_t     normalise;     /* ACC_OP_ROUTE: softmax over the chosen (else over all experts) */
+  int32_t     choose;        /* ACC_OP_ROUTE: experts a token, 1 to 64; ACC_OP_SCORE: 1 to 32 */
+  int32_t     normalise;     /* ACC_OP_ROUTE: softmax over the chosen (else over all experts); ACC_OP_SCORE: scores over their sum */
   int32_t     gate;          /* ACC_OP_RECUR: ACC_GATE_*                          */
+  int32_t     groups, keep;  /* ACC_OP_SCORE: groups of neighbouring experts (a power of two up to 64), and how many are chosen from */
+  float       scale;         /* ACC_OP_SCORE: of the weights                      */
   int32_t     group;         /* ACC_OP_GROUPED: neighbours under a scale, a power of two of 32 or more */
 } acc_op_desc;
 
@@ -729,6 +732,20 @@ int acc_exec_route(acc_op op, const acc_strided *logits, const acc_strided *expe
 /* dlogits from the gradient of the weights, both as acc_exec_route made them */
 int acc_exec_route_gradient(acc_op op, const acc_strided *logits, const acc_strided *experts, const acc_strided *weights,
                             const acc_strided *dweights, const acc_strided *dlogits, acc_stream stream);
+
+/* acc_exec_route with scores of the experts by themselves, s = 1 / (1 + e^-logit), and choices by s + bias (bias [experts] Float32, or
+ * NULL: none; it is no part of the weights).  The experts are `groups` groups of neighbours, as many in each; the `keep` groups with the
+ * largest sum of their two best are chosen from (of equal ones the lowest first), then the `choose` largest, largest first, of equal
+ * ones the lowest index first.  weights: scale s, or scale s / sum of the chosen s (0 where that is 0).  Minus infinity as a logit
+ * or a bias, and what is not a number, is never chosen; a group without an expert to choose is never kept.  What is compared are
+ * scores in 64 bits.  Everything else is as for acc_exec_route; the operator chooses at most 32 experts, and no more than are in
+ * the groups that it keeps.                                                                                   */
+int acc_exec_score(acc_op op, const acc_strided *logits, const acc_strided *bias, const acc_strided *experts, const acc_strided *weights,
+                   const acc_strided *offsets, const acc_strided *order, const acc_strided *place, acc_stream stream);
+/* dlogits from the gradient of the weights; experts as acc_exec_score gave them.  The choice itself, and with it the bias, has no
+ * gradient. */
+int acc_exec_score_gradient(acc_op op, const acc_strided *logits, const acc_strided *experts, const acc_strided *dweights,
+                            const acc_strided *dlogits, acc_stream stream);
 
 /* out[t] = sum_j weights[t, j] y[place[t, j]], slots in order; a place that names no row of y adds nothing.  weights
  * NULL: all 1 (the gradient of rows that were taken by `index`).  place, weights [tokens, choose], dense.             */
