@@ -172,33 +172,29 @@ std::string micro_source(const OpSpec &sp, bool aligned)
 struct ScoreVariant {
   int lanes = 4, per = 64;
   bool few = false;             // one workgroup, which places the slots, too
-  int threads() const { return few ? kRouteFewThreads : kRouteThreads; }
+  int threads() const { return few ? kRouteFewThreads : 512; }
+  int place_threads() const { return few ? kRouteFewThreads : kRouteThreads; }
   uint32_t key() const { return (uint32_t)lanes | (uint32_t)per << 8 | (few ? 1u << 16 : 0u); }
 };
-constexpr int kScoreThreads = 256;
-// logits of a lane: whole groups, or a part of one
-int64_t score_slice(const OpSpec &sp, int64_t experts, int lanes)
-{
-  const int64_t size = experts / sp.groups;
-  return sp.groups >= lanes ? sp.groups / lanes * size : ceil_div(size, lanes / sp.groups);
-}
+constexpr int kScoreSlice = 32;
+// logits of a lane: a group, or a part of one
+int64_t score_slice(const OpSpec &sp, int64_t experts, int lanes) { return ceil_div(experts / sp.groups, lanes / sp.groups); }
 std::string score_source(const OpSpec &sp, const ScoreVariant &v)
 {
-  int row = 8;
-  while (row < sp.choose) row *= 2;
   char text[512];
   std::snprintf(text, sizeof(text),
                 "#define OP_ELT %d\n#define OP_LANES %d\n#define OP_PER %d\n#define OP_CHOOSE %d\n#define OP_ROW %d\n#define OP_FEW %d\n#define OP_THREADS %d\n"
                 "#include \"acc_hip_device.h\"\n#include \"op_score.h\"\n",
-                sp.type, v.lanes, v.per, sp.choose, std::max(row, 32), v.few ? 1 : 0, v.threads());
+                sp.type, v.lanes, v.per, sp.choose, 32, v.few ? 1 : 0, v.place_threads());
   return text;
 }
 ScoreVariant score_variant(const OpSpec &sp, int64_t experts, int64_t tokens)
 {
   ScoreVariant v;
   v.few = tokens * experts <= kRouteAlone;
-  // (four lanes a token where that makes two waves a SIMD and a lane has 64 logits at most)
-  while (v.lanes < 64 && (score_slice(sp, experts, v.lanes) > 64 || (tokens * v.lanes < 64 * 2048 && score_slice(sp, experts, v.lanes) > 8))) v.lanes *= 4;
+  v.lanes = std::max(v.lanes, sp.groups);
+  // (32 logits a lane where that makes four waves a SIMD, fewer otherwise: what counts is how soon a token is done)
+  while (v.lanes < 64 && (score_slice(sp, experts, v.lanes) > kScoreSlice || (tokens * v.lanes < 64 * 4096 && score_slice(sp, experts, v.lanes) > 8))) v.lanes *= 2;
   v.per = 8;
   while (v.per < score_slice(sp, experts, v.lanes)) v.per *= 2;
   return v;
@@ -317,14 +313,15 @@ std::vector<std::string> all_sources(const OpSpec &sp)
   } else if (sp.kind == ACC_OP_COMBINE) {
     for (int rows : {0, 1, 2}) out.push_back(combine_source(sp, rows));
   } else if (sp.kind == ACC_OP_SCORE) {
-    for (int lanes : {4, 16, 64})
+    for (int lanes : {4, 8, 16, 32, 64})
       for (int per : {8, 16, 32, 64})
         for (bool few : {true, false}) {
+          if (per > kScoreSlice) continue;
           ScoreVariant v;
           v.lanes = lanes;
           v.per = per;
           v.few = few;
-          if (per <= 32 || lanes < 64) out.push_back(score_source(sp, v));
+          if ((per <= 32 || lanes < 64) && lanes >= sp.groups) out.push_back(score_source(sp, v));
         }
   } else if (sp.kind == ACC_OP_GROUPED) {
     for (int bm : {16, 32, 64})
@@ -1312,15 +1309,15 @@ try {
   a.keep = op->spec.keep;
   a.scale = op->spec.scale;
   // (as the other router's: a single workgroup, or up to 256 of which each reads the counts of all)
-  const int64_t at_once = kScoreThreads / v.lanes;
+  const int64_t at_once = v.threads() / v.lanes;
   a.block = v.few ? (int)std::max<int64_t>(1, tokens) : (int)std::max<int64_t>(at_once, ceil_div(ceil_div(tokens, 256), at_once) * at_once);
   a.blocks = (int32_t)std::max<int64_t>(1, ceil_div(tokens, a.block));
-  const size_t groups = (size_t)at_once * (size_t)op->spec.groups * 4;
-  if (v.few) return launch(op, who, var->fn, 1, kScoreThreads, (size_t)(6 * experts + tokens * choose) * 4 + groups, stream, a);
+  const size_t groups = (size_t)at_once * (size_t)op->spec.groups * 8;
+  if (v.few) return launch(op, who, var->fn, 1, v.threads(), (size_t)(6 * experts + tokens * choose) * 4 + groups, stream, a);
   ScratchHold counts;
   ACC_TRY(counts.acquire(op, stream, (size_t)a.blocks * (size_t)experts * 4));
   a.counts = static_cast<uint32_t *>(counts.ref.ptr);
-  ACC_TRY(launch(op, who, var->fn, a.blocks, kScoreThreads, (size_t)experts * 4 + groups, stream, a));
+  ACC_TRY(launch(op, who, var->fn, a.blocks, v.threads(), (size_t)experts * 4 + groups, stream, a));
   return launch(op, who, var->fn2, a.blocks, kRouteThreads, ((size_t)(kRouteThreads / 64 + 2) * (size_t)experts) * 4, stream, a);
 } ACC_OP_CATCH("acc_exec_score")
 
@@ -1344,7 +1341,7 @@ try {
   ACC_TRY(check_apart(who, {dlogits, bytes, "dlogits"}, {{logits, bytes, "logits"}, {chosen, 4, "experts"}, {dweights, 4, "dweights"}}));
   if (tokens == 0) return ACC_OK;
   ScoreVariant v;                                  // (any: the gradient is the same in all)
-  v.lanes = 4;
+  v.lanes = 64;
   v.per = 8;
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kScoreNames, 3, score_source_of, &var));

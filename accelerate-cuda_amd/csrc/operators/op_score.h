@@ -2,14 +2,17 @@
  * op_score.h -- a router that scores experts one by one, s = 1 / (1 + e^-x), and chooses by s + bias: the best `keep` groups of
  * neighbouring experts, by the sum of their two best, then the best OP_CHOOSE experts of those; weights are the chosen scores alone.
  *
- * A token has OP_LANES neighbouring lanes, each with up to OP_PER neighbouring logits in registers: whole groups, or an even part of
- * one.  What is ranked is Float32 in the high bits of a 64-bit number that compares as one, with the index turned round in the low
+ * A token has OP_LANES neighbouring lanes, each with up to OP_PER neighbouring logits in registers, a group or an even part of one.  What is ranked is Float32 in the high bits of a 64-bit number that compares as one, with the index turned round in the low
  * bits, so that of equal ones the lowest index is the largest.  A lane puts its numbers where they belong among its best, two
  * instructions a place, and the token's lanes then exchange what they have.
  *
  * Scores of 64 bits decide.  Float32 ones are off by 2.3 10^-7 at most, and what lies closer than several times that (and is not the
- * same logit and bias, which is a tie wherever it is computed) is decided again in 64 bits, a wave for a token: one token in some
- * hundreds.
+ * same logit and bias, which is a tie wherever it is computed) is decided again in 64 bits, a wave for a token, when the others are
+ * done: of normal logits, 256 experts and eight groups one token in some thousands.
+ *
+ * Bound by no one thing of the card's: 32768 tokens of 256 bfloat16 logits, eight chosen of four of eight groups, take 45 us, of which
+ * the placing is 10 and the instructions of the choice some 12; memory is 4.  A wave's steps wait for one another (with four waves a
+ * workgroup 55, with sixteen, which have 128 registers each, 59).
  */
 #include "op_common.h"
 
@@ -18,7 +21,7 @@
 #include "op_place.h"
 
 #define OP_NONE (-__builtin_inff())
-#define OP_SELECT_WAVES 4
+#define OP_SELECT_WAVES (OP_FEW ? 4 : 8)           /* (sixteen have too few registers each) */
 #define OP_KEYS (OP_CHOOSE + 1)                    /* one more, to see how near it is */
 
 /* (without the instructions that make quiet what is not a number: there is nothing of the kind among these) */
@@ -89,9 +92,11 @@ ACC_DEV int op_index_of(const double key)
   const int low = (int)(b & 2047ull);
   return key > (double)OP_NONE ? (key < 0.0 ? low : 2047 - low) : -1;
 }
-/* how near two ranked numbers, or two groups, may be to be told apart: some three times what they may be off */
-ACC_DEV float op_near(const float v) { return 1.5e-6f + 3e-7f * __builtin_fabsf(v); }
-ACC_DEV float op_near_groups(const float v) { return 3e-6f + 6e-7f * __builtin_fabsf(v); }
+/* How near two ranked numbers may be to be told apart.  A score is off by a unit of the reciprocal, half a one of its sum, a quarter of
+ * one of the exponential and a part of the product's in front of it, 2.3 10^-7 together, and what is ranked by half a unit more: two
+ * by twice that.  And what a group's sum may be off itself. */
+ACC_DEV float op_near(const float v) { return 6e-7f + 1.6e-7f * __builtin_fabsf(v); }
+ACC_DEV float op_off(const float best, const float next) { return 6e-7f + 1.6e-7f * (__builtin_fabsf(best) + (next > OP_NONE ? __builtin_fabsf(next) : 0.0f)); }
 
 ACC_DEV void op_insert(double (&k)[OP_KEYS], const double y)
 {
@@ -116,57 +121,62 @@ ACC_DEV float op_bias(const acc_route_args &p, const int e) { return p.bias ? p.
  * their proportions; scores that are zero in 64 bits are zero */
 ACC_DEV float op_part(const float x, const float shift) { return x < -745.0f ? 0.0f : x < 0.0f ? expf(x - shift) / (1.0f + expf(x)) : 1.0f / (1.0f + expf(-x)); }
 
-/* token t again, in 64 bits: lane j has the j-th choice */
+/* Token t again, in 64 bits: lane j has the j-th choice.  A lane has every 64th expert. */
+#define OP_AGAIN (OP_LANES * OP_PER > 64 ? OP_LANES * OP_PER / 64 : 1)
 ACC_DEV int op_again(const acc_route_args &p, const long long t, const int lane)
 {
   const int size = p.experts / p.groups;
-  unsigned long long kept = ~0ull;
-  const auto largest = [](double a, double b) { return a > b ? a : b; };
+  const auto largest = [](double a, double b) { return op_most(a, b); };
+  double v[OP_AGAIN];
+#pragma unroll
+  for (int i = 0; i < OP_AGAIN; ++i) {
+    const int e = acc_min(i * 64 + lane, p.experts - 1);
+    v[i] = op_ranked64(op_logit(p, t, e), op_bias(p, e));
+    if (i * 64 + lane >= p.experts) v[i] = (double)OP_NONE;
+  }
   if (p.keep < p.groups) {
     double mine = (double)OP_NONE;                 /* lane g: group g's */
     for (int g = 0; g < p.groups; ++g) {
       double best = (double)OP_NONE, next = best;
-      for (int i = lane; i < size; i += 64) {
-        const int e = g * size + i;
-        const double v = op_ranked64(op_logit(p, t, e), op_bias(p, e));
-        next = v > best ? best : v > next ? v : next;
-        best = v > best ? v : best;
+#pragma unroll
+      for (int i = 0; i < OP_AGAIN; ++i) {
+        const int in = i * 64 + lane - g * size;
+        const double w = in >= 0 && in < size ? v[i] : (double)OP_NONE;
+        next = op_most(next, op_least(best, w));
+        best = op_most(best, w);
       }
       const double all = acc_wave_reduce(best, largest);
       /* (the first lane that has it gives its next) */
       const unsigned long long has = __ballot(best == all);
       const double second = acc_wave_reduce(lane == __builtin_ctzll(has) ? next : best, largest);
-      const double sum = all > (double)OP_NONE ? op_sum_of(all, second) : all;
-      if (lane == g) mine = sum;
+      if (lane == g) mine = all > (double)OP_NONE ? op_sum_of(all, second) : all;
     }
     int before = 0;
     for (int g = 0; g < p.groups; ++g) {
       const double other = acc_readlane(mine, g);
       before += other > mine || (other == mine && g < lane);
     }
-    kept = __ballot(lane < p.groups && before < p.keep);
+    const unsigned long long kept = __ballot(lane < p.groups && before < p.keep);
+#pragma unroll
+    for (int i = 0; i < OP_AGAIN; ++i)
+      if (i * 64 + lane < p.experts && !(kept >> ((i * 64 + lane) / size) & 1)) v[i] = (double)OP_NONE;
   }
   int chosen = -1;
-  double last = 0.0;                               /* the choices before are those that are larger, or as large with a lower index */
-  int last_index = -1;
   for (int j = 0; j < OP_CHOOSE; ++j) {
     double best = (double)OP_NONE;
     int index = 0x7fffffff;
-    for (int e = lane; e < p.experts; e += 64) {
-      if (!(kept >> (e / size) & 1)) continue;
-      const double v = op_ranked64(op_logit(p, t, e), op_bias(p, e));
-      const bool left = last_index < 0 || v < last || (v == last && e > last_index);
-      if (left && v > best) {
-        best = v;
-        index = e;
-      }
+#pragma unroll
+    for (int i = OP_AGAIN - 1; i >= 0; --i) {
+      if (v[i] >= best && v[i] > (double)OP_NONE) index = i * 64 + lane;
+      best = op_most(best, v[i]);
     }
     const double all = acc_wave_reduce(best, largest);
-    const int first = acc_wave_reduce(best == all ? index : 0x7fffffff, [](int a, int b) { return a < b ? a : b; });
     if (!(all > (double)OP_NONE)) break;
-    last = all;
-    last_index = first;
+    const int first = acc_wave_reduce(best == all ? index : 0x7fffffff, [](int a, int b) { return a < b ? a : b; });
     if (lane == j) chosen = first;
+#pragma unroll
+    for (int i = 0; i < OP_AGAIN; ++i)
+      if (i * 64 + lane == first) v[i] = (double)OP_NONE;
   }
   return chosen;
 }
@@ -183,13 +193,14 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
   const long long mine = first + wave * share, end = acc_min(last, mine + share);
   const int lots = OP_FEW ? OP_SELECT_WAVES : 1, size = p.experts / p.groups;
   int *const counts = shared + (OP_FEW ? wave * p.experts : 0), *const base = shared + lots * p.experts, *const sums = base + p.experts, *const slots = sums + p.experts;
-  float *const groups = (float *)(OP_FEW ? slots + (last - first) * OP_CHOOSE : base) + (wave * OP_TOKENS + token) * p.groups;
+  float *const groups = (float *)(OP_FEW ? slots + (last - first) * OP_CHOOSE : base) + (wave * OP_TOKENS + token) * 2 * p.groups;      /* sums, and what they may be off */
   for (int i = tid; i < lots * p.experts; i += 64 * OP_SELECT_WAVES) shared[i] = 0;
   __syncthreads();
 
-  /* the lane's logits: `whole` groups, or a part of one that it shares with others */
-  const int whole = p.groups / OP_LANES, lanes = whole ? 1 : OP_LANES / p.groups, part = whole ? whole * size : (size + lanes - 1) / lanes;
-  const int from = whole ? sub * part : sub / lanes * size + sub % lanes * part, count = whole ? part : acc_max(0, acc_min(part, size - sub % lanes * part));
+  /* the lane's logits: a part of a group that it shares with others, or all of it */
+  const int lanes = OP_LANES / p.groups, part = (size + lanes - 1) / lanes, own = sub / lanes;
+  const int from = own * size + sub % lanes * part, count = acc_max(0, acc_min(part, size - sub % lanes * part));
+  bool later = false;
   for (long long at = mine; at < end; at += OP_TOKENS) {
     const long long t = at + token;
     const bool here = t < end;
@@ -224,50 +235,34 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
     bool unsure = false;
     if (p.keep < p.groups) {
       op_two two = {OP_NONE, OP_NONE};
-      int g = whole ? sub * whole : sub / lanes, in = 0;
 #pragma unroll
-      for (int k = 0; k < OP_PER; ++k) {
-        op_put(two, r[k]);
-        if (whole && ++in == size && g < (sub + 1) * whole) {
-          groups[g++] = op_sum_of(two.best, two.next);
-          two.best = two.next = OP_NONE;
-          in = 0;
+      for (int k = 0; k < OP_PER; ++k) op_put(two, r[k]);
+#pragma unroll
+      for (int apart = 1; apart < OP_LANES; apart *= 2) {
+        const float best = op_other(two.best, apart), next = op_other(two.next, apart);
+        if (apart < lanes) {
+          op_put(two, best);
+          op_put(two, next);
         }
       }
-      if (!whole) {
-#pragma unroll
-        for (int apart = 1; apart < OP_LANES; apart *= 2) {
-          const float best = op_other(two.best, apart), next = op_other(two.next, apart);
-          if (apart < lanes) {
-            op_put(two, best);
-            op_put(two, next);
-          }
-        }
-        groups[g] = op_sum_of(two.best, two.next);
-      }
+      const float s = op_sum_of(two.best, two.next), off = op_off(two.best, two.next);
+      groups[2 * own] = s;
+      groups[2 * own + 1] = off;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
       /* a group stays if fewer than `keep` are larger for certain, and is in doubt if as many may be */
-      const int most = whole ? whole : 1;
-      int k0 = 0;
-      for (int n = 0; n < most; ++n) {
-        const int own = (whole ? sub * whole : sub / lanes) + n;
-        const float s = groups[own], near = op_near_groups(s);
-        int before = 0, above = 0, beside = 0;
-        for (int o = 0; o < p.groups; ++o) {
-          const float v = groups[o];
-          before += v > s || (v == s && o < own);
-          above += v > s + near;
-          beside += v >= s - near && o != own;
-        }
-        const bool stays = before < p.keep;
-        unsure = unsure || (s > OP_NONE && above < p.keep && beside >= p.keep);
-        const int k1 = whole ? k0 + size : OP_PER;
-        if (!stays)
-#pragma unroll
-          for (int k = 0; k < OP_PER; ++k) r[k] = k >= k0 && k < k1 ? OP_NONE : r[k];
-        k0 = k1;
+      int before = 0, above = 0, beside = 0;
+#pragma unroll 4
+      for (int o = 0; o < p.groups; ++o) {
+        const float v = groups[2 * o], near = off + groups[2 * o + 1];
+        before += v > s || (v == s && o < own);
+        above += v > s + near;
+        beside += v >= s - near && o != own;
       }
+      unsure = s > OP_NONE && above < p.keep && beside >= p.keep;
+      if (before >= p.keep)
+#pragma unroll
+        for (int k = 0; k < OP_PER; ++k) r[k] = OP_NONE;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
     }
@@ -275,7 +270,10 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
 #pragma unroll
     for (int j = 0; j < OP_KEYS; ++j) key[j] = (double)OP_NONE;
 #pragma unroll
-    for (int k = 0; k < OP_PER; ++k) op_insert(key, op_key_of(r[k], from + k));
+    for (int k = 0; k < OP_PER; ++k) {
+      op_insert(key, op_key_of(r[k], from + k));
+      __builtin_amdgcn_sched_barrier(0);           /* (or all are made first: registers) */
+    }
 #pragma unroll
     for (int apart = 1; apart < OP_LANES; apart *= 2) {
       double other[OP_KEYS];
@@ -283,6 +281,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
       for (int j = 0; j < OP_KEYS; ++j) other[j] = op_other(key[j], apart);
 #pragma unroll
       for (int j = 0; j < OP_KEYS; ++j) op_insert(key, other[j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     /* the j-th choice is the affair of lane j % OP_LANES: whether the one behind it is too near, its weight */
     int expert[(OP_CHOOSE + OP_LANES - 1) / OP_LANES];
@@ -302,27 +301,15 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
       const int a = acc_max(op_index_of(key[OP_CHOOSE]), 0);
       const float end_logit = op_logit(p, here ? t : mine, a), end_bias = op_bias(p, a);
 #pragma unroll
-      for (int c = 0; c < OP_PER / OP_VALUES; ++c) {
-        op_elt e[OP_VALUES];
-        __builtin_memcpy(e, &raw[c], 16);
-#pragma unroll
-        for (int i = 0; i < OP_VALUES; ++i) {
-          const int k = c * OP_VALUES + i;
-          if (edge && r[k] >= end_near && op_key_of(r[k], from + k) < key[OP_CHOOSE]) unsure = unsure || (float)e[i] != end_logit || op_bias(p, from + k) != end_bias;
-        }
-      }
+      for (int k = 0; k < OP_PER; ++k)
+        if (edge && r[k] >= end_near && op_key_of(r[k], from + k) < key[OP_CHOOSE])
+          unsure = unsure || op_logit(p, t, from + k) != end_logit || op_bias(p, from + k) != end_bias;
     }
-    unsigned long long again = __ballot(unsure && here);
-    while (again) {
-      const int which = __builtin_ctzll(again) / OP_LANES;
-      again &= ~((OP_LANES == 64 ? ~0ull : (1ull << OP_LANES) - 1) << which * OP_LANES);
-      const int chosen = op_again(p, at + which, lane);
-#pragma unroll
-      for (int s = 0; s < (OP_CHOOSE + OP_LANES - 1) / OP_LANES; ++s) {
-        const int e = __builtin_amdgcn_ds_bpermute(acc_min(s * OP_LANES + sub, 63) * 4, chosen);
-        if (which == token) expert[s] = e;
-      }
-    }
+    /* (a token that is to be decided again is marked, and left for when the registers are free) */
+    const unsigned long long doubt = __ballot(unsure && here);
+    later = later || doubt != 0;
+    const bool sure = here && (doubt >> (OP_LANES < 64 ? token * OP_LANES : 0) & (OP_LANES < 64 ? (1ull << (OP_LANES & 63)) - 1 : ~0ull)) == 0;
+    if (here && !sure && sub == 0) __hip_atomic_store(p.chosen + t * OP_CHOOSE, -2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     float w[(OP_CHOOSE + OP_LANES - 1) / OP_LANES], most = OP_NONE, total = 0.0f;
 #pragma unroll
     for (int s = 0; s < (OP_CHOOSE + OP_LANES - 1) / OP_LANES; ++s) {
@@ -346,12 +333,32 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
 #pragma unroll
     for (int s = 0; s < (OP_CHOOSE + OP_LANES - 1) / OP_LANES; ++s) {
       const int j = s * OP_LANES + sub;
-      if (!here || j >= OP_CHOOSE) continue;
+      if (!sure || j >= OP_CHOOSE) continue;
       const int e = expert[s];
       p.chosen[t * OP_CHOOSE + j] = e;
       if (OP_FEW) slots[t * OP_CHOOSE + j] = e;
       p.weights[t * OP_CHOOSE + j] = e < 0 ? 0.0f : !p.normalise ? p.scale * w[s] : total > 0.0f ? p.scale * (w[s] / total) : 0.0f;
       if (e >= 0) atomicAdd(&counts[e], 1);
+    }
+  }
+  if (later) {
+    __threadfence();
+    for (long long at = mine; at < end; at += 64) {
+      const bool here = at + lane < end;
+      unsigned long long marked = __ballot(here && __hip_atomic_load(p.chosen + (at + (here ? lane : 0)) * OP_CHOOSE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == -2);
+      while (marked) {
+        const long long t = at + __builtin_ctzll(marked);
+        marked &= marked - 1;
+        const int e = op_again(p, t, lane);
+        const float x = e >= 0 ? op_logit(p, t, e) : OP_NONE;
+        const float most = acc_wave_reduce(x, [](float a, float b) { return a > b ? a : b; }), w = op_part(x, p.normalise ? acc_min(most, 0.0f) : 0.0f);
+        const float total = acc_wave_reduce(w, [](float a, float b) { return a + b; });
+        if (lane >= OP_CHOOSE) continue;
+        p.chosen[t * OP_CHOOSE + lane] = e;
+        if (OP_FEW) slots[t * OP_CHOOSE + lane] = e;
+        p.weights[t * OP_CHOOSE + lane] = e < 0 ? 0.0f : !p.normalise ? p.scale * w : total > 0.0f ? p.scale * (w / total) : 0.0f;
+        if (e >= 0) atomicAdd(&counts[e], 1);
+      }
     }
   }
   __threadfence_block();
