@@ -1618,6 +1618,7 @@ static int check_grouped(acc_op op, const char *who, const acc_strided *codes, c
   if (zeros) ACC_TRY(check_shape(who, "zeros", *zeros, {experts, groups, n}));
   if (!aligned_rows(*codes, 1, 2)) return fail(ACC_ERR_INVALID, "%s: rows of codes start on 16 bytes", who);
   ACC_TRY(check_extents(who, {experts, n, k}));
+  if (k > (1 << 30)) return fail(ACC_ERR_INVALID, "%s: rows of %lld numbers", who, (long long)k);
   a->codes = device<void>(codes);
   a->scales = device<void>(scales);
   a->zeros = device<void>(zeros);

@@ -773,7 +773,7 @@ int acc_exec_micro_rows(acc_op op, const acc_strided *xcodes, const acc_strided 
  * in the low half, rows on 16 bytes); scales [experts, ceil(k / group), n] in the operator's type, zeros the same in bytes, both with
  * n contiguous; zeros NULL: all 8.  quantise, of w [experts, n, k]: with zeros s = (high - low) / 15 of a group's range, which has 0 in
  * it, z = -low / s, without s = the largest magnitude / 7; s is rounded to the type, then the numbers, ties to even.  A group with an
- * infinity or what is not a number has a scale that is not a number.                                          */
+ * infinity or what is not a number has a scale that is not a number.  A row has at most 2^30 numbers.         */
 int acc_exec_grouped_quantise(acc_op op, const acc_strided *w, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros,
                               acc_stream stream);
 int acc_exec_grouped_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, const acc_strided *out,

@@ -242,6 +242,14 @@ int main(int, char **argv)
   REFUSED(acc_exec_score(op, &z, nullptr, &x, &x, &x, &x, &x, nullptr));
   REFUSED(acc_exec_grouped_rows(op, &x, &z, &z, nullptr, &offsets, nullptr, 0, &out, nullptr));
   OK(acc_op_destroy(op));
+  d.kind = ACC_OP_GROUPED;
+  d.group = 1 << 30;
+  OK(acc_op_create(ctx, &d, &op));
+  const int64_t most = (1 << 30) + 32;
+  const acc_strided pair = array({2}), far = array({1, most}), codes = array({1, 1, most / 2}), scales = array({1, 2, 1}), result = array({1, 1}), matrices = array({1, 1, most});
+  REFUSED(acc_exec_grouped_rows(op, &far, &codes, &scales, nullptr, &pair, nullptr, 0, &result, nullptr));
+  REFUSED(acc_exec_grouped_quantise(op, &matrices, &codes, &scales, nullptr, nullptr));
+  OK(acc_op_destroy(op));
   for (int bad = 0; bad < 6; ++bad) {
     acc_op_desc e = {};
     e.elt_type = "half";
