@@ -246,23 +246,24 @@ struct GroupedVariant {
   bool few = false;             // ... and each has a few steps
   bool sixteen = false;         // tiles of sixteen rows, whose places are known when the kernel is compiled
   bool stream = false;          // rows in LDS, waves that go over columns (else they read rows and codes for every tile)
+  bool tall = false;            // tiles of 128 rows by 256 columns
   bool elements = false;
-  int waves() const { return stream || fn == 1 ? wide : 4; }
+  int waves() const { return tall ? 8 : stream || fn == 1 ? wide : 4; }
   int ahead(const OpSpec &sp) const
   {
     // (their scales and zeros are a load of 64 lanes)
     if (stream) return few || sp.group == 32 || (sp.group == 64 && sp.type == 0) ? 2 : 4;
     return elements || bm > 32 || (bm > 16 && sp.type == 0) ? 1 : bm > 16 || fn > 1 || sp.type == 0 ? 2 : 4;
   }
-  uint32_t key() const { return kGroupedKeys | (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u) | (stream ? 512u : 0u) | (zeros ? 1024u : 0u) | (wide == 8 ? 2048u : 0u) | (sixteen ? 4096u : 0u) | (few ? 8192u : 0u); }
+  uint32_t key() const { return kGroupedKeys | (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u) | (stream ? 512u : 0u) | (zeros ? 1024u : 0u) | (wide == 8 ? 2048u : 0u) | (sixteen ? 4096u : 0u) | (few ? 8192u : 0u) | (tall ? 16384u : 0u); }
   static constexpr uint32_t kGroupedKeys = 1u << 21;               // (beside the products' keys)
 };
 std::string grouped_source(const OpSpec &sp, const GroupedVariant &v)
 {
   char text[512];
   std::snprintf(text, sizeof(text),
-                "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_GROUP %d\n#define OP_AHEAD %d\n#define OP_STREAM %d\n#define OP_WAVES %d\n#define OP_ZEROS %d\n#define OP_HEIGHT %d\n#define OP_ELEMENTS %d\n#include \"acc_hip_device.h\"\n#include \"op_grouped.h\"\n",
-                sp.type, sp.type == 1 ? 1 : 2, v.bm, v.fn, v.elements ? 4 : std::min(4, sp.group / 32), v.ahead(sp), v.stream ? 1 : 0, v.waves(), v.zeros ? 1 : 0, v.sixteen ? 16 : 0, v.elements ? 1 : 0);
+                "#define OP_ELT %d\n#define OP_TYPE %d\n#define OP_BM %d\n#define OP_FN %d\n#define OP_GROUP %d\n#define OP_AHEAD %d\n#define OP_STREAM %d\n#define OP_WIDE %d\n#define OP_WAVES %d\n#define OP_ZEROS %d\n#define OP_HEIGHT %d\n#define OP_ELEMENTS %d\n#include \"acc_hip_device.h\"\n#include \"op_grouped.h\"\n",
+                sp.type, sp.type == 1 ? 1 : 2, v.bm, v.fn, v.elements ? 4 : std::min(4, sp.group / 32), v.ahead(sp), v.stream ? 1 : 0, v.tall ? 1 : 0, v.waves(), v.zeros ? 1 : 0, v.sixteen ? 16 : 0, v.elements ? 1 : 0);
   return text;
 }
 
@@ -340,6 +341,12 @@ std::vector<std::string> all_sources(const OpSpec &sp)
         }
       }
     GroupedVariant v;
+    v.tall = true;
+    for (bool zeros : {false, true}) {
+      v.zeros = zeros;
+      if (sp.type != 0) out.push_back(grouped_source(sp, v));
+    }
+    v = {};
     v.elements = true;
     out.push_back(grouped_source(sp, v));
     // (and the products of matrices that have been made again)
@@ -631,7 +638,7 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
 }
 
 // grouped: from how many rows a segment on the matrices are made again for tiles that use them often.  us, as they are and made again:
-// 160 rows, 2 of 4096 x 4096: 41 and 53; 512, 8: 83 and 162; 2048, 8: some 330 and 229
+// 160 rows, 2 of 4096 x 4096: 41 and 53; 512, 8: 83 and 162; 2048, 8: some 330 and 184
 constexpr int64_t kGroupedMost = 128;
 // ... LDS of the form with rows in it: `height` of them, their sums by groups, and the waves' results where they share columns
 int64_t grouped_lds(const OpSpec &sp, int64_t height, int64_t steps, int64_t waves)
@@ -640,11 +647,26 @@ int64_t grouped_lds(const OpSpec &sp, int64_t height, int64_t steps, int64_t wav
   return steps * height * (256 * (sp.type == 0 ? 3 : 1) + chunks * (sp.type == 1 ? 8 : 4)) + waves * ceil_div(height, 16) * 1024;
 }
 constexpr int64_t kGroupedLds = 160 << 10;
+// ... and of tiles of 128 rows by 256 columns: three steps of rows, scales and zeros, two of sums
+int64_t grouped_tall_lds(const OpSpec &sp, bool zeros)
+{
+  const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
+  return 3 * 16 * 128 * 16 + 3 * chunks * 272 * 4 * (zeros ? 2 : 1) + 2 * chunks * 128 * 4 * (zeros && sp.type == 1 ? 2 : 1);
+}
 // ... and the tiles of 16 columns from which on rows in LDS are worth what it takes to put them there.  us, with and without, tiles: 1 row,
 // 4096 x 4096, 256: 8.2 and 7.2; 16 rows: 14 and 11; 2 rows of 4096 x 11008, 256: 16 and 15; of 11008 x 4096, 688: 13 and 18; 1 row, 8192 x 8192,
 // 512: 16 and 23; 64 rows, 16 half of 4096 x 2048, 4096: 23 and 34; 16, 8 of 4096 x 4096 in groups of 32: 29 and 44; Float32, 64, 16 of
 // 1024 x 2048, 1024: 14 and 12
 constexpr int64_t kGroupedStream = 384;
+// Whether a call is for tiles of 128 rows by 256 columns that make numbers of the codes as they go: there are enough tiles (one that is
+// 4096 long takes 80 us, however few there are), and not so many rows a matrix that making it again is little beside its products.  us,
+// with and without, rows, matrices, tiles: 640, 8 of 4096 x 4096, 128: 85 and 131; 2048, 8, 256: 97 and 184, in groups of 32 with zeros 137
+// and 204; 4096, 8, 512: 176 and 210, in groups of 32 252 and 231; 8192, 8, 1024: 338 and 308; 640, 4, 80: 86 and 106; 300, 3, 48: 85 and
+// 66; 2000, 3 of 2048 x 2048, 128: 65 and 48; 1600, 20 of 1000 x 1000, 80: 34 and 32; 4096, 32 of 4096 x 1024, 512: 65 and 168
+bool grouped_tall(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean)
+{
+  return sp.type != 0 && n >= 16 && k > 0 && pitch < (1 << 26) && mean > 64 && mean <= (sp.group >= 64 ? 512 : 256) && std::max(ceil_div(rows, 128), std::min(rows, experts)) * ceil_div(n, 256) >= 72;
+}
 // the tile for `mean` rows a segment; *height: its rows.  (Where LDS holds fewer rows than a segment has, their codes are read again:
 // 64 rows, 2 of 4096 x 4096: 18 us in tiles of 16, 26 without LDS.)
 GroupedVariant grouped_variant(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean, int64_t *height)
@@ -738,6 +760,7 @@ std::string grouped_source_of(const OpSpec &sp, uint32_t key)
   v.wide = key & 2048u ? 8 : 16;
   v.sixteen = key & 4096u;
   v.few = key & 8192u;
+  v.tall = key & 16384u;
   return grouped_source(sp, v);
 }
 
@@ -1705,7 +1728,8 @@ try {
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "x"}, {codes, 1, "codes"}, {scales, bytes, "scales"}, {zeros, 1, "zeros"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (is_empty(*out)) return ACC_OK;
   const int64_t mean = ceil_div(rows, std::max<int64_t>(1, std::min(rows, experts)));
-  if (mean > kGroupedMost && k > 0 && x->shape[0] > 0) {
+  const bool tall = grouped_tall(op->spec, rows, experts, n, k, codes->stride[1], mean);
+  if (!tall && mean > kGroupedMost && k > 0 && x->shape[0] > 0) {
     ScratchHold made;
     ACC_TRY(made.acquire(op, stream, (size_t)(experts * n * ceil_div(k, 8) * 8 * bytes)));
     acc_strided w = {};
@@ -1727,7 +1751,13 @@ try {
     return product_of_rows(op, who, x, &w, offsets, index, per, out, product, stream);
   }
   int64_t height = 0;
-  GroupedVariant v = grouped_variant(op->spec, rows, experts, n, k, codes->stride[1], mean, &height);
+  GroupedVariant v;
+  if (tall) {
+    v.tall = true;
+    height = 128;
+  } else {
+    v = grouped_variant(op->spec, rows, experts, n, k, codes->stride[1], mean, &height);
+  }
   v.zeros = zeros != nullptr;
   a.x = device<const void>(x);
   a.out = device<void>(out);
@@ -1742,6 +1772,10 @@ try {
   a.height = (int32_t)height;
   a.run = v.fn;
   size_t lds = 0;
+  if (v.tall) {
+    a.run = 16;
+    lds = (size_t)grouped_tall_lds(op->spec, v.zeros);
+  }
   if (v.stream) {
     // a workgroup a compute unit; where it has fewer tiles of columns than waves, those share them
     const int64_t all = std::max(ceil_div(rows, height), std::min(rows, experts)) * ceil_div(n, 16);

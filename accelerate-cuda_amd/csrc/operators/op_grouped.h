@@ -386,6 +386,185 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
       __syncthreads();
     }
 }
+#elif OP_WIDE
+/* The form for many rows of a matrix: tiles of 128 rows by 256 columns, eight waves of 64 by 64.  The rows of a step of 128 lie in LDS,
+ * three steps at a time: the one whose products are taken, the next one, whose sums by groups are taken meanwhile (of 16 rows by each of
+ * the four waves that share them), and the one after that, on its way there.  A wave makes its 64 columns' codes into numbers itself,
+ * in registers. */
+#define OP_ROWS 128
+#define OP_COLUMNS 256
+#define OP_LINE (OP_COLUMNS + 16)                  /* scales (zeros) of a group: 16 places in front, for a tile with fewer columns */
+
+extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args p)
+{
+  if (p.guard && *p.guard == 0u) return;
+  extern __shared__ acc_u4 shared[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4, wm = wave >> 2, wn = wave & 3;
+  const op_tile tile = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, OP_ROWS, op_segments(p.offsets, p.experts, (int)p.rows, 0, 0), (int)(blockIdx.x / p.tiles_j));
+  if (tile.begin >= tile.end) return;
+  const int steps = (p.blocks + 3) / 4, rows = tile.end - tile.begin, j0 = (int)(blockIdx.x % p.tiles_j) * OP_COLUMNS;
+  acc_u4 *const x = shared;                        /* [3][16][OP_ROWS]: eight neighbours of a row, a row's places turned by their number */
+  float *const scale = (float *)(x + 3 * 16 * OP_ROWS);                    /* [3][chunks][OP_LINE], and the zeros' */
+  float *const zero = scale + 3 * OP_CHUNKS * OP_LINE;
+  float *const sum = OP_ZEROS ? zero + 3 * OP_CHUNKS * OP_LINE : zero;     /* [2][chunks][OP_ROWS]; what products begin with, where zeros are 8 */
+  float *const offset = sum + 2 * OP_CHUNKS * OP_ROWS;                     /* the same, of half rows with zeros */
+  acc_f4 c[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[i][j] = acc_f4{0.0f, 0.0f, 0.0f, 0.0f};
+  const auto row_of = [&](const int m) { return p.index ? op_listed(p.index, tile.begin + m, tile.begin, tile.end, p.x_rows, p.per_mul, p.per_shift) : tile.begin + acc_min(m, rows - 1); };
+
+  if (tile.expert >= 0 && p.x_rows > 0 && steps > 0) {
+    /* a lane's places among the rows: eight neighbours, of four rows 32 apart */
+    const int chunk = tid & 15, first = tid >> 4, place = ((OP_CHUNKS > 1 ? chunk : chunk % 4 * 4 + chunk / 4) * OP_ROWS) + (first ^ (chunk & 7));
+    const op_elt *from[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 32 * u), 0) * p.x_stride + chunk * 8;
+    /* ... and among the scales and zeros: of 8, or of 16 columns (of the last: as many as there are) */
+    const bool scale_lane = tid < OP_CHUNKS * 32;
+    const int noted = scale_lane ? tid / 32 : (tid - OP_CHUNKS * 32) / 16 % OP_CHUNKS, at_column = acc_min(j0 + (scale_lane ? tid % 32 * 8 : tid % 16 * 16), p.nj - (scale_lane ? 8 : 16));
+    const unsigned char *const notes = scale_lane || !OP_ZEROS ? (const unsigned char *)((const op_elt *)p.scales + tile.expert * p.scales_expert + (scale_lane ? at_column : 0))
+                                                               : (const unsigned char *)p.zeros + tile.expert * p.zeros_expert + at_column;
+    const long long note_stride = scale_lane || !OP_ZEROS ? p.scales_stride * (long long)sizeof(op_elt) : p.zeros_stride;
+    acc_u4 v[4], note;
+    const auto load = [&](const int n) {
+      const int group = acc_min(((n * 128) >> p.group_shift) + noted, p.groups - 1);
+      note = ((const op_loose<unsigned char> *)(notes + group * note_stride))->v;
+      if (n * 128 + 128 <= p.k) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = ((const op_loose<op_elt> *)(from[u] + n * 128))->v;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = op_chunk<false>(from[u] + n * 128, p.k - n * 128 - chunk * 8);
+      }
+    };
+    const auto put = [&](const int to) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        acc_u4 part[1];
+        op_parts(op_eight{{v[u]}}, part);
+        x[to * 16 * OP_ROWS + place + 32 * u] = part[0];
+      }
+      if (scale_lane) {
+        op_elt e[8];
+        __builtin_memcpy(e, &note, 16);
+        float *const line = scale + (to * OP_CHUNKS + noted) * OP_LINE + 16 + (at_column - j0);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) line[t] = (float)e[t];
+      } else if (OP_ZEROS && tid < OP_CHUNKS * 48) {
+        float *const line = zero + (to * OP_CHUNKS + noted) * OP_LINE + 16 + (at_column - j0);
+#pragma unroll
+        for (int t = 0; t < 16; ++t) line[t] = (float)(note[t / 4] >> t % 4 * 8 & 255u);
+      }
+    };
+    /* the lane's fragment of rows 16 i on of a wave's */
+    const auto row16 = [&](const int buffer, const int b, const int i) {
+      const int turn = (OP_CHUNKS > 1 ? 4 * b + g : 4 * g + b) & 7;
+      return op_as_frag(x[buffer * 16 * OP_ROWS + (b * 4 + g) * OP_ROWS + wm * 64 + i * 16 + (l ^ turn)]);
+    };
+    const auto add_up = [&](const int buffer, const int slot) {
+#pragma unroll
+      for (int q = 0; q < OP_CHUNKS; ++q) {
+        acc_f4 t = {0.0f, 0.0f, 0.0f, 0.0f}, d = t;
+#pragma unroll
+        for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
+          const op_frag y = row16(buffer, b, wn);
+          t = op_mfma(op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), y, t);
+          if (OP_ELT == 1) d = op_mfma(op_as_frag(op_offsets()), y, d);
+        }
+        const int at = (slot * OP_CHUNKS + q) * OP_ROWS + wm * 64 + wn * 16 + l;
+        const float o = OP_ELT == 1 ? d[0] : 128.0f * t[0];
+        if (g == 0) {
+          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], o, 8.0f);
+          if (OP_ZEROS && OP_ELT == 1) offset[at] = o;
+        }
+      }
+    };
+
+    /* codes: 16 columns are 16 rows of bytes; columns and blocks that there are not are read as the last ones */
+    const int column = acc_min(j0 + wn * 64, p.nj - 1), left = p.nj - 1 - column, last_step = p.blocks % 4 ? steps - 1 : -1;
+    const unsigned char *const codes = (const unsigned char *)p.codes + tile.expert * p.codes_expert + column * p.codes_stride;
+    const unsigned int early = (unsigned int)acc_max(0, g - (p.blocks - 1 - (steps - 1) * 4)) * 16;
+    unsigned int at_code[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at_code[j] = (unsigned int)acc_min(16 * j + l, left) * (unsigned int)p.codes_stride + g * 16;
+    acc_u4 w[4];
+    const auto load_codes = [&](const int n, const int j) {
+      w[j] = *(const acc_u4 *)(codes + (long long)n * 64 + (at_code[j] - (n != last_step ? 0u : early)));
+    };
+
+    load(0);
+    put(0);
+    load(acc_min(1, steps - 1));
+    put(1);
+    load(acc_min(2, steps - 1));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load_codes(0, j);
+    __syncthreads();
+    add_up(0, 0);
+    int now = 0, next = 1, then = 2;
+    for (int n = 0; n < steps; ++n) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) op_turn(w[j]);
+#pragma unroll
+      for (int q = 0; q < OP_CHUNKS; ++q) {
+        op_frag y[OP_BLOCKS][4];
+        float f[4], o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int b = 0; b < OP_BLOCKS; ++b) y[b][i] = row16(now, q * OP_BLOCKS + b, i);
+          const int at = ((n & 1) * OP_CHUNKS + q) * OP_ROWS + wm * 64 + i * 16 + l;
+          f[i] = sum[at];
+          if (OP_ZEROS) o[i] = OP_ELT == 1 ? offset[at] : 128.0f * f[i];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = (now * OP_CHUNKS + q) * OP_LINE + 16 + wn * 64 + j * 16 + g * 4;
+          const acc_f4 s = *(const acc_f4 *)(scale + at), z = OP_ZEROS ? *(const acc_f4 *)(zero + at) : s;
+          op_frag numbers[OP_BLOCKS];
+#pragma unroll
+          for (int b = 0; b < OP_BLOCKS; ++b) numbers[b] = op_as_frag(op_numbers(w[j][q * OP_BLOCKS + b]));
+          if (q == OP_CHUNKS - 1) load_codes(acc_min(n + 1, steps - 1), j);
+          acc_f4 t[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], o[i], z[r]) : f[i];
+#pragma unroll
+          for (int b = 0; b < OP_BLOCKS; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = op_mfma(numbers[b], y[b][i], t[i]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c[i][j][r] = __builtin_fmaf(s[r], t[i][r], c[i][j][r]);
+          /* (the next steps' rows and sums amid the products: every wave has some to go on with) */
+          if (q == 0 && j == 0) {
+            put(then);
+            load(acc_min(n + 3, steps - 1));
+          }
+          if (q == 0 && j == 1) add_up(next, (n + 1) & 1);
+        }
+      }
+      const int was = now;
+      now = next;
+      next = then;
+      then = was;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = wm * 64 + i * 16 + l;
+    if (m >= rows) continue;
+    const bool none = tile.expert < 0 || row_of(m) < 0;
+    op_elt *const out = (op_elt *)p.out + (long long)(tile.begin + m) * p.out_stride;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) op_write4(out, j0 + wn * 64 + j * 16 + 4 * g, p.nj, c[i][j], none);
+  }
+}
 #else
 struct op_step {
   acc_u4 w[OP_FN];

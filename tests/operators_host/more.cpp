@@ -27,7 +27,7 @@
 static std::map<uint64_t, size_t> g_blocks;       // device memory: where, and how much
 static uint64_t g_next = 1ull << 50;
 static int g_wrong = 0;
-static long g_calls = 0, g_cleared = 0, g_scans = 0, g_stream = 0, g_places = 0;
+static long g_calls = 0, g_cleared = 0, g_scans = 0, g_stream = 0, g_tall = 0, g_places = 0;
 static bool g_recorded = false;
 static int64_t g_element = 2;
 static int g_choose = 0;
@@ -92,7 +92,11 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned gx, unsigned gy, unsi
     if ((int64_t)gx != (int64_t)a.tiles_i * a.tiles_j) not_so("grid of the products", gx, a.tiles_i);
     const int64_t parts = std::min<int64_t>(a.rows, a.experts + 2), least = (a.rows + parts * (a.height - 1)) / a.height;
     if (a.tiles_i < least) not_so("fewer tiles than segments may have", a.tiles_i, least);
-    if (bx >= 512 && lds) {
+    if (a.height == 128) {
+      ++g_tall;
+      const int64_t chunks = a.group >= 128 ? 1 : 128 / a.group, need = 3 * (16 * 128 * 16 + chunks * 272 * 4 * (a.zeros ? 2 : 1)) + 2 * chunks * 128 * 4 * (a.zeros ? 2 : 1);
+      if (a.run != 16 || bx != 512 || a.nj < 16 || a.codes_stride * 63 + 64 > 0xffffffffll || (int64_t)lds > need || (int64_t)lds < need - 2 * chunks * 128 * 4) not_so("LDS of the tall tiles", lds, need);
+    } else if (bx >= 512 && lds) {
       ++g_stream;
       const int64_t chunks = a.group >= 128 ? 1 : 128 / a.group, waves = bx / 64, rows = (a.height + 15) / 16;
       const int64_t need = waves * rows * 1024 + steps * a.height * (256 * (g_element == 4 ? 3 : 1) + chunks * 8);
@@ -262,6 +266,6 @@ int main(int, char **argv)
     REFUSED(acc_op_create(ctx, &e, &op));
   }
   OK(acc_context_destroy(ctx));
-  std::printf("%ld scans, %ld cleared, %ld products with rows in LDS, %ld placings\nwrong %d\n", g_scans, g_cleared, g_stream, g_places, g_wrong);
+  std::printf("%ld scans, %ld cleared, %ld products with rows in LDS, %ld of tall tiles, %ld placings\nwrong %d\n", g_scans, g_cleared, g_stream, g_tall, g_places, g_wrong);
   return g_wrong ? 1 : 0;
 }

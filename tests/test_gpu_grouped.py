@@ -117,11 +117,31 @@ def test_products_of_whole_numbers_are_exact(A, ctx, ops, elt, group, with_zeros
         assert np.array_equal(out.get(), store(want, elt)), (rows, experts, n, k)
 
 
+@pytest.mark.parametrize("group,with_zeros", ((32, False), (32, True), (64, True), (128, False), (512, True)))
+@pytest.mark.parametrize("elt", ("half", "bfloat16"))
+def test_many_rows_of_many_matrices(A, ctx, ops, elt, group, with_zeros):
+    """tiles of 128 rows by 256 columns: a last tile of one column, rows and sums that end anywhere, an index, segments of no row"""
+    rng = np.random.default_rng(group + 7)
+    for case, (rows, experts, n, k) in enumerate(((2000, 25, 900, 300), (1700, 18, 1025, 129), (3000, 40, 300, 1), (1400, 20, 1000, 640), (1500, 19, 784, 95))):
+        q, scales, zeros = matrices(rng, experts, n, k, group, elt, with_zeros, True)
+        offsets, per = segments(rng, rows, experts, ("even", "skewed", "gaps")[case % 3]), (0, 1, 3)[case % 3]
+        index = None if case % 2 else rng.integers(-2, rows * max(per, 1), rows).astype(np.int32)
+        x = rng.integers(-3, 4, (rows if index is None else rows - 1, k)).astype(np.float64)
+        say(elt, group, with_zeros, rows, experts, n, k, per, index is not None)
+        loose = case % 3
+        want, _ = expected(x, weights(q, scales, zeros, group), offsets, rows, index, per)
+        bx, out = Boxed(A, ctx, x, elt, lead=loose, extra=loose), Boxed(A, ctx, np.full((rows, n), 9.0), elt, lead=1, extra=loose, fill=3.0)
+        args = bx.array, ctx.array(packed(q)), Boxed(A, ctx, scales, elt, lead=loose, extra=loose).array, ctx.array(offsets), out.array
+        ops(elt, group).rows(*args, zeros=None if zeros is None else ctx.array(zeros), index=None if index is None else ctx.array(index), per=per)
+        ctx.sync()
+        assert np.array_equal(out.get(), store(want, elt)), (rows, experts, n, k)
+
+
 @pytest.mark.parametrize("group", (32, 128))
 @pytest.mark.parametrize("elt", TYPES)
 def test_products_of_any_numbers(A, ctx, ops, elt, group):
     rng = np.random.default_rng(group + 1)
-    for rows, experts, n, k in ((1, 1, 300, 1000), (40, 3, 129, 700), (128, 2, 64, 384), (500, 2, 90, 161)):
+    for rows, experts, n, k in ((1, 1, 300, 1000), (40, 3, 129, 700), (128, 2, 64, 384), (500, 2, 90, 161), (1500, 20, 800, 700)):
         q, scales, zeros = matrices(rng, experts, n, k, group, elt, rows > 1, False)
         x = values(store(rng.standard_normal((rows, k)), elt), elt)
         offsets = segments(rng, rows, experts, "even")
