@@ -391,15 +391,17 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
  * three steps at a time: the one whose products are taken, the next one, whose sums by groups are taken meanwhile (of 16 rows by each of
  * the four waves that share them), and the one after that, on its way there.  A wave makes its 64 columns' codes into numbers itself,
  * in registers. */
-#define OP_ROWS 128
+#define OP_ROWS 64
 #define OP_COLUMNS 256
 #define OP_LINE (OP_COLUMNS + 16)                  /* scales (zeros) of a group: 16 places in front, for a tile with fewer columns */
 
-extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args p)
+template <int N> struct op_count { static constexpr int value = N; };
+
+extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) grouped(const acc_grouped_args p)
 {
   if (p.guard && *p.guard == 0u) return;
   extern __shared__ acc_u4 shared[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4, wm = wave >> 2, wn = wave & 3;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l = lane & 15, g = lane >> 4;
   const op_tile tile = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, OP_ROWS, op_segments(p.offsets, p.experts, (int)p.rows, 0, 0), (int)(blockIdx.x / p.tiles_j));
   if (tile.begin >= tile.end) return;
   const int steps = (p.blocks + 3) / 4, rows = tile.end - tile.begin, j0 = (int)(blockIdx.x % p.tiles_j) * OP_COLUMNS;
@@ -416,11 +418,11 @@ extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args
   const auto row_of = [&](const int m) { return p.index ? op_listed(p.index, tile.begin + m, tile.begin, tile.end, p.x_rows, p.per_mul, p.per_shift) : tile.begin + acc_min(m, rows - 1); };
 
   if (tile.expert >= 0 && p.x_rows > 0 && steps > 0) {
-    /* a lane's places among the rows: eight neighbours, of four rows 32 apart */
+    /* a lane's places among the rows: eight neighbours, of four rows 16 apart */
     const int chunk = tid & 15, first = tid >> 4, place = ((OP_CHUNKS > 1 ? chunk : chunk % 4 * 4 + chunk / 4) * OP_ROWS) + (first ^ (chunk & 7));
     const op_elt *from[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 32 * u), 0) * p.x_stride + chunk * 8;
+    for (int u = 0; u < 4; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 16 * u), 0) * p.x_stride + chunk * 8;
     /* ... and among the scales and zeros: of 8, or of 16 columns (of the last: as many as there are) */
     const bool scale_lane = tid < OP_CHUNKS * 32;
     const int noted = scale_lane ? tid / 32 : (tid - OP_CHUNKS * 32) / 16 % OP_CHUNKS, at_column = acc_min(j0 + (scale_lane ? tid % 32 * 8 : tid % 16 * 16), p.nj - (scale_lane ? 8 : 16));
@@ -444,7 +446,7 @@ extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args
       for (int u = 0; u < 4; ++u) {
         acc_u4 part[1];
         op_parts(op_eight{{v[u]}}, part);
-        x[to * 16 * OP_ROWS + place + 32 * u] = part[0];
+        x[to * 16 * OP_ROWS + place + 16 * u] = part[0];
       }
       if (scale_lane) {
         op_elt e[8];
@@ -461,7 +463,7 @@ extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args
     /* the lane's fragment of rows 16 i on of a wave's */
     const auto row16 = [&](const int buffer, const int b, const int i) {
       const int turn = (OP_CHUNKS > 1 ? 4 * b + g : 4 * g + b) & 7;
-      return op_as_frag(x[buffer * 16 * OP_ROWS + (b * 4 + g) * OP_ROWS + wm * 64 + i * 16 + (l ^ turn)]);
+      return op_as_frag(x[buffer * 16 * OP_ROWS + (b * 4 + g) * OP_ROWS + i * 16 + (l ^ turn)]);
     };
     const auto add_up = [&](const int buffer, const int slot) {
 #pragma unroll
@@ -469,11 +471,11 @@ extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args
         acc_f4 t = {0.0f, 0.0f, 0.0f, 0.0f}, d = t;
 #pragma unroll
         for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
-          const op_frag y = row16(buffer, b, wn);
+          const op_frag y = row16(buffer, b, wave);
           t = op_mfma(op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), y, t);
           if (OP_ELT == 1) d = op_mfma(op_as_frag(op_offsets()), y, d);
         }
-        const int at = (slot * OP_CHUNKS + q) * OP_ROWS + wm * 64 + wn * 16 + l;
+        const int at = (slot * OP_CHUNKS + q) * OP_ROWS + wave * 16 + l;
         const float o = OP_ELT == 1 ? d[0] : 128.0f * t[0];
         if (g == 0) {
           sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], o, 8.0f);
@@ -483,7 +485,7 @@ extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args
     };
 
     /* codes: 16 columns are 16 rows of bytes; columns and blocks that there are not are read as the last ones */
-    const int column = acc_min(j0 + wn * 64, p.nj - 1), left = p.nj - 1 - column, last_step = p.blocks % 4 ? steps - 1 : -1;
+    const int column = acc_min(j0 + wave * 64, p.nj - 1), left = p.nj - 1 - column, last_step = p.blocks % 4 ? steps - 1 : -1;
     const unsigned char *const codes = (const unsigned char *)p.codes + tile.expert * p.codes_expert + column * p.codes_stride;
     const unsigned int early = (unsigned int)acc_max(0, g - (p.blocks - 1 - (steps - 1) * 4)) * 16;
     unsigned int at_code[4];
@@ -503,66 +505,73 @@ extern "C" __global__ void __launch_bounds__(512) grouped(const acc_grouped_args
     for (int j = 0; j < 4; ++j) load_codes(0, j);
     __syncthreads();
     add_up(0, 0);
-    int now = 0, next = 1, then = 2;
-    for (int n = 0; n < steps; ++n) {
-      __syncthreads();
+    /* the products of 16 M rows (a segment's last tile may have few) */
+    const auto products = [&](const auto fragments) {
+      constexpr int M = decltype(fragments)::value;
+      int now = 0, next = 1, then = 2;
+      for (int n = 0; n < steps; ++n) {
+        __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) op_turn(w[j]);
+        for (int j = 0; j < 4; ++j) op_turn(w[j]);
 #pragma unroll
-      for (int q = 0; q < OP_CHUNKS; ++q) {
-        op_frag y[OP_BLOCKS][4];
-        float f[4], o[4];
+        for (int q = 0; q < OP_CHUNKS; ++q) {
+          op_frag y[OP_BLOCKS][M];
+          float f[M], o[M];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < M; ++i) {
 #pragma unroll
-          for (int b = 0; b < OP_BLOCKS; ++b) y[b][i] = row16(now, q * OP_BLOCKS + b, i);
-          const int at = ((n & 1) * OP_CHUNKS + q) * OP_ROWS + wm * 64 + i * 16 + l;
-          f[i] = sum[at];
-          if (OP_ZEROS) o[i] = OP_ELT == 1 ? offset[at] : 128.0f * f[i];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int at = (now * OP_CHUNKS + q) * OP_LINE + 16 + wn * 64 + j * 16 + g * 4;
-          const acc_f4 s = *(const acc_f4 *)(scale + at), z = OP_ZEROS ? *(const acc_f4 *)(zero + at) : s;
-          op_frag numbers[OP_BLOCKS];
-#pragma unroll
-          for (int b = 0; b < OP_BLOCKS; ++b) numbers[b] = op_as_frag(op_numbers(w[j][q * OP_BLOCKS + b]));
-          if (q == OP_CHUNKS - 1) load_codes(acc_min(n + 1, steps - 1), j);
-          acc_f4 t[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], o[i], z[r]) : f[i];
-#pragma unroll
-          for (int b = 0; b < OP_BLOCKS; ++b)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) t[i] = op_mfma(numbers[b], y[b][i], t[i]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) c[i][j][r] = __builtin_fmaf(s[r], t[i][r], c[i][j][r]);
-          /* (the next steps' rows and sums amid the products: every wave has some to go on with) */
-          if (q == 0 && j == 0) {
-            put(then);
-            load(acc_min(n + 3, steps - 1));
+            for (int b = 0; b < OP_BLOCKS; ++b) y[b][i] = row16(now, q * OP_BLOCKS + b, i);
+            const int at = ((n & 1) * OP_CHUNKS + q) * OP_ROWS + i * 16 + l;
+            f[i] = sum[at];
+            if (OP_ZEROS) o[i] = OP_ELT == 1 ? offset[at] : 128.0f * f[i];
           }
-          if (q == 0 && j == 1) add_up(next, (n + 1) & 1);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = (now * OP_CHUNKS + q) * OP_LINE + 16 + wave * 64 + j * 16 + g * 4;
+            const acc_f4 s = *(const acc_f4 *)(scale + at), z = OP_ZEROS ? *(const acc_f4 *)(zero + at) : s;
+            op_frag numbers[OP_BLOCKS];
+#pragma unroll
+            for (int b = 0; b < OP_BLOCKS; ++b) numbers[b] = op_as_frag(op_numbers(w[j][q * OP_BLOCKS + b]));
+            if (q == OP_CHUNKS - 1) load_codes(acc_min(n + 1, steps - 1), j);
+            acc_f4 t[M];
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], o[i], z[r]) : f[i];
+#pragma unroll
+            for (int b = 0; b < OP_BLOCKS; ++b)
+#pragma unroll
+              for (int i = 0; i < M; ++i) t[i] = op_mfma(numbers[b], y[b][i], t[i]);
+#pragma unroll
+            for (int i = 0; i < M; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) c[i][j][r] = __builtin_fmaf(s[r], t[i][r], c[i][j][r]);
+            /* (the next steps' rows and sums amid the products: every wave has some to go on with) */
+            if (q == 0 && j == 0) {
+              put(then);
+              load(acc_min(n + 3, steps - 1));
+            }
+            if (q == 0 && j == 1) add_up(next, (n + 1) & 1);
+          }
         }
+        const int was = now;
+        now = next;
+        next = then;
+        then = was;
       }
-      const int was = now;
-      now = next;
-      next = then;
-      then = was;
-    }
+    };
+    if (rows > 32) products(op_count<4>{});
+    else if (rows > 16) products(op_count<2>{});
+    else products(op_count<1>{});
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int m = wm * 64 + i * 16 + l;
+    const int m = i * 16 + l;
     if (m >= rows) continue;
     const bool none = tile.expert < 0 || row_of(m) < 0;
     op_elt *const out = (op_elt *)p.out + (long long)(tile.begin + m) * p.out_stride;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) op_write4(out, j0 + wn * 64 + j * 16 + 4 * g, p.nj, c[i][j], none);
+    for (int j = 0; j < 4; ++j) op_write4(out, j0 + wave * 64 + j * 16 + 4 * g, p.nj, c[i][j], none);
   }
 }
 #else

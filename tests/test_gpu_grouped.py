@@ -120,9 +120,9 @@ def test_products_of_whole_numbers_are_exact(A, ctx, ops, elt, group, with_zeros
 @pytest.mark.parametrize("group,with_zeros", ((32, False), (32, True), (64, True), (128, False), (512, True)))
 @pytest.mark.parametrize("elt", ("half", "bfloat16"))
 def test_many_rows_of_many_matrices(A, ctx, ops, elt, group, with_zeros):
-    """tiles of 128 rows by 256 columns: a last tile of one column, rows and sums that end anywhere, an index, segments of no row"""
+    """tiles of 64 rows by 256 columns: a last tile of one column, rows and sums that end anywhere, an index, segments of no row"""
     rng = np.random.default_rng(group + 7)
-    for case, (rows, experts, n, k) in enumerate(((2000, 25, 900, 300), (1700, 18, 1025, 129), (3000, 40, 300, 1), (1400, 20, 1000, 640), (1500, 19, 784, 95))):
+    for case, (rows, experts, n, k) in enumerate(((2000, 25, 900, 300), (1700, 18, 1025, 129), (3000, 40, 700, 1), (1400, 20, 1000, 640), (1500, 19, 784, 95))):
         q, scales, zeros = matrices(rng, experts, n, k, group, elt, with_zeros, True)
         offsets, per = segments(rng, rows, experts, ("even", "skewed", "gaps")[case % 3]), (0, 1, 3)[case % 3]
         index = None if case % 2 else rng.integers(-2, rows * max(per, 1), rows).astype(np.int32)

@@ -37,12 +37,12 @@ def hip():
     return h
 
 
-@pytest.mark.parametrize("tokens", (5, 90, 1300))
-def test_routed_products_recorded_into_graphs(A, hip, tokens):
+@pytest.mark.parametrize("tokens,n", ((5, 70), (90, 70), (1300, 70), (1300, 700)))
+def test_routed_products_recorded_into_graphs(A, hip, tokens, n):
     """a router, products with the experts' 4-bit matrices through its order (each form of them, by the rows that an expert has), the
     router's gradient: two graphs replayed beside eager calls on a third stream"""
     ctx, rng = A.Context(0), np.random.default_rng(tokens)
-    k, n, e, choose, elt = 200, 70, 8, 2, "bfloat16"
+    k, e, choose, elt = 200, 8, 2, "bfloat16"
     router, product = A.ScoreRouter(ctx, elt, choose, 4, 2), A.Grouped(ctx, elt, 64)
     q, scales, zeros = matrices(rng, e, n, k, 64, elt, True, False)
     codes, scales, zeros = ctx.array(packed(q)), ctx.array(store(scales, elt)), ctx.array(zeros)
@@ -166,6 +166,21 @@ def test_a_recurrence_whose_rows_lie_gigabytes_apart(A, apart, elt):
     op.step(near[0], near[1], small[0], small[0], small[1], index=ctx.array(index))
     ctx.sync()
     assert np.array_equal(table.get(), small[0].get()) and np.array_equal(out.get(), small[1].get())
+    op.destroy()
+
+
+def test_tall_products_whose_arrays_lie_gigabytes_apart(A, apart):
+    """the same in tiles of 64 rows by 256 columns"""
+    ctx, put = apart
+    rng, rows, k, n, e, elt = np.random.default_rng(5), 1300, 300, 1500, 2, "half"
+    q, scales, zeros = matrices(rng, e, n, k, 64, elt, True, True)
+    x, offsets, pitch = rng.integers(-3, 4, (rows, k)).astype(np.float64), np.array([0, rows // 2, rows], np.int32), (6 << 30) // rows // 16 * 8
+    want, _ = expected(x, weights(q, scales, zeros, 64), offsets, rows, None, 0)
+    op = A.Grouped(ctx, elt, 64)
+    bx, out = put(store(x, elt), pitch, 0), put(store(np.zeros((rows, n)), elt), pitch, 4096)
+    op.rows(bx.array, put(packed(q), 5 << 30, 7 << 30).array, put(store(scales, elt), 5 << 29, 18 << 30).array, ctx.array(offsets), out.array, zeros=put(zeros, 5 << 30, 30 << 30).array)
+    ctx.sync()
+    assert np.array_equal(out.get(), store(want, elt))
     op.destroy()
 
 
