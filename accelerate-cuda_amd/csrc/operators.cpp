@@ -344,7 +344,7 @@ std::vector<std::string> all_sources(const OpSpec &sp)
     v.tall = true;
     for (bool zeros : {false, true}) {
       v.zeros = zeros;
-      if (sp.type != 0) out.push_back(grouped_source(sp, v));
+      out.push_back(grouped_source(sp, v));
     }
     v = {};
     v.elements = true;
@@ -638,36 +638,41 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
 }
 
 // grouped: from how many rows a segment on the matrices are made again for tiles that use them often.  us, as they are and made again:
-// 160 rows, 2 of 4096 x 4096: 41 and 53; Float32, 64, 16 of 1024 x 2048: 12 and 45
+// 160 rows, 2 of 4096 x 4096: 43 and 53; 300, 1: 60 and 46; Float32, 400, 4 of 1024 x 2048: 23 and 43
 constexpr int64_t kGroupedMost = 128;
 // ... LDS of the form with rows in it: `height` of them, their sums by groups, and the waves' results where they share columns
 int64_t grouped_lds(const OpSpec &sp, int64_t height, int64_t steps, int64_t waves)
 {
   const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
-  return steps * height * (256 * (sp.type == 0 ? 3 : 1) + chunks * (sp.type == 1 ? 8 : 4)) + waves * ceil_div(height, 16) * 1024;
+  return steps * height * (256 * (sp.type == 0 ? 3 : 1) + chunks * (sp.type == 2 ? 4 : 8)) + waves * ceil_div(height, 16) * 1024;
 }
 constexpr int64_t kGroupedLds = 160 << 10;
 // ... and of tiles of 64 rows by 256 columns: three steps of rows, scales and zeros, two of sums
 int64_t grouped_tall_lds(const OpSpec &sp, bool zeros)
 {
   const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
-  return 3 * 16 * 64 * 16 + 3 * chunks * 272 * 4 * (zeros ? 2 : 1) + 2 * chunks * 64 * 4 * (zeros && sp.type == 1 ? 2 : 1);
+  const int64_t rows = sp.type == 0 ? 32 : 64, parts = sp.type == 0 ? 3 : 1;
+  return 3 * 16 * parts * rows * 16 + 3 * chunks * 272 * 4 * (zeros ? 2 : 1) + 2 * chunks * rows * 4 * (sp.type == 0 || (zeros && sp.type == 1) ? 2 : 1);
 }
 // ... and the tiles of 16 columns from which on rows in LDS are worth what it takes to put them there.  us, with and without, tiles: 1 row,
 // 4096 x 4096, 256: 8.2 and 7.2; 16 rows: 14 and 11; 2 rows of 4096 x 11008, 256: 16 and 15; of 11008 x 4096, 688: 13 and 18; 1 row, 8192 x 8192,
 // 512: 16 and 23; 64 rows, 16 half of 4096 x 2048, 4096: 23 and 34; 16, 8 of 4096 x 4096 in groups of 32: 29 and 44; Float32, 64, 16 of
 // 1024 x 2048, 1024: 14 and 12
 constexpr int64_t kGroupedStream = 384;
-// Whether a call is for tiles of 64 rows by 256 columns that make numbers of the codes as they go: rows enough for them, tiles enough
+// Whether a call is for tiles of 64 rows (Float32: 32) by 256 columns that make numbers of the codes as they go: rows enough for them, tiles enough
 // (one that is 4096 long takes 55 us, however few there are), and not so many rows a matrix that making it again is little beside its
 // products.  us, with and without, rows (a few more or less a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 60 and 75; 2048, 8,
 // 512: 124 and 223, in groups of 32 with zeros 211 and 246; 4096, 8, 1024: 188 and 296, in groups of 32 335 and 316; 8192, 8, 2048: 326 and
 // 402; 300, 1, 80: 56 and 45; 700, 1, 176: 59 and 66; 2000, 1, 512: 97 and 85; 300, 3, 80: 59 and 66; 160, 2, 48: 54 and 43; 900, 4 of
-// 2000 x 1000, 120: 26 and 32; 1600, 20 of 1000 x 1000, 100: 28 and 32; 1000, 20 of 500 x 2000, 40: 46 and 25
+// 2000 x 1000, 120: 26 and 32; 1600, 20 of 1000 x 1000, 100: 28 and 32; 1000, 20 of 500 x 2000, 40: 46 and 25.  Float32, whose products
+// are then those of three bfloat16 parts in place of its own instructions', a third as fast: 4096, 8 of 4096 x 4096, 2048: 395 and 1177;
+// 1000, 1, 512: 105 and 263; 300, 8 in groups of 32, 160: 102 and 168; 600, 4 of 1024 x 2048, 76: 36 and 43; 400, 4, 52: 35 and 23; 100, 1
+// of 4096 x 4096, 64: 64 and 38
 bool grouped_tall(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean)
 {
-  return sp.type != 0 && n >= 16 && k > 0 && pitch < (1 << 26) && mean > 32 && mean <= (sp.group >= 64 ? 1024 : 256) &&
-         std::max(ceil_div(rows, 64), std::min(rows, experts)) * ceil_div(n, 256) >= 96;
+  const bool wide = sp.type == 0;
+  const int64_t tiles = std::max(ceil_div(rows, wide ? 32 : 64), std::min(rows, experts)) * ceil_div(n, 256);
+  return n >= 16 && k > 0 && pitch < (1 << 26) && mean > 32 && (wide || mean <= (sp.group >= 64 ? 1024 : 256)) && tiles >= (wide ? 72 : 96);
 }
 // the tile for `mean` rows a segment; *height: its rows.  (Where LDS holds fewer rows than a segment has, their codes are read again:
 // 64 rows, 2 of 4096 x 4096: 18 us in tiles of 16, 26 without LDS.)
@@ -1756,7 +1761,7 @@ try {
   GroupedVariant v;
   if (tall) {
     v.tall = true;
-    height = 64;
+    height = op->spec.type == 0 ? 32 : 64;
   } else {
     v = grouped_variant(op->spec, rows, experts, n, k, codes->stride[1], mean, &height);
   }

@@ -195,6 +195,24 @@ extern "C" __global__ void __launch_bounds__(256) grouped_values(const acc_group
 /* what products of a group begin with, -(z sum x + sum d x), in column r */
 ACC_DEV float op_begin(const float sum, const float offset, const float zero) { return __builtin_fmaf(-zero, sum, -offset); }
 
+/* the sums behind that, of 16 rows: sum x; and of half rows sum d x, of Float32 ones (whose `sum` is the first part's) the other parts' */
+template <typename F> ACC_DEV void op_sums(const int q, F fragment, acc_f4 &sum, acc_f4 &second)
+{
+  const op_frag ones = op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES});
+  sum = second = acc_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
+    const op_frag y = fragment(b, 0);
+    sum = op_mfma(ones, y, sum);
+    if (OP_ELT == 1) second = op_mfma(op_as_frag(op_offsets()), y, second);
+#pragma unroll
+    for (int part = OP_PARTS - 1; part > 0; --part) second = op_mfma(ones, fragment(b, part), second);
+  }
+}
+ACC_DEV float op_offset(const float sum, const float second) { return OP_ELT == 1 ? second : (OP_ELT == 2 ? 128.0f : 16.0f) * sum; }
+/* of Float32 rows: the other parts' beginning, behind their products */
+ACC_DEV float op_rest(const float t, const float second, const float zero) { return OP_ELT == 0 ? t + op_begin(second, 16.0f * second, zero) : t; }
+
 #if OP_STREAM
 /* The form whose rows lie in LDS, cut and in the order of fragments, with their sums by groups: p.height rows of a tile (a power of
  * two up to 16, or 16 OP_FM).  A wave goes over columns, 16 at a time, or over a part of k of the same columns as its neighbours where
@@ -217,8 +235,8 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
   const bool sums = tile.expert >= 0 && p.x_rows > 0 && steps > 0;
   acc_u4 *const notes = shared;                    /* [waves][OP_FM][64]: a wave's scales and zeros; its sums, where they meet */
   acc_u4 *const x = notes + OP_WAVES * OP_FM * 64; /* [steps][4][parts][4][height] */
-  float *const sum = (float *)(x + steps * 16 * OP_PARTS * height);       /* [steps][chunks][height], and of half the offsets' */
-  float *const offset = OP_ELT == 1 ? sum + steps * OP_CHUNKS * height : sum;
+  float *const sum = (float *)(x + steps * 16 * OP_PARTS * height);       /* [steps][chunks][height], and the second ones */
+  float *const offset = OP_ELT != 2 ? sum + steps * OP_CHUNKS * height : sum;
   const auto row_of = [&](const int i) { return p.index ? op_listed(p.index, tile.begin + i, tile.begin, tile.end, p.x_rows, p.per_mul, p.per_shift) : tile.begin + i; };
   const auto write = [&](const int jt, const acc_f4 (&c)[OP_FM]) {
 #pragma unroll
@@ -276,21 +294,27 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
         }
       }
       acc_f4 t[OP_FM];
+      float second[OP_FM];
 #pragma unroll
       for (int i = 0; i < OP_FM; ++i) {
         const int place = (n * OP_CHUNKS + q) * height + ((i * 16 + l) & (height - 1));
-        const float f = sum[place], d = OP_ELT == 1 ? offset[place] : (OP_ELT == 2 ? 128.0f : 16.0f) * f;
+        const float f = sum[place];
+        second[i] = OP_ELT != 2 ? offset[place] : 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, d, OP_ZEROS ? (float)z.v[r] : 8.0f);
+        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, op_offset(f, second[i]), OP_ZEROS ? (float)z.v[r] : 8.0f);
       }
 #pragma unroll
-      for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
-        const op_frag v = op_as_frag(op_numbers(w[b]));
+      for (int part = 0; part < OP_PARTS; ++part)
 #pragma unroll
-        for (int i = 0; i < OP_FM; ++i)
+        for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
+          const op_frag v = op_as_frag(op_numbers(w[b]));
 #pragma unroll
-          for (int part = OP_PARTS - 1; part >= 0; --part) t[i] = op_mfma(v, op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]), t[i]);
-      }
+          for (int i = 0; i < OP_FM; ++i) t[i] = op_mfma(v, op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]), t[i]);
+        }
+#pragma unroll
+      for (int i = 0; i < OP_FM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[i][r] = op_rest(t[i][r], second[i], OP_ZEROS ? (float)z.v[r] : 8.0f);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -324,19 +348,12 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
     for (int q = 0; q < OP_CHUNKS; ++q)
 #pragma unroll
       for (int i = 0; i < OP_FM; ++i) {
-        acc_f4 t = {0.0f, 0.0f, 0.0f, 0.0f}, d = t;
-#pragma unroll
-        for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b)
-#pragma unroll
-          for (int part = OP_PARTS - 1; part >= 0; --part) {
-            const op_frag y = op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]);
-            t = op_mfma(op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), y, t);
-            if (OP_ELT == 1) d = op_mfma(op_as_frag(op_offsets()), y, d);
-          }
+        acc_f4 t, d;
+        op_sums(q, [&](const int b, const int part) { return op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]); }, t, d);
         const int at = (n * OP_CHUNKS + q) * height + i * 16 + l;
         if (g == 0 && i * 16 + l < height) {
           sum[at] = t[0];
-          if (OP_ELT == 1) offset[at] = d[0];
+          if (OP_ELT != 2) offset[at] = d[0];
         }
       }
   __syncthreads();
@@ -387,12 +404,15 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
     }
 }
 #elif OP_WIDE
-/* The form for many rows of a matrix: tiles of 128 rows by 256 columns, eight waves of 64 by 64.  The rows of a step of 128 lie in LDS,
- * three steps at a time: the one whose products are taken, the next one, whose sums by groups are taken meanwhile (of 16 rows by each of
- * the four waves that share them), and the one after that, on its way there.  A wave makes its 64 columns' codes into numbers itself,
- * in registers. */
-#define OP_ROWS 64
+/* The form for many rows of a matrix: tiles of 64 rows (of Float32: 32, in three parts) by 256 columns, four waves of 64 of them, two
+ * workgroups a compute unit.  The rows of a step of 128 lie in LDS, three steps at a time: the one whose products are taken, the next
+ * one, whose sums by groups are taken meanwhile (of 16 rows by a wave), and the one after that, on its way there.  A wave makes its 64
+ * columns' codes into numbers itself, in registers: 16 columns' are used for all rows. */
+#define OP_PER (OP_ELT == 0 ? 2 : 4)               /* rows of a tile, in sixteens */
+#define OP_ROWS (16 * OP_PER)
+#define OP_SIZE ((int)sizeof(op_elt))
 #define OP_COLUMNS 256
+#define OP_SECOND (OP_ELT == 0 || (OP_ELT == 1 && OP_ZEROS))
 #define OP_LINE (OP_COLUMNS + 16)                  /* scales (zeros) of a group: 16 places in front, for a tile with fewer columns */
 
 template <int N> struct op_count { static constexpr int value = N; };
@@ -405,81 +425,79 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
   const op_tile tile = op_find_tile<OP_ALL>(p.offsets, p.experts, (int)p.rows, OP_ROWS, op_segments(p.offsets, p.experts, (int)p.rows, 0, 0), (int)(blockIdx.x / p.tiles_j));
   if (tile.begin >= tile.end) return;
   const int steps = (p.blocks + 3) / 4, rows = tile.end - tile.begin, j0 = (int)(blockIdx.x % p.tiles_j) * OP_COLUMNS;
-  acc_u4 *const x = shared;                        /* [3][16][OP_ROWS]: eight neighbours of a row, a row's places turned by their number */
-  float *const scale = (float *)(x + 3 * 16 * OP_ROWS);                    /* [3][chunks][OP_LINE], and the zeros' */
+  acc_u4 *const x = shared;                        /* [3][16][parts][OP_ROWS]: eight neighbours of a row, a row's places turned by their number */
+  float *const scale = (float *)(x + 3 * 16 * OP_PARTS * OP_ROWS);         /* [3][chunks][OP_LINE], and the zeros' */
   float *const zero = scale + 3 * OP_CHUNKS * OP_LINE;
   float *const sum = OP_ZEROS ? zero + 3 * OP_CHUNKS * OP_LINE : zero;     /* [2][chunks][OP_ROWS]; what products begin with, where zeros are 8 */
-  float *const offset = sum + 2 * OP_CHUNKS * OP_ROWS;                     /* the same, of half rows with zeros */
-  acc_f4 c[4][4];
+  float *const offset = sum + 2 * OP_CHUNKS * OP_ROWS;                     /* the second ones, where products want them */
+  acc_f4 c[OP_PER][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < OP_PER; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) c[i][j] = acc_f4{0.0f, 0.0f, 0.0f, 0.0f};
   const auto row_of = [&](const int m) { return p.index ? op_listed(p.index, tile.begin + m, tile.begin, tile.end, p.x_rows, p.per_mul, p.per_shift) : tile.begin + acc_min(m, rows - 1); };
 
   if (tile.expert >= 0 && p.x_rows > 0 && steps > 0) {
-    /* a lane's places among the rows: eight neighbours, of four rows 16 apart */
-    const int chunk = tid & 15, first = tid >> 4, place = ((OP_CHUNKS > 1 ? chunk : chunk % 4 * 4 + chunk / 4) * OP_ROWS) + (first ^ (chunk & 7));
-    const op_elt *from[4];
+    /* a lane's places among the rows: eight neighbours, of rows 16 apart */
+    const int chunk = tid & 15, first = tid >> 4, place = ((OP_CHUNKS > 1 ? chunk : chunk % 4 * 4 + chunk / 4) * OP_PARTS * OP_ROWS) + (first ^ (chunk & 7));
+    const op_elt *from[OP_PER];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 16 * u), 0) * p.x_stride + chunk * 8;
-    /* ... and among the scales and zeros: of 8, or of 16 columns (of the last: as many as there are) */
-    const bool scale_lane = tid < OP_CHUNKS * 32;
-    const int noted = scale_lane ? tid / 32 : (tid - OP_CHUNKS * 32) / 16 % OP_CHUNKS, at_column = acc_min(j0 + (scale_lane ? tid % 32 * 8 : tid % 16 * 16), p.nj - (scale_lane ? 8 : 16));
-    const unsigned char *const notes = scale_lane || !OP_ZEROS ? (const unsigned char *)((const op_elt *)p.scales + tile.expert * p.scales_expert + (scale_lane ? at_column : 0))
-                                                               : (const unsigned char *)p.zeros + tile.expert * p.zeros_expert + at_column;
-    const long long note_stride = scale_lane || !OP_ZEROS ? p.scales_stride * (long long)sizeof(op_elt) : p.zeros_stride;
-    acc_u4 v[4], note;
+    for (int u = 0; u < OP_PER; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 16 * u), 0) * p.x_stride + chunk * 8;
+    /* ... and among the scales and zeros: 16 bytes of a group's (of the last columns: as many as there are) */
+    constexpr int wide = 16 / OP_SIZE, lanes = OP_COLUMNS / wide;
+    const int scale_at = acc_min(j0 + tid % lanes * wide, p.nj - wide), zero_at = acc_min(j0 + tid % 16 * 16, p.nj - 16);
+    const op_elt *const scales = (const op_elt *)p.scales + tile.expert * p.scales_expert + scale_at;
+    const unsigned char *const zeros = (const unsigned char *)p.zeros + tile.expert * p.zeros_expert + zero_at;
+    op_eight v[OP_PER];
+    acc_u4 scale_note, zero_note;
     const auto load = [&](const int n) {
-      const int group = acc_min(((n * 128) >> p.group_shift) + noted, p.groups - 1);
-      note = ((const op_loose<unsigned char> *)(notes + group * note_stride))->v;
+      const int group = (n * 128) >> p.group_shift;
+      scale_note = ((const op_loose<op_elt> *)(scales + acc_min(group + tid / lanes % OP_CHUNKS, p.groups - 1) * p.scales_stride))->v;
+      if (OP_ZEROS) zero_note = ((const op_loose<unsigned char> *)(zeros + acc_min(group + tid / 16 % OP_CHUNKS, p.groups - 1) * p.zeros_stride))->v;
       if (n * 128 + 128 <= p.k) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = ((const op_loose<op_elt> *)(from[u] + n * 128))->v;
+        for (int u = 0; u < OP_PER; ++u) v[u] = op_row8(from[u] + n * 128, 8);
       } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = op_chunk<false>(from[u] + n * 128, p.k - n * 128 - chunk * 8);
+        for (int u = 0; u < OP_PER; ++u) v[u] = op_row8(from[u] + n * 128, p.k - n * 128 - chunk * 8);
       }
     };
     const auto put = [&](const int to) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        acc_u4 part[1];
-        op_parts(op_eight{{v[u]}}, part);
-        x[to * 16 * OP_ROWS + place + 16 * u] = part[0];
+      for (int u = 0; u < OP_PER; ++u) {
+        acc_u4 parts[OP_PARTS];
+        op_parts(v[u], parts);
+#pragma unroll
+        for (int part = 0; part < OP_PARTS; ++part) x[(to * 16 * OP_PARTS + part) * OP_ROWS + place + 16 * u] = parts[part];
       }
-      if (scale_lane) {
-        op_elt e[8];
-        __builtin_memcpy(e, &note, 16);
-        float *const line = scale + (to * OP_CHUNKS + noted) * OP_LINE + 16 + (at_column - j0);
+      if (tid < OP_CHUNKS * lanes) {
+        op_elt e[wide];
+        __builtin_memcpy(e, &scale_note, 16);
+        float *const line = scale + (to * OP_CHUNKS + tid / lanes) * OP_LINE + 16 + (scale_at - j0);
 #pragma unroll
-        for (int t = 0; t < 8; ++t) line[t] = (float)e[t];
-      } else if (OP_ZEROS && tid < OP_CHUNKS * 48) {
-        float *const line = zero + (to * OP_CHUNKS + noted) * OP_LINE + 16 + (at_column - j0);
+        for (int t = 0; t < wide; ++t) line[t] = (float)e[t];
+      }
+      if (OP_ZEROS && tid < OP_CHUNKS * 16) {
+        float *const line = zero + (to * OP_CHUNKS + tid / 16) * OP_LINE + 16 + (zero_at - j0);
 #pragma unroll
-        for (int t = 0; t < 16; ++t) line[t] = (float)(note[t / 4] >> t % 4 * 8 & 255u);
+        for (int t = 0; t < 16; ++t) line[t] = (float)(zero_note[t / 4] >> t % 4 * 8 & 255u);
       }
     };
     /* the lane's fragment of rows 16 i on of a wave's */
-    const auto row16 = [&](const int buffer, const int b, const int i) {
+    const auto row16 = [&](const int buffer, const int b, const int i, const int part) {
       const int turn = (OP_CHUNKS > 1 ? 4 * b + g : 4 * g + b) & 7;
-      return op_as_frag(x[buffer * 16 * OP_ROWS + (b * 4 + g) * OP_ROWS + i * 16 + (l ^ turn)]);
+      return op_as_frag(x[((buffer * 16 + b * 4 + g) * OP_PARTS + part) * OP_ROWS + i * 16 + (l ^ turn)]);
     };
     const auto add_up = [&](const int buffer, const int slot) {
+      if (wave >= OP_PER) return;
 #pragma unroll
       for (int q = 0; q < OP_CHUNKS; ++q) {
-        acc_f4 t = {0.0f, 0.0f, 0.0f, 0.0f}, d = t;
-#pragma unroll
-        for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
-          const op_frag y = row16(buffer, b, wave);
-          t = op_mfma(op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), y, t);
-          if (OP_ELT == 1) d = op_mfma(op_as_frag(op_offsets()), y, d);
-        }
+        acc_f4 t, d;
+        op_sums(q, [&](const int b, const int part) { return row16(buffer, b, wave, part); }, t, d);
         const int at = (slot * OP_CHUNKS + q) * OP_ROWS + wave * 16 + l;
-        const float o = OP_ELT == 1 ? d[0] : 128.0f * t[0];
         if (g == 0) {
-          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], o, 8.0f);
-          if (OP_ZEROS && OP_ELT == 1) offset[at] = o;
+          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], op_offset(t[0], d[0]), 8.0f);
+          if (OP_SECOND) offset[at] = d[0];
         }
       }
     };
@@ -515,15 +533,17 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
         for (int j = 0; j < 4; ++j) op_turn(w[j]);
 #pragma unroll
         for (int q = 0; q < OP_CHUNKS; ++q) {
-          op_frag y[OP_BLOCKS][M];
+          op_frag y[OP_BLOCKS][M][OP_PARTS];
           float f[M], o[M];
 #pragma unroll
           for (int i = 0; i < M; ++i) {
 #pragma unroll
-            for (int b = 0; b < OP_BLOCKS; ++b) y[b][i] = row16(now, q * OP_BLOCKS + b, i);
+            for (int b = 0; b < OP_BLOCKS; ++b)
+#pragma unroll
+              for (int part = 0; part < OP_PARTS; ++part) y[b][i][part] = row16(now, q * OP_BLOCKS + b, i, part);
             const int at = ((n & 1) * OP_CHUNKS + q) * OP_ROWS + i * 16 + l;
             f[i] = sum[at];
-            if (OP_ZEROS) o[i] = OP_ELT == 1 ? offset[at] : 128.0f * f[i];
+            o[i] = OP_SECOND ? offset[at] : 0.0f;
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -537,15 +557,17 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], o[i], z[r]) : f[i];
+              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], op_offset(f[i], o[i]), z[r]) : f[i];
 #pragma unroll
-            for (int b = 0; b < OP_BLOCKS; ++b)
+            for (int part = 0; part < OP_PARTS; ++part)
 #pragma unroll
-              for (int i = 0; i < M; ++i) t[i] = op_mfma(numbers[b], y[b][i], t[i]);
+              for (int b = 0; b < OP_BLOCKS; ++b)
+#pragma unroll
+                for (int i = 0; i < M; ++i) t[i] = op_mfma(numbers[b], y[b][i][part], t[i]);
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) c[i][j][r] = __builtin_fmaf(s[r], t[i][r], c[i][j][r]);
+              for (int r = 0; r < 4; ++r) c[i][j][r] = __builtin_fmaf(s[r], op_rest(t[i][r], o[i], OP_ZEROS ? z[r] : 8.0f), c[i][j][r]);
             /* (the next steps' rows and sums amid the products: every wave has some to go on with) */
             if (q == 0 && j == 0) {
               put(then);
@@ -560,12 +582,12 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
         then = was;
       }
     };
-    if (rows > 32) products(op_count<4>{});
+    if (OP_PER > 2 && rows > 32) products(op_count<OP_PER>{});
     else if (rows > 16) products(op_count<2>{});
     else products(op_count<1>{});
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < OP_PER; ++i) {
     const int m = i * 16 + l;
     if (m >= rows) continue;
     const bool none = tile.expert < 0 || row_of(m) < 0;
@@ -641,12 +663,12 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
       for (int j = 0; j < OP_FN; ++j) op_turn(s.w[j]);
 #pragma unroll
       for (int q = 0; q < OP_CHUNKS; ++q) {
-        acc_f4 t[OP_FM][OP_FN], sum[OP_FM], offset[OP_FM];
+        acc_f4 t[OP_FM][OP_FN], rest[OP_FM][OP_FN], sum[OP_FM], second[OP_FM];      /* rest: of Float32's other parts */
 #pragma unroll
         for (int i = 0; i < OP_FM; ++i) {
-          sum[i] = offset[i] = none;
+          sum[i] = second[i] = none;
 #pragma unroll
-          for (int j = 0; j < OP_FN; ++j) t[i][j] = none;
+          for (int j = 0; j < OP_FN; ++j) t[i][j] = rest[i][j] = none;
         }
 #pragma unroll
         for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
@@ -660,10 +682,14 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
 #pragma unroll
             for (int n = OP_PARTS - 1; n >= 0; --n) {
               const op_frag y = op_as_frag(part[n]);
-              sum[i] = op_mfma(ones, y, sum[i]);
-              if (OP_ELT == 1) offset[i] = op_mfma(offsets, y, offset[i]);
+              acc_f4 &sums = n == 0 ? sum[i] : second[i];
+              sums = op_mfma(ones, y, sums);
+              if (OP_ELT == 1) second[i] = op_mfma(offsets, y, second[i]);
 #pragma unroll
-              for (int j = 0; j < OP_FN; ++j) t[i][j] = op_mfma(v[j], y, t[i][j]);
+              for (int j = 0; j < OP_FN; ++j) {
+                acc_f4 &to = n == 0 ? t[i][j] : rest[i][j];
+                to = op_mfma(v[j], y, to);
+              }
             }
           }
         }
@@ -673,8 +699,10 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
           for (int r = 0; r < 4; ++r) {
             const float scale = (float)s.s[q][j].v[r], zero = OP_ZEROS ? (float)s.z[q][j].v[r] : 8.0f;
 #pragma unroll
-            for (int i = 0; i < OP_FM; ++i)
-              c[i][j][r] = __builtin_fmaf(scale, t[i][j][r] + op_begin(sum[i][r], OP_ELT == 1 ? offset[i][r] : (OP_ELT == 2 ? 128.0f : 16.0f) * sum[i][r], zero), c[i][j][r]);
+            for (int i = 0; i < OP_FM; ++i) {
+              const float first = t[i][j][r] + op_begin(sum[i][r], op_offset(sum[i][r], second[i][r]), zero);
+              c[i][j][r] = __builtin_fmaf(scale, OP_ELT == 0 ? first + op_rest(rest[i][j][r], second[i][r], zero) : first, c[i][j][r]);
+            }
           }
       }
     };

@@ -94,8 +94,8 @@ hipError_t hipModuleLaunchKernel(hipFunction_t f, unsigned gx, unsigned gy, unsi
     if (a.tiles_i < least) not_so("fewer tiles than segments may have", a.tiles_i, least);
     if (a.run == 16 && bx == 256) {
       ++g_tall;
-      const int64_t chunks = a.group >= 128 ? 1 : 128 / a.group, need = 3 * (16 * 64 * 16 + chunks * 272 * 4 * (a.zeros ? 2 : 1)) + 2 * chunks * 64 * 4 * (a.zeros ? 2 : 1);
-      if (a.height != 64 || a.nj < 16 || a.codes_stride * 63 + 64 > 0xffffffffll || (int64_t)lds > need || (int64_t)lds < need - 2 * chunks * 64 * 4) not_so("LDS of the tall tiles", lds, need);
+      const int64_t chunks = a.group >= 128 ? 1 : 128 / a.group, rows = g_element == 4 ? 32 : 64, need = 3 * (16 * rows * (g_element == 4 ? 3 : 1) * 16 + chunks * 272 * 4 * (a.zeros ? 2 : 1)) + 2 * chunks * rows * 4 * (a.zeros || g_element == 4 ? 2 : 1);
+      if (a.height != rows || a.nj < 16 || a.codes_stride * 63 + 64 > 0xffffffffll || (int64_t)lds > need || (int64_t)lds < need - 2 * chunks * rows * 4) not_so("LDS of the tall tiles", lds, need);
     } else if (bx >= 512 && lds) {
       ++g_stream;
       const int64_t chunks = a.group >= 128 ? 1 : 128 / a.group, waves = bx / 64, rows = (a.height + 15) / 16;

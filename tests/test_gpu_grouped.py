@@ -118,9 +118,9 @@ def test_products_of_whole_numbers_are_exact(A, ctx, ops, elt, group, with_zeros
 
 
 @pytest.mark.parametrize("group,with_zeros", ((32, False), (32, True), (64, True), (128, False), (512, True)))
-@pytest.mark.parametrize("elt", ("half", "bfloat16"))
+@pytest.mark.parametrize("elt", TYPES)
 def test_many_rows_of_many_matrices(A, ctx, ops, elt, group, with_zeros):
-    """tiles of 64 rows by 256 columns: a last tile of one column, rows and sums that end anywhere, an index, segments of no row"""
+    """tiles of 64 rows (Float32: 32) by 256 columns: a last tile of one column, rows and sums that end anywhere, an index, segments of no row"""
     rng = np.random.default_rng(group + 7)
     for case, (rows, experts, n, k) in enumerate(((2000, 25, 900, 300), (1700, 18, 1025, 129), (3000, 40, 700, 1), (1400, 20, 1000, 640), (1500, 19, 784, 95))):
         q, scales, zeros = matrices(rng, experts, n, k, group, elt, with_zeros, True)
