@@ -8,34 +8,43 @@
  * with a d that its place in the word decides (half: 1024, 64; bfloat16: 128; for Float32 rows 16); the matrix cores add up x (d + q)
  * over what a group has of a step, beginning with -(z sum x + sum d x), and that times s is added up in Float32: no weight is ever
  * rounded.  What is taken off again costs some of the 24 bits of a sum: of half ones eight of those beyond a 4-bit number's own, in
- * bfloat16 five, Float32 two.  Float32 rows are cut into three bfloat16 each, which hold all 24 bits.  (An infinity in a row makes the
- * row's results NaN.)
+ * bfloat16 five: a small part of what the result's rounding costs.  Float32 rows are cut into three bfloat16 each, which hold all 24 bits;
+ * the first parts, 8 bits each, are added up and what is too much of them taken off before the others come, which is exact or nearly so
+ * (150 rows of 12 matrices of 1333 x 1001 in groups of 32: 1.2e-7 off; all at once 6e-7, and up to 1.4e-6 at other sizes; it costs 4 us of
+ * 26).  (An infinity in a row makes the row's results NaN.)
  *
  * What counts is that the matrices pass by once, and that their codes are nearly all that is read.  A lane loads 16 bytes of them, 32
  * numbers of a row.  Where a matrix has many columns for a compute unit, the rows lie in LDS and waves go over the columns (OP_STREAM);
  * where it has few, what counts is how soon all of it is on its way, and the waves of a workgroup take every so many steps of the same
  * 16 OP_FN columns and add up what they have by way of LDS, in order.  64 half rows, 16 matrices of 4096 x 2048 in groups of 64 with
- * zeros: 23 us, of which the codes' loads alone take 13 (5.8 TB/s), what is in front of them 8 with the launch; bfloat16 in groups of 128,
- * 16 rows, 8 of 4096 x 4096: 19 us; 1 row, 1 of 4096 x 4096: 7.2.
+ * zeros: 22 us, of which the codes' loads alone take 13 (5.8 TB/s), what is in front of them 8 with the launch; bfloat16 in groups of 128,
+ * 16 rows, 8 of 4096 x 4096: 19 us; 1 row, 1 of 4096 x 4096: 6.4.  Many rows are matter for the matrix cores (OP_WIDE).
  */
 #include "op_matrix.h"
 
 #define OP_FM (OP_BM / 16)
 
+/* a constant in a register of the lanes' (an instruction takes one of two constants only from elsewhere, and "and, or" is one then) */
+ACC_DEV unsigned int op_lane_word(unsigned int v)
+{
+  asm("" : "+v"(v));
+  return v;
+}
 /* 8 codes as d + q: of neighbours 0 4, 1 5, 2 6, 3 7; and the d alone */
 #if OP_ELT == 1
 #define OP_ONES 0x3C003C00u
 ACC_DEV acc_u4 op_numbers(const unsigned int w)
 {
-  const unsigned int v = w >> 8;
-  return acc_u4{(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x54005400u, (v & 0x000F000Fu) | 0x64006400u, (v & 0x00F000F0u) | 0x54005400u};
+  const unsigned int v = w >> 8, a = op_lane_word(0x64006400u), b = op_lane_word(0x54005400u);
+  return acc_u4{(w & 0x000F000Fu) | a, (w & 0x00F000F0u) | b, (v & 0x000F000Fu) | a, (v & 0x00F000F0u) | b};
 }
 ACC_DEV acc_u4 op_offsets() { return acc_u4{0x64006400u, 0x54005400u, 0x64006400u, 0x54005400u}; }
 #elif OP_ELT == 2
 #define OP_ONES 0x3F803F80u
 ACC_DEV acc_u4 op_numbers(const unsigned int w)
 {
-  const auto at = [](const unsigned int v) { return (v & 0x000F000Fu) | 0x43004300u; };
+  const unsigned int d = op_lane_word(0x43004300u);
+  const auto at = [d](const unsigned int v) { return (v & 0x000F000Fu) | d; };
   return acc_u4{at(w), at(w >> 4), at(w >> 8), at(w >> 12)};
 }
 ACC_DEV acc_u4 op_offsets() { return acc_u4{0x43004300u, 0x43004300u, 0x43004300u, 0x43004300u}; }
@@ -43,7 +52,8 @@ ACC_DEV acc_u4 op_offsets() { return acc_u4{0x43004300u, 0x43004300u, 0x43004300
 #define OP_ONES 0x3F803F80u
 ACC_DEV acc_u4 op_numbers(const unsigned int w)
 {
-  const auto at = [](const unsigned int v) { return (v & 0x00780078u) | 0x41804180u; };
+  const unsigned int d = op_lane_word(0x41804180u);
+  const auto at = [d](const unsigned int v) { return (v & 0x00780078u) | d; };
   return acc_u4{at(w << 3), at(w >> 1), at(w >> 5), at(w >> 9)};
 }
 ACC_DEV acc_u4 op_offsets() { return acc_u4{0x41804180u, 0x41804180u, 0x41804180u, 0x41804180u}; }
@@ -192,8 +202,9 @@ extern "C" __global__ void __launch_bounds__(256) grouped_values(const acc_group
 }
 #else
 
-/* what products of a group begin with, -(z sum x + sum d x), in column r */
-ACC_DEV float op_begin(const float sum, const float offset, const float zero) { return __builtin_fmaf(-zero, sum, -offset); }
+/* what products of a group begin with, -(z sum x + sum d x): d is in `second`, or the same for all (OP_D) */
+#define OP_D (OP_ELT == 2 ? 128.0f : 16.0f)
+ACC_DEV float op_begin(const float sum, const float second, const float zero) { return OP_ELT == 1 ? __builtin_fmaf(-zero, sum, -second) : -(zero + OP_D) * sum; }
 
 /* the sums behind that, of 16 rows: sum x; and of half rows sum d x, of Float32 ones (whose `sum` is the first part's) the other parts' */
 template <typename F> ACC_DEV void op_sums(const int q, F fragment, acc_f4 &sum, acc_f4 &second)
@@ -209,9 +220,8 @@ template <typename F> ACC_DEV void op_sums(const int q, F fragment, acc_f4 &sum,
     for (int part = OP_PARTS - 1; part > 0; --part) second = op_mfma(ones, fragment(b, part), second);
   }
 }
-ACC_DEV float op_offset(const float sum, const float second) { return OP_ELT == 1 ? second : (OP_ELT == 2 ? 128.0f : 16.0f) * sum; }
 /* of Float32 rows: the other parts' beginning, behind their products */
-ACC_DEV float op_rest(const float t, const float second, const float zero) { return OP_ELT == 0 ? t + op_begin(second, 16.0f * second, zero) : t; }
+ACC_DEV float op_rest(const float t, const float second, const float zero) { return OP_ELT == 0 ? __builtin_fmaf(-(zero + OP_D), second, t) : t; }
 
 #if OP_STREAM
 /* The form whose rows lie in LDS, cut and in the order of fragments, with their sums by groups: p.height rows of a tile (a power of
@@ -301,7 +311,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
         const float f = sum[place];
         second[i] = OP_ELT != 2 ? offset[place] : 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, op_offset(f, second[i]), OP_ZEROS ? (float)z.v[r] : 8.0f);
+        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, second[i], OP_ZEROS ? (float)z.v[r] : 8.0f);
       }
 #pragma unroll
       for (int part = 0; part < OP_PARTS; ++part)
@@ -407,7 +417,12 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
 /* The form for many rows of a matrix: tiles of 64 rows (of Float32: 32, in three parts) by 256 columns, four waves of 64 of them, two
  * workgroups a compute unit.  The rows of a step of 128 lie in LDS, three steps at a time: the one whose products are taken, the next
  * one, whose sums by groups are taken meanwhile (of 16 rows by a wave), and the one after that, on its way there.  A wave makes its 64
- * columns' codes into numbers itself, in registers: 16 columns' are used for all rows. */
+ * columns' codes into numbers itself, in registers: 16 columns' are used for all rows.  bfloat16, 2048 rows of 8 matrices of 4096 x 4096 in
+ * groups of 128: 122 us, 564 TFLOP/s, 223 where the matrices are made again first.  Loads are not what it waits for (without those of
+ * the codes 1 us less, of the rows 7): a step's 64 instructions of the matrix cores take as long as the 200 others beside them, of which
+ * a half makes numbers, and of two waves a SIMD one covers the other only in part.  (128 rows and eight waves a workgroup: 154, a
+ * segment's short last tile being as long as a whole one; the numbers of the next 32 made ready between the products: 132 and more,
+ * for want of registers.) */
 #define OP_PER (OP_ELT == 0 ? 2 : 4)               /* rows of a tile, in sixteens */
 #define OP_ROWS (16 * OP_PER)
 #define OP_SIZE ((int)sizeof(op_elt))
@@ -445,7 +460,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
     for (int u = 0; u < OP_PER; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 16 * u), 0) * p.x_stride + chunk * 8;
     /* ... and among the scales and zeros: 16 bytes of a group's (of the last columns: as many as there are) */
     constexpr int wide = 16 / OP_SIZE, lanes = OP_COLUMNS / wide;
-    const int scale_at = acc_min(j0 + tid % lanes * wide, p.nj - wide), zero_at = acc_min(j0 + tid % 16 * 16, p.nj - 16);
+    const int scale_at = acc_min(j0 + (tid < OP_CHUNKS * lanes ? tid % lanes * wide : 0), p.nj - wide), zero_at = acc_min(j0 + tid % 16 * 16, p.nj - 16);
     const op_elt *const scales = (const op_elt *)p.scales + tile.expert * p.scales_expert + scale_at;
     const unsigned char *const zeros = (const unsigned char *)p.zeros + tile.expert * p.zeros_expert + zero_at;
     op_eight v[OP_PER];
@@ -456,7 +471,9 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
       if (OP_ZEROS) zero_note = ((const op_loose<unsigned char> *)(zeros + acc_min(group + tid / 16 % OP_CHUNKS, p.groups - 1) * p.zeros_stride))->v;
       if (n * 128 + 128 <= p.k) {
 #pragma unroll
-        for (int u = 0; u < OP_PER; ++u) v[u] = op_row8(from[u] + n * 128, 8);
+        for (int u = 0; u < OP_PER; ++u)
+#pragma unroll
+          for (int h = 0; h < 8 / OP_VALUES; ++h) v[u].v[h] = ((const op_loose<op_elt> *)(from[u] + n * 128 + h * OP_VALUES))->v;
       } else {
 #pragma unroll
         for (int u = 0; u < OP_PER; ++u) v[u] = op_row8(from[u] + n * 128, p.k - n * 128 - chunk * 8);
@@ -489,14 +506,14 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
       return op_as_frag(x[((buffer * 16 + b * 4 + g) * OP_PARTS + part) * OP_ROWS + i * 16 + (l ^ turn)]);
     };
     const auto add_up = [&](const int buffer, const int slot) {
-      if (wave >= OP_PER) return;
+      if (OP_PER < 4 && wave >= OP_PER) return;
 #pragma unroll
       for (int q = 0; q < OP_CHUNKS; ++q) {
         acc_f4 t, d;
         op_sums(q, [&](const int b, const int part) { return row16(buffer, b, wave, part); }, t, d);
         const int at = (slot * OP_CHUNKS + q) * OP_ROWS + wave * 16 + l;
         if (g == 0) {
-          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], op_offset(t[0], d[0]), 8.0f);
+          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], d[0], 8.0f);
           if (OP_SECOND) offset[at] = d[0];
         }
       }
@@ -557,7 +574,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], op_offset(f[i], o[i]), z[r]) : f[i];
+              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], o[i], z[r]) : f[i];
 #pragma unroll
             for (int part = 0; part < OP_PARTS; ++part)
 #pragma unroll
@@ -700,7 +717,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
             const float scale = (float)s.s[q][j].v[r], zero = OP_ZEROS ? (float)s.z[q][j].v[r] : 8.0f;
 #pragma unroll
             for (int i = 0; i < OP_FM; ++i) {
-              const float first = t[i][j][r] + op_begin(sum[i][r], op_offset(sum[i][r], second[i][r]), zero);
+              const float first = t[i][j][r] + op_begin(sum[i][r], second[i][r], zero);
               c[i][j][r] = __builtin_fmaf(scale, OP_ELT == 0 ? first + op_rest(rest[i][j][r], second[i][r], zero) : first, c[i][j][r]);
             }
           }

@@ -778,9 +778,9 @@ int acc_exec_grouped_quantise(acc_op op, const acc_strided *w, const acc_strided
                               acc_stream stream);
 int acc_exec_grouped_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, const acc_strided *out,
                             acc_stream stream);
-/* acc_exec_product_rows with such matrices and rows x [.., k] of the operator's type.  (For a few rows of each matrix the numbers
- * are multiplied as they are; for many the matrices are first made again in the operator's type, in scratch memory.)  A row
- * with an infinity in it gives what is not a number. */
+/* acc_exec_product_rows with such matrices and rows x [.., k] of the operator's type.  (The numbers are multiplied as they are, or, for
+ * very many rows of few matrices, the matrices first made again in the operator's type, rounded, in scratch memory.)  A row with an
+ * infinity in it gives what is not a number. */
 int acc_exec_grouped_rows(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros,
                           const acc_strided *offsets, const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream);
 
