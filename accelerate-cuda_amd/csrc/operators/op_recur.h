@@ -10,7 +10,9 @@
  * then).  A row that begins a sequence takes nothing of the row before: it replaces, it does not multiply, so that no infinity
  * and nothing that is not a number passes from one sequence to the next.
  *
- * Bound by memory: every array passes by once.  A workgroup has a tile of 64 OP_V channels and 8 OP_R rows, a wave OP_R of those, all
+ * Bound by memory: every array passes by once.  bfloat16, 32768 rows of 2048 in 8 sequences, sigmoids: 101 us, 4.0 TB/s, the gradient 170,
+ * 4.7 (a copy 5.4); what is short of that are the gates, worked out in both passes.  One sequence of 65536 half rows of 512: 56, 3.6, the
+ * tiles' waits for those before; Float32, 9001 rows of 1001: 38, 2.9, rows starting amid lines.  A workgroup has a tile of 64 OP_V channels and 8 OP_R rows, a wave OP_R of those, all
  * of them in registers; it goes over them twice, first for the tile's map, and once what comes in from the rows before is known for
  * the results.  That it finds in what the tiles before have left: their maps (A, B), or the state behind them (H), as 64-bit words
  * of a Float32 and the launch's tag, which need no fence.  A tile in which a sequence begins leaves a state at once.  Every tile

@@ -2,15 +2,16 @@
  * op_score.h -- a router that scores experts one by one, s = 1 / (1 + e^-x), and chooses by s + bias: the best `keep` groups of
  * neighbouring experts, by the sum of their two best, then the best OP_CHOOSE experts of those; weights are the chosen scores alone.
  *
- * A token has OP_LANES neighbouring lanes, each with up to OP_PER neighbouring logits in registers, a group or an even part of one.  What is ranked is Float32 in the high bits of a 64-bit number that compares as one, with the index turned round in the low
- * bits, so that of equal ones the lowest index is the largest.  A lane puts its numbers where they belong among its best, two
- * instructions a place, and the token's lanes then exchange what they have.
+ * A token has OP_LANES neighbouring lanes, each with up to OP_PER neighbouring logits in registers, a group or an even part of one.  What
+ * is ranked is Float32 in the high bits of a 64-bit number that compares as one, with the index turned round in the low bits, so that of
+ * equal ones the lowest index is the largest.  A lane puts its numbers where they belong among its best, two instructions a place, and
+ * the token's lanes then exchange what they have.
  *
  * Scores of 64 bits decide.  Float32 ones are off by 2.3 10^-7 at most, and what lies closer than several times that (and is not the
  * same logit and bias, which is a tie wherever it is computed) is decided again in 64 bits, a wave for a token, when the others are
  * done: of normal logits, 256 experts and eight groups one token in some thousands.
  *
- * Bound by no one thing of the card's: 32768 tokens of 256 bfloat16 logits, eight chosen of four of eight groups, take 45 us, of which
+ * Bound by no one thing of the card's: 32768 tokens of 256 bfloat16 logits, eight chosen of four of eight groups, take 42 us, of which
  * the placing is 10 and the instructions of the choice some 12; memory is 4.  A wave's steps wait for one another (with four waves a
  * workgroup 55, with sixteen, which have 128 registers each, 59).
  */
@@ -385,7 +386,8 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
 
 /* d logit_j = d score_j s_j (1 - s_j) of the chosen ones, zero elsewhere; d score = scale dw, or, where weights are normalised,
  * scale (dw_j - sum_i dw_i share_i) / sum s.  Bound by memory: the zeros.  A token has OP_ROW lanes, one a choice, which then write
- * 16 bytes of its row each.  (share_j (1 - s_j) is what a score's part in the sum comes to: nothing is divided by a sum of small scores.) */
+ * 16 bytes of its row each: 32768 tokens of 256 in bfloat16 11.4 us, 3.1 TB/s of the 36 MB, as a token's choices are read before its
+ * logits.  (share_j (1 - s_j) is what a score's part in the sum comes to: nothing is divided by a sum of small scores.) */
 extern "C" __global__ void __launch_bounds__(256) score_gradient(const acc_route_args p)
 {
   if (p.guard && *p.guard == 0u) return;

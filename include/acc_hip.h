@@ -644,7 +644,8 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
 
 /* What a layer of experts needs beside the skeletons: products of ragged segments of rows with a matrix each, on the
  * matrix cores; the router that makes the segments; the weighted sum that brings the rows back; and the same products on
- * 4-bit numbers.  Segments are offsets, as for acc_exec_foldseg.  The reference has no counterpart (its backend has no
+ * 4-bit numbers; and what a decoder's block has beside them: a recurrence along ragged sequences, a router by scores, products
+ * with matrices of 4-bit whole numbers under group scales.  Segments are offsets, as for acc_exec_foldseg.  The reference has no counterpart (its backend has no
  * matrix instructions and no 16-bit types).
  *
  * All work is enqueued on `stream`; the calls return without waiting.  On a stream under a guard (acc_stream_set_guard)
@@ -652,7 +653,7 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * type, and results are rounded once; they are taken in an order that shapes and segments alone decide, so that a call
  * gives the same bits every time.  No result may share memory with another array of the call (other columns of the same
  * rows are apart).  Scratch memory -- pieces of long sums, 16-bit operands whose rows start anywhere copied to where they
- * do not (2 GB at most), a router's counts -- comes from the context's pool, in stream order.  Calls may be recorded into a
+ * do not (2 GB at most), matrices made again, a router's counts, what tiles of a recurrence leave for one another -- comes from the context's pool, in stream order.  Calls may be recorded into a
  * graph once the same ones have run on that stream (their kernels are loaded then, and the pool has what they need).  What
  * scratch memory they take is from then on lent to calls recorded on that stream alone, whose graphs must therefore not run
  * side by side: replay them on the stream they were recorded on.  It is the pool's again when acc_stream_destroy is called
@@ -661,7 +662,8 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * Element types are "float", "half" and "bfloat16" (an acc_strided does not say which it holds; the operator does).
  * Extents are below 2^31, those of a product at most 2^31 - 4096; strides are in elements, and addresses are computed in
  * 64 bits.  Offsets, indices, places and orders are Int32 and are looked at on the device: values out of range name no
- * row.  An offset counts as the nearest row there is, and one that goes back as the largest before it.           */
+ * row.  An offset counts as the nearest row there is, and one that goes back as the largest before it (those of a recurrence:
+ * see there).  */
 #define ACC_STRIDED_RANK 4
 typedef struct acc_strided {
   int32_t    rank;
