@@ -430,6 +430,11 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
 #define OP_SECOND (OP_ELT == 0 || (OP_ELT == 1 && OP_ZEROS))
 #define OP_LINE (OP_COLUMNS + 16)                  /* scales (zeros) of a group: 16 places in front, for a tile with fewer columns */
 
+/* What the 16 rows' places of a step's word b, quarter g are turned by: other numbers for all 16, so that a row's eighths go to other banks;
+ * and for the quarters 0 and 1, 2 and 3, of whose lanes 16 are served at a time (four, four more twelve on, and eight of the other quarter
+ * between those), such that these still lie beside each other. */
+ACC_DEV int op_turn_of(const int b, const int g) { return OP_CHUNKS > 1 ? 4 * b + g : b | (g & 1) << 3 | ((g ^ g >> 1) & 1) << 2; }
+
 template <int N> struct op_count { static constexpr int value = N; };
 
 extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) grouped(const acc_grouped_args p)
@@ -454,7 +459,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
 
   if (tile.expert >= 0 && p.x_rows > 0 && steps > 0) {
     /* a lane's places among the rows: eight neighbours, of rows 16 apart */
-    const int chunk = tid & 15, first = tid >> 4, place = ((OP_CHUNKS > 1 ? chunk : chunk % 4 * 4 + chunk / 4) * OP_PARTS * OP_ROWS) + (first ^ (chunk & 7));
+    const int chunk = tid & 15, first = tid >> 4, place = ((OP_CHUNKS > 1 ? chunk : chunk % 4 * 4 + chunk / 4) * OP_PARTS * OP_ROWS) + (first ^ (OP_CHUNKS > 1 ? op_turn_of(chunk / 4, chunk % 4) : op_turn_of(chunk % 4, chunk / 4)));
     const op_elt *from[OP_PER];
 #pragma unroll
     for (int u = 0; u < OP_PER; ++u) from[u] = (const op_elt *)p.x + (long long)acc_max(row_of(first + 16 * u), 0) * p.x_stride + chunk * 8;
@@ -502,8 +507,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
     };
     /* the lane's fragment of rows 16 i on of a wave's */
     const auto row16 = [&](const int buffer, const int b, const int i, const int part) {
-      const int turn = (OP_CHUNKS > 1 ? 4 * b + g : 4 * g + b) & 7;
-      return op_as_frag(x[((buffer * 16 + b * 4 + g) * OP_PARTS + part) * OP_ROWS + i * 16 + (l ^ turn)]);
+      return op_as_frag(x[((buffer * 16 + b * 4 + g) * OP_PARTS + part) * OP_ROWS + i * 16 + (l ^ op_turn_of(b, g))]);
     };
     const auto add_up = [&](const int buffer, const int slot) {
       if (OP_PER < 4 && wave >= OP_PER) return;
