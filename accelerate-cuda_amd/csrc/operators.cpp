@@ -661,12 +661,12 @@ int64_t grouped_tall_lds(const OpSpec &sp, bool zeros)
 constexpr int64_t kGroupedStream = 384;
 // Whether a call is for tiles of 64 rows (Float32: 32) by 256 columns that make numbers of the codes as they go: rows enough for them, tiles enough
 // (one that is 4096 long takes 55 us, however few there are), and not so many rows a matrix that making it again is little beside its
-// products.  us, with and without, rows (a few more or less a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 60 and 75; 2048, 8,
-// 512: 118 and 223, in groups of 32 with zeros 211 and 246; 4096, 8, 1024: 188 and 296, in groups of 32 335 and 316; 8192, 8, 2048: 326 and
-// 402; 300, 1, 80: 56 and 45; 700, 1, 176: 59 and 66; 2000, 1, 512: 97 and 85; 300, 3, 80: 59 and 66; 160, 2, 48: 54 and 43; 900, 4 of
+// products.  us, with and without, rows (a few more or less a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 56 and 75; 2048, 8,
+// 512: 117 and 223, in groups of 32 with zeros 205 and 246; 4096, 8, 1024: 181 and 296, in groups of 32 335 and 316; 8192, 8, 2048: 314 and
+// 402; 300, 1, 80: 56 and 45; 700, 1, 176: 55 and 66; 2000, 1, 512: 97 and 85; 300, 3, 80: 59 and 66; 160, 2, 48: 54 and 43; 900, 4 of
 // 2000 x 1000, 120: 26 and 32; 1600, 20 of 1000 x 1000, 100: 28 and 32; 1000, 20 of 500 x 2000, 40: 46 and 25.  Float32, whose products
-// are then those of three bfloat16 parts in place of its own instructions', a third as fast: 4096, 8 of 4096 x 4096, 2048: 430 and 1177;
-// 1000, 1, 512: 105 and 263; 300, 8 in groups of 32, 160: 102 and 168; 600, 4 of 1024 x 2048, 76: 36 and 43; 400, 4, 52: 35 and 23; 100, 1
+// are then those of three bfloat16 parts in place of its own instructions', a third as fast: 4096, 8 of 4096 x 4096, 2048: 409 and 1177;
+// 1000, 1, 512: 102 and 263; 300, 8 in groups of 32, 160: 116 and 168; 600, 4 of 1024 x 2048, 76: 35 and 43; 400, 4, 52: 35 and 23; 100, 1
 // of 4096 x 4096, 64: 64 and 38
 bool grouped_tall(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean)
 {

@@ -10,8 +10,7 @@
  * rounded.  What is taken off again costs some of the 24 bits of a sum: of half ones eight of those beyond a 4-bit number's own, in
  * bfloat16 five: a small part of what the result's rounding costs.  Float32 rows are cut into three bfloat16 each, which hold all 24 bits;
  * the first parts, 8 bits each, are added up and what is too much of them taken off before the others come, which is exact or nearly so
- * (150 rows of 12 matrices of 1333 x 1001 in groups of 32: 1.2e-7 off; all at once 6e-7, and up to 1.4e-6 at other sizes; it costs 4 us of
- * 26).  (An infinity in a row makes the row's results NaN.)
+ * (150 rows of 12 matrices of 1333 x 1001 in groups of 32, 23 us: 1.2e-7 off; all at once 6e-7, and up to 1.4e-6 at other sizes).  (An infinity in a row makes the row's results NaN.)
  *
  * What counts is that the matrices pass by once, and that their codes are nearly all that is read.  A lane loads 16 bytes of them, 32
  * numbers of a row.  Where a matrix has many columns for a compute unit, the rows lie in LDS and waves go over the columns (OP_STREAM);
@@ -287,18 +286,26 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
   /* step n's products, the first of its groups being the at-th that is noted; `down`: the columns' places among the noted 16 */
   const auto add = [&](const int n, const int at, const int down, acc_u4 w) {
     op_turn(w);
+    /* (of Float32's many fragments in groups of 32 no addresses are kept from step to step: there are not the registers, and a wait for
+     * one that has been put into memory is a wait for all codes on their way: 28 us in place of 23 for 150 rows of 12 matrices of
+     * 1333 x 1001.  Elsewhere, where there are registers, it costs 3 in 100) */
+    int row = l, quarter = g;
+    if (OP_PARTS > 1 && OP_CHUNKS > 2) {
+      acc_pin(row);
+      acc_pin(quarter);
+    }
 #pragma unroll
     for (int q = 0; q < OP_CHUNKS; ++q) {
       const int noted_at = at + q;
       op_e4<op_elt> s;
       op_e4<unsigned char> z;
       if (down == 0) {
-        __builtin_memcpy(&s, __builtin_assume_aligned(my_notes + (noted_at * 16 + g * 4) * OP_SIZE, 4 * OP_SIZE), sizeof(s));
-        if (OP_ZEROS) __builtin_memcpy(&z, __builtin_assume_aligned(my_notes + OP_NOTED * OP_SIZE * 16 + noted_at * 16 + g * 4, 4), sizeof(z));
+        __builtin_memcpy(&s, __builtin_assume_aligned(my_notes + (noted_at * 16 + quarter * 4) * OP_SIZE, 4 * OP_SIZE), sizeof(s));
+        if (OP_ZEROS) __builtin_memcpy(&z, __builtin_assume_aligned(my_notes + OP_NOTED * OP_SIZE * 16 + noted_at * 16 + quarter * 4, 4), sizeof(z));
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int k = acc_min(g * 4 + r + down, 15);
+          const int k = acc_min(quarter * 4 + r + down, 15);
           s.v[r] = *(const op_elt *)(my_notes + (noted_at * 16 + k) * OP_SIZE);
           if (OP_ZEROS) z.v[r] = *(const unsigned char *)(my_notes + OP_NOTED * OP_SIZE * 16 + noted_at * 16 + k);
         }
@@ -307,7 +314,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
       float second[OP_FM];
 #pragma unroll
       for (int i = 0; i < OP_FM; ++i) {
-        const int place = (n * OP_CHUNKS + q) * height + ((i * 16 + l) & (height - 1));
+        const int place = (n * OP_CHUNKS + q) * height + ((i * 16 + row) & (height - 1));
         const float f = sum[place];
         second[i] = OP_ELT != 2 ? offset[place] : 0.0f;
 #pragma unroll
@@ -319,7 +326,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
         for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
           const op_frag v = op_as_frag(op_numbers(w[b]));
 #pragma unroll
-          for (int i = 0; i < OP_FM; ++i) t[i] = op_mfma(v, op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + g) * height + ((i * 16 + l) & (height - 1))]), t[i]);
+          for (int i = 0; i < OP_FM; ++i) t[i] = op_mfma(v, op_as_frag(x[(((n * 4 + b) * OP_PARTS + part) * 4 + quarter) * height + ((i * 16 + row) & (height - 1))]), t[i]);
         }
 #pragma unroll
       for (int i = 0; i < OP_FM; ++i)
@@ -418,7 +425,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
  * workgroups a compute unit.  The rows of a step of 128 lie in LDS, three steps at a time: the one whose products are taken, the next
  * one, whose sums by groups are taken meanwhile (of 16 rows by a wave), and the one after that, on its way there.  A wave makes its 64
  * columns' codes into numbers itself, in registers: 16 columns' are used for all rows.  bfloat16, 2048 rows of 8 matrices of 4096 x 4096 in
- * groups of 128: 122 us, 564 TFLOP/s, 223 where the matrices are made again first.  Loads are not what it waits for (without those of
+ * groups of 128: 117 us, 587 TFLOP/s, 223 where the matrices are made again first.  Loads are not what it waits for (without those of
  * the codes 1 us less, of the rows 7): a step's 64 instructions of the matrix cores take as long as the 200 others beside them, of which
  * a half makes numbers, and of two waves a SIMD one covers the other only in part.  (128 rows and eight waves a workgroup: 154, a
  * segment's short last tile being as long as a whole one; the numbers of the next 32 made ready between the products: 132 and more,
