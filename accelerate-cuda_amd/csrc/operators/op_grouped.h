@@ -138,13 +138,18 @@ extern "C" __global__ void __launch_bounds__(256) grouped_quantise(const acc_gro
   const op_elt *const w = (const op_elt *)p.w + e * p.w_expert + j * p.w_stride;
   float low = 0.0f, high = 0.0f;
   int bad = 0;
-  for (int k = first + lane * 8; k < end; k += team * 8)
-    for (int i = k; i < acc_min(k + 8, end); ++i) {
-      const float v = (float)w[i];
+  for (int k = first + lane * 8; k < end; k += team * 8) {
+    const op_eight x = op_row8(w + k, end - k);
+    op_elt e[8];
+    __builtin_memcpy(e, &x, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float v = (float)e[i];
       low = v < low ? v : low;
       high = v > high ? v : high;
       bad |= !(__builtin_fabsf(v) < __builtin_inff());
     }
+  }
   for (int apart = 1; apart < team; apart *= 2) {
     const int other = (acc_lane() ^ apart) * 4;
     const float l = __uint_as_float(__builtin_amdgcn_ds_bpermute(other, __float_as_uint(low))), h = __uint_as_float(__builtin_amdgcn_ds_bpermute(other, __float_as_uint(high)));
@@ -160,10 +165,13 @@ extern "C" __global__ void __launch_bounds__(256) grouped_quantise(const acc_gro
   const float zero = p.zeros ? (scale > 0.0f ? acc_min(acc_max(__builtin_rintf(-low / scale), 0.0f), 15.0f) : 0.0f) : 8.0f;
   unsigned char *const codes = (unsigned char *)p.codes + e * p.codes_expert + j * p.codes_stride;
   for (int k = first + lane * 8; k < acc_min(first + p.group, p.blocks * 32); k += team * 8) {
+    const op_eight x = op_row8(w + k, end - k);
+    op_elt e[8];
+    __builtin_memcpy(e, &x, sizeof(e));
     unsigned int word = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float v = k + i < end ? (float)w[k + i] : 0.0f, q = scale > 0.0f && !bad ? __builtin_rintf(v / scale) : 0.0f;
+      const float v = (float)e[i], q = scale > 0.0f && !bad ? __builtin_rintf(v / scale) : 0.0f;
       word |= (unsigned int)acc_min(acc_max(q + zero, 0.0f), 15.0f) << 4 * i;
     }
     *(unsigned int *)(codes + k / 2) = word;
