@@ -255,8 +255,7 @@ struct GroupedVariant {
     if (stream) return few || sp.group == 32 || (sp.group == 64 && sp.type == 0) ? 2 : 4;
     return elements || bm > 32 || (bm > 16 && sp.type == 0) ? 1 : bm > 16 || fn > 1 || sp.type == 0 ? 2 : 4;
   }
-  uint32_t key() const { return kGroupedKeys | (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u) | (stream ? 512u : 0u) | (zeros ? 1024u : 0u) | (wide == 8 ? 2048u : 0u) | (sixteen ? 4096u : 0u) | (few ? 8192u : 0u) | (tall ? 16384u : 0u); }
-  static constexpr uint32_t kGroupedKeys = 1u << 21;               // (beside the products' keys)
+  uint32_t key() const { return (uint32_t)(bm / 16) | (uint32_t)fn << 4 | (elements ? 256u : 0u) | (stream ? 512u : 0u) | (zeros ? 1024u : 0u) | (wide == 8 ? 2048u : 0u) | (sixteen ? 4096u : 0u) | (few ? 8192u : 0u) | (tall ? 16384u : 0u); }
 };
 std::string grouped_source(const OpSpec &sp, const GroupedVariant &v)
 {
@@ -349,16 +348,6 @@ std::vector<std::string> all_sources(const OpSpec &sp)
     v = {};
     v.elements = true;
     out.push_back(grouped_source(sp, v));
-    // (and the products of matrices that have been made again)
-    if (sp.type != 0) out.push_back(pack_source(sp));
-    for (int t = 0; t < kSkinny; ++t)
-      for (int form = 0; form < 3; ++form) {
-        ProductVariant p;
-        p.tile = t;
-        p.aligned = form == 0;
-        p.tiny = form == 2;
-        if (has_tile(sp, p, t)) out.push_back(product_source(sp, p));
-      }
   } else if (sp.kind == ACC_OP_RECUR) {
     for (int form = 0; form < 6; ++form)
       for (int rows : {8, 16, 32}) {
@@ -637,10 +626,7 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
   return experts * piece >= 2 * rows ? 0 : (int32_t)piece;
 }
 
-// grouped: from how many rows a segment on the matrices are made again for tiles that use them often.  us, as they are and made again:
-// 160 rows, 2 of 4096 x 4096: 43 and 53; 300, 1: 60 and 46; Float32, 400, 4 of 1024 x 2048: 23 and 43
-constexpr int64_t kGroupedMost = 128;
-// ... LDS of the form with rows in it: `height` of them, their sums by groups, and the waves' results where they share columns
+// grouped: LDS of the form with rows in it: `height` of them, their sums by groups, and the waves' results where they share columns
 int64_t grouped_lds(const OpSpec &sp, int64_t height, int64_t steps, int64_t waves)
 {
   const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
@@ -659,20 +645,17 @@ int64_t grouped_tall_lds(const OpSpec &sp, bool zeros)
 // 512: 16 and 23; 64 rows, 16 half of 4096 x 2048, 4096: 23 and 34; 16, 8 of 4096 x 4096 in groups of 32: 29 and 44; Float32, 64, 16 of
 // 1024 x 2048, 1024: 14 and 12
 constexpr int64_t kGroupedStream = 384;
-// Whether a call is for tiles of 64 rows (Float32: 32) by 256 columns that make numbers of the codes as they go: rows enough for them, tiles enough
-// (one that is 4096 long takes 55 us, however few there are), and not so many rows a matrix that making it again is little beside its
-// products.  us, with and without, rows (a few more or less a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 56 and 75; 2048, 8,
-// 512: 117 and 223, in groups of 32 with zeros 205 and 246; 4096, 8, 1024: 181 and 296, in groups of 32 335 and 316; 8192, 8, 2048: 314 and
-// 402; 300, 1, 80: 56 and 45; 700, 1, 176: 55 and 66; 2000, 1, 512: 97 and 85; 300, 3, 80: 59 and 66; 160, 2, 48: 54 and 43; 900, 4 of
-// 2000 x 1000, 120: 26 and 32; 1600, 20 of 1000 x 1000, 100: 28 and 32; 1000, 20 of 500 x 2000, 40: 46 and 25.  Float32, whose products
-// are then those of three bfloat16 parts in place of its own instructions', a third as fast: 4096, 8 of 4096 x 4096, 2048: 409 and 1177;
-// 1000, 1, 512: 102 and 263; 300, 8 in groups of 32, 160: 116 and 168; 600, 4 of 1024 x 2048, 76: 35 and 43; 400, 4, 52: 35 and 23; 100, 1
-// of 4096 x 4096, 64: 64 and 38
+// Whether a call is for tiles of 64 rows (Float32: 32) by 256 columns that make numbers of the codes as they go: rows enough for them, and tiles
+// enough (one that is 4096 long takes 50 us, in groups of 32 100, however few there are).  us, with and without, rows (a few more or less
+// a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 56 and 75; 200, 1 of 4096 x 4096, 64: 49 and 41; 300, 1, 80: 53 and 58, in groups of 32
+// 103 and 77; 400, 1, 112: 50 and 68, in groups of 32 99 and 99; 2000, 1, 512: 83 and 277; 600, 4 of 1024 x 2048, 48: 28 and 24; 1200, 4, 80: 29 and 38;
+// 900, 4 of 2000 x 1000, 120: 26 and 32; 1000, 20 of 500 x 2000, 40: 46 and 25.  Float32: 130, 1 of 4096 x 4096, 80: 65 and 68, in groups of 32
+// 109 and 94; 300, 1, 160: 66 and 113, 110 and 152; 300, 4 of 1024 x 2048, 48: 36 and 25; 600, 4, 80: 37 and 47, 59 and 60
 bool grouped_tall(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean)
 {
   const bool wide = sp.type == 0;
   const int64_t tiles = std::max(ceil_div(rows, wide ? 32 : 64), std::min(rows, experts)) * ceil_div(n, 256);
-  return n >= 16 && k > 0 && pitch < (1 << 26) && mean > 32 && (wide || mean <= (sp.group >= 64 ? 1024 : 256)) && tiles >= (wide ? 72 : 96);
+  return n >= 16 && k > 0 && pitch < (1 << 26) && mean > 32 && tiles >= (sp.group == 32 ? 96 : 72);
 }
 // the tile for `mean` rows a segment; *height: its rows.  (Where LDS holds fewer rows than a segment has, their codes are read again:
 // 64 rows, 2 of 4096 x 4096: 18 us in tiles of 16, 26 without LDS.)
@@ -757,7 +740,6 @@ std::string recur_source_of(const OpSpec &sp, uint32_t key)
 
 std::string grouped_source_of(const OpSpec &sp, uint32_t key)
 {
-  if (!(key & GroupedVariant::kGroupedKeys)) return product_source_of(sp, key);
   GroupedVariant v;
   v.bm = (int)(key & 15u) * 16;
   v.fn = (int)(key >> 4 & 15u);
@@ -985,9 +967,6 @@ static int launch_rows(acc_op op, const char *who, const ProductVariant &v, cons
   return rc;
 }
 
-static int product_of_rows(acc_op op, const char *who, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
-                           const acc_strided *out, acc_product_args a, acc_stream stream);
-
 int acc_exec_product_rows(acc_op op, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
                           const acc_strided *out, acc_stream stream)
 try {
@@ -1000,7 +979,7 @@ try {
   ACC_TRY(check_result(who, "the result", out, 2));
   if (index) ACC_TRY(check_unit(who, "index", index, 1));
   const int64_t experts = w->shape[0], n = w->shape[1], rows = out->shape[0];
-  const int64_t k = w->shape[2];
+  int64_t k = w->shape[2];
   if (!unit(*w, 2) && !unit(*w, 1)) return fail(ACC_ERR_INVALID, "%s: neither the second nor the third dimension of w is contiguous", who);
   if (per < 0) return fail(ACC_ERR_INVALID, "%s: a divisor of %d", who, per);
   ACC_TRY(check_shape(who, "offsets", *offsets, {experts + 1}));
@@ -1008,19 +987,10 @@ try {
   if (index) ACC_TRY(check_shape(who, "index", *index, {rows}));
   ACC_TRY(check_shape(who, "x", *x, {index ? x->shape[0] : rows, k}));
   ACC_TRY(check_extents(who, {experts, n, k, rows, x->shape[0]}));
-  const int bytes = type_bytes(op->spec.type);
+  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
   ACC_TRY(check_apart(who, {out, bytes, "the result"}, {{x, bytes, "x"}, {w, bytes, "w"}, {offsets, 4, "offsets"}, {index, 4, "index"}}));
   if (rows == 0 || n == 0) return ACC_OK;
-  return product_of_rows(op, who, x, w, offsets, index, per, out, a, stream);
-} ACC_OP_CATCH("acc_exec_product_rows")
 
-// ... the same behind the checks, for a result that has elements
-static int product_of_rows(acc_op op, const char *who, const acc_strided *x, const acc_strided *w, const acc_strided *offsets, const acc_strided *index, int32_t per,
-                           const acc_strided *out, acc_product_args a, acc_stream stream)
-{
-  const int64_t experts = w->shape[0], n = w->shape[1], rows = out->shape[0];
-  int64_t k = w->shape[2];
-  const int bytes = type_bytes(op->spec.type), epc = 16 / bytes;
   ProductVariant v;
   // (where both are contiguous -- one column, or a sum of one -- either way of reading will do)
   v.b_fast = unit(*w, 2);
@@ -1069,7 +1039,7 @@ static int product_of_rows(acc_op op, const char *who, const acc_strided *x, con
   a.experts = (int32_t)experts;
   set_divisor(per, &a);
   return launch_rows(op, who, v, var, a, stream);
-}
+} ACC_OP_CATCH("acc_exec_product_rows")
 
 int acc_exec_product_outer(acc_op op, const acc_strided *x, const acc_strided *y, const acc_strided *offsets, const acc_strided *index, int32_t per,
                            const acc_strided *out, acc_stream stream)
@@ -1736,27 +1706,6 @@ try {
   if (is_empty(*out)) return ACC_OK;
   const int64_t mean = ceil_div(rows, std::max<int64_t>(1, std::min(rows, experts)));
   const bool tall = grouped_tall(op->spec, rows, experts, n, k, codes->stride[1], mean);
-  if (!tall && mean > kGroupedMost && k > 0 && x->shape[0] > 0) {
-    ScratchHold made;
-    ACC_TRY(made.acquire(op, stream, (size_t)(experts * n * ceil_div(k, 8) * 8 * bytes)));
-    acc_strided w = {};
-    w.rank = 3;
-    w.shape[0] = experts;
-    w.shape[1] = n;
-    w.shape[2] = k;
-    w.stride[2] = 1;
-    w.stride[1] = ceil_div(k, 8) * 8;
-    w.stride[0] = n * w.stride[1];
-    w.ptr = reinterpret_cast<uint64_t>(made.ref.ptr);
-    acc_grouped_args b = a;
-    b.out = made.ref.ptr;
-    b.out_expert = w.stride[0];
-    b.out_stride = w.stride[1];
-    ACC_TRY(launch_elements(op, who, true, experts * n * a.blocks * 4, b, stream));
-    acc_product_args product = {};
-    product.guard = a.guard;
-    return product_of_rows(op, who, x, &w, offsets, index, per, out, product, stream);
-  }
   int64_t height = 0;
   GroupedVariant v;
   if (tall) {

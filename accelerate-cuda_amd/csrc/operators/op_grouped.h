@@ -433,7 +433,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
  * workgroups a compute unit.  The rows of a step of 128 lie in LDS, three steps at a time: the one whose products are taken, the next
  * one, whose sums by groups are taken meanwhile (of 16 rows by a wave), and the one after that, on its way there.  A wave makes its 64
  * columns' codes into numbers itself, in registers: 16 columns' are used for all rows.  bfloat16, 2048 rows of 8 matrices of 4096 x 4096 in
- * groups of 128: 117 us, 587 TFLOP/s, 223 where the matrices are made again first.  Loads are not what it waits for (without those of
+ * groups of 128: 117 us, 587 TFLOP/s.  Loads are not what it waits for (without those of
  * the codes 1 us less, of the rows 7): a step's 64 instructions of the matrix cores take as long as the 200 others beside them, of which
  * a half makes numbers, and of two waves a SIMD one covers the other only in part.  (128 rows and eight waves a workgroup: 154, a
  * segment's short last tile being as long as a whole one; the numbers of the next 32 made ready between the products: 132 and more,

@@ -653,7 +653,7 @@ int acc_memtable_get_stats(acc_memtable mt, acc_memtable_stats *out);
  * type, and results are rounded once; they are taken in an order that shapes and segments alone decide, so that a call
  * gives the same bits every time.  No result may share memory with another array of the call (other columns of the same
  * rows are apart).  Scratch memory -- pieces of long sums, 16-bit operands whose rows start anywhere copied to where they
- * do not (2 GB at most), matrices made again, a router's counts, what tiles of a recurrence leave for one another -- comes from the context's pool, in stream order.  Calls may be recorded into a
+ * do not (2 GB at most), a router's counts, what tiles of a recurrence leave for one another -- comes from the context's pool, in stream order.  Calls may be recorded into a
  * graph once the same ones have run on that stream (their kernels are loaded then, and the pool has what they need).  What
  * scratch memory they take is from then on lent to calls recorded on that stream alone, whose graphs must therefore not run
  * side by side: replay them on the stream they were recorded on.  It is the pool's again when acc_stream_destroy is called
@@ -780,9 +780,8 @@ int acc_exec_grouped_quantise(acc_op op, const acc_strided *w, const acc_strided
                               acc_stream stream);
 int acc_exec_grouped_values(acc_op op, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, const acc_strided *out,
                             acc_stream stream);
-/* acc_exec_product_rows with such matrices and rows x [.., k] of the operator's type.  (The numbers are multiplied as they are, or, for
- * very many rows of few matrices, the matrices first made again in the operator's type, rounded, in scratch memory.)  A row with an
- * infinity in it gives what is not a number. */
+/* acc_exec_product_rows with such matrices and rows x [.., k] of the operator's type.  The numbers are multiplied as they are, however
+ * many rows there are: no weight is rounded.  A row with an infinity in it gives what is not a number. */
 int acc_exec_grouped_rows(acc_op op, const acc_strided *x, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros,
                           const acc_strided *offsets, const acc_strided *index, int32_t per, const acc_strided *out, acc_stream stream);
 

@@ -1,0 +1,99 @@
+"""Products with matrices of 4-bit whole numbers in groups (include/acc_hip.h, section D): the numbers that they keep, whatever form a call
+takes, by results whose rounding is known to the last bit.
+
+A row of one group gives s T, T = sum x (q - z) a whole number.  Here x are whole numbers of at most 3, so T is exact in Float32 (100 times
+3 times 15: 13 bits), s T has at most 11 + 13 bits of a 16-bit scale and is exact too, and the result is the exact one rounded once.  Of
+Float32 scales the product is rounded, once, and that is the result.
+"""
+import sys
+
+import numpy as np
+import pytest
+
+from test_gpu_grouped import Boxed, expected, matrices, packed, weights
+from test_gpu_operators import segments, store, values
+
+pytestmark = pytest.mark.gpu
+TYPES = ("float", "half", "bfloat16")
+
+
+def say(*a):
+    print("[case]", *a)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def A():
+    import acchip
+    return acchip
+
+
+@pytest.fixture(scope="module")
+def ctx(A):
+    c = A.Context(0)
+    yield c
+    c.close()
+
+
+@pytest.fixture(scope="module")
+def rows(A, ctx):
+    """rows(elt, group, x, q, scales, zeros, offsets): the products, as they are in memory"""
+    made = {}
+
+    def call(elt, group, x, q, scales, zeros, offsets):
+        if (elt, group) not in made:
+            made[elt, group] = A.Grouped(ctx, elt, group)
+        out = Boxed(A, ctx, np.full((x.shape[0], q.shape[1]), 9.0), elt)
+        made[elt, group].rows(Boxed(A, ctx, x, elt).array, ctx.array(packed(q)), Boxed(A, ctx, scales, elt).array, ctx.array(np.asarray(offsets, np.int32)), out.array,
+                              zeros=None if zeros is None else ctx.array(zeros))
+        ctx.sync()
+        return out.get()
+    yield call
+    for op in made.values():
+        op.destroy()
+
+
+# (rows, matrices, n, k): a few rows, a few hundred of one matrix, tiles of 256 columns enough for the device
+FORMS = [(3, 1, 70, 100), (129, 1, 70, 100), (300, 1, 70, 31), (700, 2, 4, 100), (5000, 2, 300, 70), (1500, 25, 900, 100), (200, 2, 3100, 100)]
+
+
+@pytest.mark.parametrize("with_zeros", (False, True))
+@pytest.mark.parametrize("elt", TYPES)
+def test_no_weight_is_rounded(rows, elt, with_zeros):
+    """scales with as many bits as their type has, of which (q - z) s has more"""
+    rng = np.random.default_rng(21)
+    for m, experts, n, k in FORMS:
+        q, scales, zeros = matrices(rng, experts, n, k, 128, elt, with_zeros, False)
+        x = rng.integers(-3, 4, (m, k)).astype(np.float64)
+        offsets = segments(rng, m, experts, "even")
+        say(elt, with_zeros, m, experts, n, k)
+        want, _ = expected(x, weights(q, scales, zeros, 128), offsets, m, None, 0)
+        assert np.array_equal(rows(elt, 128, x, q, scales, zeros, offsets), store(want, elt)), (m, experts, n, k)
+
+
+def test_half_weights_beyond_the_largest(rows):
+    """(q - z) s beyond 65504, as quantising a matrix of 65504 and its negative gives, and results far below it"""
+    rng = np.random.default_rng(22)
+    for m, experts, n, k in FORMS:
+        q, _, _ = matrices(rng, experts, n, k, 128, "half", False, False)
+        scales = np.full((experts, 1, n), 8736.0)
+        x = rng.integers(-3, 4, (m, k)) * 2.0 ** -12
+        offsets = segments(rng, m, experts, "even")
+        say(m, experts, n, k)
+        want, _ = expected(x, weights(q, scales, None, 128), offsets, m, None, 0)
+        got = rows("half", 128, x, q, scales, None, offsets)
+        assert np.isfinite(values(got, "half")).all() and np.array_equal(got, store(want, "half")), (m, experts, n, k)
+
+
+@pytest.mark.parametrize("elt", TYPES)
+def test_an_infinity_in_a_row_of_any_form(rows, elt):
+    """what the row gives is not a number, however many rows come with it"""
+    rng = np.random.default_rng(23)
+    for m, experts, n, k in FORMS:
+        q, scales, zeros = matrices(rng, experts, n, k, 64, elt, True, True)
+        x = rng.integers(-3, 4, (m, k)).astype(np.float64)
+        x[1, 5], x[2, k - 1] = np.inf, -np.inf
+        offsets = segments(rng, m, experts, "even")
+        say(elt, m, experts, n, k)
+        got = values(rows(elt, 64, x, q, scales, zeros, offsets), elt)
+        assert np.isnan(got[1:3]).all() and np.isfinite(np.delete(got, (1, 2), axis=0)).all(), (m, experts, n, k)
