@@ -630,7 +630,7 @@ int32_t outer_piece(const OpSpec &sp, const ProductVariant &v, int64_t rows, int
 int64_t grouped_lds(const OpSpec &sp, int64_t height, int64_t steps, int64_t waves)
 {
   const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
-  return steps * height * (256 * (sp.type == 0 ? 3 : 1) + chunks * (sp.type == 2 ? 4 : 8)) + waves * ceil_div(height, 16) * 1024;
+  return steps * height * (256 * (sp.type == 0 ? 3 : 1) + chunks * (sp.type == 0 ? 8 : 4)) + waves * ceil_div(height, 16) * 1024;
 }
 constexpr int64_t kGroupedLds = 160 << 10;
 // ... and of tiles of 64 rows by 256 columns: three steps of rows, scales and zeros, two of sums
@@ -638,7 +638,7 @@ int64_t grouped_tall_lds(const OpSpec &sp, bool zeros)
 {
   const int64_t chunks = sp.group >= 128 ? 1 : 128 / sp.group;
   const int64_t rows = sp.type == 0 ? 32 : 64, parts = sp.type == 0 ? 3 : 1;
-  return 3 * 16 * parts * rows * 16 + 3 * chunks * 272 * 4 * (zeros ? 2 : 1) + 2 * chunks * rows * 4 * (sp.type == 0 || (zeros && sp.type == 1) ? 2 : 1);
+  return 3 * 16 * parts * rows * 16 + 3 * chunks * 272 * 4 * (zeros ? 2 : 1) + 2 * chunks * rows * 4 * (sp.type == 0 ? 2 : 1);
 }
 // ... and the tiles of 16 columns from which on rows in LDS are worth what it takes to put them there.  us, with and without, tiles: 1 row,
 // 4096 x 4096, 256: 8.2 and 7.2; 16 rows: 14 and 11; 2 rows of 4096 x 11008, 256: 16 and 15; of 11008 x 4096, 688: 13 and 18; 1 row, 8192 x 8192,

@@ -4,13 +4,14 @@
  *   w[e, n, k] = (q[e, n, k] - z[e, g, n]) s[e, g, n],   g = k / group;   z = 8 where there are no zeros
  *   out[m, n]  = sum_k x[r(m), k] w[e(m), n, k]          for a few rows of each matrix
  *
- * The products are taken of the numbers as they are: a code's four bits become the mantissa of d + q, exact in either 16-bit type,
- * with a d that its place in the word decides (half: 1024, 64; bfloat16: 128; for Float32 rows 16); the matrix cores add up x (d + q)
- * over what a group has of a step, beginning with -(z sum x + sum d x), and that times s is added up in Float32: no weight is ever
- * rounded.  What is taken off again costs some of the 24 bits of a sum: of half ones eight of those beyond a 4-bit number's own, in
- * bfloat16 five: a small part of what the result's rounding costs.  Float32 rows are cut into three bfloat16 each, which hold all 24 bits;
+ * The products are taken of the numbers as they are: a code's four bits become the highest of the mantissa of 16 + q, exact in either
+ * 16-bit type; the matrix cores add up x (16 + q) over what a group has of a step, beginning with -(z + 16) sum x, and that times s is
+ * added up in Float32: no weight is ever rounded.  What is taken off again costs two or three of the 24 bits of a sum, more where a
+ * row's numbers share a sign and the sums of x (q - z) are small beside sum x: half rows of one sign, 4096 numbers in groups of 128, are
+ * 5.3e-6 off before the result is rounded.  (With the codes at the end of the mantissa, 1024 + q and 64 + q, such rows were 1.4e-4
+ * off, and calls no faster for want of three shifts: 64 rows, 16 of 4096 x 2048: 23.4 us and 23.3 as here; 2048, 8 of 4096 x 4096: 131 and 119.) Float32 rows are cut into three bfloat16 each, which hold all 24 bits;
  * the first parts, 8 bits each, are added up and what is too much of them taken off before the others come, which is exact or nearly so
- * (150 rows of 12 matrices of 1333 x 1001 in groups of 32, 23 us: 1.2e-7 off; all at once 6e-7, and up to 1.4e-6 at other sizes).  (An infinity in a row makes the row's results NaN.)
+ * (150 rows of 12 matrices of 1333 x 1001 in groups of 32, 21 us: 1.2e-7 off; all at once 6e-7, and up to 1.4e-6 at other sizes).  (An infinity in a row makes the row's results NaN.)
  *
  * What counts is that the matrices pass by once, and that their codes are nearly all that is read.  A lane loads 16 bytes of them, 32
  * numbers of a row.  Where a matrix has many columns for a compute unit, the rows lie in LDS and waves go over the columns (OP_STREAM);
@@ -29,24 +30,16 @@ ACC_DEV unsigned int op_lane_word(unsigned int v)
   asm("" : "+v"(v));
   return v;
 }
-/* 8 codes as d + q: of neighbours 0 4, 1 5, 2 6, 3 7; and the d alone */
+/* 8 codes as OP_D + q, in 16 bits each: of neighbours 0 4, 1 5, 2 6, 3 7 */
+#define OP_D 16.0f
 #if OP_ELT == 1
 #define OP_ONES 0x3C003C00u
 ACC_DEV acc_u4 op_numbers(const unsigned int w)
 {
-  const unsigned int v = w >> 8, a = op_lane_word(0x64006400u), b = op_lane_word(0x54005400u);
-  return acc_u4{(w & 0x000F000Fu) | a, (w & 0x00F000F0u) | b, (v & 0x000F000Fu) | a, (v & 0x00F000F0u) | b};
+  const unsigned int d = op_lane_word(0x4C004C00u);
+  const auto at = [d](const unsigned int v) { return (v & 0x03C003C0u) | d; };
+  return acc_u4{at(w << 6), at(w << 2), at(w >> 2), at(w >> 6)};
 }
-ACC_DEV acc_u4 op_offsets() { return acc_u4{0x64006400u, 0x54005400u, 0x64006400u, 0x54005400u}; }
-#elif OP_ELT == 2
-#define OP_ONES 0x3F803F80u
-ACC_DEV acc_u4 op_numbers(const unsigned int w)
-{
-  const unsigned int d = op_lane_word(0x43004300u);
-  const auto at = [d](const unsigned int v) { return (v & 0x000F000Fu) | d; };
-  return acc_u4{at(w), at(w >> 4), at(w >> 8), at(w >> 12)};
-}
-ACC_DEV acc_u4 op_offsets() { return acc_u4{0x43004300u, 0x43004300u, 0x43004300u, 0x43004300u}; }
 #else
 #define OP_ONES 0x3F803F80u
 ACC_DEV acc_u4 op_numbers(const unsigned int w)
@@ -55,7 +48,6 @@ ACC_DEV acc_u4 op_numbers(const unsigned int w)
   const auto at = [d](const unsigned int v) { return (v & 0x00780078u) | d; };
   return acc_u4{at(w << 3), at(w >> 1), at(w >> 5), at(w >> 9)};
 }
-ACC_DEV acc_u4 op_offsets() { return acc_u4{0x41804180u, 0x41804180u, 0x41804180u, 0x41804180u}; }
 #endif
 
 /* a row's 8 neighbours in that order, in OP_PARTS parts that add up to them */
@@ -209,20 +201,17 @@ extern "C" __global__ void __launch_bounds__(256) grouped_values(const acc_group
 }
 #else
 
-/* what products of a group begin with, -(z sum x + sum d x): d is in `second`, or the same for all (OP_D) */
-#define OP_D (OP_ELT == 2 ? 128.0f : 16.0f)
-ACC_DEV float op_begin(const float sum, const float second, const float zero) { return OP_ELT == 1 ? __builtin_fmaf(-zero, sum, -second) : -(zero + OP_D) * sum; }
+/* what products of a group begin with */
+ACC_DEV float op_begin(const float sum, const float zero) { return -(zero + OP_D) * sum; }
 
-/* the sums behind that, of 16 rows: sum x; and of half rows sum d x, of Float32 ones (whose `sum` is the first part's) the other parts' */
+/* the sums behind that, of 16 rows: sum x, of Float32 ones that of the first part, and of the other parts in `second` */
 template <typename F> ACC_DEV void op_sums(const int q, F fragment, acc_f4 &sum, acc_f4 &second)
 {
   const op_frag ones = op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES});
   sum = second = acc_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int b = q * OP_BLOCKS; b < (q + 1) * OP_BLOCKS; ++b) {
-    const op_frag y = fragment(b, 0);
-    sum = op_mfma(ones, y, sum);
-    if (OP_ELT == 1) second = op_mfma(op_as_frag(op_offsets()), y, second);
+    sum = op_mfma(ones, fragment(b, 0), sum);
 #pragma unroll
     for (int part = OP_PARTS - 1; part > 0; --part) second = op_mfma(ones, fragment(b, part), second);
   }
@@ -252,8 +241,8 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
   const bool sums = tile.expert >= 0 && p.x_rows > 0 && steps > 0;
   acc_u4 *const notes = shared;                    /* [waves][OP_FM][64]: a wave's scales and zeros; its sums, where they meet */
   acc_u4 *const x = notes + OP_WAVES * OP_FM * 64; /* [steps][4][parts][4][height] */
-  float *const sum = (float *)(x + steps * 16 * OP_PARTS * height);       /* [steps][chunks][height], and the second ones */
-  float *const offset = OP_ELT != 2 ? sum + steps * OP_CHUNKS * height : sum;
+  float *const sum = (float *)(x + steps * 16 * OP_PARTS * height);       /* [steps][chunks][height], and Float32's second ones */
+  float *const offset = OP_ELT == 0 ? sum + steps * OP_CHUNKS * height : sum;
   const auto row_of = [&](const int i) { return p.index ? op_listed(p.index, tile.begin + i, tile.begin, tile.end, p.x_rows, p.per_mul, p.per_shift) : tile.begin + i; };
   const auto write = [&](const int jt, const acc_f4 (&c)[OP_FM]) {
 #pragma unroll
@@ -324,9 +313,9 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
       for (int i = 0; i < OP_FM; ++i) {
         const int place = (n * OP_CHUNKS + q) * height + ((i * 16 + row) & (height - 1));
         const float f = sum[place];
-        second[i] = OP_ELT != 2 ? offset[place] : 0.0f;
+        second[i] = OP_ELT == 0 ? offset[place] : 0.0f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, second[i], OP_ZEROS ? (float)z.v[r] : 8.0f);
+        for (int r = 0; r < 4; ++r) t[i][r] = op_begin(f, OP_ZEROS ? (float)z.v[r] : 8.0f);
       }
 #pragma unroll
       for (int part = 0; part < OP_PARTS; ++part)
@@ -378,7 +367,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
         const int at = (n * OP_CHUNKS + q) * height + i * 16 + l;
         if (g == 0 && i * 16 + l < height) {
           sum[at] = t[0];
-          if (OP_ELT != 2) offset[at] = d[0];
+          if (OP_ELT == 0) offset[at] = d[0];
         }
       }
   __syncthreads();
@@ -442,7 +431,6 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
 #define OP_ROWS (16 * OP_PER)
 #define OP_SIZE ((int)sizeof(op_elt))
 #define OP_COLUMNS 256
-#define OP_SECOND (OP_ELT == 0 || (OP_ELT == 1 && OP_ZEROS))
 #define OP_LINE (OP_COLUMNS + 16)                  /* scales (zeros) of a group: 16 places in front, for a tile with fewer columns */
 
 /* What the 16 rows' places of a step's word b, quarter g are turned by: other numbers for all 16, so that a row's eighths go to other banks;
@@ -464,7 +452,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
   float *const scale = (float *)(x + 3 * 16 * OP_PARTS * OP_ROWS);         /* [3][chunks][OP_LINE], and the zeros' */
   float *const zero = scale + 3 * OP_CHUNKS * OP_LINE;
   float *const sum = OP_ZEROS ? zero + 3 * OP_CHUNKS * OP_LINE : zero;     /* [2][chunks][OP_ROWS]; what products begin with, where zeros are 8 */
-  float *const offset = sum + 2 * OP_CHUNKS * OP_ROWS;                     /* the second ones, where products want them */
+  float *const offset = sum + 2 * OP_CHUNKS * OP_ROWS;                     /* Float32: the second ones */
   acc_f4 c[OP_PER][4];
 #pragma unroll
   for (int i = 0; i < OP_PER; ++i)
@@ -532,8 +520,8 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
         op_sums(q, [&](const int b, const int part) { return row16(buffer, b, wave, part); }, t, d);
         const int at = (slot * OP_CHUNKS + q) * OP_ROWS + wave * 16 + l;
         if (g == 0) {
-          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], d[0], 8.0f);
-          if (OP_SECOND) offset[at] = d[0];
+          sum[at] = OP_ZEROS ? t[0] : op_begin(t[0], 8.0f);
+          if (OP_ELT == 0) offset[at] = d[0];
         }
       }
     };
@@ -579,7 +567,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
               for (int part = 0; part < OP_PARTS; ++part) y[b][i][part] = row16(now, q * OP_BLOCKS + b, i, part);
             const int at = ((n & 1) * OP_CHUNKS + q) * OP_ROWS + i * 16 + l;
             f[i] = sum[at];
-            o[i] = OP_SECOND ? offset[at] : 0.0f;
+            o[i] = OP_ELT == 0 ? offset[at] : 0.0f;
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -593,7 +581,7 @@ extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_pe
 #pragma unroll
             for (int i = 0; i < M; ++i)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], o[i], z[r]) : f[i];
+              for (int r = 0; r < 4; ++r) t[i][r] = OP_ZEROS ? op_begin(f[i], z[r]) : f[i];
 #pragma unroll
             for (int part = 0; part < OP_PARTS; ++part)
 #pragma unroll
@@ -694,7 +682,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
     };
     const auto add = [&](op_step &s) {
       const acc_f4 none = {0.0f, 0.0f, 0.0f, 0.0f};
-      const op_frag ones = op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES}), offsets = op_as_frag(op_offsets());
+      const op_frag ones = op_as_frag(acc_u4{OP_ONES, OP_ONES, OP_ONES, OP_ONES});
 #pragma unroll
       for (int j = 0; j < OP_FN; ++j) op_turn(s.w[j]);
 #pragma unroll
@@ -720,7 +708,6 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
               const op_frag y = op_as_frag(part[n]);
               acc_f4 &sums = n == 0 ? sum[i] : second[i];
               sums = op_mfma(ones, y, sums);
-              if (OP_ELT == 1) second[i] = op_mfma(offsets, y, second[i]);
 #pragma unroll
               for (int j = 0; j < OP_FN; ++j) {
                 acc_f4 &to = n == 0 ? t[i][j] : rest[i][j];
@@ -736,7 +723,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
             const float scale = (float)s.s[q][j].v[r], zero = OP_ZEROS ? (float)s.z[q][j].v[r] : 8.0f;
 #pragma unroll
             for (int i = 0; i < OP_FM; ++i) {
-              const float first = t[i][j][r] + op_begin(sum[i][r], second[i][r], zero);
+              const float first = t[i][j][r] + op_begin(sum[i][r], zero);
               c[i][j][r] = __builtin_fmaf(scale, OP_ELT == 0 ? first + op_rest(rest[i][j][r], second[i][r], zero) : first, c[i][j][r]);
             }
           }

@@ -4,6 +4,10 @@ takes, by results whose rounding is known to the last bit.
 A row of one group gives s T, T = sum x (q - z) a whole number.  Here x are whole numbers of at most 3, so T is exact in Float32 (100 times
 3 times 15: 13 bits), s T has at most 11 + 13 bits of a 16-bit scale and is exact too, and the result is the exact one rounded once.  Of
 Float32 scales the product is rounded, once, and that is the result.
+
+Rows whose numbers share a sign: of every group the kernels add up x (16 + q) and take (16 + z) sum x off, each of them below 31 sum x;
+with whole numbers that make this less than 2^24 everything is exact again, and so is the sum over the groups, with scales that are powers
+of two.  A form that adds more than 16 to a code loses digits there.
 """
 import sys
 
@@ -97,3 +101,20 @@ def test_an_infinity_in_a_row_of_any_form(rows, elt):
         say(elt, m, experts, n, k)
         got = values(rows(elt, 64, x, q, scales, zeros, offsets), elt)
         assert np.isnan(got[1:3]).all() and np.isfinite(np.delete(got, (1, 2), axis=0)).all(), (m, experts, n, k)
+
+
+@pytest.mark.parametrize("group", (32, 64, 128, 256))
+@pytest.mark.parametrize("elt", ("half", "bfloat16"))
+def test_rows_of_one_sign(rows, elt, group):
+    """x of all 11 (8) bits and one sign: 31 sum x of a group is below 2^24, and 15 sum x of a row"""
+    rng = np.random.default_rng(group)
+    for m, experts, n, k in ((3, 1, 70, 270), (129, 1, 70, 260), (40, 2, 3100, 273), (700, 2, 4, 100), (5000, 2, 300, 70), (1500, 25, 900, 257)):
+        q, _, zeros = matrices(rng, experts, n, k, group, elt, m % 2 == 1, True)
+        scales = 2.0 ** rng.integers(-8, -6, (experts, -(-k // group), n)).astype(np.float64)
+        most = 2047 if elt == "half" else 255
+        x = rng.integers(most // 2, most + 1, (m, k)).astype(np.float64)
+        assert 31 * min(k, group) * most < 2 ** 24 and 2 * 15 * k * most < 2 ** 24
+        offsets = segments(rng, m, experts, "even")
+        say(elt, group, m, experts, n, k)
+        want, _ = expected(x, weights(q, scales, zeros, group), offsets, m, None, 0)
+        assert np.array_equal(rows(elt, group, x, q, scales, zeros, offsets), store(want, elt)), (m, experts, n, k)
