@@ -200,7 +200,7 @@ struct ScratchBlock {
   bool busy = false;
   bool recorded = false;   // `done` was recorded at the last release
   bool kept = false;       // calls recorded into a graph on `stream` have it: lent to such calls only, not freed, until the stream goes
-  bool dirty = false;      // SCRATCH_LOCKS / SCRATCH_CARRY: a launch may have left it non-zero: cleared again before it is lent
+  bool dirty = false;      // cleared before it is lent (but not to a call that is recorded): new, or of SCRATCH_LOCKS / SCRATCH_CARRY, which a launch may have left non-zero
   uint32_t epoch = 0;
 };
 
@@ -288,7 +288,8 @@ struct acc_context_s {
   int make_current() const;
   // zero-initialised when first allocated; contents persist between uses and
   // follow the block's protocol
-  // `recorded` (SCRATCH_FOLD only): the call goes into a graph, which will use the block whenever it is replayed
+  // `recorded` (SCRATCH_FOLD, and SCRATCH_FLAGS where the call clears its words itself): the call goes into a graph, which will use
+  // the block whenever it is replayed
   int scratch_acquire(size_t bytes, hipStream_t stream, int protocol, acc::ScratchRef *out, bool recorded = false);
   void scratch_release(const acc::ScratchRef &ref, hipStream_t stream);
   // a borrower could not leave a SCRATCH_LOCKS / SCRATCH_CARRY block as it found it: cleared before it is lent again

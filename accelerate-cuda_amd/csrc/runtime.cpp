@@ -145,8 +145,9 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
       if (e != hipSuccess) { (void)hipFree(b.ptr); return acc::fail_hip(e, "hipEventCreateWithFlags"); }
     }
     b.protocol = protocol;
-    // cleared below, on the stream that first uses it; not in a graph, whose blocks' contents do not matter
-    b.dirty = !recorded;
+    // cleared below, on the stream that first uses it, but not in a graph: there whoever uses it clears what it needs, and the whole
+    // block is cleared when it is first lent to a call that is not recorded.  (Where contents do not matter neither does that.)
+    b.dirty = !recorded || protocol != acc::SCRATCH_FOLD;
     if (pick >= 0) {
       scratch[pick] = b;
     } else {
@@ -158,10 +159,12 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
   // tags: the scan's are 30 bits wide, the tagged words' 32
   const bool tags_out = (protocol == acc::SCRATCH_SCAN && b.epoch + 1 >= (1u << 30)) || (protocol == acc::SCRATCH_FLAGS && b.epoch == 0xFFFFFFFFu);
   if (b.dirty || tags_out) {
-    hipError_t e = hipMemsetAsync(b.ptr, 0, b.bytes, stream);
-    if (e != hipSuccess) return acc::fail_hip(e, "hipMemsetAsync(scratch)");
-    b.dirty = false;
-    b.epoch = 0;
+    if (!recorded) {
+      hipError_t e = hipMemsetAsync(b.ptr, 0, b.bytes, stream);
+      if (e != hipSuccess) return acc::fail_hip(e, "hipMemsetAsync(scratch)");
+    }
+    b.dirty = recorded;
+    b.epoch = recorded && !tags_out ? b.epoch : 0;
   }
   if (protocol == acc::SCRATCH_SCAN || protocol == acc::SCRATCH_FLAGS) ++b.epoch;
   b.busy = true;

@@ -1,0 +1,29 @@
+"""Calls of the operators at the edges of what they take, without a GPU: on a stand-in for the HIP runtime (operators_edges/edges.cpp)."""
+import os
+import subprocess
+
+import pytest
+
+HERE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "operators_edges")
+
+
+@pytest.fixture(scope="module")
+def edges(tmp_path_factory):
+    """run(part): what the program says about it"""
+    import acchip
+    out = tmp_path_factory.mktemp("edges")
+    build = subprocess.run(["make", "-j4", "-C", HERE, "OUT=%s" % out, "%s/edges" % out], capture_output=True, text=True)
+    assert build.returncode == 0, build.stdout[-3000:] + build.stderr[-3000:]
+    acchip.lib()
+    os.symlink(os.path.join(os.path.dirname(os.path.abspath(acchip.LIB_PATH)), "acc_compile_worker"), out / "acc_compile_worker")
+    (out / "cache").mkdir()
+
+    def run(part):
+        r = subprocess.run([str(out / "edges"), str(out / "cache"), part], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0 and "wrong 0" in r.stdout, r.stdout[-3000:] + r.stderr[-3000:]
+    return run
+
+
+def test_memory_first_lent_under_capture_is_cleared_before_an_eager_call(edges):
+    """a recurrence's tagged words: no fill goes into the graph, and none is missing behind it"""
+    edges("pool")
