@@ -197,12 +197,12 @@ ACC_DEV unsigned long long *op_words(const acc_recur_args &p, const long long ti
   return (unsigned long long *)p.words + (((tile * p.strips + strip) * 3 + plane) * 64 + lane) * OP_V;
 }
 
-/* sequences without a row leave what they enter with: every tile looks at a share of the sequences */
+/* sequences without a row leave what they enter with: every tile looks at a share of the sequences (steps in 64 bits: tiles may be millions) */
 ACC_DEV void op_empty_sequences(const acc_recur_args &p, const int rows, const int share, const int lane, const int channel, const int valid)
 {
   if (!p.leave) return;
-  for (int base = share * 64; base < p.sequences; base += p.tiles * OP_WAVES * 64) {
-    const int s = base + lane, n = acc_min(s, p.sequences - 1);
+  for (long long from = share * 64ll; from < p.sequences; from += p.tiles * (OP_WAVES * 64ll)) {
+    const int base = (int)from, s = base + lane, n = acc_min(s, p.sequences - 1);
     const int begin = acc_min(acc_max(p.offsets[n], 0), rows), end = acc_min(acc_max(p.offsets[n + 1], 0), rows);
     unsigned long long none = __ballot(s < p.sequences && end <= begin);
     while (none) {

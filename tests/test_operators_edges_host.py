@@ -27,3 +27,16 @@ def edges(tmp_path_factory):
 def test_memory_first_lent_under_capture_is_cleared_before_an_eager_call(edges):
     """a recurrence's tagged words: no fill goes into the graph, and none is missing behind it"""
     edges("pool")
+
+
+def test_sequences_without_a_row_are_found_whatever_the_tiles(tmp_path):
+    """op_recur.h's own arithmetic of shares, compiled for the host: no offset outside the array is read"""
+    csrc = os.path.join(os.path.dirname(HERE), "..", "accelerate-cuda_amd", "csrc", "operators")
+    with open(os.path.join(csrc, "op_recur.h")) as f:
+        text = f.read()
+    at = text.index("ACC_DEV void op_empty_sequences")
+    (tmp_path / "function.inc").write_text(text[at:text.index("\n}\n", at) + 3])
+    build = subprocess.run(["g++", "-O1", "-fwrapv", "-std=c++17", "-I%s" % tmp_path, "-o", str(tmp_path / "shares"), os.path.join(HERE, "shares.cpp")], capture_output=True, text=True)
+    assert build.returncode == 0, build.stderr[-3000:]
+    run = subprocess.run([str(tmp_path / "shares")], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "wrong 0" in run.stdout, run.stdout[-3000:]
