@@ -169,13 +169,14 @@ ACC_DEV bool op_get(const unsigned long long *d, const unsigned int tag, op_pair
 extern "C" __global__ void __launch_bounds__(256) recur_step(const acc_recur_args p)
 {
   if (p.guard && *p.guard == 0u) return;
-  const int channel = ((int)blockIdx.x % p.strips * 256 + (int)threadIdx.x) * OP_V, valid = acc_min(p.width - channel, OP_V);
-  const long long row = blockIdx.x / p.strips;
-  if (valid <= 0) return;
-  /* (asked for before it is known whether the row counts) */
-  const int at = acc_min(channel, p.width - OP_V), down = (channel - at) * 8 * (int)sizeof(op_elt);
-  const op_pair z = op_floats(op_read((const op_elt *)p.gates + row * p.gates_stride, at) >> down);
-  const op_pair x = op_floats(op_read((const op_elt *)p.values + row * p.values_stride, at) >> down);
+  const long long row = blockIdx.x / p.strips, left = p.width - (long long)(blockIdx.x % p.strips) * (256 * OP_V) - (int)threadIdx.x * OP_V;
+  if (left <= 0) return;
+  const int channel = (int)(p.width - left), valid = acc_min<long long>(left, OP_V);
+  /* (asked for before it is known whether the row counts; op_read and op_write count bytes in 32 bits, a row may have more) */
+  const long long at = acc_min(channel, p.width - OP_V);
+  const int down = (int)(channel - at) * 8 * (int)sizeof(op_elt);
+  const op_pair z = op_floats(op_read((const op_elt *)p.gates + row * p.gates_stride + at, 0) >> down);
+  const op_pair x = op_floats(op_read((const op_elt *)p.values + row * p.values_stride + at, 0) >> down);
   const long long slot = op_slot(p, (int)row);
   if (slot < 0) return;
   op_pair h = op_state(p.enter, p.enter_stride, slot, channel, valid);
@@ -185,7 +186,7 @@ extern "C" __global__ void __launch_bounds__(256) recur_step(const acc_recur_arg
     h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
   }
   op_keep(p.leave, p.leave_stride, slot, channel, valid, h);
-  op_write((op_elt *)p.out + row * p.out_stride, channel, false, valid, h);
+  op_write((op_elt *)p.out + row * p.out_stride + channel, 0, false, valid, h);
 }
 #else
 

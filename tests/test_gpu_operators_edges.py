@@ -83,3 +83,21 @@ def test_a_narrow_gradient_of_half_a_billion_rows(A, ctx):
     want[first] = 0.0                                          # (states of zeros: nothing comes before a first row)
     assert torch.equal(dgates, want)
     op.destroy()
+
+
+@pytest.mark.parametrize("elt,width", (("float", 2 ** 30 + 65), ("half", 2 ** 31 - 4097)))
+def test_a_step_of_more_than_a_billion_channels(A, ctx, elt, width):
+    """a row of 4 GB and more: every channel is read and written where it is"""
+    dtype = {"float": torch.float32, "half": torch.float16}[elt]
+    whole = lambda t: torch.randint(-9, 10, (1, width), dtype=torch.int8, device="cuda").to(t)
+    gates, values, state = torch.full((1, width), 0.5, dtype=dtype, device="cuda"), whole(dtype), whole(torch.float32)
+    out, last = torch.full_like(values, 77.0), torch.full_like(state, 77.0)
+    op = A.Recurrence(ctx, elt, "given")
+    torch.cuda.synchronize()
+    say(elt, width)
+    op.step(gates, values, state, last, out)
+    ctx.sync()
+    state.mul_(0.5).add_(values)                               # (halves of whole numbers: exact)
+    assert torch.equal(last, state)
+    assert torch.equal(out, state.to(dtype))
+    op.destroy()
