@@ -229,7 +229,9 @@ int guarded_copy(uint64_t dst, uint64_t src, size_t bytes, uint64_t guard, hipSt
 // a kernel of an operator (operators.cpp), traced and timed as the skeletons' are (execute.cpp)
 int launch_operator(acc_context ctx, const char *entry, hipFunction_t fn, unsigned grid, unsigned block, unsigned lds, hipStream_t stream, void **args);
 
-int scan_order_before(int device, hipStream_t stream);    // ACC_OK: the caller launches, then calls scan_order_after
+// ACC_OK: the caller launches, then calls scan_order_after; or, where `apart` is given and comes back true, launches a form that needs no
+// order, and does not
+int scan_order_before(int device, hipStream_t stream, bool *apart = nullptr);
 void scan_order_after(int device);
 void scan_order_forget(int device, hipStream_t stream);
 

@@ -1791,15 +1791,16 @@ static int launch_recur(acc_op op, const char *who, bool back, acc_recur_args &a
   if (hipStreamIsCapturing(st, &capture) != hipSuccess) (void)hipGetLastError();
   const bool recorded = capture != hipStreamCaptureStatusNone;
   // Workgroups that wait for others are the device's alone, as with the scans; what runs beside a graph nobody knows, so there tiles
-  // are drawn in the order in which workgroups start.
-  const bool ordered = tiles > 1 && !recorded;
-  if (ordered) ACC_TRY(acc::scan_order_before(op->ctx->device, st));
+  // are drawn in the order in which workgroups start, and so they are where the last call's stream is being recorded and cannot be waited for.
+  bool drawn = recorded;
+  if (tiles > 1 && !recorded) ACC_TRY(acc::scan_order_before(op->ctx->device, st, &drawn));
+  const bool ordered = tiles > 1 && !drawn;
   acc::ScratchRef scratch;
   int rc = op->ctx->scratch_acquire(256 + (size_t)words * 8, st, acc::SCRATCH_FLAGS, &scratch, recorded);
   if (rc == ACC_OK) {
     a.words = reinterpret_cast<uint64_t *>(static_cast<char *>(scratch.ptr) + 256);
     a.tag = scratch.epoch;
-    if (recorded) {
+    if (drawn) {
       a.ticket = static_cast<uint32_t *>(scratch.ptr);
       rc = launch(op, who, var->fn2, ceil_div(words, 256), 256, 0, stream, a);
     }

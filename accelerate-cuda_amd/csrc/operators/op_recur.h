@@ -17,7 +17,7 @@
  * the results.  That it finds in what the tiles before have left: their maps (A, B), or the state behind them (H), as 64-bit words
  * of a Float32 and the launch's tag, which need no fence.  A tile in which a sequence begins leaves a state at once.  Every tile
  * leaves its map without having waited, so waits end as long as the tiles before are on the device: workgroups start in the order of
- * their numbers, or (in a graph, beside which anything may run) draw them from a counter.
+ * their numbers, or (in a graph, or beside one that is being recorded: what else runs then nobody knows) draw them from a counter.
  */
 #include "op_common.h"
 
@@ -482,7 +482,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
   op_empty_sequences(p, rows, tile * OP_WAVES + wave, lane, channel, valid);
 }
 
-/* in a graph: no tile has left anything yet.  (The launches of a graph carry one tag.) */
+/* where tiles are drawn: no tile has left anything yet.  (The launches of a graph carry one tag.) */
 extern "C" __global__ void __launch_bounds__(256) recur_clear(const acc_recur_args p)
 {
   const long long words = (long long)p.tiles * p.strips * 3 * 64 * OP_V, i = (long long)blockIdx.x * 256 + threadIdx.x;

@@ -269,6 +269,9 @@ namespace acc {
 // earlier scan included).  Scans that follow one another on one stream -- the common case -- cost nothing.
 // scan_order_before takes the device's lock and scan_order_after gives it back, so that the launch itself lies
 // between them: a second thread must not record its event before the first one's scan is enqueued.
+// A last stream that is under capture by now cannot be waited for: an event recorded on it becomes a part of the graph, and a stream
+// that waits for that joins the capture; one recorded before, and the device, may not be waited for meanwhile.  Who has a form that
+// needs no order takes that one; other calls are refused.
 struct ScanOrder {
   std::mutex mu;
   hipEvent_t ev = nullptr;
@@ -278,13 +281,28 @@ struct ScanOrder {
 };
 static ScanOrder g_scan_order[64];
 
-int scan_order_before(int device, hipStream_t stream)
+int scan_order_before(int device, hipStream_t stream, bool *apart)
 {
   if (device < 0 || device >= 64) return ACC_OK;
   ScanOrder &o = g_scan_order[device];
   o.mu.lock();
   hipError_t e = hipSuccess;
-  if (o.have_last && o.last != stream) {
+  bool capturing = false;
+  if (o.have_last && o.last && o.last != stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    e = hipStreamIsCapturing(o.last, &status);
+    capturing = e == hipSuccess && status != hipStreamCaptureStatusNone;
+  }
+  if (capturing && apart) {
+    *apart = true;
+    o.mu.unlock();
+    return ACC_OK;
+  }
+  if (capturing) {
+    o.mu.unlock();
+    return fail(ACC_ERR_INVALID, "a scan that fills the device has to wait for the last one's stream, which is under capture");
+  }
+  if (e == hipSuccess && o.have_last && o.last != stream) {
     if (!o.ev) e = hipEventCreateWithFlags(&o.ev, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventRecord(o.ev, o.last);
     if (e == hipSuccess) e = hipStreamWaitEvent(stream, o.ev, 0);

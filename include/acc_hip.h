@@ -472,7 +472,9 @@ int acc_exec_foldseg_nd(acc_skel s, const acc_array *env, int32_t in_rank, const
 /* scans: scanOp / scan1Op / scan'Op / scanCore, Execute.hs:328-392.
  *   scanl, scanr    : out holds n+1 elements, `total` is ignored (may be NULL)
  *   scanl1, scanr1  : out holds n elements
- *   scanl', scanr'  : out holds n elements, total is a Scalar                */
+ *   scanl', scanr'  : out holds n elements, total is a Scalar
+ * One that the device does not hold at once waits for the last such call of another stream; while that stream is
+ * under capture it is refused (ACC_ERR_INVALID).                              */
 int acc_exec_scan(acc_skel s, const acc_array *env, int64_t n, const acc_array *out,
                   const acc_array *total, acc_stream stream);
 

@@ -19,7 +19,6 @@
 #define hipMemsetAsync mock_MemsetAsync
 #define hipEventRecord mock_EventRecord
 #define hipStreamWaitEvent mock_StreamWaitEvent
-#define hipDeviceSynchronize mock_DeviceSynchronize
 #include "../tsan/mock_hip.cpp"
 #undef hipStreamIsCapturing
 #undef hipModuleLaunchKernel
@@ -28,7 +27,6 @@
 #undef hipMemsetAsync
 #undef hipEventRecord
 #undef hipStreamWaitEvent
-#undef hipDeviceSynchronize
 
 struct Launch {
   std::string name;
@@ -44,8 +42,6 @@ static std::vector<Fill> g_fills;
 static uint64_t g_next = 1ull << 50;
 static int g_filled = 0;                          // fills that were asked for on the stream under capture
 static int g_joined = 0;                          // events recorded on the stream under capture, and waits of others for what it holds
-static int g_synchronised = 0;
-static hipError_t g_synchronise = hipSuccess;
 
 extern "C" {
 hipError_t hipStreamIsCapturing(hipStream_t s, hipStreamCaptureStatus *c)
@@ -76,7 +72,6 @@ hipError_t hipMemsetAsync(void *p, int, size_t n, hipStream_t s)
 }
 hipError_t hipEventRecord(hipEvent_t, hipStream_t s) { g_joined += s && s == g_capturing; return hipSuccess; }
 hipError_t hipStreamWaitEvent(hipStream_t, hipEvent_t, unsigned) { return hipSuccess; }
-hipError_t hipDeviceSynchronize(void) { ++g_synchronised; return g_synchronise; }
 }
 
 #define OK(call)                                                                        \
@@ -179,6 +174,66 @@ static void pool(acc_context ctx)
   OK(acc_op_destroy(op));
 }
 
+// eager calls of several tiles on other streams while the one that had the last such call is under capture
+static void order(acc_context ctx)
+{
+  acc_op op = recurrence(ctx);
+  acc_stream one = nullptr, two = nullptr;
+  OK(acc_stream_create(ctx, &one));
+  OK(acc_stream_create(ctx, &two));
+  scan(op, 5000, one);                            // (the call that is to be recorded, once)
+  under_capture(one);
+  const Launch recorded = scan(op, 5000, one);
+  const Launch eager = scan(op, 5000, two);
+  IS(g_joined == 0 && g_filled == 0);             // nothing of `two` waits for the capture, and nothing of it is recorded
+  IS(recorded.recur.words != eager.recur.words);
+  // it draws its tiles from a counter, which it has cleared: there is no order between it and what runs beside it
+  IS(eager.recur.ticket);
+  IS(g_launched[g_launched.size() - 2].name == "recur_clear" && g_launched[g_launched.size() - 2].recur.ticket == eager.recur.ticket);
+  scan(op, 5000, two);
+  IS(g_joined == 0);
+  under_capture(nullptr);
+  // and when the capture is over, everything is as before
+  IS(!scan(op, 5000, two).recur.ticket);
+  IS(!scan(op, 5000, one).recur.ticket);
+
+  // a large scan of the array language has no such form: it is refused, outside the capture
+  acc_env_sig env[1] = {};
+  env[0].rank = env[0].ncomp = 1;
+  env[0].type[0] = "Int32";
+  acc_skel_desc d = {};
+  d.kind = ACC_SKEL_SCANL1;
+  d.n_env = 1;
+  d.env = env;
+  d.elt_type = "Int32";
+  d.out_rank = 1;
+  d.get = "arrIn0_0[ix]";
+  d.combine = "x + y";
+  acc_skel skel = nullptr;
+  OK(acc_skel_create(ctx, &d, &skel));
+  acc_array in = {}, out = {};
+  in.rank = in.ncomp = out.rank = out.ncomp = 1;
+  in.shape[0] = out.shape[0] = int64_t(1) << 30;
+  in.ptr[0] = 1ull << 44;
+  out.ptr[0] = 1ull << 45;
+  OK(acc_exec_scan(skel, &in, in.shape[0], &out, nullptr, one));
+  OK(acc_exec_scan(skel, &in, in.shape[0], &out, nullptr, two));
+  OK(acc_exec_scan(skel, &in, in.shape[0], &out, nullptr, one));
+  under_capture(one);
+  const size_t launched = g_launched.size();
+  IS(acc_exec_scan(skel, &in, in.shape[0], &out, nullptr, two) == ACC_ERR_INVALID);
+  IS(g_joined == 0 && g_launched.size() == launched);
+  in.shape[0] = out.shape[0] = 1000;              // (one that waits for nothing)
+  OK(acc_exec_scan(skel, &in, in.shape[0], &out, nullptr, two));
+  in.shape[0] = out.shape[0] = int64_t(1) << 30;
+  under_capture(nullptr);
+  OK(acc_exec_scan(skel, &in, in.shape[0], &out, nullptr, two));
+  OK(acc_skel_destroy(skel));
+  OK(acc_stream_destroy(ctx, one));
+  OK(acc_stream_destroy(ctx, two));
+  OK(acc_op_destroy(op));
+}
+
 int main(int, char **argv)
 {
   OK(acc_init());
@@ -187,6 +242,7 @@ int main(int, char **argv)
   OK(acc_context_create(0, &ctx));
   const std::string part = argv[2];
   if (part == "pool") pool(ctx);
+  else if (part == "order") order(ctx);
   else IS(!"a part that there is");
   OK(acc_context_destroy(ctx));
   std::printf("wrong %d\n", g_wrong);

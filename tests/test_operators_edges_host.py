@@ -29,6 +29,11 @@ def test_memory_first_lent_under_capture_is_cleared_before_an_eager_call(edges):
     edges("pool")
 
 
+def test_eager_calls_do_not_join_the_capture_of_another_stream(edges):
+    """recurrences and scans of many tiles are in order across streams; the last one's stream may be under capture by then"""
+    edges("order")
+
+
 def test_sequences_without_a_row_are_found_whatever_the_tiles(tmp_path):
     """op_recur.h's own arithmetic of shares, compiled for the host: no offset outside the array is read"""
     csrc = os.path.join(os.path.dirname(HERE), "..", "accelerate-cuda_amd", "csrc", "operators")
