@@ -199,6 +199,7 @@ struct ScratchBlock {
   hipEvent_t done = nullptr;
   bool busy = false;
   bool recorded = false;   // `done` was recorded at the last release
+  bool unsettled = false;  // it was not, and nobody has waited for the block's last use since: `stream`'s alone
   bool kept = false;       // calls recorded into a graph on `stream` have it: lent to such calls only, not freed, until the stream goes
   bool dirty = false;      // cleared before it is lent (but not to a call that is recorded): new, or of SCRATCH_LOCKS / SCRATCH_CARRY, which a launch may have left non-zero
   uint32_t epoch = 0;

@@ -110,6 +110,14 @@ int acc_context_s::make_current() const
   return ACC_OK;
 }
 
+// Whether a stream is under capture.  Asking for an event that was recorded on it before, or waiting for the device, would end the capture.
+static bool under_capture(hipStream_t stream)
+{
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (stream && hipStreamIsCapturing(stream, &status) != hipSuccess) (void)hipGetLastError();
+  return status != hipStreamCaptureStatusNone;
+}
+
 int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protocol, acc::ScratchRef *out, bool recorded)
 {
   std::lock_guard<std::mutex> lock(mu);
@@ -119,7 +127,11 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
   } else if (!scratch_multi_stream && stream != scratch_first_stream) {
     // a second stream shows up: settle everything enqueued so far once, and
     // track completion with events from here on
-    ACC_HIP_TRY(hipDeviceSynchronize());
+    if (under_capture(scratch_first_stream) || under_capture(stream)) {
+      for (acc::ScratchBlock &b : scratch) b.unsettled = true;      // (that stream's alone until it has had them once more)
+    } else {
+      ACC_HIP_TRY(hipDeviceSynchronize());
+    }
     scratch_multi_stream = true;
   }
   int pick = -1;
@@ -127,8 +139,8 @@ int acc_context_s::scratch_acquire(size_t bytes, hipStream_t stream, int protoco
     acc::ScratchBlock &b = scratch[i];
     if (b.busy || b.bytes < bytes || b.protocol != protocol) continue;
     if (b.kept && !(recorded && b.stream == stream)) continue;       // (a stream's graphs are replayed one behind the other)
-    bool reusable = (b.stream == stream) || !b.recorded;
-    if (!reusable) reusable = (hipEventQuery(b.done) == hipSuccess);
+    bool reusable = (b.stream == stream) || !(b.recorded || b.unsettled);
+    if (!reusable && b.recorded && !under_capture(b.stream)) reusable = (hipEventQuery(b.done) == hipSuccess);
     if (reusable && (pick < 0 || b.bytes < scratch[pick].bytes)) pick = static_cast<int>(i);
   }
   if (pick < 0) {
@@ -182,7 +194,7 @@ void acc_context_s::scratch_release(const acc::ScratchRef &ref, hipStream_t stre
   if (ref.index < 0) return;
   std::lock_guard<std::mutex> lock(mu);
   acc::ScratchBlock &b = scratch[ref.index];
-  b.recorded = false;
+  b.recorded = b.unsettled = false;
   if (scratch_multi_stream && !b.kept) b.recorded = (hipEventRecord(b.done, stream) == hipSuccess);
   b.stream = stream;
   b.busy = false;
@@ -200,7 +212,7 @@ void acc_context_s::scratch_forget(hipStream_t stream)
   std::lock_guard<std::mutex> lock(mu);
   for (acc::ScratchBlock &b : scratch) {
     if (!b.kept || b.stream != stream) continue;
-    b.kept = false;
+    b.kept = b.unsettled = false;
     b.recorded = (hipEventRecord(b.done, stream) == hipSuccess);      // behind whatever of a replay is still under way
     if (!b.recorded) { (void)hipGetLastError(); (void)hipStreamSynchronize(stream); }
   }
@@ -227,7 +239,7 @@ size_t acc_context_s::scratch_trim()
     b.ptr = nullptr;
     b.bytes = 0;
     b.epoch = 0;
-    b.recorded = false;
+    b.recorded = b.unsettled = false;
   }
   // empty entries at the end can go
   while (!scratch.empty() && !scratch.back().ptr && !scratch.back().busy) {

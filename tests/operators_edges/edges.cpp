@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <map>
 #include <string>
 #include <vector>
 
@@ -19,6 +20,8 @@
 #define hipMemsetAsync mock_MemsetAsync
 #define hipEventRecord mock_EventRecord
 #define hipStreamWaitEvent mock_StreamWaitEvent
+#define hipEventQuery mock_EventQuery
+#define hipDeviceSynchronize mock_DeviceSynchronize
 #include "../tsan/mock_hip.cpp"
 #undef hipStreamIsCapturing
 #undef hipModuleLaunchKernel
@@ -27,6 +30,8 @@
 #undef hipMemsetAsync
 #undef hipEventRecord
 #undef hipStreamWaitEvent
+#undef hipEventQuery
+#undef hipDeviceSynchronize
 
 struct Launch {
   std::string name;
@@ -41,6 +46,9 @@ static std::vector<Launch> g_launched;
 static std::vector<Fill> g_fills;
 static uint64_t g_next = 1ull << 50;
 static int g_filled = 0;                          // fills that were asked for on the stream under capture
+static std::map<hipEvent_t, hipStream_t> g_recorded_on;
+static int g_ended = 0;                           // captures that a call on another stream has ended
+static bool g_done = true;                        // what has been enqueued
 static int g_joined = 0;                          // events recorded on the stream under capture, and waits of others for what it holds
 
 extern "C" {
@@ -70,7 +78,24 @@ hipError_t hipMemsetAsync(void *p, int, size_t n, hipStream_t s)
   g_fills.push_back({reinterpret_cast<uint64_t>(p), reinterpret_cast<uint64_t>(p) + n, s, g_launched.size()});
   return hipSuccess;
 }
-hipError_t hipEventRecord(hipEvent_t, hipStream_t s) { g_joined += s && s == g_capturing; return hipSuccess; }
+hipError_t hipEventRecord(hipEvent_t e, hipStream_t s)
+{
+  g_joined += s && s == g_capturing;
+  g_recorded_on[e] = s;
+  return hipSuccess;
+}
+// (either ends the capture, as the HIP runtime has it)
+hipError_t hipEventQuery(hipEvent_t e)
+{
+  const bool captured = g_capturing && g_recorded_on[e] == g_capturing;
+  g_ended += captured;
+  return captured ? hipErrorCapturedEvent : g_done ? hipSuccess : hipErrorNotReady;
+}
+hipError_t hipDeviceSynchronize(void)
+{
+  g_ended += g_capturing != nullptr;
+  return g_capturing ? hipErrorStreamCaptureUnsupported : hipSuccess;
+}
 hipError_t hipStreamWaitEvent(hipStream_t, hipEvent_t, unsigned) { return hipSuccess; }
 }
 
@@ -234,6 +259,41 @@ static void order(acc_context ctx)
   OK(acc_op_destroy(op));
 }
 
+// scratch memory of eager calls while another stream is under capture: what that stream had last is not asked for
+static void beside(acc_context ctx)
+{
+  acc_op op = recurrence(ctx);
+  acc_stream one = nullptr, two = nullptr, three = nullptr;
+  OK(acc_stream_create(ctx, &one));
+  OK(acc_stream_create(ctx, &two));
+  OK(acc_stream_create(ctx, &three));
+  // one stream alone has had scratch memory, and is under capture when a second one wants some
+  const Launch first = scan(op, 5000, one);
+  under_capture(one);
+  const Launch other = scan(op, 5000, two);
+  IS(g_ended == 0 && g_joined == 0 && other.recur.words != first.recur.words);
+  const Launch recorded = scan(op, 5000, one);
+  IS(recorded.recur.words == first.recur.words);  // (that stream's own)
+  under_capture(nullptr);
+  // several have had some
+  g_done = false;
+  const Launch third = scan(op, 5000, three);
+  IS(third.recur.words != other.recur.words && third.recur.words != recorded.recur.words);
+  under_capture(two);
+  g_done = true;
+  const Launch fourth = scan(op, 6000, three);
+  IS(g_ended == 0 && g_joined == 0 && fourth.recur.words != other.recur.words);
+  under_capture(nullptr);
+  // and afterwards it is anybody's
+  const Launch fifth = scan(op, 4000, one);
+  IS(fifth.recur.words == other.recur.words || fifth.recur.words == third.recur.words || fifth.recur.words == fourth.recur.words);
+  IS(g_ended == 0);
+  OK(acc_stream_destroy(ctx, one));
+  OK(acc_stream_destroy(ctx, two));
+  OK(acc_stream_destroy(ctx, three));
+  OK(acc_op_destroy(op));
+}
+
 int main(int, char **argv)
 {
   OK(acc_init());
@@ -243,6 +303,7 @@ int main(int, char **argv)
   const std::string part = argv[2];
   if (part == "pool") pool(ctx);
   else if (part == "order") order(ctx);
+  else if (part == "beside") beside(ctx);
   else IS(!"a part that there is");
   OK(acc_context_destroy(ctx));
   std::printf("wrong %d\n", g_wrong);

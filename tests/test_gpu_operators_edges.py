@@ -1,5 +1,6 @@
 """The recurrence, the router by scores and the grouped 4-bit products at the edges of what they take (include/acc_hip.h, section D): rows and
 channels in their billions, by results that are known without a second computation as large."""
+import ctypes as C
 import sys
 
 import numpy as np
@@ -100,4 +101,63 @@ def test_a_step_of_more_than_a_billion_channels(A, ctx, elt, width):
     state.mul_(0.5).add_(values)                               # (halves of whole numbers: exact)
     assert torch.equal(last, state)
     assert torch.equal(out, state.to(dtype))
+    op.destroy()
+
+
+@pytest.fixture(scope="module")
+def hip():
+    h = C.CDLL("libamdhip64.so")
+    h.hipStreamBeginCapture.argtypes = [C.c_void_p, C.c_int]
+    h.hipStreamEndCapture.argtypes = [C.c_void_p, C.POINTER(C.c_void_p)]
+    h.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+    h.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+    h.hipGraphExecDestroy.argtypes = h.hipGraphDestroy.argtypes = [C.c_void_p]
+    return h
+
+
+def test_eager_calls_beside_a_capture(A, ctx, hip):
+    """a recurrence on one stream while the stream of the last such call is being recorded: it runs at once, and is no part of the graph; a
+    large scan, which would have to wait for that stream, is refused, and not recorded either"""
+    rng, rows, width, n = np.random.default_rng(4), 6000, 200, 1 << 26
+    z, x = (rng.standard_normal((rows, width)).astype(np.float32) for _ in range(2))
+    z, x, offsets = ctx.array(z), ctx.array(x), ctx.array(np.array([0, 2500, rows], np.int32))
+    outs = [ctx.empty((rows, width), np.float32) for _ in range(2)]
+    op = A.Recurrence(ctx, "float", "sigmoid")
+    skel = ctx.skeleton(A.SKEL_SCANL1, "Int32", env=[(1, "Int32")], get="arrIn0_0[ix]", combine="x + y")
+    ones, sums = ctx.array(np.ones(n, np.int32)), [ctx.empty((n,), np.int32) for _ in range(2)]
+    one, two = ctx.stream(), ctx.stream()
+    for stream, out, total in zip((one, two, one), (*outs, outs[0]), (*sums, sums[0])):
+        skel.scan([ones], n, total, stream=stream)
+        op.scan(z, x, offsets, out, stream=stream)
+    ctx.sync()
+    want = outs[0].get().copy()
+    assert np.array_equal(outs[1].get(), want)
+    for a in (*outs, sums[1]):
+        a.set(np.full(a.shape, 7, a.dtype))
+    graph, graph_exec = C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(one, 2) == 0
+    try:
+        op.scan(z, x, offsets, outs[0], stream=one)
+        op.scan(z, x, offsets, outs[1], stream=two)
+        with pytest.raises(A.AccError) as refused:
+            skel.scan([ones], n, sums[1], stream=two)
+        assert refused.value.code == A.ERR_INVALID
+    finally:
+        rc = hip.hipStreamEndCapture(one, C.byref(graph))
+    assert rc == 0 and graph.value and hip.hipGraphInstantiate(C.byref(graph_exec), graph, None, None, 0) == 0
+    ctx.sync()
+    assert np.array_equal(outs[1].get(), want) and np.all(outs[0].get() == 7.0) and np.all(sums[1].get() == 7)
+    skel.scan([ones], n, sums[1], stream=two)
+    ctx.sync()
+    assert np.array_equal(sums[1].get(), np.arange(1, n + 1, dtype=np.int32))
+    for replay in range(4):
+        outs[0].set(np.full((rows, width), 9.0, np.float32))
+        outs[1].set(np.full((rows, width), 9.0, np.float32))
+        ctx.sync()
+        assert hip.hipGraphLaunch(graph_exec, one) == 0
+        op.scan(z, x, offsets, outs[1], stream=two)
+        ctx.sync()
+        assert np.array_equal(outs[0].get(), want) and np.array_equal(outs[1].get(), want), replay
+    hip.hipGraphExecDestroy(graph_exec)
+    hip.hipGraphDestroy(graph)
     op.destroy()

@@ -34,6 +34,11 @@ def test_eager_calls_do_not_join_the_capture_of_another_stream(edges):
     edges("order")
 
 
+def test_eager_calls_do_not_end_the_capture_of_another_stream(edges):
+    """asking for an event of that stream would, and so would waiting for the device"""
+    edges("beside")
+
+
 def test_sequences_without_a_row_are_found_whatever_the_tiles(tmp_path):
     """op_recur.h's own arithmetic of shares, compiled for the host: no offset outside the array is read"""
     csrc = os.path.join(os.path.dirname(HERE), "..", "accelerate-cuda_amd", "csrc", "operators")
