@@ -8,7 +8,10 @@
  *
  * Both are scans of the maps h -> A h + B, the second from the last row to the first (OP_BACK; rows are counted from the end
  * then).  A row that begins a sequence takes nothing of the row before: it replaces, it does not multiply, so that no infinity
- * and nothing that is not a number passes from one sequence to the next.
+ * and nothing that is not a number passes from one sequence to the next.  A map is no good where A or B is not finite (gates above 1,
+ * whose product overflows though the state is small or 0) or the state is infinite (of which an A that has become 0 would make NaN):
+ * such a tile waits for the state in front of it, and its waves take their rows one after the other, as the definition has it.  (Half,
+ * one sequence of 65536 x 512: 56 us, 12000 where every tile's product overflows.)
  *
  * Bound by memory: every array passes by once.  bfloat16, 32768 rows of 2048 in 8 sequences, sigmoids: 101 us, 4.0 TB/s, the gradient 170,
  * 4.7 (a copy 5.4); what is short of that are the gates, worked out in both passes.  One sequence of 65536 half rows of 512: 56, 3.6, the
@@ -191,6 +194,12 @@ extern "C" __global__ void __launch_bounds__(256) recur_step(const acc_recur_arg
 #else
 
 struct op_map { op_pair a, b; };
+ACC_DEV float op_largest(const op_pair &f, float most)       /* (what is not a number is not) */
+{
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) most = __builtin_fmaxf(most, __builtin_fabsf(f.v[k]));
+  return most;
+}
 
 /* the words of a tile's strip: A, B, H */
 ACC_DEV unsigned long long *op_words(const acc_recur_args &p, const long long tile, const int strip, const int plane, const int lane)
@@ -221,6 +230,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
   __shared__ op_map maps[OP_NEAR][64];             /* of the waves' rows; then of the tiles before */
   __shared__ int ends[OP_NEAR];                    /* whether a wave's map forgets what comes in (1), from its first row on (2); then what is there */
   __shared__ unsigned int drawn;
+  __shared__ op_pair carried[64];                  /* from wave to wave, where they take turns */
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), rows = (int)p.rows;
   unsigned int number = blockIdx.x;
   if (p.ticket) {
@@ -319,6 +329,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
     all.b.v[k] = 0.0f;
   }
   mine = all;
+  float off = 0.0f;                                /* is not a number if one of the sums, or the product of all, is not finite */
   const bool fresh = __builtin_amdgcn_readfirstlane(ends[0]) == 2;
 #pragma unroll
   for (int w = 0; w < OP_WAVES; ++w) {
@@ -334,10 +345,16 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
       all.a.v[k] *= m.a.v[k];
     }
     all_ends = all_ends || e;
+#pragma unroll
+    for (int k = 0; k < OP_V; ++k) off = __builtin_fmaf(all.b.v[k], 0.0f, off);
   }
+#pragma unroll
+  for (int k = 0; k < OP_V; ++k) off = __builtin_fmaf(all.a.v[k], 0.0f, off);
+  const unsigned long long off_lanes = __ballot(off != 0.0f);
+  bool odd = off_lanes != 0;                       /* (of any channel: the waves go together) */
   const bool known = all_ends || tile == 0;
   __syncthreads();                                 /* (everybody has read them) */
-  if (wave == 0) {
+  if (wave == 0 && !odd) {
     if (known) {
       op_put(op_words(p, tile, strip, 2, lane), p.tag, all.b);
     } else {
@@ -348,7 +365,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
 
   /* What comes in.  Of the tiles in front the nearest OP_NEAR are looked at, a wave takes every eighth, until the nearest state among
    * them is followed by maps alone; those are applied to it one after the other.  (So a state is the same whoever has put it
-   * together, to the last bit.) */
+   * together, to the last bit.)  If it is infinite on the way it is the state of the tile before that counts. */
   op_pair in;
 #pragma unroll
   for (int k = 0; k < OP_V; ++k) in.v[k] = 0.0f;
@@ -384,24 +401,35 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
       const unsigned long long states = __ballot(seen == 2), nothing = __ballot(seen == 0);
       __syncthreads();
       nearest = __builtin_ctzll(states | 1ull << 63);
-      if (nearest < __builtin_ctzll(nothing)) break;           /* (lane 63 has seen nothing) */
+      if (nearest < __builtin_ctzll(nothing)) {    /* (lane 63 has seen nothing) */
+        in = maps[nearest][lane].b;
+        float most = op_largest(in, 0.0f);
+        for (int left = nearest; left > 0; left -= 4) {        /* (four at a time, those that there are not change nothing) */
+          op_map m[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) m[n] = maps[acc_max(left - 1 - n, 0)][lane];
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int k = 0; k < OP_V; ++k) {
+              in.v[k] = n < left ? __builtin_fmaf(m[n].a.v[k], in.v[k], m[n].b.v[k]) : in.v[k];
+              most = __builtin_fmaxf(most, __builtin_fabsf(in.v[k]));
+            }
+        }
+        if (nearest == 0 || __ballot(most == __builtin_inff()) == 0) break;
+        __syncthreads();                           /* (everybody has read them, and found the same) */
+      }
       if (++polls >= ACC_SPIN_LIMIT) {
         if (tid == 0) acc_report(p.status, ACC_STATUS_SCAN_LOOKBACK);
-        nearest = 0;
         break;
       }
     }
-    in = maps[nearest][lane].b;
-    for (; nearest > 0; nearest -= 8) {            /* (eight at a time, those that there are not change nothing) */
-      op_map m[8];
+    /* (where what comes in is not a number, neither is what goes out, whatever the map) */
+    bool none = !all_ends;
 #pragma unroll
-      for (int n = 0; n < 8; ++n) m[n] = maps[acc_max(nearest - 1 - n, 0)][lane];
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int k = 0; k < OP_V; ++k) in.v[k] = n < nearest ? __builtin_fmaf(m[n].a.v[k], in.v[k], m[n].b.v[k]) : in.v[k];
-    }
-    if (wave == 0 && !known) {
+    for (int k = 0; k < OP_V; ++k) none = none && in.v[k] != in.v[k];
+    odd = (off_lanes & ~__ballot(none)) != 0 || __ballot(op_largest(in, 0.0f) == __builtin_inff()) != 0;
+    if (wave == 0 && !known && !odd) {
       op_pair h;
 #pragma unroll
       for (int k = 0; k < OP_V; ++k) h.v[k] = __builtin_fmaf(all.a.v[k], in.v[k], all.b.v[k]);
@@ -412,72 +440,83 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) __attribute__((amdgp
   /* the results, sequence after sequence: what comes in, or what one that begins here enters with */
   op_pair h;
 #pragma unroll
-  for (int k = 0; k < OP_V; ++k) h.v[k] = mine_ends ? mine.b.v[k] : __builtin_fmaf(mine.a.v[k], in.v[k], mine.b.v[k]);
+  for (int k = 0; k < OP_V; ++k) h.v[k] = odd ? in.v[k] : mine_ends ? mine.b.v[k] : __builtin_fmaf(mine.a.v[k], in.v[k], mine.b.v[k]);
 #if OP_BACK
   shift_rows(hw);
   if (OP_GATE) shift_rows(vw);
 #endif
-  for (int begin = 0; begin < OP_R;) {
-    const unsigned long long more = resets & ~0ull << begin << 1;
-    const int next = more ? __builtin_ctzll(more) : OP_R;
-    const unsigned long long run = here & ~0ull << begin & ((1ull << next) - 1);
-    if (resets >> begin & 1) {
-      h = entered;
-      if (begin != latest) h = entering(begin);
+  for (int turn = 0; turn < (odd ? OP_WAVES : 1); ++turn) {
+    if (odd) {
+      __syncthreads();
+      if (turn != wave) continue;
+      if (wave > 0) h = carried[lane];
     }
-    const int final = run & leaves ? __builtin_ctzll(run & leaves) : -1;
-    const long long slot = final >= 0 ? op_slot(p, sequence_of(final)) : -1;
+    for (int begin = 0; begin < OP_R;) {
+      const unsigned long long more = resets & ~0ull << begin << 1;
+      const int next = more ? __builtin_ctzll(more) : OP_R;
+      const unsigned long long run = here & ~0ull << begin & ((1ull << next) - 1);
+      if (resets >> begin & 1) {
+        h = entered;
+        if (begin != latest) h = entering(begin);
+      }
+      const int final = run & leaves ? __builtin_ctzll(run & leaves) : -1;
+      const long long slot = final >= 0 ? op_slot(p, sequence_of(final)) : -1;
 #if OP_BACK
-    const op_pair started = op_state(p.state, p.state_stride, slot, channel, valid);
-    op_elt *dgates = (op_elt *)p.dgates + (first + OP_R - 1) * p.dgates_stride, *dvalues = (op_elt *)p.dvalues + (first + OP_R - 1) * p.dvalues_stride;
-    asm volatile("" : "+s"(dgates), "+s"(dvalues));      /* (or the rows' addresses are kept in registers from sequence to sequence) */
+      const op_pair started = op_state(p.state, p.state_stride, slot, channel, valid);
+      op_elt *dgates = (op_elt *)p.dgates + (first + OP_R - 1) * p.dgates_stride, *dvalues = (op_elt *)p.dvalues + (first + OP_R - 1) * p.dvalues_stride;
+      asm volatile("" : "+s"(dgates), "+s"(dvalues));      /* (or the rows' addresses are kept in registers from sequence to sequence) */
 #else
-    op_elt *out = (op_elt *)p.out + first * p.out_stride;
-    asm volatile("" : "+s"(out));                        /* (or the rows' addresses are kept in registers from sequence to sequence) */
+      op_elt *out = (op_elt *)p.out + first * p.out_stride;
+      asm volatile("" : "+s"(out));                        /* (or the rows' addresses are kept in registers from sequence to sequence) */
 #endif
 #pragma unroll
-    for (int r = 0; r < OP_R; ++r) {
-      if (run >> r & 1) {
-        const op_pair z = op_again(zw[r]), x = op_again(xw[r]);
+      for (int r = 0; r < OP_R; ++r) {
+        if (run >> r & 1) {
+          const op_pair z = op_again(zw[r]), x = op_again(xw[r]);
 #if OP_BACK
-        op_pair b = op_again(hw[r]), dz, dx;
-        if (r == final) b = started;
+          op_pair b = op_again(hw[r]), dz, dx;
+          if (r == final) b = started;
 #if OP_GATE
-        const op_pair v = op_again(vw[r]);
+          const op_pair v = op_again(vw[r]);
 #endif
 #pragma unroll
-        for (int k = 0; k < OP_V; ++k) {
-          const op_gate g = op_gate_of(z.v[k]);
-          const float d = x.v[k] + h.v[k];
-          h.v[k] = g.keep * d;
+          for (int k = 0; k < OP_V; ++k) {
+            const op_gate g = op_gate_of(z.v[k]);
+            const float d = x.v[k] + h.v[k];
+            h.v[k] = g.keep * d;
 #if OP_GATE
-          dx.v[k] = g.take * d;
-          dz.v[k] = (b.v[k] - v.v[k]) * (g.keep * dx.v[k]);
+            dx.v[k] = g.take * d;
+            dz.v[k] = (b.v[k] - v.v[k]) * (g.keep * dx.v[k]);
 #else
-          dx.v[k] = d;
-          dz.v[k] = b.v[k] * d;
+            dx.v[k] = d;
+            dz.v[k] = b.v[k] * d;
+#endif
+          }
+          op_write(dgates, channel, whole, valid, dz);
+          op_write(dvalues, channel, whole, valid, dx);
+#else
+#pragma unroll
+          for (int k = 0; k < OP_V; ++k) {
+            const op_gate g = op_gate_of(z.v[k]);
+            h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
+          }
+          op_write(out, channel, whole, valid, h);
 #endif
         }
-        op_write(dgates, channel, whole, valid, dz);
-        op_write(dvalues, channel, whole, valid, dx);
+#if OP_BACK
+        dgates -= p.dgates_stride;
+        dvalues -= p.dvalues_stride;
 #else
-#pragma unroll
-        for (int k = 0; k < OP_V; ++k) {
-          const op_gate g = op_gate_of(z.v[k]);
-          h.v[k] = __builtin_fmaf(g.keep, h.v[k], g.take * x.v[k]);
-        }
-        op_write(out, channel, whole, valid, h);
+        out += p.out_stride;
 #endif
       }
-#if OP_BACK
-      dgates -= p.dgates_stride;
-      dvalues -= p.dvalues_stride;
-#else
-      out += p.out_stride;
-#endif
+      if (final >= 0) op_keep(p.leave, p.leave_stride, slot, channel, valid, h);
+      begin = next;
     }
-    if (final >= 0) op_keep(p.leave, p.leave_stride, slot, channel, valid, h);
-    begin = next;
+    if (odd) {
+      carried[lane] = h;
+      if (wave == OP_WAVES - 1) op_put(op_words(p, tile, strip, 2, lane), p.tag, h);
+    }
   }
   op_empty_sequences(p, rows, tile * OP_WAVES + wave, lane, channel, valid);
 }

@@ -794,6 +794,8 @@ int acc_exec_grouped_rows(acc_op op, const acc_strided *x, const acc_strided *co
  * or NULL: what sequences begin with (NULL: zeros) and where the states behind their last rows go; both may be the same array.
  * Sequence s has row index[s] of them, or row s without index; one that the states do not have begins with zeros and is not
  * kept.  A sequence without rows leaves the state that it begins with.  No two sequences may leave the same row.
+ * Gates may be any numbers: products of them, and states, beyond Float32's range give what the definition gives, row by
+ * row, though a long sequence then takes its tiles one behind the other.
  * (For long sequences tiles of rows wait for what earlier ones leave, as those of acc_exec_scan do: ACC_ERR_STUCK.) */
 int acc_exec_recur(acc_op op, const acc_strided *gates, const acc_strided *values, const acc_strided *offsets, const acc_strided *index,
                    const acc_strided *state, const acc_strided *last, const acc_strided *out, acc_stream stream);
