@@ -97,7 +97,7 @@ ACC_DEV int op_index_of(const double key)
  * one of the exponential and a part of the product's in front of it, 2.3 10^-7 together, and what is ranked by half a unit more: two
  * by twice that.  And what a group's sum may be off itself. */
 ACC_DEV float op_near(const float v) { return 6e-7f + 1.6e-7f * __builtin_fabsf(v); }
-ACC_DEV float op_off(const float best, const float next) { return 6e-7f + 1.6e-7f * (__builtin_fabsf(best) + (next > OP_NONE ? __builtin_fabsf(next) : 0.0f)); }
+ACC_DEV float op_off(const float best, const float next) { return 6e-7f + 1.6e-7f * __builtin_fabsf(best) + (next > OP_NONE ? 1.6e-7f * __builtin_fabsf(next) : 0.0f); }
 
 ACC_DEV void op_insert(double (&k)[OP_KEYS], const double y)
 {
@@ -114,6 +114,8 @@ ACC_DEV void op_put(op_two &t, const float v)
   t.best = v > t.best ? v : t.best;
 }
 template <typename T> ACC_DEV T op_sum_of(const T best, const T next) { return next > (T)OP_NONE ? best + next : best; }
+/* (of biases of the type's lowest value, too, the sum of a group that has something to choose is no infinity: near others, not none) */
+ACC_DEV float op_group_sum(const op_two &t) { return t.best > OP_NONE ? acc_max(-3.40282347e38f, acc_min(3.40282347e38f, op_sum_of(t.best, t.next))) : OP_NONE; }
 
 ACC_DEV float op_logit(const acc_route_args &p, const long long t, const int e) { return (float)((const op_elt *)p.logits)[t * p.logits_stride + e]; }
 ACC_DEV float op_bias(const acc_route_args &p, const int e) { return p.bias ? p.bias[e] : 0.0f; }
@@ -246,7 +248,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_SELECT_WAVES) score(const a
           op_put(two, next);
         }
       }
-      const float s = op_sum_of(two.best, two.next), off = op_off(two.best, two.next);
+      const float s = op_group_sum(two), off = op_off(two.best, two.next);
       groups[2 * own] = s;
       groups[2 * own + 1] = off;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
