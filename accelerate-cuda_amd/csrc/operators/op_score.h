@@ -121,8 +121,8 @@ ACC_DEV float op_logit(const acc_route_args &p, const long long t, const int e) 
 ACC_DEV float op_bias(const acc_route_args &p, const int e) { return p.bias ? p.bias[e] : 0.0f; }
 
 /* the weight of a chosen logit from those of all: `shift` is taken off the exponents where all are negative, so that small scores keep
- * their proportions; scores that are zero in 64 bits are zero */
-ACC_DEV float op_part(const float x, const float shift) { return x < -745.0f ? 0.0f : x < 0.0f ? expf(x - shift) / (1.0f + expf(x)) : 1.0f / (1.0f + expf(-x)); }
+ * their proportions; scores that are zero in 64 bits, where e^-x is beyond the largest number, are zero */
+ACC_DEV float op_part(const float x, const float shift) { return x < -709.78268f ? 0.0f : x < 0.0f ? expf(x - shift) / (1.0f + expf(x)) : 1.0f / (1.0f + expf(-x)); }
 
 /* Token t again, in 64 bits: lane j has the j-th choice.  A lane has every 64th expert. */
 #define OP_AGAIN (OP_LANES * OP_PER > 64 ? OP_LANES * OP_PER / 64 : 1)

@@ -47,3 +47,31 @@ def test_biases_that_are_masks(A, ctx, elt, t, size, groups, keep, choose):
         say(elt, t, size, groups, keep, name)
         b = bias.reshape(-1)
         same(routed(A, ctx, x, b, elt, choose, groups, keep, True, 1.0), plain(x, b, choose, groups, keep, True, 1.0), 1.0)
+
+
+@pytest.mark.parametrize("normalise", (True, False))
+def test_scores_that_64_bits_do_not_hold(A, ctx, normalise):
+    """from 709.78 below 0 on e^-x is an infinity: a score is 0 there, for the choice and for the weight; one just above is not"""
+    rng, t, e, choose = np.random.default_rng(5), 300, 24, 4
+    x = (-rng.uniform(705, 714, (t, e))).astype(np.float32).astype(np.float64)
+    x[::3] = (-rng.uniform(709.8, 760, x[::3].shape)).astype(np.float32)
+    x[1::9, :] = -760.0
+    x[1::9, 5], x[1::9, 7] = np.float32(-709.78271484375), np.float32(-709.78265380859375)
+    for groups, keep in ((1, 1), (4, 2)):
+        say(normalise, groups)
+        want = plain(x, None, choose, groups, keep, normalise, 1.0)
+        if normalise:
+            assert np.any(want[1].sum(1) == 0) and np.any(want[1].sum(1) > 0.9)
+        got = routed(A, ctx, x, None, "float", choose, groups, keep, normalise, 1.0)
+        same(got, want, 1.0)
+        # the gradient: of a token whose scores are all 0 none, and of the others their parts'
+        op = A.ScoreRouter(ctx, "float", choose, groups, keep, normalise, 1.0)
+        dw, back = rng.standard_normal((t, choose)).astype(np.float32), ctx.empty((t, e), np.float32)
+        op.gradient(ctx.array(x.astype(np.float32)), ctx.array(got[0]), ctx.array(dw), back)
+        ctx.sync()
+        op.destroy()
+        share = want[1]
+        d = share * (dw - (dw * share).sum(1, keepdims=True)) if normalise else share * dw
+        full = np.zeros((t, e))
+        np.put_along_axis(full, got[0].astype(np.int64), d, 1)
+        assert np.all(np.abs(back.get() - full) <= 200 * 2.0 ** -24 * np.abs(dw).sum(1, keepdims=True) + 1e-37)
