@@ -151,7 +151,8 @@ extern "C" __global__ void __launch_bounds__(256) grouped_quantise(const acc_gro
   }
   if (!here) return;
   /* (divisions as IEEE has them: a number between two codes is rounded the same way wherever this is computed) */
-  const op_elt kept = (op_elt)(p.zeros ? (high - low) / 15.0f : (high > -low ? high : -low) / 7.0f);
+  const float range = high - low < __builtin_inff() ? (high - low) / 15.0f : (high * 0.0625f - low * 0.0625f) / 15.0f * 16.0f;
+  const op_elt kept = (op_elt)(p.zeros ? range : (high > -low ? high : -low) / 7.0f);
   const float scale = (float)kept;
   bad |= !(scale < __builtin_inff());
   const float zero = p.zeros ? (scale > 0.0f ? acc_min(acc_max(__builtin_rintf(-low / scale), 0.0f), 15.0f) : 0.0f) : 8.0f;

@@ -118,3 +118,30 @@ def test_rows_of_one_sign(rows, elt, group):
         say(elt, group, m, experts, n, k)
         want, _ = expected(x, weights(q, scales, zeros, group), offsets, m, None, 0)
         assert np.array_equal(rows(elt, group, x, q, scales, zeros, offsets), store(want, elt)), (m, experts, n, k)
+
+
+@pytest.mark.parametrize("elt", ("float", "bfloat16"))
+def test_quantising_a_range_beyond_the_largest_number(A, ctx, elt):
+    """high - low of a group of numbers is an infinity, its fifteenth is not: the same formula of sixteenths"""
+    rng, f, group = np.random.default_rng(31), np.float32, 32
+    w = values(store(rng.uniform(-1, 1, (2, 6, 96)), elt), elt).astype(f)
+    most = values(store(np.array([3.3e38]), elt), elt).astype(f)[0]
+    w[0, 2, :32] *= most
+    w[1, 4, 40], w[1, 4, 41] = most, -most
+    w[1, 5, 70], w[1, 5, 71] = most, -most / 2
+    full = w.reshape(2, 6, 3, group)
+    low, high = np.minimum(full.min(3), 0), np.maximum(full.max(3), 0)
+    with np.errstate(over="ignore"):
+        ranges = high - low
+    assert np.isinf(ranges).sum() == 3
+    scale = np.where(np.isinf(ranges), (high * f(0.0625) - low * f(0.0625)) / f(15) * f(16), np.where(np.isinf(ranges), 0, ranges) / f(15)).astype(f)
+    scale = values(store(scale, elt), elt).astype(f)
+    zero = np.clip(np.rint(-low / scale), 0, 15)
+    q = np.clip(np.rint(full / scale[..., None]) + zero[..., None], 0, 15).astype(np.uint8).reshape(2, 6, 96)
+    codes, scales, zeros = ctx.empty((2, 6, 48), np.uint8), Boxed(A, ctx, np.zeros((2, 3, 6)), elt), ctx.empty((2, 3, 6), np.uint8)
+    op = A.Grouped(ctx, elt, group)
+    op.quantise(Boxed(A, ctx, w, elt).array, codes, scales.array, zeros=zeros)
+    ctx.sync()
+    op.destroy()
+    assert np.array_equal(scales.get(), store(np.swapaxes(scale, 1, 2), elt)) and np.array_equal(zeros.get(), np.swapaxes(zero, 1, 2).astype(np.uint8))
+    assert np.array_equal(codes.get(), packed(q))
