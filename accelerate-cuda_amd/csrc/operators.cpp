@@ -1638,13 +1638,18 @@ static int check_grouped(acc_op op, const char *who, const acc_strided *codes, c
   return ACC_OK;
 }
 
-static int launch_elements(acc_op op, const char *who, bool back, int64_t threads, const acc_grouped_args &a, acc_stream stream)
+static int launch_elements(acc_op op, const char *who, bool back, int64_t threads, acc_grouped_args &a, acc_stream stream)
 {
   GroupedVariant v;
   v.elements = true;
   const OpVariant *var = nullptr;
   ACC_TRY(op->variant(v.key(), kGroupedElementNames, 2, grouped_source_of, &var));
-  return launch(op, who, back ? var->fn2 : var->fn, ceil_div(threads, 256), 256, 0, stream, a);
+  const int64_t groups = ceil_div(threads, 256), most = kThreads / 256;
+  for (int64_t first = 0; first < groups; first += most) {
+    a.first = first * 256;
+    ACC_TRY(launch(op, who, back ? var->fn2 : var->fn, std::min(most, groups - first), 256, 0, stream, a));
+  }
+  return ACC_OK;
 }
 
 int acc_exec_grouped_quantise(acc_op op, const acc_strided *w, const acc_strided *codes, const acc_strided *scales, const acc_strided *zeros, acc_stream stream)

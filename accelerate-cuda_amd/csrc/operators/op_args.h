@@ -106,6 +106,7 @@ struct acc_grouped_args {
   int32_t tiles_i, tiles_j;
   uint32_t per_mul, per_shift;
   const uint32_t *guard;
+  int64_t first;                /* quantise, values: the launch's first thread of all */
 };
 
 /* the recurrence: see op_recur.h */

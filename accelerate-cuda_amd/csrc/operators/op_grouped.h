@@ -123,7 +123,7 @@ extern "C" __global__ void __launch_bounds__(256) grouped_quantise(const acc_gro
 {
   if (p.guard && *p.guard == 0u) return;
   const int team = acc_min(64, p.group / 8), lane = (int)threadIdx.x % team;
-  const long long n = ((long long)blockIdx.x * 256 + threadIdx.x) / team, rows = (long long)p.experts * p.nj;
+  const long long n = (p.first + (long long)blockIdx.x * 256 + threadIdx.x) / team, rows = (long long)p.experts * p.nj;
   const bool here = n < rows * p.groups;
   const long long row = here ? n / p.groups : 0, e = row / p.nj, j = row % p.nj;
   const int g = here ? (int)(n % p.groups) : 0, first = g * p.group, end = acc_min(p.k, first + p.group);
@@ -178,7 +178,7 @@ extern "C" __global__ void __launch_bounds__(256) grouped_quantise(const acc_gro
 extern "C" __global__ void __launch_bounds__(256) grouped_values(const acc_grouped_args p)
 {
   if (p.guard && *p.guard == 0u) return;
-  const long long n = (long long)blockIdx.x * 256 + threadIdx.x, row = n / (p.blocks * 4);
+  const long long n = p.first + (long long)blockIdx.x * 256 + threadIdx.x, row = n / (p.blocks * 4);
   if (row >= (long long)p.experts * p.nj) return;
   const long long e = row / p.nj, j = row % p.nj;
   const int k = (int)(n % (p.blocks * 4)) * 8, g = k / p.group, left = p.k - k;

@@ -294,6 +294,33 @@ static void beside(acc_context ctx)
   OK(acc_op_destroy(op));
 }
 
+// matrices of more numbers than a launch has threads for, by a matrix that is there many times
+static void parts(acc_context ctx)
+{
+  acc_op_desc d = {};
+  d.kind = ACC_OP_GROUPED;
+  d.elt_type = "half";
+  d.group = 32;
+  acc_op op = nullptr;
+  OK(acc_op_create(ctx, &d, &op));
+  const int64_t experts = 100, n = 1 << 15, k = (1 << 15) - 7, blocks = (k + 31) / 32;
+  acc_strided w = array({experts, n, k}), codes = array({experts, n, 16 * blocks}), scales = array({experts, blocks, n}), zeros = array({experts, blocks, n});
+  for (const char *name : {"grouped_quantise", "grouped_values"}) {
+    const size_t since = g_launched.size();
+    if (!std::strcmp(name, "grouped_quantise")) OK(acc_exec_grouped_quantise(op, &w, &codes, &scales, &zeros, nullptr));
+    else OK(acc_exec_grouped_values(op, &codes, &scales, &zeros, &w, nullptr));
+    int64_t done = 0;
+    for (size_t i = since; i < g_launched.size(); ++i) {
+      const Launch &l = g_launched[i];
+      IS(l.name == name && (uint64_t)l.grid * l.block <= 0xffffffffull && l.block % 64 == 0);
+      IS(l.grouped.first == done);                // (one behind the other, teams of lanes whole)
+      done += (int64_t)l.grid * l.block;
+    }
+    IS(done >= experts * n * blocks * 4 && g_launched.size() - since > 2);
+  }
+  OK(acc_op_destroy(op));
+}
+
 int main(int, char **argv)
 {
   OK(acc_init());
@@ -304,6 +331,7 @@ int main(int, char **argv)
   if (part == "pool") pool(ctx);
   else if (part == "order") order(ctx);
   else if (part == "beside") beside(ctx);
+  else if (part == "parts") parts(ctx);
   else IS(!"a part that there is");
   OK(acc_context_destroy(ctx));
   std::printf("wrong %d\n", g_wrong);

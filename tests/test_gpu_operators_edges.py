@@ -161,3 +161,29 @@ def test_eager_calls_beside_a_capture(A, ctx, hip):
     hip.hipGraphExecDestroy(graph_exec)
     hip.hipGraphDestroy(graph)
     op.destroy()
+
+
+def test_more_numbers_than_a_launch_has_threads_for(A, ctx):
+    """33 times the same matrix of 2^30 numbers, quantised and made again: the last is as the first"""
+    n, k, experts, group = 2 ** 15, 2 ** 15, 33, 128
+    w = torch.empty((n, k), dtype=torch.float16, device="cuda").normal_()
+    codes, scales, zeros = (torch.full((experts, *shape), 99, dtype=t, device="cuda") for shape, t in (((n, k // 2), torch.uint8), ((k // group, n), torch.float16), ((k // group, n), torch.uint8)))
+    op = A.Grouped(ctx, "half", group)
+    torch.cuda.synchronize()
+    say("quantise")
+    op.quantise(w.expand(experts, n, k), codes, scales, zeros=zeros)
+    ctx.sync()
+    for a in (codes, scales, zeros):
+        assert all(torch.equal(a[0], a[e]) for e in range(1, experts))
+    full = w.reshape(n, k // group, group).float()
+    low, high = full.amin(2).clamp(max=0.0), full.amax(2).clamp(min=0.0)
+    assert torch.equal(scales[-1], ((high - low) / 15.0).half().t())
+    del full, low, high
+    made = torch.full((experts, n, k), 77.0, dtype=torch.float16, device="cuda")
+    say("values")
+    op.values(codes, scales, made, zeros=zeros)
+    ctx.sync()
+    assert all(torch.equal(made[0], made[e]) for e in range(1, experts))
+    off = (made[-1].float() - w.float()).abs().reshape(n, k // group, group).amax(2)
+    assert torch.all(off <= scales[-1].t().float() * 0.51 + 0.01)          # (half a step; scales and what is made again are rounded, too)
+    op.destroy()

@@ -39,6 +39,11 @@ def test_eager_calls_do_not_end_the_capture_of_another_stream(edges):
     edges("beside")
 
 
+def test_more_numbers_than_a_launch_has_threads_for(edges):
+    """matrices of 2^36 numbers and more are quantised, and made again, in several launches"""
+    edges("parts")
+
+
 def test_sequences_without_a_row_are_found_whatever_the_tiles(tmp_path):
     """op_recur.h's own arithmetic of shares, compiled for the host: no offset outside the array is read"""
     csrc = os.path.join(os.path.dirname(HERE), "..", "accelerate-cuda_amd", "csrc", "operators")
