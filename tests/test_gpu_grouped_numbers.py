@@ -8,6 +8,12 @@ Float32 scales the product is rounded, once, and that is the result.
 Rows whose numbers share a sign: of every group the kernels add up x (16 + q) and take (16 + z) sum x off, each of them below 31 sum x;
 with whole numbers that make this less than 2^24 everything is exact again, and so is the sum over the groups, with scales that are powers
 of two.  A form that adds more than 16 to a code loses digits there.
+
+Float32 rows are cut into three parts of 8 bits, each of what the one before has left.  With x of 17 bits, whole numbers of 2^-16 between 1
+and 2, four of a group not 0, all that is added up is a whole number of 2^-16 below 31 x 4 x 2 = 2^8: 24 bits, exact, and so are the results of
+one group.  With x of 24 bits, one of a group not 0 and s = 1: -(z + 16) x1 + x1 (16 + q) is exact (13 bits), and so is what the second part
+adds (within 21); the third part's product rounds once, below 32 |x|, the second parts' beginning once more, to a result below 16 |x|, and
+up to two groups of the row add up once: half a unit of 2^-23 times that, (16 + 8 + 16) |x| 2^-23 of the larger |x|, is more than any of it.
 """
 import sys
 
@@ -57,8 +63,8 @@ def rows(A, ctx):
         op.destroy()
 
 
-# (rows, matrices, n, k): a few rows, a few hundred of one matrix, tiles of 256 columns enough for the device
-FORMS = [(3, 1, 70, 100), (129, 1, 70, 100), (300, 1, 70, 31), (700, 2, 4, 100), (5000, 2, 300, 70), (1500, 25, 900, 100), (200, 2, 3100, 100)]
+# (rows, matrices, n, k): a few rows, a few hundred of one matrix, tiles of 256 columns enough for the device, rows in LDS (the last two)
+FORMS = [(3, 1, 70, 100), (129, 1, 70, 100), (300, 1, 70, 31), (700, 2, 4, 100), (5000, 2, 300, 70), (1500, 25, 900, 100), (200, 2, 3100, 100), (40, 2, 3200, 100), (9, 1, 6200, 100)]
 
 
 @pytest.mark.parametrize("with_zeros", (False, True))
@@ -145,3 +151,53 @@ def test_quantising_a_range_beyond_the_largest_number(A, ctx, elt):
     op.destroy()
     assert np.array_equal(scales.get(), store(np.swapaxes(scale, 1, 2), elt)) and np.array_equal(zeros.get(), np.swapaxes(zero, 1, 2).astype(np.uint8))
     assert np.array_equal(codes.get(), packed(q))
+
+
+def in_parts(x, parts):
+    """the first `parts` of the three 8-bit parts of Float32 numbers, added up"""
+    left, total = x.astype(np.float32), np.zeros(x.shape, np.float32)
+    for _ in range(parts):
+        part = (left.view(np.uint32) & np.uint32(0xffff0000)).view(np.float32)
+        total, left = total + part, left - part
+    return total.astype(np.float64)
+
+
+@pytest.mark.parametrize("with_zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64, 128))
+def test_all_three_parts_of_float32_rows(rows, group, with_zeros):
+    rng = np.random.default_rng(group + 5)
+    for m, experts, n, k in FORMS:
+        k = min(k, group)
+        q, _, zeros = matrices(rng, experts, n, k, group, "float", with_zeros, True)
+        scales = np.full((experts, 1, n), 0.25)
+        x = np.zeros((m, k))
+        for r in range(m):
+            x[r, rng.permutation(k)[:4]] = (2.0 ** 16 + rng.integers(2 ** 7, 2 ** 15, 4) * 2 + 1) * rng.choice([-1, 1], 4) * 2.0 ** -16
+        offsets = segments(rng, m, experts, "even")
+        say(group, with_zeros, m, experts, n, k)
+        w = weights(q, scales, zeros, group)
+        want, _ = expected(x, w, offsets, m, None, 0)
+        two, _ = expected(in_parts(x, 2), w, offsets, m, None, 0)
+        assert np.array_equal(in_parts(x, 3), x) and np.mean(two != want) > 0.2
+        assert np.array_equal(rows("float", group, x, q, scales, zeros, offsets), want.astype(np.float32)), (m, experts, n, k)
+
+
+@pytest.mark.parametrize("with_zeros", (False, True))
+@pytest.mark.parametrize("group", (32, 64))
+def test_float32_rows_of_all_their_bits(rows, group, with_zeros):
+    rng = np.random.default_rng(group + 6)
+    for m, experts, n, k in FORMS:
+        k = min(k, 2 * group)
+        q, _, zeros = matrices(rng, experts, n, k, group, "float", with_zeros, True)
+        scales = np.ones((experts, -(-k // group), n))
+        x = np.zeros((m, k))
+        for first in range(0, k, group):
+            x[np.arange(m), rng.integers(first, min(k, first + group), m)] = rng.uniform(1, 2, m).astype(np.float32) * rng.choice([-1, 1], m)
+        offsets = segments(rng, m, experts, "even")
+        say(group, with_zeros, m, experts, n, k)
+        w = weights(q, scales, zeros, group)
+        want, _ = expected(x, w, offsets, m, None, 0)
+        bound = 40 * 2.0 ** -23 * np.abs(x).max(1, keepdims=True)
+        two, _ = expected(in_parts(x, 2), w, offsets, m, None, 0)
+        assert np.mean(np.abs(two - want) > bound) > 0.2       # (two parts alone would not do)
+        assert np.all(np.abs(rows("float", group, x, q, scales, zeros, offsets) - want) <= bound), (m, experts, n, k)
