@@ -641,24 +641,24 @@ int64_t grouped_tall_lds(const OpSpec &sp, bool zeros)
   return 3 * 16 * parts * rows * 16 + 3 * chunks * 272 * 4 * (zeros ? 2 : 1) + 2 * chunks * rows * 4 * (sp.type == 0 ? 2 : 1);
 }
 // ... and the tiles of 16 columns from which on rows in LDS are worth what it takes to put them there.  us, with and without, tiles: 1 row,
-// 4096 x 4096, 256: 8.2 and 7.2; 16 rows: 14 and 11; 2 rows of 4096 x 11008, 256: 16 and 15; of 11008 x 4096, 688: 13 and 18; 1 row, 8192 x 8192,
-// 512: 16 and 23; 64 rows, 16 half of 4096 x 2048, 4096: 23 and 34; 16, 8 of 4096 x 4096 in groups of 32: 29 and 44; Float32, 64, 16 of
-// 1024 x 2048, 1024: 14 and 12
+// 4096 x 4096, 256: 7.8 and 7.6; 16 rows: 14 and 10; 2 rows of 4096 x 11008, 256: 17 and 14; of 11008 x 4096, 688: 14 and 17; 1 row, 8192 x 8192,
+// 512: 15 and 23; 64 rows, 16 half of 4096 x 2048, 4096: 24 and 33; 16, 8 of 4096 x 4096 in groups of 32: 26 and 36; Float32, 64, 16 of
+// 1024 x 2048, 1024: 15 and 13
 constexpr int64_t kGroupedStream = 384;
 // Whether a call is for tiles of 64 rows (Float32: 32) by 256 columns that make numbers of the codes as they go: rows enough for them, and tiles
-// enough (one that is 4096 long takes 50 us, in groups of 32 100, however few there are).  us, with and without, rows (a few more or less
-// a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 56 and 75; 200, 1 of 4096 x 4096, 64: 49 and 41; 300, 1, 80: 53 and 58, in groups of 32
-// 103 and 77; 400, 1, 112: 50 and 68, in groups of 32 99 and 99; 2000, 1, 512: 83 and 277; 600, 4 of 1024 x 2048, 48: 28 and 24; 1200, 4, 80: 29 and 38;
-// 900, 4 of 2000 x 1000, 120: 26 and 32; 1000, 20 of 500 x 2000, 40: 46 and 25.  Float32: 130, 1 of 4096 x 4096, 80: 65 and 68, in groups of 32
-// 109 and 94; 300, 1, 160: 66 and 113, 110 and 152; 300, 4 of 1024 x 2048, 48: 36 and 25; 600, 4, 80: 37 and 47, 59 and 60
+// enough (one that is 4096 long takes 50 us, in groups of 32 75, however few there are).  us, with and without, rows (a few more or less
+// a segment), matrices, tiles: 320, 8 of 4096 x 4096, 128: 59 and 75; 200, 1 of 4096 x 4096, 64: 50 and 41; 300, 1, 80: 54 and 59, in groups of
+// 32 81 and 70; 400, 1, 112: 52 and 69, in groups of 32 76 and 76; 2000, 1, 512: 85 and 278; 600, 4 of 1024 x 2048, 48: 29 and 24; 1200, 4, 80: 31
+// and 39; 900, 4 of 2000 x 1000, 120: 22 and 27; 1000, 20 of 500 x 2000, 40: 37 and 24.  Float32: 130, 1 of 4096 x 4096, 80: 65 and 71, in groups
+// of 32 91 and 93; 300, 1, 160: 66 and 113, 91 and 145; 300, 4 of 1024 x 2048, 48: 36 and 25; 600, 4, 80: 37 and 47, 49 and 57
 bool grouped_tall(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean)
 {
   const bool wide = sp.type == 0;
   const int64_t tiles = std::max(ceil_div(rows, wide ? 32 : 64), std::min(rows, experts)) * ceil_div(n, 256);
-  return n >= 16 && k > 0 && pitch < (1 << 26) && mean > 32 && tiles >= (sp.group == 32 ? 96 : 72);
+  return n >= 16 && k > 0 && pitch < (1 << 26) && mean > 32 && tiles >= (!wide && sp.group == 32 ? 96 : 72);
 }
 // the tile for `mean` rows a segment; *height: its rows.  (Where LDS holds fewer rows than a segment has, their codes are read again:
-// 64 rows, 2 of 4096 x 4096: 18 us in tiles of 16, 26 without LDS.)
+// 64 rows, 2 of 4096 x 4096: 28 us in tiles of 16, 31 without LDS.)
 GroupedVariant grouped_variant(const OpSpec &sp, int64_t rows, int64_t experts, int64_t n, int64_t k, int64_t pitch, int64_t mean, int64_t *height)
 {
   GroupedVariant v;
