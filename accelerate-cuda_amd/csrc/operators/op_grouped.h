@@ -18,7 +18,7 @@
  * where it has few, what counts is how soon all of it is on its way, and the waves of a workgroup take every so many steps of the same
  * 16 OP_FN columns and add up what they have by way of LDS, in order.  64 half rows, 16 matrices of 4096 x 2048 in groups of 64 with
  * zeros: 22 us, of which the codes' loads alone take 13 (5.8 TB/s), what is in front of them 8 with the launch; bfloat16 in groups of 128,
- * 16 rows, 8 of 4096 x 4096: 19 us; 1 row, 1 of 4096 x 4096: 6.4.  Many rows are matter for the matrix cores (OP_WIDE).
+ * 16 rows, 8 of 4096 x 4096: 21 us; 1 row, 1 of 4096 x 4096: 6.4.  Many rows are matter for the matrix cores (OP_WIDE).
  */
 #include "op_matrix.h"
 
@@ -285,7 +285,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
   const auto add = [&](const int n, const int at, const int down, acc_u4 w) {
     op_turn(w);
     /* (of Float32's many fragments in groups of 32 no addresses are kept from step to step: there are not the registers, and a wait for
-     * one that has been put into memory is a wait for all codes on their way: 28 us in place of 23 for 150 rows of 12 matrices of
+     * one that has been put into memory is a wait for all codes on their way: 27 us in place of 23 for 150 rows of 12 matrices of
      * 1333 x 1001.  Elsewhere, where there are registers, it costs 3 in 100) */
     int row = l, quarter = g;
     if (OP_PARTS > 1 && OP_CHUNKS > 2) {
@@ -423,7 +423,7 @@ extern "C" __global__ void __launch_bounds__(64 * OP_WAVES) grouped(const acc_gr
  * workgroups a compute unit.  The rows of a step of 128 lie in LDS, three steps at a time: the one whose products are taken, the next
  * one, whose sums by groups are taken meanwhile (of 16 rows by a wave), and the one after that, on its way there.  A wave makes its 64
  * columns' codes into numbers itself, in registers: 16 columns' are used for all rows.  bfloat16, 2048 rows of 8 matrices of 4096 x 4096 in
- * groups of 128: 117 us, 587 TFLOP/s.  Loads are not what it waits for (without those of
+ * groups of 128: 110 us, 624 TFLOP/s.  Loads are not what it waits for (without those of
  * the codes 1 us less, of the rows 7): a step's 64 instructions of the matrix cores take as long as the 200 others beside them, of which
  * a half makes numbers, and of two waves a SIMD one covers the other only in part.  (128 rows and eight waves a workgroup: 154, a
  * segment's short last tile being as long as a whole one; the numbers of the next 32 made ready between the products: 132 and more,

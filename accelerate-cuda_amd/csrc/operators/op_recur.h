@@ -13,7 +13,7 @@
  * such a tile waits for the state in front of it, and its waves take their rows one after the other, as the definition has it.  (Half,
  * one sequence of 65536 x 512: 56 us, 12000 where every tile's product overflows.)
  *
- * Bound by memory: every array passes by once.  bfloat16, 32768 rows of 2048 in 8 sequences, sigmoids: 101 us, 4.0 TB/s, the gradient 170,
+ * Bound by memory: every array passes by once.  bfloat16, 32768 rows of 2048 in 8 sequences, sigmoids: 102 us, 3.9 TB/s, the gradient 170,
  * 4.7 (a copy 5.4); what is short of that are the gates, worked out in both passes.  One sequence of 65536 half rows of 512: 56, 3.6, the
  * tiles' waits for those before; Float32, 9001 rows of 1001: 38, 2.9, rows starting amid lines.  A workgroup has a tile of 64 OP_V channels and 8 OP_R rows, a wave OP_R of those, all
  * of them in registers; it goes over them twice, first for the tile's map, and once what comes in from the rows before is known for
