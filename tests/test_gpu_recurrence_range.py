@@ -134,7 +134,7 @@ def test_gradients_beyond_the_largest_number(A, ctx, ops, elt):
             assert same(ds.get(), dstate) and same(values(dvalues.get(), elt), values(store(g, elt), elt))
             want = g * 1.0
             want[[0, rows // 3]] = g[[0, rows // 3]] * np.float32(0.0)         # (states of zeros come before first rows)
-        assert same(values(dgates.get(), elt), values(store(want, elt), elt))
+            assert same(values(dgates.get(), elt), values(store(want, elt), elt))
 
 
 @pytest.mark.parametrize("gate", ("given", "sigmoid"))
